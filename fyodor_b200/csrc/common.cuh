@@ -2,6 +2,7 @@
 #pragma once
 #include <cstdint>
 #include <cuda_fp16.h>
+#include <cuda_bf16.h>
 
 #define FYB_DEV __device__ __forceinline__
 #define FYB_HOST_DEV __host__ __device__ __forceinline__
@@ -105,6 +106,20 @@ FYB_DEV void ldmatrix_x4(unsigned (&r)[4], const void *p)
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(smem_u32(p)));
 }
+
+FYB_DEV void raise_error(unsigned *error, unsigned code)
+{
+    if (error) atomicOr(error, code);
+}
+
+// ---- rows of F32, F16 or BF16 values ---------------------------------------
+FYB_DEV float row_value(float v) { return v; }
+FYB_DEV float row_value(__half v) { return __half2float(v); }
+FYB_DEV float row_value(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <typename T> FYB_DEV T row_round(float v);
+template <> FYB_DEV float row_round<float>(float v) { return v; }
+template <> FYB_DEV __half row_round<__half>(float v) { return __float2half_rn(v); }
+template <> FYB_DEV __nv_bfloat16 row_round<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
 // L2-coherent loads for data produced by other CTAs of the same launch.
 FYB_DEV float ldcg_f32(const float *p) { return __ldcg(p); }

@@ -5,6 +5,7 @@
 #include <algorithm>
 #include <cuda_runtime.h>
 #include <cuda_fp16.h>
+#include "fyodor_b200.h"
 
 namespace fyb {
 
@@ -205,6 +206,12 @@ inline size_t decode_attn_partials_floats(const DecodeGeometry &g)
 int decode_supported(const DecodeGeometry &g, unsigned type_out);
 int decode_grid(int sms, const DecodeGeometry &g);
 int launch_decode(const DecodeLaunch &L, cudaStream_t s);
+
+// ---------------------------------------------------------------- rope.cu
+struct RopeTable;
+struct RopeRows;
+int rope_table_of(const fyb_rope_desc *d, RopeTable *t);
+bool rope_vectors(const RopeTable &t, unsigned hd, size_t width, const RopeRows &r);
 
 // ---------------------------------------------------------------- batch.cu
 // Elementwise kernels of the batched decode step (B <= BATCH_MAX sequences).

@@ -227,6 +227,137 @@ int fyb_batch_decode_greedy(void *batch, const uint32_t *tokens, const uint32_t 
 double fyb_batch_time_greedy(void *batch, const uint32_t *tokens, const uint32_t *positions, size_t steps);
 unsigned long long fyb_batch_launches_per_step(const void *batch);
 
+/* ---- paged 8-bit KV cache (no counterpart in the reference, whose cache is
+   one F32 array per sequence, backend/core/llm_cpu.c:510-535) --------------
+   The cache is a pool of blocks of block_size tokens. A request's tokens lie
+   in the blocks its row of a block table names, token t in block
+   table[t / block_size] at offset t % block_size, so requests of any length
+   share the pool. K and V are stored in 8 bits with one F32 scale for each
+   (block, KV head): value = stored * scale. A serving step runs
+   fyb_kv_blocks once, then per layer fyb_kv8_append (with RoPE) and
+   fyb_kv8_attention; all of them read lengths, tables and slots on the
+   device, so a CUDA graph of the step serves every later step.
+
+   q, k, v rows are `type` F32, F16 or BF16 (GGML ids 0, 1, 30), strides in
+   elements; a row's heads are contiguous. Every pointer below is a device
+   pointer unless a line says otherwise; `error` (may be NULL) is a device
+   word that receives 4 when an index read on the device is out of range (the
+   row or position concerned is then left out) and 2 for non-finite values
+   given to the cache; kernels set it and never clear it. */
+#define FYB_KV8_INT8 0u /* signed integers -127..127 */
+#define FYB_KV8_E4M3 1u /* 8-bit floats, 4 exponent and 3 mantissa bits, largest 448 */
+typedef struct fyb_kv8_cache {
+    void *k, *v;              /* [blocks][kv_heads][block_size][head_dim] bytes, 16-byte aligned */
+    float *k_scale, *v_scale; /* [blocks][kv_heads] */
+    uint32_t blocks, kv_heads;
+    uint32_t block_size;      /* 16, 32, 64, 128 or 256 tokens */
+    uint32_t head_dim;        /* 64 or 128 */
+    uint32_t format;          /* FYB_KV8_INT8 or FYB_KV8_E4M3 */
+} fyb_kv8_cache;
+
+/* One step's block tables and slot maps from request lengths, in one launch.
+   Request r holds lengths[r] tokens and brings new_tokens[r] more; its blocks
+   are table[r * table_stride ..]. The blocks it needs beyond those it has are
+   popped, requests in order, from the stack free_list[0 .. free_count[0]):
+   the j-th block of the step is free_list[free_count[0] - 1 - j], written to
+   the table. Requests are served whole or not at all: status[r] 0 served, 1
+   too few free blocks (all later requests that need one are refused too), 2
+   invalid (negative counts, more tokens than the table holds, rows beyond
+   max_rows). Outputs: lengths_out[r] (lengths + new when served),
+   free_count_out[0], row_start [requests + 1] (the step's rows, request after
+   request, clamped to max_rows) and, per row 0..max_rows, slots (block *
+   block_size + offset; -1 for rows of refused requests and rows beyond the
+   last), positions (token index in its request, 0 beyond the last row) and
+   row_request (-1 beyond the last row). lengths_out and free_count_out are
+   buffers of their own (-1 when they are the inputs): a step can be repeated.
+   requests <= 16384, max_rows < 2^30, block_size a power of two. */
+int fyb_kv_blocks(const int32_t *lengths, const int32_t *new_tokens, uint32_t requests, int32_t *table,
+    size_t table_stride, uint32_t block_size, const int32_t *free_list, const int32_t *free_count,
+    int32_t *lengths_out, int32_t *free_count_out, int32_t *row_start, int32_t *slots, int32_t *positions,
+    int32_t *row_request, uint32_t max_rows, int32_t *status, void *stream);
+/* Gives the blocks of every request with done[r] != 0 back: pushed on
+   free_list (of free_capacity entries; blocks beyond it stay with their
+   request) in request order, table entries set to -1, lengths[r] to 0,
+   free_count[0] raised. In place. requests <= 16384. */
+int fyb_kv_release(int32_t *lengths, const int32_t *done, uint32_t requests, int32_t *table, size_t table_stride,
+    uint32_t block_size, int32_t *free_list, int32_t *free_count, uint32_t free_capacity, void *stream);
+
+/* Rotary positions. The engine's frequencies (backend/core/llm_cpu.c:216-229)
+   scaled for long contexts, on the host: freq[j], j < dims / 2, and in
+   *magnitude what cos and sin are multiplied by. */
+#define FYB_ROPE_PLAIN 0u  /* base^(-2j/dims) */
+#define FYB_ROPE_LINEAR 1u /* divided by factor */
+#define FYB_ROPE_NTK 2u    /* base grown to base * factor^(dims / (dims - 2)) */
+#define FYB_ROPE_YARN 3u   /* between plain and linear by the turns a dimension makes over original_context (beta_fast,
+                              beta_slow); magnitude 0.1 ln(factor) + 1 */
+#define FYB_ROPE_BANDS 4u  /* plain above high_freq turns, linear below low_freq turns, blended between */
+typedef struct fyb_rope_scaling {
+    uint32_t kind;
+    float factor, original_context;
+    float beta_fast, beta_slow; /* YARN (32 and 1 where 0) */
+    float low_freq, high_freq;  /* BANDS (1 and 4 where 0) */
+} fyb_rope_scaling;
+/* scaling may be NULL (plain); factors (may be NULL): dims / 2 divisors of the
+   frequencies (a model's rope_freqs tensor). Host pointers. */
+int fyb_rope_frequencies(uint32_t dims, float base, const fyb_rope_scaling *scaling, const float *factors,
+    float *freq, float *magnitude);
+/* cos / sin [rows][dims / 2] of the angles (float)(first + row) * freq[j], times
+   magnitude (freq on the device). */
+int fyb_rope_tables(const float *freq, uint32_t dims, float magnitude, uint32_t first, uint32_t rows, float *cos_table,
+    float *sin_table, void *stream);
+
+#define FYB_ROPE_INTERLEAVED 0u /* pairs (2j, 2j + 1) */
+#define FYB_ROPE_HALF 1u        /* pairs (j, j + dims / 2) */
+typedef struct fyb_rope_desc {
+    const float *cos_table, *sin_table; /* [table_rows][dims / 2], 16-byte aligned */
+    uint32_t table_rows;
+    uint32_t dims;                      /* the first dims (even) of every head are rotated, the rest is copied */
+    uint32_t layout;
+} fyb_rope_desc;
+/* q_out / k_out = q / k [rows][heads][head_dim] rotated to positions[row] (k may be
+   NULL with kv_heads 0). An output may be its input (same stride). A row whose
+   position is outside the table is not written. */
+int fyb_rope(const fyb_rope_desc *rope, const int32_t *positions, size_t rows, uint32_t head_dim, uint32_t type,
+    const void *q, size_t q_stride, void *q_out, size_t q_out_stride, uint32_t heads, const void *k, size_t k_stride,
+    void *k_out, size_t k_out_stride, uint32_t kv_heads, uint32_t *error, void *stream);
+
+/* Append K and V rows [rows][kv_heads][head_dim] at slots[row] (a negative slot
+   is skipped). Rows of one block are adjacent in the list and ascend (what
+   fyb_kv_blocks makes of each request); tokens are appended: those below the
+   first new one of a block stay, those above it are no longer valid. The
+   block's scale becomes max(old scale, max|x| * (1 / 127 or 1 / 448)) (the old
+   scale counts only if the block holds older tokens); where it grows the older
+   tokens are stored anew, q' = round(q * (old / new)); new ones are
+   round(x / scale), to nearest even, every step in F32. Infinities are stored as the largest
+   value, NaN as 0, neither counts for the scale. With `rope` K is rotated to
+   positions[row] first, and q (may be NULL with heads 0) to q_out as by
+   fyb_rope, in the same launch; half pairs then need dims a multiple of 8. */
+int fyb_kv8_append(const fyb_kv8_cache *cache, const int32_t *slots, size_t rows, uint32_t type, const void *k,
+    size_t k_stride, const void *v, size_t v_stride, const fyb_rope_desc *rope, const int32_t *positions,
+    const void *q, size_t q_stride, void *q_out, size_t q_out_stride, uint32_t heads, uint32_t *error, void *stream);
+/* k_out / v_out [rows][kv_heads][head_dim] F32 = the values held at slots[row] (0 for a
+   negative slot), as plan_read_kv returns a plan's rows. */
+int fyb_kv8_read(const fyb_kv8_cache *cache, const int32_t *slots, size_t rows, float *k_out, float *v_out,
+    uint32_t *error, void *stream);
+
+/* Causal attention of the newest rows of each request over its blocks.
+   Request r has lengths[r] tokens in the cache (its rows of this step among
+   them) and the rows row_start[r] .. row_start[r + 1] of q and out, at most
+   max_rows each (row_start NULL: one row per request, row r); row j of n
+   attends tokens 0 .. lengths[r] - n + j, scores q.k * scale, softmax and sums
+   in F32. A row that attends nothing is 0. q [rows][heads][head_dim] and out
+   of `type`; heads a multiple of kv_heads, at most 64 per KV head. Infinities
+   and NaN in slots past a request's length have no effect.
+   workspace: fyb_kv8_attention_workspace() bytes on this device, zero before
+   the first call (calls leave it so); calls that overlap in time need
+   workspaces of their own. Results do not depend on timing. */
+size_t fyb_kv8_attention_workspace(uint32_t requests, uint32_t max_rows, uint32_t heads, uint32_t kv_heads,
+    uint32_t head_dim);
+int fyb_kv8_attention(const fyb_kv8_cache *cache, const int32_t *lengths, const int32_t *row_start, uint32_t requests,
+    uint32_t max_rows, size_t rows, const int32_t *table, size_t table_stride, uint32_t type, const void *q,
+    size_t q_stride, void *out, size_t out_stride, uint32_t heads, float scale, void *workspace,
+    size_t workspace_bytes, uint32_t *error, void *stream);
+
 /* ---- tensor parallelism across processes (no reference counterpart) -----
    A process whose environment holds NYA_CUDA_TP_SIZE=N (2..8) and
    NYA_CUDA_TP_RANK=r (and NYA_CUDA_DEVICE for its GPU) creates plans that hold
