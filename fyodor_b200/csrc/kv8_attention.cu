@@ -3,22 +3,11 @@
 //
 // S = (q . k_q) k_scale scale, p = exp(S - max), out = sum p v_scale v_q / sum p,
 // the maximum and the sum kept while the cache passes by once.
-#include "kv8.cuh"
+#include "kv8_attention.cuh"
 
 namespace fyb {
 
 constexpr unsigned KA_THREADS = 128;
-
-struct Kv8Attention {
-    fyb_kv8_cache c;
-    const int *lengths, *row_start, *table;
-    size_t table_stride, rows, q_stride, out_stride;
-    const void *q;
-    void *out;
-    unsigned requests, max_rows, heads, shift;
-    float scale;
-    unsigned *error;
-};
 
 // One CTA per (row, head): thread = position for the scores, thread = head
 // dimension for the value sums.
@@ -71,7 +60,7 @@ __global__ void __launch_bounds__(KA_THREADS) kv8_attention_kernel(Kv8Attention 
 #pragma unroll
                     for (int e = 0; e < 16; ++e) dot = fmaf(q_s[w * 16 + e], kv8_number<FMT>((x[e / 4] >> 8 * (e % 4)) & 0xffu), dot);
                 }
-                s = dot * A.c.k_scale[at] * A.scale;
+                s = dot * A.c.k_scale[at] * (A.scale * 0.69314718f);
             } else {
                 raise_error(A.error, ERR_BOUNDS);
             }
@@ -131,7 +120,7 @@ extern "C" size_t fyb_kv8_attention_workspace(uint32_t requests, uint32_t max_ro
     if (!requests || !max_rows || !kv_heads || heads < kv_heads || heads % kv_heads || heads / kv_heads > 64 ||
         (head_dim != 64 && head_dim != 128))
         return 0;
-    return 16;
+    return KA_COUNTER_BYTES + kv8_decode_part_bytes(head_dim);
 }
 
 extern "C" int fyb_kv8_attention(const fyb_kv8_cache *cache, const int32_t *lengths, const int32_t *row_start,
@@ -144,16 +133,22 @@ extern "C" int fyb_kv8_attention(const fyb_kv8_cache *cache, const int32_t *leng
         return -1;
     const size_t need = fyb_kv8_attention_workspace(requests, max_rows, heads, cache->kv_heads, cache->head_dim);
     const size_t row = (size_t)heads * cache->head_dim;
-    if (!need || !lengths || !table || !q || !out || q_stride < row || out_stride < row || !workspace ||
+    if (!need || !lengths || !table || !q || !out || q_stride < row || out_stride < row || !workspace || (uintptr_t)workspace % 16 ||
         workspace_bytes < need || (!row_start && rows != requests))
         return -1;
     if (!rows) return 0;
     Kv8Attention A{};
     A.c = *cache;
     A.lengths = lengths; A.row_start = row_start; A.table = table; A.table_stride = table_stride;
-    A.rows = rows; A.q = q; A.q_stride = q_stride; A.out = out; A.out_stride = out_stride;
+    A.rows = (unsigned)rows; A.q = q; A.q_stride = q_stride; A.out = out; A.out_stride = out_stride;
     A.requests = requests; A.max_rows = max_rows; A.heads = heads; A.shift = kv8_shift(cache);
-    A.scale = scale; A.error = error;
+    A.scale = scale * 1.44269504f; A.error = error;
+    A.type = type; A.group = heads / cache->kv_heads; A.row_tile = max_rows;
+    unsigned char *ws = static_cast<unsigned char *>(workspace);
+    A.counters = reinterpret_cast<unsigned *>(ws);
+    A.part_ml = reinterpret_cast<float2 *>(ws + KA_COUNTER_BYTES);
+    A.part_o = reinterpret_cast<float *>(A.part_ml + 2 * KA_GRID * KV8_DECODE_ROWS);
+    if ((unsigned long long)max_rows * A.group <= KV8_DECODE_ROWS) return launch_kv8_decode(A, (cudaStream_t)stream);
     const dim3 grid((unsigned)rows, heads);
     cudaStream_t s = (cudaStream_t)stream;
     if (type == T_F32) attention_launch<float>(A, grid, s);
