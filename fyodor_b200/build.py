@@ -28,11 +28,14 @@ def _nvcc():
 
 
 # Sources compiled once per variant (object suffix, extra flags): each
-# instantiation of the persistent decode kernel is its own compilation, so
-# they run in parallel.
+# instantiation of the persistent decode kernel, and each head dimension and
+# format of the many-row attention over the 8-bit cache, is its own
+# compilation, so they run in parallel.
 VARIANTS = {
     "decode_inst.cu": [("%d_%d" % (hd, g), ["-DFYB_DK_HD=%d" % hd, "-DFYB_DK_G=%d" % g])
                        for hd in (128, 64) for g in (1, 2, 4, 8)],
+    "kv8_tiles_inst.cu": [("%d_%d" % (hd, f), ["-DFYB_KT_HD=%d" % hd, "-DFYB_KT_FMT=%d" % f])
+                          for hd in (128, 64) for f in (0, 1)],
 }
 
 
@@ -73,7 +76,7 @@ def build(verbose=False):
     os.makedirs(OBJ, exist_ok=True)
     todo = units()
     # the longest compilations first
-    todo.sort(key=lambda u: u[0] != "decode_inst.cu")
+    todo.sort(key=lambda u: u[0] not in VARIANTS)
     with concurrent.futures.ThreadPoolExecutor(max_workers=min(os.cpu_count() or 8, len(todo))) as ex:
         objs = list(ex.map(lambda u: _compile(u, verbose), todo))
     newest = max(os.path.getmtime(o) for o in objs)

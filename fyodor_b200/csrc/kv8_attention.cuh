@@ -1,6 +1,6 @@
 // kv8_attention.cuh - how the attention over the paged 8-bit cache is split
-// over the GPU, shared by its two kernels (kv8_decode.cu: few query rows per
-// KV head, kv8_tiles.cu: many).
+// over the GPU, shared by its two kernels (kv8_decode.cu: few query rows
+// per KV head, kv8_tiles.cuh: many).
 //
 // Work is a line of units. A segment is the cache that one row tile of one
 // request attends in one KV head, a unit TILE positions of it. CTA c of C takes
@@ -336,8 +336,7 @@ template <unsigned FMT> FYB_DEV void kv8_halves(unsigned x, unsigned &a, unsigne
     }
 }
 
-int launch_kv8_decode(const Kv8Attention &A, cudaStream_t s);
-size_t kv8_decode_part_bytes(unsigned head_dim);
+int launch_kv8_decode(const Kv8Attention &A, const CUtensorMap &k, const CUtensorMap &v, unsigned grid, cudaStream_t s);
 constexpr unsigned KV8_DECODE_ROWS = 8;  // most query rows per KV head of the decode kernel
 
 }  // namespace fyb

@@ -399,29 +399,6 @@ __global__ void __launch_bounds__(KD_THREADS, 2) kv8_decode_kernel(Kv8Attention 
     }
 }
 
-int kv8_tensor_map(CUtensorMap *map, const fyb_kv8_cache &c, const void *pool)
-{
-    using Encode = decltype(&cuTensorMapEncodeTiled);
-    static const Encode encode = [] {
-        void *f = nullptr;
-        cudaDriverEntryPointQueryResult found;
-        if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &f, 12000, cudaEnableDefault, &found) != cudaSuccess ||
-            found != cudaDriverEntryPointSuccess) {
-            cudaGetLastError();
-            f = nullptr;
-        }
-        return (Encode)f;
-    }();
-    if (!encode) return -2;
-    const cuuint64_t dims[2] = {c.head_dim, (cuuint64_t)c.blocks * c.kv_heads * c.block_size}, strides[1] = {c.head_dim};
-    const cuuint32_t box[2] = {c.head_dim, std::min(c.block_size, 64u)}, step[2] = {1, 1};
-    return encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void *>(pool), dims, strides, box, step,
-                  CU_TENSOR_MAP_INTERLEAVE_NONE, c.head_dim == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
-                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS ? 0 : -2;
-}
-
-size_t kv8_decode_part_bytes(unsigned hd) { return (size_t)2 * KA_GRID * KV8_DECODE_ROWS * (hd + 2) * sizeof(float); }
-
 template <int HD, unsigned FMT, int W> static int decode_launch(const Kv8Attention &A, const CUtensorMap &k,
     const CUtensorMap &v, unsigned grid, cudaStream_t s)
 {
@@ -437,13 +414,8 @@ template <int HD, unsigned FMT, int W> static int decode_launch(const Kv8Attenti
     return cudaGetLastError() == cudaSuccess ? 0 : -2;
 }
 
-int launch_kv8_decode(const Kv8Attention &A, cudaStream_t s)
+int launch_kv8_decode(const Kv8Attention &A, const CUtensorMap &k, const CUtensorMap &v, unsigned grid, cudaStream_t s)
 {
-    CUtensorMap k, v;
-    if (kv8_tensor_map(&k, A.c, A.c.k) || kv8_tensor_map(&v, A.c, A.c.v)) return -2;
-    // no more CTAs than the most units the tables can hold
-    const unsigned long long tiles = (((unsigned long long)A.table_stride << A.shift) + KD_TILE - 1) / KD_TILE;
-    const unsigned grid = (unsigned)std::min<unsigned long long>(KA_GRID, tiles * A.requests * A.c.kv_heads);
     const bool wide = A.max_rows * A.group > 4, e4m3 = A.c.format == FYB_KV8_E4M3;
     if (A.c.head_dim == 128) {
         if (e4m3) return wide ? decode_launch<128, FYB_KV8_E4M3, 2>(A, k, v, grid, s) : decode_launch<128, FYB_KV8_E4M3, 1>(A, k, v, grid, s);
