@@ -8,27 +8,29 @@
 //   P = 2^(D1 scale - m) v_scale    one thread per position and half the rows
 //   D2[hd][row] += V^T P^T          M = 128, K = 128 positions
 //
-// K and V come as 8-bit tiles by TMA and are converted to fp16 in shared memory
-// (exact); both products read the converted tile as it lies, [position][hd] in
-// 128-byte swizzled rows: K as a K-major, V as an M-major operand. The weights,
-// and q of F32 rows, are two fp16 halves hi + lo (22 bits, an MMA each); q of
-// 16-bit rows is one half, which holds it (a bf16 value 2^24 below its tile's
-// largest loses bits that no score shows). Row sums, maxima and accumulators
-// are F32.
+// K and V come as 8-bit tiles by TMA; four warps convert them to fp16 (exact) on
+// their way from shared to tensor memory, V transposed, where both products
+// read them as operand A: a tile's fp16 form never loads shared memory, whose
+// bandwidth bounds this kernel otherwise (operands staged there instead: 5800
+// cycles a tile at N = 64). The weights, and q of F32 rows, are two fp16 halves
+// hi + lo (22 bits, an MMA each); q of 16-bit rows is one half, which holds it
+// (a bf16 value 2^24 below its tile's largest loses bits that no score shows).
 //
-// The maximum m of a row moves only when a score is more than 2^8 above it, so
-// D2 stays in tensor memory across tiles and is rescaled a few times a segment.
+// The maximum m of a row moves only when a score is more than 2^8 above it. The
+// tensor core rounds its running sums towards zero, about 2^-26 a step, so D2
+// gathers KT_FLUSH tiles and is then added to sums in shared memory, rounded to
+// nearest (2000 steps in D2 alone: 3e-5 off), and a product's low halves go
+// first, while the sum is small. Row sums and maxima are F32.
 //
 // Roles: warps 0-7 softmax (two groups of four, a group takes half the rows),
-// 8-11 conversion and q, 12 TMA, 13 MMA. Per tile at N = 64 the softmax issues
-// about 9 instructions a score, 580 cycles; the conversions 380; the MMAs of F32
-// rows 1024, of 16-bit rows 768; the tile's bytes pass an SM in 1480 cycles.
+// 8-11 conversion and q, 12 TMA, 13 MMA.
 #pragma once
 #include "kv8_attention.cuh"
 
 namespace fyb {
 
 constexpr int KT_TILE = 128, KT_SOFT = 8, KT_CONV = 4, KT_THREADS = 32 * (KT_SOFT + KT_CONV + 2), KT_META = 8;
+constexpr int KT_FLUSH = 2;  // tiles D2 gathers before it is added to the sums
 
 // ---- tcgen05 -------------------------------------------------------------------
 // Operand in 128-byte swizzled rows, eight-row groups 1024 bytes apart. K-major:
@@ -38,21 +40,28 @@ FYB_DEV uint64_t kt_desc(unsigned addr, unsigned lead)
 {
     return (uint64_t)(addr >> 4 & 0x3FFFu) | (uint64_t)(lead >> 4) << 16 | 64ull << 32 | 1ull << 46 | 2ull << 61;
 }
-// F32 accumulator, fp16 operands, M = 128; mn: both operands M/N-major
+// F32 accumulator, fp16 operands, M = 128; mn: B is N-major
 FYB_HOST_DEV constexpr uint32_t kt_idesc(unsigned N, bool mn)
 {
-    return 1u << 4 | (mn ? 3u << 15 : 0u) | N >> 3 << 17 | 128u >> 4 << 24;
+    return 1u << 4 | (mn ? 1u << 16 : 0u) | N >> 3 << 17 | 128u >> 4 << 24;
 }
-FYB_DEV void kt_mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool accumulate)
+// D (tensor memory) (+)= A (tensor memory: row m in lane m, 16 K values in 8 columns) x B (shared memory)
+FYB_DEV void kt_mma(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool accumulate)
 {
     asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-                 " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n"
-                 :: "r"(d), "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate) : "memory");
+                 " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n"
+                 :: "r"(d), "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate) : "memory");
 }
 FYB_DEV void kt_commit(uint64_t *bar)
 {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];"
                  :: "r"(smem_u32(bar)) : "memory");
+}
+FYB_DEV bool kt_elect()
+{
+    unsigned one;
+    asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(one));
+    return one != 0;
 }
 FYB_DEV void kt_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 FYB_DEV void kt_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
@@ -71,9 +80,52 @@ FYB_DEV void kt_st16(uint32_t addr, const float *r)
                     "f"(r[8]), "f"(r[9]), "f"(r[10]), "f"(r[11]), "f"(r[12]), "f"(r[13]), "f"(r[14]), "f"(r[15])
                  : "memory");
 }
+// 16 lanes x 32 columns: registers 4j, 4j + 1 of lane 4g + t go to TMEM lane g, columns 8j + 2t and + 1; 4j + 2, 4j + 3
+// to TMEM lane g + 8
+FYB_DEV void kt_st256(uint32_t addr, const unsigned *r)
+{
+    asm volatile("tcgen05.st.sync.aligned.16x256b.x4.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
+                 :: "r"(addr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+                    "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+                 : "memory");
+}
 FYB_DEV void kt_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 FYB_DEV void kt_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
+// Out of line, as rarely run code is kept small here: the roles' loops together have to stay in the instruction
+// cache (with everything inlined a tile took 7000 cycles, half of them waiting for instructions).
+static __device__ __noinline__ void kt_timeout(volatile unsigned *dead, unsigned *error)
+{
+    *dead = 1;
+    raise_error(error, ERR_TIMEOUT);
+}
+// A bounded wait that gives up when it, or another of the CTA (*dead), has run out.
+FYB_DEV void kt_wait(uint64_t *bar, unsigned parity, volatile unsigned *dead, unsigned *error)
+{
+    if (__builtin_expect(mbar_try_wait(bar, parity & 1), 1)) return;
+    for (unsigned i = 0; !mbar_try_wait(bar, parity & 1); ++i) {
+        if (__builtin_expect(i < 1u << 22 && !*dead, 1)) continue;
+        kt_timeout(dead, error);
+        break;
+    }
+}
+// v[0..C) over the 32 lanes by op: lane i % C returns element i (lanes beyond C repeat)
+template <int C, typename Op> FYB_DEV float kt_reduce(float (&v)[C], unsigned lane, Op op)
+{
+#pragma unroll
+    for (int half = C / 2; half; half /= 2) {
+        const bool up = lane & (unsigned)half;
+#pragma unroll
+        for (int i = 0; i < half; ++i) {
+            const float give = up ? v[i] : v[i + half], keep = up ? v[i + half] : v[i];
+            v[i] = op(keep, __shfl_xor_sync(0xffffffffu, give, half));
+        }
+    }
+    float r = v[0];
+#pragma unroll
+    for (int o = C; o < 32; o <<= 1) r = op(r, __shfl_xor_sync(0xffffffffu, r, o));
+    return r;
+}
 FYB_DEV unsigned kt_pack(float lo, float hi)  // fp16 pair
 {
     const __half2 p = __floats2half2_rn(lo, hi);
@@ -84,21 +136,24 @@ FYB_DEV int kt_exponent(float x) { return x > 0.f ? max(-126, (int)(__float_as_u
 FYB_DEV float kt_power(int e) { return e < -126 ? __uint_as_float(1u << max(0, e + 149)) : __uint_as_float((unsigned)(min(e, 127) + 127) << 23); }
 
 template <int HD, int N, int QP> struct KtShape {
-    static constexpr int STAGE = KT_TILE * HD, F16 = KT_TILE * 256;  // an 8-bit tile; a converted one (128 values a row)
-    static constexpr int QB = N * HD * 2, PB = KT_TILE * 128;        // one half of q; one half of P
-    static constexpr int P_STAGES = QP * N * HD < 16384 ? 2 : 1;  // what fits
-    static constexpr int OFF_K8 = 0, OFF_V8 = OFF_K8 + 2 * STAGE, OFF_KF = OFF_V8 + 2 * STAGE, OFF_VF = OFF_KF + F16,
-                         OFF_Q = OFF_VF + F16, OFF_P = OFF_Q + QP * QB, OFF_END = OFF_P + P_STAGES * 2 * PB;
+    static constexpr int STAGE = KT_TILE * HD, STAGES = QP * N * HD > 8192 ? 2 : 3;  // an 8-bit tile; as many as fit
+    static constexpr int QB = N * HD * 2, PB = KT_TILE * 128;                        // one half of q; one half of P
+    static constexpr int OFF_K8 = 0, OFF_V8 = OFF_K8 + STAGES * STAGE, OFF_Q = OFF_V8 + STAGES * STAGE,
+                         OFF_P = OFF_Q + QP * QB, OFF_O = OFF_P + 4 * PB, OFF_END = OFF_O + N * HD * 4;
+    // tensor memory: D1 of two tiles, D2 of two flush periods, K and V of two tiles
+    static constexpr int D1 = 0, D2 = 2 * N, K = 4 * N, V = K + HD, COLS = V + KT_TILE <= 256 ? 256 : 512;
 };
 template <int N> struct KtShared {
     float ks[KT_META][KT_TILE / 16], vs[KT_META][KT_TILE / 16];  // scales by 16 positions; ks NaN: not loaded
-    float m[N], own[N], top[4][N], sum[4][N];
+    int exponent[KT_META], hole[KT_META];                         // 2^exponent is above every value scale of the tile; whether some were not loaded
+    alignas(16) float m[N];
+    float own[N], alpha[N], top[4][N], sum[4][N];
     int limit[N];                                                 // positions a row attends
     float2 ml[N];
     float factor[2], row_factor[2][N], q_top[KT_CONV];            // score factors: of the tile's q, and beside it of a row
     int uneven[2];                                                // whether some row has a factor of its own
-    uint64_t k8_full[2], k8_empty[2], v8_full[2], v8_empty[2], kf_full, kf_empty, vf_full, d1_full[2], d1_empty[2],
-        p_full[2], o_done[2], q_full[2], q_empty[2], meta_full[KT_META], drained;
+    uint64_t k8_full[3], k8_empty[3], v8_full[3], v8_empty[3], kf_full[2], kf_empty[2], vf_full[2], d1_full[2],
+        d1_empty[2], p_full[2], o_done[2], q_full[2], q_empty[2], meta_full[KT_META], drained;
     uint32_t tmem;
     unsigned flag, dead;
 };
@@ -108,45 +163,41 @@ __global__ void __launch_bounds__(KT_THREADS, 1) kv8_tiles_kernel(Kv8Attention A
     const __grid_constant__ CUtensorMap vmap)
 {
     using S = KtShape<HD, N, QP>;
-    constexpr int C = N / 2, TM = N == 64 ? 256 : 128;  // columns of a softmax thread; TMEM columns
-    constexpr int KH = HD / 64;
+    constexpr int C = N / 2;  // columns of a softmax thread
     extern __shared__ unsigned char kt_smem[];
     unsigned char *ring = kt_smem + ((1024u - (smem_u32(kt_smem) & 1023u)) & 1023u);
     KtShared<N> &sh = *reinterpret_cast<KtShared<N> *>(ring + S::OFF_END);
-    const unsigned tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, kv = A.c.kv_heads, G = A.group;
+    const unsigned tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), kv = A.c.kv_heads, G = A.group;
     if (tid == 0) {
-        for (int i = 0; i < 2; ++i) {
+        for (int i = 0; i < S::STAGES; ++i) {
             mbar_init(sh.k8_full + i, 1); mbar_init(sh.k8_empty + i, KT_CONV);
             mbar_init(sh.v8_full + i, 1); mbar_init(sh.v8_empty + i, KT_CONV);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(sh.kf_full + i, KT_CONV); mbar_init(sh.kf_empty + i, 1); mbar_init(sh.vf_full + i, KT_CONV);
             mbar_init(sh.d1_full + i, 1); mbar_init(sh.d1_empty + i, KT_SOFT);
             mbar_init(sh.p_full + i, KT_SOFT); mbar_init(sh.o_done + i, 1);
             mbar_init(sh.q_full + i, KT_CONV); mbar_init(sh.q_empty + i, KT_SOFT);
         }
-        mbar_init(&sh.kf_full, KT_CONV); mbar_init(&sh.kf_empty, 1); mbar_init(&sh.vf_full, KT_CONV);
         for (int i = 0; i < KT_META; ++i) mbar_init(sh.meta_full + i, 1);
         mbar_init(&sh.drained, 1);
         sh.dead = 0;
         fence_barrier_init();
     }
     if (warp == KT_SOFT + KT_CONV + 1) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" :: "r"(smem_u32(&sh.tmem)), "r"(TM) : "memory");
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" :: "r"(smem_u32(&sh.tmem)), "r"(S::COLS) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
-    if (KH == 1)  // head_dim 64: the upper 64 rows of D2 come from zeros
-        for (unsigned i = tid; i < S::F16 / 2 / 16; i += KT_THREADS)
-            reinterpret_cast<uint4 *>(ring + S::OFF_VF + S::F16 / 2)[i] = make_uint4(0, 0, 0, 0);
     kt_fence_before();
     const Kv8Place place = kv8_place<KT_TILE, KT_THREADS>(A);  // CTA barriers inside
     kt_fence_after();
-    const uint32_t tmem = *(volatile uint32_t *)&sh.tmem, d2 = tmem + 2 * N;
+    const uint32_t tmem = *(volatile uint32_t *)&sh.tmem;
     Kv8Walk<KT_TILE> walk(A, place);
     Kv8Segment s;
     unsigned n = 0;  // tiles of this CTA so far
     volatile unsigned *dead = &sh.dead;  // a wait ran out: nobody waits any more, the error word is set
     auto wait = [&](uint64_t *bar, unsigned parity) {
-        if (*dead || mbar_wait_bounded(bar, parity & 1)) return;
-        *dead = 1;
-        raise_error(A.error, ERR_TIMEOUT);
+        kt_wait(bar, parity, dead, A.error);
     };
     auto arrive = [&](uint64_t *bar) { __syncwarp(); if (lane == 0) mbar_arrive(bar); };
 
@@ -163,7 +214,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1) kv8_tiles_kernel(Kv8Attention A
         };
         auto bar = [] { asm volatile("bar.sync 1, 256;" ::: "memory"); };
         constexpr float P_SCALE = 32.f;
-        unsigned seg = 0;
+        unsigned seg = 0, period = 0;
         while (walk.next(s)) {
             const int j0 = s.row_tile * (int)A.row_tile, nrows = min((int)A.row_tile, s.q.rows - j0) * (int)G;
             const int all = max(0, s.q.len - s.q.n + j0 + 1);  // positions every row attends
@@ -179,147 +230,187 @@ __global__ void __launch_bounds__(KT_THREADS, 1) kv8_tiles_kernel(Kv8Attention A
             arrive(sh.q_empty + (seg & 1));
             ++seg;
             group_bar();
-            float l[C], vref = 0.f;
+            // sums of p of the columns in work and of the other half of the group's; they change places per half
+            float l[16], l_other[16], vref = 0.f;
             int vexp = -200;
+            float *o = reinterpret_cast<float *>(ring + S::OFF_O) + col * HD + pos;  // this thread's sums, HD apart
+            const bool mine = HD == 128 || pos < HD;
 #pragma unroll
-            for (int i = 0; i < C; ++i) l[i] = 0.f;
+            for (int i = 0; i < 16; ++i) l[i] = l_other[i] = 0.f;
+            if (mine) {
+#pragma unroll 8
+                for (int i = 0; i < C; ++i) o[i * HD] = 0.f;
+            }
+            auto swap_halves = [&] {
+                if (C == 16) return;
+#pragma unroll
+                for (int i = 0; i < 16; ++i) { const float v = l[i]; l[i] = l_other[i]; l_other[i] = v; }
+            };
+            // adds the D2 of a finished period to o
+            auto flush = [&](unsigned which) {
+                kt_fence_after();
+#pragma unroll 1
+                for (int i0 = 0; i0 < C; i0 += 16) {
+                    float y[16];
+                    kt_ld16(tmem + S::D2 + (which & 1) * N + lanes + col + i0, y);
+                    float *oc = o + i0 * HD;
+                    kt_wait_ld();
+                    if (mine) {
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) oc[i * HD] += y[i];
+                    }
+                }
+                kt_fence_before();
+            };
+            bool pending = false;  // the period before has ended and is not in o yet
+            bool fresh = true;     // some row may not have a maximum yet
             for (int t = s.t0; t < s.t1; ++t, ++n) {
                 const unsigned b = n & 1, slot = n % KT_META;
+                const int step = (t - s.t0) % KT_FLUSH;
+                if (step == 0 && t > s.t0) { pending = true; ++period; }
                 wait(sh.meta_full + slot, n / KT_META);
-                const float ks = sh.ks[slot][pos >> 4], vs = sh.vs[slot][pos >> 4];
-                // largest value scale of the tile
-                int e = -200;
-#pragma unroll
-                for (int i = 0; i < KT_TILE / 16; ++i) {
-                    const float v = sh.vs[slot][i];
-                    if (v > 0.f) e = max(e, max(kt_exponent(v) + 1, -100));
+                const float ks = sh.ks[slot][pos >> 4], vs = sh.vs[slot][pos >> 4], f = factor * ks;
+                const int e = sh.exponent[slot];
+                const bool hole = sh.hole[slot], raw = fresh || hole || t * KT_TILE + KT_TILE > all, grow = e > vexp;
+                float down = 1.f;
+                if (__builtin_expect(grow, 0)) {
+                    down = vexp < -126 ? 0.f : kt_power(vexp - e);
+                    vexp = e;
+                    vref = kt_power(-e) * P_SCALE;
+                }
+                fresh = fresh && hole;
+                const float wv = vs * vref;
+                if (n >= 2) wait(sh.o_done + b, (n >> 1) - 1);
+                if (pending && step == 1) {  // its last tile is two back
+                    flush(period - 1);
+                    pending = false;
                 }
                 wait(sh.d1_full + b, n >> 1);
                 kt_fence_after();
-                float x[C];
+#pragma unroll 1
+                for (int i0 = 0; i0 < C; i0 += 16) {
+                    const unsigned c0 = col + i0;
+                    const float4 *m4 = reinterpret_cast<const float4 *>(sh.m + c0);
+                    float x[16];
+                    kt_ld16(tmem + S::D1 + lanes + b * N + c0, x);
+                    kt_wait_ld();
+                    if (__builtin_expect(uneven, 0)) {
 #pragma unroll
-                for (int i = 0; i < C; i += 16) kt_ld16(tmem + lanes + b * N + col + i, x + i);
-                kt_wait_ld();
-                kt_fence_before();
-                arrive(sh.d1_empty + b);
-                const float f = factor * ks;
-                if (uneven) {
-#pragma unroll
-                    for (int i = 0; i < C; ++i) x[i] *= sh.own[col + i];
-                }
-                const int at = t * KT_TILE + (int)pos;
-                float over = -INFINITY;
-                if (t * KT_TILE + KT_TILE <= all && !__any_sync(0xffffffffu, isnan(ks))) {
-#pragma unroll
-                    for (int i = 0; i < C; ++i) {
-                        x[i] *= f;
-                        over = fmaxf(over, x[i] - sh.m[col + i]);
+                        for (int i = 0; i < 16; ++i) x[i] *= sh.own[c0 + i];
                     }
-                } else {
-#pragma unroll
-                    for (int i = 0; i < C; ++i) {
-                        x[i] = at < sh.limit[col + i] && !isnan(ks) ? x[i] * f : -INFINITY;
-                        over = fmaxf(over, x[i] - sh.m[col + i]);
-                    }
-                }
-                if (group_or(over > 8.f || e > vexp)) {
-                    // ---- new maxima, and D2 and l in their units
-#pragma unroll
-                    for (int i = 0; i < C; ++i) {
-                        const float top = warp_max(x[i]);
-                        if (lane == 0) sh.top[warp & 3][col + i] = top;
-                    }
-                    group_bar();
-                    float down = 1.f;
-                    if (e > vexp) {
-                        down = vexp < -126 ? 0.f : kt_power(vexp - e);
-                        vexp = e;
-                        vref = kt_power(-e) * P_SCALE;
-                    }
-                    const bool has = t > s.t0;
-                    if (has) {
-                        wait(sh.o_done + (b ^ 1), (n - 1) >> 1);
-                        kt_fence_after();
-                    }
-#pragma unroll
-                    for (int i0 = 0; i0 < C; i0 += 16) {
-                        float y[16];
-                        if (has) { kt_ld16(d2 + lanes + col + i0, y); kt_wait_ld(); }
+                    // x: the scores less m, or (raw) the scores themselves
+                    float over = -INFINITY;
+                    if (__builtin_expect(raw, 0)) {
+                        const int at = isnan(ks) ? 0x7fffffff : t * KT_TILE + (int)pos;
 #pragma unroll
                         for (int i = 0; i < 16; ++i) {
-                            const unsigned c = col + i0 + i;
-                            const float old = sh.m[c];
-                            const float top = fmaxf(fmaxf(sh.top[0][c], sh.top[1][c]), fmaxf(sh.top[2][c], sh.top[3][c]));
-                            const float alpha = top > old + 8.f ? ex2(old - top) : 1.f;  // each row by its own scores
-                            l[i0 + i] *= alpha;
-                            y[i] *= alpha * down;
+                            x[i] = at < sh.limit[c0 + i] ? x[i] * f : -INFINITY;
+                            over = fmaxf(over, x[i] - sh.m[c0 + i]);
                         }
-                        if (has) { kt_st16(d2 + lanes + col + i0, y); kt_wait_st(); }
-                    }
-                    group_bar();
-                    if (pos < C) {
-                        const unsigned c = col + pos;
-                        const float top = fmaxf(fmaxf(sh.top[0][c], sh.top[1][c]), fmaxf(sh.top[2][c], sh.top[3][c]));
-                        if (top > sh.m[c] + 8.f) sh.m[c] = top;
-                    }
-                    group_bar();
-                }
-                // ---- weights, in halves, to shared memory
-                const float wv = vs * vref;
-                if (n >= S::P_STAGES) {
-                    const unsigned k = n - S::P_STAGES;
-                    wait(sh.o_done + (k & 1), k >> 1);
-                }
-                unsigned char *row = ring + S::OFF_P + n % S::P_STAGES * 2 * S::PB + pos * 128;
+                    } else {
 #pragma unroll
-                for (int i = 0; i < C; i += 8) {
-                    unsigned h[4], lo[4];
-#pragma unroll
-                    for (int j = 0; j < 8; j += 2) {
-                        const float p0 = ex2(x[i + j] - sh.m[col + i + j]), p1 = ex2(x[i + j + 1] - sh.m[col + i + j + 1]);
-                        l[i + j] += p0;
-                        l[i + j + 1] += p1;
-                        const float w0 = p0 * wv, w1 = p1 * wv;
-                        h[j / 2] = kt_pack(w0, w1);
-                        const float2 u = kt_unpack(h[j / 2]);
-                        lo[j / 2] = kt_pack(w0 - u.x, w1 - u.y);
+                        for (int i = 0; i < 16; i += 4) {
+                            const float4 m = m4[i / 4];
+                            x[i] = fmaf(x[i], f, -m.x); x[i + 1] = fmaf(x[i + 1], f, -m.y);
+                            x[i + 2] = fmaf(x[i + 2], f, -m.z); x[i + 3] = fmaf(x[i + 3], f, -m.w);
+                            over = fmaxf(fmaxf(over, fmaxf(x[i], x[i + 1])), fmaxf(x[i + 2], x[i + 3]));
+                        }
                     }
-                    const unsigned chunk = (((col + i) >> 3) ^ (pos & 7u)) << 4;
-                    *reinterpret_cast<uint4 *>(row + chunk) = make_uint4(h[0], h[1], h[2], h[3]);
-                    *reinterpret_cast<uint4 *>(row + S::PB + chunk) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+                    if (__builtin_expect(group_or(over > 8.f || grow), 0)) {
+                        // ---- new maxima, and the sums so far in their units
+                        if (!raw) {
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) x[i] += sh.m[c0 + i];
+                        }
+                        {
+                            float y[16];
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) y[i] = x[i];
+                            const float top = kt_reduce<16>(y, lane, [](float u, float v) { return fmaxf(u, v); });
+                            if (lane < 16) sh.top[warp & 3][c0 + lane] = top;
+                        }
+                        group_bar();
+                        if (pos < 16) {
+                            const unsigned c = c0 + pos;
+                            const float old = sh.m[c], top = fmaxf(fmaxf(sh.top[0][c], sh.top[1][c]), fmaxf(sh.top[2][c], sh.top[3][c]));
+                            const bool up = top > old + 8.f;  // each row by its own scores
+                            sh.alpha[c] = up ? ex2(old - top) : 1.f;
+                            if (up) sh.m[c] = top;
+                        }
+                        if (t > s.t0) wait(sh.o_done + (b ^ 1), (n - 1) >> 1);
+                        if (pending) {
+                            flush(period - 1);
+                            pending = false;
+                        }
+                        kt_fence_after();
+                        group_bar();
+                        const uint32_t d2 = tmem + S::D2 + (period & 1) * N + lanes + c0;
+                        float y[16];
+                        if (step) { kt_ld16(d2, y); kt_wait_ld(); }
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) {
+                            const float alpha = sh.alpha[c0 + i], both = alpha * down;
+                            l[i] *= alpha;
+                            if (mine) o[(i0 + i) * HD] *= both;
+                            y[i] *= both;
+                            x[i] -= sh.m[c0 + i];
+                        }
+                        if (step) { kt_st16(d2, y); kt_wait_st(); }
+                        kt_fence_before();
+                    } else if (__builtin_expect(raw, 0)) {
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) x[i] -= sh.m[c0 + i];
+                    }
+                    // ---- weights, in halves, to shared memory
+                    unsigned char *row = ring + S::OFF_P + b * 2 * S::PB + pos * 128;
+#pragma unroll
+                    for (int i = 0; i < 16; i += 8) {
+                        unsigned h[4], lo[4];
+#pragma unroll
+                        for (int j = 0; j < 8; j += 2) {
+                            const float p0 = ex2(x[i + j]), p1 = ex2(x[i + j + 1]);
+                            l[i + j] += p0;
+                            l[i + j + 1] += p1;
+                            const float w0 = p0 * wv, w1 = p1 * wv;
+                            h[j / 2] = kt_pack(w0, w1);
+                            const float2 u = kt_unpack(h[j / 2]);
+                            lo[j / 2] = kt_pack(w0 - u.x, w1 - u.y);
+                        }
+                        const unsigned chunk = (((c0 + i) >> 3) ^ (pos & 7u)) << 4;
+                        *reinterpret_cast<uint4 *>(row + chunk) = make_uint4(h[0], h[1], h[2], h[3]);
+                        *reinterpret_cast<uint4 *>(row + S::PB + chunk) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+                    }
+                    swap_halves();
                 }
-                fence_proxy_async();
                 kt_fence_before();
-                arrive(sh.p_full + n % S::P_STAGES);
+                fence_proxy_async();
+                __syncwarp();
+                if (lane == 0) { mbar_arrive(sh.d1_empty + b); mbar_arrive(sh.p_full + b); }
             }
             // ---- the segment's part: sums over positions, D2 in F32
             wait(sh.o_done + ((n - 1) & 1), (n - 1) >> 1);
-            kt_fence_after();
-#pragma unroll
-            for (int i = 0; i < C; ++i) {
-                const float v = warp_sum(l[i]);
-                if (lane == 0) sh.sum[warp & 3][col + i] = v;
-            }
+#pragma unroll 1
+            for (int back = pending ? 1 : 0; back >= 0; --back) flush(period - (unsigned)back);
+            ++period;
             const float back = vexp < -126 ? 0.f : kt_power(vexp) / P_SCALE;
-            float *o = reinterpret_cast<float *>(ring + S::OFF_P);  // P has been read
-            bar();
-#pragma unroll
+#pragma unroll 1
             for (int i0 = 0; i0 < C; i0 += 16) {
-                float y[16];
-                kt_ld16(d2 + lanes + col + i0, y);
-                kt_wait_ld();
-                if (HD == 128 || pos < HD) {
+                if (mine) {
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) o[(col + i0 + i) * HD + pos] = y[i] * back;
+                    for (int i = 0; i < 16; ++i) o[(i0 + i) * HD] *= back;
                 }
+                const float sum = kt_reduce<16>(l, lane, [](float u, float v) { return u + v; });
+                if (lane < 16) sh.sum[warp & 3][col + i0 + lane] = sum;
+                swap_halves();
             }
-            kt_fence_before();
+            group_bar();
             if (pos < C) {
                 const unsigned c = col + pos;
                 sh.ml[c] = make_float2(sh.m[c], sh.sum[0][c] + sh.sum[1][c] + sh.sum[2][c] + sh.sum[3][c]);
             }
             bar();
-            kv8_finish<N, HD, 32 * KT_SOFT>(A, s, place.units, tid, sh.ml, o, (unsigned)nrows, o, N * HD, &sh.flag, bar,
+            float *all_o = reinterpret_cast<float *>(ring + S::OFF_O);
+            kv8_finish<N, HD, 32 * KT_SOFT>(A, s, place.units, tid, sh.ml, all_o, (unsigned)nrows, all_o, N * HD, &sh.flag, bar,
                 [&](unsigned rho, unsigned chunk, float4 v) {
                     const size_t r = (size_t)(s.q.first + j0 + (int)(rho / G));
                     kv8_store4(A.out, A.type, r * A.out_stride + (size_t)(s.head * G + rho % G) * HD + 4 * chunk, v);
@@ -330,36 +421,74 @@ __global__ void __launch_bounds__(KT_THREADS, 1) kv8_tiles_kernel(Kv8Attention A
         // ================================================== q, and 8 bits to fp16
         const unsigned ct = tid - 32 * KT_SOFT;
         constexpr int PER = 128 / N, QV = HD / PER;  // threads of a q row, values of a thread
-        constexpr unsigned RC = HD / 16, STEP = 128 / RC;  // chunks of an 8-bit row; rows that the threads take at once
+        const unsigned cw = warp - KT_SOFT;
+        const uint32_t lanes = (cw * 32u) << 16;
         auto conv_bar = [] { asm volatile("bar.sync 2, 128;" ::: "memory"); };
-        auto convert = [&](unsigned src, unsigned dst, int rows, unsigned slot) {
-            const unsigned c = ct % RC, r0 = ct / RC;
+        // K of tile i: a thread converts its position's row, column c of its lane gets values 2c and 2c + 1
+        auto keys = [&](unsigned i) {
+            const unsigned st = i % S::STAGES, pos = ct;
+            wait(sh.k8_full + st, i / S::STAGES);
+            if (i >= 2) wait(sh.kf_empty + (i & 1), (i >> 1) - 1);
+            kt_fence_after();
+            const unsigned char *src = ring + S::OFF_K8 + st * S::STAGE + pos * HD;
+            const unsigned z = kv8_swizzle<HD>(pos);
+#pragma unroll 2
+            for (unsigned c = 0; c < HD / 16; c += 2) {
+                unsigned h[16];
 #pragma unroll
-            for (unsigned i = 0; i < KT_TILE / STEP; ++i) {
-                const unsigned r = r0 + i * STEP;
-                uint4 v = *reinterpret_cast<const uint4 *>(ring + src + r * HD + ((c ^ kv8_swizzle<HD>(r)) << 4));
-                // rows past the last position or never loaded: 0, not what lies there (a NaN stays one times 0)
-                if (rows >= 0 && ((int)r >= rows || isnan(sh.ks[slot][r >> 4]))) v = make_uint4(0, 0, 0, 0);
-                unsigned h[8];
-                kv8_halves<FMT>(v.x, h[0], h[1]);
-                kv8_halves<FMT>(v.y, h[2], h[3]);
-                kv8_halves<FMT>(v.z, h[4], h[5]);
-                kv8_halves<FMT>(v.w, h[6], h[7]);
-                const unsigned half = c / 4, k = 2 * (c % 4), z = r & 7u;
-                unsigned char *row = ring + dst + half * (S::F16 / 2) + r * 128;
-                // the two halves' lanes start on different banks
-                const uint4 a = make_uint4(h[0], h[1], h[2], h[3]), b = make_uint4(h[4], h[5], h[6], h[7]);
-                *reinterpret_cast<uint4 *>(row + (((k + half) ^ z) << 4)) = half ? b : a;
-                *reinterpret_cast<uint4 *>(row + (((k + 1 - half) ^ z) << 4)) = half ? a : b;
+                for (int k = 0; k < 2; ++k) {
+                    const uint4 v = *reinterpret_cast<const uint4 *>(src + (((c + k) ^ z) << 4));
+                    kv8_halves<FMT>(v.x, h[8 * k], h[8 * k + 1]);
+                    kv8_halves<FMT>(v.y, h[8 * k + 2], h[8 * k + 3]);
+                    kv8_halves<FMT>(v.z, h[8 * k + 4], h[8 * k + 5]);
+                    kv8_halves<FMT>(v.w, h[8 * k + 6], h[8 * k + 7]);
+                }
+                kt_st16(tmem + S::K + (i & 1) * (HD / 2) + lanes + c * 8, reinterpret_cast<float *>(h));
             }
-            fence_proxy_async();
+            arrive(sh.k8_empty + st);
+            kt_wait_st();
+            kt_fence_before();
+            arrive(sh.kf_full + (i & 1));
         };
-        auto keys = [&](unsigned i) {  // K of tile i
-            wait(sh.k8_full + (i & 1), i >> 1);
-            if (i) wait(&sh.kf_empty, i - 1);
-            convert(S::OFF_K8 + (i & 1) * S::STAGE, S::OFF_KF, -1, 0);
-            arrive(sh.k8_empty + (i & 1));
-            arrive(&sh.kf_full);
+        // V of tile n, transposed: lane = head dimension, column c gets positions 2c and 2c + 1; positions from `rows`
+        // on, or never loaded, are 0 and not what lies there (a NaN stays one times 0)
+        auto values = [&](int rows) {
+            const unsigned st = n % S::STAGES, slot = n % KT_META;
+            wait(sh.v8_full + st, n / S::STAGES);
+            if (n >= 2) wait(sh.o_done + (n & 1), (n >> 1) - 1);
+            kt_fence_after();
+            const bool patchy = sh.hole[slot] || rows < KT_TILE;
+            if (cw < HD / 32) {
+                const unsigned r = lane & 15, chunk = 2 * cw + (lane >> 4), t4 = lane & 3;
+                const unsigned src = smem_u32(ring + S::OFF_V8 + st * S::STAGE) + r * HD + ((chunk ^ kv8_swizzle<HD>(r)) << 4);
+#pragma unroll 1
+                for (int j0 = 0; j0 < KT_TILE / 16; j0 += 4) {
+                    unsigned lo[16], hi[16];  // dimensions 0..15 and 16..31 of the warp's, 64 positions
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        unsigned w[4];
+                        asm volatile("ldmatrix.sync.aligned.m16n16.x2.trans.shared.b8 {%0,%1,%2,%3}, [%4];"
+                                     : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(src + (j0 + j) * 16 * HD));
+                        const int first = (j0 + j) * 16;
+                        if (__builtin_expect(patchy, 0)) {
+                            const int left = isnan(sh.ks[slot][j0 + j]) ? 0 : rows - first - 4 * (int)t4;
+                            const unsigned keep = left >= 4 ? 0xffffffffu : left <= 0 ? 0u : (1u << 8 * left) - 1;
+                            w[0] &= keep; w[1] &= keep; w[2] &= keep; w[3] &= keep;
+                        }
+                        kv8_halves<FMT>(w[0], lo[4 * j], lo[4 * j + 1]);
+                        kv8_halves<FMT>(w[1], lo[4 * j + 2], lo[4 * j + 3]);
+                        kv8_halves<FMT>(w[2], hi[4 * j], hi[4 * j + 1]);
+                        kv8_halves<FMT>(w[3], hi[4 * j + 2], hi[4 * j + 3]);
+                    }
+                    const uint32_t dst = tmem + S::V + (n & 1) * (KT_TILE / 2) + lanes + j0 * 8;
+                    kt_st256(dst, lo);
+                    kt_st256(dst + (16u << 16), hi);
+                }
+                kt_wait_st();
+            }
+            kt_fence_before();
+            arrive(sh.v8_empty + st);
+            arrive(sh.vf_full + (n & 1));
         };
         unsigned seg = 0, k_at = 0;  // K tiles converted
         while (walk.next(s)) {
@@ -369,42 +498,41 @@ __global__ void __launch_bounds__(KT_THREADS, 1) kv8_tiles_kernel(Kv8Attention A
             // tile's largest gets its own, so that no row's low half runs into fp16's smallest numbers
             {
                 const unsigned row = ct / PER, d0 = ct % PER * QV;
-                float x[QV];
+                const bool real = (int)row < nrows;
+                const size_t r = (size_t)(s.q.first + j0 + (real ? (int)(row / G) : 0));
+                const size_t base = r * A.q_stride + (size_t)(s.head * G + (real ? row % G : 0)) * HD + d0;
                 float own = 0.f;
                 auto size_of = [](float v) { v = fabsf(v); return v <= 3.4028235e38f ? v : 0.f; };  // 0 for inf and NaN
-                if ((int)row < nrows) {
-                    const size_t r = (size_t)(s.q.first + j0 + (int)(row / G));
-                    const size_t base = r * A.q_stride + (size_t)(s.head * G + row % G) * HD + d0;
-#pragma unroll
-                    for (int i = 0; i < QV; i += 4) {
-                        const float4 v = kv8_load4(A.q, A.type, base + i);
-                        x[i] = v.x; x[i + 1] = v.y; x[i + 2] = v.z; x[i + 3] = v.w;
-                        own = fmaxf(own, fmaxf(fmaxf(size_of(v.x), size_of(v.y)), fmaxf(size_of(v.z), size_of(v.w))));
-                    }
-                } else {
-#pragma unroll
-                    for (int i = 0; i < QV; ++i) x[i] = 0.f;
+#pragma unroll 2
+                for (int i = 0; i < QV; i += 4) {
+                    const float4 v = kv8_load4(A.q, A.type, base + i);
+                    own = fmaxf(own, fmaxf(fmaxf(size_of(v.x), size_of(v.y)), fmaxf(size_of(v.z), size_of(v.w))));
                 }
+                if (!real) own = 0.f;
 #pragma unroll
                 for (int o = 1; o < PER; o <<= 1) own = fmaxf(own, __shfl_xor_sync(0xffffffffu, own, o));
                 float top = warp_max(own);
-                if (lane == 0) sh.q_top[warp - KT_SOFT] = top;
+                if (lane == 0) sh.q_top[cw] = top;
                 conv_bar();
                 top = fmaxf(fmaxf(sh.q_top[0], sh.q_top[1]), fmaxf(sh.q_top[2], sh.q_top[3]));
                 const int below = own > 0.f ? kt_exponent(top) - kt_exponent(own) : 0, extra = below > 12 ? below : 0;
                 const int common = 14 - kt_exponent(top), e = common + extra;
-                const float up = kt_power(min(e, 127)), up2 = kt_power(e - min(e, 127));
-                if (k_at) wait(&sh.kf_empty, k_at - 1);  // the last segment's products have read their q
+                const float up = real ? kt_power(min(e, 127)) : 0.f, up2 = kt_power(e - min(e, 127));
+                if (k_at) wait(sh.kf_empty + ((k_at - 1) & 1), (k_at - 1) >> 1);  // the last segment's products have read their q
                 if (seg >= 2) wait(sh.q_empty + (seg & 1), (seg >> 1) - 1);
-#pragma unroll
+#pragma unroll 1
                 for (int i = 0; i < QV; i += 8) {
                     unsigned h[4], lo[4];
 #pragma unroll
-                    for (int j = 0; j < 8; j += 2) {
-                        const float a = x[i + j] * up * up2, b = x[i + j + 1] * up * up2;
-                        h[j / 2] = kt_pack(a, b);
-                        const float2 u = kt_unpack(h[j / 2]);
-                        lo[j / 2] = kt_pack(a - u.x, b - u.y);
+                    for (int j = 0; j < 8; j += 4) {
+                        const float4 v = kv8_load4(A.q, A.type, base + i + j);
+                        const float x0 = real ? v.x * up * up2 : 0.f, x1 = real ? v.y * up * up2 : 0.f,
+                                    x2 = real ? v.z * up * up2 : 0.f, x3 = real ? v.w * up * up2 : 0.f;
+                        h[j / 2] = kt_pack(x0, x1);
+                        h[j / 2 + 1] = kt_pack(x2, x3);
+                        const float2 a = kt_unpack(h[j / 2]), b = kt_unpack(h[j / 2 + 1]);
+                        lo[j / 2] = kt_pack(x0 - a.x, x1 - a.y);
+                        lo[j / 2 + 1] = kt_pack(x2 - b.x, x3 - b.y);
                     }
                     const unsigned d = d0 + i, chunk = d % 64 / 8;
                     unsigned char *q = ring + S::OFF_Q + d / 64 * (N * 128) + row * 128 + ((chunk ^ (row & 7u)) << 4);
@@ -422,15 +550,13 @@ __global__ void __launch_bounds__(KT_THREADS, 1) kv8_tiles_kernel(Kv8Attention A
                 arrive(sh.q_full + (seg & 1));
                 ++seg;
             }
-            // K one tile ahead of V: V's buffer is free only when the tile before has been weighted
-            keys(k_at++);
-            for (int t = s.t0; t < s.t1; ++t, ++n) {
+#pragma unroll 1
+            for (int t = s.t0 - 1; t < s.t1; ++t) {  // K one tile ahead of V
                 if (t + 1 < s.t1) keys(k_at++);
-                wait(sh.v8_full + (n & 1), n >> 1);
-                if (n) wait(sh.o_done + ((n - 1) & 1), (n - 1) >> 1);
-                convert(S::OFF_V8 + (n & 1) * S::STAGE, S::OFF_VF, any - t * KT_TILE < 0 ? 0 : any - t * KT_TILE, n % KT_META);
-                arrive(sh.v8_empty + (n & 1));
-                arrive(&sh.vf_full);
+                if (t >= s.t0) {
+                    values(any - t * KT_TILE);
+                    ++n;
+                }
             }
         }
     } else if (warp == KT_SOFT + KT_CONV) {
@@ -453,7 +579,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1) kv8_tiles_kernel(Kv8Attention A
                     vs = ok ? A.c.v_scale[(size_t)id * kv + s.head] : 0.f;
                     if (!ok) id = -1;
                 }
-                const unsigned b = n & 1, slot = n % KT_META;
+                const unsigned b = n % S::STAGES, slot = n % KT_META;
                 const unsigned group_block = (unsigned)(b0 & 31) + (lane % (KT_TILE / 16) * 16 >> min(A.shift, 7u));
                 const float gk = __shfl_sync(0xffffffffu, ks, group_block & 31u), gv = __shfl_sync(0xffffffffu, vs, group_block & 31u);
                 const unsigned box_block = (unsigned)(b0 & 31) + (lane % per * box >> A.shift);
@@ -461,8 +587,10 @@ __global__ void __launch_bounds__(KT_THREADS, 1) kv8_tiles_kernel(Kv8Attention A
                 const bool load = lane < per && mine >= 0;
                 const unsigned boxes = __popc(__ballot_sync(0xffffffffu, load));
                 const int row = (int)((((unsigned)mine * kv + s.head) << A.shift) + ((unsigned)(t * KT_TILE + (int)(lane % per * box)) & (size - 1)));
-                if (n >= 2) wait(sh.k8_empty + b, (n >> 1) - 1);
-                if (lane < KT_TILE / 16) { sh.ks[slot][lane] = gk; sh.vs[slot][lane] = gv; }
+                if (n >= S::STAGES) wait(sh.k8_empty + b, n / S::STAGES - 1);
+                const bool hole = __any_sync(0xffffffffu, isnan(gk));
+                const int top = __reduce_max_sync(0xffffffffu, gv > 0.f ? max(kt_exponent(gv) + 1, -100) : -200);
+                if (lane < KT_TILE / 16) { sh.ks[slot][lane] = gk; sh.vs[slot][lane] = gv; sh.exponent[slot] = top; sh.hole[slot] = hole; }
                 __syncwarp();
                 if (lane == 0) {
                     mbar_arrive(sh.meta_full + slot);
@@ -470,7 +598,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1) kv8_tiles_kernel(Kv8Attention A
                 }
                 __syncwarp();
                 if (load && !*dead) tma_load_rows(ring + S::OFF_K8 + b * S::STAGE + lane * box * HD, &kmap, row, sh.k8_full + b);
-                if (n >= 2) wait(sh.v8_empty + b, (n >> 1) - 1);
+                if (n >= S::STAGES) wait(sh.v8_empty + b, n / S::STAGES - 1);
                 __syncwarp();
                 if (lane == 0) {
                     if (boxes) mbar_expect_tx(sh.v8_full + b, boxes * box * HD); else mbar_arrive(sh.v8_full + b);
@@ -480,57 +608,77 @@ __global__ void __launch_bounds__(KT_THREADS, 1) kv8_tiles_kernel(Kv8Attention A
             }
         }
         if (*dead) {  // copies in flight land before the CTA leaves its shared memory
-            for (unsigned i = 0; i < min(n, 2u); ++i) {
-                mbar_wait_bounded(sh.k8_full + ((n - 1 - i) & 1), (n - 1 - i) >> 1 & 1);
-                mbar_wait_bounded(sh.v8_full + ((n - 1 - i) & 1), (n - 1 - i) >> 1 & 1);
+            for (unsigned i = 0; i < min(n, (unsigned)S::STAGES); ++i) {
+                const unsigned k = n - 1 - i;
+                mbar_wait_bounded(sh.k8_full + k % S::STAGES, k / S::STAGES & 1);
+                mbar_wait_bounded(sh.v8_full + k % S::STAGES, k / S::STAGES & 1);
             }
         }
-    } else if (lane == 0) {
+    } else {
         // ================================================== MMA
-        const unsigned kf = smem_u32(ring + S::OFF_KF), vf = smem_u32(ring + S::OFF_VF), qs = smem_u32(ring + S::OFF_Q),
-                       ps = smem_u32(ring + S::OFF_P);
-        unsigned k_at = 0;
+        // The warp runs as one and an elected lane issues: operands then sit in uniform registers. (With the role in
+        // a branch of one lane an MMA took 135 cycles to issue, four times what it takes to run.)
+        const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
+        const uint64_t qs = kt_desc(smem_u32(ring + S::OFF_Q), 16), ps = kt_desc(smem_u32(ring + S::OFF_P), S::PB);
+        unsigned k_at = 0, period = 0;
         auto scores = [&] {
             const unsigned b = k_at & 1;
-            wait(&sh.kf_full, k_at);
+            wait(sh.kf_full + b, k_at >> 1);
             if (k_at >= 2) wait(sh.d1_empty + b, (k_at >> 1) - 1);
             kt_fence_after();
+            __syncwarp();
+            if (kt_elect()) {
+                const uint32_t d = tm + S::D1 + b * N, a = tm + S::K + b * (HD / 2);
 #pragma unroll
-            for (int part = 0; part < QP; ++part)
+                for (int part = 0; part < QP; ++part)
 #pragma unroll
-                for (int k = 0; k < HD / 16; ++k)
-                    kt_mma(tmem + b * N, kt_desc(kf + k / 4 * (S::F16 / 2) + k % 4 * 32, 16),
-                           kt_desc(qs + part * S::QB + k / 4 * (N * 128) + k % 4 * 32, 16), kt_idesc(N, false), part || k);
-            kt_commit(&sh.kf_empty);
-            kt_commit(sh.d1_full + b);
+                    for (int k = 0; k < HD / 16; ++k)
+                        kt_mma(d, a + 8 * k, qs + (((QP - 1 - part) * S::QB + k / 4 * (N * 128) + k % 4 * 32) >> 4),
+                               kt_idesc(N, false), part || k);
+                kt_commit(sh.kf_empty + b);
+                kt_commit(sh.d1_full + b);
+            }
+            __syncwarp();
             ++k_at;
         };
         while (walk.next(s)) {
-            scores();
-            for (int t = s.t0; t < s.t1; ++t, ++n) {
+#pragma unroll 1
+            for (int t = s.t0 - 1; t < s.t1; ++t) {  // scores one tile ahead of values
                 if (t + 1 < s.t1) scores();
-                const unsigned b = n % S::P_STAGES;
-                wait(&sh.vf_full, n);
-                wait(sh.p_full + b, n / S::P_STAGES);
+                if (t < s.t0) continue;
+                const unsigned b = n & 1;
+                const int step = (t - s.t0) % KT_FLUSH;
+                if (step == 0 && t > s.t0) ++period;
+                wait(sh.vf_full + b, n >> 1);
+                wait(sh.p_full + b, n >> 1);
                 kt_fence_after();
+                __syncwarp();
+                if (kt_elect()) {
+                    const uint32_t d = tm + S::D2 + (period & 1) * N, a = tm + S::V + b * (KT_TILE / 2);
+                    const uint64_t p = ps + (b * 2 * S::PB >> 4);
 #pragma unroll
-                for (int part = 0; part < 2; ++part)
+                    for (int part = 0; part < 2; ++part)
 #pragma unroll
-                    for (int k = 0; k < KT_TILE / 16; ++k)
-                        kt_mma(d2, kt_desc(vf + k * 2048, S::F16 / 2),
-                               kt_desc(ps + (2 * b + (unsigned)part) * S::PB + k * 2048, S::PB), kt_idesc(N, true),
-                               t > s.t0 || part || k);
-                kt_commit(sh.o_done + (n & 1));
+                        for (int k = 0; k < KT_TILE / 16; ++k)
+                            kt_mma(d, a + 8 * k, p + (((1 - part) * S::PB + k * 2048) >> 4), kt_idesc(N, true), step || part || k);
+                    kt_commit(sh.o_done + b);
+                }
+                __syncwarp();
+                ++n;
             }
+            ++period;
         }
-        kt_commit(&sh.drained);
-        mbar_wait_bounded(&sh.drained, 0);
+        if (kt_elect()) {
+            kt_commit(&sh.drained);
+            mbar_wait_bounded(&sh.drained, 0);
+        }
+        __syncwarp();
     }
     kt_fence_before();
     __syncthreads();
     if (warp == KT_SOFT + KT_CONV + 1) {
         kt_fence_after();
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" :: "r"(tmem), "r"(TM) : "memory");
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" :: "r"(tmem), "r"(S::COLS) : "memory");
     }
 }
 
