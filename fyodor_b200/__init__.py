@@ -247,50 +247,19 @@ class SynthModel:
 # every output as it was.
 KV8_INT8, KV8_E4M3 = 0, 1
 ROPE_KINDS = {"plain": 0, "linear": 1, "ntk": 2, "yarn": 3, "bands": 4}
-ROPE_LAYOUTS = {"interleaved": 0, "half": 1}
-_row_types = None
+_native = None
 
 
-def _row_type(t):
-    """GGML id of a row tensor's type."""
-    global _row_types
-    if _row_types is None:
-        import torch
-        _row_types = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}
-    r = _row_types.get(t.dtype)
-    if r is None:
-        raise ValueError("rows are float32, float16 or bfloat16, not %s" % t.dtype)
-    return r
-
-
-def _stream_of(t, stream):
-    import torch
-    index = t.get_device()
-    if index != torch.cuda.current_device():
-        raise ValueError("tensors are on device %d, the current device is %d" % (index, torch.cuda.current_device()))
-    return torch.cuda.current_stream(index).cuda_stream if stream is None else stream
-
-
-def _dev(name, t, kind, count=None):
-    """Pointer of a contiguous device tensor of one element type, of `count` elements at least."""
-    if t.dtype is not kind or not t.is_cuda or not t.is_contiguous():
-        raise ValueError("%s has to be a contiguous %s tensor on the GPU" % (name, kind))
-    if count is not None and t.numel() < count:
-        raise ValueError("%s has %d elements, %d are needed" % (name, t.numel(), count))
-    return t.data_ptr()
-
-
-def _rows_of(name, t, heads=None, head_dim=None):
-    """(pointer, row stride) of rows [rows][heads][head_dim] whose heads are contiguous."""
-    if t.dim() != 3 or not t.is_cuda:
-        raise ValueError("%s has to be [rows][heads][head_dim] on the GPU" % name)
-    n, h, d = t.shape
-    if (heads is not None and h != heads) or (head_dim is not None and d != head_dim):
-        raise ValueError("%s has rows of %d x %d, not %s x %s" % (name, h, d, heads, head_dim))
-    sr, sh, sd = t.stride()
-    if (sd != 1 and d > 1) or (sh != d and h > 1):
-        raise ValueError("the heads of a row of %s have to be contiguous" % name)
-    return t.data_ptr(), sr if n > 1 else max(sr, h * d)
+def _bind_tensors():
+    """The extension that takes torch tensors (csrc/tensors.cc), bound to the library on first use."""
+    global _native
+    if _native is None:
+        import torch  # noqa: F401  (the extension links against it)
+        from . import _tensors as ext
+        ext.bind(*(C.cast(f, C.c_void_p).value for f in (lib.fyb_kv_blocks, lib.fyb_kv_release, lib.fyb_rope,
+                                                         lib.fyb_kv8_append, lib.fyb_kv8_read, lib.fyb_kv8_attention)))
+        _native = ext
+    return _native
 
 
 def _check(r, what):
@@ -300,14 +269,6 @@ def _check(r, what):
         raise RuntimeError("%s failed to launch (%d)" % (what, r))
 
 
-def _rope_desc(cos, sin, layout):
-    import torch
-    if cos.dim() != 2 or cos.shape != sin.shape or layout not in ROPE_LAYOUTS:
-        raise ValueError("cos and sin are [positions][dims / 2] of one shape, layout one of %s" % sorted(ROPE_LAYOUTS))
-    return RopeDesc(_dev("cos", cos, torch.float32), _dev("sin", sin, torch.float32), cos.shape[0], 2 * cos.shape[1],
-                    ROPE_LAYOUTS[layout])
-
-
 def kv_blocks(lengths, new_tokens, table, free_list, free_count, block_size, lengths_out, free_count_out, row_start,
               slots, positions, row_request, status, stream=None):
     """Block tables and slot maps of one serving step (fyb_kv_blocks). All
@@ -315,30 +276,13 @@ def kv_blocks(lengths, new_tokens, table, free_list, free_count, block_size, len
     [requests][blocks], extended in place; free_list with free_count [1]
     entries; row_start [requests + 1]; slots, positions and row_request
     [max_rows]."""
-    import torch
-    i32, n, rows = torch.int32, lengths.numel(), slots.numel()
-    if table.dim() != 2 or table.shape[0] != n:
-        raise ValueError("table has to be [requests][blocks]")
-    r = lib.fyb_kv_blocks(
-        _dev("lengths", lengths, i32), _dev("new_tokens", new_tokens, i32, n), n, _dev("table", table, i32), table.shape[1],
-        block_size, _dev("free_list", free_list, i32), _dev("free_count", free_count, i32, 1),
-        _dev("lengths_out", lengths_out, i32, n), _dev("free_count_out", free_count_out, i32, 1),
-        _dev("row_start", row_start, i32, n + 1), _dev("slots", slots, i32), _dev("positions", positions, i32, rows),
-        _dev("row_request", row_request, i32, rows), rows, _dev("status", status, i32, n),
-        _stream_of(lengths, stream))
-    _check(r, "fyb_kv_blocks")
+    (_native or _bind_tensors()).kv_blocks(lengths, new_tokens, table, free_list, free_count, block_size, lengths_out,
+                                      free_count_out, row_start, slots, positions, row_request, status, stream)
 
 
 def kv_release(lengths, done, table, free_list, free_count, block_size, stream=None):
     """Give the blocks of the requests with done[r] != 0 back (fyb_kv_release, in place)."""
-    import torch
-    i32, n = torch.int32, lengths.numel()
-    if table.dim() != 2 or table.shape[0] != n:
-        raise ValueError("table has to be [requests][blocks]")
-    r = lib.fyb_kv_release(_dev("lengths", lengths, i32), _dev("done", done, i32, n), n, _dev("table", table, i32),
-                           table.shape[1], block_size, _dev("free_list", free_list, i32),
-                           _dev("free_count", free_count, i32, 1), free_list.numel(), _stream_of(lengths, stream))
-    _check(r, "fyb_kv_release")
+    (_native or _bind_tensors()).kv_release(lengths, done, table, free_list, free_count, block_size, stream)
 
 
 def rope_frequencies(dims, base, kind="plain", factor=1.0, original_context=0.0, beta_fast=0.0, beta_slow=0.0,
@@ -361,38 +305,21 @@ def rope_frequencies(dims, base, kind="plain", factor=1.0, original_context=0.0,
 def rope_tables(freq, magnitude, rows, first=0, stream=None):
     """cos and sin [rows][len(freq)] of positions first .. first + rows (device tensors; freq on the device)."""
     import torch
+    if not freq.is_cuda or freq.dtype != torch.float32 or not freq.is_contiguous() or \
+            freq.get_device() != torch.cuda.current_device():
+        raise ValueError("freq has to be a contiguous float32 tensor on the current CUDA device")
     c, s = (torch.empty((rows, freq.numel()), dtype=torch.float32, device=freq.device) for _ in range(2))
-    _check(lib.fyb_rope_tables(_dev("freq", freq, torch.float32), 2 * freq.numel(), magnitude, first, rows,
-                               c.data_ptr(), s.data_ptr(), _stream_of(freq, stream)), "fyb_rope_tables")
+    if stream is None:
+        stream = torch.cuda.current_stream(freq.device).cuda_stream
+    _check(lib.fyb_rope_tables(freq.data_ptr(), 2 * freq.numel(), magnitude, first, rows, c.data_ptr(), s.data_ptr(),
+                               stream), "fyb_rope_tables")
     return c, s
 
 
 def rope(q, k, positions, cos, sin, layout, q_out, k_out, error=None, stream=None):
     """q_out, k_out = q, k [rows][heads][head_dim] rotated to positions[row]
     by the tables (fyb_rope); k and k_out may be None; outputs may be their inputs."""
-    import torch
-    qp, qs = _rows_of("q", q)
-    rows, heads, hd = q.shape
-    op, os_ = _rows_of("q_out", q_out, heads, hd)
-    kp = ks = kop = kos = kv = 0
-    if k is not None:
-        kv = k.shape[1]
-        kp, ks = _rows_of("k", k, kv, hd)
-        kop, kos = _rows_of("k_out", k_out, kv, hd)
-        if k.dtype != q.dtype or k_out.dtype != q.dtype or k.shape[0] != rows or k_out.shape[0] != rows:
-            raise ValueError("k and k_out have to have q's type and rows")
-    if q_out.dtype != q.dtype or q_out.shape[0] != rows:
-        raise ValueError("q_out has to have q's type and rows")
-    d = _rope_desc(cos, sin, layout)
-    _check(lib.fyb_rope(C.byref(d), _dev("positions", positions, torch.int32, rows), rows, hd, _row_type(q), qp, qs, op,
-                        os_, heads, kp, ks, kop, kos, kv, _error_ptr(error), _stream_of(q, stream)), "fyb_rope")
-
-
-def _error_ptr(error):
-    if error is None:
-        return None
-    import torch
-    return _dev("error", error, torch.int32, 1)
+    (_native or _bind_tensors()).rope(q, k, positions, cos, sin, layout, q_out, k_out, error, stream)
 
 
 class KV8Cache:
@@ -407,12 +334,15 @@ class KV8Cache:
                 v_scale.shape != k.shape[:2]:
             raise ValueError("k, v: [blocks][kv_heads][block_size][head_dim] int8 or float8_e4m3fn; scales "
                              "[blocks][kv_heads]")
+        for name, t, kind in (("k", k, k.dtype), ("v", v, k.dtype), ("k_scale", k_scale, torch.float32),
+                              ("v_scale", v_scale, torch.float32)):
+            if t.dtype is not kind or not t.is_cuda or not t.is_contiguous() or t.device != k.device:
+                raise ValueError("%s has to be a contiguous %s tensor on the cache's GPU" % (name, kind))
         self.tensors = k, v, k_scale, v_scale
         blocks, self.kv_heads, self.block_size, self.head_dim = k.shape
-        self.desc = KV8CacheDesc(_dev("k", k, k.dtype), _dev("v", v, k.dtype),
-                                 _dev("k_scale", k_scale, torch.float32), _dev("v_scale", v_scale, torch.float32),
-                                 blocks, self.kv_heads, self.block_size, self.head_dim, kinds[k.dtype])
-        self._i32, self._ref = torch.int32, C.byref(self.desc)
+        self.desc = KV8CacheDesc(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), blocks,
+                                 self.kv_heads, self.block_size, self.head_dim, kinds[k.dtype])
+        self._handle = C.addressof(self.desc)
 
     @classmethod
     def empty(cls, blocks, kv_heads, block_size, head_dim, format="int8", device="cuda"):
@@ -428,34 +358,11 @@ class KV8Cache:
         """Store K and V rows [rows][kv_heads][head_dim] at slots[row]
         (fyb_kv8_append). With cos / sin K is rotated to positions[row] first,
         and q to q_out in the same launch."""
-        kp, ks = _rows_of("k", k, self.kv_heads, self.head_dim)
-        vp, vs = _rows_of("v", v, self.kv_heads, self.head_dim)
-        rows = k.shape[0]
-        if v.dtype != k.dtype or v.shape[0] != rows:
-            raise ValueError("v has to have k's type and rows")
-        rope = pos = qp = qo = None
-        qs = os_ = heads = 0
-        if cos is not None:
-            rope = C.byref(_rope_desc(cos, sin, layout))
-            pos = _dev("positions", positions, self._i32, rows)
-        if q is not None:
-            heads = q.shape[1]
-            qp, qs = _rows_of("q", q, heads, self.head_dim)
-            qo, os_ = _rows_of("q_out", q_out, heads, self.head_dim)
-            if q.dtype != k.dtype or q_out.dtype != k.dtype or q.shape[0] != rows or q_out.shape[0] != rows:
-                raise ValueError("q and q_out have to have k's type and rows")
-        _check(lib.fyb_kv8_append(self._ref, _dev("slots", slots, self._i32, rows), rows, _row_type(k), kp, ks, vp, vs,
-                                  rope, pos, qp, qs, qo, os_, heads, _error_ptr(error), _stream_of(k, stream)),
-               "fyb_kv8_append")
+        (_native or _bind_tensors()).append(self._handle, k, v, slots, positions, cos, sin, layout, q, q_out, error, stream)
 
     def read(self, slots, k_out, v_out, error=None, stream=None):
         """The values held at slots into k_out, v_out [len(slots)][kv_heads][head_dim] float32 (fyb_kv8_read)."""
-        rows = slots.numel()
-        need = rows * self.kv_heads * self.head_dim
-        f32 = self.tensors[2].dtype
-        _check(lib.fyb_kv8_read(self._ref, _dev("slots", slots, self._i32), rows, _dev("k_out", k_out, f32, need),
-                                _dev("v_out", v_out, f32, need), _error_ptr(error), _stream_of(slots, stream)),
-               "fyb_kv8_read")
+        (_native or _bind_tensors()).read(self._handle, slots, k_out, v_out, error, stream)
 
     def attention_workspace(self, requests, most_rows, heads):
         """A zeroed workspace for attention() calls of this size (one for each stream that calls)."""
@@ -472,18 +379,8 @@ class KV8Cache:
         blocks (fyb_kv8_attention): q, out [rows][heads][head_dim], lengths
         [requests], table [requests][blocks]; row_start [requests + 1] where a
         request has other than one row, at most most_rows each."""
-        qp, qs = _rows_of("q", q, None, self.head_dim)
-        rows, heads = q.shape[0], q.shape[1]
-        op, os_ = _rows_of("out", out, heads, self.head_dim)
-        n = lengths.numel()
-        if out.dtype != q.dtype or out.shape[0] != rows or table.dim() != 2 or table.shape[0] != n:
-            raise ValueError("out has to have q's type and rows, table [requests][blocks]")
-        _check(lib.fyb_kv8_attention(
-            self._ref, _dev("lengths", lengths, self._i32),
-            None if row_start is None else _dev("row_start", row_start, self._i32, n + 1), n, most_rows, rows,
-            _dev("table", table, self._i32), table.shape[1], _row_type(q), qp, qs, op, os_, heads,
-            self.head_dim ** -0.5 if scale is None else scale, workspace.data_ptr(), workspace.numel(),
-            _error_ptr(error), _stream_of(q, stream)), "fyb_kv8_attention")
+        (_native or _bind_tensors()).attention(self._handle, q, lengths, table, out, workspace, row_start, most_rows, scale,
+                                          error, stream)
 
 
 # ---------------------------------------------------------------- provider

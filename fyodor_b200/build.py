@@ -1,20 +1,25 @@
-"""Build the provider library libfyodor_b200.so for sm_100a with nvcc.
+"""Build the provider library libfyodor_b200.so for sm_100a with nvcc, and
+the extension _tensors.so that hands torch tensors to it.
 
 Usage: python fyodor_b200/build.py (the package import would load the library).
-The library is written next to this file so it travels with the source
-tree; it links the CUDA runtime statically and NCCL dynamically.
+Both are written next to this file so they travel with the source tree; the
+library links the CUDA runtime statically and NCCL dynamically. Where torch
+is not installed the extension is left out (the engine does not need it).
 """
 import concurrent.futures
+import importlib.util
 import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
 CSRC = os.path.join(HERE, "csrc")
 OBJ = os.path.join(ROOT, "_build", "obj")
 LIB = os.path.join(HERE, "libfyodor_b200.so")
+TENSORS = os.path.join(HERE, "_tensors.so")
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 COMMON = ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC,-O3", "-I" + os.path.join(ROOT, "include")]
@@ -72,13 +77,39 @@ def _compile(unit, verbose):
     return obj
 
 
+def _tensors():
+    """The extension for torch tensors (csrc/tensors.cc), or None without torch."""
+    spec = importlib.util.find_spec("torch")
+    if spec is None or not spec.submodule_search_locations:
+        return None
+    torch = spec.submodule_search_locations[0]
+    src = os.path.join(CSRC, "tensors.cc")
+    header = os.path.join(ROOT, "include", "fyodor_b200.h")
+    if os.path.exists(TENSORS) and os.path.getmtime(TENSORS) >= max(os.path.getmtime(src), os.path.getmtime(header)):
+        return TENSORS
+    cuda = os.path.dirname(os.path.dirname(_nvcc()))
+    include = [os.path.join(torch, "include"), os.path.join(torch, "include", "torch", "csrc", "api", "include"),
+               os.path.join(cuda, "include"), os.path.join(ROOT, "include"), sysconfig.get_paths()["include"]]
+    lib = os.path.join(torch, "lib")
+    cmd = [shutil.which("g++") or "g++", "-std=c++17", "-O2", "-fPIC", "-shared"] + ["-I" + i for i in include]
+    cmd += [src, "-o", TENSORS + ".tmp", "-L" + lib, "-lc10", "-lc10_cuda", "-ltorch", "-ltorch_cpu", "-ltorch_python",
+            "-Wl,-rpath," + lib]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError("g++ failed for tensors.cc:\n%s\n%s" % (r.stdout, r.stderr))
+    os.replace(TENSORS + ".tmp", TENSORS)
+    return TENSORS
+
+
 def build(verbose=False):
     os.makedirs(OBJ, exist_ok=True)
     todo = units()
     # the longest compilations first
     todo.sort(key=lambda u: u[0] not in VARIANTS)
-    with concurrent.futures.ThreadPoolExecutor(max_workers=min(os.cpu_count() or 8, len(todo))) as ex:
+    with concurrent.futures.ThreadPoolExecutor(max_workers=min(os.cpu_count() or 8, len(todo) + 1)) as ex:
+        tensors = ex.submit(_tensors)
         objs = list(ex.map(lambda u: _compile(u, verbose), todo))
+        tensors.result()
     newest = max(os.path.getmtime(o) for o in objs)
     if os.path.exists(LIB) and os.path.getmtime(LIB) >= newest:
         return LIB

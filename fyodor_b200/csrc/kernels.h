@@ -3,6 +3,7 @@
 #include <cstddef>
 #include <cstdint>
 #include <algorithm>
+#include <atomic>
 #include <cuda_runtime.h>
 #include <cuda_fp16.h>
 #include "fyodor_b200.h"
@@ -206,6 +207,22 @@ inline size_t decode_attn_partials_floats(const DecodeGeometry &g)
 int decode_supported(const DecodeGeometry &g, unsigned type_out);
 int decode_grid(int sms, const DecodeGeometry &g);
 int launch_decode(const DecodeLaunch &L, cudaStream_t s);
+
+// Lets a kernel use `bytes` of dynamic shared memory: asked of the driver once
+// per device and kernel (`done`: a static of the caller's instantiation).
+inline int allow_shared(const void *kernel, size_t bytes, std::atomic<unsigned> &done)
+{
+    int device = 0;
+    if (cudaGetDevice(&device) != cudaSuccess) return -2;
+    const unsigned bit = device < 32 ? 1u << device : 0u;
+    if (done.load(std::memory_order_relaxed) & bit) return 0;
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) != cudaSuccess) {
+        cudaGetLastError();
+        return -2;
+    }
+    done.fetch_or(bit, std::memory_order_relaxed);
+    return 0;
+}
 
 // ---------------------------------------------------------------- rope.cu
 struct RopeTable;

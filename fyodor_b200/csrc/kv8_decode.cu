@@ -406,10 +406,8 @@ template <int HD, unsigned FMT, int W> static int decode_launch(const Kv8Attenti
     constexpr size_t smem = 1024 + (size_t)STAGES * KdShape<HD>::STAGE + KD_WARPS * R * HD * 4 + STAGES * sizeof(KdMeta) +
                             KD_WARPS * R * 8 + 2 * STAGES * 8 + 16;
     static_assert(smem <= 113 * 1024, "two CTAs per SM");
-    if (cudaFuncSetAttribute(kv8_decode_kernel<HD, FMT, W>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) {
-        cudaGetLastError();
-        return -2;
-    }
+    static std::atomic<unsigned> allowed{0};
+    if (allow_shared((const void *)kv8_decode_kernel<HD, FMT, W>, smem, allowed)) return -2;
     kv8_decode_kernel<HD, FMT, W><<<grid, KD_THREADS, smem, s>>>(A, k, v);
     return cudaGetLastError() == cudaSuccess ? 0 : -2;
 }

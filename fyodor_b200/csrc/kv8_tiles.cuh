@@ -242,9 +242,10 @@ __global__ void __launch_bounds__(KT_THREADS, 1) kv8_tiles_kernel(Kv8Attention A
                 for (int i = 0; i < C; ++i) o[i * HD] = 0.f;
             }
             auto swap_halves = [&] {
-                if (C == 16) return;
+                if constexpr (C > 16) {
 #pragma unroll
-                for (int i = 0; i < 16; ++i) { const float v = l[i]; l[i] = l_other[i]; l_other[i] = v; }
+                    for (int i = 0; i < 16; ++i) { const float v = l[i]; l[i] = l_other[i]; l_other[i] = v; }
+                }
             };
             // adds the D2 of a finished period to o
             auto flush = [&](unsigned which) {
@@ -687,10 +688,8 @@ int kv8_tiles_go(const Kv8Attention &A, const CUtensorMap &k, const CUtensorMap 
 {
     constexpr size_t smem = 1024 + KtShape<HD, N, QP>::OFF_END + sizeof(KtShared<N>);
     static_assert(smem <= 227 * 1024, "shared memory of one CTA");
-    if (cudaFuncSetAttribute(kv8_tiles_kernel<HD, FMT, N, QP>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) {
-        cudaGetLastError();
-        return -2;
-    }
+    static std::atomic<unsigned> allowed{0};
+    if (allow_shared((const void *)kv8_tiles_kernel<HD, FMT, N, QP>, smem, allowed)) return -2;
     kv8_tiles_kernel<HD, FMT, N, QP><<<grid, KT_THREADS, smem, s>>>(A, k, v);
     return cudaGetLastError() == cudaSuccess ? 0 : -2;
 }

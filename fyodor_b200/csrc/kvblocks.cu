@@ -181,11 +181,9 @@ extern "C" int fyb_kv_blocks(const int32_t *lengths, const int32_t *new_tokens, 
     const KvBlocksArgs A{lengths, new_tokens, free_list, free_count, table, lengths_out, free_count_out, row_start,
                          slots, positions, row_request, status, stride, requests, (unsigned)shift, max_rows};
     const size_t smem = (size_t)2 * (requests + 1) * sizeof(unsigned);
-    if (smem > 48 * 1024 &&
-        cudaFuncSetAttribute(kv_blocks_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) {
-        cudaGetLastError();
+    static std::atomic<unsigned> allowed{0};
+    if (smem > 48 * 1024 && allow_shared((const void *)kv_blocks_kernel, 2 * (KB_REQUESTS + 1) * sizeof(unsigned), allowed))
         return -2;
-    }
     const size_t most = std::max<size_t>(max_rows, requests);
     const unsigned grid = (unsigned)std::min<size_t>((most + KB_THREADS - 1) / KB_THREADS, 148);
     kv_blocks_kernel<<<grid, KB_THREADS, smem, (cudaStream_t)stream>>>(A);
