@@ -160,6 +160,10 @@ def _load():
     lib.fyb_plan_time_projection.argtypes = [_P, C.c_uint, C.c_uint, C.c_uint, C.POINTER(C.c_size_t)]
     lib.fyb_batch_create.restype = _P
     lib.fyb_batch_create.argtypes = [_P, C.c_uint]
+    lib.fyb_batch_create_kv8.restype = _P
+    lib.fyb_batch_create_kv8.argtypes = [_P, C.c_uint, C.c_uint32, C.c_uint32, C.c_uint32]
+    lib.fyb_batch_free_blocks.restype = C.c_long
+    lib.fyb_batch_free_blocks.argtypes = [_P]
     lib.fyb_batch_free.argtypes = [_P]
     lib.fyb_batch_step.argtypes = [_P, _P, _P, _P, _P]
     lib.fyb_batch_decode_greedy.argtypes = [_P, _P, _P, C.c_size_t, _P]
@@ -186,7 +190,7 @@ EXPORTS = ["nya_cuda_backend", "fyb_version", "fyb_device_count", "fyb_dequantiz
            "fyb_plan_time_greedy", "fyb_plan_launches_per_token", "fyb_plan_decode_form", "fyb_plan_profile", "fyb_plan_trace",
            "fyb_plan_tp_info", "fyb_plan_tp_handle", "fyb_plan_tp_connect", "fyb_plan_tp_disconnect",
            "fyb_plan_tp_connect_local", "fyb_plan_error", "fyb_plan_time_projection",
-           "fyb_batch_create", "fyb_batch_free", "fyb_batch_step", "fyb_batch_decode_greedy", "fyb_batch_time_greedy",
+           "fyb_batch_create", "fyb_batch_create_kv8", "fyb_batch_free_blocks", "fyb_batch_free", "fyb_batch_step", "fyb_batch_decode_greedy", "fyb_batch_time_greedy",
            "fyb_batch_launches_per_step",
            "fyb_synth_create",
            "fyb_synth_free", "fyb_synth_fill"]
@@ -280,9 +284,11 @@ def kv_blocks(lengths, new_tokens, table, free_list, free_count, block_size, len
                                       free_count_out, row_start, slots, positions, row_request, status, stream)
 
 
-def kv_release(lengths, done, table, free_list, free_count, block_size, stream=None):
-    """Give the blocks of the requests with done[r] != 0 back (fyb_kv_release, in place)."""
-    (_native or _bind_tensors()).kv_release(lengths, done, table, free_list, free_count, block_size, stream)
+def kv_release(lengths, keep, table, free_list, free_count, block_size, stream=None):
+    """Shorten every request to keep[r] tokens and give back the blocks it
+    needs no more (fyb_kv_release, in place): 0 for a finished request, the
+    accepted prefix for one whose draft was rejected."""
+    (_native or _bind_tensors()).kv_release(lengths, keep, table, free_list, free_count, block_size, stream)
 
 
 def rope_frequencies(dims, base, kind="plain", factor=1.0, original_context=0.0, beta_fast=0.0, beta_slow=0.0,
@@ -474,12 +480,20 @@ class Provider:
 class Batch:
     """B sequences (1..16) of one plan's model decoded together (fyb_batch_*):
     each sequence has its own KV cache and position; every projection reads
-    each weight once per step for all of them. The plan must outlive it."""
+    each weight once per step for all of them. The plan must outlive it.
 
-    def __init__(self, plan, batch):
+    kv "int8" or "e4m3": a paged 8-bit cache of `blocks` blocks of block_size
+    tokens that the sequences share, instead of an fp16 cache of the plan's
+    capacity each (fyb_batch_create_kv8)."""
+
+    def __init__(self, plan, batch, kv=None, blocks=0, block_size=32):
         self.plan, self.B = plan, batch
         self.V = plan.model.vocabulary
-        self.ptr = lib.fyb_batch_create(C.c_void_p(plan.ptr), batch)
+        if kv is None:
+            self.ptr = lib.fyb_batch_create(C.c_void_p(plan.ptr), batch)
+        else:
+            self.ptr = lib.fyb_batch_create_kv8(C.c_void_p(plan.ptr), batch, blocks, block_size,
+                                                {"int8": KV8_INT8, "e4m3": KV8_E4M3}[kv])
         if not self.ptr:
             raise ValueError("batch of %d declined" % batch)
 
@@ -513,12 +527,17 @@ class Batch:
         t, p = self._req(tokens, positions)
         return lib.fyb_batch_time_greedy(C.c_void_p(self.ptr), _ptr(t), _ptr(p), steps)
 
+    def free_blocks(self):
+        """Blocks of a paged batch that no sequence holds."""
+        return lib.fyb_batch_free_blocks(C.c_void_p(self.ptr))
+
     def launches_per_step(self):
         return lib.fyb_batch_launches_per_step(C.c_void_p(self.ptr))
 
     def close(self):
         if self.ptr:
-            lib.fyb_batch_free(C.c_void_p(self.ptr))
+            if self.plan.ptr:  # collected after its plan: the plan's context, which the batch needs to free, is gone
+                lib.fyb_batch_free(C.c_void_p(self.ptr))
             self.ptr = None
 
     def __del__(self):

@@ -100,6 +100,17 @@ __global__ void bt_rope_kv_kernel(const float *y, unsigned qkv_rows, unsigned H,
     *reinterpret_cast<__half2 *>(dst) = __halves2half2(__float2half_rn(a), __float2half_rn(c2));
 }
 
+// The fused QKV rows y[b][qkv_rows] in natural order: thread (b, t, j) moves
+// rows j and j + 8 of tile t to rows 16t + 2j and 16t + 2j + 1.
+__global__ void bt_qkv_rows_kernel(const float *y, unsigned qkv_rows, float *out, unsigned nseq)
+{
+    const unsigned i = blockIdx.x * blockDim.x + threadIdx.x;
+    if (i >= nseq * (qkv_rows / 2)) return;
+    const unsigned b = i / (qkv_rows / 2), t = i % (qkv_rows / 2) / 8, j = i % 8;
+    const float *yr = y + (size_t)b * qkv_rows + 16 * t;
+    reinterpret_cast<float2 *>(out + (size_t)b * qkv_rows + 16 * t)[j] = make_float2(yr[j], yr[j + 8]);
+}
+
 // h[b][8t + j] = gate / (1 + expf(-gate)) * up (llm_cpu.c:336-342) from the
 // fused gate/up rows y[b][2 ffn].
 __global__ void bt_swiglu_kernel(const float *y, unsigned ffn, float *h, unsigned nseq)
@@ -183,6 +194,14 @@ int launch_bt_rope_kv(const float *y, unsigned qkv_rows, unsigned H, unsigned Hk
     const unsigned n = nseq * (qkv_rows / 16) * 8;
     bt_rope_kv_kernel<<<(n + 255) / 256, 256, 0, s>>>(y, qkv_rows, H, Hkv, hd, positions, rope_cos, rope_sin, q, kc,
                                                         vc, capacity, nseq, slot_div);
+    return cudaGetLastError() == cudaSuccess ? 0 : -2;
+}
+
+int launch_bt_qkv_rows(const float *y, unsigned qkv_rows, float *out, unsigned nseq, cudaStream_t s)
+{
+    if (qkv_rows % 16) return -1;
+    const unsigned n = nseq * (qkv_rows / 2);
+    bt_qkv_rows_kernel<<<(n + 255) / 256, 256, 0, s>>>(y, qkv_rows, out, nseq);
     return cudaGetLastError() == cudaSuccess ? 0 : -2;
 }
 

@@ -124,32 +124,35 @@ __global__ void __launch_bounds__(KB_THREADS) kv_blocks_kernel(KvBlocksArgs A)
     }
 }
 
-__global__ void __launch_bounds__(KB_THREADS) kv_release_kernel(int *lengths, const int *done, unsigned n, int *table,
+__global__ void __launch_bounds__(KB_THREADS) kv_release_kernel(int *lengths, const int *keep, unsigned n, int *table,
     size_t stride, unsigned shift, int *free_list, int *free_count, unsigned capacity)
 {
     __shared__ uint2 warp_sums[KB_THREADS / 32];
     __shared__ unsigned carry_s;
     const unsigned size = 1u << shift, tid = threadIdx.x, limit = 1u << 30;
     unsigned carry = (unsigned)max(free_count[0], 0);
+    auto blocks = [&](int tokens) { return (long long)((unsigned)tokens + size - 1) >> shift; };
     for (unsigned base = 0; base < n; base += KB_THREADS) {
         const unsigned r = base + tid;
-        const int len = r < n && done[r] ? lengths[r] : 0;
-        const long long held = len > 0 ? ((long long)len + size - 1) >> shift : 0;
-        unsigned mine = held <= (long long)stride ? (unsigned)held : 0u;
-        uint2 v = kb_scan(make_uint2(mine, 0u), limit, 1u, warp_sums);
+        const int len = r < n ? max(lengths[r], 0) : 0, left = r < n ? min(max(keep[r], 0), len) : 0;
+        const long long held = blocks(len), stay = blocks(left);
+        const unsigned mine = held <= (long long)stride ? (unsigned)(held - stay) : 0u;
+        const uint2 v = kb_scan(make_uint2(mine, 0u), limit, 1u, warp_sums);
         const unsigned end = min(v.x + carry, limit);
         // what would not fit stays with its request, and so does all after it
-        if (mine && end <= capacity) {
+        const bool fits = end <= capacity || carry + v.x == carry;
+        if (fits && left < len) {
             for (unsigned b = 0; b < mine; ++b) {
-                free_list[end - mine + b] = table[(size_t)r * stride + b];
-                table[(size_t)r * stride + b] = -1;
+                int *entry = table + (size_t)r * stride + (size_t)stay + b;
+                free_list[end - mine + b] = *entry;
+                *entry = -1;
             }
-            lengths[r] = 0;
+            lengths[r] = left;
         }
         if (tid == 0) carry_s = carry;
         __syncthreads();
-        if (mine && end <= capacity) atomicMax(&carry_s, end);
-        const bool full = __syncthreads_or(mine && end > capacity);
+        if (fits && mine) atomicMax(&carry_s, end);
+        const bool full = __syncthreads_or(!fits);
         carry = carry_s;
         __syncthreads();
         if (full) break;
@@ -190,14 +193,14 @@ extern "C" int fyb_kv_blocks(const int32_t *lengths, const int32_t *new_tokens, 
     return cudaGetLastError() == cudaSuccess ? 0 : -2;
 }
 
-extern "C" int fyb_kv_release(int32_t *lengths, const int32_t *done, uint32_t requests, int32_t *table, size_t stride,
+extern "C" int fyb_kv_release(int32_t *lengths, const int32_t *keep, uint32_t requests, int32_t *table, size_t stride,
     uint32_t block_size, int32_t *free_list, int32_t *free_count, uint32_t free_capacity, void *stream)
 {
     const int shift = log2_block(block_size);
-    if (!lengths || !done || !table || !free_list || !free_count || requests == 0 || requests > KB_REQUESTS ||
+    if (!lengths || !keep || !table || !free_list || !free_count || requests == 0 || requests > KB_REQUESTS ||
         shift < 0 || stride == 0 || stride > 0x7fffffffu || free_capacity >= 1u << 30)
         return -1;
-    kv_release_kernel<<<1, KB_THREADS, 0, (cudaStream_t)stream>>>(lengths, done, requests, table, stride,
+    kv_release_kernel<<<1, KB_THREADS, 0, (cudaStream_t)stream>>>(lengths, keep, requests, table, stride,
                                                                   (unsigned)shift, free_list, free_count, free_capacity);
     return cudaGetLastError() == cudaSuccess ? 0 : -2;
 }

@@ -32,7 +32,7 @@
 namespace fyb { struct Plan; }
 struct Batch;
 static void batch_free(Batch *bt);
-static Batch *batch_create(fyb::Plan *p, unsigned batch, bool chunk);
+static Batch *batch_create(fyb::Plan *p, unsigned batch, bool chunk, const fyb_kv8_cache *paged = nullptr);
 static int prefill_chunks(fyb::Plan *p, Batch *bt, const uint32_t *tokens, size_t count, size_t position, float *out);
 
 namespace fyb {
@@ -1240,6 +1240,16 @@ struct Batch {
     cudaGraphExec_t graphs[2] = {nullptr, nullptr};  // logits step, greedy step
     bool sized[2] = {false, false};
     unsigned long long launches = 0;
+    // a paged 8-bit cache in place of kc / vc (fyb_batch_create_kv8)
+    bool paged = false;
+    fyb_kv8_cache cache = {};            // layer 0; layer l's tensors follow
+    unsigned table_stride = 0;
+    int32_t *kv_len = nullptr;           // [B] lengths | free count
+    int32_t *kv_next = nullptr;          // the same after the step
+    int32_t *kv_ones = nullptr, *kv_table = nullptr, *kv_free = nullptr;
+    int32_t *kv_step = nullptr;          // [B + 1] row starts | [B] slots | [B] positions | [B] requests | [B] status
+    float *qkv = nullptr;                // [B][QKV rows] in natural order
+    std::vector<uint32_t> held;          // tokens of each sequence
 };
 
 static void batch_free(Batch *bt)
@@ -1281,6 +1291,48 @@ static AttentionLaunch batch_attention(const Batch *bt, unsigned l)
     return A;
 }
 
+// The step's cache part over the paged 8-bit cache: block tables and slots of
+// every sequence's new token, once for all layers.
+static int batch_blocks(const Batch *bt, cudaStream_t s)
+{
+    const unsigned B = bt->B;
+    int32_t *st = bt->kv_step;
+    const int r = fyb_kv_blocks(bt->kv_len, bt->kv_ones, B, bt->kv_table, bt->table_stride, bt->cache.block_size,
+                                bt->kv_free, bt->kv_len + B, bt->kv_next, bt->kv_next + B, st, st + B + 1,
+                                st + 2 * B + 1, st + 3 * B + 1, B, st + 4 * B + 1, s);
+    if (r) return r;
+    return cudaMemcpyAsync(bt->kv_len, bt->kv_next, (B + 1) * 4, cudaMemcpyDeviceToDevice, s) == cudaSuccess ? 0 : -2;
+}
+
+static fyb_kv8_cache batch_layer_cache(const Batch *bt, unsigned l)
+{
+    fyb_kv8_cache c = bt->cache;
+    const size_t scales = (size_t)c.blocks * c.kv_heads, bytes = scales * c.block_size * c.head_dim;
+    c.k = (unsigned char *)c.k + l * bytes;
+    c.v = (unsigned char *)c.v + l * bytes;
+    c.k_scale += l * scales;
+    c.v_scale += l * scales;
+    return c;
+}
+
+// Layer l's append (q and K rotated on the way) and attention over it.
+static int batch_paged_attention(Batch *bt, unsigned l, unsigned qkv_rows, cudaStream_t s)
+{
+    const Plan *p = bt->p;
+    const unsigned B = bt->B, nq = p->H * p->hd, nk = p->Hkv * p->hd;
+    const fyb_kv8_cache c = batch_layer_cache(bt, l);
+    const fyb_rope_desc rope = {p->rope_cos, p->rope_sin, (uint32_t)bt->capacity, p->hd, FYB_ROPE_INTERLEAVED};
+    int r = launch_bt_qkv_rows(bt->y, qkv_rows, bt->qkv, B, s);
+    if (r) return r;
+    r = fyb_kv8_append(&c, bt->kv_step + B + 1, B, T_F32, bt->qkv + nq, qkv_rows, bt->qkv + nq + nk, qkv_rows, &rope,
+                       bt->kv_step + 2 * B + 1, bt->qkv, qkv_rows, bt->q, nq, p->H, p->err_dev, s);
+    if (r) return r;
+    bt->launches += 2;  // the caller counts one
+    return fyb_kv8_attention(&c, bt->kv_next, nullptr, B, 1, B, bt->kv_table, bt->table_stride, T_F32, bt->q, nq,
+                             bt->attn, nq, p->H, 1.0f / std::sqrt((float)p->hd), bt->attn_ws, bt->attn_ws_bytes,
+                             p->err_dev, s);
+}
+
 // One batched step reading tokens and positions from bt->req; greedy steps
 // advance every sequence to its argmax token at the next position.
 static int batch_enqueue(Batch *bt, bool greedy, bool logits = true)
@@ -1295,15 +1347,21 @@ static int batch_enqueue(Batch *bt, bool greedy, bool logits = true)
     bt->launches = 0;
 #define BRUN(expr) do { const int r_ = (expr); ++bt->launches; if (r_) return r_; } while (0)
     BRUN(launch_gather_batch(p->embd, p->embd_row_bytes, p->embd_type, p->d, bt->req, R, bt->x, s));
+    if (bt->paged) BRUN(batch_blocks(bt, s));
     for (unsigned l = 0; l < p->nl; ++l) {
         const LayerW &L = p->layers[l];
         const size_t qkv_rows = (size_t)L.qkv.tiles * 16, gu_rows = (size_t)L.gateup.tiles * 16;
         BRUN(launch_bt_add_norm(bt->x, l ? bt->delta : nullptr, L.attn_norm, bt->xn, p->d, p->eps, R, s));
         BRUN(device_matmul(&L.qkv, nullptr, 0, qkv_rows, p->d, L.qkv.type, bt->xn, bt->y, R, sc, s, sms));
-        BRUN(launch_bt_rope_kv(bt->y, (unsigned)qkv_rows, p->H, p->Hkv, p->hd, bt->req + B, p->rope_cos, p->rope_sin,
-                               bt->q, bt->kc + (size_t)l * slots * per_seq, bt->vc + (size_t)l * slots * per_seq,
-                               (unsigned)bt->capacity, R, bt->chunk ? R : 1u, s));
-        BRUN(launch_attention(batch_attention(bt, l), s));
+        if (bt->paged) {
+            BRUN(batch_paged_attention(bt, l, (unsigned)qkv_rows, s));
+        } else {
+            BRUN(launch_bt_rope_kv(bt->y, (unsigned)qkv_rows, p->H, p->Hkv, p->hd, bt->req + B, p->rope_cos,
+                                   p->rope_sin, bt->q, bt->kc + (size_t)l * slots * per_seq,
+                                   bt->vc + (size_t)l * slots * per_seq, (unsigned)bt->capacity, R,
+                                   bt->chunk ? R : 1u, s));
+            BRUN(launch_attention(batch_attention(bt, l), s));
+        }
         BRUN(device_matmul(&L.o, nullptr, 0, p->d, (size_t)p->H * p->hd, L.o.type, bt->attn, bt->delta, R, sc, s, sms));
         BRUN(launch_bt_add_norm(bt->x, bt->delta, L.ffn_norm, bt->xn, p->d, p->eps, R, s));
         BRUN(device_matmul(&L.gateup, nullptr, 0, gu_rows, p->d, L.gateup.type, bt->xn, bt->y, R, sc, s, sms));
@@ -1335,6 +1393,7 @@ static int batch_run(Batch *bt, bool greedy)
         if (r) return r;
         if (cudaStreamSynchronize(s) != cudaSuccess) return -2;
         bt->sized[m] = true;
+        for (uint32_t &n : bt->held) ++n;
         return 0;
     }
     if (!bt->graphs[m]) {
@@ -1347,7 +1406,9 @@ static int batch_run(Batch *bt, bool greedy)
         cudaGraphDestroy(g);
         if (e != cudaSuccess) { bt->graphs[m] = nullptr; cudaGetLastError(); return -2; }
     }
-    return cudaGraphLaunch(bt->graphs[m], s) == cudaSuccess ? 0 : -2;
+    if (cudaGraphLaunch(bt->graphs[m], s) != cudaSuccess) return -2;
+    for (uint32_t &n : bt->held) ++n;
+    return 0;
 }
 
 static int batch_set(Batch *bt, const uint32_t *tokens, const uint32_t *positions, size_t steps)
@@ -1358,12 +1419,28 @@ static int batch_set(Batch *bt, const uint32_t *tokens, const uint32_t *position
         r.token[b] = tokens[b];
         r.position[b] = positions[b];
     }
-    return launch_bt_set(r, bt->req, bt->B, bt->p->ctx->stream);
+    cudaStream_t s = bt->p->ctx->stream;
+    if (!bt->paged) return launch_bt_set(r, bt->req, bt->B, s);
+    const size_t size = bt->cache.block_size;
+    size_t need = 0;
+    bool shorter = false;
+    for (unsigned b = 0; b < bt->B; ++b) {
+        if (positions[b] > bt->held[b]) return -1;  // a gap in the sequence
+        need += (positions[b] + steps + size - 1) / size;
+        shorter = shorter || positions[b] < bt->held[b];
+    }
+    if (need > bt->cache.blocks) return -1;
+    int e = launch_bt_set(r, bt->req, bt->B, s);
+    if (!e && shorter)
+        e = fyb_kv_release(bt->kv_len, (const int32_t *)(bt->req + bt->B), bt->B, bt->kv_table, bt->table_stride,
+                           bt->cache.block_size, bt->kv_free, bt->kv_len + bt->B, bt->cache.blocks, s);
+    if (!e) bt->held.assign(positions, positions + bt->B);
+    return e;
 }
 
 // A batch of `batch` sequences with their own caches, or (chunk) a prompt
 // chunker of up to `batch` consecutive positions of the plan's own sequence.
-static Batch *batch_create(Plan *p, unsigned batch, bool chunk)
+static Batch *batch_create(Plan *p, unsigned batch, bool chunk, const fyb_kv8_cache *paged)
 {
     if (!p || p->failed || batch < 1 || batch > BATCH_MAX || p->tp_size != 1 || p->hd % 16 || p->ffn % 8 ||
         p->d % 4)
@@ -1376,7 +1453,7 @@ static Batch *batch_create(Plan *p, unsigned batch, bool chunk)
     bt->rows = batch;
     bt->chunk = chunk;
     bt->capacity = p->capacity;
-    const size_t kv = chunk ? 0 : (size_t)p->nl * batch * p->Hkv * bt->capacity * p->hd;
+    const size_t kv = chunk || paged ? 0 : (size_t)p->nl * batch * p->Hkv * bt->capacity * p->hd;
     const size_t qkv_rows = (size_t)p->layers[0].qkv.tiles * 16;
     const size_t ywidth = std::max<size_t>(qkv_rows, (size_t)p->layers[0].gateup.tiles * 16);
     bool ok = true;
@@ -1388,6 +1465,30 @@ static Batch *batch_create(Plan *p, unsigned batch, bool chunk)
     };
     if (chunk) {
         bt->kc = p->kcache; bt->vc = p->vcache;
+    } else if (paged) {
+        bt->paged = true;
+        bt->cache = *paged;
+        const size_t scales = (size_t)p->nl * paged->blocks * p->Hkv, bytes = scales * paged->block_size * p->hd;
+        bt->cache.k = A(bytes); bt->cache.v = A(bytes);
+        bt->cache.k_scale = (float *)A(scales * 4); bt->cache.v_scale = (float *)A(scales * 4);
+        bt->table_stride = (unsigned)((bt->capacity + paged->block_size - 1) / paged->block_size);
+        bt->kv_len = (int32_t *)A((batch + 1) * 4); bt->kv_next = (int32_t *)A((batch + 1) * 4);
+        bt->kv_ones = (int32_t *)A(batch * 4);
+        bt->kv_table = (int32_t *)A((size_t)batch * bt->table_stride * 4);
+        bt->kv_free = (int32_t *)A((size_t)paged->blocks * 4);
+        bt->kv_step = (int32_t *)A((5 * batch + 1) * 4);
+        bt->qkv = (float *)A((size_t)batch * qkv_rows * 4);
+        bt->held.assign(batch, 0);
+        if (ok) {
+            // all blocks free, popped from the highest stack entry: block 0 first
+            std::vector<int32_t> free(paged->blocks), len(batch + 1, 0), ones(batch, 1);
+            for (uint32_t i = 0; i < paged->blocks; ++i) free[i] = (int32_t)(paged->blocks - 1 - i);
+            len[batch] = (int32_t)paged->blocks;
+            ok = cudaMemcpy(bt->kv_free, free.data(), free.size() * 4, cudaMemcpyHostToDevice) == cudaSuccess &&
+                 cudaMemcpy(bt->kv_len, len.data(), len.size() * 4, cudaMemcpyHostToDevice) == cudaSuccess &&
+                 cudaMemcpy(bt->kv_ones, ones.data(), ones.size() * 4, cudaMemcpyHostToDevice) == cudaSuccess &&
+                 cudaMemset(bt->kv_table, 0xff, (size_t)batch * bt->table_stride * 4) == cudaSuccess;
+        }
     } else {
         bt->kc = (__half *)A(kv * 2); bt->vc = (__half *)A(kv * 2);
     }
@@ -1403,11 +1504,11 @@ static Batch *batch_create(Plan *p, unsigned batch, bool chunk)
     bt->splits = (unsigned)std::max<size_t>(4, std::min<size_t>(16, ((size_t)4 * p->ctx->sms + seqs * p->Hkv - 1) /
                                                                         (seqs * p->Hkv)));
     if (ok) {
-        AttentionLaunch L = batch_attention(bt, 0);
-        bt->attn_ws_bytes = attention_workspace_bytes(L);
+        bt->attn_ws_bytes = paged ? fyb_kv8_attention_workspace(batch, 1, p->H, p->Hkv, p->hd)
+                                  : attention_workspace_bytes(batch_attention(bt, 0));
         bt->attn_ws = A(bt->attn_ws_bytes);
     }
-    if (ok) ok = (chunk || (cudaMemset(bt->kc, 0, kv * 2) == cudaSuccess && cudaMemset(bt->vc, 0, kv * 2) == cudaSuccess)) &&
+    if (ok) ok = (chunk || paged || (cudaMemset(bt->kc, 0, kv * 2) == cudaSuccess && cudaMemset(bt->vc, 0, kv * 2) == cudaSuccess)) &&
                  cudaMemset(bt->attn_ws, 0, bt->attn_ws_bytes) == cudaSuccess &&
                  cudaMemset(bt->req, 0, (3 * BATCH_MAX + 1) * 4) == cudaSuccess &&
                  grow((void **)&bt->log, &bt->log_bytes, (size_t)BATCH_MAX * 4, true) == 0 &&
@@ -1420,6 +1521,26 @@ static Batch *batch_create(Plan *p, unsigned batch, bool chunk)
 }
 
 extern "C" void *fyb_batch_create(void *plan, unsigned batch) { return batch_create((Plan *)plan, batch, false); }
+
+extern "C" void *fyb_batch_create_kv8(void *plan, unsigned batch, uint32_t blocks, uint32_t block_size, uint32_t format)
+{
+    const Plan *p = (const Plan *)plan;
+    if (!p || blocks == 0 || block_size < 16 || block_size > 256 || (block_size & (block_size - 1)) ||
+        format > FYB_KV8_E4M3 || (unsigned long long)blocks * p->Hkv * block_size > 0x7fffffffull)
+        return nullptr;
+    fyb_kv8_cache c = {};
+    c.blocks = blocks; c.kv_heads = p->Hkv; c.block_size = block_size; c.head_dim = p->hd; c.format = format;
+    return batch_create((Plan *)plan, batch, false, &c);
+}
+
+extern "C" long fyb_batch_free_blocks(const void *batch)
+{
+    const Batch *bt = (const Batch *)batch;
+    if (!bt || !bt->paged) return -1;
+    long free = (long)bt->cache.blocks;
+    for (const uint32_t n : bt->held) free -= (long)((n + bt->cache.block_size - 1) / bt->cache.block_size);
+    return free;
+}
 
 // Prompt chunks into the plan's cache; out receives the logits of the last
 // token, or with bt->all_logits (one chunk, a draft to verify) [count][V].

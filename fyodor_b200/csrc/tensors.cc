@@ -195,7 +195,7 @@ PyObject *kv_release(PyObject *, PyObject *const *a, Py_ssize_t n)
         if (table.dim() != 2 || table.size(0) != req) refuse("table", "has to be [requests][blocks]");
         const int64_t free = c.tensor(a[3], "free_list").numel();
         if (req > 0x7fffffff || free > 0x7fffffff) refuse("lengths or free_list", "has too many elements");
-        return answer(entry.kv_release(c.ints(a[0], "lengths"), c.ints(a[1], "done", req), (uint32_t)req,
+        return answer(entry.kv_release(c.ints(a[0], "lengths"), c.ints(a[1], "keep", req), (uint32_t)req,
                                        c.ints(a[2], "table"), (size_t)table.size(1), u32(a[5], "block_size"),
                                        c.ints(a[3], "free_list"), c.ints(a[4], "free_count", 1), (uint32_t)free,
                                        c.stream(a[6])),

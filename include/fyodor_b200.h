@@ -220,6 +220,15 @@ double fyb_plan_time_projection(void *plan, unsigned layer, unsigned which, unsi
    capacity), after two untimed steps from the same start; < 0 on error.
    fyb_batch_launches_per_step: kernels in the last step enqueued. */
 void *fyb_batch_create(void *plan, unsigned batch);
+/* The same over a paged 8-bit cache: the sequences share `blocks` blocks of
+   block_size tokens per layer (FYB_KV8_INT8 or FYB_KV8_E4M3; fyb_kv_blocks,
+   fyb_kv8_append and fyb_kv8_attention make the step's cache part). Sequence
+   b's position may be at most the tokens it holds; an earlier one gives the
+   blocks past it back first. A step, or a run of greedy steps, that needs more
+   blocks than there are is refused (-1) before anything is launched. */
+void *fyb_batch_create_kv8(void *plan, unsigned batch, uint32_t blocks, uint32_t block_size, uint32_t format);
+/* Blocks of a paged batch that no sequence holds (-1 for other batches). */
+long fyb_batch_free_blocks(const void *batch);
 void fyb_batch_free(void *batch);
 int fyb_batch_step(void *batch, const uint32_t *tokens, const uint32_t *positions, float *logits, uint32_t *argmax);
 int fyb_batch_decode_greedy(void *batch, const uint32_t *tokens, const uint32_t *positions, size_t steps,
@@ -275,11 +284,13 @@ int fyb_kv_blocks(const int32_t *lengths, const int32_t *new_tokens, uint32_t re
     size_t table_stride, uint32_t block_size, const int32_t *free_list, const int32_t *free_count,
     int32_t *lengths_out, int32_t *free_count_out, int32_t *row_start, int32_t *slots, int32_t *positions,
     int32_t *row_request, uint32_t max_rows, int32_t *status, void *stream);
-/* Gives the blocks of every request with done[r] != 0 back: pushed on
-   free_list (of free_capacity entries; blocks beyond it stay with their
-   request) in request order, table entries set to -1, lengths[r] to 0,
-   free_count[0] raised. In place. requests <= 16384. */
-int fyb_kv_release(int32_t *lengths, const int32_t *done, uint32_t requests, int32_t *table, size_t table_stride,
+/* Shortens every request r to keep[r] tokens (longer than it is: nothing; 0 or
+   less: finished): the blocks it needs no more are pushed on free_list (of
+   free_capacity entries; a request whose blocks do not fit stays as it is, and
+   so do all after it) in request order, their table entries set to -1,
+   lengths[r] set, free_count[0] raised. What rejects drafts and ends requests.
+   In place. requests <= 16384. */
+int fyb_kv_release(int32_t *lengths, const int32_t *keep, uint32_t requests, int32_t *table, size_t table_stride,
     uint32_t block_size, int32_t *free_list, int32_t *free_count, uint32_t free_capacity, void *stream);
 
 /* Rotary positions. The engine's frequencies (backend/core/llm_cpu.c:216-229)

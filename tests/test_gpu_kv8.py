@@ -125,18 +125,21 @@ def test_release_gives_blocks_back():
         at += held[r]
     free = np.full(len(ids), -5, np.int32)
     free[:11] = ids[at:]
-    done = (rng.random(n) < 0.5).astype(np.int32)
-    want = np.concatenate([free[:11]] + [table[r, :held[r]] for r in range(n) if done[r]])
+    # finished, shortened, shortened to more than they hold, and a negative count
+    keep = np.where(rng.random(n) < 0.3, 0, rng.integers(-3, width * block + 20, n))
+    left = np.minimum(np.maximum(keep, 0), lengths)
+    stay = -(-left // block)
+    want = np.concatenate([free[:11]] + [table[r, stay[r]:held[r]] for r in range(n)])
     t, le, fr, fc = i32(table), i32(lengths), i32(free), i32([11])
-    F.kv_release(le, i32(done), t, fr, fc, block)
+    F.kv_release(le, i32(keep), t, fr, fc, block)
     assert fc.item() == len(want) and (fr.cpu().numpy()[:len(want)] == want).all()
-    assert (le.cpu().numpy() == np.where(done, 0, lengths)).all()
-    assert (t.cpu().numpy() == np.where(done[:, None] != 0, -1, table)).all()
-    F.kv_release(le, i32(done), t, fr, fc, block)  # nothing left to give
-    assert fc.item() == len(want)
+    assert (le.cpu().numpy() == left).all()
+    assert (t.cpu().numpy() == np.where(np.arange(width)[None] < stay[:, None], table, -1)).all()
+    F.kv_release(le, i32(keep), t, fr, fc, block)  # nothing left to give
+    assert fc.item() == len(want) and (le.cpu().numpy() == left).all()
     # a free list with room for the first blocks only keeps the rest with their requests
     t, le, fr, fc = i32([[1, 2], [3, 4], [5, -1]]), i32([32, 20, 3]), i32([9, 0, 0, 0]), i32([1])
-    F.kv_release(le, i32([1, 1, 1]), t, fr, fc, 16)
+    F.kv_release(le, i32([0, 0, 0]), t, fr, fc, 16)
     assert fc.item() == 3 and fr.tolist() == [9, 1, 2, 0] and le.tolist() == [0, 20, 3]
     assert t.tolist() == [[-1, -1], [3, 4], [5, -1]]
 
@@ -638,5 +641,135 @@ def test_steps_together():
         cache.attention(q, lengths, table, out, ws, row_start=start, most_rows=max(new))
         want, tol = reference(cache, table.cpu().numpy(), lengths.tolist(), start.tolist(), q, hd ** -0.5)
         assert ((out.cpu().double() - want).abs() <= tol + want.abs() * 2.0 ** -24 + 2.0 ** -25).all(), step
-    F.kv_release(lengths, i32([1, 0, 1]), table, free, count, size)
+    F.kv_release(lengths, i32([0, 999, -1]), table, free, count, size)
     assert lengths.tolist()[0] == 0 and count.item() == 40 - -(-lengths.tolist()[1] // size)
+
+
+# ---------------------------------------------------------------- a plan's batched decode over the cache
+CFG = dict(layers=2, embedding=512, heads=8, kv_heads=2, feed_forward=1024, vocabulary=1024, context=64,
+           matrix_type=F.Q4_K, seed=21, norm_mode=2)
+
+
+class RefModel:
+    """The engine's dense LLaMA step (llm_cpu.c:424-578) in 64 bits, its cache in the 8 bits of RefCache."""
+
+    def __init__(self, model, fmt, size):
+        import oracle as O
+        self.w, self.m = {}, model
+        for i in range(3 + 9 * model.layers):
+            t = model.tensor(i)
+            shape = [int(t.dimensions[d]) for d in range(t.dimension_count)][::-1]
+            x = O.dequantize(model.tensor_bytes(i), t.type, int(np.prod(shape)))
+            self.w[t.name.decode()] = x.reshape(shape).astype(np.float64)
+        self.fmt, self.size = fmt, size
+        self.freq = F.rope_frequencies(model.head_dim, 500000.0)[0]
+
+    def session(self, capacity):
+        return [RefCache(-(-capacity // self.size), self.m.kv_heads, self.size, self.m.head_dim, self.fmt)
+                for _ in range(self.m.layers)]
+
+    def norm(self, x, name):
+        return x / np.sqrt(np.mean(x * x) + 1e-5) * self.w[name]
+
+    def turn(self, x, pos):
+        angle = (np.float32(pos) * self.freq).astype(np.float64)
+        c, s = np.cos(angle), np.sin(angle)
+        y = np.empty_like(x)
+        y[:, 0::2], y[:, 1::2] = x[:, 0::2] * c - x[:, 1::2] * s, x[:, 0::2] * s + x[:, 1::2] * c
+        return y
+
+    def step(self, session, token, pos):
+        m, w = self.m, self.w
+        x = w["token_embd.weight"][token].copy()
+        for l in range(m.layers):
+            n = "blk.%d." % l
+            h = self.norm(x, n + "attn_norm.weight")
+            q, k, v = (w[n + "attn_%s.weight" % c] @ h for c in "qkv")
+            q = self.turn(q.reshape(m.heads, m.head_dim), pos)
+            k = self.turn(k.reshape(m.kv_heads, m.head_dim), pos)
+            cache = session[l]
+            for name, row in (("k", k), ("v", v.reshape(m.kv_heads, m.head_dim))):
+                cache.append(name, torch.tensor(row, dtype=torch.float32)[None], [pos])
+            kk, vv = (cache.values(c, list(range(pos + 1))).double().numpy() for c in "kv")
+            out = np.empty_like(q)
+            for g in range(m.heads):
+                s = kk[:, g // (m.heads // m.kv_heads)] @ q[g] / np.sqrt(m.head_dim)
+                p = np.exp(s - s.max())
+                out[g] = p @ vv[:, g // (m.heads // m.kv_heads)] / p.sum()
+            x = x + w[n + "attn_output.weight"] @ out.reshape(-1)
+            h = self.norm(x, n + "ffn_norm.weight")
+            gate, up = w[n + "ffn_gate.weight"] @ h, w[n + "ffn_up.weight"] @ h
+            x = x + w[n + "ffn_down.weight"] @ (gate / (1 + np.exp(-gate)) * up)
+        return w["output.weight"] @ self.norm(x, "output_norm.weight")
+
+
+@pytest.mark.parametrize("kv", sorted(STORED))
+@pytest.mark.parametrize("nseq", [1, 5, 12])
+def test_batch_over_the_cache(provider, nseq, kv):
+    """Batched decode with the paged 8-bit cache against the same step in 64
+    bits over the same 8-bit cache: logits within 1e-3 of the logit scale, the
+    bound of every plan test. Sequences go on at ragged positions, some going
+    back over rows they have written."""
+    m = F.SynthModel(**CFG)
+    plan = provider.plan(m, CFG["context"])
+    batch = F.Batch(plan, nseq, kv=kv, blocks=4 * nseq, block_size=16)
+    ref = RefModel(m, kv, 16)
+    refs = [ref.session(CFG["context"]) for _ in range(nseq)]
+    rng = np.random.default_rng(nseq)
+    pos = np.zeros(nseq, np.uint32)
+    worst = 0.0
+    for s in range(24):
+        toks = rng.integers(0, m.vocabulary, nseq).astype(np.uint32)
+        lg, am = batch.step(toks, pos)
+        assert (am == lg.argmax(1)).all()
+        for b in range(nseq):
+            e = ref.step(refs[b], int(toks[b]), int(pos[b]))
+            worst = max(worst, float(np.max(np.abs(lg[b] - e)) / (1 + np.max(np.abs(e)))))
+        held = int(sum(-(-(int(p) + 1) // 16) for p in pos))
+        assert batch.free_blocks() == 4 * nseq - held
+        pos = np.where(rng.random(nseq) < 0.1, pos * 2 // 3, pos + 1).astype(np.uint32)
+    assert worst <= 1e-3
+    batch.close()
+    plan.close()
+    m.close()
+
+
+def test_batch_greedy_and_refusals(provider):
+    """Greedy steps on the device are the same steps one by one; a gap, a
+    position past the plan's capacity and a step that needs more blocks than the
+    pool has are refused, and the batch goes on after them."""
+    m = F.SynthModel(**CFG)
+    plan = provider.plan(m, CFG["context"])
+    nseq = 3
+    batch, other = (F.Batch(plan, nseq, kv="int8", blocks=4 * nseq, block_size=16) for _ in range(2))
+    rng = np.random.default_rng(3)
+    for s in range(20):  # the same history in both: a block keeps the scale of rows that were taken back
+        toks = rng.integers(0, m.vocabulary, nseq).astype(np.uint32)
+        for x in (batch, other):
+            x.step(toks, np.full(nseq, s, np.uint32))
+    start, first = np.full(nseq, 17, np.uint32), rng.integers(0, m.vocabulary, nseq).astype(np.uint32)
+    got = other.decode_greedy(first, start, 8)
+    assert other.free_blocks() == 2 * nseq
+    cur = first
+    for i in range(8):
+        _, cur = batch.step(cur, start + np.uint32(i))
+        assert (cur == got[i]).all(), i
+    with pytest.raises(RuntimeError):
+        batch.step(cur, np.full(nseq, 26, np.uint32))
+    with pytest.raises(RuntimeError):
+        batch.decode_greedy(cur, np.full(nseq, 25, np.uint32), 40)
+    batch.step(cur, np.full(nseq, 25, np.uint32))
+    tight = F.Batch(plan, nseq, kv="e4m3", blocks=nseq, block_size=16)
+    assert tight.decode_greedy(cur, np.zeros(nseq, np.uint32), 16).shape == (16, nseq)
+    with pytest.raises(RuntimeError):
+        tight.step(cur, np.full(nseq, 16, np.uint32))
+    assert tight.free_blocks() == 0
+    tight.step(cur, np.full(nseq, 15, np.uint32))
+    assert tight.time_greedy(cur, np.full(nseq, 3, np.uint32), 4) > 0
+    assert not F.lib.fyb_batch_create_kv8(C.c_void_p(plan.ptr), 4, 16, 24, 0)
+    assert not F.lib.fyb_batch_create_kv8(C.c_void_p(plan.ptr), 17, 16, 16, 0)
+    assert not F.lib.fyb_batch_create_kv8(C.c_void_p(plan.ptr), 4, 0, 16, 0)
+    for x in (tight, other, batch):
+        x.close()
+    plan.close()
+    m.close()

@@ -178,10 +178,10 @@ def test_blocks_refuse():
     for kw in (dict(n=0), dict(n=16385), dict(stride=0), dict(block=0), dict(block=24), dict(rows=1 << 30),
                dict(lengths_out=P), dict(count_out=P)):
         assert call(**kw) == -1, kw
-    names = ["lengths", "done", "n", "table", "stride", "block", "free", "count", "capacity", "stream"]
+    names = ["lengths", "keep", "n", "table", "stride", "block", "free", "count", "capacity", "stream"]
     good = dict(zip(names, [P, P, 1, P, 1, 16, P, P, 4, None]))
     call = lambda **kw: F.lib.fyb_kv_release(*(good | kw).values())  # noqa: E731
-    for kw in (dict(lengths=None), dict(done=None), dict(table=None), dict(free=None), dict(count=None), dict(n=0),
+    for kw in (dict(lengths=None), dict(keep=None), dict(table=None), dict(free=None), dict(count=None), dict(n=0),
                dict(n=16385), dict(stride=0), dict(block=24), dict(capacity=1 << 30)):
         assert call(**kw) == -1, kw
 
@@ -194,3 +194,8 @@ def test_wrappers_refuse_host_tensors():
     q = torch.zeros((1, 2, 64))
     with pytest.raises(ValueError):
         F.rope(q, None, torch.zeros(1, dtype=torch.int32), torch.zeros((4, 32)), torch.zeros((4, 32)), "half", q, None)
+
+
+def test_batch_refuses():
+    assert not F.lib.fyb_batch_create_kv8(None, 4, 16, 32, 0)
+    assert F.lib.fyb_batch_free_blocks(None) == -1
