@@ -25,17 +25,24 @@ struct Kv8Append {
     size_t k_stride, v_stride, rows;
     RopeTable rope;   // rope.cos null: K is stored as it comes
     RopeRows q;       // rotated in the same launch (heads 0: none)
-    unsigned shift, window, items;
-    bool vec;
+    RopeWork work;
+    unsigned shift, window, parts, q_rows;  // parts: CTAs of a window; q_rows: CTAs of a row of q
+    bool vec, many;
     unsigned *error;
 };
 
-// E consecutive values of one head's row at e, rotated when `turn`.
-template <typename T, int HD, int E>
-FYB_DEV void kv8_row(const Kv8Append &A, const T *row, unsigned e, bool turn, size_t tab, float (&x)[E])
+// E consecutive values of one head's row as they lie there; and as they are stored, rotated when `turn` (half pairs
+// fetch the other half, which the same CTA has in its cache).
+template <typename T, int E> FYB_DEV RopePack<T, E> kv8_get(const Kv8Append &A, const T *p)
 {
-    if (A.vec) row_load<T, E, true>(row + e, x); else row_load<T, E, false>(row + e, x);
-    if (!turn) return;
+    return A.vec ? rope_get<T, E, true>(p) : rope_get<T, E, false>(p);
+}
+template <typename T, int E> FYB_DEV void kv8_values(const Kv8Append &A, const RopePack<T, E> &own, const T *row, unsigned e,
+    bool turn, size_t tab, float (&x)[E])
+{
+#pragma unroll
+    for (int i = 0; i < E; ++i) x[i] = row_value(own.t[i]);
+    if (!turn || e >= A.rope.dims) return;
     const float *c = A.rope.cos + tab, *s = A.rope.sin + tab;
     if (A.rope.layout == 0) {
 #pragma unroll
@@ -43,43 +50,73 @@ FYB_DEV void kv8_row(const Kv8Append &A, const T *row, unsigned e, bool turn, si
             if (e + i < A.rope.dims) rope_turn(x[i], x[i + 1], c[(e + i) / 2], s[(e + i) / 2]);
     } else {
         const unsigned pairs = A.rope.dims / 2;
-        if (e >= A.rope.dims) return;
         const bool low = e < pairs;  // dims / 2 is a multiple of E: a run lies in one half
-        float y[E];
-        const unsigned other = low ? e + pairs : e - pairs, p = low ? e : e - pairs;
-        if (A.vec) row_load<T, E, true>(row + other, y); else row_load<T, E, false>(row + other, y);
+        const unsigned p = low ? e : e - pairs;
+        const RopePack<T, E> y = kv8_get<T, E>(A, row + (low ? e + pairs : e - pairs));
 #pragma unroll
         for (int i = 0; i < E; ++i) {
-            if (low) rope_turn(x[i], y[i], c[p + i], s[p + i]);
-            else { rope_turn(y[i], x[i], c[p + i], s[p + i]); }
+            float o = row_value(y.t[i]);
+            if (low) rope_turn(x[i], o, c[p + i], s[p + i]); else rope_turn(o, x[i], c[p + i], s[p + i]);
         }
     }
 }
 
-// Grid (windows of rows, 2 * kv_heads + CTAs for q).
-template <typename T, int HD, unsigned FMT>
-__global__ void __launch_bounds__(KV8_THREADS) kv8_append_kernel(Kv8Append A)
+// q rows: CTA = 256 items of one row
+template <typename T, int HD> FYB_DEV void kv8_turn_q(const Kv8Append &A, unsigned cta)
 {
-    constexpr int E = HD / 32;
-    const unsigned tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const size_t row0 = (size_t)blockIdx.x * A.window, row1 = min(row0 + A.window, A.rows);
-    const unsigned part = blockIdx.y, kv = A.c.kv_heads;
-    if (part >= 2 * kv) {
-        const unsigned i = (part - 2 * kv) * KV8_THREADS + tid, head = i / A.items, item = i % A.items;
-        if (head >= A.q.heads) return;
-        for (size_t r = row0; r < row1; ++r) {
-            const int pos = A.positions[r];
-            if (pos < 0 || (unsigned)pos >= A.rope.rows) { if (i == 0) raise_error(A.error, ERR_BOUNDS); continue; }
-            const T *in = static_cast<const T *>(A.q.in) + r * A.q.in_stride + (size_t)head * HD;
-            T *out = static_cast<T *>(A.q.out) + r * A.q.out_stride + (size_t)head * HD;
-            const size_t t = (size_t)pos * (A.rope.dims / 2);
-            if (A.vec) rope_item<T, 16 / sizeof(T), true>(in, out, A.rope.cos + t, A.rope.sin + t, A.rope.dims, A.rope.layout, item);
-            else if (A.rope.layout == 0) rope_item<T, 2, false>(in, out, A.rope.cos + t, A.rope.sin + t, A.rope.dims, 0, item);
-            else rope_item<T, 1, false>(in, out, A.rope.cos + t, A.rope.sin + t, A.rope.dims, 1, item);
+    const size_t r = cta / A.q_rows;
+    const unsigned i = cta % A.q_rows * KV8_THREADS + threadIdx.x;
+    const unsigned groups = A.many ? (A.q.heads + ROPE_HEADS - 1) / ROPE_HEADS : A.q.heads;
+    unsigned head, item;  // heads head, head + groups, ...
+    if (!rope_place(A.work, groups, i, head, item)) return;
+    const int pos = A.positions[r];
+    const T *in = static_cast<const T *>(A.q.in) + r * A.q.in_stride + (size_t)head * HD;
+    T *out = static_cast<T *>(A.q.out) + r * A.q.out_stride + (size_t)head * HD;
+    auto at = [&](const float *&c, const float *&s) {
+        if (pos < 0 || (unsigned)pos >= A.rope.rows) {
+            if (i == 0) raise_error(A.error, ERR_BOUNDS);
+            return false;
         }
+        const size_t t = (size_t)pos * (A.rope.dims / 2);
+        c = A.rope.cos + t;
+        s = A.rope.sin + t;
+        return true;
+    };
+    constexpr int V = 16 / sizeof(T);
+    if (A.many)
+        rope_item<T, V, true, ROPE_HEADS>(in, out, (size_t)groups * HD, (A.q.heads - head + groups - 1) / groups,
+                                          A.rope.dims, A.rope.layout, item, at);
+    else if (A.vec) rope_item<T, V, true, 1>(in, out, HD, 1, A.rope.dims, A.rope.layout, item, at);
+    else if (A.rope.layout == 0) rope_item<T, 2, false, 1>(in, out, HD, 1, A.rope.dims, 0, item, at);
+    else rope_item<T, 1, false, 1>(in, out, HD, 1, A.rope.dims, 1, item, at);
+}
+
+// Four stored bytes of values already divided by the scale.
+template <unsigned FMT> FYB_DEV unsigned kv8_store4(float a, float b, float c, float d)
+{
+    if constexpr (FMT == FYB_KV8_INT8) {
+        return kv8_store<FMT>(a) | kv8_store<FMT>(b) << 8 | kv8_store<FMT>(c) << 16 | kv8_store<FMT>(d) << 24;
+    } else {
+        const unsigned lo = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
+        return lo | (unsigned)__nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, __NV_E4M3) << 16;
+    }
+}
+
+// CTAs: (window of rows, part), part = one KV head of K or of V; then those of q.
+template <typename T, int HD, unsigned FMT>
+__global__ void __launch_bounds__(KV8_THREADS, 4) kv8_append_kernel(Kv8Append A)
+{
+    // a warp's rows of a run: the first HOLD stay in registers between the two passes
+    constexpr int E = HD / 32, WARPS = KV8_THREADS / 32, HOLD = 8;
+    const unsigned tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, kv = A.c.kv_heads;
+    const unsigned windows = (unsigned)((A.rows + A.window - 1) / A.window);
+    if (blockIdx.x >= windows * A.parts) {
+        kv8_turn_q<T, HD>(A, blockIdx.x - windows * A.parts);
         return;
     }
-    __shared__ unsigned run_s, first_s, peak_s;
+    const unsigned part = blockIdx.x % A.parts;
+    const size_t row0 = (size_t)(blockIdx.x / A.parts) * A.window;
+    __shared__ unsigned run_s, first_s, peak_s, leaders_s[KV8_THREADS / 32];
     const bool is_k = part < kv, turn = is_k && A.rope.cos;
     const unsigned head = is_k ? part : part - kv, size = 1u << A.shift;
     const T *src = static_cast<const T *>(is_k ? A.k : A.v) + (size_t)head * HD;
@@ -97,15 +134,24 @@ __global__ void __launch_bounds__(KV8_THREADS) kv8_append_kernel(Kv8Append A)
         }
         return slot >> A.shift;
     };
-    for (size_t r0 = row0; r0 < row1; ++r0) {
-        const int b = block_of(r0);
-        if (b < 0) {
-            if (tid == 0 && A.slots[r0] >= 0) raise_error(A.error, ERR_BOUNDS);
-            continue;
+    // ---- the rows of the window that begin a run
+    {
+        const size_t r = row0 + tid;
+        bool leads = false;
+        if (tid < A.window && r < A.rows) {
+            const int b = block_of(r);
+            leads = b >= 0 && (r == 0 || block_of(r - 1) != b);
+            if (b < 0 && A.slots[r] >= 0) raise_error(A.error, ERR_BOUNDS);
         }
-        if (r0 > 0 && block_of(r0 - 1) == b) continue;
-        // the run of rows in block b (at most one per slot) and its lowest offset
+        const unsigned mask = __ballot_sync(0xffffffffu, leads);
+        if (lane == 0) leaders_s[warp] = mask;
         __syncthreads();
+    }
+    for (unsigned w = 0; w < (A.window + 31) / 32; ++w)
+    for (unsigned left = leaders_s[w]; left; left &= left - 1) {
+        const size_t r0 = row0 + 32 * w + (unsigned)__ffs((int)left) - 1;
+        const int b = A.slots[r0] >> A.shift;
+        // ---- the run of rows in block b (at most one per slot) and its lowest offset
         if (tid == 0) { run_s = size; first_s = size; peak_s = 0u; }
         __syncthreads();
         const bool in = tid < size && r0 + tid < A.rows && block_of(r0 + tid) == b;
@@ -113,17 +159,31 @@ __global__ void __launch_bounds__(KV8_THREADS) kv8_append_kernel(Kv8Append A)
         __syncthreads();
         const unsigned run = run_s;
         if (tid < run) atomicMin(&first_s, (unsigned)A.slots[r0 + tid] & (size - 1));
+        // ---- largest magnitude
+        RopePack<T, E> held[HOLD];
         float peak = 0.f;
         bool bad = false;
-        for (unsigned i = warp; i < run; i += KV8_THREADS / 32) {
-            float x[E];
+        auto row_at = [&](unsigned i) { return src + (r0 + i) * stride; };
+        auto value = [&](unsigned i, const RopePack<T, E> &own, float (&y)[E]) {
             const size_t tab = turn ? (size_t)A.positions[r0 + i] * (A.rope.dims / 2) : 0;
-            kv8_row<T, HD, E>(A, src + (r0 + i) * stride, lane * E, turn, tab, x);
+            kv8_values<T, E>(A, own, row_at(i), lane * E, turn, tab, y);
+        };
+        auto look = [&](unsigned i, const RopePack<T, E> &own) {
+            float y[E];
+            value(i, own, y);
 #pragma unroll
             for (int e = 0; e < E; ++e) {
-                if (isfinite(x[e])) peak = fmaxf(peak, fabsf(x[e])); else bad = true;
+                const float m = fabsf(y[e]);
+                if (m <= 3.4028235e38f) peak = fmaxf(peak, m); else bad = true;
             }
-        }
+        };
+#pragma unroll
+        for (int h = 0; h < HOLD; ++h)
+            if (warp + h * WARPS < run) held[h] = kv8_get<T, E>(A, row_at(warp + h * WARPS) + lane * E);
+#pragma unroll
+        for (int h = 0; h < HOLD; ++h)
+            if (warp + h * WARPS < run) look(warp + h * WARPS, held[h]);
+        for (unsigned i = warp + HOLD * WARPS; i < run; i += WARPS) look(i, kv8_get<T, E>(A, row_at(i) + lane * E));
         if (bad) raise_error(A.error, ERR_NONFINITE);
         peak = warp_max(peak);
         if (lane == 0) atomicMax(&peak_s, __float_as_uint(peak));  // non-negative: ordered as integers
@@ -135,68 +195,78 @@ __global__ void __launch_bounds__(KV8_THREADS) kv8_append_kernel(Kv8Append A)
         unsigned char *blk = pool + at * size * HD;
         if (now > was && first) {
             const float keep = __fdiv_rn(was, now);
-            unsigned *w = reinterpret_cast<unsigned *>(blk);
+            unsigned *words = reinterpret_cast<unsigned *>(blk);
             for (unsigned i = tid; i < first * HD / 4; i += KV8_THREADS) {
-                const unsigned old = w[i];
-                unsigned q = 0;
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    q |= kv8_store<FMT>(__fmul_rn(kv8_number<FMT>((old >> 8 * e) & 0xffu), keep)) << 8 * e;
-                w[i] = q;
+                const unsigned old = words[i];
+                words[i] = kv8_store4<FMT>(__fmul_rn(kv8_number<FMT>(old & 0xffu), keep), __fmul_rn(kv8_number<FMT>(old >> 8 & 0xffu), keep),
+                                           __fmul_rn(kv8_number<FMT>(old >> 16 & 0xffu), keep), __fmul_rn(kv8_number<FMT>(old >> 24), keep));
             }
         }
-        for (unsigned i = warp; i < run; i += KV8_THREADS / 32) {
-            float x[E];
-            const size_t tab = turn ? (size_t)A.positions[r0 + i] * (A.rope.dims / 2) : 0;
-            kv8_row<T, HD, E>(A, src + (r0 + i) * stride, lane * E, turn, tab, x);
-            unsigned q = 0;
+        // ---- stored values
+        auto store = [&](unsigned i, const RopePack<T, E> &own) {
+            float y[E], q[4] = {0.f, 0.f, 0.f, 0.f};
+            value(i, own, y);
 #pragma unroll
             for (int e = 0; e < E; ++e) {
-                float y = now > 0.f ? __fdiv_rn(x[e], now) : 0.f;
-                if (!isfinite(x[e])) y = isnan(x[e]) ? 0.f : copysignf(kv8_top(FMT), x[e]);
-                q |= kv8_store<FMT>(y) << 8 * e;
+                q[e] = now > 0.f ? __fdiv_rn(y[e], now) : 0.f;
+                if (!(fabsf(y[e]) <= 3.4028235e38f)) q[e] = isnan(y[e]) ? 0.f : copysignf(kv8_top(FMT), y[e]);
             }
+            const unsigned bytes = kv8_store4<FMT>(q[0], q[1], q[2], q[3]);
             unsigned char *dst = blk + ((unsigned)A.slots[r0 + i] & (size - 1)) * HD + lane * E;
-            if constexpr (E == 4) *reinterpret_cast<unsigned *>(dst) = q;
-            else *reinterpret_cast<unsigned short *>(dst) = (unsigned short)q;
-        }
+            if constexpr (E == 4) *reinterpret_cast<unsigned *>(dst) = bytes;
+            else *reinterpret_cast<unsigned short *>(dst) = (unsigned short)bytes;
+        };
+#pragma unroll
+        for (int h = 0; h < HOLD; ++h)
+            if (warp + h * WARPS < run) store(warp + h * WARPS, held[h]);
+        for (unsigned i = warp + HOLD * WARPS; i < run; i += WARPS) store(i, kv8_get<T, E>(A, row_at(i) + lane * E));
         __syncthreads();
         if (tid == 0) scales[at] = now;
     }
 }
 
-// Values at slots: thread = 4 consecutive values of K and of V.
+// Values at slots: thread = word j (four values) of K and of V of READ_ROWS rows, all loads out before the first is
+// used. Grid (rows / READ_ROWS, words of a row / 256).
+constexpr int READ_ROWS = 4;
 template <unsigned FMT>
 __global__ void __launch_bounds__(256) kv8_read_kernel(fyb_kv8_cache c, const int *slots, size_t rows, float *k, float *v,
     unsigned shift, unsigned *error)
 {
     const unsigned per_head = c.head_dim / 4, per_row = c.kv_heads * per_head;
-    const size_t n = rows * per_row;
-    for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (size_t)gridDim.x * 256) {
-        const size_t r = i / per_row;
-        const unsigned j = (unsigned)(i % per_row), head = j / per_head, e = j % per_head;
-        const int slot = slots[r];
-        float4 a = make_float4(0.f, 0.f, 0.f, 0.f), b = a;
-        if (slot >= 0 && slot < (int)(c.blocks << shift)) {
-            const size_t at = (size_t)(slot >> shift) * c.kv_heads + head;
-            const size_t off = ((at << shift) + ((unsigned)slot & ((1u << shift) - 1))) * per_head + e;
-            const unsigned kw = static_cast<const unsigned *>(c.k)[off], vw = static_cast<const unsigned *>(c.v)[off];
-            const float ks = c.k_scale[at], vs = c.v_scale[at];
-            auto four = [](unsigned w, float s) {
-                return make_float4(kv8_number<FMT>(w & 0xffu) * s, kv8_number<FMT>((w >> 8) & 0xffu) * s,
-                                   kv8_number<FMT>((w >> 16) & 0xffu) * s, kv8_number<FMT>(w >> 24) * s);
-            };
-            a = four(kw, ks);
-            b = four(vw, vs);
-        } else if (slot >= 0) {
-            raise_error(error, ERR_BOUNDS);
-        }
-        reinterpret_cast<float4 *>(k)[i] = a;
-        reinterpret_cast<float4 *>(v)[i] = b;
+    const unsigned j = blockIdx.y * 256 + threadIdx.x, head = j / per_head, e = j % per_head;
+    if (j >= per_row) return;
+    const size_t r0 = (size_t)blockIdx.x * READ_ROWS;
+    int slot[READ_ROWS];
+    unsigned kw[READ_ROWS], vw[READ_ROWS];
+    float ks[READ_ROWS], vs[READ_ROWS];
+#pragma unroll
+    for (int u = 0; u < READ_ROWS; ++u) slot[u] = r0 + u < rows ? slots[r0 + u] : -1;
+#pragma unroll
+    for (int u = 0; u < READ_ROWS; ++u) {
+        kw[u] = vw[u] = 0;
+        ks[u] = vs[u] = 0.f;
+        if (slot[u] < 0) continue;
+        if (slot[u] >= (int)(c.blocks << shift)) { raise_error(error, ERR_BOUNDS); continue; }
+        const size_t at = (size_t)(slot[u] >> shift) * c.kv_heads + head;
+        const size_t off = ((at << shift) + ((unsigned)slot[u] & ((1u << shift) - 1))) * per_head + e;
+        kw[u] = static_cast<const unsigned *>(c.k)[off];
+        vw[u] = static_cast<const unsigned *>(c.v)[off];
+        ks[u] = c.k_scale[at];
+        vs[u] = c.v_scale[at];
+    }
+    auto four = [](unsigned w, float s) {
+        return make_float4(kv8_number<FMT>(w & 0xffu) * s, kv8_number<FMT>((w >> 8) & 0xffu) * s,
+                           kv8_number<FMT>((w >> 16) & 0xffu) * s, kv8_number<FMT>(w >> 24) * s);
+    };
+#pragma unroll
+    for (int u = 0; u < READ_ROWS; ++u) {
+        if (r0 + u >= rows) break;
+        reinterpret_cast<float4 *>(k)[(r0 + u) * per_row + j] = four(kw[u], ks[u]);
+        reinterpret_cast<float4 *>(v)[(r0 + u) * per_row + j] = four(vw[u], vs[u]);
     }
 }
 
-template <typename T> static void append_launch(const Kv8Append &A, dim3 grid, cudaStream_t s)
+template <typename T> static void append_launch(const Kv8Append &A, unsigned grid, cudaStream_t s)
 {
     if (A.c.head_dim == 128) {
         if (A.c.format == FYB_KV8_INT8) kv8_append_kernel<T, 128, FYB_KV8_INT8><<<grid, KV8_THREADS, 0, s>>>(A);
@@ -237,17 +307,21 @@ extern "C" int fyb_kv8_append(const fyb_kv8_cache *cache, const int32_t *slots, 
     const size_t el = 16 / width;  // elements of a 16-byte access
     A.vec = ((uintptr_t)k | (uintptr_t)v) % 16 == 0 && k_stride % el == 0 && v_stride % el == 0;
     if (rope) A.vec = A.vec && rope_vectors(A.rope, hd, width, A.q);
-    unsigned q_parts = 0;
+    A.q_rows = 0;
     if (heads) {
-        A.items = rope_items(hd, A.rope.dims, A.rope.layout, A.vec ? (unsigned)el : A.rope.layout == 0 ? 2u : 1u);
-        q_parts = (unsigned)(((size_t)heads * A.items + KV8_THREADS - 1) / KV8_THREADS);
+        A.work = rope_work(hd, A.rope.dims, A.rope.layout, A.vec ? (unsigned)el : A.rope.layout == 0 ? 2u : 1u, q == q_out);
+        A.many = A.vec && rope_many(rows, heads, A.work);
+        const unsigned groups = A.many ? (heads + ROPE_HEADS - 1) / ROPE_HEADS : heads;
+        A.q_rows = (unsigned)(((size_t)groups * (A.work.turned + A.work.copied) + KV8_THREADS - 1) / KV8_THREADS);
     }
-    if (2 * (size_t)kv + q_parts > 65535) return -1;
     // a CTA looks at one row while that makes at most 16 CTAs per SM, at up to
     // a block of rows beyond: a prompt's rows mostly follow one another
     A.window = 1;
-    while (A.window < cache->block_size && rows / A.window * 2 * kv > 16 * 148) A.window *= 2;
-    const dim3 grid((unsigned)((rows + A.window - 1) / A.window), 2 * kv + q_parts);
+    A.parts = 2 * kv;
+    while (A.window < cache->block_size && rows / A.window * A.parts > 16 * 148) A.window *= 2;
+    const size_t ctas = (rows + A.window - 1) / A.window * A.parts + rows * A.q_rows;
+    if (ctas > 0x7fffffffu) return -1;
+    const unsigned grid = (unsigned)ctas;
     cudaStream_t s = (cudaStream_t)stream;
     if (type == T_F32) append_launch<float>(A, grid, s);
     else if (type == T_F16) append_launch<__half>(A, grid, s);
@@ -261,8 +335,9 @@ extern "C" int fyb_kv8_read(const fyb_kv8_cache *cache, const int32_t *slots, si
     if (kv8_check(cache) || !k || !v || ((uintptr_t)k | (uintptr_t)v) % 16 || rows > 0x7fffffffu) return -1;
     if (!rows) return 0;
     if (!slots) return -1;
-    const size_t n = rows * cache->kv_heads * (cache->head_dim / 4);
-    const unsigned grid = (unsigned)std::min<size_t>((n + 255) / 256, 148 * 16);
+    const unsigned words = cache->kv_heads * (cache->head_dim / 4);
+    const dim3 grid((unsigned)((rows + READ_ROWS - 1) / READ_ROWS), (words + 255) / 256);
+    if (grid.y > 65535) return -1;
     if (cache->format == FYB_KV8_INT8)
         kv8_read_kernel<FYB_KV8_INT8><<<grid, 256, 0, (cudaStream_t)stream>>>(*cache, slots, rows, k, v, kv8_shift(cache), error);
     else

@@ -15,28 +15,34 @@ namespace fyb {
 
 constexpr unsigned ROPE_THREADS = 256;
 
-// Grid (rows, items of a row / 256): thread = one item of one head of q or k.
-template <typename T, int V, bool VEC>
+// Grid (rows, items of a row / 256): thread = one item of up to HU heads of q or k.
+template <typename T, int V, bool VEC, int HU>
 __global__ void __launch_bounds__(ROPE_THREADS) rope_kernel(RopeTable tab, const int *positions, RopeRows q, RopeRows k,
-    unsigned hd, unsigned items, unsigned *error)
+    unsigned hd, RopeWork work, unsigned *error)
 {
     const size_t row = blockIdx.x;
     const unsigned i = blockIdx.y * ROPE_THREADS + threadIdx.x;
     const int pos = positions[row];
-    if (pos < 0 || (unsigned)pos >= tab.rows) {
-        if (i == 0) raise_error(error, ERR_BOUNDS);
-        return;
-    }
-    unsigned head = i / items;
-    const unsigned item = i % items;
-    if (head >= q.heads + k.heads) return;
-    const bool is_q = head < q.heads;
+    const unsigned q_groups = (q.heads + HU - 1) / HU, k_groups = (k.heads + HU - 1) / HU;
+    unsigned group, item;
+    if (!rope_place(work, q_groups + k_groups, i, group, item)) return;
+    const bool is_q = group < q_groups;
     const RopeRows &r = is_q ? q : k;
-    if (!is_q) head -= q.heads;
+    if (!is_q) group -= q_groups;
+    const unsigned head = group, groups = is_q ? q_groups : k_groups;  // heads group, group + groups, ...
     const T *in = static_cast<const T *>(r.in) + row * r.in_stride + (size_t)head * hd;
     T *out = static_cast<T *>(r.out) + row * r.out_stride + (size_t)head * hd;
-    const size_t t = (size_t)pos * (tab.dims / 2);
-    rope_item<T, V, VEC>(in, out, tab.cos + t, tab.sin + t, tab.dims, tab.layout, item);
+    rope_item<T, V, VEC, HU>(in, out, (size_t)groups * hd, (r.heads - head + groups - 1) / groups, tab.dims, tab.layout,
+        item, [&](const float *&c, const float *&s) {
+            if (pos < 0 || (unsigned)pos >= tab.rows) {
+                if (i == 0) raise_error(error, ERR_BOUNDS);
+                return false;
+            }
+            const size_t t = (size_t)pos * (tab.dims / 2);
+            c = tab.cos + t;
+            s = tab.sin + t;
+            return true;
+        });
 }
 
 // cos / sin of (float)(first + row) * freq[j], the engine's F32 angle.
@@ -80,14 +86,18 @@ static int rope_launch(const RopeTable &t, const int *positions, size_t rows, un
     constexpr int V = 16 / sizeof(T);
     const bool vec = rope_vectors(t, hd, sizeof(T), q) && rope_vectors(t, hd, sizeof(T), k);
     const unsigned step = vec ? V : t.layout == 0 ? 2 : 1;
-    const unsigned items = rope_items(hd, t.dims, t.layout, step);
-    const size_t per_row = (size_t)(q.heads + k.heads) * items;
+    const bool in_place = q.in == q.out && (!k.heads || k.in == k.out);
+    const RopeWork work = rope_work(hd, t.dims, t.layout, step, in_place);
+    const bool many = vec && rope_many(rows, q.heads + k.heads, work);
+    const size_t hu = many ? ROPE_HEADS : 1;
+    const size_t per_row = ((q.heads + hu - 1) / hu + (k.heads + hu - 1) / hu) * (work.turned + work.copied);
     const size_t y = (per_row + ROPE_THREADS - 1) / ROPE_THREADS;
     if (y > 65535) return -1;
     const dim3 grid((unsigned)rows, (unsigned)y);
-    if (vec) rope_kernel<T, V, true><<<grid, ROPE_THREADS, 0, s>>>(t, positions, q, k, hd, items, error);
-    else if (t.layout == 0) rope_kernel<T, 2, false><<<grid, ROPE_THREADS, 0, s>>>(t, positions, q, k, hd, items, error);
-    else rope_kernel<T, 1, false><<<grid, ROPE_THREADS, 0, s>>>(t, positions, q, k, hd, items, error);
+    if (many) rope_kernel<T, V, true, ROPE_HEADS><<<grid, ROPE_THREADS, 0, s>>>(t, positions, q, k, hd, work, error);
+    else if (vec) rope_kernel<T, V, true, 1><<<grid, ROPE_THREADS, 0, s>>>(t, positions, q, k, hd, work, error);
+    else if (t.layout == 0) rope_kernel<T, 2, false, 1><<<grid, ROPE_THREADS, 0, s>>>(t, positions, q, k, hd, work, error);
+    else rope_kernel<T, 1, false, 1><<<grid, ROPE_THREADS, 0, s>>>(t, positions, q, k, hd, work, error);
     return cudaGetLastError() == cudaSuccess ? 0 : -2;
 }
 
