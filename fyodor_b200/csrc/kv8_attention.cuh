@@ -4,7 +4,7 @@
 //
 // Work is a line of units. A segment is the cache that one row tile of one
 // request attends in one KV head, a unit TILE positions of it. CTA c of C takes
-// units [U c / C, U (c + 1) / C), C at most U: every CTA streams the same number of tiles
+// units [U c / C, U (c + 1) / C): every CTA streams the same number of tiles
 // whatever the lengths, its loads running on from one segment to the next. A
 // segment that crosses CTAs leaves one partial (maximum, sum, weighted values)
 // per CTA; the last CTA to finish its part joins them in CTA order, so results
@@ -30,8 +30,8 @@ struct Kv8Attention {
     unsigned *error;
 };
 
-// Grid of either kernel, two CTAs per SM; the workspace is sized for it.
-constexpr unsigned KA_GRID = 2 * 148;
+// Largest grid of either kernel, three CTAs per SM; the workspace is sized for it.
+constexpr unsigned KA_GRID = 3 * 148;
 constexpr size_t KA_COUNTER_BYTES = (KA_GRID * 4 + 255) / 256 * 256;
 
 // ---- segments and units ------------------------------------------------------
@@ -70,26 +70,26 @@ template <int TILE> FYB_DEV unsigned kv8_units(const Kv8Attention &A, const Kv8R
     for (int i = 0; i < kv8_row_tiles(A, q); ++i) u += (unsigned)kv8_tiles<TILE>(A, q, i);
     return u * A.c.kv_heads;
 }
-// CTAs that take part (each has a unit at least), and where their ranges begin.
-FYB_DEV unsigned kv8_ctas(unsigned U) { return min(gridDim.x, U); }
-FYB_DEV unsigned kv8_cta_begin(unsigned U, unsigned c)
+// CTAs that take part, and where their ranges begin. Few units go to fewer
+// CTAs, LEAST each: a tile more takes a CTA 0.35 us, joining parts 3 us.
+template <int LEAST> FYB_DEV unsigned kv8_ctas(unsigned U) { return min(gridDim.x, max(1u, U / LEAST)); }
+FYB_DEV unsigned kv8_cta_begin(unsigned U, unsigned C, unsigned c)
 {
-    const unsigned C = kv8_ctas(U);
     return c >= C ? U : (unsigned)((unsigned long long)U * c / C);
 }
 // The CTA whose range holds unit u.
-FYB_DEV unsigned kv8_cta_of(unsigned U, unsigned u)
+FYB_DEV unsigned kv8_cta_of(unsigned U, unsigned C, unsigned u)
 {
-    return (unsigned)((((unsigned long long)u + 1) * kv8_ctas(U) - 1) / U);
+    return (unsigned)((((unsigned long long)u + 1) * C - 1) / U);
 }
 
 // Where a CTA stands on the line of units.
 struct Kv8Place {
-    unsigned units, begin, end;     // all units; this CTA's
+    unsigned units, ctas, begin, end;  // all units and the CTAs that share them; this CTA's
     unsigned request, before;       // request of `begin`, units before it
 };
 // Every thread of the CTA (THREADS of them) calls this once.
-template <int TILE, int THREADS> FYB_DEV Kv8Place kv8_place(const Kv8Attention &A)
+template <int TILE, int THREADS, int LEAST> FYB_DEV Kv8Place kv8_place(const Kv8Attention &A)
 {
     __shared__ unsigned warp_sum[THREADS / 32];
     __shared__ unsigned found[2];
@@ -114,8 +114,9 @@ template <int TILE, int THREADS> FYB_DEV Kv8Place kv8_place(const Kv8Attention &
     }
     Kv8Place p;
     p.units = total;
-    p.begin = kv8_cta_begin(total, blockIdx.x);
-    p.end = kv8_cta_begin(total, blockIdx.x + 1);
+    p.ctas = kv8_ctas<LEAST>(total);
+    p.begin = kv8_cta_begin(total, p.ctas, blockIdx.x);
+    p.end = kv8_cta_begin(total, p.ctas, blockIdx.x + 1);
     if (mine && before <= p.begin && p.begin < before + mine) {
         unsigned r = r0, at = before;
         for (;; ++r) {
@@ -192,7 +193,7 @@ template <int TILE> struct Kv8Walk {
 // whole segment; otherwise leaves a partial, and the last CTA to do so joins
 // all parts. valid(row, &src): whether row is a query row, and which.
 template <int R, int HD, int THREADS, typename Bar, typename Put>
-FYB_DEV void kv8_finish(const Kv8Attention &A, const Kv8Segment &s, unsigned units, unsigned tid, const float2 *ml,
+FYB_DEV void kv8_finish(const Kv8Attention &A, const Kv8Segment &s, const Kv8Place &place, unsigned tid, const float2 *ml,
     const float *o, unsigned rows, float *weights, unsigned max_weights, unsigned *flag, Bar bar, Put put)
 {
     if (s.t0 == 0 && s.t1 == s.tiles) {
@@ -205,7 +206,8 @@ FYB_DEV void kv8_finish(const Kv8Attention &A, const Kv8Segment &s, unsigned uni
         }
         return;
     }
-    const unsigned c0 = kv8_cta_of(units, s.first_unit), c1 = kv8_cta_of(units, s.first_unit + (unsigned)s.tiles - 1);
+    const unsigned c0 = kv8_cta_of(place.units, place.ctas, s.first_unit);
+    const unsigned c1 = kv8_cta_of(place.units, place.ctas, s.first_unit + (unsigned)s.tiles - 1);
     // the segment that ends a CTA's range goes to its second slot, any other to its first
     const unsigned slot = 2 * blockIdx.x + (blockIdx.x == c0 ? 1 : 0);
     for (unsigned i = tid; i < rows * (HD / 4); i += THREADS)

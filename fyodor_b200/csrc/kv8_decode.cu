@@ -22,7 +22,7 @@ constexpr int KD_TILE = 64, KD_WARPS = 4, KD_THREADS = 32 * (KD_WARPS + 1);
 
 template <int HD> struct KdShape {
     static constexpr int STAGE = 2 * KD_TILE * HD;             // K and V bytes
-    static constexpr int STAGES = HD == 128 ? 5 : 10;
+    static constexpr int STAGES = HD == 128 ? 4 : 8;           // 64 KB: three CTAs per SM with four rows, two with eight
 };
 struct KdMeta { float ks[KD_TILE / 16], vs[KD_TILE / 16]; };   // scales of the tile's blocks; ks NaN: block not loaded
 
@@ -67,8 +67,10 @@ FYB_DEV int exponent_of(float x) { return x > 0.f ? max(-126, (int)(__float_as_u
 FYB_DEV float power_of_two(int e) { return e < -126 ? __uint_as_float(1u << max(0, e + 149)) : __uint_as_float((unsigned)(min(e, 127) + 127) << 23); }
 
 // W: rows a thread holds scores of (1: up to four query rows, 2: up to eight).
-template <int HD, unsigned FMT, int W>
-__global__ void __launch_bounds__(KD_THREADS, 2) kv8_decode_kernel(Kv8Attention A, const __grid_constant__ CUtensorMap kmap,
+// QL: whether q has low halves of its own (F32 rows at W = 2; 16-bit rows fit
+// the high half, and at W = 1 the low halves are columns that cost nothing).
+template <int HD, unsigned FMT, int W, bool QL>
+__global__ void __launch_bounds__(KD_THREADS, W == 1 ? 3 : 2) kv8_decode_kernel(Kv8Attention A, const __grid_constant__ CUtensorMap kmap,
     const __grid_constant__ CUtensorMap vmap)
 {
     constexpr int R = 4 * W, STAGES = KdShape<HD>::STAGES, STAGE = KdShape<HD>::STAGE, MT = HD / 16;
@@ -82,11 +84,11 @@ __global__ void __launch_bounds__(KD_THREADS, 2) kv8_decode_kernel(Kv8Attention 
     volatile unsigned *dead = flag + 1;   // a wait ran out: nobody waits any more, the error word is set
     const unsigned tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, kv = A.c.kv_heads;
     if (tid == 0) {
-        for (int i = 0; i < STAGES; ++i) { mbar_init(full + i, 1); mbar_init(empty + i, KD_WARPS); }
+        for (int i = 0; i < STAGES; ++i) { mbar_init(full + i, 2); mbar_init(empty + i, KD_WARPS); }
         *dead = 0;
         fence_barrier_init();
     }
-    const Kv8Place place = kv8_place<KD_TILE, KD_THREADS>(A);  // a CTA barrier inside
+    const Kv8Place place = kv8_place<KD_TILE, KD_THREADS, 5>(A);  // a CTA barrier inside
     Kv8Walk<KD_TILE> walk(A, place);
     Kv8Segment s;
     unsigned stage = 0, phase = 0;
@@ -108,21 +110,17 @@ __global__ void __launch_bounds__(KD_THREADS, 2) kv8_decode_kernel(Kv8Attention 
             float ks = 0.f, vs = 0.f;
             for (int t = s.t0; t < s.t1; ++t) {
                 const int b0 = t * KD_TILE >> A.shift;   // first block of the tile; per of them, or a part of one
-                if (b0 / 32 != have) {
+                const bool fetch = b0 / 32 != have;
+                if (fetch) {
                     have = b0 / 32;
                     const int b = have * 32 + (int)lane;
                     id = b < blocks ? ids[b] : -1;
-                    const bool ok = id >= 0 && (unsigned)id < A.c.blocks;
-                    if (b < blocks && !ok) raise_error(A.error, ERR_BOUNDS);
-                    ks = ok ? A.c.k_scale[(size_t)id * kv + s.head] : NAN;
-                    vs = ok ? A.c.v_scale[(size_t)id * kv + s.head] : 0.f;
-                    if (!ok) id = -1;
+                    if (b < blocks && (unsigned)id >= A.c.blocks) {  // negative ones too
+                        raise_error(A.error, ERR_BOUNDS);
+                        id = -1;
+                    }
                 }
                 wait(empty + stage, phase ^ 1);
-                // groups of 16 positions and the blocks they lie in
-                const unsigned group_block = (unsigned)(b0 & 31) + (lane % (KD_TILE / 16) * 16 >> min(A.shift, 6u));
-                const float gk = __shfl_sync(0xffffffffu, ks, group_block), gv = __shfl_sync(0xffffffffu, vs, group_block);
-                if (lane < KD_TILE / 16) { meta[stage].ks[lane] = gk; meta[stage].vs[lane] = gv; }
                 const int mine = __shfl_sync(0xffffffffu, id, (b0 & 31) + (int)(lane % per));
                 const bool load = lane < per && mine >= 0;
                 const unsigned boxes = __popc(__ballot_sync(0xffffffffu, load));
@@ -137,6 +135,17 @@ __global__ void __launch_bounds__(KD_THREADS, 2) kv8_decode_kernel(Kv8Attention 
                     tma_load_rows(dst, &kmap, row, full + stage);
                     tma_load_rows(dst + KD_TILE * HD, &vmap, row, full + stage);
                 }
+                // the scales come while the tile does
+                if (fetch) {
+                    ks = id >= 0 ? A.c.k_scale[(size_t)id * kv + s.head] : NAN;
+                    vs = id >= 0 ? A.c.v_scale[(size_t)id * kv + s.head] : 0.f;
+                }
+                // groups of 16 positions and the blocks they lie in
+                const unsigned group_block = (unsigned)(b0 & 31) + (lane % (KD_TILE / 16) * 16 >> min(A.shift, 6u));
+                const float gk = __shfl_sync(0xffffffffu, ks, group_block), gv = __shfl_sync(0xffffffffu, vs, group_block);
+                if (lane < KD_TILE / 16) { meta[stage].ks[lane] = gk; meta[stage].vs[lane] = gv; }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(full + stage);
                 ++issued;
                 advance();
             }
@@ -168,7 +177,7 @@ __global__ void __launch_bounds__(KD_THREADS, 2) kv8_decode_kernel(Kv8Attention 
             head = s.head * G + rho % G;
         };
         // ---- q: column g of the B fragments, normalized by a power of two and split in halves
-        unsigned qh[MT][2], ql[W == 2 ? MT : 1][2];
+        unsigned qh[MT][2], ql[QL ? MT : 1][2];
         float factor[W];  // score factor of this thread's rows
         int limit[W];     // positions they attend
         {
@@ -206,7 +215,7 @@ __global__ void __launch_bounds__(KD_THREADS, 2) kv8_decode_kernel(Kv8Attention 
                     qh[k][1] = low ? pack(l[2], l[3]) : pack(h[2], h[3]);
                 } else {
                     qh[k][0] = pack(h[0], h[1]); qh[k][1] = pack(h[2], h[3]);
-                    ql[k][0] = pack(l[0], l[1]); ql[k][1] = pack(l[2], l[3]);
+                    if constexpr (QL) { ql[k][0] = pack(l[0], l[1]); ql[k][1] = pack(l[2], l[3]); }
                 }
             }
 #pragma unroll
@@ -245,7 +254,7 @@ __global__ void __launch_bounds__(KD_THREADS, 2) kv8_decode_kernel(Kv8Attention 
                     kv8_halves<FMT>(r[3], b[1], b[3]);
                     mma_f16(c[0], a, qh[k][0], qh[k][1]);
                     mma_f16(c[1], b, qh[k + 1][0], qh[k + 1][1]);
-                    if constexpr (W == 2) {
+                    if constexpr (QL) {
                         mma_f16(c[0], a, ql[k][0], ql[k][1]);
                         mma_f16(c[1], b, ql[k + 1][0], ql[k + 1][1]);
                     }
@@ -388,7 +397,7 @@ __global__ void __launch_bounds__(KD_THREADS, 2) kv8_decode_kernel(Kv8Attention 
             if (at < R * HD / 4 && at % (HD / 4) == 0) ml_s[at / (HD / 4)] = joined[i];
         }
         bar();
-        kv8_finish<R, HD, 32 * KD_WARPS>(A, s, place.units, tid, ml_s, o_s, (unsigned)nrows, o_s + R * HD,
+        kv8_finish<R, HD, 32 * KD_WARPS>(A, s, place, tid, ml_s, o_s, (unsigned)nrows, o_s + R * HD,
             (KD_WARPS - 1) * R * HD, flag, bar, [&](unsigned rho, unsigned chunk, float4 v) {
                 size_t row;
                 unsigned head;
@@ -399,28 +408,33 @@ __global__ void __launch_bounds__(KD_THREADS, 2) kv8_decode_kernel(Kv8Attention 
     }
 }
 
-template <int HD, unsigned FMT, int W> static int decode_launch(const Kv8Attention &A, const CUtensorMap &k,
+template <int HD, unsigned FMT, int W, bool QL> static int decode_launch(const Kv8Attention &A, const CUtensorMap &k,
     const CUtensorMap &v, unsigned grid, cudaStream_t s)
 {
     constexpr int R = 4 * W, STAGES = KdShape<HD>::STAGES;
     constexpr size_t smem = 1024 + (size_t)STAGES * KdShape<HD>::STAGE + KD_WARPS * R * HD * 4 + STAGES * sizeof(KdMeta) +
                             KD_WARPS * R * 8 + 2 * STAGES * 8 + 16;
-    static_assert(smem <= 113 * 1024, "two CTAs per SM");
+    static_assert(smem <= (W == 1 ? 75 : 113) * 1024, "three, or two, CTAs per SM");
     static std::atomic<unsigned> allowed{0};
-    if (allow_shared((const void *)kv8_decode_kernel<HD, FMT, W>, smem, allowed)) return -2;
-    kv8_decode_kernel<HD, FMT, W><<<grid, KD_THREADS, smem, s>>>(A, k, v);
+    if (allow_shared((const void *)kv8_decode_kernel<HD, FMT, W, QL>, smem, allowed)) return -2;
+    grid = std::min(grid, (W == 1 ? 3u : 2u) * 148);
+    kv8_decode_kernel<HD, FMT, W, QL><<<grid, KD_THREADS, smem, s>>>(A, k, v);
     return cudaGetLastError() == cudaSuccess ? 0 : -2;
+}
+
+template <int HD, unsigned FMT> static int decode_rows(const Kv8Attention &A, const CUtensorMap &k, const CUtensorMap &v,
+    unsigned grid, cudaStream_t s)
+{
+    if (A.max_rows * A.group <= 4) return decode_launch<HD, FMT, 1, false>(A, k, v, grid, s);
+    return A.type == T_F32 ? decode_launch<HD, FMT, 2, true>(A, k, v, grid, s)
+                           : decode_launch<HD, FMT, 2, false>(A, k, v, grid, s);
 }
 
 int launch_kv8_decode(const Kv8Attention &A, const CUtensorMap &k, const CUtensorMap &v, unsigned grid, cudaStream_t s)
 {
-    const bool wide = A.max_rows * A.group > 4, e4m3 = A.c.format == FYB_KV8_E4M3;
-    if (A.c.head_dim == 128) {
-        if (e4m3) return wide ? decode_launch<128, FYB_KV8_E4M3, 2>(A, k, v, grid, s) : decode_launch<128, FYB_KV8_E4M3, 1>(A, k, v, grid, s);
-        return wide ? decode_launch<128, FYB_KV8_INT8, 2>(A, k, v, grid, s) : decode_launch<128, FYB_KV8_INT8, 1>(A, k, v, grid, s);
-    }
-    if (e4m3) return wide ? decode_launch<64, FYB_KV8_E4M3, 2>(A, k, v, grid, s) : decode_launch<64, FYB_KV8_E4M3, 1>(A, k, v, grid, s);
-    return wide ? decode_launch<64, FYB_KV8_INT8, 2>(A, k, v, grid, s) : decode_launch<64, FYB_KV8_INT8, 1>(A, k, v, grid, s);
+    const bool e4m3 = A.c.format == FYB_KV8_E4M3;
+    if (A.c.head_dim == 128) return e4m3 ? decode_rows<128, FYB_KV8_E4M3>(A, k, v, grid, s) : decode_rows<128, FYB_KV8_INT8>(A, k, v, grid, s);
+    return e4m3 ? decode_rows<64, FYB_KV8_E4M3>(A, k, v, grid, s) : decode_rows<64, FYB_KV8_INT8>(A, k, v, grid, s);
 }
 
 }  // namespace fyb

@@ -189,7 +189,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1) kv8_tiles_kernel(Kv8Attention A
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
     kt_fence_before();
-    const Kv8Place place = kv8_place<KT_TILE, KT_THREADS>(A);  // CTA barriers inside
+    const Kv8Place place = kv8_place<KT_TILE, KT_THREADS, 2>(A);  // CTA barriers inside
     kt_fence_after();
     const uint32_t tmem = *(volatile uint32_t *)&sh.tmem;
     Kv8Walk<KT_TILE> walk(A, place);
@@ -411,7 +411,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1) kv8_tiles_kernel(Kv8Attention A
             }
             bar();
             float *all_o = reinterpret_cast<float *>(ring + S::OFF_O);
-            kv8_finish<N, HD, 32 * KT_SOFT>(A, s, place.units, tid, sh.ml, all_o, (unsigned)nrows, all_o, N * HD, &sh.flag, bar,
+            kv8_finish<N, HD, 32 * KT_SOFT>(A, s, place, tid, sh.ml, all_o, (unsigned)nrows, all_o, N * HD, &sh.flag, bar,
                 [&](unsigned rho, unsigned chunk, float4 v) {
                     const size_t r = (size_t)(s.q.first + j0 + (int)(rho / G));
                     kv8_store4(A.out, A.type, r * A.out_stride + (size_t)(s.head * G + rho % G) * HD + 4 * chunk, v);
