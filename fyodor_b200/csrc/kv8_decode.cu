@@ -20,9 +20,9 @@ namespace fyb {
 
 constexpr int KD_TILE = 64, KD_WARPS = 4, KD_THREADS = 32 * (KD_WARPS + 1);
 
-template <int HD> struct KdShape {
+template <int HD, int W> struct KdShape {
     static constexpr int STAGE = 2 * KD_TILE * HD;             // K and V bytes
-    static constexpr int STAGES = HD == 128 ? 4 : 8;           // 64 KB: three CTAs per SM with four rows, two with eight
+    static constexpr int STAGES = (W == 1 ? 4 : 3) * (128 / HD);  // with the sums of the rows, three CTAs per SM
 };
 struct KdMeta { float ks[KD_TILE / 16], vs[KD_TILE / 16]; };   // scales of the tile's blocks; ks NaN: block not loaded
 
@@ -70,10 +70,10 @@ FYB_DEV float power_of_two(int e) { return e < -126 ? __uint_as_float(1u << max(
 // QL: whether q has low halves of its own (F32 rows at W = 2; 16-bit rows fit
 // the high half, and at W = 1 the low halves are columns that cost nothing).
 template <int HD, unsigned FMT, int W, bool QL>
-__global__ void __launch_bounds__(KD_THREADS, W == 1 ? 3 : 2) kv8_decode_kernel(Kv8Attention A, const __grid_constant__ CUtensorMap kmap,
+__global__ void __launch_bounds__(KD_THREADS, 3) kv8_decode_kernel(Kv8Attention A, const __grid_constant__ CUtensorMap kmap,
     const __grid_constant__ CUtensorMap vmap)
 {
-    constexpr int R = 4 * W, STAGES = KdShape<HD>::STAGES, STAGE = KdShape<HD>::STAGE, MT = HD / 16;
+    constexpr int R = 4 * W, STAGES = KdShape<HD, W>::STAGES, STAGE = KdShape<HD, W>::STAGE, MT = HD / 16;
     extern __shared__ unsigned char kd_smem[];
     unsigned char *ring = kd_smem + ((1024u - (smem_u32(kd_smem) & 1023u)) & 1023u);
     float *o_s = reinterpret_cast<float *>(ring + STAGES * STAGE);          // [warps][R][HD], then weights of a join
@@ -411,13 +411,12 @@ __global__ void __launch_bounds__(KD_THREADS, W == 1 ? 3 : 2) kv8_decode_kernel(
 template <int HD, unsigned FMT, int W, bool QL> static int decode_launch(const Kv8Attention &A, const CUtensorMap &k,
     const CUtensorMap &v, unsigned grid, cudaStream_t s)
 {
-    constexpr int R = 4 * W, STAGES = KdShape<HD>::STAGES;
-    constexpr size_t smem = 1024 + (size_t)STAGES * KdShape<HD>::STAGE + KD_WARPS * R * HD * 4 + STAGES * sizeof(KdMeta) +
+    constexpr int R = 4 * W, STAGES = KdShape<HD, W>::STAGES;
+    constexpr size_t smem = 1024 + (size_t)STAGES * KdShape<HD, W>::STAGE + KD_WARPS * R * HD * 4 + STAGES * sizeof(KdMeta) +
                             KD_WARPS * R * 8 + 2 * STAGES * 8 + 16;
-    static_assert(smem <= (W == 1 ? 75 : 113) * 1024, "three, or two, CTAs per SM");
+    static_assert(smem <= 75 * 1024, "three CTAs per SM");
     static std::atomic<unsigned> allowed{0};
     if (allow_shared((const void *)kv8_decode_kernel<HD, FMT, W, QL>, smem, allowed)) return -2;
-    grid = std::min(grid, (W == 1 ? 3u : 2u) * 148);
     kv8_decode_kernel<HD, FMT, W, QL><<<grid, KD_THREADS, smem, s>>>(A, k, v);
     return cudaGetLastError() == cudaSuccess ? 0 : -2;
 }
