@@ -70,7 +70,7 @@ FYB_DEV float power_of_two(int e) { return e < -126 ? __uint_as_float(1u << max(
 // QL: whether q has low halves of its own (F32 rows at W = 2; 16-bit rows fit
 // the high half, and at W = 1 the low halves are columns that cost nothing).
 template <int HD, unsigned FMT, int W, bool QL>
-__global__ void __launch_bounds__(KD_THREADS, 3) kv8_decode_kernel(Kv8Attention A, const __grid_constant__ CUtensorMap kmap,
+__global__ void __launch_bounds__(KD_THREADS, 3) kv8_decode_kernel(const __grid_constant__ Kv8Attention A, const __grid_constant__ CUtensorMap kmap,
     const __grid_constant__ CUtensorMap vmap)
 {
     constexpr int R = 4 * W, STAGES = KdShape<HD, W>::STAGES, STAGE = KdShape<HD, W>::STAGE, MT = HD / 16;

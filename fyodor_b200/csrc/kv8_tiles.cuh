@@ -22,14 +22,20 @@
 // nearest (2000 steps in D2 alone: 3e-5 off), and a product's low halves go
 // first, while the sum is small. Row sums and maxima are F32.
 //
-// Roles: warps 0-7 softmax (two groups of four, a group takes half the rows),
-// 8-11 conversion and q, 12 TMA, 13 MMA.
+// Roles: N / 4 warps softmax (groups of four, 16 rows each; a thread has a
+// position and its group's rows), four K, four V and q, one TMA, one MMA.
 #pragma once
 #include "kv8_attention.cuh"
 
 namespace fyb {
 
-constexpr int KT_TILE = 128, KT_SOFT = 8, KT_CONV = 4, KT_THREADS = 32 * (KT_SOFT + KT_CONV + 2), KT_META = 8;
+constexpr int KT_TILE = 128, KT_CONV = 4, KT_META = 8;
+// Softmax warps (four for every 16 rows), and all threads: four warps convert K, four V, one loads, one issues.
+#ifndef FYB_KT_SOFT64
+#define FYB_KT_SOFT64 16
+#endif
+FYB_HOST_DEV constexpr int kt_soft(int N) { return N == 64 ? FYB_KT_SOFT64 : 8; }
+FYB_HOST_DEV constexpr int kt_threads(int N) { return 32 * (kt_soft(N) + 2 * KT_CONV + 2); }
 constexpr int KT_FLUSH = 2;  // tiles D2 gathers before it is added to the sums
 
 // ---- tcgen05 -------------------------------------------------------------------
@@ -109,22 +115,26 @@ FYB_DEV void kt_wait(uint64_t *bar, unsigned parity, volatile unsigned *dead, un
         break;
     }
 }
-// v[0..C) over the 32 lanes by op: lane i % C returns element i (lanes beyond C repeat)
-template <int C, typename Op> FYB_DEV float kt_reduce(float (&v)[C], unsigned lane, Op op)
+// The CTA's k-th segment, walked from the start; t1 = 0 past the last.
+static __device__ __noinline__ void kt_segment(const Kv8Attention &A, const Kv8Place &place, unsigned k, Kv8Segment *s)
+{
+    Kv8Walk<KT_TILE> walk(A, place);
+    for (unsigned i = 0; i <= k; ++i)
+        if (!walk.next(*s)) { s->t1 = 0; break; }
+}
+// Sums of v[0..16) over the 32 lanes: lane i % 16 returns element i.
+FYB_DEV float kt_sum16(float (&v)[16], unsigned lane)
 {
 #pragma unroll
-    for (int half = C / 2; half; half /= 2) {
+    for (int half = 8; half; half /= 2) {
         const bool up = lane & (unsigned)half;
 #pragma unroll
         for (int i = 0; i < half; ++i) {
             const float give = up ? v[i] : v[i + half], keep = up ? v[i + half] : v[i];
-            v[i] = op(keep, __shfl_xor_sync(0xffffffffu, give, half));
+            v[i] = keep + __shfl_xor_sync(0xffffffffu, give, half);
         }
     }
-    float r = v[0];
-#pragma unroll
-    for (int o = C; o < 32; o <<= 1) r = op(r, __shfl_xor_sync(0xffffffffu, r, o));
-    return r;
+    return v[0] + __shfl_xor_sync(0xffffffffu, v[0], 16);
 }
 FYB_DEV unsigned kt_pack(float lo, float hi)  // fp16 pair
 {
@@ -143,7 +153,13 @@ template <int HD, int N, int QP> struct KtShape {
     // tensor memory: D1 of two tiles, D2 of two flush periods, K and V of two tiles
     static constexpr int D1 = 0, D2 = 2 * N, K = 4 * N, V = K + HD, COLS = V + KT_TILE <= 256 ? 256 : 512;
 };
+// The CTA's parts of segments, walked by the TMA warp alone and handed to the others here: KT_SEGS of them at a
+// time; t1 = 0 ends the line.
+constexpr int KT_SEGS = 4;
 template <int N> struct KtShared {
+    Kv8Segment seg[KT_SEGS], walked[kt_threads(N) / 32];
+    Kv8Place place;
+    uint64_t seg_full[KT_SEGS], seg_empty[KT_SEGS];
     float ks[KT_META][KT_TILE / 16], vs[KT_META][KT_TILE / 16];  // scales by 16 positions; ks NaN: not loaded
     int exponent[KT_META], hole[KT_META];                         // 2^exponent is above every value scale of the tile; whether some were not loaded
     alignas(16) float m[N];
@@ -159,11 +175,11 @@ template <int N> struct KtShared {
 };
 
 template <int HD, unsigned FMT, int N, int QP>
-__global__ void __launch_bounds__(KT_THREADS, 1) kv8_tiles_kernel(Kv8Attention A, const __grid_constant__ CUtensorMap kmap,
+__global__ void __launch_bounds__(kt_threads(N), 1) kv8_tiles_kernel(const __grid_constant__ Kv8Attention A, const __grid_constant__ CUtensorMap kmap,
     const __grid_constant__ CUtensorMap vmap)
 {
     using S = KtShape<HD, N, QP>;
-    constexpr int C = N / 2;  // columns of a softmax thread
+    constexpr int KT_SOFT = kt_soft(N), C = 4 * N / KT_SOFT;  // softmax warps; columns of a softmax thread
     extern __shared__ unsigned char kt_smem[];
     unsigned char *ring = kt_smem + ((1024u - (smem_u32(kt_smem) & 1023u)) & 1023u);
     KtShared<N> &sh = *reinterpret_cast<KtShared<N> *>(ring + S::OFF_END);
@@ -180,26 +196,42 @@ __global__ void __launch_bounds__(KT_THREADS, 1) kv8_tiles_kernel(Kv8Attention A
             mbar_init(sh.q_full + i, KT_CONV); mbar_init(sh.q_empty + i, KT_SOFT);
         }
         for (int i = 0; i < KT_META; ++i) mbar_init(sh.meta_full + i, 1);
+        for (int i = 0; i < KT_SEGS; ++i) { mbar_init(sh.seg_full + i, 1); mbar_init(sh.seg_empty + i, KT_SOFT + 2 * KT_CONV + 1); }
         mbar_init(&sh.drained, 1);
         sh.dead = 0;
         fence_barrier_init();
     }
-    if (warp == KT_SOFT + KT_CONV + 1) {
+    if (warp == KT_SOFT + 2 * KT_CONV + 1) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" :: "r"(smem_u32(&sh.tmem)), "r"(S::COLS) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
     kt_fence_before();
-    const Kv8Place place = kv8_place<KT_TILE, KT_THREADS, 2>(A);  // CTA barriers inside
+    {
+        const Kv8Place place = kv8_place<KT_TILE, kt_threads(N), 2>(A);  // CTA barriers inside
+        if (tid == 0) sh.place = place;
+    }
+    __syncthreads();
     kt_fence_after();
     const uint32_t tmem = *(volatile uint32_t *)&sh.tmem;
-    Kv8Walk<KT_TILE> walk(A, place);
-    Kv8Segment s;
-    unsigned n = 0;  // tiles of this CTA so far
+    unsigned n = 0, seg = 0;  // tiles and segments of this CTA so far
     volatile unsigned *dead = &sh.dead;  // a wait ran out: nobody waits any more, the error word is set
     auto wait = [&](uint64_t *bar, unsigned parity) {
         kt_wait(bar, parity, dead, A.error);
     };
     auto arrive = [&](uint64_t *bar) { __syncwarp(); if (lane == 0) mbar_arrive(bar); };
+    // The segment that comes next; done() with it before the next is asked for. Once a wait has run out every warp
+    // walks by itself: all of them still take the same steps, so none is left at a barrier.
+    auto next = [&]() -> const Kv8Segment * {
+        wait(sh.seg_full + seg % KT_SEGS, seg / KT_SEGS);
+        const Kv8Segment *s = sh.seg + seg % KT_SEGS;
+        if (__builtin_expect(*dead, 0)) {
+            s = sh.walked + warp;
+            if (lane == 0) kt_segment(A, sh.place, seg, sh.walked + warp);
+            __syncwarp();
+        }
+        return s->t1 ? s : nullptr;
+    };
+    auto done = [&] { arrive(sh.seg_empty + seg % KT_SEGS); ++seg; };
 
     if (warp < KT_SOFT) {
         // ================================================== softmax
@@ -212,14 +244,16 @@ __global__ void __launch_bounds__(KT_THREADS, 1) kv8_tiles_kernel(Kv8Attention A
                          : "=r"(r) : "r"((unsigned)x), "r"(3 + group) : "memory");
             return r != 0;
         };
-        auto bar = [] { asm volatile("bar.sync 1, 256;" ::: "memory"); };
+        auto bar = [] { asm volatile("bar.sync 1, %0;" :: "n"(32 * KT_SOFT) : "memory"); };
         constexpr float P_SCALE = 32.f;
-        unsigned seg = 0, period = 0;
-        while (walk.next(s)) {
-            const int j0 = s.row_tile * (int)A.row_tile, nrows = min((int)A.row_tile, s.q.rows - j0) * (int)G;
-            const int all = max(0, s.q.len - s.q.n + j0 + 1);  // positions every row attends
+        unsigned period = 0;
+        while (const Kv8Segment *sp = next()) {
+            const Kv8Segment &s = *sp;
+            const int t0 = s.t0, t1 = s.t1;
+            const int all = max(0, s.q.len - s.q.n + s.row_tile * (int)A.row_tile + 1);  // positions every row attends
             if (pos < C) {
-                const int row = (int)(col + pos);
+                const int row = (int)(col + pos), j0 = s.row_tile * (int)A.row_tile;
+                const int nrows = min((int)A.row_tile, s.q.rows - j0) * (int)G;
                 sh.limit[row] = row < nrows ? s.q.len - s.q.n + j0 + row / (int)G + 1 : 0;
                 sh.m[row] = -3.4e38f;
             }
@@ -228,23 +262,21 @@ __global__ void __launch_bounds__(KT_THREADS, 1) kv8_tiles_kernel(Kv8Attention A
             const bool uneven = sh.uneven[seg & 1];
             if (pos < C) sh.own[col + pos] = sh.row_factor[seg & 1][col + pos];
             arrive(sh.q_empty + (seg & 1));
-            ++seg;
             group_bar();
-            // sums of p of the columns in work and of the other half of the group's; they change places per half
-            float l[16], l_other[16], vref = 0.f;
+            float l[C], vref = 0.f;  // l: sums of p; the 16 columns in work are kept first
             int vexp = -200;
             float *o = reinterpret_cast<float *>(ring + S::OFF_O) + col * HD + pos;  // this thread's sums, HD apart
             const bool mine = HD == 128 || pos < HD;
 #pragma unroll
-            for (int i = 0; i < 16; ++i) l[i] = l_other[i] = 0.f;
+            for (int i = 0; i < C; ++i) l[i] = 0.f;
             if (mine) {
 #pragma unroll 8
                 for (int i = 0; i < C; ++i) o[i * HD] = 0.f;
             }
-            auto swap_halves = [&] {
+            auto next_half = [&] {
                 if constexpr (C > 16) {
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) { const float v = l[i]; l[i] = l_other[i]; l_other[i] = v; }
+                    for (int i = 0; i < 16; ++i) { const float v = l[i]; l[i] = l[C - 16 + i]; l[C - 16 + i] = v; }
                 }
             };
             // adds the D2 of a finished period to o
@@ -252,9 +284,8 @@ __global__ void __launch_bounds__(KT_THREADS, 1) kv8_tiles_kernel(Kv8Attention A
                 kt_fence_after();
 #pragma unroll 1
                 for (int i0 = 0; i0 < C; i0 += 16) {
-                    float y[16];
+                    float y[16], *oc = o + i0 * HD;
                     kt_ld16(tmem + S::D2 + (which & 1) * N + lanes + col + i0, y);
-                    float *oc = o + i0 * HD;
                     kt_wait_ld();
                     if (mine) {
 #pragma unroll
@@ -265,10 +296,10 @@ __global__ void __launch_bounds__(KT_THREADS, 1) kv8_tiles_kernel(Kv8Attention A
             };
             bool pending = false;  // the period before has ended and is not in o yet
             bool fresh = true;     // some row may not have a maximum yet
-            for (int t = s.t0; t < s.t1; ++t, ++n) {
+            for (int t = t0; t < t1; ++t, ++n) {
                 const unsigned b = n & 1, slot = n % KT_META;
-                const int step = (t - s.t0) % KT_FLUSH;
-                if (step == 0 && t > s.t0) { pending = true; ++period; }
+                const int step = (t - t0) % KT_FLUSH;
+                if (step == 0 && t > t0) { pending = true; ++period; }
                 wait(sh.meta_full + slot, n / KT_META);
                 const float ks = sh.ks[slot][pos >> 4], vs = sh.vs[slot][pos >> 4], f = factor * ks;
                 const int e = sh.exponent[slot];
@@ -323,12 +354,10 @@ __global__ void __launch_bounds__(KT_THREADS, 1) kv8_tiles_kernel(Kv8Attention A
 #pragma unroll
                             for (int i = 0; i < 16; ++i) x[i] += sh.m[c0 + i];
                         }
-                        {
-                            float y[16];
 #pragma unroll
-                            for (int i = 0; i < 16; ++i) y[i] = x[i];
-                            const float top = kt_reduce<16>(y, lane, [](float u, float v) { return fmaxf(u, v); });
-                            if (lane < 16) sh.top[warp & 3][c0 + lane] = top;
+                        for (int i = 0; i < 16; ++i) {
+                            const unsigned top = __reduce_max_sync(0xffffffffu, isnan(x[i]) ? 0u : float_order_key(x[i]));
+                            if (lane == 0) sh.top[warp & 3][c0 + i] = top ? float_from_order_key(top) : -INFINITY;
                         }
                         group_bar();
                         if (pos < 16) {
@@ -338,7 +367,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1) kv8_tiles_kernel(Kv8Attention A
                             sh.alpha[c] = up ? ex2(old - top) : 1.f;
                             if (up) sh.m[c] = top;
                         }
-                        if (t > s.t0) wait(sh.o_done + (b ^ 1), (n - 1) >> 1);
+                        if (t > t0) wait(sh.o_done + (b ^ 1), (n - 1) >> 1);
                         if (pending) {
                             flush(period - 1);
                             pending = false;
@@ -381,7 +410,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1) kv8_tiles_kernel(Kv8Attention A
                         *reinterpret_cast<uint4 *>(row + chunk) = make_uint4(h[0], h[1], h[2], h[3]);
                         *reinterpret_cast<uint4 *>(row + S::PB + chunk) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
                     }
-                    swap_halves();
+                    next_half();
                 }
                 kt_fence_before();
                 fence_proxy_async();
@@ -400,9 +429,12 @@ __global__ void __launch_bounds__(KT_THREADS, 1) kv8_tiles_kernel(Kv8Attention A
 #pragma unroll
                     for (int i = 0; i < 16; ++i) o[(i0 + i) * HD] *= back;
                 }
-                const float sum = kt_reduce<16>(l, lane, [](float u, float v) { return u + v; });
+                float y[16];
+#pragma unroll
+                for (int i = 0; i < 16; ++i) y[i] = l[i];
+                const float sum = kt_sum16(y, lane);
                 if (lane < 16) sh.sum[warp & 3][col + i0 + lane] = sum;
-                swap_halves();
+                next_half();
             }
             group_bar();
             if (pos < C) {
@@ -411,20 +443,19 @@ __global__ void __launch_bounds__(KT_THREADS, 1) kv8_tiles_kernel(Kv8Attention A
             }
             bar();
             float *all_o = reinterpret_cast<float *>(ring + S::OFF_O);
-            kv8_finish<N, HD, 32 * KT_SOFT>(A, s, place, tid, sh.ml, all_o, (unsigned)nrows, all_o, N * HD, &sh.flag, bar,
+            const int j0 = s.row_tile * (int)A.row_tile, nrows = min((int)A.row_tile, s.q.rows - j0) * (int)G;
+            kv8_finish<N, HD, 32 * KT_SOFT>(A, s, sh.place, tid, sh.ml, all_o, (unsigned)nrows, all_o, N * HD, &sh.flag, bar,
                 [&](unsigned rho, unsigned chunk, float4 v) {
                     const size_t r = (size_t)(s.q.first + j0 + (int)(rho / G));
                     kv8_store4(A.out, A.type, r * A.out_stride + (size_t)(s.head * G + rho % G) * HD + 4 * chunk, v);
                 });
             bar();
+            done();
         }
     } else if (warp < KT_SOFT + KT_CONV) {
-        // ================================================== q, and 8 bits to fp16
+        // ================================================== K, 8 bits to fp16
         const unsigned ct = tid - 32 * KT_SOFT;
-        constexpr int PER = 128 / N, QV = HD / PER;  // threads of a q row, values of a thread
-        const unsigned cw = warp - KT_SOFT;
-        const uint32_t lanes = (cw * 32u) << 16;
-        auto conv_bar = [] { asm volatile("bar.sync 2, 128;" ::: "memory"); };
+        const uint32_t lanes = ((ct >> 5) * 32u) << 16;
         // K of tile i: a thread converts its position's row, column c of its lane gets values 2c and 2c + 1
         auto keys = [&](unsigned i) {
             const unsigned st = i % S::STAGES, pos = ct;
@@ -451,6 +482,18 @@ __global__ void __launch_bounds__(KT_THREADS, 1) kv8_tiles_kernel(Kv8Attention A
             kt_fence_before();
             arrive(sh.kf_full + (i & 1));
         };
+        unsigned k_at = 0;
+        while (const Kv8Segment *s = next()) {
+#pragma unroll 1
+            for (int left = s->t1 - s->t0; left; --left) keys(k_at++);
+            done();
+        }
+    } else if (warp < KT_SOFT + 2 * KT_CONV) {
+        // ================================================== q; V, 8 bits to fp16
+        const unsigned ct = tid - 32 * (KT_SOFT + KT_CONV), cw = ct >> 5;
+        const uint32_t lanes = (cw * 32u) << 16;
+        constexpr int PER = 128 / N, QV = HD / PER;  // threads of a q row, values of a thread
+        auto conv_bar = [] { asm volatile("bar.sync 2, 128;" ::: "memory"); };
         // V of tile n, transposed: lane = head dimension, column c gets positions 2c and 2c + 1; positions from `rows`
         // on, or never loaded, are 0 and not what lies there (a NaN stays one times 0)
         auto values = [&](int rows) {
@@ -491,8 +534,8 @@ __global__ void __launch_bounds__(KT_THREADS, 1) kv8_tiles_kernel(Kv8Attention A
             arrive(sh.v8_empty + st);
             arrive(sh.vf_full + (n & 1));
         };
-        unsigned seg = 0, k_at = 0;  // K tiles converted
-        while (walk.next(s)) {
+        while (const Kv8Segment *sp = next()) {
+            const Kv8Segment &s = *sp;
             const int j0 = s.row_tile * (int)A.row_tile, nrows = min((int)A.row_tile, s.q.rows - j0) * (int)G;
             const int any = kv8_attended(A, s.q, s.row_tile);
             // ---- q rows, by a power of two that all rows of the tile share; a row whose values are 2^12 below the
@@ -519,7 +562,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1) kv8_tiles_kernel(Kv8Attention A
                 const int below = own > 0.f ? kt_exponent(top) - kt_exponent(own) : 0, extra = below > 12 ? below : 0;
                 const int common = 14 - kt_exponent(top), e = common + extra;
                 const float up = real ? kt_power(min(e, 127)) : 0.f, up2 = kt_power(e - min(e, 127));
-                if (k_at) wait(sh.kf_empty + ((k_at - 1) & 1), (k_at - 1) >> 1);  // the last segment's products have read their q
+                if (n) wait(sh.kf_empty + ((n - 1) & 1), (n - 1) >> 1);  // the last segment's products have read their q
                 if (seg >= 2) wait(sh.q_empty + (seg & 1), (seg >> 1) - 1);
 #pragma unroll 1
                 for (int i = 0; i < QV; i += 8) {
@@ -549,21 +592,27 @@ __global__ void __launch_bounds__(KT_THREADS, 1) kv8_tiles_kernel(Kv8Attention A
                              : "=r"(some) : "r"((unsigned)extra) : "memory");
                 if (ct == 0) sh.uneven[seg & 1] = (int)some;
                 arrive(sh.q_full + (seg & 1));
-                ++seg;
             }
+            const int t1 = s.t1;
 #pragma unroll 1
-            for (int t = s.t0 - 1; t < s.t1; ++t) {  // K one tile ahead of V
-                if (t + 1 < s.t1) keys(k_at++);
-                if (t >= s.t0) {
-                    values(any - t * KT_TILE);
-                    ++n;
-                }
-            }
+            for (int t = s.t0; t < t1; ++t, ++n) values(any - t * KT_TILE);
+            done();
         }
-    } else if (warp == KT_SOFT + KT_CONV) {
+    } else if (warp == KT_SOFT + 2 * KT_CONV) {
         // ================================================== TMA
         const unsigned size = 1u << A.shift, box = min(size, 64u), per = KT_TILE / box;
-        while (walk.next(s)) {
+        __syncwarp();
+        Kv8Walk<KT_TILE> walk(A, sh.place);
+        Kv8Segment s;
+        for (;; ++seg) {
+            const bool more = walk.next(s);
+            if (seg >= KT_SEGS) wait(sh.seg_empty + seg % KT_SEGS, seg / KT_SEGS - 1);
+            if (lane == 0 && !*dead) {
+                if (more) sh.seg[seg % KT_SEGS] = s; else sh.seg[seg % KT_SEGS].t1 = 0;
+                mbar_arrive(sh.seg_full + seg % KT_SEGS);
+            }
+            __syncwarp();
+            if (!more) break;
             const int blocks = (kv8_attended(A, s.q, s.row_tile) + (int)size - 1) >> A.shift;
             const int *ids = A.table + (size_t)s.request * A.table_stride;
             int have = -1, id = 0;  // lane holds block 32 * have + lane
@@ -642,14 +691,16 @@ __global__ void __launch_bounds__(KT_THREADS, 1) kv8_tiles_kernel(Kv8Attention A
             __syncwarp();
             ++k_at;
         };
-        while (walk.next(s)) {
+        while (const Kv8Segment *s = next()) {
+            wait(sh.q_full + (seg & 1), seg >> 1);
+            const int tiles = s->t1 - s->t0;
 #pragma unroll 1
-            for (int t = s.t0 - 1; t < s.t1; ++t) {  // scores one tile ahead of values
-                if (t + 1 < s.t1) scores();
-                if (t < s.t0) continue;
+            for (int t = -1; t < tiles; ++t) {  // scores one tile ahead of values
+                if (t + 1 < tiles) scores();
+                if (t < 0) continue;
                 const unsigned b = n & 1;
-                const int step = (t - s.t0) % KT_FLUSH;
-                if (step == 0 && t > s.t0) ++period;
+                const int step = t % KT_FLUSH;
+                if (step == 0 && t > 0) ++period;
                 wait(sh.vf_full + b, n >> 1);
                 wait(sh.p_full + b, n >> 1);
                 kt_fence_after();
@@ -668,6 +719,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1) kv8_tiles_kernel(Kv8Attention A
                 ++n;
             }
             ++period;
+            done();
         }
         if (kt_elect()) {
             kt_commit(&sh.drained);
@@ -677,7 +729,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1) kv8_tiles_kernel(Kv8Attention A
     }
     kt_fence_before();
     __syncthreads();
-    if (warp == KT_SOFT + KT_CONV + 1) {
+    if (warp == KT_SOFT + 2 * KT_CONV + 1) {
         kt_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" :: "r"(tmem), "r"(S::COLS) : "memory");
     }
@@ -690,7 +742,7 @@ int kv8_tiles_go(const Kv8Attention &A, const CUtensorMap &k, const CUtensorMap 
     static_assert(smem <= 227 * 1024, "shared memory of one CTA");
     static std::atomic<unsigned> allowed{0};
     if (allow_shared((const void *)kv8_tiles_kernel<HD, FMT, N, QP>, smem, allowed)) return -2;
-    kv8_tiles_kernel<HD, FMT, N, QP><<<grid, KT_THREADS, smem, s>>>(A, k, v);
+    kv8_tiles_kernel<HD, FMT, N, QP><<<grid, kt_threads(N), smem, s>>>(A, k, v);
     return cudaGetLastError() == cudaSuccess ? 0 : -2;
 }
 
