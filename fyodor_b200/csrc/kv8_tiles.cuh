@@ -79,6 +79,16 @@ FYB_DEV void kt_ld16(uint32_t addr, float *r)
                    "=f"(r[8]), "=f"(r[9]), "=f"(r[10]), "=f"(r[11]), "=f"(r[12]), "=f"(r[13]), "=f"(r[14]), "=f"(r[15])
                  : "r"(addr) : "memory");
 }
+FYB_DEV void kt_ld4(uint32_t addr, float *r)
+{
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x4.b32 {%0,%1,%2,%3}, [%4];"
+                 : "=f"(r[0]), "=f"(r[1]), "=f"(r[2]), "=f"(r[3]) : "r"(addr) : "memory");
+}
+FYB_DEV void kt_st4(uint32_t addr, const float *r)
+{
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1,%2,%3,%4};"
+                 :: "r"(addr), "f"(r[0]), "f"(r[1]), "f"(r[2]), "f"(r[3]) : "memory");
+}
 FYB_DEV void kt_st16(uint32_t addr, const float *r)
 {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
@@ -98,22 +108,17 @@ FYB_DEV void kt_st256(uint32_t addr, const unsigned *r)
 FYB_DEV void kt_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 FYB_DEV void kt_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-// Out of line, as rarely run code is kept small here: the roles' loops together have to stay in the instruction
-// cache (with everything inlined a tile took 7000 cycles, half of them waiting for instructions).
-static __device__ __noinline__ void kt_timeout(volatile unsigned *dead, unsigned *error)
-{
-    *dead = 1;
-    raise_error(error, ERR_TIMEOUT);
-}
-// A bounded wait that gives up when it, or another of the CTA (*dead), has run out.
-FYB_DEV void kt_wait(uint64_t *bar, unsigned parity, volatile unsigned *dead, unsigned *error)
+// A bounded wait that gives up when it, or another of the CTA (*dead), has run out; the kernel's end raises the error
+// word for it. Kept to a few instructions: the roles' loops together have to stay in the instruction cache (with
+// everything inlined a tile took 7000 cycles, half of them waiting for instructions).
+FYB_DEV void kt_wait(uint64_t *bar, unsigned parity, volatile unsigned *dead)
 {
     if (__builtin_expect(mbar_try_wait(bar, parity & 1), 1)) return;
-    for (unsigned i = 0; !mbar_try_wait(bar, parity & 1); ++i) {
-        if (__builtin_expect(i < 1u << 22 && !*dead, 1)) continue;
-        kt_timeout(dead, error);
-        break;
-    }
+    for (unsigned i = 0; !mbar_try_wait(bar, parity & 1); ++i)
+        if (__builtin_expect(i >= 1u << 22 || *dead, 0)) {
+            *dead = 1;
+            break;
+        }
 }
 // The CTA's k-th segment, walked from the start; t1 = 0 past the last.
 static __device__ __noinline__ void kt_segment(const Kv8Attention &A, const Kv8Place &place, unsigned k, Kv8Segment *s)
@@ -216,7 +221,7 @@ __global__ void __launch_bounds__(kt_threads(N), 1) kv8_tiles_kernel(const __gri
     unsigned n = 0, seg = 0;  // tiles and segments of this CTA so far
     volatile unsigned *dead = &sh.dead;  // a wait ran out: nobody waits any more, the error word is set
     auto wait = [&](uint64_t *bar, unsigned parity) {
-        kt_wait(bar, parity, dead, A.error);
+        kt_wait(bar, parity, dead);
     };
     auto arrive = [&](uint64_t *bar) { __syncwarp(); if (lane == 0) mbar_arrive(bar); };
     // The segment that comes next; done() with it before the next is asked for. Once a wait has run out every warp
@@ -374,18 +379,22 @@ __global__ void __launch_bounds__(kt_threads(N), 1) kv8_tiles_kernel(const __gri
                         }
                         kt_fence_after();
                         group_bar();
-                        const uint32_t d2 = tmem + S::D2 + (period & 1) * N + lanes + c0;
-                        float y[16];
-                        if (step) { kt_ld16(d2, y); kt_wait_ld(); }
+                        // four columns at a time: few registers where there are none to spare
 #pragma unroll
-                        for (int i = 0; i < 16; ++i) {
-                            const float alpha = sh.alpha[c0 + i], both = alpha * down;
-                            l[i] *= alpha;
-                            if (mine) o[(i0 + i) * HD] *= both;
-                            y[i] *= both;
-                            x[i] -= sh.m[c0 + i];
+                        for (int i = 0; i < 16; i += 4) {
+                            const uint32_t d2 = tmem + S::D2 + (period & 1) * N + lanes + c0 + i;
+                            float y[4];
+                            if (step) { kt_ld4(d2, y); kt_wait_ld(); }
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) {
+                                const float alpha = sh.alpha[c0 + i + j], both = alpha * down;
+                                l[i + j] *= alpha;
+                                if (mine) o[(i0 + i + j) * HD] *= both;
+                                y[j] *= both;
+                                x[i + j] -= sh.m[c0 + i + j];
+                            }
+                            if (step) { kt_st4(d2, y); kt_wait_st(); }
                         }
-                        if (step) { kt_st16(d2, y); kt_wait_st(); }
                         kt_fence_before();
                     } else if (__builtin_expect(raw, 0)) {
 #pragma unroll
@@ -729,6 +738,7 @@ __global__ void __launch_bounds__(kt_threads(N), 1) kv8_tiles_kernel(const __gri
     }
     kt_fence_before();
     __syncthreads();
+    if (tid == 0 && *dead) raise_error(A.error, ERR_TIMEOUT);
     if (warp == KT_SOFT + 2 * KT_CONV + 1) {
         kt_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" :: "r"(tmem), "r"(S::COLS) : "memory");
