@@ -30,12 +30,13 @@
 namespace fyb {
 
 constexpr int KT_TILE = 128, KT_CONV = 4, KT_META = 8;
-// Softmax warps (four for every 16 rows), and all threads: four warps convert K, four V, one loads, one issues.
-#ifndef FYB_KT_SOFT64
-#define FYB_KT_SOFT64 16
-#endif
-FYB_HOST_DEV constexpr int kt_soft(int N) { return N == 64 ? FYB_KT_SOFT64 : 8; }
-FYB_HOST_DEV constexpr int kt_threads(int N) { return 32 * (kt_soft(N) + 2 * KT_CONV + 2); }
+// Warps: four softmax for every 16 rows; four that convert K and four that convert V, at 32 rows the same four (with
+// 16 warps or fewer a thread has 128 registers, with 18 it has 96: 309 against 274 us for the ragged drafts of 8).
+FYB_HOST_DEV constexpr int kt_soft(int N) { return N / 4; }
+FYB_HOST_DEV constexpr bool kt_split(int N) { return N > 32; }
+FYB_HOST_DEV constexpr int kt_conv(int N) { return kt_split(N) ? 2 * KT_CONV : KT_CONV; }
+FYB_HOST_DEV constexpr int kt_threads(int N) { return 32 * (kt_soft(N) + kt_conv(N) + 2); }
+
 constexpr int KT_FLUSH = 2;  // tiles D2 gathers before it is added to the sums
 
 // ---- tcgen05 -------------------------------------------------------------------
@@ -184,7 +185,9 @@ __global__ void __launch_bounds__(kt_threads(N), 1) kv8_tiles_kernel(const __gri
     const __grid_constant__ CUtensorMap vmap)
 {
     using S = KtShape<HD, N, QP>;
-    constexpr int KT_SOFT = kt_soft(N), C = 4 * N / KT_SOFT;  // softmax warps; columns of a softmax thread
+    constexpr int KT_SOFT = kt_soft(N), C = 16;  // softmax warps; columns of a softmax thread
+    constexpr bool SPLIT = kt_split(N);
+    constexpr unsigned W_TMA = KT_SOFT + kt_conv(N), W_MMA = W_TMA + 1;
     extern __shared__ unsigned char kt_smem[];
     unsigned char *ring = kt_smem + ((1024u - (smem_u32(kt_smem) & 1023u)) & 1023u);
     KtShared<N> &sh = *reinterpret_cast<KtShared<N> *>(ring + S::OFF_END);
@@ -201,12 +204,12 @@ __global__ void __launch_bounds__(kt_threads(N), 1) kv8_tiles_kernel(const __gri
             mbar_init(sh.q_full + i, KT_CONV); mbar_init(sh.q_empty + i, KT_SOFT);
         }
         for (int i = 0; i < KT_META; ++i) mbar_init(sh.meta_full + i, 1);
-        for (int i = 0; i < KT_SEGS; ++i) { mbar_init(sh.seg_full + i, 1); mbar_init(sh.seg_empty + i, KT_SOFT + 2 * KT_CONV + 1); }
+        for (int i = 0; i < KT_SEGS; ++i) { mbar_init(sh.seg_full + i, 1); mbar_init(sh.seg_empty + i, KT_SOFT + kt_conv(N) + 1); }
         mbar_init(&sh.drained, 1);
         sh.dead = 0;
         fence_barrier_init();
     }
-    if (warp == KT_SOFT + 2 * KT_CONV + 1) {
+    if (warp == W_MMA) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" :: "r"(smem_u32(&sh.tmem)), "r"(S::COLS) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
@@ -238,6 +241,35 @@ __global__ void __launch_bounds__(kt_threads(N), 1) kv8_tiles_kernel(const __gri
     };
     auto done = [&] { arrive(sh.seg_empty + seg % KT_SEGS); ++seg; };
 
+    // K of tile i: a thread converts its position's row, column c of its lane gets values 2c and 2c + 1
+    auto keys = [&](unsigned i) {
+        const unsigned ct = tid & 127;
+        const uint32_t lanes = (ct & 96u) << 16;
+        const unsigned st = i % S::STAGES, pos = ct;
+        wait(sh.k8_full + st, i / S::STAGES);
+        if (i >= 2) wait(sh.kf_empty + (i & 1), (i >> 1) - 1);
+        kt_fence_after();
+        const unsigned char *src = ring + S::OFF_K8 + st * S::STAGE + pos * HD;
+        const unsigned z = kv8_swizzle<HD>(pos);
+#pragma unroll 2
+        for (unsigned c = 0; c < HD / 16; c += 2) {
+            unsigned h[16];
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                const uint4 v = *reinterpret_cast<const uint4 *>(src + (((c + k) ^ z) << 4));
+                kv8_halves<FMT>(v.x, h[8 * k], h[8 * k + 1]);
+                kv8_halves<FMT>(v.y, h[8 * k + 2], h[8 * k + 3]);
+                kv8_halves<FMT>(v.z, h[8 * k + 4], h[8 * k + 5]);
+                kv8_halves<FMT>(v.w, h[8 * k + 6], h[8 * k + 7]);
+            }
+            kt_st16(tmem + S::K + (i & 1) * (HD / 2) + lanes + c * 8, reinterpret_cast<float *>(h));
+        }
+        arrive(sh.k8_empty + st);
+        kt_wait_st();
+        kt_fence_before();
+        arrive(sh.kf_full + (i & 1));
+    };
+
     if (warp < KT_SOFT) {
         // ================================================== softmax
         const unsigned group = warp >> 2, pos = (warp & 3) * 32 + lane, col = group * C;
@@ -268,7 +300,7 @@ __global__ void __launch_bounds__(kt_threads(N), 1) kv8_tiles_kernel(const __gri
             if (pos < C) sh.own[col + pos] = sh.row_factor[seg & 1][col + pos];
             arrive(sh.q_empty + (seg & 1));
             group_bar();
-            float l[C], vref = 0.f;  // l: sums of p; the 16 columns in work are kept first
+            float l[C], vref = 0.f;  // l: sums of p
             int vexp = -200;
             float *o = reinterpret_cast<float *>(ring + S::OFF_O) + col * HD + pos;  // this thread's sums, HD apart
             const bool mine = HD == 128 || pos < HD;
@@ -278,12 +310,6 @@ __global__ void __launch_bounds__(kt_threads(N), 1) kv8_tiles_kernel(const __gri
 #pragma unroll 8
                 for (int i = 0; i < C; ++i) o[i * HD] = 0.f;
             }
-            auto next_half = [&] {
-                if constexpr (C > 16) {
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) { const float v = l[i]; l[i] = l[C - 16 + i]; l[C - 16 + i] = v; }
-                }
-            };
             // adds the D2 of a finished period to o
             auto flush = [&](unsigned which) {
                 kt_fence_after();
@@ -419,7 +445,6 @@ __global__ void __launch_bounds__(kt_threads(N), 1) kv8_tiles_kernel(const __gri
                         *reinterpret_cast<uint4 *>(row + chunk) = make_uint4(h[0], h[1], h[2], h[3]);
                         *reinterpret_cast<uint4 *>(row + S::PB + chunk) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
                     }
-                    next_half();
                 }
                 kt_fence_before();
                 fence_proxy_async();
@@ -443,7 +468,6 @@ __global__ void __launch_bounds__(kt_threads(N), 1) kv8_tiles_kernel(const __gri
                 for (int i = 0; i < 16; ++i) y[i] = l[i];
                 const float sum = kt_sum16(y, lane);
                 if (lane < 16) sh.sum[warp & 3][col + i0 + lane] = sum;
-                next_half();
             }
             group_bar();
             if (pos < C) {
@@ -461,45 +485,18 @@ __global__ void __launch_bounds__(kt_threads(N), 1) kv8_tiles_kernel(const __gri
             bar();
             done();
         }
-    } else if (warp < KT_SOFT + KT_CONV) {
+    } else if (SPLIT && warp < KT_SOFT + KT_CONV) {
         // ================================================== K, 8 bits to fp16
-        const unsigned ct = tid - 32 * KT_SOFT;
-        const uint32_t lanes = ((ct >> 5) * 32u) << 16;
-        // K of tile i: a thread converts its position's row, column c of its lane gets values 2c and 2c + 1
-        auto keys = [&](unsigned i) {
-            const unsigned st = i % S::STAGES, pos = ct;
-            wait(sh.k8_full + st, i / S::STAGES);
-            if (i >= 2) wait(sh.kf_empty + (i & 1), (i >> 1) - 1);
-            kt_fence_after();
-            const unsigned char *src = ring + S::OFF_K8 + st * S::STAGE + pos * HD;
-            const unsigned z = kv8_swizzle<HD>(pos);
-#pragma unroll 2
-            for (unsigned c = 0; c < HD / 16; c += 2) {
-                unsigned h[16];
-#pragma unroll
-                for (int k = 0; k < 2; ++k) {
-                    const uint4 v = *reinterpret_cast<const uint4 *>(src + (((c + k) ^ z) << 4));
-                    kv8_halves<FMT>(v.x, h[8 * k], h[8 * k + 1]);
-                    kv8_halves<FMT>(v.y, h[8 * k + 2], h[8 * k + 3]);
-                    kv8_halves<FMT>(v.z, h[8 * k + 4], h[8 * k + 5]);
-                    kv8_halves<FMT>(v.w, h[8 * k + 6], h[8 * k + 7]);
-                }
-                kt_st16(tmem + S::K + (i & 1) * (HD / 2) + lanes + c * 8, reinterpret_cast<float *>(h));
-            }
-            arrive(sh.k8_empty + st);
-            kt_wait_st();
-            kt_fence_before();
-            arrive(sh.kf_full + (i & 1));
-        };
         unsigned k_at = 0;
         while (const Kv8Segment *s = next()) {
 #pragma unroll 1
             for (int left = s->t1 - s->t0; left; --left) keys(k_at++);
             done();
         }
-    } else if (warp < KT_SOFT + 2 * KT_CONV) {
-        // ================================================== q; V, 8 bits to fp16
-        const unsigned ct = tid - 32 * (KT_SOFT + KT_CONV), cw = ct >> 5;
+    } else if (warp < W_TMA) {
+        // ================================================== q; V (and K), 8 bits to fp16
+        const unsigned ct = tid & 127, cw = ct >> 5;
+        unsigned k_at = 0;
         const uint32_t lanes = (cw * 32u) << 16;
         constexpr int PER = 128 / N, QV = HD / PER;  // threads of a q row, values of a thread
         auto conv_bar = [] { asm volatile("bar.sync 2, 128;" ::: "memory"); };
@@ -604,10 +601,15 @@ __global__ void __launch_bounds__(kt_threads(N), 1) kv8_tiles_kernel(const __gri
             }
             const int t1 = s.t1;
 #pragma unroll 1
-            for (int t = s.t0; t < t1; ++t, ++n) values(any - t * KT_TILE);
+            for (int t = SPLIT ? s.t0 : s.t0 - 1; t < t1; ++t) {
+                if (!SPLIT && t + 1 < t1) keys(k_at++);  // one tile ahead: V's buffer frees later
+                if (!SPLIT && t < s.t0) continue;
+                values(any - t * KT_TILE);
+                ++n;
+            }
             done();
         }
-    } else if (warp == KT_SOFT + 2 * KT_CONV) {
+    } else if (warp == W_TMA) {
         // ================================================== TMA
         const unsigned size = 1u << A.shift, box = min(size, 64u), per = KT_TILE / box;
         __syncwarp();
@@ -739,7 +741,7 @@ __global__ void __launch_bounds__(kt_threads(N), 1) kv8_tiles_kernel(const __gri
     kt_fence_before();
     __syncthreads();
     if (tid == 0 && *dead) raise_error(A.error, ERR_TIMEOUT);
-    if (warp == KT_SOFT + 2 * KT_CONV + 1) {
+    if (warp == W_MMA) {
         kt_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" :: "r"(tmem), "r"(S::COLS) : "memory");
     }
