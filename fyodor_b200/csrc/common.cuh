@@ -101,6 +101,15 @@ FYB_DEV void bulk_copy_g2s(void *dst, const void *src, unsigned bytes, uint64_t 
         " cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1], %2, [%3], pol;\n}\n"
         :: "r"(smem_u32(dst)), "l"(src), "r"(bytes), "r"(smem_u32(bar)) : "memory");
 }
+// shared -> global bulk copy (16-byte aligned, bytes a multiple of 16) of this thread's current bulk group
+FYB_DEV void bulk_copy_s2g(void *dst, const void *src, unsigned bytes)
+{
+    asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" :: "l"(dst), "r"(smem_u32(src)), "r"(bytes) : "memory");
+}
+FYB_DEV void bulk_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
+// Until at most N of this thread's bulk groups have yet to read their shared memory (bulk_read) or to end (bulk_drain).
+template <int N> FYB_DEV void bulk_read() { asm volatile("cp.async.bulk.wait_group.read %0;" :: "n"(N) : "memory"); }
+FYB_DEV void bulk_drain() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
 FYB_DEV void ldmatrix_x4(unsigned (&r)[4], const void *p)
 {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"

@@ -229,6 +229,8 @@ struct RopeTable;
 struct RopeRows;
 int rope_table_of(const fyb_rope_desc *d, RopeTable *t);
 bool rope_vectors(const RopeTable &t, unsigned hd, size_t width, const RopeRows &r);
+int rope_run(unsigned type, const RopeTable &t, const int *positions, size_t rows, unsigned hd, const RopeRows &q,
+    const RopeRows &k, unsigned *error, cudaStream_t s);
 
 // ---------------------------------------------------------------- batch.cu
 // Elementwise kernels of the batched decode step (B <= BATCH_MAX sequences).
