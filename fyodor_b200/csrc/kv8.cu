@@ -16,7 +16,8 @@
 
 namespace fyb {
 
-constexpr unsigned KV8_THREADS = 256;
+constexpr unsigned KV8_THREADS = 256;  // of a CTA of rows that each lie in a block of their own, and of q's rows
+constexpr unsigned KV8_RUN_THREADS = 512;  // of runs: 16 warps, four rows each of a run of 64
 
 struct Kv8Append {
     fyb_kv8_cache c;
@@ -45,6 +46,12 @@ template <typename T, int E> FYB_DEV void kv8_values(const Kv8Append &A, const R
     if (!turn || e >= A.rope.dims) return;
     const float *c = A.rope.cos + tab, *s = A.rope.sin + tab;
     if (A.rope.layout == 0) {
+        if (E == 4 && A.vec && e + 4 <= A.rope.dims) {
+            const float2 cv = *reinterpret_cast<const float2 *>(c + e / 2), sv = *reinterpret_cast<const float2 *>(s + e / 2);
+            rope_turn(x[0], x[1], cv.x, sv.x);
+            rope_turn(x[E - 2], x[E - 1], cv.y, sv.y);
+            return;
+        }
 #pragma unroll
         for (int i = 0; i < E; i += 2)
             if (e + i < A.rope.dims) rope_turn(x[i], x[i + 1], c[(e + i) / 2], s[(e + i) / 2]);
@@ -102,21 +109,54 @@ template <unsigned FMT> FYB_DEV unsigned kv8_store4(float a, float b, float c, f
     }
 }
 
+// round(y / now) of four finite values, as the IEEE quotient rounds. The product with the reciprocal is within 2^-22 of
+// the quotient, relatively: where rounding it leaves no doubt the quotient rounds alike, and the division, ten times the
+// instructions, is left to the others (one value in some thousands).
+template <unsigned FMT> FYB_DEV unsigned kv8_quotients(const float (&y)[4], float now, float inv)
+{
+    float r[4];
+    bool sure = true;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) r[e] = __fmul_rn(y[e], inv);
+    if constexpr (FMT == FYB_KV8_INT8) {
+        int q[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const float whole = rintf(r[e]);
+            sure = sure && fabsf(r[e] - whole) < 0.4999f;  // |r| <= 128: off by 4e-5 at the most; false for NaN
+            q[e] = __float2int_rn(whole);
+        }
+        if (sure) {  // -127..127 by the choice of the scale, but for roundings that `sure` leaves out
+            const unsigned lo = __byte_perm((unsigned)q[0], (unsigned)q[1], 0x0040), hi = __byte_perm((unsigned)q[2], (unsigned)q[3], 0x0040);
+            return __byte_perm(lo, hi, 0x5410);
+        }
+    } else {
+        const float up = 1.f + 0x1p-20f, down = 1.f - 0x1p-20f;
+        const unsigned a = kv8_store4<FMT>(r[0] * up, r[1] * up, r[2] * up, r[3] * up);
+        const unsigned b = kv8_store4<FMT>(r[0] * down, r[1] * down, r[2] * down, r[3] * down);
+        sure = a == b && inv <= 3.4028235e38f;
+        if (sure) return a;
+    }
+    return kv8_store4<FMT>(__fdiv_rn(y[0], now), __fdiv_rn(y[1], now), __fdiv_rn(y[2], now), __fdiv_rn(y[3], now));
+}
+
 // CTAs: (window of rows, part), part = one KV head of K or of V; then those of q.
-template <typename T, int HD, unsigned FMT>
-__global__ void __launch_bounds__(KV8_THREADS, 4) kv8_append_kernel(Kv8Append A)
+template <typename T, int HD, unsigned FMT, unsigned THREADS>
+__global__ void __launch_bounds__(THREADS, 1024 / THREADS) kv8_append_kernel(Kv8Append A)
 {
     // a warp's rows of a run: the first HOLD stay in registers between the two passes
-    constexpr int E = HD / 32, WARPS = KV8_THREADS / 32, HOLD = 8;
+    constexpr int E = HD / 32, WARPS = THREADS / 32, HOLD = THREADS == KV8_THREADS ? 1 : 4;
     const unsigned tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, kv = A.c.kv_heads;
     const unsigned windows = (unsigned)((A.rows + A.window - 1) / A.window);
-    if (blockIdx.x >= windows * A.parts) {
+    if (THREADS == KV8_THREADS && blockIdx.x >= windows * A.parts) {
         kv8_turn_q<T, HD>(A, blockIdx.x - windows * A.parts);
         return;
     }
     const unsigned part = blockIdx.x % A.parts;
     const size_t row0 = (size_t)(blockIdx.x / A.parts) * A.window;
-    __shared__ unsigned run_s, first_s, peak_s, leaders_s[KV8_THREADS / 32];
+    __shared__ unsigned run_s, first_s, peak_s, bad_s, leaders_s[THREADS / 32];
+    // slots (-1 for rows that are not stored) and positions of the window, the row before it and a block's rows after
+    __shared__ int slot_s[1 + 256 + 256], pos_s[1 + 256 + 256];
     const bool is_k = part < kv, turn = is_k && A.rope.cos;
     const unsigned head = is_k ? part : part - kv, size = 1u << A.shift;
     const T *src = static_cast<const T *>(is_k ? A.k : A.v) + (size_t)head * HD;
@@ -124,102 +164,128 @@ __global__ void __launch_bounds__(KV8_THREADS, 4) kv8_append_kernel(Kv8Append A)
     unsigned char *pool = static_cast<unsigned char *>(is_k ? A.c.k : A.c.v);
     float *scales = is_k ? A.c.k_scale : A.c.v_scale;
     const int limit = (int)(A.c.blocks << A.shift);
-    // the block of row r, or -1 for a row that is not stored
-    auto block_of = [&](size_t r) {
-        const int slot = A.slots[r];
-        if (slot < 0 || slot >= limit) return -1;
-        if (turn) {
-            const int pos = A.positions[r];
-            if (pos < 0 || (unsigned)pos >= A.rope.rows) return -1;
+    for (unsigned j = tid; j < 1 + A.window + size; j += THREADS) {
+        const size_t r = row0 + j - 1;  // row0 - 1 for j = 0: past the end where there is none
+        int slot = -1, pos = 0;
+        if (r < A.rows) {
+            slot = A.slots[r];
+            if (turn) pos = A.positions[r];
+            if (slot >= 0 && (slot >= limit || pos < 0 || (turn && (unsigned)pos >= A.rope.rows))) {
+                slot = -1;
+                raise_error(A.error, ERR_BOUNDS);
+            }
         }
-        return slot >> A.shift;
-    };
+        slot_s[j] = slot;
+        pos_s[j] = pos;
+    }
+    __syncthreads();
+    // the block of the window's row i (-1 is the row before it), or -1 for a row that is not stored
+    auto block_of = [&](unsigned i) { return slot_s[1 + i] >> A.shift; };
     // ---- the rows of the window that begin a run
     {
-        const size_t r = row0 + tid;
-        bool leads = false;
-        if (tid < A.window && r < A.rows) {
-            const int b = block_of(r);
-            leads = b >= 0 && (r == 0 || block_of(r - 1) != b);
-            if (b < 0 && A.slots[r] >= 0) raise_error(A.error, ERR_BOUNDS);
-        }
+        const bool leads = tid < A.window && block_of(tid) >= 0 && block_of(tid - 1) != block_of(tid);
         const unsigned mask = __ballot_sync(0xffffffffu, leads);
         if (lane == 0) leaders_s[warp] = mask;
         __syncthreads();
     }
     for (unsigned w = 0; w < (A.window + 31) / 32; ++w)
     for (unsigned left = leaders_s[w]; left; left &= left - 1) {
-        const size_t r0 = row0 + 32 * w + (unsigned)__ffs((int)left) - 1;
-        const int b = A.slots[r0] >> A.shift;
+        const unsigned i0 = 32 * w + (unsigned)__ffs((int)left) - 1;
+        const size_t r0 = row0 + i0;
+        const int b = block_of(i0);
         // ---- the run of rows in block b (at most one per slot) and its lowest offset
-        if (tid == 0) { run_s = size; first_s = size; peak_s = 0u; }
+        if (tid == 0) { run_s = size; first_s = size; peak_s = 0u; bad_s = 0u; }
         __syncthreads();
-        const bool in = tid < size && r0 + tid < A.rows && block_of(r0 + tid) == b;
+        const bool in = tid < size && block_of(i0 + tid) == b;
         if (!in && tid < size) atomicMin(&run_s, tid);
         __syncthreads();
         const unsigned run = run_s;
-        if (tid < run) atomicMin(&first_s, (unsigned)A.slots[r0 + tid] & (size - 1));
+        if (tid < run) atomicMin(&first_s, (unsigned)slot_s[1 + i0 + tid] & (size - 1));
+        const size_t at = (size_t)b * kv + head;
+        const float before = scales[at];  // asked for early; counts only if the block holds older tokens
         // ---- largest magnitude
-        RopePack<T, E> held[HOLD];
+        float held[HOLD][E];
         float peak = 0.f;
         bool bad = false;
         auto row_at = [&](unsigned i) { return src + (r0 + i) * stride; };
         auto value = [&](unsigned i, const RopePack<T, E> &own, float (&y)[E]) {
-            const size_t tab = turn ? (size_t)A.positions[r0 + i] * (A.rope.dims / 2) : 0;
+            const size_t tab = turn ? (size_t)pos_s[1 + i0 + i] * (A.rope.dims / 2) : 0;
             kv8_values<T, E>(A, own, row_at(i), lane * E, turn, tab, y);
         };
-        auto look = [&](unsigned i, const RopePack<T, E> &own) {
-            float y[E];
-            value(i, own, y);
+        auto look = [&](const float (&y)[E]) {
 #pragma unroll
             for (int e = 0; e < E; ++e) {
                 const float m = fabsf(y[e]);
                 if (m <= 3.4028235e38f) peak = fmaxf(peak, m); else bad = true;
             }
         };
+        {
+            RopePack<T, E> raw[HOLD];
 #pragma unroll
-        for (int h = 0; h < HOLD; ++h)
-            if (warp + h * WARPS < run) held[h] = kv8_get<T, E>(A, row_at(warp + h * WARPS) + lane * E);
+            for (int h = 0; h < HOLD; ++h)
+                if (warp + h * WARPS < run) raw[h] = kv8_get<T, E>(A, row_at(warp + h * WARPS) + lane * E);
 #pragma unroll
-        for (int h = 0; h < HOLD; ++h)
-            if (warp + h * WARPS < run) look(warp + h * WARPS, held[h]);
-        for (unsigned i = warp + HOLD * WARPS; i < run; i += WARPS) look(i, kv8_get<T, E>(A, row_at(i) + lane * E));
-        if (bad) raise_error(A.error, ERR_NONFINITE);
+            for (int h = 0; h < HOLD; ++h)
+                if (warp + h * WARPS < run) {
+                    value(warp + h * WARPS, raw[h], held[h]);
+                    look(held[h]);
+                }
+        }
+        for (unsigned i = warp + HOLD * WARPS; i < run; i += WARPS) {
+            float y[E];
+            value(i, kv8_get<T, E>(A, row_at(i) + lane * E), y);
+            look(y);
+        }
+        if (bad) {
+            raise_error(A.error, ERR_NONFINITE);
+            bad_s = 1;
+        }
         peak = warp_max(peak);
         if (lane == 0) atomicMax(&peak_s, __float_as_uint(peak));  // non-negative: ordered as integers
         __syncthreads();
         const unsigned first = first_s;
-        const size_t at = (size_t)b * kv + head;
-        const float was = first ? scales[at] : 0.f;
+        const float was = first ? before : 0.f;
         const float now = fmaxf(was, kv8_scale(FMT, __uint_as_float(peak_s)));
         unsigned char *blk = pool + at * size * HD;
         if (now > was && first) {
             const float keep = __fdiv_rn(was, now);
             unsigned *words = reinterpret_cast<unsigned *>(blk);
-            for (unsigned i = tid; i < first * HD / 4; i += KV8_THREADS) {
+            for (unsigned i = tid; i < first * HD / 4; i += THREADS) {
                 const unsigned old = words[i];
                 words[i] = kv8_store4<FMT>(__fmul_rn(kv8_number<FMT>(old & 0xffu), keep), __fmul_rn(kv8_number<FMT>(old >> 8 & 0xffu), keep),
                                            __fmul_rn(kv8_number<FMT>(old >> 16 & 0xffu), keep), __fmul_rn(kv8_number<FMT>(old >> 24), keep));
             }
         }
         // ---- stored values
-        auto store = [&](unsigned i, const RopePack<T, E> &own) {
-            float y[E], q[4] = {0.f, 0.f, 0.f, 0.f};
-            value(i, own, y);
+        const bool plain = now > 0.f && !bad_s;
+        const float inv = __frcp_rn(now);
+        auto store = [&](unsigned i, const float (&y)[E]) {
+            float q[4] = {0.f, 0.f, 0.f, 0.f};
+            unsigned bytes;
+            if (plain) {
 #pragma unroll
-            for (int e = 0; e < E; ++e) {
-                q[e] = now > 0.f ? __fdiv_rn(y[e], now) : 0.f;
-                if (!(fabsf(y[e]) <= 3.4028235e38f)) q[e] = isnan(y[e]) ? 0.f : copysignf(kv8_top(FMT), y[e]);
+                for (int e = 0; e < E; ++e) q[e] = y[e];
+                bytes = kv8_quotients<FMT>(q, now, inv);
+            } else {
+#pragma unroll
+                for (int e = 0; e < E; ++e) {
+                    q[e] = now > 0.f ? __fdiv_rn(y[e], now) : 0.f;
+                    if (!(fabsf(y[e]) <= 3.4028235e38f)) q[e] = isnan(y[e]) ? 0.f : copysignf(kv8_top(FMT), y[e]);
+                }
+                bytes = kv8_store4<FMT>(q[0], q[1], q[2], q[3]);
             }
-            const unsigned bytes = kv8_store4<FMT>(q[0], q[1], q[2], q[3]);
-            unsigned char *dst = blk + ((unsigned)A.slots[r0 + i] & (size - 1)) * HD + lane * E;
+            unsigned char *dst = blk + ((unsigned)slot_s[1 + i0 + i] & (size - 1)) * HD + lane * E;
             if constexpr (E == 4) *reinterpret_cast<unsigned *>(dst) = bytes;
             else *reinterpret_cast<unsigned short *>(dst) = (unsigned short)bytes;
         };
 #pragma unroll
         for (int h = 0; h < HOLD; ++h)
             if (warp + h * WARPS < run) store(warp + h * WARPS, held[h]);
-        for (unsigned i = warp + HOLD * WARPS; i < run; i += WARPS) store(i, kv8_get<T, E>(A, row_at(i) + lane * E));
+        for (unsigned i = warp + HOLD * WARPS; i < run; i += WARPS) {
+            float y[E];
+            value(i, kv8_get<T, E>(A, row_at(i) + lane * E), y);
+            store(i, y);
+        }
         __syncthreads();
         if (tid == 0) scales[at] = now;
     }
@@ -266,14 +332,19 @@ __global__ void __launch_bounds__(256) kv8_read_kernel(fyb_kv8_cache c, const in
     }
 }
 
+template <typename T, int HD, unsigned FMT> static void append_kernel(const Kv8Append &A, unsigned grid, cudaStream_t s)
+{
+    if (A.window > 1) kv8_append_kernel<T, HD, FMT, KV8_RUN_THREADS><<<grid, KV8_RUN_THREADS, 0, s>>>(A);
+    else kv8_append_kernel<T, HD, FMT, KV8_THREADS><<<grid, KV8_THREADS, 0, s>>>(A);
+}
 template <typename T> static void append_launch(const Kv8Append &A, unsigned grid, cudaStream_t s)
 {
     if (A.c.head_dim == 128) {
-        if (A.c.format == FYB_KV8_INT8) kv8_append_kernel<T, 128, FYB_KV8_INT8><<<grid, KV8_THREADS, 0, s>>>(A);
-        else kv8_append_kernel<T, 128, FYB_KV8_E4M3><<<grid, KV8_THREADS, 0, s>>>(A);
+        if (A.c.format == FYB_KV8_INT8) append_kernel<T, 128, FYB_KV8_INT8>(A, grid, s);
+        else append_kernel<T, 128, FYB_KV8_E4M3>(A, grid, s);
     } else {
-        if (A.c.format == FYB_KV8_INT8) kv8_append_kernel<T, 64, FYB_KV8_INT8><<<grid, KV8_THREADS, 0, s>>>(A);
-        else kv8_append_kernel<T, 64, FYB_KV8_E4M3><<<grid, KV8_THREADS, 0, s>>>(A);
+        if (A.c.format == FYB_KV8_INT8) append_kernel<T, 64, FYB_KV8_INT8>(A, grid, s);
+        else append_kernel<T, 64, FYB_KV8_E4M3>(A, grid, s);
     }
 }
 
@@ -307,22 +378,25 @@ extern "C" int fyb_kv8_append(const fyb_kv8_cache *cache, const int32_t *slots, 
     const size_t el = 16 / width;  // elements of a 16-byte access
     A.vec = ((uintptr_t)k | (uintptr_t)v) % 16 == 0 && k_stride % el == 0 && v_stride % el == 0;
     if (rope) A.vec = A.vec && rope_vectors(A.rope, hd, width, A.q);
-    A.q_rows = 0;
-    if (heads) {
-        A.work = rope_work(hd, A.rope.dims, A.rope.layout, A.vec ? (unsigned)el : A.rope.layout == 0 ? 2u : 1u, q == q_out);
-        A.many = A.vec && rope_many(rows, heads, A.work);
-        const unsigned groups = A.many ? (heads + ROPE_HEADS - 1) / ROPE_HEADS : heads;
-        A.q_rows = (unsigned)(((size_t)groups * (A.work.turned + A.work.copied) + KV8_THREADS - 1) / KV8_THREADS);
-    }
     // a CTA looks at one row while that makes at most 16 CTAs per SM, at up to
     // a block of rows beyond: a prompt's rows mostly follow one another
     A.window = 1;
     A.parts = 2 * kv;
     while (A.window < cache->block_size && rows / A.window * A.parts > 16 * 148) A.window *= 2;
+    cudaStream_t s = (cudaStream_t)stream;
+    A.q_rows = 0;
+    if (heads && A.window > 1) {  // a launch more is little beside a prompt
+        const int r = rope_run(type, A.rope, positions, rows, hd, A.q, RopeRows{}, error, s);
+        if (r) return r;
+    } else if (heads) {
+        A.work = rope_work(hd, A.rope.dims, A.rope.layout, A.vec ? (unsigned)el : A.rope.layout == 0 ? 2u : 1u, q == q_out);
+        A.many = A.vec && rope_many(rows, heads, A.work);
+        const unsigned groups = A.many ? (heads + ROPE_HEADS - 1) / ROPE_HEADS : heads;
+        A.q_rows = (unsigned)(((size_t)groups * (A.work.turned + A.work.copied) + KV8_THREADS - 1) / KV8_THREADS);
+    }
     const size_t ctas = (rows + A.window - 1) / A.window * A.parts + rows * A.q_rows;
     if (ctas > 0x7fffffffu) return -1;
     const unsigned grid = (unsigned)ctas;
-    cudaStream_t s = (cudaStream_t)stream;
     if (type == T_F32) append_launch<float>(A, grid, s);
     else if (type == T_F16) append_launch<__half>(A, grid, s);
     else append_launch<__nv_bfloat16>(A, grid, s);

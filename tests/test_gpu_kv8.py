@@ -190,6 +190,36 @@ def test_rope(kind, layout, hd, dims):
             assert (got[..., dims:] == x[..., dims:]).all()
 
 
+@pytest.mark.parametrize("kind,layout,hd,dims", [("f32", "half", 128, 128), ("bf16", "interleaved", 128, 64),
+                                                 ("f16", "half", 64, 32), ("f32", "interleaved", 64, 64)])
+@pytest.mark.parametrize("heads,kv", [(32, 8), (7, 0)])
+def test_rope_many_rows(kind, layout, hd, dims, heads, kv):
+    """Enough rows that they go through shared memory: strided, in place, with
+    positions outside the table, and beside a row count that is no multiple of anything."""
+    rows, ctx = 9001, 500
+    cos, sin = tables(ctx, dims)
+    pos = torch.randint(0, ctx, (rows,), dtype=torch.int32)
+    pos[[5, rows - 1]] = torch.tensor([-1, ctx], dtype=torch.int32)
+    fine = ((pos >= 0) & (pos < ctx))
+    y = torch.randn((rows, heads + kv + 1, hd), device="cuda").to(ROW_TYPES[kind])
+    q, k = y[:, :heads], y[:, heads:heads + kv] if kv else None
+    c, s = (t[pos.clamp(0, ctx - 1).long().cuda()].cpu() for t in (cos, sin))
+    for inplace in (False, True):
+        err = torch.zeros(1, dtype=torch.int32, device="cuda")
+        base = y.clone()
+        qi, ki = base[:, :heads], base[:, heads:heads + kv] if kv else None
+        qo, ko = (qi, ki) if inplace else (torch.full_like(q, 7.0), torch.full_like(k, 7.0) if kv else None)
+        F.rope(qi, ki, pos.cuda(), cos, sin, layout, qo, ko, error=err)
+        assert err.item() == 4
+        for x, got in ((q, qo), (k, ko)) if kv else ((q, qo),):
+            want = turn(x.cpu(), c, s, layout)
+            assert ((got.cpu().double() - want).abs() <= rope_bound(x.cpu(), want, kind))[fine].all()
+            assert (got[..., dims:] == x[..., dims:])[fine.cuda()].all()
+            left = x if inplace else torch.full_like(x, 7.0)
+            assert torch.equal(got[~fine.cuda()], left[~fine.cuda()])
+        assert torch.equal(base[:, heads + kv:], y[:, heads + kv:])
+
+
 def test_rope_unaligned_and_out_of_table():
     """Odd strides and offsets take the scalar path; positions outside the
     table leave their rows as they were and raise the error word."""
@@ -295,6 +325,37 @@ def test_append_steps(fmt, kind, hd, size):
     ko, vo = (torch.empty(len(held), heads, hd, device="cuda") for _ in "kv")
     cache.read(i32(held), ko, vo)
     assert torch.equal(ko.cpu(), ref.values("k", held)) and torch.equal(vo.cpu(), ref.values("v", held))
+
+
+@pytest.mark.parametrize("fmt", sorted(STORED))
+@pytest.mark.parametrize("kind,hd,size,layout", [("bf16", 128, 64, "interleaved"), ("f32", 64, 256, "half"),
+                                                 ("f16", 128, 16, None)])
+def test_append_prompts(fmt, kind, hd, size, layout):
+    """Prompts of several requests, long enough that CTAs take runs of rows: to the byte, q as by fyb_rope."""
+    g = torch.Generator().manual_seed(size)
+    kv, heads, ctx = 4, 6, 1500
+    news, starts, used, slots, pos = [700, 1, 1311, 260], [0, 5, 77, 256], 0, [], []
+    order = torch.randperm(400, generator=g).tolist()
+    for n, p0 in zip(news, starts):
+        own = order[used:used + -(-(p0 + n) // size)]
+        used += len(own)
+        slots += [own[p // size] * size + p % size for p in range(p0, p0 + n)]
+        pos += range(p0, p0 + n)
+    cache, ref = F.KV8Cache.empty(400, kv, size, hd, fmt), RefCache(400, kv, size, hd, fmt)
+    k, v = (torch.randn(len(slots), kv, hd, generator=g).to(ROW_TYPES[kind]) for _ in "kv")
+    q = torch.randn(len(slots), heads, hd, generator=g).to(ROW_TYPES[kind]).cuda()
+    kw, rotated = {}, k
+    if layout:
+        cos, sin = tables(ctx, hd)
+        qa, qb, kb = torch.empty_like(q), torch.empty_like(q), torch.empty(len(slots), kv, hd, device="cuda")
+        F.rope(q, None, i32(pos), cos, sin, layout, qb, None)
+        F.rope(k.cuda().float(), None, i32(pos), cos, sin, layout, kb, None)
+        rotated, kw = kb.cpu(), dict(positions=i32(pos), cos=cos, sin=sin, layout=layout, q=q, q_out=qa)
+    cache.append(k.cuda(), v.cuda(), i32(slots), **kw)
+    ref.append("k", rotated, slots)
+    ref.append("v", v, slots)
+    same_cache(cache, ref)
+    assert not layout or torch.equal(qa, qb)
 
 
 def test_append_refuses_rows_and_values():
