@@ -16,8 +16,7 @@
 
 namespace fyb {
 
-constexpr unsigned KV8_THREADS = 256;  // of a CTA of rows that each lie in a block of their own, and of q's rows
-constexpr unsigned KV8_RUN_THREADS = 512;  // of runs: 16 warps, four rows each of a run of 64
+constexpr unsigned KV8_THREADS = 256;
 
 struct Kv8Append {
     fyb_kv8_cache c;
@@ -141,14 +140,16 @@ template <unsigned FMT> FYB_DEV unsigned kv8_quotients(const float (&y)[4], floa
 }
 
 // CTAs: (window of rows, part), part = one KV head of K or of V; then those of q.
-template <typename T, int HD, unsigned FMT, unsigned THREADS>
-__global__ void __launch_bounds__(THREADS, 1024 / THREADS) kv8_append_kernel(Kv8Append A)
+template <typename T, int HD, unsigned FMT>
+__global__ void __launch_bounds__(KV8_THREADS, 4) kv8_append_kernel(Kv8Append A)
 {
-    // a warp's rows of a run: the first HOLD stay in registers between the two passes
-    constexpr int E = HD / 32, WARPS = THREADS / 32, HOLD = THREADS == KV8_THREADS ? 1 : 4;
+    // A warp's rows of a run: the first HOLD stay in registers between the two passes, others are fetched again (from
+    // L1 and L2). 4544 rows, 8 KV heads: held 1, 2, 4, 8 took 25, 21, 23, 33 us (8 no longer fit the registers).
+    constexpr unsigned THREADS = KV8_THREADS;
+    constexpr int E = HD / 32, WARPS = THREADS / 32, HOLD = 2;
     const unsigned tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, kv = A.c.kv_heads;
     const unsigned windows = (unsigned)((A.rows + A.window - 1) / A.window);
-    if (THREADS == KV8_THREADS && blockIdx.x >= windows * A.parts) {
+    if (blockIdx.x >= windows * A.parts) {
         kv8_turn_q<T, HD>(A, blockIdx.x - windows * A.parts);
         return;
     }
@@ -332,19 +333,14 @@ __global__ void __launch_bounds__(256) kv8_read_kernel(fyb_kv8_cache c, const in
     }
 }
 
-template <typename T, int HD, unsigned FMT> static void append_kernel(const Kv8Append &A, unsigned grid, cudaStream_t s)
-{
-    if (A.window > 1) kv8_append_kernel<T, HD, FMT, KV8_RUN_THREADS><<<grid, KV8_RUN_THREADS, 0, s>>>(A);
-    else kv8_append_kernel<T, HD, FMT, KV8_THREADS><<<grid, KV8_THREADS, 0, s>>>(A);
-}
 template <typename T> static void append_launch(const Kv8Append &A, unsigned grid, cudaStream_t s)
 {
     if (A.c.head_dim == 128) {
-        if (A.c.format == FYB_KV8_INT8) append_kernel<T, 128, FYB_KV8_INT8>(A, grid, s);
-        else append_kernel<T, 128, FYB_KV8_E4M3>(A, grid, s);
+        if (A.c.format == FYB_KV8_INT8) kv8_append_kernel<T, 128, FYB_KV8_INT8><<<grid, KV8_THREADS, 0, s>>>(A);
+        else kv8_append_kernel<T, 128, FYB_KV8_E4M3><<<grid, KV8_THREADS, 0, s>>>(A);
     } else {
-        if (A.c.format == FYB_KV8_INT8) append_kernel<T, 64, FYB_KV8_INT8>(A, grid, s);
-        else append_kernel<T, 64, FYB_KV8_E4M3>(A, grid, s);
+        if (A.c.format == FYB_KV8_INT8) kv8_append_kernel<T, 64, FYB_KV8_INT8><<<grid, KV8_THREADS, 0, s>>>(A);
+        else kv8_append_kernel<T, 64, FYB_KV8_E4M3><<<grid, KV8_THREADS, 0, s>>>(A);
     }
 }
 
@@ -378,11 +374,13 @@ extern "C" int fyb_kv8_append(const fyb_kv8_cache *cache, const int32_t *slots, 
     const size_t el = 16 / width;  // elements of a 16-byte access
     A.vec = ((uintptr_t)k | (uintptr_t)v) % 16 == 0 && k_stride % el == 0 && v_stride % el == 0;
     if (rope) A.vec = A.vec && rope_vectors(A.rope, hd, width, A.q);
-    // a CTA looks at one row while that makes at most 16 CTAs per SM, at up to
-    // a block of rows beyond: a prompt's rows mostly follow one another
+    // a CTA looks at one row while that makes at most 16 CTAs per SM; beyond,
+    // at the rows of up to a block (a prompt's mostly follow one another), 8
+    // CTAs per SM: what a CTA does once is then spread over its rows (16: 26 us
+    // where 8 take 21)
     A.window = 1;
     A.parts = 2 * kv;
-    while (A.window < cache->block_size && rows / A.window * A.parts > 16 * 148) A.window *= 2;
+    while (A.window < cache->block_size && rows / A.window * A.parts > (A.window == 1 ? 16 : 8) * 148) A.window *= 2;
     cudaStream_t s = (cudaStream_t)stream;
     A.q_rows = 0;
     if (heads && A.window > 1) {  // a launch more is little beside a prompt
