@@ -88,48 +88,79 @@ struct Kv8Place {
     unsigned units, ctas, begin, end;  // all units and the CTAs that share them; this CTA's
     unsigned request, before;       // request of `begin`, units before it
 };
-// Every thread of the CTA (THREADS of them) calls this once.
+// Every thread of the CTA (THREADS of them) calls this once. Where no segment is
+// longer than 2 LEAST units and every segment can have a CTA, each gets one: no
+// parts to join, and a request's result does not depend on the others.
 template <int TILE, int THREADS, int LEAST> FYB_DEV Kv8Place kv8_place(const Kv8Attention &A)
 {
-    __shared__ unsigned warp_sum[THREADS / 32];
-    __shared__ unsigned found[2];
-    const unsigned tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    __shared__ uint2 warp_sum[THREADS / 32];
+    __shared__ unsigned found[4], longest;
+    const unsigned tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, kv = A.c.kv_heads;
     const unsigned per = (A.requests + THREADS - 1) / THREADS, r0 = min(tid * per, A.requests),
                    r1 = min(r0 + per, A.requests);
-    unsigned mine = 0;
-    for (unsigned r = r0; r < r1; ++r) mine += kv8_units<TILE>(A, kv8_request(A, r, blockIdx.x == 0));
-    unsigned upto = mine;
+    unsigned units = 0, segments = 0, most = 0;
+    for (unsigned r = r0; r < r1; ++r) {
+        const Kv8Request q = kv8_request(A, r, blockIdx.x == 0);
+        const int tiles = kv8_row_tiles(A, q);
+        units += kv8_units<TILE>(A, q);
+        segments += (unsigned)tiles * kv;
+        if (tiles) most = max(most, (unsigned)kv8_tiles<TILE>(A, q, tiles - 1));  // the last row tile attends most
+    }
+    uint2 upto = make_uint2(units, segments);
 #pragma unroll
     for (unsigned o = 1; o < 32; o <<= 1) {
-        const unsigned x = __shfl_up_sync(0xffffffffu, upto, o);
-        if (lane >= o) upto += x;
+        const unsigned x = __shfl_up_sync(0xffffffffu, upto.x, o), y = __shfl_up_sync(0xffffffffu, upto.y, o);
+        if (lane >= o) { upto.x += x; upto.y += y; }
     }
     if (lane == 31) warp_sum[warp] = upto;
-    if (tid < 2) found[tid] = 0;
+    if (tid < 4) found[tid] = 0;
+    if (tid == 0) longest = 0;
     __syncthreads();
-    unsigned before = upto - mine, total = 0;
+    most = __reduce_max_sync(0xffffffffu, most);
+    if (lane == 0) atomicMax(&longest, most);
+    unsigned before = upto.x - units, segments_before = upto.y - segments, total = 0, all = 0;
     for (unsigned w = 0; w < THREADS / 32; ++w) {
-        if (w < warp) before += warp_sum[w];
-        total += warp_sum[w];
+        if (w < warp) { before += warp_sum[w].x; segments_before += warp_sum[w].y; }
+        total += warp_sum[w].x;
+        all += warp_sum[w].y;
     }
+    __syncthreads();
     Kv8Place p;
     p.units = total;
-    p.ctas = kv8_ctas<LEAST>(total);
+    const bool whole = longest <= 2 * LEAST && all <= gridDim.x;  // a segment for each CTA
+    p.ctas = whole ? all : kv8_ctas<LEAST>(total);
     p.begin = kv8_cta_begin(total, p.ctas, blockIdx.x);
     p.end = kv8_cta_begin(total, p.ctas, blockIdx.x + 1);
-    if (mine && before <= p.begin && p.begin < before + mine) {
-        unsigned r = r0, at = before;
+    if (whole ? segments && segments_before <= blockIdx.x && blockIdx.x < segments_before + segments
+              : units && before <= p.begin && p.begin < before + units) {
+        unsigned r = r0, at = before, seg = segments_before;
         for (;; ++r) {
-            const unsigned u = kv8_units<TILE>(A, kv8_request(A, r, false));
-            if (p.begin < at + u) break;
+            const Kv8Request q = kv8_request(A, r, false);
+            const unsigned u = kv8_units<TILE>(A, q), n = (unsigned)kv8_row_tiles(A, q) * kv;
+            if (whole ? blockIdx.x < seg + n : p.begin < at + u) break;
             at += u;
+            seg += n;
         }
         found[0] = r;
         found[1] = at;
+        if (whole) {
+            // segment blockIdx.x - seg of the request: its units
+            const Kv8Request q = kv8_request(A, r, false);
+            unsigned left = blockIdx.x - seg, u = at;
+            int i = 0;
+            for (; left >= kv; ++i, left -= kv) u += (unsigned)kv8_tiles<TILE>(A, q, i) * kv;
+            const unsigned tiles = (unsigned)kv8_tiles<TILE>(A, q, i);
+            found[2] = u + left * tiles;
+            found[3] = u + (left + 1) * tiles;
+        }
     }
     __syncthreads();
     p.request = found[0];
     p.before = found[1];
+    if (whole) {
+        p.begin = found[2];
+        p.end = found[3];
+    }
     return p;
 }
 
@@ -187,6 +218,20 @@ template <int TILE> struct Kv8Walk {
     }
 };
 
+// Maximum and sum over groups of G lanes; every lane of the warp takes part.
+template <int G> FYB_DEV float group_max(float x)
+{
+#pragma unroll
+    for (int o = G / 2; o; o >>= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
+    return x;
+}
+template <int G> FYB_DEV float group_sum(float x)
+{
+#pragma unroll
+    for (int o = G / 2; o; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+    return x;
+}
+
 // ---- joining the parts of a segment -------------------------------------------
 // `threads` threads hold the segment's part as ml[R] and o[R][HD] in shared
 // memory; bar(): a barrier over them. Writes the rows out when the CTA has the
@@ -222,23 +267,30 @@ FYB_DEV void kv8_finish(const Kv8Attention &A, const Kv8Segment &s, const Kv8Pla
     if (tid == 0) A.counters[c0] = 0;
     const unsigned parts = c1 - c0 + 1;
     auto slot_of = [&](unsigned p) { return (size_t)(2 * (c0 + p) + (p == 0 ? 1 : 0)); };
-    // weights of the parts: 2^(m - max m) / sum, as many rows at a time as fit
+    // weights of the parts: 2^(m - max m) / sum, as many rows at a time as fit,
+    // the threads shared out among the rows: it is L2's latency that takes time
+    constexpr unsigned G = THREADS / R < 32 ? THREADS / R : 32;
+    static_assert(G > 0 && (G & (G - 1)) == 0 && THREADS / G >= R, "");
     const unsigned batch = max(1u, min(rows, max_weights / parts));
     for (unsigned row0 = 0; row0 < rows; row0 += batch) {
         const unsigned some = min(batch, rows - row0);
         bar();
-        for (unsigned i = tid; i < some; i += THREADS) {
-            float m = -INFINITY, l = 0.f;
-            for (unsigned p = 0; p < parts; ++p) m = fmaxf(m, __ldcg(&A.part_ml[slot_of(p) * R + row0 + i].x));
-            for (unsigned p = 0; p < parts; ++p) {
+        const unsigned i = tid / G, lane = tid % G;
+        float m = -INFINITY, l = 0.f;
+        if (i < some)
+            for (unsigned p = lane; p < parts; p += G) m = fmaxf(m, __ldcg(&A.part_ml[slot_of(p) * R + row0 + i].x));
+        m = group_max<G>(m);
+        if (i < some)
+            for (unsigned p = lane; p < parts; p += G) {
                 const float2 x = __ldcg(&A.part_ml[slot_of(p) * R + row0 + i]);
                 const float w = exp2f(x.x - m);
                 weights[p * some + i] = w;
                 l += x.y * w;
             }
-            const float n = l > 0.f || isnan(l) ? 1.f / l : 0.f;
-            for (unsigned p = 0; p < parts; ++p) weights[p * some + i] *= n;
-        }
+        l = group_sum<G>(l);
+        const float n = l > 0.f || isnan(l) ? 1.f / l : 0.f;
+        if (i < some)
+            for (unsigned p = lane; p < parts; p += G) weights[p * some + i] *= n;
         bar();
         for (unsigned i = tid; i < some * (HD / 4); i += THREADS) {
             const unsigned row = i / (HD / 4);
