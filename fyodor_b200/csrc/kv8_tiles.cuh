@@ -313,15 +313,12 @@ __global__ void __launch_bounds__(kt_threads(N), 1) kv8_tiles_kernel(const __gri
             // adds the D2 of a finished period to o
             auto flush = [&](unsigned which) {
                 kt_fence_after();
-#pragma unroll 1
-                for (int i0 = 0; i0 < C; i0 += 16) {
-                    float y[16], *oc = o + i0 * HD;
-                    kt_ld16(tmem + S::D2 + (which & 1) * N + lanes + col + i0, y);
-                    kt_wait_ld();
-                    if (mine) {
+                float y[16];
+                kt_ld16(tmem + S::D2 + (which & 1) * N + lanes + col, y);
+                kt_wait_ld();
+                if (mine) {
 #pragma unroll
-                        for (int i = 0; i < 16; ++i) oc[i * HD] += y[i];
-                    }
+                    for (int i = 0; i < 16; ++i) o[i * HD] += y[i];
                 }
                 kt_fence_before();
             };
@@ -350,101 +347,97 @@ __global__ void __launch_bounds__(kt_threads(N), 1) kv8_tiles_kernel(const __gri
                 }
                 wait(sh.d1_full + b, n >> 1);
                 kt_fence_after();
-#pragma unroll 1
-                for (int i0 = 0; i0 < C; i0 += 16) {
-                    const unsigned c0 = col + i0;
-                    const float4 *m4 = reinterpret_cast<const float4 *>(sh.m + c0);
-                    float x[16];
-                    kt_ld16(tmem + S::D1 + lanes + b * N + c0, x);
-                    kt_wait_ld();
-                    if (__builtin_expect(uneven, 0)) {
+                const float4 *m4 = reinterpret_cast<const float4 *>(sh.m + col);
+                float x[16];
+                kt_ld16(tmem + S::D1 + lanes + b * N + col, x);
+                kt_wait_ld();
+                if (__builtin_expect(uneven, 0)) {
 #pragma unroll
-                        for (int i = 0; i < 16; ++i) x[i] *= sh.own[c0 + i];
+                    for (int i = 0; i < 16; ++i) x[i] *= sh.own[col + i];
+                }
+                // x: the scores less m, or (raw) the scores themselves
+                float over = -INFINITY;
+                if (__builtin_expect(raw, 0)) {
+                    const int at = isnan(ks) ? 0x7fffffff : t * KT_TILE + (int)pos;
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        x[i] = at < sh.limit[col + i] ? x[i] * f : -INFINITY;
+                        over = fmaxf(over, x[i] - sh.m[col + i]);
                     }
-                    // x: the scores less m, or (raw) the scores themselves
-                    float over = -INFINITY;
-                    if (__builtin_expect(raw, 0)) {
-                        const int at = isnan(ks) ? 0x7fffffff : t * KT_TILE + (int)pos;
+                } else {
 #pragma unroll
-                        for (int i = 0; i < 16; ++i) {
-                            x[i] = at < sh.limit[c0 + i] ? x[i] * f : -INFINITY;
-                            over = fmaxf(over, x[i] - sh.m[c0 + i]);
-                        }
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < 16; i += 4) {
-                            const float4 m = m4[i / 4];
-                            x[i] = fmaf(x[i], f, -m.x); x[i + 1] = fmaf(x[i + 1], f, -m.y);
-                            x[i + 2] = fmaf(x[i + 2], f, -m.z); x[i + 3] = fmaf(x[i + 3], f, -m.w);
-                            over = fmaxf(fmaxf(over, fmaxf(x[i], x[i + 1])), fmaxf(x[i + 2], x[i + 3]));
-                        }
+                    for (int i = 0; i < 16; i += 4) {
+                        const float4 m = m4[i / 4];
+                        x[i] = fmaf(x[i], f, -m.x); x[i + 1] = fmaf(x[i + 1], f, -m.y);
+                        x[i + 2] = fmaf(x[i + 2], f, -m.z); x[i + 3] = fmaf(x[i + 3], f, -m.w);
+                        over = fmaxf(fmaxf(over, fmaxf(x[i], x[i + 1])), fmaxf(x[i + 2], x[i + 3]));
                     }
-                    if (__builtin_expect(group_or(over > 8.f || grow), 0)) {
-                        // ---- new maxima, and the sums so far in their units
-                        if (!raw) {
+                }
+                if (__builtin_expect(group_or(over > 8.f || grow), 0)) {
+                    // ---- new maxima, and the sums so far in their units
+                    if (!raw) {
 #pragma unroll
-                            for (int i = 0; i < 16; ++i) x[i] += sh.m[c0 + i];
-                        }
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) {
-                            const unsigned top = __reduce_max_sync(0xffffffffu, isnan(x[i]) ? 0u : float_order_key(x[i]));
-                            if (lane == 0) sh.top[warp & 3][c0 + i] = top ? float_from_order_key(top) : -INFINITY;
-                        }
-                        group_bar();
-                        if (pos < 16) {
-                            const unsigned c = c0 + pos;
-                            const float old = sh.m[c], top = fmaxf(fmaxf(sh.top[0][c], sh.top[1][c]), fmaxf(sh.top[2][c], sh.top[3][c]));
-                            const bool up = top > old + 8.f;  // each row by its own scores
-                            sh.alpha[c] = up ? ex2(old - top) : 1.f;
-                            if (up) sh.m[c] = top;
-                        }
-                        if (t > t0) wait(sh.o_done + (b ^ 1), (n - 1) >> 1);
-                        if (pending) {
-                            flush(period - 1);
-                            pending = false;
-                        }
-                        kt_fence_after();
-                        group_bar();
-                        // four columns at a time: few registers where there are none to spare
-#pragma unroll
-                        for (int i = 0; i < 16; i += 4) {
-                            const uint32_t d2 = tmem + S::D2 + (period & 1) * N + lanes + c0 + i;
-                            float y[4];
-                            if (step) { kt_ld4(d2, y); kt_wait_ld(); }
-#pragma unroll
-                            for (int j = 0; j < 4; ++j) {
-                                const float alpha = sh.alpha[c0 + i + j], both = alpha * down;
-                                l[i + j] *= alpha;
-                                if (mine) o[(i0 + i + j) * HD] *= both;
-                                y[j] *= both;
-                                x[i + j] -= sh.m[c0 + i + j];
-                            }
-                            if (step) { kt_st4(d2, y); kt_wait_st(); }
-                        }
-                        kt_fence_before();
-                    } else if (__builtin_expect(raw, 0)) {
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) x[i] -= sh.m[c0 + i];
+                        for (int i = 0; i < 16; ++i) x[i] += sh.m[col + i];
                     }
-                    // ---- weights, in halves, to shared memory
-                    unsigned char *row = ring + S::OFF_P + b * 2 * S::PB + pos * 128;
 #pragma unroll
-                    for (int i = 0; i < 16; i += 8) {
-                        unsigned h[4], lo[4];
-#pragma unroll
-                        for (int j = 0; j < 8; j += 2) {
-                            const float p0 = ex2(x[i + j]), p1 = ex2(x[i + j + 1]);
-                            l[i + j] += p0;
-                            l[i + j + 1] += p1;
-                            const float w0 = p0 * wv, w1 = p1 * wv;
-                            h[j / 2] = kt_pack(w0, w1);
-                            const float2 u = kt_unpack(h[j / 2]);
-                            lo[j / 2] = kt_pack(w0 - u.x, w1 - u.y);
-                        }
-                        const unsigned chunk = (((c0 + i) >> 3) ^ (pos & 7u)) << 4;
-                        *reinterpret_cast<uint4 *>(row + chunk) = make_uint4(h[0], h[1], h[2], h[3]);
-                        *reinterpret_cast<uint4 *>(row + S::PB + chunk) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+                    for (int i = 0; i < 16; ++i) {
+                        const unsigned top = __reduce_max_sync(0xffffffffu, isnan(x[i]) ? 0u : float_order_key(x[i]));
+                        if (lane == 0) sh.top[warp & 3][col + i] = top ? float_from_order_key(top) : -INFINITY;
                     }
+                    group_bar();
+                    if (pos < 16) {
+                        const unsigned c = col + pos;
+                        const float old = sh.m[c], top = fmaxf(fmaxf(sh.top[0][c], sh.top[1][c]), fmaxf(sh.top[2][c], sh.top[3][c]));
+                        const bool up = top > old + 8.f;  // each row by its own scores
+                        sh.alpha[c] = up ? ex2(old - top) : 1.f;
+                        if (up) sh.m[c] = top;
+                    }
+                    if (t > t0) wait(sh.o_done + (b ^ 1), (n - 1) >> 1);
+                    if (pending) {
+                        flush(period - 1);
+                        pending = false;
+                    }
+                    kt_fence_after();
+                    group_bar();
+                    // four columns at a time: few registers where there are none to spare
+#pragma unroll
+                    for (int i = 0; i < 16; i += 4) {
+                        const uint32_t d2 = tmem + S::D2 + (period & 1) * N + lanes + col + i;
+                        float y[4];
+                        if (step) { kt_ld4(d2, y); kt_wait_ld(); }
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            const float alpha = sh.alpha[col + i + j], both = alpha * down;
+                            l[i + j] *= alpha;
+                            if (mine) o[(i + j) * HD] *= both;
+                            y[j] *= both;
+                            x[i + j] -= sh.m[col + i + j];
+                        }
+                        if (step) { kt_st4(d2, y); kt_wait_st(); }
+                    }
+                    kt_fence_before();
+                } else if (__builtin_expect(raw, 0)) {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) x[i] -= sh.m[col + i];
+                }
+                // ---- weights, in halves, to shared memory
+                unsigned char *row = ring + S::OFF_P + b * 2 * S::PB + pos * 128;
+#pragma unroll
+                for (int i = 0; i < 16; i += 8) {
+                    unsigned h[4], lo[4];
+#pragma unroll
+                    for (int j = 0; j < 8; j += 2) {
+                        const float p0 = ex2(x[i + j]), p1 = ex2(x[i + j + 1]);
+                        l[i + j] += p0;
+                        l[i + j + 1] += p1;
+                        const float w0 = p0 * wv, w1 = p1 * wv;
+                        h[j / 2] = kt_pack(w0, w1);
+                        const float2 u = kt_unpack(h[j / 2]);
+                        lo[j / 2] = kt_pack(w0 - u.x, w1 - u.y);
+                    }
+                    const unsigned chunk = (((col + i) >> 3) ^ (pos & 7u)) << 4;
+                    *reinterpret_cast<uint4 *>(row + chunk) = make_uint4(h[0], h[1], h[2], h[3]);
+                    *reinterpret_cast<uint4 *>(row + S::PB + chunk) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
                 }
                 kt_fence_before();
                 fence_proxy_async();
@@ -457,18 +450,15 @@ __global__ void __launch_bounds__(kt_threads(N), 1) kv8_tiles_kernel(const __gri
             for (int back = pending ? 1 : 0; back >= 0; --back) flush(period - (unsigned)back);
             ++period;
             const float back = vexp < -126 ? 0.f : kt_power(vexp) / P_SCALE;
-#pragma unroll 1
-            for (int i0 = 0; i0 < C; i0 += 16) {
-                if (mine) {
+            if (mine) {
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) o[(i0 + i) * HD] *= back;
-                }
-                float y[16];
-#pragma unroll
-                for (int i = 0; i < 16; ++i) y[i] = l[i];
-                const float sum = kt_sum16(y, lane);
-                if (lane < 16) sh.sum[warp & 3][col + i0 + lane] = sum;
+                for (int i = 0; i < 16; ++i) o[i * HD] *= back;
             }
+            float y[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) y[i] = l[i];
+            const float sum = kt_sum16(y, lane);
+            if (lane < 16) sh.sum[warp & 3][col + lane] = sum;
             group_bar();
             if (pos < C) {
                 const unsigned c = col + pos;

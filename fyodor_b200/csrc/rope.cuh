@@ -28,20 +28,6 @@ template <typename T, int V, bool VEC> FYB_DEV void row_load(const T *p, float (
         for (int i = 0; i < V; ++i) x[i] = row_value(p[i]);
     }
 }
-template <typename T, int V, bool VEC> FYB_DEV void row_store(T *p, const float (&x)[V])
-{
-    if constexpr (VEC) {
-        struct alignas(V * sizeof(T)) Pack { T t[V]; };
-        Pack u;
-#pragma unroll
-        for (int i = 0; i < V; ++i) u.t[i] = row_round<T>(x[i]);
-        *reinterpret_cast<Pack *>(p) = u;
-    } else {
-#pragma unroll
-        for (int i = 0; i < V; ++i) p[i] = row_round<T>(x[i]);
-    }
-}
-
 // One operand of a rotation: rows of `heads` heads, strides in elements.
 struct RopeRows {
     const void *in = nullptr;
@@ -72,7 +58,7 @@ template <int V, bool VEC> FYB_DEV void rope_row(const float *p, float (&x)[V])
 // one per V pairs (both halves) and one per V values that are only copied.
 // V divides the rotated part (both halves of it) and the head, or is 2
 // (interleaved) or 1 (half).
-
+//
 // A row's work, rotated items of all head groups before copied ones: the lanes of a warp then do the same, and
 // neighbouring lanes work on neighbouring memory.
 struct RopeWork {
@@ -182,10 +168,7 @@ FYB_DEV void rope_item(const T *in, T *out, size_t apart, unsigned count, unsign
 
 // Heads that a thread takes: two (they share the cosines and sines) once that leaves two full waves of threads, one
 // below, where the length of a thread is the time of the call.
-#ifndef FYB_ROPE_HEADS
-#define FYB_ROPE_HEADS 2
-#endif
-constexpr int ROPE_HEADS = FYB_ROPE_HEADS;
+constexpr int ROPE_HEADS = 2;
 inline bool rope_many(size_t rows, unsigned heads, const RopeWork &w)
 {
     return rows * (heads / ROPE_HEADS) * (w.turned + w.copied) >= (size_t)2 * 148 * 2048;
