@@ -2,7 +2,17 @@
 // argument checks, the workspace, and which kernel runs.
 //
 // Up to eight query rows per KV head (rows of a request x heads of a group) run
-// on kv8_decode.cu, more on kv8_tiles.cuh, in row tiles of up to 64.
+// on kv8_decode.cu, more on kv8_tiles.cuh in row tiles of 32 rows, or of 64
+// where a request can bring more. Both sides, head_dim 128, int8 (us):
+//
+//   eight rows    16 requests of 8100   decode  62   tiles of 32   97
+//                  1 request of 300             10                 16
+//   32 rows       32 requests of 8100   of 32  184   of 64        235
+//   64 rows       32 requests of 8100          266                247
+//   512 rows       1 request of 16000          166                131
+//
+// (Below a wave of segments tiles of 32 also win at 64 rows, 19 against 31 us
+// for one request of 512, but the lengths that decide it are on the device.)
 #include "kv8_attention.cuh"
 
 namespace fyb {

@@ -22,6 +22,12 @@
 // nearest (2000 steps in D2 alone: 3e-5 off), and a product's low halves go
 // first, while the sum is small. Row sums and maxima are F32.
 //
+// Bound by the softmax warps' latency on one tile: taking out exponentials, low
+// halves, flushes, conversions or MMAs one at a time changes less than 5 %. At
+// N = 64 the row tiles of a long chunk also read K and V from L2 once each.
+// Ragged drafts of 8 (32 requests of 128 to 32768, 32/8 heads, 0.97 GB): 274 us,
+// 0.55 of a measured copy; a chunk of 500 rows at 16001: 355 us.
+//
 // Roles: N / 4 warps softmax (groups of four, 16 rows each; a thread has a
 // position and its group's rows), four K, four V and q, one TMA, one MMA.
 #pragma once
