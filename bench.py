@@ -333,6 +333,8 @@ def run_provider(args):
         pass
 
     cpu = None
+    import oracle as O
+    args.no_cpu_baseline |= not O.reference_available()  # the engine's sources were not here to build it from
     if rank == 0 and world == 1 and not args.no_cpu_baseline:
         rate, n, threads = cpu_reference_rate(model.ptr, model.vocabulary, args.cpu_seconds)
         cpu = {"value": rate, "unit": "tok/s", "cores": threads, "kind": "reference",
