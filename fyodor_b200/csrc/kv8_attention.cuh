@@ -83,13 +83,19 @@ FYB_DEV unsigned kv8_cta_of(unsigned U, unsigned C, unsigned u)
     return (unsigned)((((unsigned long long)u + 1) * C - 1) / U);
 }
 
+// Longest segment that goes whole to a CTA. Many rows: 4 requests of 500 to 800
+// with eight rows of four heads take 31 us on the line's ranges and 21 so, one
+// of 1000 with 100 rows 46 and 33; one of 1200 with eight rows, 21.6 and 24.3,
+// is beyond it.
+constexpr unsigned KA_WHOLE = 8;
+
 // Where a CTA stands on the line of units.
 struct Kv8Place {
     unsigned units, ctas, begin, end;  // all units and the CTAs that share them; this CTA's
     unsigned request, before;       // request of `begin`, units before it
 };
 // Every thread of the CTA (THREADS of them) calls this once. Where no segment is
-// longer than 2 LEAST units and every segment can have a CTA, each gets one: no
+// longer than KA_WHOLE units and every segment can have a CTA, each gets one: no
 // parts to join, and a request's result does not depend on the others (16
 // requests of 20 to 60 tokens: 17.6 us on the line's ranges, 6.2 so; one of 300
 // with eight rows of four heads: 28.8 and 17.3).
@@ -129,7 +135,7 @@ template <int TILE, int THREADS, int LEAST> FYB_DEV Kv8Place kv8_place(const Kv8
     __syncthreads();
     Kv8Place p;
     p.units = total;
-    const bool whole = longest <= 2 * LEAST && all <= gridDim.x;  // a segment for each CTA
+    const bool whole = longest <= KA_WHOLE && all <= gridDim.x;  // a segment for each CTA
     p.ctas = whole ? all : kv8_ctas<LEAST>(total);
     p.begin = kv8_cta_begin(total, p.ctas, blockIdx.x);
     p.end = kv8_cta_begin(total, p.ctas, blockIdx.x + 1);
