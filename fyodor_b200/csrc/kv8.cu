@@ -118,15 +118,15 @@ template <unsigned FMT> FYB_DEV unsigned kv8_quotients(const float (&y)[4], floa
 #pragma unroll
     for (int e = 0; e < 4; ++e) r[e] = __fmul_rn(y[e], inv);
     if constexpr (FMT == FYB_KV8_INT8) {
-        int q[4];
+        unsigned q[4];  // the whole number in the low bits of r + 1.5 x 2^23
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            const float whole = rintf(r[e]);
-            sure = sure && fabsf(r[e] - whole) < 0.4999f;  // |r| <= 128: off by 4e-5 at the most; false for NaN
-            q[e] = __float2int_rn(whole);
+            const float sum = __fadd_rn(r[e], 12582912.f);
+            sure = sure && fabsf(r[e] - __fsub_rn(sum, 12582912.f)) < 0.4999f;  // |r| <= 128: off by 4e-5 at the most; false for NaN
+            q[e] = __float_as_uint(sum);
         }
         if (sure) {  // -127..127 by the choice of the scale, but for roundings that `sure` leaves out
-            const unsigned lo = __byte_perm((unsigned)q[0], (unsigned)q[1], 0x0040), hi = __byte_perm((unsigned)q[2], (unsigned)q[3], 0x0040);
+            const unsigned lo = __byte_perm(q[0], q[1], 0x0040), hi = __byte_perm(q[2], q[3], 0x0040);
             return __byte_perm(lo, hi, 0x5410);
         }
     } else {
