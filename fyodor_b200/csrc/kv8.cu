@@ -144,7 +144,8 @@ template <typename T, int HD, unsigned FMT>
 __global__ void __launch_bounds__(KV8_THREADS, 4) kv8_append_kernel(Kv8Append A)
 {
     // A warp's rows of a run: the first HOLD stay in registers between the two passes, others are fetched again (from
-    // L1 and L2). 4544 rows, 8 KV heads: held 1, 2, 4, 8 took 25, 21, 23, 33 us (8 no longer fit the registers).
+    // L1 and L2). 4544 rows, 8 KV heads: held 1, 2, 4, 8 took 25, 21, 23, 33 us (8 no longer fit the registers). The
+    // loops fetch one row at a time: two or three, unrolled, took 24 and 25 us, out of the instruction cache.
     constexpr unsigned THREADS = KV8_THREADS;
     constexpr int E = HD / 32, WARPS = THREADS / 32, HOLD = 2;
     const unsigned tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, kv = A.c.kv_heads;
