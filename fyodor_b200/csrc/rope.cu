@@ -240,7 +240,9 @@ extern "C" int fyb_rope_frequencies(uint32_t dims, float base, const fyb_rope_sc
     double lo = 0, hi = 0;
     if (kind == FYB_ROPE_YARN) {
         lo = std::max(0.0, std::floor(pair_of(sc->beta_fast > 0.f ? sc->beta_fast : 32.0)));
-        hi = std::min(pairs - 1.0, std::ceil(pair_of(sc->beta_slow > 0.f ? sc->beta_slow : 1.0)));
+        // past the last pair where every dimension makes more turns than beta_slow: the ramp is then cut off by the
+        // pairs there are, and not made steeper
+        hi = std::min(dims - 1.0, std::ceil(pair_of(sc->beta_slow > 0.f ? sc->beta_slow : 1.0)));
         if (hi - lo < 1e-3) hi = lo + 1e-3;
     }
     for (unsigned j = 0; j < pairs; ++j) {

@@ -1,0 +1,23 @@
+"""The paged 8-bit KV cache on the host side, beside test_kv8.py: where rotary
+frequencies leave the usual contexts, and calls that have nothing to do."""
+import numpy as np
+import pytest
+
+import fyodor_b200 as F
+
+
+@pytest.mark.parametrize("dims,base,factor,ctx", [(128, 10000.0, 16.0, 65536.0), (128, 10000.0, 4.0, 131072.0),
+                                                  (64, 10000.0, 8.0, 1048576.0), (128, 1000000.0, 4.0, 32768.0)])
+def test_frequencies_yarn_past_the_last_pair(dims, base, factor, ctx):
+    """Long original contexts: the slowest pair still makes more than beta_slow
+    turns, so the ramp ends past it and no pair is interpolated whole. F32
+    results of a formula in 64 bits: half a unit, 2^-24."""
+    got, _ = F.rope_frequencies(dims, base, "yarn", factor, ctx)
+    j = np.arange(dims // 2)
+    f = base ** (-2.0 * j / dims)
+    at = lambda turns: dims * np.log(ctx / (2 * np.pi * turns)) / (2 * np.log(base))  # noqa: E731
+    lo, hi = np.floor(at(32.0)), np.ceil(at(1.0))
+    assert 0 <= lo < hi <= dims - 1 and (hi > dims // 2 - 1) == (ctx > 32768)
+    ramp = np.clip((j - lo) / (hi - lo), 0, 1)
+    want = f * (1 - ramp) + f / factor * ramp
+    assert np.all(np.abs(got - want) <= 2.0 ** -24 * want * (1 + 1e-6))
