@@ -375,6 +375,9 @@ extern "C" int fyb_kv8_append(const fyb_kv8_cache *cache, const int32_t *slots, 
     const size_t el = 16 / width;  // elements of a 16-byte access
     A.vec = ((uintptr_t)k | (uintptr_t)v) % 16 == 0 && k_stride % el == 0 && v_stride % el == 0;
     if (rope) A.vec = A.vec && rope_vectors(A.rope, hd, width, A.q);
+    // K's interleaved pairs take two cosines and two sines in an access, q or no q: even table rows, on 8 bytes
+    if (rope && A.rope.layout == 0)
+        A.vec = A.vec && A.rope.dims % 4 == 0 && ((uintptr_t)A.rope.cos | (uintptr_t)A.rope.sin) % 8 == 0;
     // a CTA looks at one row while that makes at most 16 CTAs per SM; beyond,
     // at the rows of up to a block (a prompt's mostly follow one another), 8
     // CTAs per SM: what a CTA does once is then spread over its rows (16: 26 us
