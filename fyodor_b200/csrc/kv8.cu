@@ -7,10 +7,12 @@
 // in F32, so the stored bytes are defined to the bit. Bound by memory: each row is read once and written in a byte a
 // value.
 //
-// The rows of one block are adjacent in the slot list, so the first of them
-// (the row whose predecessor lies in another block) speaks for the block: one
-// CTA takes its whole run for one KV head of K or of V, and no two CTAs touch
-// the same block of a head.
+// The rows of one block are neighbours in the slot list, but for rows that are
+// left out, so the first of them (the row whose predecessor lies in another
+// block) speaks for the block: one CTA takes its whole run for one KV head of K
+// or of V, and no two CTAs touch the same block of a head. A K row left out for
+// its position still belongs to its block's run; a row without a slot belongs to
+// none and ends none.
 #include "rope.cuh"
 #include "kv8.cuh"
 
@@ -156,24 +158,29 @@ __global__ void __launch_bounds__(KV8_THREADS, 4) kv8_append_kernel(Kv8Append A)
     }
     const unsigned part = blockIdx.x % A.parts;
     const size_t row0 = (size_t)(blockIdx.x / A.parts) * A.window;
-    __shared__ unsigned run_s, first_s, peak_s, bad_s, leaders_s[THREADS / 32];
-    // slots (-1 for rows that are not stored) and positions of the window, the row before it and a block's rows after
-    __shared__ int slot_s[1 + 256 + 256], pos_s[1 + 256 + 256];
+    __shared__ unsigned run_s, last_s, first_s, peak_s, bad_s, leaders_s[THREADS / 32];
+    // slots (-1: none) and positions (-1: not stored) of the window and of a block's rows before and after it
+    __shared__ int slot_s[255 + 256 + 256], pos_s[255 + 256 + 256];
     const bool is_k = part < kv, turn = is_k && A.rope.cos;
-    const unsigned head = is_k ? part : part - kv, size = 1u << A.shift;
+    const unsigned head = is_k ? part : part - kv, size = 1u << A.shift, back = size - 1;
     const T *src = static_cast<const T *>(is_k ? A.k : A.v) + (size_t)head * HD;
     const size_t stride = is_k ? A.k_stride : A.v_stride;
     unsigned char *pool = static_cast<unsigned char *>(is_k ? A.c.k : A.c.v);
     float *scales = is_k ? A.c.k_scale : A.c.v_scale;
     const int limit = (int)(A.c.blocks << A.shift);
-    for (unsigned j = tid; j < 1 + A.window + size; j += THREADS) {
-        const size_t r = row0 + j - 1;  // row0 - 1 for j = 0: past the end where there is none
-        int slot = -1, pos = 0;
+    for (unsigned j = tid; j < back + A.window + size; j += THREADS) {
+        const size_t r = row0 + j - back;  // past the end where there is no row before
+        int slot = -1, pos = -1;
         if (r < A.rows) {
             slot = A.slots[r];
-            if (turn) pos = A.positions[r];
-            if (slot >= 0 && (slot >= limit || pos < 0 || (turn && (unsigned)pos >= A.rope.rows))) {
-                slot = -1;
+            pos = turn ? A.positions[r] : 0;
+            if (slot < 0) {
+                slot = pos = -1;
+            } else if (slot >= limit) {
+                slot = pos = -1;
+                raise_error(A.error, ERR_BOUNDS);
+            } else if (turn && (unsigned)pos >= A.rope.rows) {
+                pos = -1;
                 raise_error(A.error, ERR_BOUNDS);
             }
         }
@@ -181,11 +188,16 @@ __global__ void __launch_bounds__(KV8_THREADS, 4) kv8_append_kernel(Kv8Append A)
         pos_s[j] = pos;
     }
     __syncthreads();
-    // the block of the window's row i (-1 is the row before it), or -1 for a row that is not stored
-    auto block_of = [&](unsigned i) { return slot_s[1 + i] >> A.shift; };
+    // the block of the window's row i (negative: a row before it), or -1 for a row without a slot
+    auto block_of = [&](int i) { return slot_s[(int)back + i] >> A.shift; };
     // ---- the rows of the window that begin a run
     {
-        const bool leads = tid < A.window && block_of(tid) >= 0 && block_of(tid - 1) != block_of(tid);
+        bool leads = tid < A.window && block_of((int)tid) >= 0;
+        if (leads) {
+            int i = (int)tid - 1;
+            while (i > (int)tid - (int)back && block_of(i) < 0) --i;
+            leads = block_of(i) != block_of((int)tid);
+        }
         const unsigned mask = __ballot_sync(0xffffffffu, leads);
         if (lane == 0) leaders_s[warp] = mask;
         __syncthreads();
@@ -194,15 +206,28 @@ __global__ void __launch_bounds__(KV8_THREADS, 4) kv8_append_kernel(Kv8Append A)
     for (unsigned left = leaders_s[w]; left; left &= left - 1) {
         const unsigned i0 = 32 * w + (unsigned)__ffs((int)left) - 1;
         const size_t r0 = row0 + i0;
-        const int b = block_of(i0);
-        // ---- the run of rows in block b (at most one per slot) and its lowest offset
-        if (tid == 0) { run_s = size; first_s = size; peak_s = 0u; bad_s = 0u; }
+        const int b = block_of((int)i0);
+        auto stored = [&](unsigned i) { return pos_s[back + i0 + i] >= 0; };
+        // ---- the run of rows in block b: up to another block's, and to the last that is stored; its lowest offset
+        if (tid == 0) { run_s = size; last_s = 0u; first_s = size; peak_s = 0u; bad_s = 0u; }
         __syncthreads();
-        const bool in = tid < size && block_of(i0 + tid) == b;
-        if (!in && tid < size) atomicMin(&run_s, tid);
+        const int own = tid < size ? block_of((int)(i0 + tid)) : -1;
+        const unsigned others = __ballot_sync(0xffffffffu, own >= 0 && own != b);
+        const unsigned kept = __ballot_sync(0xffffffffu, own == b && stored(tid));
+        if (lane == 0) {
+            if (others) atomicMin(&run_s, 32 * warp + (unsigned)__ffs((int)others) - 1);
+            if (kept) atomicMax(&last_s, 32 * warp + 32 - (unsigned)__clz((int)kept));
+        }
         __syncthreads();
-        const unsigned run = run_s;
-        if (tid < run) atomicMin(&first_s, (unsigned)slot_s[1 + i0 + tid] & (size - 1));
+        const unsigned run = min(run_s, last_s);
+        // the rows of it that this warp takes, warp + WARPS h for every bit h
+        static_assert(WARPS * 32 >= 256, "the longest run");
+        const unsigned mine = __ballot_sync(0xffffffffu, warp + WARPS * lane < run && stored(warp + WARPS * lane));
+        if (own == b && tid < run_s) atomicMin(&first_s, (unsigned)slot_s[back + i0 + tid] & (size - 1));
+        if (!run) {  // none of them is stored: the block stays as it is
+            __syncthreads();
+            continue;
+        }
         const size_t at = (size_t)b * kv + head;
         const float before = scales[at];  // asked for early; counts only if the block holds older tokens
         // ---- largest magnitude
@@ -211,7 +236,7 @@ __global__ void __launch_bounds__(KV8_THREADS, 4) kv8_append_kernel(Kv8Append A)
         bool bad = false;
         auto row_at = [&](unsigned i) { return src + (r0 + i) * stride; };
         auto value = [&](unsigned i, const RopePack<T, E> &own, float (&y)[E]) {
-            const size_t tab = turn ? (size_t)pos_s[1 + i0 + i] * (A.rope.dims / 2) : 0;
+            const size_t tab = turn ? (size_t)pos_s[back + i0 + i] * (A.rope.dims / 2) : 0;
             kv8_values<T, E>(A, own, row_at(i), lane * E, turn, tab, y);
         };
         auto look = [&](const float (&y)[E]) {
@@ -225,15 +250,16 @@ __global__ void __launch_bounds__(KV8_THREADS, 4) kv8_append_kernel(Kv8Append A)
             RopePack<T, E> raw[HOLD];
 #pragma unroll
             for (int h = 0; h < HOLD; ++h)
-                if (warp + h * WARPS < run) raw[h] = kv8_get<T, E>(A, row_at(warp + h * WARPS) + lane * E);
+                if (mine >> h & 1) raw[h] = kv8_get<T, E>(A, row_at(warp + h * WARPS) + lane * E);
 #pragma unroll
             for (int h = 0; h < HOLD; ++h)
-                if (warp + h * WARPS < run) {
+                if (mine >> h & 1) {
                     value(warp + h * WARPS, raw[h], held[h]);
                     look(held[h]);
                 }
         }
-        for (unsigned i = warp + HOLD * WARPS; i < run; i += WARPS) {
+        for (unsigned i = warp + HOLD * WARPS, more = mine >> HOLD; more; i += WARPS, more >>= 1) {
+            if (!(more & 1)) continue;
             float y[E];
             value(i, kv8_get<T, E>(A, row_at(i) + lane * E), y);
             look(y);
@@ -276,14 +302,15 @@ __global__ void __launch_bounds__(KV8_THREADS, 4) kv8_append_kernel(Kv8Append A)
                 }
                 bytes = kv8_store4<FMT>(q[0], q[1], q[2], q[3]);
             }
-            unsigned char *dst = blk + ((unsigned)slot_s[1 + i0 + i] & (size - 1)) * HD + lane * E;
+            unsigned char *dst = blk + ((unsigned)slot_s[back + i0 + i] & (size - 1)) * HD + lane * E;
             if constexpr (E == 4) *reinterpret_cast<unsigned *>(dst) = bytes;
             else *reinterpret_cast<unsigned short *>(dst) = (unsigned short)bytes;
         };
 #pragma unroll
         for (int h = 0; h < HOLD; ++h)
-            if (warp + h * WARPS < run) store(warp + h * WARPS, held[h]);
-        for (unsigned i = warp + HOLD * WARPS; i < run; i += WARPS) {
+            if (mine >> h & 1) store(warp + h * WARPS, held[h]);
+        for (unsigned i = warp + HOLD * WARPS, more = mine >> HOLD; more; i += WARPS, more >>= 1) {
+            if (!(more & 1)) continue;
             float y[E];
             value(i, kv8_get<T, E>(A, row_at(i) + lane * E), y);
             store(i, y);

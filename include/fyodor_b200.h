@@ -333,9 +333,13 @@ int fyb_rope(const fyb_rope_desc *rope, const int32_t *positions, size_t rows, u
     void *k_out, size_t k_out_stride, uint32_t kv_heads, uint32_t *error, void *stream);
 
 /* Append K and V rows [rows][kv_heads][head_dim] at slots[row] (a negative slot
-   is skipped). Rows of one block are adjacent in the list and ascend (what
-   fyb_kv_blocks makes of each request); tokens are appended: those below the
-   first new one of a block stay, those above it are no longer valid. The
+   is skipped). Rows of one block follow one another in the list and ascend (what
+   fyb_kv_blocks makes of each request); rows without a slot may lie between
+   them, all rows of a block within block_size of each other. Tokens are
+   appended: those below the first new one of a block stay, those above it are
+   no longer valid. A row whose position is out of the table is left out of K,
+   its neighbours in the block are not; a block none of whose rows is stored
+   stays as it is. The
    block's scale becomes max(old scale, max|x| * (1 / 127 or 1 / 448)) (the old
    scale counts only if the block holds older tokens); where it grows the older
    tokens are stored anew, q' = round(q * (old / new)); new ones are

@@ -40,3 +40,69 @@ def test_append_turns_k_alone(layout, dims, kind, hd, rows):
         ref.append("k", turned.cpu(), slots)
         ref.append("v", v, slots)
         same_cache(cache, ref)
+
+
+def left_out(ref, name, rows, slots, drop):
+    """ref.append of rows of which `drop` have a slot but are not stored: they belong to their block's rows (the first
+    of which says where its older tokens end), and neither count for its scale nor change its bytes."""
+    size = ref.size
+    lost = {b for b in (int(s) // size for s in slots if s >= 0)
+            if all(drop[i] for i, s in enumerate(slots) if s >= 0 and s // size == b)}
+    slots = [-1 if s >= 0 and s // size in lost else s for s in slots]
+    rows, kept = rows.float().clone(), {}
+    for i, s in enumerate(slots):
+        if drop[i] and s >= 0:
+            rows[i] = 0
+            kept[s] = ref.x[name][s // size, :, s % size].clone()
+    ref.append(name, rows, slots)
+    for s, x in kept.items():
+        ref.x[name][s // size, :, s % size] = x
+
+
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+@pytest.mark.parametrize("kind,hd,size", [("f32", 128, 16), ("bf16", 64, 32), ("f16", 128, 256)])
+@pytest.mark.parametrize("rows", [7, 40, 1500])
+def test_rows_left_out_of_a_block(fmt, kind, hd, size, rows):
+    """Rows with a position outside the table, without a slot or with one past the pool, among rows of their block:
+    the others are stored as if alone, from a single row a CTA to windows of a block. The blocks had another owner
+    before, with larger scales, and the first has older tokens of its own."""
+    kv, heads, ctx, first = 3, 2, 2000, 5
+    rng = np.random.default_rng(rows + size)
+    blocks = -(-(first + rows) // size) + 3
+    order = rng.permutation(blocks).tolist()
+    slot = lambda p: order[p // size] * size + p % size  # noqa: E731
+    cos, sin = tables(ctx, hd)
+    cache, ref = F.KV8Cache.empty(blocks, kv, size, hd, fmt), RefCache(blocks, kv, size, hd, fmt)
+
+    def append(k, v, slots, pos):
+        q = torch.randn(len(slots), heads, hd).to(ROW_TYPES[kind]).cuda()
+        qo, turned = torch.empty_like(q), torch.empty(len(slots), kv, hd, device="cuda")
+        err = torch.zeros(1, dtype=torch.int32, device="cuda")
+        cache.append(k.cuda(), v.cuda(), i32(slots), i32(pos), cos, sin, "half", q, qo, error=err)
+        F.rope(k.cuda().float(), None, i32(pos), cos, sin, "half", turned, None)
+        mine = [s if s < blocks * size else -1 for s in slots]
+        left_out(ref, "k", turned.cpu(), mine, [not 0 <= p < ctx for p in pos])
+        ref.append("v", v, mine)
+        same_cache(cache, ref)
+        return err.item()
+
+    whole = [b * size + t for b in range(blocks) for t in range(size)]
+    k, v = (torch.randn(len(whole), kv, hd).to(ROW_TYPES[kind]) * 50 for _ in "kv")
+    append(k, v, whole, [0] * len(whole))
+    k, v = (torch.randn(first, kv, hd).to(ROW_TYPES[kind]) for _ in "kv")
+    assert append(k, v, [slot(p) for p in range(first)], list(range(first))) == 0
+    for what in ("middle", "edges", "many", "slots"):
+        k, v = (torch.randn(rows, kv, hd).to(ROW_TYPES[kind]) for _ in "kv")
+        at = np.arange(first, first + rows)
+        pos, slots = at.copy(), [slot(int(p)) for p in at]
+        if what == "middle":
+            pos[at % size == size // 2] = ctx
+        if what == "edges":
+            pos[(at % size == 0) | (at % size == size - 1) | (at == first)] = -1
+        if what == "many":
+            pos[rng.random(rows) < 0.7] = ctx + 7
+        if what == "slots":  # rows of a block stay within its size of one another
+            gone = rng.random(rows) < 0.3
+            slots = [(-1 if p % 2 else 2 ** 31 - 1) if g else s for g, p, s in zip(gone, at, slots)]
+        err = append(k, v, slots, [int(p) for p in pos])
+        assert err == (4 if any(not 0 <= p < ctx for p in pos) or any(s > blocks * size for s in slots) else 0)
