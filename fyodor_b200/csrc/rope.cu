@@ -80,7 +80,7 @@ __global__ void __launch_bounds__(ROPE_THREADS) rope_rows_kernel(RopeTable tab, 
         pos_s[s] = turns ? pos : -1;
         if (!turns) raise_error(error, ERR_BOUNDS);
         mbar_expect_tx(full + s, st.q_bytes + st.k_bytes + (turns ? 2 * st.t_bytes : 0));
-        bulk_copy_g2s(base, static_cast<const T *>(q.in) + row * q.in_stride, st.q_bytes, full + s);
+        if (q.heads) bulk_copy_g2s(base, static_cast<const T *>(q.in) + row * q.in_stride, st.q_bytes, full + s);
         if (k.heads) bulk_copy_g2s(base + st.q_bytes, static_cast<const T *>(k.in) + row * k.in_stride, st.k_bytes, full + s);
         if (turns) {
             const size_t t = (size_t)pos * (tab.dims / 2);
@@ -116,7 +116,7 @@ __global__ void __launch_bounds__(ROPE_THREADS) rope_rows_kernel(RopeTable tab, 
         if (tid == 0) {
             if (turns) {
                 const size_t row = row_of(i);
-                bulk_copy_s2g(static_cast<T *>(q.out) + row * q.out_stride, base, st.q_bytes);
+                if (q.heads) bulk_copy_s2g(static_cast<T *>(q.out) + row * q.out_stride, base, st.q_bytes);
                 if (k.heads) bulk_copy_s2g(static_cast<T *>(k.out) + row * k.out_stride, base + st.q_bytes, st.k_bytes);
             }
             bulk_commit();

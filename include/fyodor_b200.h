@@ -326,7 +326,7 @@ typedef struct fyb_rope_desc {
     uint32_t layout;
 } fyb_rope_desc;
 /* q_out / k_out = q / k [rows][heads][head_dim] rotated to positions[row] (k may be
-   NULL with kv_heads 0). An output may be its input (same stride). A row whose
+   NULL with kv_heads 0, q with heads 0, not both). An output may be its input (same stride). A row whose
    position is outside the table is not written. */
 int fyb_rope(const fyb_rope_desc *rope, const int32_t *positions, size_t rows, uint32_t head_dim, uint32_t type,
     const void *q, size_t q_stride, void *q_out, size_t q_out_stride, uint32_t heads, const void *k, size_t k_stride,

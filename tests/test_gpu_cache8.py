@@ -1,5 +1,8 @@
-"""GPU tests of the paged 8-bit KV cache beside test_gpu_kv8.py: appends whose
-tables, rows or slots are not as regular as a model's, to the byte."""
+"""GPU tests of the paged 8-bit KV cache beside test_gpu_kv8.py: operands that
+are left out, appends whose tables, rows or slots are not as regular as a
+model's, to the byte."""
+import ctypes as C
+
 import numpy as np
 import pytest
 
@@ -106,3 +109,24 @@ def test_rows_left_out_of_a_block(fmt, kind, hd, size, rows):
             slots = [(-1 if p % 2 else 2 ** 31 - 1) if g else s for g, p, s in zip(gone, at, slots)]
         err = append(k, v, slots, [int(p) for p in pos])
         assert err == (4 if any(not 0 <= p < ctx for p in pos) or any(s > blocks * size for s in slots) else 0)
+
+
+@pytest.mark.parametrize("kind,hd,dims", [("bf16", 128, 128), ("f32", 64, 32)])
+@pytest.mark.parametrize("rows", [3, 9001])
+def test_rope_of_k_alone(kind, hd, dims, rows):
+    """No q, from a few rows to enough that they go through shared memory: k as it is beside a q."""
+    kv, ctx = 8, 700
+    cos, sin = tables(ctx, dims)
+    pos = torch.randint(0, ctx, (rows,), dtype=torch.int32).cuda()
+    k = torch.randn(rows, kv, hd, device="cuda").to(ROW_TYPES[kind])
+    beside, alone, none = torch.empty_like(k), torch.full_like(k, 7.0), k[:, :0]
+    F.rope(k, k, pos, cos, sin, "half", torch.empty_like(k), beside)
+    desc = F.RopeDesc(cos.data_ptr(), sin.data_ptr(), ctx, dims, 1)
+    stream = torch.cuda.current_stream().cuda_stream
+    type_ = {"f32": 0, "bf16": 30}[kind]
+    assert F.lib.fyb_rope(C.byref(desc), pos.data_ptr(), rows, hd, type_, None, 0, None, 0, 0, k.data_ptr(), kv * hd,
+                          alone.data_ptr(), kv * hd, kv, None, stream) == 0
+    assert torch.equal(alone, beside)
+    alone.fill_(7.0)
+    F.rope(none, k, pos, cos, sin, "half", none, alone)
+    assert torch.equal(alone, beside)
