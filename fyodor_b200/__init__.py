@@ -90,6 +90,11 @@ class KV8CacheDesc(C.Structure):
                 ("head_dim", C.c_uint32), ("format", C.c_uint32)]
 
 
+class KV8Handle(C.Structure):
+    """A cache and its GPU, as the calls on torch tensors take it (csrc/tensors.cc)."""
+    _fields_ = [("cache", KV8CacheDesc), ("device", C.c_int32)]
+
+
 class RopeDesc(C.Structure):
     """fyb_rope_desc (include/fyodor_b200.h)."""
     _fields_ = [("cos_table", C.c_void_p), ("sin_table", C.c_void_p), ("table_rows", C.c_uint32),
@@ -346,9 +351,10 @@ class KV8Cache:
                 raise ValueError("%s has to be a contiguous %s tensor on the cache's GPU" % (name, kind))
         self.tensors = k, v, k_scale, v_scale
         blocks, self.kv_heads, self.block_size, self.head_dim = k.shape
-        self.desc = KV8CacheDesc(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), blocks,
-                                 self.kv_heads, self.block_size, self.head_dim, kinds[k.dtype])
-        self._handle = C.addressof(self.desc)
+        self._held = KV8Handle(KV8CacheDesc(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), blocks,
+                                            self.kv_heads, self.block_size, self.head_dim, kinds[k.dtype]),
+                               k.get_device())
+        self.desc, self._handle = self._held.cache, C.addressof(self._held)
 
     @classmethod
     def empty(cls, blocks, kv_heads, block_size, head_dim, format="int8", device="cuda"):

@@ -32,22 +32,39 @@ struct Refused {};  // a Python exception is set
     throw Refused();
 }
 
-// One call: its device, taken from the first tensor seen.
+// The cache handle: what the Python object (KV8Handle) holds the address of.
+struct CacheHandle {
+    fyb_kv8_cache cache;
+    int32_t device;
+};
+
+// One call: its device, taken from the cache or the first tensor seen.
 struct Call {
     int device = -1;
-    const at::Tensor &tensor(PyObject *o, const char *name)
+    void on(int d, const char *name)
     {
-        if (!THPVariable_Check(o)) refuse(name, "has to be a tensor");
-        const at::Tensor &t = THPVariable_Unpack(o);
-        if (!t.is_cuda()) refuse(name, "has to be on the GPU");
-        const int d = t.get_device();
         if (device < 0) {
             if (d != c10::cuda::current_device()) refuse(name, "is not on the current CUDA device");
             device = d;
         } else if (d != device) {
             refuse(name, "is on another device than the tensors before it");
         }
+    }
+    const at::Tensor &tensor(PyObject *o, const char *name)
+    {
+        if (!THPVariable_Check(o)) refuse(name, "has to be a tensor");
+        const at::Tensor &t = THPVariable_Unpack(o);
+        if (!t.is_cuda()) refuse(name, "has to be on the GPU");
+        on(t.get_device(), name);
         return t;
+    }
+    const fyb_kv8_cache *cache(PyObject *o)
+    {
+        const CacheHandle *h = static_cast<const CacheHandle *>(PyLong_AsVoidPtr(o));
+        if (PyErr_Occurred()) throw Refused();
+        if (!h) refuse("cache", "has no address");
+        on(h->device, "cache");
+        return &h->cache;
     }
     // a contiguous tensor of `kind` with `least` elements at least
     void *flat(PyObject *o, const char *name, at::ScalarType kind, int64_t least = 0)
@@ -133,15 +150,6 @@ fyb_rope_desc rope_desc(Call &c, PyObject *cos, PyObject *sin, PyObject *layout)
     else if (!strcmp(l, "half")) d.layout = FYB_ROPE_HALF;
     else refuse("layout", "is 'interleaved' or 'half'");
     return d;
-}
-
-// The cache handle: a fyb_kv8_cache at the address that the Python object holds.
-const fyb_kv8_cache *cache_of(PyObject *o)
-{
-    const fyb_kv8_cache *c = static_cast<const fyb_kv8_cache *>(PyLong_AsVoidPtr(o));
-    if (PyErr_Occurred()) throw Refused();
-    if (!c) refuse("cache", "has no address");
-    return c;
 }
 
 PyObject *answer(int r, const char *what)
@@ -234,7 +242,7 @@ PyObject *append(PyObject *, PyObject *const *a, Py_ssize_t n)
 {
     return guarded(n, 12, [&] {
         Call c;
-        const fyb_kv8_cache *cache = cache_of(a[0]);
+        const fyb_kv8_cache *cache = c.cache(a[0]);
         const Rows k = rows_of(c, a[1], "k"), v = rows_of(c, a[2], "v");
         alike(k, v, "v");
         if (k.heads != cache->kv_heads || v.heads != cache->kv_heads || k.dim != cache->head_dim)
@@ -267,7 +275,7 @@ PyObject *read(PyObject *, PyObject *const *a, Py_ssize_t n)
 {
     return guarded(n, 6, [&] {
         Call c;
-        const fyb_kv8_cache *cache = cache_of(a[0]);
+        const fyb_kv8_cache *cache = c.cache(a[0]);
         const int64_t rows = c.tensor(a[1], "slots").numel(), need = rows * cache->kv_heads * cache->head_dim;
         const int32_t *slots = c.ints(a[1], "slots");
         float *k = static_cast<float *>(c.flat(a[2], "k_out", at::kFloat, need));
@@ -281,7 +289,7 @@ PyObject *attention(PyObject *, PyObject *const *a, Py_ssize_t n)
 {
     return guarded(n, 11, [&] {
         Call c;
-        const fyb_kv8_cache *cache = cache_of(a[0]);
+        const fyb_kv8_cache *cache = c.cache(a[0]);
         const Rows q = rows_of(c, a[1], "q"), out = rows_of(c, a[4], "out");
         alike(q, out, "out");
         if (q.heads != out.heads || q.dim != cache->head_dim || q.heads > 0x7fffffff)

@@ -130,3 +130,28 @@ def test_rope_of_k_alone(kind, hd, dims, rows):
     alone.fill_(7.0)
     F.rope(none, k, pos, cos, sin, "half", none, alone)
     assert torch.equal(alone, beside)
+
+
+def test_cache_of_another_gpu_is_refused():
+    """A cache whose tensors are not on the current device, beside tensors that are: as for any tensor, nothing is
+    launched. (One GPU is enough: the cache only says that it is elsewhere.)"""
+    cache = F.KV8Cache.empty(4, 2, 16, 64)
+    k, v = torch.randn(2, 3, 2, 64, device="cuda")
+    q, lengths, table, slots = torch.randn(1, 4, 64, device="cuda"), i32([3]), i32([[0]]), i32([0, 1, 2])
+    ws = cache.attention_workspace(1, 1, 4)
+    ko, vo = torch.full((2, 3, 2, 64), 7.0, device="cuda")
+    out = torch.full_like(q, 7.0)
+    calls = [lambda: cache.append(k, v, slots), lambda: cache.read(slots, ko, vo),
+             lambda: cache.attention(q, lengths, table, out, ws)]
+    here = torch.cuda.current_device()
+    assert cache._held.device == here
+    cache._held.device = here + 1
+    for call in calls:
+        with pytest.raises(ValueError, match="cache"):
+            call()
+    assert all((t.view(torch.uint8) == 0).all() for t in cache.tensors)
+    assert (ko == 7.0).all() and (vo == 7.0).all() and (out == 7.0).all()
+    cache._held.device = here
+    for call in calls:
+        call()
+    assert (ko != 7.0).all() and (out != 7.0).all()
