@@ -1653,7 +1653,7 @@ extern "C" int fyb_batch_decode_greedy(void *batch, const uint32_t *tokens, cons
 }
 
 // Milliseconds per greedy step of `steps` graph replays (CUDA events on the
-// plan's stream), after two untimed steps from the same tokens and positions
+// plan's stream), after two untimed ones, each from the same tokens and positions
 // (the first sizes the scratch, the second captures the graph); < 0 on error.
 extern "C" double fyb_batch_time_greedy(void *batch, const uint32_t *tokens, const uint32_t *positions, size_t steps)
 {
@@ -1662,8 +1662,9 @@ extern "C" double fyb_batch_time_greedy(void *batch, const uint32_t *tokens, con
     DeviceScope scope(bt->p->ctx->device);
     cudaStream_t s = bt->p->ctx->stream;
     if (grow((void **)&bt->log, &bt->log_bytes, steps * bt->B * 4, true)) return -1.0;
-    if (batch_set(bt, tokens, positions, steps)) return -1.0;
-    for (int w = 0; w < 2; ++w) if (batch_run(bt, true)) return -1.0;  // sizes, then captures
+    // sizes, then captures: one step each from the given positions, so none goes past them
+    for (int w = 0; w < 2; ++w)
+        if (batch_set(bt, tokens, positions, steps) || batch_run(bt, true)) return -1.0;
     // the timed steps start again from the given tokens and positions
     if (batch_set(bt, tokens, positions, steps)) return -1.0;
     cudaEvent_t e0, e1;

@@ -1,0 +1,39 @@
+"""GPU tests of a plan's batched decode over the paged 8-bit cache beside
+test_gpu_kv8.py: the end of its capacity."""
+import numpy as np
+import pytest
+
+import fyodor_b200 as F
+
+pytestmark = pytest.mark.gpu
+
+CFG = dict(layers=2, embedding=512, heads=8, kv_heads=2, feed_forward=1024, vocabulary=1024, context=64,
+           matrix_type=F.Q4_K, seed=21, norm_mode=2)
+
+
+@pytest.mark.parametrize("kv", ["int8", None])
+def test_timing_ends_at_the_capacity(provider, kv):
+    """Timing a single step at the last position of the plan, or of the pool, takes no step past it: the batch goes
+    on after it. The capacity is no multiple of the block size, so the tables would hold more."""
+    m, nseq, capacity = F.SynthModel(**CFG), 3, 40
+    plan = provider.plan(m, capacity)
+    batch = F.Batch(plan, nseq, **(dict(kv=kv, blocks=3 * nseq, block_size=16) if kv else {}))
+    cur = np.arange(nseq, dtype=np.uint32)
+    batch.decode_greedy(cur, np.zeros(nseq, np.uint32), capacity - 1)
+    last = np.full(nseq, capacity - 1, np.uint32)
+    want = batch.step(cur, last)[0]
+    assert batch.time_greedy(cur, last, 1) > 0
+    assert plan.error() == 0
+    assert (batch.step(cur, last)[0] == want).all()
+    assert batch.time_greedy(cur, last, 2) < 0
+    if kv:
+        assert batch.free_blocks() == 0
+        tight = F.Batch(plan, nseq, kv=kv, blocks=nseq, block_size=16)
+        tight.decode_greedy(cur, np.zeros(nseq, np.uint32), 15)
+        assert tight.time_greedy(cur, np.full(nseq, 15, np.uint32), 1) > 0
+        assert tight.free_blocks() == 0 and plan.error() == 0
+        tight.step(cur, np.full(nseq, 15, np.uint32))
+        tight.close()
+    batch.close()
+    plan.close()
+    m.close()
