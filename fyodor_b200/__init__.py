@@ -486,7 +486,8 @@ class Provider:
 class Batch:
     """B sequences (1..16) of one plan's model decoded together (fyb_batch_*):
     each sequence has its own KV cache and position; every projection reads
-    each weight once per step for all of them. The plan must outlive it.
+    each weight once per step for all of them. A plan that is closed frees its
+    batches, which then refuse every step.
 
     kv "int8" or "e4m3": a paged 8-bit cache of `blocks` blocks of block_size
     tokens that the sequences share, instead of an fp16 cache of the plan's
@@ -495,13 +496,21 @@ class Batch:
     def __init__(self, plan, batch, kv=None, blocks=0, block_size=32):
         self.plan, self.B = plan, batch
         self.V = plan.model.vocabulary
+        self._ptr = None
         if kv is None:
-            self.ptr = lib.fyb_batch_create(C.c_void_p(plan.ptr), batch)
+            ptr = lib.fyb_batch_create(C.c_void_p(plan.ptr), batch)
         else:
-            self.ptr = lib.fyb_batch_create_kv8(C.c_void_p(plan.ptr), batch, blocks, block_size,
-                                                {"int8": KV8_INT8, "e4m3": KV8_E4M3}[kv])
-        if not self.ptr:
+            ptr = lib.fyb_batch_create_kv8(C.c_void_p(plan.ptr), batch, blocks, block_size,
+                                           {"int8": KV8_INT8, "e4m3": KV8_E4M3}[kv])
+        if not ptr:
             raise ValueError("batch of %d declined" % batch)
+        self._ptr = ptr
+        plan._batches.add(ptr)
+
+    @property
+    def ptr(self):
+        """The batch, or None once it or its plan is closed."""
+        return self._ptr if self._ptr in self.plan._batches else None
 
     def _req(self, tokens, positions):
         t = np.ascontiguousarray(tokens, np.uint32)
@@ -542,9 +551,9 @@ class Batch:
 
     def close(self):
         if self.ptr:
-            if self.plan.ptr:  # collected after its plan: the plan's context, which the batch needs to free, is gone
-                lib.fyb_batch_free(C.c_void_p(self.ptr))
-            self.ptr = None
+            self.plan._batches.remove(self._ptr)
+            lib.fyb_batch_free(C.c_void_p(self._ptr))
+        self._ptr = None
 
     def __del__(self):
         self.close()
@@ -557,6 +566,7 @@ class Plan:
         self.provider, self.ptr, self.model = provider, ptr, model
         self.api = provider.api
         self.logits = np.empty(model.vocabulary, np.float32)
+        self._batches = set()  # alive; freed with the plan, in whatever order Python collects the two
 
     def token(self, token, position, logits=True):
         out = self.logits if logits else None
@@ -670,6 +680,8 @@ class Plan:
 
     def close(self):
         if self.ptr:
+            while self._batches:
+                lib.fyb_batch_free(C.c_void_p(self._batches.pop()))
             self.api.plan_free(self.ptr)
             self.ptr = None
 

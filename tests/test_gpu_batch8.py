@@ -1,11 +1,13 @@
 """GPU tests of a plan's batched decode over the paged 8-bit cache beside
-test_gpu_kv8.py: the end of its capacity."""
+test_gpu_kv8.py: the ends of its capacity and of its life."""
 import numpy as np
 import pytest
 
 import fyodor_b200 as F
 
 pytestmark = pytest.mark.gpu
+
+import torch  # noqa: E402
 
 CFG = dict(layers=2, embedding=512, heads=8, kv_heads=2, feed_forward=1024, vocabulary=1024, context=64,
            matrix_type=F.Q4_K, seed=21, norm_mode=2)
@@ -36,4 +38,24 @@ def test_timing_ends_at_the_capacity(provider, kv):
         tight.close()
     batch.close()
     plan.close()
+    m.close()
+
+
+def test_batches_end_with_their_plan(provider):
+    """A plan that is closed closes its batches: their memory comes back, and they refuse further steps."""
+    m = F.SynthModel(**CFG)
+    plan = provider.plan(m, CFG["context"])
+    zero = np.zeros(2, np.uint32)
+    free = torch.cuda.mem_get_info()[0]
+    paged, plain = F.Batch(plan, 2, kv="int8", blocks=1 << 18, block_size=16), F.Batch(plan, 2)
+    held = free - torch.cuda.mem_get_info()[0]
+    assert held >= 2 * 2 * (1 << 18) * 16 * 2 * 64  # layers, K and V, blocks, tokens, KV heads, dimensions
+    paged.step(zero, zero)
+    plan.close()
+    assert torch.cuda.mem_get_info()[0] - free > -(64 << 20)
+    for batch in (paged, plain):
+        assert not batch.ptr
+        with pytest.raises(RuntimeError):
+            batch.step(zero, zero)
+        batch.close()
     m.close()
