@@ -255,6 +255,7 @@ class SynthModel:
 # given. Nothing synchronizes. A refused argument raises ValueError and leaves
 # every output as it was.
 KV8_INT8, KV8_E4M3 = 0, 1
+KV8_FORMATS = {"int8": KV8_INT8, "e4m3": KV8_E4M3}
 ROPE_KINDS = {"plain": 0, "linear": 1, "ntk": 2, "yarn": 3, "bands": 4}
 _native = None
 
@@ -269,6 +270,12 @@ def _bind_tensors():
                                                          lib.fyb_kv8_append, lib.fyb_kv8_read, lib.fyb_kv8_attention)))
         _native = ext
     return _native
+
+
+def _format(name):
+    if name not in KV8_FORMATS:
+        raise ValueError("the format of an 8-bit cache is one of %s" % sorted(KV8_FORMATS))
+    return KV8_FORMATS[name]
 
 
 def _check(r, what):
@@ -360,7 +367,7 @@ class KV8Cache:
     def empty(cls, blocks, kv_heads, block_size, head_dim, format="int8", device="cuda"):
         """A cache of its own tensors."""
         import torch
-        kind = {"int8": torch.int8, "e4m3": torch.float8_e4m3fn}[format]
+        kind = (torch.int8, torch.float8_e4m3fn)[_format(format)]
         k, v = (torch.zeros((blocks, kv_heads, block_size, head_dim), dtype=torch.int8, device=device).view(kind)
                 for _ in range(2))
         return cls(k, v, *(torch.zeros((blocks, kv_heads), device=device) for _ in range(2)))
@@ -500,8 +507,7 @@ class Batch:
         if kv is None:
             ptr = lib.fyb_batch_create(C.c_void_p(plan.ptr), batch)
         else:
-            ptr = lib.fyb_batch_create_kv8(C.c_void_p(plan.ptr), batch, blocks, block_size,
-                                           {"int8": KV8_INT8, "e4m3": KV8_E4M3}[kv])
+            ptr = lib.fyb_batch_create_kv8(C.c_void_p(plan.ptr), batch, blocks, block_size, _format(kv))
         if not ptr:
             raise ValueError("batch of %d declined" % batch)
         self._ptr = ptr

@@ -1,5 +1,5 @@
 """GPU tests of a plan's batched decode over the paged 8-bit cache beside
-test_gpu_kv8.py: the ends of its capacity and of its life."""
+test_gpu_kv8.py: the ends of its capacity and of its life, what it refuses."""
 import numpy as np
 import pytest
 
@@ -58,4 +58,15 @@ def test_batches_end_with_their_plan(provider):
         with pytest.raises(RuntimeError):
             batch.step(zero, zero)
         batch.close()
+    m.close()
+
+
+def test_unknown_format_is_refused(provider):
+    m = F.SynthModel(**CFG)
+    plan = provider.plan(m, 64)
+    with pytest.raises(ValueError):
+        F.Batch(plan, 2, kv="int4", blocks=8)
+    with pytest.raises(ValueError):
+        F.KV8Cache.empty(4, 2, 16, 64, "int4")
+    plan.close()
     m.close()

@@ -1,5 +1,5 @@
 """The paged 8-bit KV cache on the host side, beside test_kv8.py: where rotary
-frequencies leave the usual contexts, and calls that have nothing to do."""
+frequencies leave the usual contexts, and what is refused before a GPU is asked."""
 import numpy as np
 import pytest
 
@@ -21,3 +21,8 @@ def test_frequencies_yarn_past_the_last_pair(dims, base, factor, ctx):
     ramp = np.clip((j - lo) / (hi - lo), 0, 1)
     want = f * (1 - ramp) + f / factor * ramp
     assert np.all(np.abs(got - want) <= 2.0 ** -24 * want * (1 + 1e-6))
+
+
+def test_unknown_format_is_a_value_error():
+    with pytest.raises(ValueError, match="e4m3"):
+        F.KV8Cache.empty(4, 2, 16, 64, "int4", device="cpu")
