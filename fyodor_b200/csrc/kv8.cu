@@ -384,11 +384,11 @@ extern "C" int fyb_kv8_append(const fyb_kv8_cache *cache, const int32_t *slots, 
     const unsigned hd = cache->head_dim, kv = cache->kv_heads;
     const size_t width = type == T_F32 ? 4 : 2;
     Kv8Append A{};
-    if (!k || !v || k_stride < (size_t)kv * hd || v_stride < (size_t)kv * hd || (heads && !rope) || heads > 65536)
+    if ((rows && (!k || !v)) || k_stride < (size_t)kv * hd || v_stride < (size_t)kv * hd || (heads && !rope) || heads > 65536)
         return -1;
     if (rope && (rope_table_of(rope, &A.rope) || A.rope.dims > hd || (A.rope.layout != 0 && A.rope.dims % 8)))
         return -1;
-    if (heads && (!q || !q_out || q_stride < (size_t)heads * hd || q_out_stride < (size_t)heads * hd ||
+    if (heads && ((rows && (!q || !q_out)) || q_stride < (size_t)heads * hd || q_out_stride < (size_t)heads * hd ||
                   (q == q_out && q_stride != q_out_stride)))
         return -1;
     if (!rows) return 0;
@@ -435,7 +435,7 @@ extern "C" int fyb_kv8_append(const fyb_kv8_cache *cache, const int32_t *slots, 
 extern "C" int fyb_kv8_read(const fyb_kv8_cache *cache, const int32_t *slots, size_t rows, float *k, float *v,
     uint32_t *error, void *stream)
 {
-    if (kv8_check(cache) || !k || !v || ((uintptr_t)k | (uintptr_t)v) % 16 || rows > 0x7fffffffu) return -1;
+    if (kv8_check(cache) || (rows && (!k || !v)) || ((uintptr_t)k | (uintptr_t)v) % 16 || rows > 0x7fffffffu) return -1;
     if (!rows) return 0;
     if (!slots) return -1;
     const unsigned words = cache->kv_heads * (cache->head_dim / 4);

@@ -70,7 +70,7 @@ extern "C" int fyb_kv8_attention(const fyb_kv8_cache *cache, const int32_t *leng
         return -1;
     const size_t need = fyb_kv8_attention_workspace(requests, max_rows, heads, cache->kv_heads, cache->head_dim);
     const size_t row = (size_t)heads * cache->head_dim;
-    if (!need || !lengths || !table || !q || !out || q_stride < row || out_stride < row || !workspace ||
+    if (!need || !lengths || !table || (rows && (!q || !out)) || q_stride < row || out_stride < row || !workspace ||
         (uintptr_t)workspace % 16 || workspace_bytes < need || (!row_start && rows != requests))
         return -1;
     if (!rows) return 0;

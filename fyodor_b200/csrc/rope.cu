@@ -283,7 +283,7 @@ extern "C" int fyb_rope(const fyb_rope_desc *rope, const int32_t *positions, siz
 {
     RopeTable t;
     if (rope_table_of(rope, &t) || hd < t.dims || hd % 2 || hd > 65536 || heads > 65536 || kv_heads > 65536 ||
-        rows > 0x7fffffffu || heads + kv_heads == 0 || (heads && (!q || !q_out)) || (kv_heads && (!k || !k_out)) ||
+        rows > 0x7fffffffu || heads + kv_heads == 0 || (rows && heads && (!q || !q_out)) || (rows && kv_heads && (!k || !k_out)) ||
         q_stride < (size_t)heads * hd || q_out_stride < (size_t)heads * hd || k_stride < (size_t)kv_heads * hd ||
         k_out_stride < (size_t)kv_heads * hd || (heads && q == q_out && q_stride != q_out_stride) ||
         (kv_heads && k == k_out && k_stride != k_out_stride))

@@ -248,7 +248,8 @@ unsigned long long fyb_batch_launches_per_step(const void *batch);
    device, so a CUDA graph of the step serves every later step.
 
    q, k, v rows are `type` F32, F16 or BF16 (GGML ids 0, 1, 30), strides in
-   elements; a row's heads are contiguous. Every pointer below is a device
+   elements; a row's heads are contiguous. A call of no rows does nothing and may
+   pass NULL for the rows. Every pointer below is a device
    pointer unless a line says otherwise; `error` (may be NULL) is a device
    word that receives 4 when an index read on the device is out of range (the
    row or position concerned is then left out) and 2 for non-finite values

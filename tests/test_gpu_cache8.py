@@ -155,3 +155,20 @@ def test_cache_of_another_gpu_is_refused():
     for call in calls:
         call()
     assert (ko != 7.0).all() and (out != 7.0).all()
+
+
+def test_no_rows():
+    """Steps without a row, as torch makes them (empty tensors have no address): nothing is done and nothing refused."""
+    cache, empty = F.KV8Cache.empty(4, 2, 16, 64), i32([])
+    before = [t.clone() for t in cache.tensors]
+    k, q = torch.empty(0, 2, 64, device="cuda"), torch.empty(0, 4, 64, device="cuda")
+    cos, sin = tables(8, 64)
+    F.rope(q, k, empty, cos, sin, "half", q, k)
+    F.rope(q, None, empty, cos, sin, "interleaved", torch.empty_like(q), None)
+    cache.append(k, k, empty)
+    cache.append(k, k, empty, empty, cos, sin, "half", q, q)
+    cache.read(empty, k, k)
+    cache.attention(q, i32([3, 7]), i32([[0], [1]]), q, cache.attention_workspace(2, 4, 4), row_start=i32([0, 0, 0]),
+                    most_rows=4)
+    torch.cuda.synchronize()
+    assert all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in zip(cache.tensors, before))
