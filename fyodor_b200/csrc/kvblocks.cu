@@ -57,7 +57,7 @@ __global__ void __launch_bounds__(KB_THREADS) kv_blocks_kernel(KvBlocksArgs A)
     const unsigned size = 1u << A.shift, tid = threadIdx.x, n = A.n;
     const unsigned count = (unsigned)max(A.free_count[0], 0);
     const unsigned row_limit = A.max_rows + 1, blk_limit = count + 1;
-    const long long holds = (long long)A.stride << A.shift;
+    const long long holds = min((long long)A.stride << A.shift, 0x7fffffffll);  // lengths and positions are 31 bits
     auto valid = [&](int len, int more) { return len >= 0 && more >= 0 && (long long)len + more <= holds; };
     auto blocks = [&](int tokens) { return (unsigned)(((long long)tokens + size - 1) >> A.shift); };
 

@@ -272,8 +272,8 @@ typedef struct fyb_kv8_cache {
    the j-th block of the step is free_list[free_count[0] - 1 - j], written to
    the table. Requests are served whole or not at all: status[r] 0 served, 1
    too few free blocks (all later requests that need one are refused too), 2
-   invalid (negative counts, more tokens than the table holds, rows beyond
-   max_rows). Outputs: lengths_out[r] (lengths + new when served),
+   invalid (negative counts, more tokens than the table holds or than 2^31 - 1,
+   rows beyond max_rows). Outputs: lengths_out[r] (lengths + new when served),
    free_count_out[0], row_start [requests + 1] (the step's rows, request after
    request, clamped to max_rows) and, per row 0..max_rows, slots (block *
    block_size + offset; -1 for rows of refused requests and rows beyond the

@@ -1,5 +1,5 @@
-"""GPU tests of the paged 8-bit KV cache beside test_gpu_kv8.py: operands that
-are left out, appends whose tables, rows or slots are not as regular as a
+"""GPU tests of the paged 8-bit KV cache beside test_gpu_kv8.py: lengths
+at their end, operands that are left out, appends whose tables, rows or slots are not as regular as a
 model's, to the byte."""
 import ctypes as C
 
@@ -172,3 +172,19 @@ def test_no_rows():
                     most_rows=4)
     torch.cuda.synchronize()
     assert all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in zip(cache.tensors, before))
+
+
+def test_more_tokens_than_31_bits():
+    """A table wide enough for more than 2^31 tokens: a request that would pass 2^31 - 1 is invalid by itself, and the
+    requests after it get their blocks."""
+    block, width = 1 << 19, 4097
+    lengths, new = i32([5, 2 ** 31 - 1, 2 ** 31 - 2, 0]), i32([1, 1, 1, 3])
+    table = torch.arange(4 * width, dtype=torch.int32, device="cuda").reshape(4, width) % 4000
+    free, count = i32(range(100, 110)), i32([10])
+    out, left, start, status = (torch.full((m,), 77, dtype=torch.int32, device="cuda") for m in (4, 1, 5, 4))
+    slots, pos, who = (torch.full((8,), 77, dtype=torch.int32, device="cuda") for _ in range(3))
+    F.kv_blocks(lengths, new, table, free, count, block, out, left, start, slots, pos, who, status)
+    assert status.tolist() == [0, 2, 0, 0] and left.item() == 9
+    assert out.tolist() == [6, 2 ** 31 - 1, 2 ** 31 - 1, 3] and start.tolist() == [0, 1, 1, 2, 5]
+    assert table[3, 0].item() == 109 and slots[2:5].tolist() == [109 * block + i for i in range(3)]
+    assert pos.tolist() == [5, 2 ** 31 - 2, 0, 1, 2, 0, 0, 0] and who.tolist() == [0, 2, 3, 3, 3, -1, -1, -1]
