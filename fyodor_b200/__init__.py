@@ -500,10 +500,11 @@ class Batch:
     tokens that the sequences share, instead of an fp16 cache of the plan's
     capacity each (fyb_batch_create_kv8)."""
 
+    _ptr = None  # until it is made, and where it is declined
+
     def __init__(self, plan, batch, kv=None, blocks=0, block_size=32):
         self.plan, self.B = plan, batch
         self.V = plan.model.vocabulary
-        self._ptr = None
         if kv is None:
             ptr = lib.fyb_batch_create(C.c_void_p(plan.ptr), batch)
         else:
@@ -516,7 +517,7 @@ class Batch:
     @property
     def ptr(self):
         """The batch, or None once it or its plan is closed."""
-        return self._ptr if self._ptr in self.plan._batches else None
+        return self._ptr if self._ptr and self._ptr in self.plan._batches else None
 
     def _req(self, tokens, positions):
         t = np.ascontiguousarray(tokens, np.uint32)

@@ -1258,8 +1258,8 @@ static void batch_free(Batch *bt)
     DeviceScope scope(bt->p->ctx->device);
     cudaStreamSynchronize(bt->p->ctx->stream);
     for (auto &g : bt->graphs) if (g) cudaGraphExecDestroy(g);
-    for (void *a : bt->allocations) cudaFree(a);  // the attention workspace among them
-    for (void *a : {(void *)bt->log, (void *)bt->counters, (void *)bt->partials, (void *)bt->gemm})  // grown buffers
+    for (void *a : bt->allocations) cudaFree(a);  // the attention workspace and the log among them
+    for (void *a : {(void *)bt->counters, (void *)bt->partials, (void *)bt->gemm})  // grown buffers
         if (a) cudaFree(a);
     cudaGetLastError();
     delete bt;
@@ -1499,6 +1499,8 @@ static Batch *batch_create(Plan *p, unsigned batch, bool chunk, const fyb_kv8_ca
     bt->h = (float *)A((size_t)batch * p->ffn * 4);
     bt->logits = (float *)A((size_t)batch * p->V * 4);
     bt->req = (unsigned *)A((3 * BATCH_MAX + 1) * 4); bt->tokens = (unsigned *)A(BATCH_MAX * 4);
+    // tokens of as many greedy steps as the capacity allows: the captured step holds its address
+    bt->log = (unsigned *)A((size_t)batch * (chunk ? 1 : bt->capacity) * 4);
     // partitions of each (sequence, KV head): about four waves of the SMs, 4..16
     const size_t seqs = chunk ? 1 : batch;
     bt->splits = (unsigned)std::max<size_t>(4, std::min<size_t>(16, ((size_t)4 * p->ctx->sms + seqs * p->Hkv - 1) /
@@ -1511,7 +1513,6 @@ static Batch *batch_create(Plan *p, unsigned batch, bool chunk, const fyb_kv8_ca
     if (ok) ok = (chunk || paged || (cudaMemset(bt->kc, 0, kv * 2) == cudaSuccess && cudaMemset(bt->vc, 0, kv * 2) == cudaSuccess)) &&
                  cudaMemset(bt->attn_ws, 0, bt->attn_ws_bytes) == cudaSuccess &&
                  cudaMemset(bt->req, 0, (3 * BATCH_MAX + 1) * 4) == cudaSuccess &&
-                 grow((void **)&bt->log, &bt->log_bytes, (size_t)BATCH_MAX * 4, true) == 0 &&
                  cudaDeviceSynchronize() == cudaSuccess;
     if (!ok) {
         batch_free(bt);
@@ -1642,7 +1643,6 @@ extern "C" int fyb_batch_decode_greedy(void *batch, const uint32_t *tokens, cons
     DeviceScope scope(bt->p->ctx->device);
     if (!scope.ok) return -1;
     cudaStream_t s = bt->p->ctx->stream;
-    if (grow((void **)&bt->log, &bt->log_bytes, steps * bt->B * 4, true)) return -2;
     int r = batch_set(bt, tokens, positions, steps);
     for (size_t i = 0; i < steps && !r; ++i) r = batch_run(bt, true);
     if (r) return r;
@@ -1661,7 +1661,6 @@ extern "C" double fyb_batch_time_greedy(void *batch, const uint32_t *tokens, con
     if (!bt || !tokens || !positions || steps == 0) return -1.0;
     DeviceScope scope(bt->p->ctx->device);
     cudaStream_t s = bt->p->ctx->stream;
-    if (grow((void **)&bt->log, &bt->log_bytes, steps * bt->B * 4, true)) return -1.0;
     // sizes, then captures: one step each from the given positions, so none goes past them
     for (int w = 0; w < 2; ++w)
         if (batch_set(bt, tokens, positions, steps) || batch_run(bt, true)) return -1.0;

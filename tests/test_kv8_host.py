@@ -55,3 +55,9 @@ def test_no_rows_need_no_rows():
                                        None, None)
     assert attention() == 0
     assert attention(lengths=None) == attention(starts=None) == -1
+
+
+def test_a_batch_that_was_never_made_closes():
+    batch = F.Batch.__new__(F.Batch)
+    assert batch.ptr is None
+    batch.close()
