@@ -276,17 +276,18 @@ __global__ void __launch_bounds__(KD_THREADS, 3) kv8_decode_kernel(const __grid_
                         if (base + (int)posB >= limit[w]) x[1][w] = -INFINITY;
                     }
                 }
-                // ---- running maximum: moved only when a score is 2^8 above it
+                // ---- running maximum: moved only when a score is 2^8 above it. Their difference says so: it is exact
+                // where they are near, and m + 8 is not (from 2^27 on it can round to m + 16, a weight of 2^16)
                 bool over = false;
 #pragma unroll
-                for (int w = 0; w < W; ++w) over = over || fmaxf(x[0][w], x[1][w]) > m[w] + 8.f;
+                for (int w = 0; w < W; ++w) over = over || fmaxf(x[0][w], x[1][w]) - m[w] > 8.f;
                 if (__any_sync(0xffffffffu, over)) {
 #pragma unroll
                     for (int w = 0; w < W; ++w) {
                         float top = fmaxf(x[0][w], x[1][w]);
 #pragma unroll
                         for (int o = 4; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-                        if (top > m[w] + 8.f) {  // each row by its own scores: the same on all lanes that hold it
+                        if (top - m[w] > 8.f) {  // each row by its own scores: the same on all lanes that hold it
                             const float alpha = ex2(m[w] - top);
                             m[w] = top;
                             l[w] *= alpha;

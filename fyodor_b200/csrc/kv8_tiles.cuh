@@ -394,7 +394,7 @@ __global__ void __launch_bounds__(kt_threads(N), 1) kv8_tiles_kernel(const __gri
                     if (pos < 16) {
                         const unsigned c = col + pos;
                         const float old = sh.m[c], top = fmaxf(fmaxf(sh.top[0][c], sh.top[1][c]), fmaxf(sh.top[2][c], sh.top[3][c]));
-                        const bool up = top > old + 8.f;  // each row by its own scores
+                        const bool up = top - old > 8.f;  // each row by its own scores; old + 8 could round up
                         sh.alpha[c] = up ? ex2(old - top) : 1.f;
                         if (up) sh.m[c] = top;
                     }

@@ -188,3 +188,34 @@ def test_more_tokens_than_31_bits():
     assert out.tolist() == [6, 2 ** 31 - 1, 2 ** 31 - 1, 3] and start.tolist() == [0, 1, 1, 2, 5]
     assert table[3, 0].item() == 109 and slots[2:5].tolist() == [109 * block + i for i in range(3)]
     assert pos.tolist() == [5, 2 ** 31 - 2, 0, 1, 2, 0, 0, 0] and who.tolist() == [0, 2, 3, 3, 3, -1, -1, -1]
+
+
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+@pytest.mark.parametrize("group,new,hd", [(4, 1, 128), (8, 1, 64), (4, 5, 128), (1, 40, 64)])
+@pytest.mark.parametrize("rising", [False, True])
+def test_scores_beyond_their_resolution(fmt, group, new, hd, rising):
+    """Scores of 2^26 to 2^30, where neighbouring F32 numbers are 8 to 64 apart: which weight a token gets is down to
+    rounding, but every row is still a mean of its values (all of them 1 to 2 here)."""
+    n, kv, size, length, top = 24, 2, 32, 300, {"int8": 127.0, "e4m3": 448.0}[fmt]
+    g = torch.Generator(device="cuda").manual_seed(group + new)
+    blocks = n * -(-length // size)
+    k = torch.zeros(blocks, kv, size, hd, device="cuda")
+    k[..., 0] = 96
+    k[..., 1] = torch.randint(0, 8, k.shape[:3], generator=g, device="cuda").float()
+    if rising:  # the largest scores of a request in its later tiles
+        k[..., 1] = 2 * (torch.arange(blocks, device="cuda") % -(-length // size) // 4)[:, None, None] + k[..., 1] // 4
+    v = torch.randint(64, 97, k.shape, generator=g, device="cuda").float()
+    kind = torch.int8 if fmt == "int8" else torch.float8_e4m3fn
+    one = torch.ones(blocks, kv, device="cuda")
+    cache = F.KV8Cache(k.to(kind), v.to(kind), one, one / 64)
+    table = torch.arange(blocks, dtype=torch.int32, device="cuda").reshape(n, -1)
+    q = torch.zeros(n * new, kv * group, hd, device="cuda")
+    q[..., 0] = 2.0 ** (26 + 4 * torch.rand(q.shape[:2], generator=g, device="cuda")) / 96
+    q[..., 1] = 2.0 ** torch.randint(1, 5, q.shape[:2], generator=g, device="cuda")
+    out, ws = torch.empty_like(q), cache.attention_workspace(n, new, kv * group)
+    for sign in (1, -1):
+        cache.attention(sign * q, i32([length] * n), table, out, ws, row_start=i32(range(0, n * new + 1, new)),
+                        most_rows=new, scale=0.6931472)
+        assert out.isfinite().all(), int((~out.isfinite()).any(2).sum())
+        # a mean to 22 bits a weight, as far as sums of 300 weights in F32 go
+        assert (out >= 1 - 300 * 2.0 ** -22).all() and (out <= 1.5 + 300 * 2.0 ** -22).all()
