@@ -1227,7 +1227,6 @@ struct Batch {
     unsigned *req = nullptr;             // [B] tokens | [B] positions | [B] lengths | step
     unsigned *tokens = nullptr;          // [B] argmax of the last step
     unsigned *log = nullptr;             // [steps][B] greedy tokens
-    size_t log_bytes = 0;
     void *attn_ws = nullptr;
     size_t attn_ws_bytes = 0;
     unsigned splits = 1;

@@ -1,5 +1,6 @@
 """GPU tests of a plan's batched decode over the paged 8-bit cache beside
-test_gpu_kv8.py: the ends of its capacity and of its life, what it refuses."""
+test_gpu_kv8.py: runs of several lengths, the ends of its
+capacity and of its life, what it refuses."""
 import numpy as np
 import pytest
 
@@ -37,6 +38,27 @@ def test_timing_ends_at_the_capacity(provider, kv):
         tight.step(cur, np.full(nseq, 15, np.uint32))
         tight.close()
     batch.close()
+    plan.close()
+    m.close()
+
+
+@pytest.mark.parametrize("kv", ["int8", None])
+def test_longer_runs_after_shorter_ones(provider, kv):
+    """Greedy runs of growing length replay one captured step: each run's tokens are those of single steps."""
+    m, nseq = F.SynthModel(**CFG), 3
+    plan = provider.plan(m, CFG["context"])
+    batch, other = (F.Batch(plan, nseq, **(dict(kv=kv, blocks=4 * nseq, block_size=16) if kv else {})) for _ in range(2))
+    cur, at = np.arange(nseq, dtype=np.uint32), 0
+    for steps in (1, 2, 5, 40):
+        got = batch.decode_greedy(cur, np.full(nseq, at, np.uint32), steps)
+        for i in range(steps):
+            _, cur = other.step(cur, np.full(nseq, at + i, np.uint32), logits=False)
+            assert (got[i] == cur).all(), (steps, i)
+        at += steps
+    with pytest.raises(RuntimeError):
+        batch.decode_greedy(cur, np.full(nseq, at, np.uint32), CFG["context"])
+    batch.close()
+    other.close()
     plan.close()
     m.close()
 
