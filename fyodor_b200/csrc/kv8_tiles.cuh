@@ -174,6 +174,7 @@ template <int N> struct KtShared {
     uint64_t seg_full[KT_SEGS], seg_empty[KT_SEGS];
     float ks[KT_META][KT_TILE / 16], vs[KT_META][KT_TILE / 16];  // scales by 16 positions; ks NaN: not loaded
     int exponent[KT_META], hole[KT_META];                         // 2^exponent is above every value scale of the tile; whether some were not loaded
+    unsigned char lower[KT_META][N];                              // what a tile lowers its rows' maxima by
     alignas(16) float m[N];
     float own[N], alpha[N], top[4][N], sum[4][N];
     int limit[N];                                                 // positions a row attends
@@ -395,8 +396,11 @@ __global__ void __launch_bounds__(kt_threads(N), 1) kv8_tiles_kernel(const __gri
                         const unsigned c = col + pos;
                         const float old = sh.m[c], top = fmaxf(fmaxf(sh.top[0][c], sh.top[1][c]), fmaxf(sh.top[2][c], sh.top[3][c]));
                         const bool up = top - old > 8.f;  // each row by its own scores; old + 8 could round up
-                        sh.alpha[c] = up ? ex2(old - top) : 1.f;
-                        if (up) sh.m[c] = top;
+                        // volatile: its address, formed ahead, is a register too many in the loop (48 bytes spilled,
+                        // chunk 370 to 391 us)
+                        const float now = (up ? top : old) - (float)*((volatile unsigned char *)&sh.lower[0][0] + (n % KT_META) * N + c);
+                        sh.alpha[c] = now != old ? ex2(old - now) : 1.f;
+                        sh.m[c] = now;
                     }
                     if (t > t0) wait(sh.o_done + (b ^ 1), (n - 1) >> 1);
                     if (pending) {
@@ -624,6 +628,7 @@ __global__ void __launch_bounds__(kt_threads(N), 1) kv8_tiles_kernel(const __gri
             const int *ids = A.table + (size_t)s.request * A.table_stride;
             int have = -1, id = 0;  // lane holds block 32 * have + lane
             float ks = 0.f, vs = 0.f;
+            int seen = -200;        // largest exponent so far
             for (int t = s.t0; t < s.t1; ++t, ++n) {
                 const int b0 = t * KT_TILE >> A.shift;
                 if (b0 / 32 != have) {
@@ -646,7 +651,27 @@ __global__ void __launch_bounds__(kt_threads(N), 1) kv8_tiles_kernel(const __gri
                 const int row = (int)((((unsigned)mine * kv + s.head) << A.shift) + ((unsigned)(t * KT_TILE + (int)(lane % per * box)) & (size - 1)));
                 if (n >= S::STAGES) wait(sh.k8_empty + b, n / S::STAGES - 1);
                 const bool hole = __any_sync(0xffffffffu, isnan(gk));
-                const int top = __reduce_max_sync(0xffffffffu, gv > 0.f ? max(kt_exponent(gv) + 1, -100) : -200);
+                const int ex = gv > 0.f ? max(kt_exponent(gv) + 1, -100) : -200, top = __reduce_max_sync(0xffffffffu, ex);
+                // The tile's weights are relative to its largest value scale: a row that ends before the positions that
+                // have it gets its maximum lowered by as much, or its weights would lose bits to tokens after it (scales
+                // 2^15 apart, heads of one row each: 8e-5 of the row's largest value)
+                int low[N / 32] = {};
+                if (__builtin_expect(top > seen, 0)) {
+#pragma unroll
+                    for (int i = 0; i < N / 32; ++i) {
+                        const int ends = s.q.len - s.q.n + s.row_tile * (int)A.row_tile + (int)((lane + 32 * i) / G) + 1 - t * KT_TILE;
+                        int mine_ex = seen;
+#pragma unroll 1
+                        for (int g = 0; g < KT_TILE / 16; ++g) {
+                            const int eg = __shfl_sync(0xffffffffu, ex, g);
+                            if (16 * g < ends) mine_ex = max(mine_ex, eg);
+                        }
+                        low[i] = ends > 0 ? min(top - mine_ex, 64) : 0;
+                    }
+                    seen = top;
+                }
+#pragma unroll
+                for (int i = 0; i < N / 32; ++i) sh.lower[slot][lane + 32 * i] = (unsigned char)low[i];
                 if (lane < KT_TILE / 16) { sh.ks[slot][lane] = gk; sh.vs[slot][lane] = gv; sh.exponent[slot] = top; sh.hole[slot] = hole; }
                 __syncwarp();
                 if (lane == 0) {

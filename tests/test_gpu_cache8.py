@@ -12,7 +12,7 @@ pytestmark = pytest.mark.gpu
 
 import torch  # noqa: E402
 
-from .test_gpu_kv8 import ROW_TYPES, RefCache, i32, same_cache, tables  # noqa: E402
+from .test_gpu_kv8 import ROW_TYPES, RefCache, i32, run_attention, same_cache, tables  # noqa: E402
 
 
 def shifted(t, by):
@@ -219,3 +219,18 @@ def test_scores_beyond_their_resolution(fmt, group, new, hd, rising):
         assert out.isfinite().all(), int((~out.isfinite()).any(2).sum())
         # a mean to 22 bits a weight, as far as sums of 300 weights in F32 go
         assert (out >= 1 - 300 * 2.0 ** -22).all() and (out <= 1.5 + 300 * 2.0 ** -22).all()
+
+
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+@pytest.mark.parametrize("heads,kv,hd,size", [(2, 2, 128, 16), (2, 2, 64, 32), (8, 2, 128, 16), (6, 2, 64, 16)])
+@pytest.mark.parametrize("lengths,new", [([60], [60]), ([200, 131, 40], [60, 64, 33]), ([700, 9], [300, 9]), ([90], [8])])
+def test_values_that_grow(fmt, heads, kv, hd, size, lengths, new):
+    """Value scales that grow from block to block by a factor of a hundred: a token's result is as near as its own
+    values allow, whatever the tokens after it bring (the bound is test_gpu_kv8's, by the values a row attends)."""
+    def grow(cache, table):
+        vs = cache.tensors[3]
+        for row in table:
+            for i, b in enumerate(row):
+                if b >= 0:
+                    vs[int(b)] *= 100.0 ** (i % 7)
+    run_attention(lengths, new, heads, kv, hd, size, fmt, "f32", seed=sum(new), change=grow)
