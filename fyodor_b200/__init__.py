@@ -376,7 +376,7 @@ class KV8Cache:
                error=None, stream=None):
         """Store K and V rows [rows][kv_heads][head_dim] at slots[row]
         (fyb_kv8_append). With cos / sin K is rotated to positions[row] first,
-        and q to q_out in the same launch."""
+        and q to q_out in the same call."""
         (_native or _bind_tensors()).append(self._handle, k, v, slots, positions, cos, sin, layout, q, q_out, error, stream)
 
     def read(self, slots, k_out, v_out, error=None, stream=None):

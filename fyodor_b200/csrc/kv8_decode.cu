@@ -12,8 +12,8 @@
 // Bound by HBM: 2 head_dim bytes per position and KV head, read once for all
 // rows. A position's 256 bytes (head_dim 128) pass an SM in 11.6 cycles at the
 // measured copy rate, 46 warp instructions; the loop below issues about 15.
-// Ragged batch of 32 (128 to 32768 positions, 32/8 heads, 1.05 GB): 171 us, 6.1
-// TB/s, 0.95 of a measured copy; 16 requests of 8100 with eight rows: 62 us, 4.3
+// Ragged batch of 32 (128 to 32768 positions, 32/8 heads, 1.05 GB): 173 us, 6.1
+// TB/s, 0.94 of a measured copy; 16 requests of 8100 with eight rows: 60 us, 4.4
 // TB/s, where the two passes of the low halves and the joins show.
 // A producer warp keeps the TMA ring full across segments while four warps take
 // 16 positions of every 64-position tile each.

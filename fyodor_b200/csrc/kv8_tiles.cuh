@@ -5,7 +5,7 @@
 // Per tile of 128 positions, N = 32 or 64 query rows of one KV head:
 //
 //   D1[position][row] = K Q^T       tcgen05.mma kind::f16, M = 128, K = head_dim
-//   P = 2^(D1 scale - m) v_scale    one thread per position and half the rows
+//   P = 2^(D1 scale - m) v_scale    one thread per position and 16 rows
 //   D2[hd][row] += V^T P^T          M = 128, K = 128 positions
 //
 // K and V come as 8-bit tiles by TMA; four warps convert them to fp16 (exact) on
@@ -25,8 +25,8 @@
 // Bound by the softmax warps' latency on one tile: taking out exponentials, low
 // halves, flushes, conversions or MMAs one at a time changes less than 5 %. At
 // N = 64 the row tiles of a long chunk also read K and V from L2 once each.
-// Ragged drafts of 8 (32 requests of 128 to 32768, 32/8 heads, 0.97 GB): 274 us,
-// 0.55 of a measured copy; a chunk of 500 rows at 16001: 355 us.
+// Ragged drafts of 8 (32 requests of 128 to 32768, 32/8 heads, 0.97 GB): 280 us,
+// 0.54 of a measured copy; a chunk of 500 rows at 16001: 354 us.
 //
 // Roles: N / 4 warps softmax (groups of four, 16 rows each; a thread has a
 // position and its group's rows), four K, four V and q, one TMA, one MMA.
@@ -36,8 +36,9 @@
 namespace fyb {
 
 constexpr int KT_TILE = 128, KT_CONV = 4, KT_META = 8;
-// Warps: four softmax for every 16 rows; four that convert K and four that convert V, at 32 rows the same four (with
-// 16 warps or fewer a thread has 128 registers, with 18 it has 96: 309 against 274 us for the ragged drafts of 8).
+// Warps: four softmax for every 16 rows; four that convert K and four that convert V, at 32 rows the same four (14
+// warps: a thread has 128 registers; with 18 it has 96, 309 against 274 us for the ragged drafts of 8). At 64 rows 26
+// warps have 72 each.
 FYB_HOST_DEV constexpr int kt_soft(int N) { return N / 4; }
 FYB_HOST_DEV constexpr bool kt_split(int N) { return N > 32; }
 FYB_HOST_DEV constexpr int kt_conv(int N) { return kt_split(N) ? 2 * KT_CONV : KT_CONV; }

@@ -347,7 +347,7 @@ int fyb_rope(const fyb_rope_desc *rope, const int32_t *positions, size_t rows, u
    round(x / scale), to nearest even, every step in F32. Infinities are stored as the largest
    value, NaN as 0, neither counts for the scale. With `rope` K is rotated to
    positions[row] first, and q (may be NULL with heads 0) to q_out as by
-   fyb_rope, in the same launch; half pairs then need dims a multiple of 8. */
+   fyb_rope, in the same call; half pairs then need dims a multiple of 8. */
 int fyb_kv8_append(const fyb_kv8_cache *cache, const int32_t *slots, size_t rows, uint32_t type, const void *k,
     size_t k_stride, const void *v, size_t v_stride, const fyb_rope_desc *rope, const int32_t *positions,
     const void *q, size_t q_stride, void *q_out, size_t q_out_stride, uint32_t heads, uint32_t *error, void *stream);

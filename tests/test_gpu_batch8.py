@@ -1,6 +1,6 @@
 """GPU tests of a plan's batched decode over the paged 8-bit cache beside
-test_gpu_kv8.py: runs of several lengths, the ends of its
-capacity and of its life, what it refuses."""
+test_gpu_kv8.py: runs of several lengths, the ends of its capacity and of its
+life, what it refuses."""
 import numpy as np
 import pytest
 

@@ -1,6 +1,6 @@
-"""GPU tests of the paged 8-bit KV cache beside test_gpu_kv8.py: lengths
-at their end, operands that are left out, appends whose tables, rows or slots are not as regular as a
-model's, to the byte."""
+"""GPU tests of the paged 8-bit KV cache beside test_gpu_kv8.py: lengths at
+their end, operands that are left out, appends whose tables, rows or slots are
+not as regular as a model's (to the byte), scores and value scales far apart."""
 import ctypes as C
 
 import numpy as np
