@@ -95,6 +95,18 @@ class KV8Handle(C.Structure):
     _fields_ = [("cache", KV8CacheDesc), ("device", C.c_int32)]
 
 
+class KV4CacheDesc(C.Structure):
+    """fyb_kv4_cache (include/fyodor_b200.h)."""
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("k_scale", C.c_void_p), ("v_scale", C.c_void_p),
+                ("blocks", C.c_uint32), ("kv_heads", C.c_uint32), ("block_size", C.c_uint32),
+                ("head_dim", C.c_uint32)]
+
+
+class KV4Handle(C.Structure):
+    """The same as KV8Handle for a 4-bit cache."""
+    _fields_ = [("cache", KV4CacheDesc), ("device", C.c_int32)]
+
+
 class RopeDesc(C.Structure):
     """fyb_rope_desc (include/fyodor_b200.h)."""
     _fields_ = [("cos_table", C.c_void_p), ("sin_table", C.c_void_p), ("table_rows", C.c_uint32),
@@ -144,6 +156,13 @@ def _load():
     lib.fyb_kv8_attention_workspace.argtypes = [u32] * 5
     lib.fyb_kv8_attention.argtypes = [C.POINTER(KV8CacheDesc), _P, _P, u32, u32, size, _P, size, u32, _P, size, _P,
                                       size, u32, C.c_float, _P, size, _P, _P]
+    for name in ("append", "read", "attention_workspace", "attention"):  # the same but for the cache
+        f, g = getattr(lib, "fyb_kv4_" + name), getattr(lib, "fyb_kv8_" + name)
+        f.restype = g.restype
+        f.argtypes = [C.POINTER(KV4CacheDesc) if a is C.POINTER(KV8CacheDesc) else a for a in g.argtypes]
+    lib.fyb_logprobs_workspace.restype = size
+    lib.fyb_logprobs_workspace.argtypes = [size, u32, u32]
+    lib.fyb_logprobs.argtypes = [u32, _P, size, size, u32, _P, _P, _P, _P, u32, _P, _P, _P, size, _P, _P]
     lib.fyb_plan_tp_info.argtypes = [_P, _P, _P]
     lib.fyb_plan_tp_handle.argtypes = [_P, _P, C.c_size_t]
     lib.fyb_plan_tp_connect.argtypes = [_P, _P, C.c_size_t]
@@ -191,6 +210,8 @@ EXPORTS = ["nya_cuda_backend", "fyb_version", "fyb_device_count", "fyb_dequantiz
            "fyb_attention_decode", "fyb_attention_verify",
            "fyb_attention_decode_static", "fyb_kv_blocks", "fyb_kv_release", "fyb_rope_frequencies", "fyb_rope_tables",
            "fyb_rope", "fyb_kv8_append", "fyb_kv8_read", "fyb_kv8_attention_workspace", "fyb_kv8_attention",
+           "fyb_kv4_append", "fyb_kv4_read", "fyb_kv4_attention_workspace", "fyb_kv4_attention",
+           "fyb_logprobs_workspace", "fyb_logprobs",
            "fyb_plan_decode_greedy", "fyb_plan_verify",
            "fyb_plan_time_greedy", "fyb_plan_launches_per_token", "fyb_plan_decode_form", "fyb_plan_profile", "fyb_plan_trace",
            "fyb_plan_tp_info", "fyb_plan_tp_handle", "fyb_plan_tp_connect", "fyb_plan_tp_disconnect",
@@ -249,7 +270,7 @@ class SynthModel:
         self.close()
 
 
-# ---------------------------------------------------------------- paged 8-bit KV cache
+# ---------------------------------------------------------------- paged 8-bit and 4-bit KV caches, log probabilities
 # The calls below take torch tensors on the current CUDA device and run on
 # torch's current stream of it unless `stream` (a cudaStream_t as an int) is
 # given. Nothing synchronizes. A refused argument raises ValueError and leaves
@@ -267,7 +288,9 @@ def _bind_tensors():
         import torch  # noqa: F401  (the extension links against it)
         from . import _tensors as ext
         ext.bind(*(C.cast(f, C.c_void_p).value for f in (lib.fyb_kv_blocks, lib.fyb_kv_release, lib.fyb_rope,
-                                                         lib.fyb_kv8_append, lib.fyb_kv8_read, lib.fyb_kv8_attention)))
+                                                         lib.fyb_kv8_append, lib.fyb_kv8_read, lib.fyb_kv8_attention,
+                                                         lib.fyb_kv4_append, lib.fyb_kv4_read, lib.fyb_kv4_attention,
+                                                         lib.fyb_logprobs)))
         _native = ext
     return _native
 
@@ -400,6 +423,84 @@ class KV8Cache:
         request has other than one row, at most most_rows each."""
         (_native or _bind_tensors()).attention(self._handle, q, lengths, table, out, workspace, row_start, most_rows, scale,
                                           error, stream)
+
+
+class KV4Cache:
+    """A paged 4-bit KV cache over tensors of the caller: k and v
+    [blocks][kv_heads][block_size][head_dim / 2] uint8, k_scale and v_scale
+    [blocks][kv_heads][block_size][head_dim / 64][2] float16, scale and low of
+    each group of 64 values (fyb_kv4_cache)."""
+
+    def __init__(self, k, v, k_scale, v_scale):
+        import torch
+        if k.dim() != 4 or k.shape != v.shape or k_scale.shape != (*k.shape[:3], k.shape[3] // 32, 2) or \
+                v_scale.shape != k_scale.shape:
+            raise ValueError("k, v: [blocks][kv_heads][block_size][head_dim / 2]; scales [blocks][kv_heads][block_size]"
+                             "[head_dim / 64][2]")
+        for name, t, kind in (("k", k, torch.uint8), ("v", v, torch.uint8), ("k_scale", k_scale, torch.float16),
+                              ("v_scale", v_scale, torch.float16)):
+            if t.dtype is not kind or not t.is_cuda or not t.is_contiguous() or t.device != k.device:
+                raise ValueError("%s has to be a contiguous %s tensor on the cache's GPU" % (name, kind))
+        self.tensors = k, v, k_scale, v_scale
+        blocks, self.kv_heads, self.block_size, half = k.shape
+        self.head_dim = 2 * half
+        self._held = KV4Handle(KV4CacheDesc(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), blocks,
+                                            self.kv_heads, self.block_size, self.head_dim), k.get_device())
+        self.desc, self._handle = self._held.cache, C.addressof(self._held)
+
+    @classmethod
+    def empty(cls, blocks, kv_heads, block_size, head_dim, device="cuda"):
+        """A cache of its own tensors."""
+        import torch
+        k, v = (torch.zeros((blocks, kv_heads, block_size, head_dim // 2), dtype=torch.uint8, device=device)
+                for _ in range(2))
+        return cls(k, v, *(torch.zeros((blocks, kv_heads, block_size, head_dim // 64, 2), dtype=torch.float16,
+                                       device=device) for _ in range(2)))
+
+    def append(self, k, v, slots, positions=None, cos=None, sin=None, layout="interleaved", q=None, q_out=None,
+               error=None, stream=None):
+        """Store K and V rows [rows][kv_heads][head_dim] at slots[row], no slot
+        twice (fyb_kv4_append). With cos / sin K is rotated to positions[row]
+        first, and q to q_out in the same call."""
+        (_native or _bind_tensors()).append4(self._handle, k, v, slots, positions, cos, sin, layout, q, q_out, error, stream)
+
+    def read(self, slots, k_out, v_out, error=None, stream=None):
+        """The values held at slots into k_out, v_out [len(slots)][kv_heads][head_dim] float32 (fyb_kv4_read)."""
+        (_native or _bind_tensors()).read4(self._handle, slots, k_out, v_out, error, stream)
+
+    def attention_workspace(self, requests, most_rows, heads):
+        """A zeroed workspace for attention() calls of this size (one for each stream that calls)."""
+        import torch
+        need = lib.fyb_kv4_attention_workspace(requests, most_rows, heads, self.kv_heads, self.head_dim)
+        if not need:
+            raise ValueError("no attention of %d requests, %d rows, %d heads over %d KV heads of %d" %
+                             (requests, most_rows, heads, self.kv_heads, self.head_dim))
+        return torch.zeros(need, dtype=torch.uint8, device=self.tensors[0].device)
+
+    def attention(self, q, lengths, table, out, workspace, row_start=None, most_rows=1, scale=None, error=None,
+                  stream=None):
+        """KV8Cache.attention over this cache (fyb_kv4_attention)."""
+        (_native or _bind_tensors()).attention4(self._handle, q, lengths, table, out, workspace, row_start, most_rows, scale,
+                                           error, stream)
+
+
+def logprobs_workspace(rows, vocabulary, top=0, device="cuda"):
+    """A zeroed workspace for logprobs() calls of this size (one for each stream that calls)."""
+    import torch
+    need = lib.fyb_logprobs_workspace(rows, vocabulary, top) if min(rows, vocabulary, top) >= 0 else 0
+    if not need:
+        raise ValueError("no log probabilities of %d rows of %d with %d alternatives" % (rows, vocabulary, top))
+    return torch.zeros(need, dtype=torch.uint8, device=device)
+
+
+def logprobs(logits, tokens, logprob, entropy, rank, top_tokens, top_logprobs, workspace, error=None, stream=None):
+    """Of each row of logits [rows][vocabulary]: log probability and rank of
+    tokens[row], entropy, and the most probable tokens with their log
+    probabilities (fyb_logprobs). tokens and rank int32, logprob and entropy
+    float32 [rows]; top_tokens int32 and top_logprobs float32 [rows][top]; any
+    output may be None (tokens with logprob and rank)."""
+    (_native or _bind_tensors()).logprobs(logits, tokens, logprob, entropy, rank, top_tokens, top_logprobs, workspace, error,
+                                     stream)
 
 
 # ---------------------------------------------------------------- provider

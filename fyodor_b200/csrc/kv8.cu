@@ -71,36 +71,6 @@ template <typename T, int E> FYB_DEV void kv8_values(const Kv8Append &A, const R
     }
 }
 
-// q rows: CTA = 256 items of one row
-template <typename T, int HD> FYB_DEV void kv8_turn_q(const Kv8Append &A, unsigned cta)
-{
-    const size_t r = cta / A.q_rows;
-    const unsigned i = cta % A.q_rows * KV8_THREADS + threadIdx.x;
-    const unsigned groups = A.many ? (A.q.heads + ROPE_HEADS - 1) / ROPE_HEADS : A.q.heads;
-    unsigned head, item;  // heads head, head + groups, ...
-    if (!rope_place(A.work, groups, i, head, item)) return;
-    const int pos = A.positions[r];
-    const T *in = static_cast<const T *>(A.q.in) + r * A.q.in_stride + (size_t)head * HD;
-    T *out = static_cast<T *>(A.q.out) + r * A.q.out_stride + (size_t)head * HD;
-    auto at = [&](const float *&c, const float *&s) {
-        if (pos < 0 || (unsigned)pos >= A.rope.rows) {
-            if (i == 0) raise_error(A.error, ERR_BOUNDS);
-            return false;
-        }
-        const size_t t = (size_t)pos * (A.rope.dims / 2);
-        c = A.rope.cos + t;
-        s = A.rope.sin + t;
-        return true;
-    };
-    constexpr int V = 16 / sizeof(T);
-    if (A.many)
-        rope_item<T, V, true, ROPE_HEADS>(in, out, (size_t)groups * HD, (A.q.heads - head + groups - 1) / groups,
-                                          A.rope.dims, A.rope.layout, item, at);
-    else if (A.vec) rope_item<T, V, true, 1>(in, out, HD, 1, A.rope.dims, A.rope.layout, item, at);
-    else if (A.rope.layout == 0) rope_item<T, 2, false, 1>(in, out, HD, 1, A.rope.dims, 0, item, at);
-    else rope_item<T, 1, false, 1>(in, out, HD, 1, A.rope.dims, 1, item, at);
-}
-
 // Four stored bytes of values already divided by the scale.
 template <unsigned FMT> FYB_DEV unsigned kv8_store4(float a, float b, float c, float d)
 {
@@ -156,7 +126,7 @@ __global__ void __launch_bounds__(KV8_THREADS, 4) kv8_append_kernel(Kv8Append A)
     const unsigned tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, kv = A.c.kv_heads;
     const unsigned windows = (unsigned)((A.rows + A.window - 1) / A.window);
     if (blockIdx.x >= windows * A.parts) {
-        kv8_turn_q<T, HD>(A, blockIdx.x - windows * A.parts);
+        rope_row_of_q<T, HD, KV8_THREADS>(A, blockIdx.x - windows * A.parts);
         return;
     }
     const unsigned part = blockIdx.x % A.parts;

@@ -1,5 +1,5 @@
 // rope.cuh - rotary positions of one run of a head's values, shared by the
-// stand-alone kernel (rope.cu) and the cache append (kv8.cu).
+// stand-alone kernel (rope.cu) and the cache appends (kv8.cu, kv4.cu).
 #pragma once
 #include "common.cuh"
 #include "kernels.h"
@@ -172,6 +172,36 @@ constexpr int ROPE_HEADS = 2;
 inline bool rope_many(size_t rows, unsigned heads, const RopeWork &w)
 {
     return rows * (heads / ROPE_HEADS) * (w.turned + w.copied) >= (size_t)2 * 148 * 2048;
+}
+
+// A row of q beside a cache append (kv8.cu, kv4.cu), whose arguments A are: CTA `cta` takes THREADS items of it.
+template <typename T, int HD, unsigned THREADS, typename Append> FYB_DEV void rope_row_of_q(const Append &A, unsigned cta)
+{
+    const size_t r = cta / A.q_rows;
+    const unsigned i = cta % A.q_rows * THREADS + threadIdx.x;
+    const unsigned groups = A.many ? (A.q.heads + ROPE_HEADS - 1) / ROPE_HEADS : A.q.heads;
+    unsigned head, item;  // heads head, head + groups, ...
+    if (!rope_place(A.work, groups, i, head, item)) return;
+    const int pos = A.positions[r];
+    const T *in = static_cast<const T *>(A.q.in) + r * A.q.in_stride + (size_t)head * HD;
+    T *out = static_cast<T *>(A.q.out) + r * A.q.out_stride + (size_t)head * HD;
+    auto at = [&](const float *&c, const float *&s) {
+        if (pos < 0 || (unsigned)pos >= A.rope.rows) {
+            if (i == 0) raise_error(A.error, ERR_BOUNDS);
+            return false;
+        }
+        const size_t t = (size_t)pos * (A.rope.dims / 2);
+        c = A.rope.cos + t;
+        s = A.rope.sin + t;
+        return true;
+    };
+    constexpr int V = 16 / sizeof(T);
+    if (A.many)
+        rope_item<T, V, true, ROPE_HEADS>(in, out, (size_t)groups * HD, (A.q.heads - head + groups - 1) / groups,
+                                          A.rope.dims, A.rope.layout, item, at);
+    else if (A.vec) rope_item<T, V, true, 1>(in, out, HD, 1, A.rope.dims, A.rope.layout, item, at);
+    else if (A.rope.layout == 0) rope_item<T, 2, false, 1>(in, out, HD, 1, A.rope.dims, 0, item, at);
+    else rope_item<T, 1, false, 1>(in, out, HD, 1, A.rope.dims, 1, item, at);
 }
 
 }  // namespace fyb

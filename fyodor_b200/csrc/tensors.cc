@@ -1,5 +1,5 @@
-// tensors.cc - the paged 8-bit cache's entry points for torch tensors, as a
-// CPython extension (fyodor_b200/_tensors.so).
+// tensors.cc - the entry points of the paged caches and of the log
+// probabilities for torch tensors, as a CPython extension (fyodor_b200/_tensors.so).
 //
 // A decode step calls them thousands of times a second on kernels of a few
 // microseconds; through ctypes the checks and conversions of a dozen tensors
@@ -22,6 +22,10 @@ struct {
     decltype(&fyb_kv8_append) append;
     decltype(&fyb_kv8_read) read;
     decltype(&fyb_kv8_attention) attention;
+    decltype(&fyb_kv4_append) append4;
+    decltype(&fyb_kv4_read) read4;
+    decltype(&fyb_kv4_attention) attention4;
+    decltype(&fyb_logprobs) logprobs;
 } entry;
 
 struct Refused {};  // a Python exception is set
@@ -32,9 +36,9 @@ struct Refused {};  // a Python exception is set
     throw Refused();
 }
 
-// The cache handle: what the Python object (KV8Handle) holds the address of.
-struct CacheHandle {
-    fyb_kv8_cache cache;
+// The cache handle: what the Python object (KV8Handle, KV4Handle) holds the address of.
+template <typename Cache> struct CacheHandle {
+    Cache cache;
     int32_t device;
 };
 
@@ -58,9 +62,9 @@ struct Call {
         on(t.get_device(), name);
         return t;
     }
-    const fyb_kv8_cache *cache(PyObject *o)
+    template <typename Cache> const Cache *cache(PyObject *o)
     {
-        const CacheHandle *h = static_cast<const CacheHandle *>(PyLong_AsVoidPtr(o));
+        const CacheHandle<Cache> *h = static_cast<const CacheHandle<Cache> *>(PyLong_AsVoidPtr(o));
         if (PyErr_Occurred()) throw Refused();
         if (!h) refuse("cache", "has no address");
         on(h->device, "cache");
@@ -108,13 +112,14 @@ Rows rows_of(Call &c, PyObject *o, const char *name)
     if (r.stride < 0) refuse(name, "has a negative stride");
     return r;
 }
-uint32_t type_of(const Rows &r, const char *name)
+uint32_t type_of(at::ScalarType kind, const char *name)
 {
-    if (r.kind == at::kFloat) return 0;
-    if (r.kind == at::kHalf) return 1;
-    if (r.kind == at::kBFloat16) return 30;
+    if (kind == at::kFloat) return 0;
+    if (kind == at::kHalf) return 1;
+    if (kind == at::kBFloat16) return 30;
     refuse(name, "has to be float32, float16 or bfloat16");
 }
+uint32_t type_of(const Rows &r, const char *name) { return type_of(r.kind, name); }
 void alike(const Rows &a, const Rows &b, const char *name)
 {
     if (a.rows != b.rows || a.dim != b.dim || a.kind != b.kind) refuse(name, "has other rows, head_dim or type than it has to have");
@@ -238,11 +243,11 @@ PyObject *rope(PyObject *, PyObject *const *a, Py_ssize_t n)
 }
 
 // (cache, k, v, slots, positions, cos, sin, layout, q, q_out, error, stream)
-PyObject *append(PyObject *, PyObject *const *a, Py_ssize_t n)
+template <typename Cache, typename Entry> PyObject *append_of(Entry entry, const char *what, PyObject *const *a, Py_ssize_t n)
 {
     return guarded(n, 12, [&] {
         Call c;
-        const fyb_kv8_cache *cache = c.cache(a[0]);
+        const Cache *cache = c.cache<Cache>(a[0]);
         const Rows k = rows_of(c, a[1], "k"), v = rows_of(c, a[2], "v");
         alike(k, v, "v");
         if (k.heads != cache->kv_heads || v.heads != cache->kv_heads || k.dim != cache->head_dim)
@@ -263,33 +268,33 @@ PyObject *append(PyObject *, PyObject *const *a, Py_ssize_t n)
             alike(k, qo, "q_out");
             if (q.heads != qo.heads || q.heads > 65536) refuse("q_out", "has other heads than q");
         }
-        return answer(entry.append(cache, slots, (size_t)k.rows, type_of(k, "k"), k.p, (size_t)k.stride, v.p,
+        return answer(entry(cache, slots, (size_t)k.rows, type_of(k, "k"), k.p, (size_t)k.stride, v.p,
                                    (size_t)v.stride, turn ? &d : nullptr, positions, q.p, (size_t)q.stride, qo.p,
                                    (size_t)qo.stride, (uint32_t)q.heads, c.error(a[10]), c.stream(a[11])),
-                      "fyb_kv8_append");
+                      what);
     });
 }
 
 // (cache, slots, k_out, v_out, error, stream)
-PyObject *read(PyObject *, PyObject *const *a, Py_ssize_t n)
+template <typename Cache, typename Entry> PyObject *read_of(Entry entry, const char *what, PyObject *const *a, Py_ssize_t n)
 {
     return guarded(n, 6, [&] {
         Call c;
-        const fyb_kv8_cache *cache = c.cache(a[0]);
+        const Cache *cache = c.cache<Cache>(a[0]);
         const int64_t rows = c.tensor(a[1], "slots").numel(), need = rows * cache->kv_heads * cache->head_dim;
         const int32_t *slots = c.ints(a[1], "slots");
         float *k = static_cast<float *>(c.flat(a[2], "k_out", at::kFloat, need));
         float *v = static_cast<float *>(c.flat(a[3], "v_out", at::kFloat, need));
-        return answer(entry.read(cache, slots, (size_t)rows, k, v, c.error(a[4]), c.stream(a[5])), "fyb_kv8_read");
+        return answer(entry(cache, slots, (size_t)rows, k, v, c.error(a[4]), c.stream(a[5])), what);
     });
 }
 
 // (cache, q, lengths, table, out, workspace, row_start, most_rows, scale, error, stream)
-PyObject *attention(PyObject *, PyObject *const *a, Py_ssize_t n)
+template <typename Cache, typename Entry> PyObject *attention_of(Entry entry, const char *what, PyObject *const *a, Py_ssize_t n)
 {
     return guarded(n, 11, [&] {
         Call c;
-        const fyb_kv8_cache *cache = c.cache(a[0]);
+        const Cache *cache = c.cache<Cache>(a[0]);
         const Rows q = rows_of(c, a[1], "q"), out = rows_of(c, a[4], "out");
         alike(q, out, "out");
         if (q.heads != out.heads || q.dim != cache->head_dim || q.heads > 0x7fffffff)
@@ -301,22 +306,60 @@ PyObject *attention(PyObject *, PyObject *const *a, Py_ssize_t n)
         if (!ws.is_contiguous()) refuse("workspace", "has to be contiguous");
         const double scale = a[8] == Py_None ? 1.0 / std::sqrt((double)cache->head_dim) : PyFloat_AsDouble(a[8]);
         if (PyErr_Occurred()) throw Refused();
-        return answer(entry.attention(cache, c.ints(a[2], "lengths"),
+        return answer(entry(cache, c.ints(a[2], "lengths"),
                                       a[6] == Py_None ? nullptr : c.ints(a[6], "row_start", req + 1), (uint32_t)req,
                                       u32(a[7], "most_rows"), (size_t)q.rows, c.ints(a[3], "table"),
                                       (size_t)table.size(1), type_of(q, "q"), q.p, (size_t)q.stride, out.p,
                                       (size_t)out.stride, (uint32_t)q.heads, (float)scale, ws.data_ptr(),
                                       (size_t)ws.nbytes(), c.error(a[9]), c.stream(a[10])),
-                      "fyb_kv8_attention");
+                      what);
+    });
+}
+
+#define CACHE_METHODS(name) \
+    PyObject *name(PyObject *, PyObject *const *a, Py_ssize_t n) { return name##_of<fyb_kv8_cache>(entry.name, "fyb_kv8_" #name, a, n); } \
+    PyObject *name##4(PyObject *, PyObject *const *a, Py_ssize_t n) { return name##_of<fyb_kv4_cache>(entry.name##4, "fyb_kv4_" #name, a, n); }
+CACHE_METHODS(append)
+CACHE_METHODS(read)
+CACHE_METHODS(attention)
+
+// (logits, tokens, logprob, entropy, rank, top_tokens, top_logprobs, workspace, error, stream)
+PyObject *logprobs(PyObject *, PyObject *const *a, Py_ssize_t n)
+{
+    return guarded(n, 10, [&] {
+        Call c;
+        const at::Tensor &x = c.tensor(a[0], "logits");
+        if (x.dim() != 2 || (x.stride(1) != 1 && x.size(1) > 1)) refuse("logits", "has to be [rows][vocabulary], a row's logits contiguous");
+        const int64_t rows = x.size(0), values = x.size(1), stride = rows < 2 ? values : x.stride(0);
+        if (stride < values || values > 0x7fffffff) refuse("logits", "has overlapping rows or too many logits in one");
+        auto floats = [&](PyObject *o, const char *name, int64_t least) {
+            return o == Py_None ? nullptr : static_cast<float *>(c.flat(o, name, at::kFloat, least));
+        };
+        auto ints = [&](PyObject *o, const char *name, int64_t least) { return o == Py_None ? nullptr : c.ints(o, name, least); };
+        int64_t top = 0;
+        if (a[5] != Py_None) {
+            const at::Tensor &t = c.tensor(a[5], "top_tokens");
+            if (t.dim() != 2 || t.size(0) != rows || t.size(1) > 0x7fffffff) refuse("top_tokens", "has to be [rows][top]");
+            top = t.size(1);
+        }
+        const at::Tensor &ws = c.tensor(a[7], "workspace");
+        if (!ws.is_contiguous()) refuse("workspace", "has to be contiguous");
+        return answer(entry.logprobs(type_of(x.scalar_type(), "logits"), x.data_ptr(), (size_t)stride, (size_t)rows,
+                                     (uint32_t)values, ints(a[1], "tokens", rows), floats(a[2], "logprob", rows),
+                                     ints(a[4], "rank", rows), floats(a[3], "entropy", rows), (uint32_t)top,
+                                     top ? ints(a[5], "top_tokens", rows * top) : nullptr,
+                                     top ? floats(a[6], "top_logprobs", rows * top) : nullptr, ws.data_ptr(),
+                                     (size_t)ws.nbytes(), c.error(a[8]), c.stream(a[9])),
+                      "fyb_logprobs");
     });
 }
 
 // Addresses of the C entry points, in the order of `entry`.
 PyObject *bind(PyObject *, PyObject *const *a, Py_ssize_t n)
 {
-    return guarded(n, 6, [&]() -> PyObject * {
+    return guarded(n, 10, [&]() -> PyObject * {
         void **e = reinterpret_cast<void **>(&entry);
-        for (int i = 0; i < 6; ++i) {
+        for (int i = 0; i < 10; ++i) {
             e[i] = PyLong_AsVoidPtr(a[i]);
             if (PyErr_Occurred()) throw Refused();
         }
@@ -326,7 +369,7 @@ PyObject *bind(PyObject *, PyObject *const *a, Py_ssize_t n)
 
 #define METHOD(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(name)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {METHOD(bind), METHOD(kv_blocks), METHOD(kv_release), METHOD(rope), METHOD(append), METHOD(read),
-                         METHOD(attention), {nullptr, nullptr, 0, nullptr}};
+                         METHOD(attention), METHOD(append4), METHOD(read4), METHOD(attention4), METHOD(logprobs), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_tensors", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

@@ -374,6 +374,72 @@ int fyb_kv8_attention(const fyb_kv8_cache *cache, const int32_t *lengths, const 
     size_t q_stride, void *out, size_t out_stride, uint32_t heads, float scale, void *workspace,
     size_t workspace_bytes, uint32_t *error, void *stream);
 
+/* ---- paged 4-bit KV cache (no counterpart in the reference) ---------------
+   The cache of the section above in 4.5 bits a value: blocks, tables, slots,
+   lengths, row types, strides and error words as there (fyb_kv_blocks and
+   fyb_kv_release serve both). Each group of 64 values of a head of a token is
+   held as low + scale * n, n = 0..15, scale and low F16. Of the group's finite
+   values, those beyond +-61440 taken as +-61440, low and high are the least and
+   the greatest rounded to F16, scale is (high - low) / 15 rounded to F16, and n
+   is the whole number nearest to (x - low) / scale, ties to even, in 0..15 (0
+   where scale is 0). Infinities are held as 0 or 15, NaN as 0 would be; both
+   raise 2 in `error`. A group without a finite value has low and scale 0. A row
+   depends on no other: tokens may be written in any order, and again.
+   A token's row of a head is head_dim / 8 words of 32 bits, each eight values,
+   the first in the lowest bits: word w holds dimensions 8w.. of a head of 64;
+   of a head of 128 word 2j holds dimensions 8j.., word 2j + 1 64 + 8j... */
+typedef struct fyb_kv4_cache {
+    void *k, *v;             /* [blocks][kv_heads][block_size][head_dim / 2] bytes, 16-byte aligned */
+    void *k_scale, *v_scale; /* [blocks][kv_heads][block_size][head_dim / 64][2] F16: scale, low; 16-byte aligned */
+    uint32_t blocks, kv_heads;
+    uint32_t block_size;     /* 16, 32, 64, 128 or 256 tokens */
+    uint32_t head_dim;       /* 64 or 128 */
+} fyb_kv4_cache;
+/* Append K and V rows at slots[row] (a negative slot is skipped, every other
+   occurs once in a call). A row whose slot is out of range is left out, one
+   whose position is out of the table is left out of K. With `rope` K is rotated
+   in F32 to positions[row] first, and q (may be NULL with heads 0) to q_out as
+   by fyb_rope, in the same call. */
+int fyb_kv4_append(const fyb_kv4_cache *cache, const int32_t *slots, size_t rows, uint32_t type, const void *k,
+    size_t k_stride, const void *v, size_t v_stride, const fyb_rope_desc *rope, const int32_t *positions,
+    const void *q, size_t q_stride, void *q_out, size_t q_out_stride, uint32_t heads, uint32_t *error, void *stream);
+/* k_out / v_out [rows][kv_heads][head_dim] F32, 16-byte aligned = the values held at slots[row] (0 for a negative slot). */
+int fyb_kv4_read(const fyb_kv4_cache *cache, const int32_t *slots, size_t rows, float *k_out, float *v_out,
+    uint32_t *error, void *stream);
+/* Causal attention of the newest rows of each request over its blocks:
+   fyb_kv8_attention's arguments, workspace rules and results over this cache. */
+size_t fyb_kv4_attention_workspace(uint32_t requests, uint32_t max_rows, uint32_t heads, uint32_t kv_heads,
+    uint32_t head_dim);
+int fyb_kv4_attention(const fyb_kv4_cache *cache, const int32_t *lengths, const int32_t *row_start, uint32_t requests,
+    uint32_t max_rows, size_t rows, const int32_t *table, size_t table_stride, uint32_t type, const void *q,
+    size_t q_stride, void *out, size_t out_stride, uint32_t heads, float scale, void *workspace,
+    size_t workspace_bytes, uint32_t *error, void *stream);
+
+/* ---- log probabilities (the engine's callers take them from whole logits on
+   the host; no counterpart in the reference) --------------------------------
+   Of each row x of logits [rows][vocabulary] (`type` F32, F16 or BF16, stride in
+   elements), in F32 and natural units:
+     logprob[r]       x[t] - ln sum exp x, t = tokens[r]
+     rank[r]          logits above x[t], and equal ones before it
+     entropy[r]       - sum p ln p
+     top_tokens, top_logprobs [rows][top]   the most probable tokens, of equal
+                      ones the first; -1 and -inf beyond those of probability > 0
+   tokens and logprob may be NULL together, rank (needs tokens) and entropy
+   alone, top_tokens and top_logprobs with top 0. A negative token asks for none
+   (logprob 0, rank -1); one past the vocabulary is taken so and raises 4 in
+   `error`. A logit of -inf is a token that cannot be answered: logprob -inf, no
+   part in the entropy; a row of nothing else has logprob -inf and entropy 0. A
+   row with NaN or +inf raises 2: its logprob, entropy and top_logprobs are NaN,
+   NaN is not among its alternatives.
+   top <= 32, rows <= 2^31 - 1. workspace: fyb_logprobs_workspace() bytes, 16-byte aligned,
+   zero before the first call (calls leave it so); calls that overlap in time
+   need workspaces of their own. Results do not depend on timing. */
+#define FYB_LOGPROBS_TOP 32u
+size_t fyb_logprobs_workspace(size_t rows, uint32_t vocabulary, uint32_t top);
+int fyb_logprobs(uint32_t type, const void *logits, size_t stride, size_t rows, uint32_t vocabulary,
+    const int32_t *tokens, float *logprob, int32_t *rank, float *entropy, uint32_t top, int32_t *top_tokens,
+    float *top_logprobs, void *workspace, size_t workspace_bytes, uint32_t *error, void *stream);
+
 /* ---- tensor parallelism across processes (no reference counterpart) -----
    A process whose environment holds NYA_CUDA_TP_SIZE=N (2..8) and
    NYA_CUDA_TP_RANK=r (and NYA_CUDA_DEVICE for its GPU) creates plans that hold
