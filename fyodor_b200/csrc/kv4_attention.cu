@@ -1,18 +1,23 @@
-// kv4_attention.cu - attention over the paged 4-bit cache.
+// kv4_attention.cu - the entry point of attention over the paged 4-bit cache:
+// argument checks, the workspace, and which kernel runs. Up to eight query rows
+// per KV head run on kv4_decode.cu.
 //
-// A warp takes one query row of one head and walks the positions it attends:
+// Many rows: a warp takes one query row of one head and walks the positions it attends:
 // lanes share out the head's dimensions, and of a group the score is scale (q . n)
 // + low sum(q), so the held numbers are used as they lie.
-#include "kv8_attention.cuh"
-#include "kv4.cuh"
+#include "kv4_attention.cuh"
 
 namespace fyb {
 
 constexpr int K4_WARPS = 8;
 
-struct Kv4Attention : Kv8Attention {
-    const __half2 *ks, *vs;
-};
+// K or V as token rows of head_dim / 2 bytes, boxes of one block (128 rows at most), rows of 64 bytes in the swizzle of
+// 64 bytes: 16-byte chunk c of token row t lies at chunk c ^ (t >> 1 & 3).
+static int kv4_tensor_map(CUtensorMap *map, const fyb_kv8_cache &c, const void *pool)
+{
+    return kv8_tensor_map(map, pool, c.head_dim / 2, (size_t)c.blocks * c.kv_heads * c.block_size,
+                          std::min(c.block_size, (unsigned)K4_TILE), c.head_dim == 128 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_NONE);
+}
 
 // Lane's 16 bits of a token's row (HD 128: four values, HD 64: two, 8 bits) from its first dimension.
 template <typename T, int HD> __global__ void __launch_bounds__(32 * K4_WARPS) kv4_rows_kernel(const __grid_constant__ Kv4Attention A)
@@ -106,9 +111,22 @@ extern "C" int fyb_kv4_attention(const fyb_kv4_cache *cache, const int32_t *leng
     A.rows = (unsigned)rows; A.q = q; A.q_stride = q_stride; A.out = out; A.out_stride = out_stride;
     A.requests = requests; A.max_rows = max_rows; A.heads = heads; A.group = heads / cache->kv_heads;
     A.shift = kv4_shift(cache); A.type = type; A.scale = scale * 1.44269504f; A.error = error;
+    cudaStream_t s = (cudaStream_t)stream;
+    unsigned char *ws = static_cast<unsigned char *>(workspace);
+    A.counters = reinterpret_cast<unsigned *>(ws);
+    A.part_ml = reinterpret_cast<float2 *>(ws + KA_COUNTER_BYTES);
+    A.part_o = reinterpret_cast<float *>(A.part_ml + 2 * KA_GRID * KV8_DECODE_ROWS);
+    if ((unsigned long long)max_rows * A.group <= KV8_DECODE_ROWS) {
+        CUtensorMap k, v;
+        if (kv4_tensor_map(&k, A.c, A.c.k) || kv4_tensor_map(&v, A.c, A.c.v)) return -2;
+        A.row_tile = max_rows;
+        // no more CTAs than the most units the tables can hold
+        const unsigned long long holds = (unsigned long long)table_stride << A.shift;
+        const unsigned long long units = (holds + K4_TILE - 1) / K4_TILE * requests * cache->kv_heads;
+        return launch_kv4_decode(A, k, v, (unsigned)std::min<unsigned long long>(KA_GRID, units), s);
+    }
     const size_t grid = (rows * heads + K4_WARPS - 1) / K4_WARPS;
     if (grid > 0x7fffffffu) return -1;
-    cudaStream_t s = (cudaStream_t)stream;
     if (type == T_F32) rows_launch<float>(A, (unsigned)grid, s);
     else if (type == T_F16) rows_launch<__half>(A, (unsigned)grid, s);
     else rows_launch<__nv_bfloat16>(A, (unsigned)grid, s);

@@ -1,0 +1,17 @@
+// kv4_attention.cuh - what the kernels of attention over the paged 4-bit cache
+// share: their arguments and the loads of the cache. The work is split over the
+// GPU as the 8-bit cache's is (kv8_attention.cuh).
+#pragma once
+#include "kv8_attention.cuh"
+#include "kv4.cuh"
+
+namespace fyb {
+
+struct Kv4Attention : Kv8Attention {
+    const __half2 *ks, *vs;  // scale and low of each group
+};
+
+int launch_kv4_decode(const Kv4Attention &A, const CUtensorMap &k, const CUtensorMap &v, unsigned grid, cudaStream_t s);
+constexpr int K4_TILE = 128;  // positions of a unit
+
+}  // namespace fyb

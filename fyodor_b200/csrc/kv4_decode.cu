@@ -1,0 +1,478 @@
+// kv4_decode.cu - attention over the paged 4-bit cache for up to eight query
+// rows per KV head: single tokens of grouped heads, short drafts.
+//
+// With k = low + scale n in groups of 64 dimensions, and q_g a group's part of q,
+//
+//   q . k = sum_g scale_g (q_g . n_g) + low_g sum(q_g)
+//   o_g   = sum_t (p_t scale_tg) n_tg + sum_t p_t low_tg
+//
+// so the tensor cores multiply the whole numbers n themselves, S^T = N Q^T and
+// O_g^T = N_g^T W_g^T with mma.sync m16n8k16: a masked word of the cache is already
+// a pair of fp16 operands, the subnormal n 2^-24 (or 16 n 2^-24 for the upper
+// number of a byte, which q and the output take back), with nothing to convert.
+// Scales and lows meet the scores and the weights in F32.
+//
+// q and the weights are two fp16 halves, hi + lo, 22 bits: with up to four rows
+// the eight columns are the hi and lo halves of the rows, one MMA for both; with up
+// to eight they are the rows, with low halves in an MMA of their own for F32 rows.
+// Rows of 16 bits fit the high half, and their weights are rounded to it (2^-11,
+// below the output's own rounding).
+#include "kv4_attention.cuh"
+
+namespace fyb {
+
+constexpr int K4_WARPS = 4, K4_THREADS = 32 * (K4_WARPS + 1);
+
+template <int HD> struct K4Shape {
+    static constexpr int ROW = HD / 2, SCALES = HD / 64 * 4;               // bytes of a token's row, of its scales
+    static constexpr int OFF_V = K4_TILE * ROW, OFF_KS = 2 * OFF_V, OFF_VS = OFF_KS + K4_TILE * SCALES,
+                         STAGE = OFF_VS + K4_TILE * SCALES, STAGES = 3 * (128 / HD);
+};
+
+// W: rows a thread holds scores of (1: up to four query rows, 2: up to eight). LO: whether q and the weights have low
+// halves at W = 2 (at W = 1 they are columns that cost nothing).
+template <int HD, int W, bool LO>
+__global__ void __launch_bounds__(K4_THREADS, 3) kv4_decode_kernel(const __grid_constant__ Kv4Attention A, const __grid_constant__ CUtensorMap kmap,
+    const __grid_constant__ CUtensorMap vmap)
+{
+    using S = K4Shape<HD>;
+    constexpr int R = 4 * W, G = HD / 64, NW = HD / 32, J = W == 1 ? 2 : 1;  // NW: words of K a thread takes of a token
+    extern __shared__ unsigned char k4_smem[];
+    unsigned char *ring = k4_smem + ((1024u - (smem_u32(k4_smem) & 1023u)) & 1023u);
+    float *o_s = reinterpret_cast<float *>(ring + S::STAGES * S::STAGE);    // [warps][R][HD], then weights of a join
+    float2 *ml_s = reinterpret_cast<float2 *>(o_s + K4_WARPS * R * HD);     // [warps][R], then [R]
+    uint64_t *full = reinterpret_cast<uint64_t *>(ml_s + K4_WARPS * R), *empty = full + S::STAGES;
+    unsigned *here = reinterpret_cast<unsigned *>(empty + S::STAGES);       // [stages] which groups of 16 positions are loaded
+    unsigned *flag = here + S::STAGES;
+    volatile unsigned *dead = flag + 1;   // a wait ran out: nobody waits any more, the error word is set
+    const unsigned tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, kv = A.c.kv_heads;
+    if (tid == 0) {
+        for (int i = 0; i < S::STAGES; ++i) { mbar_init(full + i, 1); mbar_init(empty + i, K4_WARPS); }
+        *dead = 0;
+        fence_barrier_init();
+    }
+    const Kv8Place place = kv8_place<K4_TILE, K4_THREADS, 5>(A);  // a CTA barrier inside
+    Kv8Walk<K4_TILE> walk(A, place);
+    Kv8Segment s;
+    unsigned stage = 0, phase = 0;
+    auto advance = [&] { if (++stage == S::STAGES) { stage = 0; phase ^= 1; } };
+    auto wait = [&](uint64_t *bar, unsigned ph) {
+        if (*dead || mbar_wait_bounded(bar, ph)) return;
+        *dead = 1;
+        if (lane == 0) raise_error(A.error, ERR_TIMEOUT);
+    };
+
+    if (warp == K4_WARPS) {
+        // ---- producer: block ids 32 at a time, tiles and scales by bulk copies
+        const unsigned size = 1u << A.shift, box = min(size, (unsigned)K4_TILE), per = K4_TILE / box;
+        unsigned issued = 0;
+        while (walk.next(s)) {
+            const int blocks = (kv8_attended(A, s.q, s.row_tile) + (int)size - 1) >> A.shift;
+            const int *ids = A.table + (size_t)s.request * A.table_stride;
+            int have = -1, id = 0;    // lane holds block 32 * have + lane
+            for (int t = s.t0; t < s.t1; ++t) {
+                const int b0 = t * K4_TILE >> A.shift;   // first block of the tile; `per` of them, or a part of one
+                if (b0 / 32 != have) {
+                    have = b0 / 32;
+                    const int b = have * 32 + (int)lane;
+                    id = b < blocks ? ids[b] : -1;
+                    if (b < blocks && (unsigned)id >= A.c.blocks) {  // negative ones too
+                        raise_error(A.error, ERR_BOUNDS);
+                        id = -1;
+                    }
+                }
+                wait(empty + stage, phase ^ 1);
+                const int mine = __shfl_sync(0xffffffffu, id, (b0 & 31) + (int)(lane % per));
+                const bool load = lane < per && mine >= 0;
+                const unsigned boxes = __ballot_sync(0xffffffffu, load);
+                // groups of 16 positions whose block is among the loaded ones
+                const unsigned groups = __ballot_sync(0xffffffffu, lane < K4_TILE / 16 && (boxes >> (lane * 16 / box) & 1));
+                if (lane == 0) {
+                    here[stage] = groups;
+                    if (boxes) mbar_expect_tx(full + stage, __popc(boxes) * 2 * box * (S::ROW + S::SCALES)); else mbar_arrive(full + stage);
+                }
+                __syncwarp();
+                if (load && !*dead) {
+                    const unsigned row = (((unsigned)mine * kv + s.head) << A.shift) + ((unsigned)(t * K4_TILE) & (size - 1));
+                    unsigned char *dst = ring + stage * S::STAGE;
+                    tma_load_rows(dst + lane * box * S::ROW, &kmap, (int)row, full + stage);
+                    tma_load_rows(dst + S::OFF_V + lane * box * S::ROW, &vmap, (int)row, full + stage);
+                    bulk_copy_g2s(dst + S::OFF_KS + lane * box * S::SCALES, A.ks + (size_t)row * G, box * S::SCALES, full + stage);
+                    bulk_copy_g2s(dst + S::OFF_VS + lane * box * S::SCALES, A.vs + (size_t)row * G, box * S::SCALES, full + stage);
+                }
+                __syncwarp();
+                ++issued;
+                advance();
+            }
+        }
+        if (*dead) {  // copies in flight land before the CTA leaves its shared memory
+            for (unsigned i = 0; i < min(issued, (unsigned)S::STAGES); ++i) mbar_wait_bounded(full + i, (issued - 1 - i) / S::STAGES & 1);
+        }
+        return;
+    }
+
+    // ---- consumers
+    const unsigned g = lane >> 2, t4 = lane & 3;
+    // Positions of a tile's 16 in the order of the MMAs: a thread has, of K, rows tau and tau + 8, of V rows ta, ta ^ X
+    // and both + 8 (the same as k indexes 2 t4, 2 t4 + 1 and both + 8). Chosen so that the rows that one phase of a
+    // load reads lie in different banks (rows of 64 bytes in the swizzle of 64, of 32 bytes in none).
+    constexpr unsigned X = HD == 128 ? 3 : 7;
+    auto order = [](unsigned t) { return HD == 128 ? (t & 1) + 4 * (t >> 1) : t; };
+    const unsigned ta = order(t4), tau = order(g >> 1) ^ (g & 1 ? X : 0u);
+    auto swizzled = [](unsigned pos, unsigned byte) { return pos * S::ROW + (HD == 128 ? byte ^ ((pos >> 1 & 3) << 4) : byte); };
+    constexpr float P_SCALE = 32.f;  // keeps small weights clear of fp16's smallest numbers; the largest is 2^14
+    auto bar = [] { asm volatile("bar.sync 1, %0;" :: "n"(32 * K4_WARPS) : "memory"); };
+
+    while (walk.next(s)) {
+        const unsigned GR = A.group;
+        const int j0 = s.row_tile * (int)A.row_tile, nrows = min((int)A.row_tile, s.q.rows - j0) * (int)GR;
+        auto row_of = [&](unsigned rho, size_t &row, unsigned &head) {
+            row = (size_t)(s.q.first + j0 + (int)(rho / GR));
+            head = s.head * GR + rho % GR;
+        };
+        // ---- q: column g of the B fragments, normalized by a power of two and split in halves
+        unsigned qh[2 * NW][2], ql[LO ? 2 * NW : 1][2];
+        float fn[W], fq[W][G];  // score factors of this thread's rows, and times the sums of q
+        int limit[W];           // positions they attend
+        {
+            const unsigned rho = W == 1 ? g >> 1 : g;
+            float x[NW][8];
+            float top = 0.f, sum[G] = {};
+#pragma unroll
+            for (int i = 0; i < NW; ++i) {
+                float4 a = make_float4(0.f, 0.f, 0.f, 0.f), b = a;
+                if ((int)rho < nrows) {
+                    size_t row;
+                    unsigned head;
+                    row_of(rho, row, head);
+                    const size_t at = row * A.q_stride + (size_t)head * HD + 64 * (i % G) + 16 * t4 + 8 * (i / G);
+                    a = kv8_load4(A.q, A.type, at);
+                    b = kv8_load4(A.q, A.type, at + 4);
+                }
+                x[i][0] = a.x; x[i][1] = a.y; x[i][2] = a.z; x[i][3] = a.w;
+                x[i][4] = b.x; x[i][5] = b.y; x[i][6] = b.z; x[i][7] = b.w;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) top = fmaxf(top, fabsf(x[i][j]));
+            }
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+            // largest magnitude to [2^12, 2^13): the low halves stay normal numbers of fp16
+            const int e = 12 - exponent_of(top);
+            const float up = power_of_two(min(e, 127)), up2 = power_of_two(e - min(e, 127));
+#pragma unroll
+            for (int i = 0; i < NW; ++i) {
+                __half h[8], l[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const float y = x[i][j] * up * up2;
+                    sum[i % G] += y;
+                    split_half(j & 1 ? y * 0.0625f : y, h[j], l[j]);
+                }
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    const unsigned h0 = pack(h[2 * j], h[2 * j + 4]), h1 = pack(h[2 * j + 1], h[2 * j + 5]);
+                    const unsigned l0 = pack(l[2 * j], l[2 * j + 4]), l1 = pack(l[2 * j + 1], l[2 * j + 5]);
+                    const bool low = W == 1 && (g & 1);
+                    qh[2 * i + j][0] = low ? l0 : h0;
+                    qh[2 * i + j][1] = low ? l1 : h1;
+                    if constexpr (LO) { ql[2 * i + j][0] = l0; ql[2 * i + j][1] = l1; }
+                }
+            }
+#pragma unroll
+            for (int h = 0; h < G; ++h) {
+                sum[h] += __shfl_xor_sync(0xffffffffu, sum[h], 1);
+                sum[h] += __shfl_xor_sync(0xffffffffu, sum[h], 2);
+            }
+#pragma unroll
+            for (int w = 0; w < W; ++w) {
+                // the lane group that holds query row W t4 + w as its column
+                const int from = (int)((W == 1 ? 2 * t4 : 2 * t4 + w) * 4);
+                const unsigned mine = W * t4 + w;
+                fn[w] = ldexpf(A.scale, -__shfl_sync(0xffffffffu, e, from));
+#pragma unroll
+                for (int h = 0; h < G; ++h) fq[w][h] = fn[w] * __shfl_sync(0xffffffffu, sum[h], from);
+                limit[w] = (int)mine < nrows ? s.q.len - s.q.n + j0 + (int)(mine / GR) + 1 : 0;
+            }
+        }
+        const int any = kv8_attended(A, s.q, s.row_tile);                   // positions some row attends
+        const int all = max(0, s.q.len - s.q.n + j0 + 1);                    // positions every row attends
+        float acc[G][4][4], m[W], l[W], zero[W][G], vref = 0.f;              // zero: sums of p low
+        int vexp = -200;  // v scales are relative to 2^vexp
+#pragma unroll
+        for (int h = 0; h < G; ++h)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) acc[h][k][0] = acc[h][k][1] = acc[h][k][2] = acc[h][k][3] = 0.f;
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+            m[w] = -3.4e38f;
+            l[w] = 0.f;
+#pragma unroll
+            for (int h = 0; h < G; ++h) zero[w][h] = 0.f;
+        }
+
+        for (int t = s.t0; t < s.t1; ++t) {
+            wait(full + stage, phase);
+            const unsigned char *tile = ring + stage * S::STAGE;
+            const unsigned loaded = here[stage];
+#pragma unroll 1
+            for (int u0 = 0; u0 < 2; u0 += J) {
+                // J groups of 16 positions at a time, from position `first`
+                const unsigned in_tile = (warp * 2 + (unsigned)u0) * 16, use = loaded >> (in_tile / 16) & ((1u << J) - 1);
+                const int first = t * K4_TILE + (int)in_tile;
+                if (first >= any || !use) continue;
+                // ---- scores
+                float c[J][G][4];
+#pragma unroll
+                for (int u = 0; u < J; ++u) {
+#pragma unroll
+                    for (int h = 0; h < G; ++h) c[u][h][0] = c[u][h][1] = c[u][h][2] = c[u][h][3] = 0.f;
+                    unsigned ka[NW], kb[NW];
+                    const unsigned pa = in_tile + 16 * u + tau;
+                    if constexpr (HD == 128) {
+                        const uint4 a = *reinterpret_cast<const uint4 *>(tile + swizzled(pa, 16 * t4));
+                        const uint4 b = *reinterpret_cast<const uint4 *>(tile + swizzled(pa + 8, 16 * t4));
+                        ka[0] = a.x; ka[1] = a.y; ka[2] = a.z; ka[3] = a.w;
+                        kb[0] = b.x; kb[1] = b.y; kb[2] = b.z; kb[3] = b.w;
+                    } else {
+                        const uint2 a = *reinterpret_cast<const uint2 *>(tile + swizzled(pa, 8 * t4));
+                        const uint2 b = *reinterpret_cast<const uint2 *>(tile + swizzled(pa + 8, 8 * t4));
+                        ka[0] = a.x; ka[1] = a.y;
+                        kb[0] = b.x; kb[1] = b.y;
+                    }
+#pragma unroll
+                    for (int i = 0; i < NW; ++i) {
+#pragma unroll
+                        for (int j = 0; j < 2; ++j) {
+                            const unsigned x = ka[i] >> (8 * j), y = kb[i] >> (8 * j);
+                            const unsigned a[4] = {x & 0x000f000fu, y & 0x000f000fu, x & 0x00f000f0u, y & 0x00f000f0u};
+                            mma_f16(c[u][i % G], a, qh[2 * i + j][0], qh[2 * i + j][1]);
+                            if constexpr (LO) mma_f16(c[u][i % G], a, ql[2 * i + j][0], ql[2 * i + j][1]);
+                        }
+                    }
+                }
+                // ---- scales and lows of this thread's positions; what is not attended may hold anything
+                float2 ks[J][2][G], vs[J][2][G];
+#pragma unroll
+                for (int u = 0; u < J; ++u)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const unsigned pos = in_tile + 16 * u + tau + 8 * h;
+                        unsigned kw[G], vw[G];
+                        if constexpr (G == 2) {
+                            const uint2 a = *reinterpret_cast<const uint2 *>(tile + S::OFF_KS + pos * 8);
+                            const uint2 b = *reinterpret_cast<const uint2 *>(tile + S::OFF_VS + pos * 8);
+                            kw[0] = a.x; kw[1] = a.y;
+                            vw[0] = b.x; vw[1] = b.y;
+                        } else {
+                            kw[0] = *reinterpret_cast<const unsigned *>(tile + S::OFF_KS + pos * 4);
+                            vw[0] = *reinterpret_cast<const unsigned *>(tile + S::OFF_VS + pos * 4);
+                        }
+#pragma unroll
+                        for (int i = 0; i < G; ++i) {
+                            ks[u][h][i] = __half22float2(*reinterpret_cast<const __half2 *>(&kw[i]));
+                            vs[u][h][i] = __half22float2(*reinterpret_cast<const __half2 *>(&vw[i]));
+                        }
+                    }
+                float x[J][2][W];  // [group of 16][position tau, tau + 8][row], in units of log2
+#pragma unroll
+                for (int u = 0; u < J; ++u)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+#pragma unroll
+                        for (int w = 0; w < W; ++w) {
+                            float dot = 0.f, low = 0.f;
+#pragma unroll
+                            for (int i = 0; i < G; ++i) {
+                                const float n = W == 1 ? c[u][i][2 * h] + c[u][i][2 * h + 1] : c[u][i][2 * h + w];
+                                dot = fmaf(n, ks[u][h][i].x, dot);
+                                low = fmaf(ks[u][h][i].y, fq[w][i], low);
+                            }
+                            x[u][h][w] = fmaf(dot * 16777216.f, fn[w], low);  // n was 2^24 too small
+                        }
+                if (first + 16 * J > all || use != (1u << J) - 1) {
+#pragma unroll
+                    for (int u = 0; u < J; ++u)
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            const int pos = first + 16 * u + (int)tau + 8 * h;
+                            const bool is = use >> u & 1;
+#pragma unroll
+                            for (int w = 0; w < W; ++w)
+                                if (pos >= limit[w] || !is) x[u][h][w] = -INFINITY;
+                            if (pos >= any || !is) {
+#pragma unroll
+                                for (int i = 0; i < G; ++i) vs[u][h][i] = make_float2(0.f, 0.f);
+                            }
+                        }
+                }
+                // ---- running maximum: moved only when a score is 2^8 above it. Their difference says so: it is exact
+                // where they are near, and m + 8 is not (from 2^27 on it can round to m + 16, a weight of 2^16)
+                bool over = false;
+                float top[W];
+#pragma unroll
+                for (int w = 0; w < W; ++w) {
+                    top[w] = fmaxf(x[0][0][w], x[0][1][w]);
+                    if constexpr (J == 2) top[w] = fmaxf(top[w], fmaxf(x[J - 1][0][w], x[J - 1][1][w]));
+                    over = over || top[w] - m[w] > 8.f;
+                }
+                if (__any_sync(0xffffffffu, over)) {
+#pragma unroll
+                    for (int w = 0; w < W; ++w) {
+#pragma unroll
+                        for (int o = 4; o < 32; o <<= 1) top[w] = fmaxf(top[w], __shfl_xor_sync(0xffffffffu, top[w], o));
+                        if (top[w] - m[w] > 8.f) {  // each row by its own scores: the same on all lanes that hold it
+                            const float alpha = ex2(m[w] - top[w]);
+                            m[w] = top[w];
+                            l[w] *= alpha;
+#pragma unroll
+                            for (int h = 0; h < G; ++h) {
+                                zero[w][h] *= alpha;
+#pragma unroll
+                                for (int k = 0; k < 4; ++k) {
+                                    if constexpr (W == 1) { acc[h][k][0] *= alpha; acc[h][k][1] *= alpha; acc[h][k][2] *= alpha; acc[h][k][3] *= alpha; }
+                                    else { acc[h][k][w] *= alpha; acc[h][k][2 + w] *= alpha; }
+                                }
+                            }
+                        }
+                    }
+                }
+                // ---- value scales relative to the largest power of two so far (they are not negative: ordered as integers)
+                float most = 0.f;
+#pragma unroll
+                for (int u = 0; u < J; ++u)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+#pragma unroll
+                        for (int i = 0; i < G; ++i) most = fmaxf(most, vs[u][h][i].x);
+                most = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(most)));
+                const int e = exponent_of(most) + 1;
+                if (e > vexp && most > 0.f) {
+                    const float down = vexp < -126 ? 0.f : power_of_two(vexp - e);
+#pragma unroll
+                    for (int h = 0; h < G; ++h)
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) { acc[h][k][0] *= down; acc[h][k][1] *= down; acc[h][k][2] *= down; acc[h][k][3] *= down; }
+                    vexp = e;
+                    vref = power_of_two(-e) * P_SCALE;
+                }
+                // ---- weights and values
+#pragma unroll
+                for (int u = 0; u < J; ++u) {
+                    unsigned b[G][2], bl[G][2];
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        float p[W];
+#pragma unroll
+                        for (int w = 0; w < W; ++w) {
+                            p[w] = ex2(x[u][h][w] - m[w]);
+                            l[w] += p[w];
+                        }
+#pragma unroll
+                        for (int i = 0; i < G; ++i) {
+                            __half ph[W], pl[W];
+                            const float unit = vs[u][h][i].x * vref;
+#pragma unroll
+                            for (int w = 0; w < W; ++w) {
+                                zero[w][i] = fmaf(p[w], vs[u][h][i].y, zero[w][i]);
+                                split_half(p[w] * unit, ph[w], pl[w]);
+                            }
+                            if constexpr (W == 1) b[i][h] = movmatrix(pack(ph[0], pl[0]));
+                            else {
+                                b[i][h] = movmatrix(pack(ph[0], ph[1]));
+                                if constexpr (LO) bl[i][h] = movmatrix(pack(pl[0], pl[1]));
+                            }
+                        }
+                    }
+                    unsigned v[4][G];  // eight numbers of each group of positions ta, ta ^ X, and both + 8
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const unsigned pos = in_tile + 16 * u + ((i & 1 ? ta ^ X : ta) + (i & 2 ? 8 : 0));
+                        if constexpr (G == 2) {
+                            const uint2 y = *reinterpret_cast<const uint2 *>(tile + S::OFF_V + swizzled(pos, 8 * g));
+                            v[i][0] = y.x;
+                            v[i][1] = y.y;
+                        } else {
+                            v[i][0] = *reinterpret_cast<const unsigned *>(tile + S::OFF_V + swizzled(pos, 4 * g));
+                        }
+                    }
+#pragma unroll
+                    for (int i = 0; i < G; ++i)
+#pragma unroll
+                        for (int half = 0; half < 2; ++half) {
+                            const unsigned ab = __byte_perm(v[0][i], v[1][i], half ? 0x7632 : 0x5410);
+                            const unsigned cd = __byte_perm(v[2][i], v[3][i], half ? 0x7632 : 0x5410);
+#pragma unroll
+                            for (int j = 0; j < 2; ++j) {
+                                const unsigned y = ab >> (8 * j), z = cd >> (8 * j);
+                                const unsigned a[4] = {y & 0x000f000fu, y & 0x00f000f0u, z & 0x000f000fu, z & 0x00f000f0u};
+                                mma_f16(acc[i][2 * half + j], a, b[i][0], b[i][1]);
+                                if constexpr (LO) mma_f16(acc[i][2 * half + j], a, bl[i][0], bl[i][1]);
+                            }
+                        }
+                }
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(empty + stage);
+            advance();
+        }
+        // ---- the four warps' parts: sums over the lanes of a row, then over the warps
+        const float back = vexp < -126 ? 0.f : power_of_two(vexp) * (16777216.f / P_SCALE);
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+#pragma unroll
+            for (int o = 4; o < 32; o <<= 1) {
+                l[w] += __shfl_xor_sync(0xffffffffu, l[w], o);
+#pragma unroll
+                for (int h = 0; h < G; ++h) zero[w][h] += __shfl_xor_sync(0xffffffffu, zero[w][h], o);
+            }
+            if (g == 0) ml_s[warp * R + W * t4 + w] = make_float2(m[w], l[w]);
+        }
+#pragma unroll
+        for (int h = 0; h < G; ++h)
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+#pragma unroll
+                for (int w = 0; w < W; ++w) {
+                    const float even = W == 1 ? acc[h][k][0] + acc[h][k][1] : acc[h][k][w];
+                    const float odd = W == 1 ? acc[h][k][2] + acc[h][k][3] : acc[h][k][2 + w];
+                    *reinterpret_cast<float2 *>(o_s + (warp * R + W * t4 + w) * HD + 64 * h + 8 * g + 2 * k) =
+                        make_float2(fmaf(even, back, zero[w][h]), fmaf(odd, back * 0.0625f, zero[w][h]));
+                }
+        bar();
+        kv8_join_warps<R, HD, K4_WARPS>(tid, ml_s, o_s, bar);
+        kv8_finish<R, HD, 32 * K4_WARPS>(A, s, place, tid, ml_s, o_s, (unsigned)nrows, o_s + R * HD,
+            (K4_WARPS - 1) * R * HD, flag, bar, [&](unsigned rho, unsigned chunk, float4 v) {
+                size_t row;
+                unsigned head;
+                row_of(rho, row, head);
+                kv8_store4(A.out, A.type, row * A.out_stride + (size_t)head * HD + 4 * chunk, v);
+            });
+        bar();
+    }
+}
+
+template <int HD, int W, bool LO> static int decode_launch(const Kv4Attention &A, const CUtensorMap &k, const CUtensorMap &v,
+    unsigned grid, cudaStream_t s)
+{
+    using S = K4Shape<HD>;
+    constexpr int R = 4 * W;
+    constexpr size_t smem = 1024 + (size_t)S::STAGES * S::STAGE + K4_WARPS * R * HD * 4 + K4_WARPS * R * 8 + S::STAGES * 20 + 16;
+    static_assert(smem <= 75 * 1024, "three CTAs per SM");
+    static std::atomic<unsigned> allowed{0};
+    if (allow_shared((const void *)kv4_decode_kernel<HD, W, LO>, smem, allowed)) return -2;
+    kv4_decode_kernel<HD, W, LO><<<grid, K4_THREADS, smem, s>>>(A, k, v);
+    return cudaGetLastError() == cudaSuccess ? 0 : -2;
+}
+
+template <int HD> static int decode_rows(const Kv4Attention &A, const CUtensorMap &k, const CUtensorMap &v, unsigned grid, cudaStream_t s)
+{
+    if (A.max_rows * A.group <= 4) return decode_launch<HD, 1, false>(A, k, v, grid, s);
+    return A.type == T_F32 ? decode_launch<HD, 2, true>(A, k, v, grid, s) : decode_launch<HD, 2, false>(A, k, v, grid, s);
+}
+
+int launch_kv4_decode(const Kv4Attention &A, const CUtensorMap &k, const CUtensorMap &v, unsigned grid, cudaStream_t s)
+{
+    return A.c.head_dim == 128 ? decode_rows<128>(A, k, v, grid, s) : decode_rows<64>(A, k, v, grid, s);
+}
+
+}  // namespace fyb

@@ -22,7 +22,7 @@ TilesLaunch kv8_tiles_128_0, kv8_tiles_128_1, kv8_tiles_64_0, kv8_tiles_64_1;
 
 constexpr unsigned KT_GRID = 148, KT_ROWS = 64;  // one CTA per SM; most query rows of a row tile
 
-int kv8_tensor_map(CUtensorMap *map, const fyb_kv8_cache &c, const void *pool)
+int kv8_tensor_map(CUtensorMap *map, const void *pool, unsigned row_bytes, size_t rows, unsigned box_rows, CUtensorMapSwizzle swizzle)
 {
     using Encode = decltype(&cuTensorMapEncodeTiled);
     static const Encode encode = [] {
@@ -36,11 +36,16 @@ int kv8_tensor_map(CUtensorMap *map, const fyb_kv8_cache &c, const void *pool)
         return (Encode)f;
     }();
     if (!encode) return -2;
-    const cuuint64_t dims[2] = {c.head_dim, (cuuint64_t)c.blocks * c.kv_heads * c.block_size}, strides[1] = {c.head_dim};
-    const cuuint32_t box[2] = {c.head_dim, std::min(c.block_size, 64u)}, step[2] = {1, 1};
+    const cuuint64_t dims[2] = {row_bytes, rows}, strides[1] = {row_bytes};
+    const cuuint32_t box[2] = {row_bytes, box_rows}, step[2] = {1, 1};
     return encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void *>(pool), dims, strides, box, step,
-                  CU_TENSOR_MAP_INTERLEAVE_NONE, c.head_dim == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
-                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS ? 0 : -2;
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS ? 0 : -2;
+}
+int kv8_tensor_map(CUtensorMap *map, const fyb_kv8_cache &c, const void *pool)
+{
+    return kv8_tensor_map(map, pool, c.head_dim, (size_t)c.blocks * c.kv_heads * c.block_size, std::min(c.block_size, 64u),
+                          c.head_dim == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B);
 }
 
 // Partials of a call: two per CTA of its kernel, `rows` query rows each.

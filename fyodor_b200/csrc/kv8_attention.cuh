@@ -1,6 +1,7 @@
-// kv8_attention.cuh - how the attention over the paged 8-bit cache is split
-// over the GPU, shared by its two kernels (kv8_decode.cu: few query rows
-// per KV head, kv8_tiles.cuh: many).
+// kv8_attention.cuh - how the attention over the paged caches is split over the
+// GPU, shared by the kernels of the 8-bit cache (kv8_decode.cu: few query rows
+// per KV head, kv8_tiles.cuh: many) and of the 4-bit cache (kv4_decode.cu,
+// kv4_tiles.cuh).
 //
 // Work is a line of units. A segment is the cache that one row tile of one
 // request attends in one KV head, a unit TILE positions of it. CTA c of C takes
@@ -361,6 +362,8 @@ FYB_DEV void kv8_store4(void *p, unsigned type, size_t at, float4 v)
 // row t lies at chunk c ^ (t & 7) (128-byte rows) or c ^ (t >> 1 & 3) (64-byte
 // rows), so eight token rows of one chunk are read without bank conflicts.
 int kv8_tensor_map(CUtensorMap *map, const fyb_kv8_cache &c, const void *pool);
+// Any pool of `rows` rows of row_bytes bytes, boxes of box_rows rows.
+int kv8_tensor_map(CUtensorMap *map, const void *pool, unsigned row_bytes, size_t rows, unsigned box_rows, CUtensorMapSwizzle swizzle);
 FYB_DEV void tma_load_rows(void *dst, const CUtensorMap *map, int row, uint64_t *bar)
 {
     asm volatile(
@@ -378,6 +381,67 @@ FYB_DEV float ex2(float x)
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
+}
+
+FYB_DEV void mma_f16(float (&d)[4], const unsigned (&a)[4], unsigned b0, unsigned b1)
+{
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+FYB_DEV unsigned movmatrix(unsigned x)
+{
+    unsigned y;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+// hi = fp16(w), lo = fp16(w - hi)
+FYB_DEV void split_half(float w, __half &hi, __half &lo)
+{
+    hi = __float2half_rn(w);
+    lo = __float2half_rn(w - __half2float(hi));
+}
+FYB_DEV unsigned pack(__half lo, __half hi)
+{
+    const __half2 p = __halves2half2(lo, hi);
+    return *reinterpret_cast<const unsigned *>(&p);
+}
+// 2^-(exponent of x) and its inverse for a positive finite x (1 for 0).
+FYB_DEV int exponent_of(float x) { return x > 0.f ? max(-126, (int)(__float_as_uint(x) >> 23) - 127) : 0; }
+FYB_DEV float power_of_two(int e) { return e < -126 ? __uint_as_float(1u << max(0, e + 149)) : __uint_as_float((unsigned)(min(e, 127) + 127) << 23); }
+
+// The parts that the warps of a CTA hold of R rows, ml_s[WARPS][R] (maximum, sum) and o_s[WARPS][R][HD], joined into
+// those of warp 0. The 32 WARPS threads call it behind a barrier; bar(): a barrier over them.
+template <int R, int HD, int WARPS, typename Bar> FYB_DEV void kv8_join_warps(unsigned tid, float2 *ml_s, float *o_s, Bar bar)
+{
+    constexpr unsigned THREADS = 32 * WARPS, STEPS = (R * HD / 4 + THREADS - 1) / THREADS;
+    float2 joined[STEPS];
+#pragma unroll
+    for (unsigned i = 0; i < STEPS; ++i) {
+        const unsigned at = tid + THREADS * i, row = at / (HD / 4);
+        if (at >= R * HD / 4) break;
+        float mm = ml_s[row].x, ll = 0.f;
+#pragma unroll
+        for (int w = 1; w < WARPS; ++w) mm = fmaxf(mm, ml_s[w * R + row].x);
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int w = 0; w < WARPS; ++w) {
+            const float f = ex2(ml_s[w * R + row].x - mm);
+            const float4 y = reinterpret_cast<const float4 *>(o_s)[w * R * HD / 4 + at];
+            ll = fmaf(ml_s[w * R + row].y, f, ll);
+            v.x = fmaf(y.x, f, v.x); v.y = fmaf(y.y, f, v.y); v.z = fmaf(y.z, f, v.z); v.w = fmaf(y.w, f, v.w);
+        }
+        reinterpret_cast<float4 *>(o_s)[at] = v;  // this thread alone reads and writes element `at` of warp 0's part
+        joined[i] = make_float2(mm, ll);
+    }
+    bar();
+#pragma unroll
+    for (unsigned i = 0; i < STEPS; ++i) {
+        const unsigned at = tid + THREADS * i;
+        if (at < R * HD / 4 && at % (HD / 4) == 0) ml_s[at / (HD / 4)] = joined[i];
+    }
+    bar();
 }
 
 // Four stored bytes as two fp16 pairs (bytes 0, 1 and 2, 3), exactly.

@@ -29,13 +29,6 @@ template <int HD, int W> struct KdShape {
 };
 struct KdMeta { float ks[KD_TILE / 16], vs[KD_TILE / 16]; };   // scales of the tile's blocks; ks NaN: block not loaded
 
-FYB_DEV void mma_f16(float (&d)[4], const unsigned (&a)[4], unsigned b0, unsigned b1)
-{
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
 // Two 16 x 16 byte matrices (row addresses from lanes 0..15 and 16..31),
 // transposed: lane 4g + t gets column g (r0, r2) and g + 8 (r1, r3) of rows 4t..4t+3.
 FYB_DEV void ldmatrix_trans_b8(unsigned (&r)[4], unsigned addr)
@@ -48,27 +41,6 @@ FYB_DEV void ldmatrix_b16(unsigned (&r)[4], unsigned addr)
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
 }
-FYB_DEV unsigned movmatrix(unsigned x)
-{
-    unsigned y;
-    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
-    return y;
-}
-// hi = fp16(w), lo = fp16(w - hi)
-FYB_DEV void split_half(float w, __half &hi, __half &lo)
-{
-    hi = __float2half_rn(w);
-    lo = __float2half_rn(w - __half2float(hi));
-}
-FYB_DEV unsigned pack(__half lo, __half hi)
-{
-    const __half2 p = __halves2half2(lo, hi);
-    return *reinterpret_cast<const unsigned *>(&p);
-}
-// 2^-(exponent of x) and its inverse for a positive finite x (1 for 0).
-FYB_DEV int exponent_of(float x) { return x > 0.f ? max(-126, (int)(__float_as_uint(x) >> 23) - 127) : 0; }
-FYB_DEV float power_of_two(int e) { return e < -126 ? __uint_as_float(1u << max(0, e + 149)) : __uint_as_float((unsigned)(min(e, 127) + 127) << 23); }
-
 // W: rows a thread holds scores of (1: up to four query rows, 2: up to eight).
 // QL: whether q has low halves of its own (F32 rows at W = 2; 16-bit rows fit
 // the high half, and at W = 1 the low halves are columns that cost nothing).
@@ -375,32 +347,7 @@ __global__ void __launch_bounds__(KD_THREADS, 3) kv8_decode_kernel(const __grid_
             }
         }
         bar();
-        float2 joined[(R * HD / 4 + 127) / 128];
-#pragma unroll
-        for (int i = 0; i < (R * HD / 4 + 127) / 128; ++i) {
-            const unsigned at = tid + 128 * i, row = at / (HD / 4);
-            if (at >= R * HD / 4) break;
-            float mm = ml_s[row].x, ll = 0.f;
-#pragma unroll
-            for (int w = 1; w < KD_WARPS; ++w) mm = fmaxf(mm, ml_s[w * R + row].x);
-            float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-            for (int w = 0; w < KD_WARPS; ++w) {
-                const float f = ex2(ml_s[w * R + row].x - mm);
-                const float4 y = reinterpret_cast<const float4 *>(o_s)[w * R * HD / 4 + at];
-                ll = fmaf(ml_s[w * R + row].y, f, ll);
-                v.x = fmaf(y.x, f, v.x); v.y = fmaf(y.y, f, v.y); v.z = fmaf(y.z, f, v.z); v.w = fmaf(y.w, f, v.w);
-            }
-            reinterpret_cast<float4 *>(o_s)[at] = v;  // this thread alone reads and writes element `at` of warp 0's part
-            joined[i] = make_float2(mm, ll);
-        }
-        bar();
-#pragma unroll
-        for (int i = 0; i < (R * HD / 4 + 127) / 128; ++i) {
-            const unsigned at = tid + 128 * i;
-            if (at < R * HD / 4 && at % (HD / 4) == 0) ml_s[at / (HD / 4)] = joined[i];
-        }
-        bar();
+        kv8_join_warps<R, HD, KD_WARPS>(tid, ml_s, o_s, bar);
         kv8_finish<R, HD, 32 * KD_WARPS>(A, s, place, tid, ml_s, o_s, (unsigned)nrows, o_s + R * HD,
             (KD_WARPS - 1) * R * HD, flag, bar, [&](unsigned rho, unsigned chunk, float4 v) {
                 size_t row;
