@@ -34,13 +34,15 @@ def _nvcc():
 
 # Sources compiled once per variant (object suffix, extra flags): each
 # instantiation of the persistent decode kernel, and each head dimension and
-# format of the many-row attention over the 8-bit cache, is its own
-# compilation, so they run in parallel.
+# format (8-bit cache) or row tile (4-bit cache) of the many-row attention, is
+# its own compilation, so they run in parallel.
 VARIANTS = {
     "decode_inst.cu": [("%d_%d" % (hd, g), ["-DFYB_DK_HD=%d" % hd, "-DFYB_DK_G=%d" % g])
                        for hd in (128, 64) for g in (1, 2, 4, 8)],
     "kv8_tiles_inst.cu": [("%d_%d" % (hd, f), ["-DFYB_KT_HD=%d" % hd, "-DFYB_KT_FMT=%d" % f])
                           for hd in (128, 64) for f in (0, 1)],
+    "kv4_tiles_inst.cu": [("%d_%d" % (hd, n), ["-DFYB_K4_HD=%d" % hd, "-DFYB_K4_NR=%d" % n])
+                          for hd in (128, 64) for n in (32, 64, 128)],
 }
 
 

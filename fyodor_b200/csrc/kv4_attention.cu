@@ -1,81 +1,33 @@
 // kv4_attention.cu - the entry point of attention over the paged 4-bit cache:
-// argument checks, the workspace, and which kernel runs. Up to eight query rows
-// per KV head run on kv4_decode.cu.
+// argument checks, the workspace, and which kernel runs.
 //
-// Many rows: a warp takes one query row of one head and walks the positions it attends:
-// lanes share out the head's dimensions, and of a group the score is scale (q . n)
-// + low sum(q), so the held numbers are used as they lie.
+// Up to eight query rows per KV head (rows of a request x heads of a group), and
+// rows of F32 whatever their number, run on kv4_decode.cu, many rows in row tiles of
+// eight; many rows of 16 bits on kv4_tiles.cuh, in row tiles of 32, 64 or 128.
 #include "kv4_attention.cuh"
 
 namespace fyb {
 
-constexpr int K4_WARPS = 8;
+using TilesLaunch = int(const Kv4Attention &, const CUtensorMap &, const CUtensorMap &, unsigned, cudaStream_t);
+TilesLaunch kv4_tiles_128_32, kv4_tiles_128_64, kv4_tiles_128_128, kv4_tiles_64_32, kv4_tiles_64_64, kv4_tiles_64_128;
+
+constexpr unsigned K4T_GRID = 148;  // one CTA per SM
 
 // K or V as token rows of head_dim / 2 bytes, boxes of one block (128 rows at most), rows of 64 bytes in the swizzle of
 // 64 bytes: 16-byte chunk c of token row t lies at chunk c ^ (t >> 1 & 3).
-static int kv4_tensor_map(CUtensorMap *map, const fyb_kv8_cache &c, const void *pool)
+static int kv4_tensor_map(CUtensorMap *map, const fyb_kv4_cache &c, const void *pool)
 {
     return kv8_tensor_map(map, pool, c.head_dim / 2, (size_t)c.blocks * c.kv_heads * c.block_size,
                           std::min(c.block_size, (unsigned)K4_TILE), c.head_dim == 128 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_NONE);
 }
 
-// Lane's 16 bits of a token's row (HD 128: four values, HD 64: two, 8 bits) from its first dimension.
-template <typename T, int HD> __global__ void __launch_bounds__(32 * K4_WARPS) kv4_rows_kernel(const __grid_constant__ Kv4Attention A)
+// Row tile of the many-row kernel.
+static unsigned tile_rows(unsigned long long group_rows) { return group_rows <= 32 ? 32 : group_rows <= 64 ? 64 : 128; }
+// Query rows of a call's partials, two for each CTA of its kernel (F32 rows need 2 KA_GRID of eight: fewer than tiles do).
+static size_t part_rows(unsigned long long group_rows)
 {
-    constexpr int E = HD / 32, GROUPS = HD / 64;
-    const unsigned lane = threadIdx.x & 31, kv = A.c.kv_heads, size = 1u << A.shift;
-    const size_t item = (size_t)blockIdx.x * K4_WARPS + (threadIdx.x >> 5);
-    if (item >= (size_t)A.rows * A.heads) return;
-    const unsigned row = (unsigned)(item / A.heads), head = (unsigned)(item % A.heads), kvh = head / A.group;
-    // the request of the row
-    unsigned r = row;
-    Kv8Request q = kv8_request(A, 0, item == 0);
-    if (A.row_start) {
-        for (r = 0; r < A.requests; ++r) {
-            q = kv8_request(A, r, lane == 0 && head == 0 && (int)row == max(0, A.row_start[r]));
-            if ((int)row >= q.first && (int)row < q.first + q.n) break;
-        }
-        if (r == A.requests || (int)row >= q.first + q.rows) return;
-    } else {
-        q = kv8_request(A, r, lane == 0 && head == 0);
-    }
-    const int last = q.len - q.n + ((int)row - q.first) + 1;
-    const unsigned e = lane * E, group = e / 64, word = HD == 64 ? e / 8 : (e % 64 / 8) * 2 + group;
-    const T *qp = static_cast<const T *>(A.q) + row * A.q_stride + (size_t)head * HD + e;
-    float x[E], sum = 0.f, o[E] = {}, m = -INFINITY, l = 0.f;
-#pragma unroll
-    for (int i = 0; i < E; ++i) { x[i] = row_value(qp[i]); sum += x[i]; }
-    for (int t = 0; t < last; ++t) {
-        const int id = A.table[(size_t)r * A.table_stride + (t >> A.shift)];
-        if ((unsigned)id >= A.c.blocks) {
-            if (lane == 0 && kvh * A.group == head) raise_error(A.error, ERR_BOUNDS);
-            t |= (int)size - 1;
-            continue;
-        }
-        const size_t at = ((size_t)id * kv + kvh) * size + ((unsigned)t & (size - 1));
-        const unsigned kw = static_cast<const unsigned *>(A.c.k)[at * (HD / 8) + word] >> (e % 8 * 4);
-        const unsigned vw = static_cast<const unsigned *>(A.c.v)[at * (HD / 8) + word] >> (e % 8 * 4);
-        const float2 ks = __half22float2(A.ks[at * GROUPS + group]), vs = __half22float2(A.vs[at * GROUPS + group]);
-        float dot = 0.f;
-#pragma unroll
-        for (int i = 0; i < E; ++i) dot = fmaf(x[i], (float)(kw >> (4 * i) & 15u), dot);
-        const float score = warp_sum(fmaf(dot, ks.x, sum * ks.y)) * A.scale;
-        const float top = fmaxf(m, score), keep = m == top ? 1.f : exp2f(m - top), p = exp2f(score - top);
-        m = top;
-        l = fmaf(l, keep, p);
-#pragma unroll
-        for (int i = 0; i < E; ++i) o[i] = fmaf(o[i], keep, p * fmaf((float)(vw >> (4 * i) & 15u), vs.x, vs.y));
-    }
-    const float n = l > 0.f || isnan(l) ? 1.f / l : 0.f;
-    T *out = static_cast<T *>(A.out) + row * A.out_stride + (size_t)head * HD + e;
-#pragma unroll
-    for (int i = 0; i < E; ++i) out[i] = row_round<T>(o[i] * n);
-}
-
-template <typename T> static void rows_launch(const Kv4Attention &A, unsigned grid, cudaStream_t s)
-{
-    if (A.c.head_dim == 128) kv4_rows_kernel<T, 128><<<grid, 32 * K4_WARPS, 0, s>>>(A);
-    else kv4_rows_kernel<T, 64><<<grid, 32 * K4_WARPS, 0, s>>>(A);
+    static_assert(2 * KA_GRID * KV8_DECODE_ROWS <= 2 * K4T_GRID * 32, "");
+    return group_rows <= KV8_DECODE_ROWS ? 2 * KA_GRID * KV8_DECODE_ROWS : 2 * K4T_GRID * tile_rows(group_rows);
 }
 
 }  // namespace fyb
@@ -85,7 +37,10 @@ using namespace fyb;
 extern "C" size_t fyb_kv4_attention_workspace(uint32_t requests, uint32_t max_rows, uint32_t heads, uint32_t kv_heads,
     uint32_t head_dim)
 {
-    return fyb_kv8_attention_workspace(requests, max_rows, heads, kv_heads, head_dim);
+    if (!requests || !max_rows || !kv_heads || heads < kv_heads || heads % kv_heads || heads / kv_heads > 64 ||
+        (head_dim != 64 && head_dim != 128))
+        return 0;
+    return KA_COUNTER_BYTES + part_rows((unsigned long long)max_rows * (heads / kv_heads)) * (head_dim + 2) * sizeof(float);
 }
 
 extern "C" int fyb_kv4_attention(const fyb_kv4_cache *cache, const int32_t *lengths, const int32_t *row_start,
@@ -103,32 +58,40 @@ extern "C" int fyb_kv4_attention(const fyb_kv4_cache *cache, const int32_t *leng
         return -1;
     if (!rows) return 0;
     Kv4Attention A{};
-    A.c.k = cache->k; A.c.v = cache->v;
     A.c.blocks = cache->blocks; A.c.kv_heads = cache->kv_heads; A.c.block_size = cache->block_size;
     A.c.head_dim = cache->head_dim;
     A.ks = static_cast<const __half2 *>(cache->k_scale); A.vs = static_cast<const __half2 *>(cache->v_scale);
     A.lengths = lengths; A.row_start = row_start; A.table = table; A.table_stride = table_stride;
     A.rows = (unsigned)rows; A.q = q; A.q_stride = q_stride; A.out = out; A.out_stride = out_stride;
-    A.requests = requests; A.max_rows = max_rows; A.heads = heads; A.group = heads / cache->kv_heads;
+    A.requests = requests; A.max_rows = max_rows; A.heads = heads; A.group = heads / cache->kv_heads; A.split = 1;
     A.shift = kv4_shift(cache); A.type = type; A.scale = scale * 1.44269504f; A.error = error;
-    cudaStream_t s = (cudaStream_t)stream;
+    const unsigned long long group_rows = (unsigned long long)max_rows * A.group;
     unsigned char *ws = static_cast<unsigned char *>(workspace);
     A.counters = reinterpret_cast<unsigned *>(ws);
     A.part_ml = reinterpret_cast<float2 *>(ws + KA_COUNTER_BYTES);
-    A.part_o = reinterpret_cast<float *>(A.part_ml + 2 * KA_GRID * KV8_DECODE_ROWS);
-    if ((unsigned long long)max_rows * A.group <= KV8_DECODE_ROWS) {
-        CUtensorMap k, v;
-        if (kv4_tensor_map(&k, A.c, A.c.k) || kv4_tensor_map(&v, A.c, A.c.v)) return -2;
-        A.row_tile = max_rows;
-        // no more CTAs than the most units the tables can hold
-        const unsigned long long holds = (unsigned long long)table_stride << A.shift;
-        const unsigned long long units = (holds + K4_TILE - 1) / K4_TILE * requests * cache->kv_heads;
+    A.part_o = reinterpret_cast<float *>(A.part_ml + part_rows(group_rows));
+    CUtensorMap k, v;
+    if (kv4_tensor_map(&k, *cache, cache->k) || kv4_tensor_map(&v, *cache, cache->v)) return -2;
+    // no more CTAs than the most units the tables can hold
+    const unsigned long long holds = (unsigned long long)table_stride << A.shift;
+    const unsigned long long tiles = std::min<unsigned long long>((holds + K4_TILE - 1) / K4_TILE * requests, 1u << 20);
+    cudaStream_t s = (cudaStream_t)stream;
+    if (group_rows <= KV8_DECODE_ROWS || type == T_F32) {
+        // more heads than a row tile holds: parts of a group, each as a KV head of its own over the same cache
+        while (A.group > KV8_DECODE_ROWS || cache->kv_heads * A.split * A.group != heads) {
+            ++A.split;
+            A.group = heads / cache->kv_heads / A.split;
+        }
+        A.c.kv_heads = cache->kv_heads * A.split;
+        A.row_tile = std::min(max_rows, KV8_DECODE_ROWS / A.group);
+        const unsigned long long units = tiles * A.c.kv_heads * std::min<unsigned long long>((max_rows + A.row_tile - 1) / A.row_tile, 1u << 20);
         return launch_kv4_decode(A, k, v, (unsigned)std::min<unsigned long long>(KA_GRID, units), s);
     }
-    const size_t grid = (rows * heads + K4_WARPS - 1) / K4_WARPS;
-    if (grid > 0x7fffffffu) return -1;
-    if (type == T_F32) rows_launch<float>(A, (unsigned)grid, s);
-    else if (type == T_F16) rows_launch<__half>(A, (unsigned)grid, s);
-    else rows_launch<__nv_bfloat16>(A, (unsigned)grid, s);
-    return cudaGetLastError() == cudaSuccess ? 0 : -2;
+    const unsigned n = tile_rows(group_rows);
+    A.row_tile = n / A.group;
+    const unsigned long long units = tiles * A.c.kv_heads * std::min<unsigned long long>((max_rows + A.row_tile - 1) / A.row_tile, 1u << 20);
+    const unsigned grid = (unsigned)std::min<unsigned long long>(K4T_GRID, units);
+    TilesLaunch *go = cache->head_dim == 128 ? (n == 32 ? kv4_tiles_128_32 : n == 64 ? kv4_tiles_128_64 : kv4_tiles_128_128)
+                                             : (n == 32 ? kv4_tiles_64_32 : n == 64 ? kv4_tiles_64_64 : kv4_tiles_64_128);
+    return go(A, k, v, grid, s);
 }

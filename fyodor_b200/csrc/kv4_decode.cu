@@ -45,7 +45,7 @@ __global__ void __launch_bounds__(K4_THREADS, 3) kv4_decode_kernel(const __grid_
     unsigned *here = reinterpret_cast<unsigned *>(empty + S::STAGES);       // [stages] which groups of 16 positions are loaded
     unsigned *flag = here + S::STAGES;
     volatile unsigned *dead = flag + 1;   // a wait ran out: nobody waits any more, the error word is set
-    const unsigned tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, kv = A.c.kv_heads;
+    const unsigned tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, kv = A.c.kv_heads / A.split;
     if (tid == 0) {
         for (int i = 0; i < S::STAGES; ++i) { mbar_init(full + i, 1); mbar_init(empty + i, K4_WARPS); }
         *dead = 0;
@@ -93,7 +93,7 @@ __global__ void __launch_bounds__(K4_THREADS, 3) kv4_decode_kernel(const __grid_
                 }
                 __syncwarp();
                 if (load && !*dead) {
-                    const unsigned row = (((unsigned)mine * kv + s.head) << A.shift) + ((unsigned)(t * K4_TILE) & (size - 1));
+                    const unsigned row = (((unsigned)mine * kv + s.head / A.split) << A.shift) + ((unsigned)(t * K4_TILE) & (size - 1));
                     unsigned char *dst = ring + stage * S::STAGE;
                     tma_load_rows(dst + lane * box * S::ROW, &kmap, (int)row, full + stage);
                     tma_load_rows(dst + S::OFF_V + lane * box * S::ROW, &vmap, (int)row, full + stage);
@@ -466,7 +466,7 @@ template <int HD, int W, bool LO> static int decode_launch(const Kv4Attention &A
 
 template <int HD> static int decode_rows(const Kv4Attention &A, const CUtensorMap &k, const CUtensorMap &v, unsigned grid, cudaStream_t s)
 {
-    if (A.max_rows * A.group <= 4) return decode_launch<HD, 1, false>(A, k, v, grid, s);
+    if (A.row_tile * A.group <= 4) return decode_launch<HD, 1, false>(A, k, v, grid, s);
     return A.type == T_F32 ? decode_launch<HD, 2, true>(A, k, v, grid, s) : decode_launch<HD, 2, false>(A, k, v, grid, s);
 }
 

@@ -242,31 +242,26 @@ template <int G> FYB_DEV float group_sum(float x)
 }
 
 // ---- joining the parts of a segment -------------------------------------------
-// `threads` threads hold the segment's part as ml[R] and o[R][HD] in shared
-// memory; bar(): a barrier over them. Writes the rows out when the CTA has the
-// whole segment; otherwise leaves a partial, and the last CTA to do so joins
-// all parts. valid(row, &src): whether row is a query row, and which.
-template <int R, int HD, int THREADS, typename Bar, typename Put>
-FYB_DEV void kv8_finish(const Kv8Attention &A, const Kv8Segment &s, const Kv8Place &place, unsigned tid, const float2 *ml,
-    const float *o, unsigned rows, float *weights, unsigned max_weights, unsigned *flag, Bar bar, Put put)
+// A CTA that has not the whole of a segment leaves a partial; the last CTA to do so joins all of them.
+struct Kv8Parts {
+    unsigned first, last, slot;  // CTAs that share the segment; this CTA's partial
+};
+FYB_DEV Kv8Parts kv8_parts(const Kv8Segment &s, const Kv8Place &place)
 {
-    if (s.t0 == 0 && s.t1 == s.tiles) {
-        for (unsigned i = tid; i < rows * (HD / 4); i += THREADS) {
-            const unsigned row = i / (HD / 4);
-            float4 v = reinterpret_cast<const float4 *>(o)[i];
-            const float l = ml[row].y, n = l > 0.f || isnan(l) ? 1.f / l : 0.f;
-            v.x *= n; v.y *= n; v.z *= n; v.w *= n;
-            put(row, i % (HD / 4), v);
-        }
-        return;
-    }
-    const unsigned c0 = kv8_cta_of(place.units, place.ctas, s.first_unit);
-    const unsigned c1 = kv8_cta_of(place.units, place.ctas, s.first_unit + (unsigned)s.tiles - 1);
+    Kv8Parts p;
+    p.first = kv8_cta_of(place.units, place.ctas, s.first_unit);
+    p.last = kv8_cta_of(place.units, place.ctas, s.first_unit + (unsigned)s.tiles - 1);
     // the segment that ends a CTA's range goes to its second slot, any other to its first
-    const unsigned slot = 2 * blockIdx.x + (blockIdx.x == c0 ? 1 : 0);
-    for (unsigned i = tid; i < rows * (HD / 4); i += THREADS)
-        reinterpret_cast<float4 *>(A.part_o + (size_t)slot * R * HD)[i] = reinterpret_cast<const float4 *>(o)[i];
-    for (unsigned i = tid; i < rows; i += THREADS) A.part_ml[(size_t)slot * R + i] = ml[i];
+    p.slot = 2 * blockIdx.x + (blockIdx.x == p.first ? 1 : 0);
+    return p;
+}
+// THREADS threads call it once the CTA's partial (of `rows` of R rows) is written: the last CTA of the segment puts the
+// joined rows out. bar(): a barrier over them.
+template <int R, int HD, int THREADS, typename Bar, typename Put>
+FYB_DEV void kv8_arrive(const Kv8Attention &A, const Kv8Parts &of, unsigned tid, unsigned rows, float *weights,
+    unsigned max_weights, unsigned *flag, Bar bar, Put put)
+{
+    const unsigned c0 = of.first, c1 = of.last;
     __threadfence();
     bar();
     if (tid == 0) *flag = atomicAdd(&A.counters[c0], 1u) == c1 - c0;
@@ -315,6 +310,29 @@ FYB_DEV void kv8_finish(const Kv8Attention &A, const Kv8Segment &s, const Kv8Pla
         }
     }
     bar();
+}
+// `threads` threads hold the segment's part as ml[R] and o[R][HD] in shared
+// memory; bar(): a barrier over them. Writes the rows out when the CTA has the
+// whole segment, otherwise leaves a partial. put(row, chunk, v): four values of a row.
+template <int R, int HD, int THREADS, typename Bar, typename Put>
+FYB_DEV void kv8_finish(const Kv8Attention &A, const Kv8Segment &s, const Kv8Place &place, unsigned tid, const float2 *ml,
+    const float *o, unsigned rows, float *weights, unsigned max_weights, unsigned *flag, Bar bar, Put put)
+{
+    if (s.t0 == 0 && s.t1 == s.tiles) {
+        for (unsigned i = tid; i < rows * (HD / 4); i += THREADS) {
+            const unsigned row = i / (HD / 4);
+            float4 v = reinterpret_cast<const float4 *>(o)[i];
+            const float l = ml[row].y, n = l > 0.f || isnan(l) ? 1.f / l : 0.f;
+            v.x *= n; v.y *= n; v.z *= n; v.w *= n;
+            put(row, i % (HD / 4), v);
+        }
+        return;
+    }
+    const Kv8Parts of = kv8_parts(s, place);
+    for (unsigned i = tid; i < rows * (HD / 4); i += THREADS)
+        reinterpret_cast<float4 *>(A.part_o + (size_t)of.slot * R * HD)[i] = reinterpret_cast<const float4 *>(o)[i];
+    for (unsigned i = tid; i < rows; i += THREADS) A.part_ml[(size_t)of.slot * R + i] = ml[i];
+    kv8_arrive<R, HD, THREADS>(A, of, tid, rows, weights, max_weights, flag, bar, put);
 }
 
 // Four values of one query row in the rows' type.

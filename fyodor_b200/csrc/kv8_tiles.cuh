@@ -32,6 +32,7 @@
 // position and its group's rows), four K, four V and q, one TMA, one MMA.
 #pragma once
 #include "kv8_attention.cuh"
+#include "kt_mma.cuh"
 
 namespace fyb {
 
@@ -46,88 +47,6 @@ FYB_HOST_DEV constexpr int kt_threads(int N) { return 32 * (kt_soft(N) + kt_conv
 
 constexpr int KT_FLUSH = 2;  // tiles D2 gathers before it is added to the sums
 
-// ---- tcgen05 -------------------------------------------------------------------
-// Operand in 128-byte swizzled rows, eight-row groups 1024 bytes apart. K-major:
-// a row is 64 K values of one M/N index. M/N-major: a row is 64 M/N values of one
-// K index, `lead` bytes to the next 64.
-FYB_DEV uint64_t kt_desc(unsigned addr, unsigned lead)
-{
-    return (uint64_t)(addr >> 4 & 0x3FFFu) | (uint64_t)(lead >> 4) << 16 | 64ull << 32 | 1ull << 46 | 2ull << 61;
-}
-// F32 accumulator, fp16 operands, M = 128; mn: B is N-major
-FYB_HOST_DEV constexpr uint32_t kt_idesc(unsigned N, bool mn)
-{
-    return 1u << 4 | (mn ? 1u << 16 : 0u) | N >> 3 << 17 | 128u >> 4 << 24;
-}
-// D (tensor memory) (+)= A (tensor memory: row m in lane m, 16 K values in 8 columns) x B (shared memory)
-FYB_DEV void kt_mma(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool accumulate)
-{
-    asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-                 " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n"
-                 :: "r"(d), "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate) : "memory");
-}
-FYB_DEV void kt_commit(uint64_t *bar)
-{
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];"
-                 :: "r"(smem_u32(bar)) : "memory");
-}
-FYB_DEV bool kt_elect()
-{
-    unsigned one;
-    asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(one));
-    return one != 0;
-}
-FYB_DEV void kt_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
-FYB_DEV void kt_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-// 16 consecutive columns of this thread's TMEM lane
-FYB_DEV void kt_ld16(uint32_t addr, float *r)
-{
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
-                 : "=f"(r[0]), "=f"(r[1]), "=f"(r[2]), "=f"(r[3]), "=f"(r[4]), "=f"(r[5]), "=f"(r[6]), "=f"(r[7]),
-                   "=f"(r[8]), "=f"(r[9]), "=f"(r[10]), "=f"(r[11]), "=f"(r[12]), "=f"(r[13]), "=f"(r[14]), "=f"(r[15])
-                 : "r"(addr) : "memory");
-}
-FYB_DEV void kt_ld4(uint32_t addr, float *r)
-{
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x4.b32 {%0,%1,%2,%3}, [%4];"
-                 : "=f"(r[0]), "=f"(r[1]), "=f"(r[2]), "=f"(r[3]) : "r"(addr) : "memory");
-}
-FYB_DEV void kt_st4(uint32_t addr, const float *r)
-{
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1,%2,%3,%4};"
-                 :: "r"(addr), "f"(r[0]), "f"(r[1]), "f"(r[2]), "f"(r[3]) : "memory");
-}
-FYB_DEV void kt_st16(uint32_t addr, const float *r)
-{
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
-                 :: "r"(addr), "f"(r[0]), "f"(r[1]), "f"(r[2]), "f"(r[3]), "f"(r[4]), "f"(r[5]), "f"(r[6]), "f"(r[7]),
-                    "f"(r[8]), "f"(r[9]), "f"(r[10]), "f"(r[11]), "f"(r[12]), "f"(r[13]), "f"(r[14]), "f"(r[15])
-                 : "memory");
-}
-// 16 lanes x 32 columns: registers 4j, 4j + 1 of lane 4g + t go to TMEM lane g, columns 8j + 2t and + 1; 4j + 2, 4j + 3
-// to TMEM lane g + 8
-FYB_DEV void kt_st256(uint32_t addr, const unsigned *r)
-{
-    asm volatile("tcgen05.st.sync.aligned.16x256b.x4.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
-                 :: "r"(addr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
-                    "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
-                 : "memory");
-}
-FYB_DEV void kt_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
-FYB_DEV void kt_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-
-// A bounded wait that gives up when it, or another of the CTA (*dead), has run out; the kernel's end raises the error
-// word for it. Kept to a few instructions: the roles' loops together have to stay in the instruction cache (with
-// everything inlined a tile took 7000 cycles, half of them waiting for instructions).
-FYB_DEV void kt_wait(uint64_t *bar, unsigned parity, volatile unsigned *dead)
-{
-    if (__builtin_expect(mbar_try_wait(bar, parity & 1), 1)) return;
-    for (unsigned i = 0; !mbar_try_wait(bar, parity & 1); ++i)
-        if (__builtin_expect(i >= 1u << 22 || *dead, 0)) {
-            *dead = 1;
-            break;
-        }
-}
 // The CTA's k-th segment, walked from the start; t1 = 0 past the last.
 static __device__ __noinline__ void kt_segment(const Kv8Attention &A, const Kv8Place &place, unsigned k, Kv8Segment *s)
 {
@@ -149,15 +68,6 @@ FYB_DEV float kt_sum16(float (&v)[16], unsigned lane)
     }
     return v[0] + __shfl_xor_sync(0xffffffffu, v[0], 16);
 }
-FYB_DEV unsigned kt_pack(float lo, float hi)  // fp16 pair
-{
-    const __half2 p = __floats2half2_rn(lo, hi);
-    return *reinterpret_cast<const unsigned *>(&p);
-}
-FYB_DEV float2 kt_unpack(unsigned p) { return __half22float2(*reinterpret_cast<const __half2 *>(&p)); }
-FYB_DEV int kt_exponent(float x) { return x > 0.f ? max(-126, (int)(__float_as_uint(x) >> 23) - 127) : 0; }
-FYB_DEV float kt_power(int e) { return e < -126 ? __uint_as_float(1u << max(0, e + 149)) : __uint_as_float((unsigned)(min(e, 127) + 127) << 23); }
-
 template <int HD, int N, int QP> struct KtShape {
     static constexpr int STAGE = KT_TILE * HD, STAGES = QP * N * HD > 8192 ? 2 : 3;  // an 8-bit tile; as many as fit
     static constexpr int QB = N * HD * 2, PB = KT_TILE * 128;                        // one half of q; one half of P
