@@ -88,6 +88,7 @@ extern "C" int fyb_kv4_attention(const fyb_kv4_cache *cache, const int32_t *leng
         return launch_kv4_decode(A, k, v, (unsigned)std::min<unsigned long long>(KA_GRID, units), s);
     }
     const unsigned n = tile_rows(group_rows);
+    A.vec = (uintptr_t)q % 16 == 0 && q_stride % 8 == 0;
     A.row_tile = n / A.group;
     const unsigned long long units = tiles * A.c.kv_heads * std::min<unsigned long long>((max_rows + A.row_tile - 1) / A.row_tile, 1u << 20);
     const unsigned grid = (unsigned)std::min<unsigned long long>(K4T_GRID, units);

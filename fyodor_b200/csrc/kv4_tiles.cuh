@@ -13,11 +13,13 @@
 // is a fifteenth of its group's range), in the order of a word's numbers: 0 4 1 5
 // 2 6 3 7. q lies in the same order, the output is put back.
 //
-// Row tiles of 128 rows (prompt chunks): two groups of softmax warps take tiles in
-// turn, each with maxima, sums and O of its own, P in the place of its S. Row tiles
-// of 64 or 32 rows (drafts): the lanes hold two or four copies of the rows, and copy c
-// takes the positions of its part of a tile, its P being 0 elsewhere: every thread has
-// positions to do, and what the copies hold is joined like any parts.
+// P lies in the upper half of its S. Row tiles of 128 rows (prompt chunks): two
+// groups of softmax warps take tiles in turn, each with maxima, sums and O of its own.
+// Row tiles of 64 or 32 rows (drafts): the lanes hold two or four copies of the rows,
+// and copy c takes the positions of its part of a tile, its P being 0 elsewhere: every
+// thread has positions to do, and what the copies hold is joined like any parts. One
+// group and one O leave room for q in tensor memory, which saves its reads and its
+// place in shared memory.
 //
 // The maximum m of a row moves only when a score is more than 2^8 above it.
 #pragma once
@@ -33,13 +35,14 @@ FYB_HOST_DEV constexpr int k4t_threads(int NR) { return 32 * (4 * k4t_groups(NR)
 template <int HD, int NR> struct K4tShape {
     static constexpr int ROW = HD / 2, SCALES = HD / 64 * 4;                 // bytes of a token's row, of its scales
     static constexpr int RAW_V = K4_TILE * ROW, RAW_KS = 2 * RAW_V, RAW_VS = RAW_KS + K4_TILE * SCALES,
-                         RAW = RAW_VS + K4_TILE * SCALES, STAGES = HD == 128 ? 2 : 4;
+                         RAW = RAW_VS + K4_TILE * SCALES, STAGES = HD == 64 || NR < 128 ? 4 : 2;
     static constexpr int HALF = 128 * 128, TILE = HD / 64 * HALF;             // fp16 rows of 64 values in 128 bytes
     static constexpr int O_STRIDE = 20;                                       // floats between lanes of 16 columns of O on their way out
-    static constexpr int OFF_K = 0, OFF_V = 2 * TILE, OFF_Q = 4 * TILE, OFF_RAW = 5 * TILE, OFF_O = OFF_RAW + STAGES * RAW,
+    static constexpr bool Q_TM = NR < 128;                                    // q in tensor memory
+    static constexpr int OFF_K = 0, OFF_V = 2 * TILE, OFF_Q = 4 * TILE, OFF_RAW = (Q_TM ? 4 : 5) * TILE, OFF_O = OFF_RAW + STAGES * RAW,
                          OFF_END = OFF_O + k4t_groups(NR) * 128 * O_STRIDE * 4;
-    // tensor memory columns: S of two tiles, O of each group, P beside them or (two groups) in the upper half of S
-    static constexpr int O = 256, P0 = k4t_groups(NR) == 2 ? 64 : 256 + HD, P_STEP = k4t_groups(NR) == 2 ? 128 : 64;
+    // tensor memory columns: S of two tiles with P in the upper half, O of each group, q
+    static constexpr int P = 64, O = 256, Q = 256 + HD;
 };
 template <int NR> struct K4tShared {
     Kv8Segment seg[K4T_SEGS], walked[k4t_threads(NR) / 32];
@@ -75,6 +78,23 @@ FYB_DEV uint4 k4t_values(unsigned x, __half2 scale, __half2 low)
         out[2 * i + 1] = *reinterpret_cast<const unsigned *>(&v);
     }
     return make_uint4(out[0], out[1], out[2], out[3]);
+}
+
+// Eight values of a query row of 16 bits; vec: in one access.
+FYB_DEV void k4t_load8(const Kv4Attention &A, size_t at, float4 &a, float4 &b)
+{
+    if (A.vec) {
+        const uint4 u = __ldg(reinterpret_cast<const uint4 *>(static_cast<const unsigned short *>(A.q) + at));
+        auto two = [&](unsigned w) {
+            return A.type == T_F16 ? kt_unpack(w) : make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+        };
+        const float2 p = two(u.x), q = two(u.y), r = two(u.z), s = two(u.w);
+        a = make_float4(p.x, p.y, q.x, q.y);
+        b = make_float4(r.x, r.y, s.x, s.y);
+    } else {
+        a = kv8_load4(A.q, A.type, at);
+        b = kv8_load4(A.q, A.type, at + 4);
+    }
 }
 
 template <int HD, int NR>
@@ -140,14 +160,6 @@ __global__ void __launch_bounds__(k4t_threads(NR), 1) kv4_tiles_kernel(const __g
         const uint32_t o_at = tmem + lanes + S::O + wg * HD;
         float *stage = reinterpret_cast<float *>(ring + S::OFF_O);
         auto bar = [] { asm volatile("bar.sync 1, %0;" :: "n"(32 * SOFT) : "memory"); };
-        if constexpr (CP > 1) {  // P of other copies' positions is 0 from here on
-            float z[16];
-#pragma unroll
-            for (int i = 0; i < 16; ++i) z[i] = 0.f;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) kt_st16(tmem + lanes + S::P0 + 16 * i, z);
-            kt_wait_st();
-        }
         constexpr float P_UP = 6.f;  // weights are 2^6 times themselves, clear of fp16's smallest numbers; the largest is 2^14
         while (const Kv8Segment *sp = next()) {
             const Kv8Segment &s = *sp;
@@ -164,37 +176,37 @@ __global__ void __launch_bounds__(k4t_threads(NR), 1) kv4_tiles_kernel(const __g
                 if (GROUPS == 2 && b != wg) continue;
                 wait(sh.meta_full + n % K4T_META, n / K4T_META);
                 const unsigned here = sh.here[n % K4T_META];
-                const bool raw = here != 0xffu || (t + 1) * K4_TILE > all;
                 wait(sh.s_full + b, n >> 1);
                 kt_fence_after();
-                const uint32_t s_at = tmem + lanes + b * 128 + first, p_at = tmem + lanes + S::P0 + b * S::P_STEP + first / 2;
-                // scores of 32 positions in units of log2, -inf where not attended
-                auto masked = [&](float (&x)[32], unsigned c) {
-                    if (__builtin_expect(!raw, 1)) return;
-                    const unsigned p0 = first + 32 * c;
+                const uint32_t s_at = tmem + lanes + b * 128 + first, p_at = tmem + lanes + b * 128 + S::P;
+                if (__builtin_expect(here != 0xffu || (t + 1) * K4_TILE > all, 0)) {
+                    // what the row does not attend becomes -inf where it lies: the rest has one form, and fits the
+                    // instruction cache with the other roles
+#pragma unroll 1
+                    for (unsigned c = 0; c < CW; c += 16) {
+                        float y[16];
+                        kt_ld16(s_at + c, y);
+                        kt_wait_ld();
+                        const int left = here >> ((first + c) / 16) & 1 ? limit - (t * K4_TILE + (int)(first + c)) : 0;
 #pragma unroll
-                    for (int i = 0; i < 32; ++i)
-                        x[i] = t * K4_TILE + (int)p0 + i < limit && (here >> ((p0 + i) / 16) & 1) ? x[i] * f : -INFINITY;
-                };
-                auto highest = [&](const float (&x)[32]) {
-                    float h = x[0];
-#pragma unroll
-                    for (int i = 1; i < 32; ++i) h = fmaxf(h, x[i]);
-                    return raw ? h : h * f;
-                };
+                        for (int i = 0; i < 16; ++i) y[i] = i < left ? y[i] : -INFINITY;
+                        kt_st16(s_at + c, y);
+                    }
+                    kt_wait_st();
+                }
                 constexpr unsigned KEEP = CHUNKS < 2 ? CHUNKS : 2;  // blocks that stay in registers between the two looks at them
-                float x[KEEP][32], top = -INFINITY;
+                float x[KEEP][32], tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
                 for (unsigned c = 0; c < CHUNKS; c += KEEP) {
 #pragma unroll
                     for (unsigned k = 0; k < KEEP; ++k) kt_ld32(s_at + 32 * (c + k), x[k]);
                     kt_wait_ld();
 #pragma unroll
-                    for (unsigned k = 0; k < KEEP; ++k) {
-                        masked(x[k], c + k);
-                        top = fmaxf(top, highest(x[k]));
-                    }
+                    for (unsigned k = 0; k < KEEP; ++k)
+#pragma unroll
+                        for (int i = 0; i < 32; i += 2) tops[i / 2 % 4] = fmaxf(tops[i / 2 % 4], fmaxf(x[k][i], x[k][i + 1]));
                 }
+                const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])) * f;
                 const bool up = top - m > 8.f + P_UP;
                 if (__any_sync(0xffffffffu, up)) {
                     // ---- new maxima, and the sums so far in their units
@@ -216,34 +228,40 @@ __global__ void __launch_bounds__(k4t_threads(NR), 1) kv4_tiles_kernel(const __g
                         kt_wait_st();
                     }
                 }
-                if (GROUPS == 1 && n >= 2) {  // P's place is free
-                    wait(sh.o_done + b, (n >> 1) - 1);
-                    kt_fence_after();
-                }
                 // ---- weights, blocks from the last to the first: P takes the place of scores that have been read
+                const F2 f2x = f2(f, f), mx = f2(-m, -m);
+                F2 sums[2] = {f2(0.f, 0.f), f2(0.f, 0.f)};
                 auto weights = [&](float (&y)[32], unsigned c) {
                     unsigned w[16];
 #pragma unroll
                     for (int i = 0; i < 32; i += 2) {
-                        const float p0 = ex2(raw ? y[i] - m : fmaf(y[i], f, -m)), p1 = ex2(raw ? y[i + 1] - m : fmaf(y[i + 1], f, -m));
-                        l += p0;
-                        l += p1;
+                        const float2 e = f2_get(f2_fma(f2(y[i], y[i + 1]), f2x, mx));
+                        const float p0 = ex2(e.x), p1 = ex2(e.y);
+                        sums[i / 2 % 2] = f2_add(sums[i / 2 % 2], f2(p0, p1));
                         w[i / 2] = kt_pack(p0, p1);
                     }
-                    kt_st16(p_at + 16 * c, reinterpret_cast<const float *>(w));
+                    kt_st16(p_at + first / 2 + 16 * c, reinterpret_cast<const float *>(w));
                 };
+                if constexpr (CP > 1) {  // 0 for the positions of the other copies
+                    float z[16];
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) z[i] = 0.f;
+#pragma unroll
+                    for (unsigned c = 0; c < 64; c += 16)
+                        if (c < first / 2 || c >= (first + CW) / 2) kt_st16(p_at + c, z);
+                }
 #pragma unroll
                 for (unsigned c = CHUNKS; c; c -= KEEP) {
                     if (c != CHUNKS) {
 #pragma unroll
                         for (unsigned k = 0; k < KEEP; ++k) kt_ld32(s_at + 32 * (c - KEEP + k), x[k]);
                         kt_wait_ld();
-#pragma unroll
-                        for (unsigned k = 0; k < KEEP; ++k) masked(x[k], c - KEEP + k);
                     }
 #pragma unroll
                     for (unsigned k = KEEP; k; --k) weights(x[k - 1], c - KEEP + k - 1);
                 }
+                const float2 l2 = f2_get(f2_add(sums[0], sums[1]));
+                l += l2.x + l2.y;
                 kt_wait_st();
                 kt_fence_before();
                 arrive(sh.p_full + b);
@@ -333,36 +351,75 @@ __global__ void __launch_bounds__(k4t_threads(NR), 1) kv4_tiles_kernel(const __g
             const Kv8Segment &s = *sp;
             const int any = kv8_attended(A, s.q, s.row_tile), t0 = s.t0, t1 = s.t1;
             if (!is_v) {
-                // ---- q rows by a power of two each, a thread a lane's row
-                const unsigned rho = ct % NR;
+                // ---- q rows by a power of two each. The score factor's sign goes with q: a row's largest product is its
+                // largest score
                 const int j0 = s.row_tile * (int)A.row_tile, nrows = min((int)A.row_tile, s.q.rows - j0) * (int)GR;
-                const bool real = (int)rho < nrows;
-                const size_t row = (size_t)(s.q.first + j0 + (real ? (int)(rho / GR) : 0));
-                const size_t base = row * A.q_stride + (size_t)(s.head * GR + (real ? rho % GR : 0)) * HD;
-                float top = 0.f;
-                if (real) {
-#pragma unroll 8
-                    for (int i = 0; i < HD; i += 4) {
-                        const float4 v = kv8_load4(A.q, A.type, base + i);
-                        top = fmaxf(top, fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w))));
-                    }
-                }
-                const int e = 12 - kt_exponent(top);
-                // the score factor's sign goes with q: a row's largest product is its largest score
-                const float up = copysignf(kt_power(min(e, 127)), A.scale), up2 = kt_power(e - min(e, 127));
-                if (seg) wait(&sh.q_empty, seg - 1);  // the last segment's products have read their q
-#pragma unroll 2
-                for (int i = 0; i < HD; i += 8) {
-                    float4 a = make_float4(0.f, 0.f, 0.f, 0.f), b = a;
+                auto at_of = [&](unsigned rho) {
+                    return (size_t)(s.q.first + j0 + (int)(rho / GR)) * A.q_stride + (size_t)(s.head * GR + rho % GR) * HD;
+                };
+                auto size_of = [](float4 a) { return fmaxf(fmaxf(fabsf(a.x), fabsf(a.y)), fmaxf(fabsf(a.z), fabsf(a.w))); };
+                auto halves = [&](float4 a, float4 b, int e) {
+                    const float up = copysignf(kt_power(min(e, 127)), A.scale), up2 = kt_power(e - min(e, 127));
+                    auto pair = [&](float y, float z) { return kt_pack(y * up * up2, z * up * up2); };
+                    return make_uint4(pair(a.x, b.x), pair(a.y, b.y), pair(a.z, b.z), pair(a.w, b.w));
+                };
+                // at least the smallest normal number: -inf times it stays -inf
+                auto factor_of = [&](int e) { return fmaxf(ldexpf(fabsf(A.scale), -e), 1.17549435e-38f); };
+                if constexpr (S::Q_TM) {
+                    // to tensor memory, a thread a lane's row
+                    const unsigned rho = ct % NR;
+                    const bool real = (int)rho < nrows;
+                    const size_t at = at_of(real ? rho : 0);
+                    float top = 0.f;
                     if (real) {
-                        a = kv8_load4(A.q, A.type, base + i);
-                        b = kv8_load4(A.q, A.type, base + i + 4);
+#pragma unroll 8
+                        for (int i = 0; i < HD; i += 8) {
+                            float4 a, b;
+                            k4t_load8(A, at + i, a, b);
+                            top = fmaxf(top, fmaxf(size_of(a), size_of(b)));
+                        }
                     }
-                    auto pair = [&](float u, float v) { return kt_pack(u * up * up2, v * up * up2); };
-                    unsigned char *q = ring + S::OFF_Q + i / 64 * S::HALF + ct * 128 + (((i % 64 / 8) ^ (ct & 7u)) << 4);
-                    *reinterpret_cast<uint4 *>(q) = make_uint4(pair(a.x, b.x), pair(a.y, b.y), pair(a.z, b.z), pair(a.w, b.w));
+                    const int e = 12 - kt_exponent(top);
+                    if (seg) wait(&sh.q_empty, seg - 1);  // the last segment's products have read their q
+                    kt_fence_after();
+#pragma unroll 2
+                    for (int i = 0; i < HD; i += 32) {
+                        uint4 h[4];
+#pragma unroll
+                        for (int u = 0; u < 4; ++u) {
+                            float4 a = make_float4(0.f, 0.f, 0.f, 0.f), b = a;
+                            if (real) k4t_load8(A, at + i + 8 * u, a, b);
+                            h[u] = halves(a, b, e);
+                        }
+                        kt_st16(tmem + (cw << 21) + S::Q + i / 2, reinterpret_cast<const float *>(h));
+                    }
+                    kt_wait_st();
+                    sh.factor[seg % K4T_SEGS][ct] = factor_of(e);
+                    kt_fence_before();
+                } else {
+                    // to shared memory, eight values a lane
+                    constexpr unsigned LANES = HD / 8, STEP = 32 / LANES, STEPS = NR / K4T_CONV / STEP, AHEAD = 4;  // lanes of a row, rows of a load
+                    const unsigned piece = lane % LANES;
+#pragma unroll 1
+                    for (unsigned i = 0; i < STEPS; i += AHEAD) {
+                        float4 x[AHEAD][2];
+#pragma unroll
+                        for (unsigned u = 0; u < AHEAD; ++u) {
+                            const unsigned rho = (cw * STEPS + i + u) * STEP + lane / LANES;
+                            x[u][0] = x[u][1] = make_float4(0.f, 0.f, 0.f, 0.f);
+                            if ((int)rho < nrows) k4t_load8(A, at_of(rho) + 8 * piece, x[u][0], x[u][1]);
+                        }
+                        if (seg && i == 0) wait(&sh.q_empty, seg - 1);  // the last segment's products have read their q
+#pragma unroll
+                        for (unsigned u = 0; u < AHEAD; ++u) {
+                            const unsigned rho = (cw * STEPS + i + u) * STEP + lane / LANES;
+                            const int e = 12 - kt_exponent(group_max<LANES>(fmaxf(size_of(x[u][0]), size_of(x[u][1]))));
+                            *reinterpret_cast<uint4 *>(ring + S::OFF_Q + piece / 8 * S::HALF + rho * 128 + ((piece % 8 ^ (rho & 7u)) << 4)) =
+                                halves(x[u][0], x[u][1], e);
+                            if (piece == 0) sh.factor[seg % K4T_SEGS][rho] = factor_of(e);
+                        }
+                    }
                 }
-                sh.factor[seg % K4T_SEGS][ct] = ldexpf(fabsf(A.scale), -e);
                 fence_proxy_async();
                 arrive(sh.q_full + seg % K4T_SEGS);
             }
@@ -376,27 +433,41 @@ __global__ void __launch_bounds__(k4t_threads(NR), 1) kv4_tiles_kernel(const __g
                 // V of positions that no row attends, or never loaded, is 0 and not what lies there (a NaN stays one times 0)
                 const unsigned here = sh.raw_here[st];
                 const bool patchy = is_v && (here != 0xffu || any < (t + 1) * K4_TILE);
-#pragma unroll 4
-                for (unsigned i = 0; i < 8; ++i) {
-                    const unsigned tok = tok0 + 4 * i, sw = ((j ^ (tok & 7u)) << 4) + tok * 128;
-                    unsigned w[G64], sc[G64];
-                    if constexpr (G64 == 2) {
-                        const uint2 x = *reinterpret_cast<const uint2 *>(raw + tok * 64 + ((8 * j) ^ ((tok >> 1 & 3) << 4)));
-                        const uint2 y = *reinterpret_cast<const uint2 *>(scales + tok * 8);
-                        w[0] = x.x; w[1] = x.y;
-                        sc[0] = y.x; sc[1] = y.y;
-                    } else {
-                        w[0] = *reinterpret_cast<const unsigned *>(raw + tok * 32 + 4 * j);
-                        sc[0] = *reinterpret_cast<const unsigned *>(scales + tok * 4);
-                    }
-                    if (__builtin_expect(patchy, 0) && (t * K4_TILE + (int)tok >= any || !(here >> (tok / 16) & 1))) {
+                // four tokens' words and scales at a time, before the first of their stores (which they might overlap, as
+                // far as the compiler can tell: a token after the other took 1500 cycles a tile)
 #pragma unroll
-                        for (int h = 0; h < G64; ++h) sc[h] = 0;
+                for (unsigned i0 = 0; i0 < 8; i0 += 4) {
+                    unsigned w[4][G64], sc[4][G64];
+#pragma unroll
+                    for (unsigned i = 0; i < 4; ++i) {
+                        const unsigned tok = tok0 + 4 * (i0 + i);
+                        if constexpr (G64 == 2) {
+                            const uint2 x = *reinterpret_cast<const uint2 *>(raw + tok * 64 + ((8 * j) ^ ((tok >> 1 & 3) << 4)));
+                            const uint2 y = *reinterpret_cast<const uint2 *>(scales + tok * 8);
+                            w[i][0] = x.x; w[i][1] = x.y;
+                            sc[i][0] = y.x; sc[i][1] = y.y;
+                        } else {
+                            w[i][0] = *reinterpret_cast<const unsigned *>(raw + tok * 32 + 4 * j);
+                            sc[i][0] = *reinterpret_cast<const unsigned *>(scales + tok * 4);
+                        }
+                    }
+                    if (__builtin_expect(patchy, 0)) {
+#pragma unroll
+                        for (unsigned i = 0; i < 4; ++i) {
+                            const unsigned tok = tok0 + 4 * (i0 + i);
+                            const bool is = t * K4_TILE + (int)tok < any && (here >> (tok / 16) & 1);
+#pragma unroll
+                            for (int h = 0; h < G64; ++h) sc[i][h] = is ? sc[i][h] : 0;
+                        }
                     }
 #pragma unroll
-                    for (int h = 0; h < G64; ++h) {
-                        const __half2 sl = *reinterpret_cast<const __half2 *>(&sc[h]);
-                        *reinterpret_cast<uint4 *>(dst + h * S::HALF + sw) = k4t_values(w[h], __low2half2(sl), __high2half2(sl));
+                    for (unsigned i = 0; i < 4; ++i) {
+                        const unsigned tok = tok0 + 4 * (i0 + i), sw = ((j ^ (tok & 7u)) << 4) + tok * 128;
+#pragma unroll
+                        for (int h = 0; h < G64; ++h) {
+                            const __half2 sl = *reinterpret_cast<const __half2 *>(&sc[i][h]);
+                            *reinterpret_cast<uint4 *>(dst + h * S::HALF + sw) = k4t_values(w[i][h], __low2half2(sl), __high2half2(sl));
+                        }
                     }
                 }
                 arrive(sh.raw_empty + st);
@@ -475,16 +546,15 @@ __global__ void __launch_bounds__(k4t_threads(NR), 1) kv4_tiles_kernel(const __g
         auto scores = [&](bool last) {
             const unsigned b = at & 1;
             wait(sh.k_full + b, at >> 1);
-            // two groups: P of the tile before the last, which lies in this S, has been read. One: its S was read before
-            // its P was full, which this warp has waited for
-            if (GROUPS == 2 && at >= 2) wait(sh.o_done + b, (at >> 1) - 1);
+            if (at >= 2) wait(sh.o_done + b, (at >> 1) - 1);  // P of the tile before the last, in this S, has been read
             kt_fence_after();
             __syncwarp();
             if (kt_elect()) {
 #pragma unroll
                 for (int k = 0; k < HD / 16; ++k) {
                     const uint64_t step = (uint64_t)((k / 4 * S::HALF + k % 4 * 32) >> 4);
-                    kt_mma_ss(tm + b * 128, qs + step, ks + (b * S::TILE >> 4) + step, kt_idesc(128, false), k > 0);
+                    if constexpr (S::Q_TM) kt_mma(tm + b * 128, tm + S::Q + 8 * k, ks + (b * S::TILE >> 4) + step, kt_idesc(128, false), k > 0);
+                    else kt_mma_ss(tm + b * 128, qs + step, ks + (b * S::TILE >> 4) + step, kt_idesc(128, false), k > 0);
                 }
                 kt_commit(sh.k_empty + b);
                 kt_commit(sh.s_full + b);
@@ -510,7 +580,7 @@ __global__ void __launch_bounds__(k4t_threads(NR), 1) kv4_tiles_kernel(const __g
                 if (kt_elect()) {
 #pragma unroll
                     for (int k = 0; k < K4_TILE / 16; ++k)
-                        kt_mma(tm + S::O + g * HD, tm + S::P0 + b * S::P_STEP + 8 * k, vs + ((b * S::TILE + k * 2048) >> 4),
+                        kt_mma(tm + S::O + g * HD, tm + b * 128 + S::P + 8 * k, vs + ((b * S::TILE + k * 2048) >> 4),
                                kt_idesc(HD, true), (begun >> g & 1) || k);
                     kt_commit(sh.v_empty + b);
                     kt_commit(sh.o_done + b);

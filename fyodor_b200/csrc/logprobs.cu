@@ -50,40 +50,6 @@ struct Logprobs {
 constexpr size_t LP_COUNTER_BYTES = (LP_GRID * 4 + 255) / 256 * 256;
 constexpr size_t LP_PART_BYTES = 2 * LP_GRID * (sizeof(LpSums) + 4);
 
-// ---- pairs of F32 -------------------------------------------------------------
-struct F2 {
-    unsigned long long v;
-};
-FYB_DEV F2 f2(float a, float b)
-{
-    F2 r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(a), "f"(b));
-    return r;
-}
-FYB_DEV float2 f2_get(F2 a)
-{
-    float2 r;
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(a.v));
-    return r;
-}
-FYB_DEV F2 f2_add(F2 a, F2 b)
-{
-    F2 r;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
-    return r;
-}
-FYB_DEV F2 f2_mul(F2 a, F2 b)
-{
-    F2 r;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
-    return r;
-}
-FYB_DEV F2 f2_fma(F2 a, F2 b, F2 c)
-{
-    F2 r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
-    return r;
-}
 FYB_DEV float lp_exp2(float x)
 {
     float y;
