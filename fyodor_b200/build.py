@@ -42,7 +42,7 @@ VARIANTS = {
     "kv8_tiles_inst.cu": [("%d_%d" % (hd, f), ["-DFYB_KT_HD=%d" % hd, "-DFYB_KT_FMT=%d" % f])
                           for hd in (128, 64) for f in (0, 1)],
     "kv4_tiles_inst.cu": [("%d_%d" % (hd, n), ["-DFYB_K4_HD=%d" % hd, "-DFYB_K4_NR=%d" % n])
-                          for hd in (128, 64) for n in (32, 64, 128)],
+                          for hd in (128, 64) for n in (32, 64, 256)],
 }
 
 

@@ -3,13 +3,13 @@
 //
 // Up to eight query rows per KV head (rows of a request x heads of a group), and
 // rows of F32 whatever their number, run on kv4_decode.cu, many rows in row tiles of
-// eight; many rows of 16 bits on kv4_tiles.cuh, in row tiles of 32, 64 or 128.
+// eight; many rows of 16 bits on kv4_tiles.cuh, in row tiles of 32, 64 or 256.
 #include "kv4_attention.cuh"
 
 namespace fyb {
 
 using TilesLaunch = int(const Kv4Attention &, const CUtensorMap &, const CUtensorMap &, unsigned, cudaStream_t);
-TilesLaunch kv4_tiles_128_32, kv4_tiles_128_64, kv4_tiles_128_128, kv4_tiles_64_32, kv4_tiles_64_64, kv4_tiles_64_128;
+TilesLaunch kv4_tiles_128_32, kv4_tiles_128_64, kv4_tiles_128_256, kv4_tiles_64_32, kv4_tiles_64_64, kv4_tiles_64_256;
 
 constexpr unsigned K4T_GRID = 148;  // one CTA per SM
 
@@ -22,7 +22,7 @@ static int kv4_tensor_map(CUtensorMap *map, const fyb_kv4_cache &c, const void *
 }
 
 // Row tile of the many-row kernel.
-static unsigned tile_rows(unsigned long long group_rows) { return group_rows <= 32 ? 32 : group_rows <= 64 ? 64 : 128; }
+static unsigned tile_rows(unsigned long long group_rows) { return group_rows <= 32 ? 32 : group_rows <= 64 ? 64 : 256; }
 // Query rows of a call's partials, two for each CTA of its kernel (F32 rows need 2 KA_GRID of eight: fewer than tiles do).
 static size_t part_rows(unsigned long long group_rows)
 {
@@ -89,10 +89,11 @@ extern "C" int fyb_kv4_attention(const fyb_kv4_cache *cache, const int32_t *leng
     }
     const unsigned n = tile_rows(group_rows);
     A.vec = (uintptr_t)q % 16 == 0 && q_stride % 8 == 0;
+    A.vec_out = (uintptr_t)out % 16 == 0 && out_stride % 8 == 0;
     A.row_tile = n / A.group;
     const unsigned long long units = tiles * A.c.kv_heads * std::min<unsigned long long>((max_rows + A.row_tile - 1) / A.row_tile, 1u << 20);
     const unsigned grid = (unsigned)std::min<unsigned long long>(K4T_GRID, units);
-    TilesLaunch *go = cache->head_dim == 128 ? (n == 32 ? kv4_tiles_128_32 : n == 64 ? kv4_tiles_128_64 : kv4_tiles_128_128)
-                                             : (n == 32 ? kv4_tiles_64_32 : n == 64 ? kv4_tiles_64_64 : kv4_tiles_64_128);
+    TilesLaunch *go = cache->head_dim == 128 ? (n == 32 ? kv4_tiles_128_32 : n == 64 ? kv4_tiles_128_64 : kv4_tiles_128_256)
+                                             : (n == 32 ? kv4_tiles_64_32 : n == 64 ? kv4_tiles_64_64 : kv4_tiles_64_256);
     return go(A, k, v, grid, s);
 }

@@ -10,7 +10,7 @@ namespace fyb {
 struct Kv4Attention : Kv8Attention {
     const __half2 *ks, *vs;  // scale and low of each group
     unsigned split;          // parts of a KV head's group of query heads, each counted as a head (c.kv_heads, group)
-    bool vec;                // rows of 16 bits begin on 16 bytes
+    bool vec, vec_out;       // rows of 16 bits of q, of out begin on 16 bytes
 };
 
 int launch_kv4_decode(const Kv4Attention &A, const CUtensorMap &k, const CUtensorMap &v, unsigned grid, cudaStream_t s);

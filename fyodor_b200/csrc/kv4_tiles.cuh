@@ -13,13 +13,14 @@
 // is a fifteenth of its group's range), in the order of a word's numbers: 0 4 1 5
 // 2 6 3 7. q lies in the same order, the output is put back.
 //
-// P lies in the upper half of its S. Row tiles of 128 rows (prompt chunks): two
-// groups of softmax warps take tiles in turn, each with maxima, sums and O of its own.
-// Row tiles of 64 or 32 rows (drafts): the lanes hold two or four copies of the rows,
-// and copy c takes the positions of its part of a tile, its P being 0 elsewhere: every
-// thread has positions to do, and what the copies hold is joined like any parts. One
-// group and one O leave room for q in tensor memory, which saves its reads and its
-// place in shared memory.
+// P lies in the upper half of its S. Row tiles of 256 rows (prompt chunks) are two
+// groups of 128 lanes, each with four softmax warps, S and O of its own, over the
+// same K and V: a tile is converted once for both, and one group's products run while
+// the other's weights are made. Row tiles of 64 or 32 rows (drafts): one group, whose
+// lanes hold two or four copies of the rows; copy c takes the positions of its part of
+// a tile, its P being 0 elsewhere: every thread has positions to do, and what the
+// copies hold is joined like any parts. One O leaves room for S of two tiles and for q
+// in tensor memory, which saves its reads and its place in shared memory.
 //
 // The maximum m of a row moves only when a score is more than 2^8 above it.
 #pragma once
@@ -28,30 +29,33 @@
 
 namespace fyb {
 
-constexpr int K4T_CONV = 4, K4T_META = 8, K4T_SEGS = 4;
-FYB_HOST_DEV constexpr int k4t_groups(int NR) { return NR == 128 ? 2 : 1; }      // groups of four softmax warps
+constexpr int K4T_CONV = 4, K4T_META = 8;
+FYB_HOST_DEV constexpr unsigned k4t_segs(int NR) { return NR == 256 ? 2 : 4; }   // segments handed on at a time (room for no more)
+FYB_HOST_DEV constexpr int k4t_groups(int NR) { return NR == 256 ? 2 : 1; }      // groups of four softmax warps
 FYB_HOST_DEV constexpr int k4t_threads(int NR) { return 32 * (4 * k4t_groups(NR) + 2 * K4T_CONV + 2); }
 
 template <int HD, int NR> struct K4tShape {
     static constexpr int ROW = HD / 2, SCALES = HD / 64 * 4;                 // bytes of a token's row, of its scales
-    static constexpr int RAW_V = K4_TILE * ROW, RAW_KS = 2 * RAW_V, RAW_VS = RAW_KS + K4_TILE * SCALES,
-                         RAW = RAW_VS + K4_TILE * SCALES, STAGES = HD == 64 || NR < 128 ? 4 : 2;
-    static constexpr int HALF = 128 * 128, TILE = HD / 64 * HALF;             // fp16 rows of 64 values in 128 bytes
-    static constexpr int O_STRIDE = 20;                                       // floats between lanes of 16 columns of O on their way out
-    static constexpr bool Q_TM = NR < 128;                                    // q in tensor memory
-    static constexpr int OFF_K = 0, OFF_V = 2 * TILE, OFF_Q = 4 * TILE, OFF_RAW = (Q_TM ? 4 : 5) * TILE, OFF_O = OFF_RAW + STAGES * RAW,
-                         OFF_END = OFF_O + k4t_groups(NR) * 128 * O_STRIDE * 4;
-    // tensor memory columns: S of two tiles with P in the upper half, O of each group, q
+    static constexpr int RAW = K4_TILE * (ROW + SCALES), RAW_S = K4_TILE * ROW;  // a tile of K or V as it lies in the cache
+    static constexpr bool Q_TM = NR < 256;                                   // q in tensor memory
+    // raw tiles on their way: as many as there is room for
+    static constexpr int KS = HD == 64 || Q_TM ? 4 : 2, VS = HD == 64 || Q_TM ? 4 : 1;
+    static constexpr int HALF = 128 * 128, TILE = HD / 64 * HALF;            // fp16 rows of 64 values in 128 bytes
+    static constexpr int O_STRIDE = 20;                                      // floats between lanes of 16 columns of O of copies
+    static constexpr int OFF_K = 0, OFF_V = 2 * TILE, OFF_Q = 4 * TILE, OFF_RK = OFF_Q + (Q_TM ? 0 : 2 * TILE), OFF_RV = OFF_RK + KS * RAW,
+                         OFF_O = OFF_RV + VS * RAW, STAGED = Q_TM ? 128 * O_STRIDE : 256, OFF_END = OFF_O + STAGED * 4;
+    // tensor memory columns: two S with P in the upper half, O of each group, q
     static constexpr int P = 64, O = 256, Q = 256 + HD;
 };
 template <int NR> struct K4tShared {
-    Kv8Segment seg[K4T_SEGS], walked[k4t_threads(NR) / 32];
+    static constexpr unsigned SEGS = k4t_segs(NR);
+    Kv8Segment seg[SEGS], walked[k4t_threads(NR) / 32];
     Kv8Place place;
-    uint64_t seg_full[K4T_SEGS], seg_empty[K4T_SEGS], raw_full[4], raw_empty[4], k_full[2], k_empty[2], v_full[2], v_empty[2],
-        s_full[2], p_full[2], o_done[2], o_free[2], q_full[K4T_SEGS], q_empty, meta_full[K4T_META], drained;
-    float factor[K4T_SEGS][128];                 // score factor of each lane's row
-    float2 ml[k4t_groups(NR) * 128], joined[NR];
-    unsigned here[K4T_META], raw_here[4];        // which groups of 16 positions are loaded, by tile and by stage
+    uint64_t seg_full[SEGS], seg_empty[SEGS], rk_full[4], rk_empty[4], rv_full[4], rv_empty[4], k_full[2], k_empty[2],
+        v_full[2], v_empty[2], s_full[2], p_full[2], o_done[2], o_free[2], q_full[SEGS], q_empty, meta_full[K4T_META], drained;
+    float factor[SEGS][k4t_groups(NR) * 128];  // score factor of each lane's row
+    float2 ml[NR < 256 ? 128 : 1];
+    unsigned here[K4T_META];                       // which groups of 16 positions of a tile are loaded
     uint32_t tmem;
     unsigned flag, dead;
 };
@@ -103,14 +107,18 @@ __global__ void __launch_bounds__(k4t_threads(NR), 1) kv4_tiles_kernel(const __g
 {
     using S = K4tShape<HD, NR>;
     constexpr unsigned GROUPS = k4t_groups(NR), SOFT = 4 * GROUPS, W_CONV = SOFT, W_TMA = SOFT + 2 * K4T_CONV, W_MMA = W_TMA + 1;
-    constexpr unsigned CP = 128 / NR, CW = 128 / CP, CHUNKS = CW / 32;   // copies, and the positions and blocks of 32 of a copy
+    constexpr unsigned CP = GROUPS == 2 ? 1 : 128 / NR, CW = 128 / CP, CHUNKS = CW / 32;   // copies, and the positions and blocks of 32 of a copy
+    constexpr unsigned SEGS = k4t_segs(NR);
     constexpr int G64 = HD / 64;
     extern __shared__ unsigned char k4t_smem[];
     unsigned char *ring = k4t_smem + ((1024u - (smem_u32(k4t_smem) & 1023u)) & 1023u);
     K4tShared<NR> &sh = *reinterpret_cast<K4tShared<NR> *>(ring + S::OFF_END);
     const unsigned tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), kv = A.c.kv_heads, GR = A.group;
     if (tid == 0) {
-        for (int i = 0; i < S::STAGES; ++i) { mbar_init(sh.raw_full + i, 1); mbar_init(sh.raw_empty + i, 2 * K4T_CONV); }
+        for (int i = 0; i < 4; ++i) {
+            mbar_init(sh.rk_full + i, 1); mbar_init(sh.rk_empty + i, K4T_CONV);
+            mbar_init(sh.rv_full + i, 1); mbar_init(sh.rv_empty + i, K4T_CONV);
+        }
         for (int i = 0; i < 2; ++i) {
             mbar_init(sh.k_full + i, K4T_CONV); mbar_init(sh.k_empty + i, 1);
             mbar_init(sh.v_full + i, K4T_CONV); mbar_init(sh.v_empty + i, 1);
@@ -119,7 +127,11 @@ __global__ void __launch_bounds__(k4t_threads(NR), 1) kv4_tiles_kernel(const __g
         }
         mbar_init(&sh.q_empty, 1); mbar_init(&sh.drained, 1);
         for (int i = 0; i < K4T_META; ++i) mbar_init(sh.meta_full + i, 1);
-        for (int i = 0; i < K4T_SEGS; ++i) { mbar_init(sh.q_full + i, K4T_CONV); mbar_init(sh.seg_full + i, 1); mbar_init(sh.seg_empty + i, SOFT + 2 * K4T_CONV + 1); }
+        for (unsigned i = 0; i < SEGS; ++i) {
+            mbar_init(sh.q_full + i, GROUPS * K4T_CONV);
+            mbar_init(sh.seg_full + i, 1);
+            mbar_init(sh.seg_empty + i, SOFT + 2 * K4T_CONV + 1);
+        }
         sh.dead = 0;
         fence_barrier_init();
     }
@@ -142,8 +154,8 @@ __global__ void __launch_bounds__(k4t_threads(NR), 1) kv4_tiles_kernel(const __g
     // The segment that comes next; done() with it before the next is asked for. Once a wait has run out every warp
     // walks by itself: all of them still take the same steps, so none is left at a barrier.
     auto next = [&]() -> const Kv8Segment * {
-        wait(sh.seg_full + seg % K4T_SEGS, seg / K4T_SEGS);
-        const Kv8Segment *s = sh.seg + seg % K4T_SEGS;
+        wait(sh.seg_full + seg % SEGS, seg / SEGS);
+        const Kv8Segment *s = sh.seg + seg % SEGS;
         if (__builtin_expect(*dead, 0)) {
             s = sh.walked + warp;
             if (lane == 0) k4t_segment(A, sh.place, seg, sh.walked + warp);
@@ -151,14 +163,16 @@ __global__ void __launch_bounds__(k4t_threads(NR), 1) kv4_tiles_kernel(const __g
         }
         return s->t1 ? s : nullptr;
     };
-    auto done = [&] { arrive(sh.seg_empty + seg % K4T_SEGS); ++seg; };
+    auto done = [&] { arrive(sh.seg_empty + seg % SEGS); ++seg; };
 
     if (warp < SOFT) {
         // ================================================== softmax
-        const unsigned wg = warp >> 2, at = tid & 127, rho = at % NR, first = at / NR * CW;  // lane of tensor memory; its row and first position of a tile
+        // this thread's lane of tensor memory, its row, and its first position of a tile
+        const unsigned wg = warp >> 2, at = tid & 127, rho = GROUPS == 2 ? tid : at % NR, first = CP > 1 ? at / NR * CW : 0;
         const uint32_t lanes = (warp & 3) << 21;
         const uint32_t o_at = tmem + lanes + S::O + wg * HD;
         float *stage = reinterpret_cast<float *>(ring + S::OFF_O);
+        unsigned k = 0;  // tiles of this group so far
         auto bar = [] { asm volatile("bar.sync 1, %0;" :: "n"(32 * SOFT) : "memory"); };
         constexpr float P_UP = 6.f;  // weights are 2^6 times themselves, clear of fp16's smallest numbers; the largest is 2^14
         while (const Kv8Segment *sp = next()) {
@@ -167,16 +181,18 @@ __global__ void __launch_bounds__(k4t_threads(NR), 1) kv4_tiles_kernel(const __g
             const int nrows = min((int)A.row_tile, s.q.rows - j0) * (int)GR;
             const int limit = (int)rho < nrows ? s.q.len - s.q.n + j0 + (int)(rho / GR) + 1 : 0;  // positions the row attends
             const int all = max(0, s.q.len - s.q.n + j0 + 1);                                      // positions every row attends
-            wait(sh.q_full + seg % K4T_SEGS, seg / K4T_SEGS);
-            const float f = sh.factor[seg % K4T_SEGS][at];
+            wait(sh.q_full + seg % SEGS, seg / SEGS);
+            const float f = sh.factor[seg % SEGS][GROUPS == 2 ? tid : at];
             float m = -3.4e38f, l = 0.f;   // m: the maximum less P_UP
-            unsigned mine = 0;             // tiles of this group so far
-            for (int t = t0; t < t1; ++t, ++n) {
-                const unsigned b = n & 1;
-                if (GROUPS == 2 && b != wg) continue;
+            const bool mine = GROUPS == 1 || wg == 0 || nrows > 128;  // whether the group has rows
+            const unsigned tiles = (unsigned)(t1 - t0);
+            if (!mine) n += tiles;
+            for (int t = t0; mine && t < t1; ++t, ++n, ++k) {
+                // S of a tile: the group's, or the tile's of two; what it waits for has come k, or k / 2, times before
+                const unsigned b = GROUPS == 2 ? wg : k & 1, turn = GROUPS == 2 ? k : k >> 1;
                 wait(sh.meta_full + n % K4T_META, n / K4T_META);
                 const unsigned here = sh.here[n % K4T_META];
-                wait(sh.s_full + b, n >> 1);
+                wait(sh.s_full + b, turn);
                 kt_fence_after();
                 const uint32_t s_at = tmem + lanes + b * 128 + first, p_at = tmem + lanes + b * 128 + S::P;
                 if (__builtin_expect(here != 0xffu || (t + 1) * K4_TILE > all, 0)) {
@@ -213,8 +229,8 @@ __global__ void __launch_bounds__(k4t_threads(NR), 1) kv4_tiles_kernel(const __g
                     const float now = up ? top - P_UP : m, alpha = up ? ex2(m - now) : 1.f;
                     m = now;
                     l *= alpha;
-                    if (mine) {
-                        if (GROUPS == 2) wait(sh.o_done + b, (n >> 1) - 1); else wait(sh.o_done + (b ^ 1), (n - 1) >> 1);
+                    if (t > t0) {
+                        if (GROUPS == 2) wait(sh.o_done + b, k - 1); else wait(sh.o_done + (b ^ 1), (k - 1) >> 1);
                         kt_fence_after();
 #pragma unroll 1
                         for (int c = 0; c < HD; c += 16) {
@@ -265,79 +281,108 @@ __global__ void __launch_bounds__(k4t_threads(NR), 1) kv4_tiles_kernel(const __g
                 kt_wait_st();
                 kt_fence_before();
                 arrive(sh.p_full + b);
-                ++mine;
             }
-            // ---- the segment's part: what copies and groups hold of a row, joined
-            if (mine) {
-                const unsigned last = n - 1 - (GROUPS == 2 && ((n - 1) & 1) != wg ? 1 : 0);
-                wait(sh.o_done + (last & 1), last >> 1);
-            }
-            kt_fence_after();
-            sh.ml[tid] = make_float2(m, l);
-            bar();
+            // ---- the segment's part
             const bool whole = s.t0 == 0 && s.t1 == s.tiles;
-            constexpr unsigned PARTS = GROUPS * CP;
-            float own;
-            {
-                float top = -INFINITY, sum = 0.f;
-#pragma unroll
-                for (unsigned p = 0; p < PARTS; ++p) top = fmaxf(top, sh.ml[p * NR + rho].x);
-#pragma unroll
-                for (unsigned p = 0; p < PARTS; ++p) {
-                    const float2 y = sh.ml[p * NR + rho];
-                    sum = fmaf(y.y, ex2(y.x - top), sum);
-                }
-                own = ex2(m - top);
-                if (whole) own *= sum > 0.f || isnan(sum) ? 1.f / sum : 0.f;
-                if (tid < NR) sh.joined[rho] = make_float2(top, sum);
-            }
             const Kv8Parts of = kv8_parts(s, sh.place);
-            auto put = [&](unsigned row, unsigned chunk, float4 v) {
+            auto place_of = [&](unsigned row) {
                 const size_t r = (size_t)(s.q.first + j0 + (int)(row / GR));
-                kv8_store4(A.out, A.type, r * A.out_stride + (size_t)(s.head * GR + row % GR) * HD + 4 * chunk, v);
+                return r * A.out_stride + (size_t)(s.head * GR + row % GR) * HD;
             };
-#pragma unroll 1
-            for (unsigned c = 0; c < HD; c += 16) {
-                float y[16];
+            auto put = [&](unsigned row, unsigned chunk, float4 v) { kv8_store4(A.out, A.type, place_of(row) + 4 * chunk, v); };
+            // columns 8 chunk.. of a row, in the order of a word's numbers
+            auto leave = [&](unsigned row, size_t out, unsigned chunk, const float *z) {
+                const float4 lo = make_float4(z[0], z[2], z[4], z[6]), hi = make_float4(z[1], z[3], z[5], z[7]);
+                if (!whole) {
+                    float4 *o = reinterpret_cast<float4 *>(A.part_o + ((size_t)of.slot * NR + row) * HD) + 2 * chunk;
+                    o[0] = lo;
+                    o[1] = hi;
+                } else if (A.vec_out) {
+                    auto two = [&](float x, float y) {
+                        if (A.type == T_F16) return kt_pack(x, y);
+                        const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+                        return *reinterpret_cast<const unsigned *>(&h);
+                    };
+                    *reinterpret_cast<uint4 *>(static_cast<unsigned short *>(A.out) + out + 8 * chunk) =
+                        make_uint4(two(lo.x, lo.y), two(lo.z, lo.w), two(hi.x, hi.y), two(hi.z, hi.w));
+                } else {
+                    kv8_store4(A.out, A.type, out + 8 * chunk, lo);
+                    kv8_store4(A.out, A.type, out + 8 * chunk + 4, hi);
+                }
+            };
+            if constexpr (GROUPS == 2) {
                 if (mine) {
+                    wait(sh.o_done + wg, k - 1);
+                    kt_fence_after();
+                    const float own = !whole ? 1.f : l > 0.f || isnan(l) ? 1.f / l : 0.f;
+                    const bool real = (int)rho < nrows;
+                    const size_t out = real ? place_of(rho) : 0;
+#pragma unroll 1
+                    for (unsigned c = 0; c < HD; c += 16) {
+                        float y[16];
+                        kt_ld16(o_at + c, y);
+                        kt_wait_ld();
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) y[i] *= own;
+                        if (real) {
+                            leave(rho, out, c / 8, y);
+                            leave(rho, out, c / 8 + 1, y + 8);
+                        }
+                    }
+                    kt_fence_before();
+                    arrive(sh.o_free + wg);
+                    if (!whole && real) A.part_ml[(size_t)of.slot * NR + rho] = make_float2(m, l);
+                }
+            } else {
+                // what the copies hold of a row, joined
+                wait(sh.o_done + ((k - 1) & 1), (k - 1) >> 1);
+                kt_fence_after();
+                sh.ml[tid] = make_float2(m, l);
+                bar();
+                float own;
+                {
+                    float top = -INFINITY, sum = 0.f;
+#pragma unroll
+                    for (unsigned p = 0; p < CP; ++p) top = fmaxf(top, sh.ml[p * NR + rho].x);
+#pragma unroll
+                    for (unsigned p = 0; p < CP; ++p) {
+                        const float2 y = sh.ml[p * NR + rho];
+                        sum = fmaf(y.y, ex2(y.x - top), sum);
+                    }
+                    own = ex2(m - top);
+                    if (whole) own *= sum > 0.f || isnan(sum) ? 1.f / sum : 0.f;
+                    if (!whole && (int)tid < nrows) A.part_ml[(size_t)of.slot * NR + tid] = make_float2(top, sum);
+                }
+#pragma unroll 1
+                for (unsigned c = 0; c < HD; c += 16) {
+                    float y[16];
                     kt_ld16(o_at + c, y);
                     kt_wait_ld();
-                }
 #pragma unroll
-                for (int i = 0; i < 16; i += 4)
-                    *reinterpret_cast<float4 *>(stage + tid * S::O_STRIDE + i) = mine ? make_float4(y[i] * own, y[i + 1] * own, y[i + 2] * own, y[i + 3] * own)
-                                                                                      : make_float4(0.f, 0.f, 0.f, 0.f);
-                bar();
-                for (unsigned i = tid; i < (unsigned)nrows * 2; i += 32 * SOFT) {
-                    const unsigned row = i >> 1, half = i & 1;
-                    float z[8];
+                    for (int i = 0; i < 16; i += 4)
+                        *reinterpret_cast<float4 *>(stage + tid * S::O_STRIDE + i) = make_float4(y[i] * own, y[i + 1] * own, y[i + 2] * own, y[i + 3] * own);
+                    bar();
+                    for (unsigned i = tid; i < (unsigned)nrows * 2; i += 32 * SOFT) {
+                        const unsigned row = i >> 1, half = i & 1;
+                        float z[8];
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) z[j] = 0.f;
+                        for (int j = 0; j < 8; ++j) z[j] = 0.f;
 #pragma unroll
-                    for (unsigned p = 0; p < PARTS; ++p)
+                        for (unsigned p = 0; p < CP; ++p)
 #pragma unroll
-                        for (int j = 0; j < 8; j += 4) {
-                            const float4 u = *reinterpret_cast<const float4 *>(stage + (p * NR + row) * S::O_STRIDE + 8 * half + j);
-                            z[j] += u.x; z[j + 1] += u.y; z[j + 2] += u.z; z[j + 3] += u.w;
-                        }
-                    const float4 lo = make_float4(z[0], z[2], z[4], z[6]), hi = make_float4(z[1], z[3], z[5], z[7]);
-                    const unsigned chunk = (c + 8 * half) / 4;
-                    if (whole) {
-                        put(row, chunk, lo);
-                        put(row, chunk + 1, hi);
-                    } else {
-                        float4 *o = reinterpret_cast<float4 *>(A.part_o + ((size_t)of.slot * NR + row) * HD);
-                        o[chunk] = lo;
-                        o[chunk + 1] = hi;
+                            for (int j = 0; j < 8; j += 4) {
+                                const float4 u = *reinterpret_cast<const float4 *>(stage + (p * NR + row) * S::O_STRIDE + 8 * half + j);
+                                z[j] += u.x; z[j + 1] += u.y; z[j + 2] += u.z; z[j + 3] += u.w;
+                            }
+                        leave(row, place_of(row), c / 8 + half, z);
                     }
+                    bar();
                 }
-                bar();
+                kt_fence_before();
+                arrive(sh.o_free);
             }
-            kt_fence_before();
-            arrive(sh.o_free + wg);
             if (!whole) {
-                if ((int)tid < nrows) A.part_ml[(size_t)of.slot * NR + tid] = sh.joined[tid];
-                kv8_arrive<NR, HD, 32 * SOFT>(A, of, tid, (unsigned)nrows, stage, GROUPS * 128 * S::O_STRIDE, &sh.flag, bar, put);
+                kv8_arrive<NR, HD, 32 * SOFT, 4>(A, of, tid, (unsigned)nrows, stage, S::STAGED, &sh.flag, bar, put);
                 bar();
             }
             done();
@@ -350,7 +395,7 @@ __global__ void __launch_bounds__(k4t_threads(NR), 1) kv4_tiles_kernel(const __g
         while (const Kv8Segment *sp = next()) {
             const Kv8Segment &s = *sp;
             const int any = kv8_attended(A, s.q, s.row_tile), t0 = s.t0, t1 = s.t1;
-            if (!is_v) {
+            if (GROUPS == 2 || !is_v) {
                 // ---- q rows by a power of two each. The score factor's sign goes with q: a row's largest product is its
                 // largest score
                 const int j0 = s.row_tile * (int)A.row_tile, nrows = min((int)A.row_tile, s.q.rows - j0) * (int)GR;
@@ -394,44 +439,43 @@ __global__ void __launch_bounds__(k4t_threads(NR), 1) kv4_tiles_kernel(const __g
                         kt_st16(tmem + (cw << 21) + S::Q + i / 2, reinterpret_cast<const float *>(h));
                     }
                     kt_wait_st();
-                    sh.factor[seg % K4T_SEGS][ct] = factor_of(e);
+                    sh.factor[seg % SEGS][ct] = factor_of(e);
                     kt_fence_before();
                 } else {
                     // to shared memory, eight values a lane
-                    constexpr unsigned LANES = HD / 8, STEP = 32 / LANES, STEPS = NR / K4T_CONV / STEP, AHEAD = 4;  // lanes of a row, rows of a load
-                    const unsigned piece = lane % LANES;
+                    constexpr unsigned LANES = HD / 8, STEP = 32 / LANES, STEPS = NR / (2 * K4T_CONV) / STEP, AHEAD = 4;  // lanes of a row, rows of a load
+                    const unsigned piece = lane % LANES, row0 = (warp - W_CONV) * STEPS * STEP + lane / LANES;
 #pragma unroll 1
                     for (unsigned i = 0; i < STEPS; i += AHEAD) {
                         float4 x[AHEAD][2];
 #pragma unroll
                         for (unsigned u = 0; u < AHEAD; ++u) {
-                            const unsigned rho = (cw * STEPS + i + u) * STEP + lane / LANES;
+                            const unsigned rho = row0 + (i + u) * STEP;
                             x[u][0] = x[u][1] = make_float4(0.f, 0.f, 0.f, 0.f);
                             if ((int)rho < nrows) k4t_load8(A, at_of(rho) + 8 * piece, x[u][0], x[u][1]);
                         }
                         if (seg && i == 0) wait(&sh.q_empty, seg - 1);  // the last segment's products have read their q
 #pragma unroll
                         for (unsigned u = 0; u < AHEAD; ++u) {
-                            const unsigned rho = (cw * STEPS + i + u) * STEP + lane / LANES;
+                            const unsigned rho = row0 + (i + u) * STEP;
                             const int e = 12 - kt_exponent(group_max<LANES>(fmaxf(size_of(x[u][0]), size_of(x[u][1]))));
-                            *reinterpret_cast<uint4 *>(ring + S::OFF_Q + piece / 8 * S::HALF + rho * 128 + ((piece % 8 ^ (rho & 7u)) << 4)) =
+                            *reinterpret_cast<uint4 *>(ring + S::OFF_Q + rho / 128 * S::TILE + piece / 8 * S::HALF + rho % 128 * 128 + ((piece % 8 ^ (rho & 7u)) << 4)) =
                                 halves(x[u][0], x[u][1], e);
-                            if (piece == 0) sh.factor[seg % K4T_SEGS][rho] = factor_of(e);
+                            if (piece == 0) sh.factor[seg % SEGS][rho] = factor_of(e);
                         }
                     }
                 }
                 fence_proxy_async();
-                arrive(sh.q_full + seg % K4T_SEGS);
+                arrive(sh.q_full + seg % SEGS);
             }
             for (int t = t0; t < t1; ++t, ++n) {
-                const unsigned b = n & 1, st = n % S::STAGES;
-                wait(sh.raw_full + st, n / S::STAGES);
+                const unsigned b = n & 1, stages = is_v ? S::VS : S::KS, st = n % stages;
+                wait((is_v ? sh.rv_full : sh.rk_full) + st, n / stages);
                 if (n >= 2) wait((is_v ? sh.v_empty : sh.k_empty) + b, (n >> 1) - 1);
-                const unsigned char *raw = ring + S::OFF_RAW + st * S::RAW + (is_v ? S::RAW_V : 0);
-                const unsigned char *scales = ring + S::OFF_RAW + st * S::RAW + (is_v ? S::RAW_VS : S::RAW_KS);
+                const unsigned char *raw = ring + (is_v ? S::OFF_RV : S::OFF_RK) + st * S::RAW, *scales = raw + S::RAW_S;
                 unsigned char *dst = ring + (is_v ? S::OFF_V : S::OFF_K) + b * S::TILE;
                 // V of positions that no row attends, or never loaded, is 0 and not what lies there (a NaN stays one times 0)
-                const unsigned here = sh.raw_here[st];
+                const unsigned here = sh.here[n % K4T_META];
                 const bool patchy = is_v && (here != 0xffu || any < (t + 1) * K4_TILE);
                 // four tokens' words and scales at a time, before the first of their stores (which they might overlap, as
                 // far as the compiler can tell: a token after the other took 1500 cycles a tile)
@@ -470,7 +514,7 @@ __global__ void __launch_bounds__(k4t_threads(NR), 1) kv4_tiles_kernel(const __g
                         }
                     }
                 }
-                arrive(sh.raw_empty + st);
+                arrive((is_v ? sh.rv_empty : sh.rk_empty) + st);
                 fence_proxy_async();
                 arrive((is_v ? sh.v_full : sh.k_full) + b);
             }
@@ -484,10 +528,10 @@ __global__ void __launch_bounds__(k4t_threads(NR), 1) kv4_tiles_kernel(const __g
         Kv8Segment s;
         for (;; ++seg) {
             const bool more = walk.next(s);
-            if (seg >= K4T_SEGS) wait(sh.seg_empty + seg % K4T_SEGS, seg / K4T_SEGS - 1);
+            if (seg >= SEGS) wait(sh.seg_empty + seg % SEGS, seg / SEGS - 1);
             if (lane == 0 && !*dead) {
-                if (more) sh.seg[seg % K4T_SEGS] = s; else sh.seg[seg % K4T_SEGS].t1 = 0;
-                mbar_arrive(sh.seg_full + seg % K4T_SEGS);
+                if (more) sh.seg[seg % SEGS] = s; else sh.seg[seg % SEGS].t1 = 0;
+                mbar_arrive(sh.seg_full + seg % SEGS);
             }
             __syncwarp();
             if (!more) break;
@@ -505,35 +549,39 @@ __global__ void __launch_bounds__(k4t_threads(NR), 1) kv4_tiles_kernel(const __g
                         id = -1;
                     }
                 }
-                const unsigned st = n % S::STAGES;
-                if (n >= S::STAGES) wait(sh.raw_empty + st, n / S::STAGES - 1);
                 const int own = __shfl_sync(0xffffffffu, id, (b0 & 31) + (int)(lane % per));
                 const bool load = lane < per && own >= 0;
                 const unsigned boxes = __ballot_sync(0xffffffffu, load);
                 // groups of 16 positions whose block is among the loaded ones
                 const unsigned groups = __ballot_sync(0xffffffffu, lane < K4_TILE / 16 && (boxes >> (lane * 16 / box) & 1));
-                if (lane == 0) {
-                    sh.here[n % K4T_META] = groups;
-                    sh.raw_here[st] = groups;
-                    mbar_arrive(sh.meta_full + n % K4T_META);
-                    if (boxes) mbar_expect_tx(sh.raw_full + st, __popc(boxes) * 2 * box * (S::ROW + S::SCALES)); else mbar_arrive(sh.raw_full + st);
-                }
-                __syncwarp();
-                if (load && !*dead) {
-                    const unsigned row = (((unsigned)own * kv + s.head) << A.shift) + ((unsigned)(t * K4_TILE) & (size - 1));
-                    unsigned char *dst = ring + S::OFF_RAW + st * S::RAW;
-                    tma_load_rows(dst + lane * box * S::ROW, &kmap, (int)row, sh.raw_full + st);
-                    tma_load_rows(dst + S::RAW_V + lane * box * S::ROW, &vmap, (int)row, sh.raw_full + st);
-                    bulk_copy_g2s(dst + S::RAW_KS + lane * box * S::SCALES, A.ks + (size_t)row * G64, box * S::SCALES, sh.raw_full + st);
-                    bulk_copy_g2s(dst + S::RAW_VS + lane * box * S::SCALES, A.vs + (size_t)row * G64, box * S::SCALES, sh.raw_full + st);
-                }
-                __syncwarp();
+                const unsigned row = (((unsigned)own * kv + s.head) << A.shift) + ((unsigned)(t * K4_TILE) & (size - 1));
+                auto bring = [&](const CUtensorMap &map, const __half2 *scale, unsigned off, unsigned stages, uint64_t *full, uint64_t *empty, bool first) {
+                    const unsigned st = n % stages;
+                    if (n >= stages) wait(empty + st, n / stages - 1);
+                    if (lane == 0) {
+                        if (first) {
+                            sh.here[n % K4T_META] = groups;
+                            mbar_arrive(sh.meta_full + n % K4T_META);
+                        }
+                        if (boxes) mbar_expect_tx(full + st, __popc(boxes) * box * (S::ROW + S::SCALES)); else mbar_arrive(full + st);
+                    }
+                    __syncwarp();
+                    if (load && !*dead) {
+                        unsigned char *dst = ring + off + st * S::RAW;
+                        tma_load_rows(dst + lane * box * S::ROW, &map, (int)row, full + st);
+                        bulk_copy_g2s(dst + S::RAW_S + lane * box * S::SCALES, scale + (size_t)row * G64, box * S::SCALES, full + st);
+                    }
+                    __syncwarp();
+                };
+                bring(kmap, A.ks, S::OFF_RK, S::KS, sh.rk_full, sh.rk_empty, true);
+                bring(vmap, A.vs, S::OFF_RV, S::VS, sh.rv_full, sh.rv_empty, false);
             }
         }
         if (*dead) {  // copies in flight land before the CTA leaves its shared memory
-            for (unsigned i = 0; i < min(n, (unsigned)S::STAGES); ++i) {
+            for (unsigned i = 0; i < min(n, 4u); ++i) {
                 const unsigned k = n - 1 - i;
-                mbar_wait_bounded(sh.raw_full + k % S::STAGES, k / S::STAGES & 1);
+                if (i < S::KS) mbar_wait_bounded(sh.rk_full + k % S::KS, k / S::KS & 1);
+                if (i < S::VS) mbar_wait_bounded(sh.rv_full + k % S::VS, k / S::VS & 1);
             }
         }
     } else {
@@ -542,52 +590,75 @@ __global__ void __launch_bounds__(k4t_threads(NR), 1) kv4_tiles_kernel(const __g
         const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
         const uint64_t qs = kt_desc(smem_u32(ring + S::OFF_Q), 16), ks = kt_desc(smem_u32(ring + S::OFF_K), 16),
                        vs = kt_desc(smem_u32(ring + S::OFF_V), S::HALF);
-        unsigned at = 0;  // tiles whose scores have been asked for
-        auto scores = [&](bool last) {
-            const unsigned b = at & 1;
-            wait(sh.k_full + b, at >> 1);
-            if (at >= 2) wait(sh.o_done + b, (at >> 1) - 1);  // P of the tile before the last, in this S, has been read
+        // what has been asked for so far: scores and values (tiles; each group's), segments of a group
+        unsigned ns = 0, scored[2] = {0, 0}, valued[2] = {0, 0}, segs[2] = {0, 0};
+        auto scores = [&](unsigned g, bool last_group, bool last) {
+            const unsigned b = GROUPS == 2 ? g : ns & 1, turn = GROUPS == 2 ? scored[g] : ns >> 1;
+            if (turn) wait(sh.o_done + b, turn - 1);  // P in this S has been read
             kt_fence_after();
             __syncwarp();
             if (kt_elect()) {
 #pragma unroll
                 for (int k = 0; k < HD / 16; ++k) {
-                    const uint64_t step = (uint64_t)((k / 4 * S::HALF + k % 4 * 32) >> 4);
-                    if constexpr (S::Q_TM) kt_mma(tm + b * 128, tm + S::Q + 8 * k, ks + (b * S::TILE >> 4) + step, kt_idesc(128, false), k > 0);
-                    else kt_mma_ss(tm + b * 128, qs + step, ks + (b * S::TILE >> 4) + step, kt_idesc(128, false), k > 0);
+                    const uint64_t step = (uint64_t)((k / 4 * S::HALF + k % 4 * 32) >> 4), kt = ks + ((ns & 1) * S::TILE >> 4) + step;
+                    if constexpr (S::Q_TM) kt_mma(tm + b * 128, tm + S::Q + 8 * k, kt, kt_idesc(128, false), k > 0);
+                    else kt_mma_ss(tm + b * 128, qs + (g * S::TILE >> 4) + step, kt, kt_idesc(128, false), k > 0);
                 }
-                kt_commit(sh.k_empty + b);
+                if (last_group) kt_commit(sh.k_empty + (ns & 1));
                 kt_commit(sh.s_full + b);
-                if (last) kt_commit(&sh.q_empty);
+                if (last_group && last) kt_commit(&sh.q_empty);
             }
             __syncwarp();
-            ++at;
+            ++scored[g];
+        };
+        auto values = [&](unsigned g, bool last_group, bool first) {
+            const unsigned b = GROUPS == 2 ? g : n & 1, turn = GROUPS == 2 ? valued[g] : n >> 1;
+            wait(sh.p_full + b, turn);
+            if (first && segs[g]) wait(sh.o_free + g, segs[g] - 1);
+            kt_fence_after();
+            __syncwarp();
+            if (kt_elect()) {
+#pragma unroll
+                for (int k = 0; k < K4_TILE / 16; ++k)
+                    kt_mma(tm + S::O + g * HD, tm + b * 128 + S::P + 8 * k, vs + (((n & 1) * S::TILE + k * 2048) >> 4), kt_idesc(HD, true), !first || k);
+                if (last_group) kt_commit(sh.v_empty + (n & 1));
+                kt_commit(sh.o_done + b);
+            }
+            __syncwarp();
+            ++valued[g];
+            if (first) ++segs[g];
         };
         while (const Kv8Segment *s = next()) {
-            wait(sh.q_full + seg % K4T_SEGS, seg / K4T_SEGS);
+            wait(sh.q_full + seg % SEGS, seg / SEGS);
             const int tiles = s->t1 - s->t0;
-            unsigned begun = 0;  // groups whose O of this segment holds something
+            const int nrows = min((int)A.row_tile, s->q.rows - s->row_tile * (int)A.row_tile) * (int)GR;
+            const bool two = GROUPS == 2 && nrows > 128;
+            auto ask = [&](unsigned g, int t) {
+                if (g == 0) wait(sh.k_full + (ns & 1), ns >> 1);
+                const bool last_group = g || !two;
+                scores(g, last_group, t + 1 == tiles);
+                if (last_group) ++ns;
+            };
+            auto give = [&](unsigned g, int t) {
+                if (g == 0) wait(sh.v_full + (n & 1), n >> 1);
+                const bool last_group = g || !two;
+                values(g, last_group, t == 0);
+                if (last_group) ++n;
+            };
+            // one group: scores a tile ahead of values. Two: P takes the place of a group's scores, so its next come after,
+            // and the other group's weights are made meanwhile
+            ask(0, 0);
+            if (two) ask(1, 0);
 #pragma unroll 1
-            for (int t = -1; t < tiles; ++t) {  // scores one tile ahead of values
-                if (t + 1 < tiles) scores(t + 2 == tiles);
-                if (t < 0) continue;
-                const unsigned b = n & 1, g = GROUPS == 2 ? b : 0;
-                wait(sh.v_full + b, n >> 1);
-                wait(sh.p_full + b, n >> 1);
-                if (!(begun >> g & 1) && seg) wait(sh.o_free + g, seg - 1);
-                kt_fence_after();
-                __syncwarp();
-                if (kt_elect()) {
-#pragma unroll
-                    for (int k = 0; k < K4_TILE / 16; ++k)
-                        kt_mma(tm + S::O + g * HD, tm + b * 128 + S::P + 8 * k, vs + ((b * S::TILE + k * 2048) >> 4),
-                               kt_idesc(HD, true), (begun >> g & 1) || k);
-                    kt_commit(sh.v_empty + b);
-                    kt_commit(sh.o_done + b);
+            for (int t = 0; t < tiles; ++t) {
+                const bool more = t + 1 < tiles;
+                if (GROUPS == 1 && more) ask(0, t + 1);
+                give(0, t);
+                if (GROUPS == 2 && more) ask(0, t + 1);
+                if (two) {
+                    give(1, t);
+                    if (more) ask(1, t + 1);
                 }
-                __syncwarp();
-                begun |= 1u << g;
-                ++n;
             }
             done();
         }

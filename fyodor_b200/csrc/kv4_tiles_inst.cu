@@ -5,7 +5,7 @@
 
 #ifndef FYB_K4_HD
 #define FYB_K4_HD 128
-#define FYB_K4_NR 128
+#define FYB_K4_NR 256
 #endif
 #define FYB_K4_NAME2(hd, nr) kv4_tiles_##hd##_##nr
 #define FYB_K4_NAME(hd, nr) FYB_K4_NAME2(hd, nr)
