@@ -14,6 +14,28 @@ namespace fyb {
 
 constexpr unsigned KV4_THREADS = 256;
 
+// Where a CTA's threads stand among rows of `per_row` words: rows of a CTA, or CTAs of a row.
+struct Kv4Grid {
+    unsigned per_row, rows, parts;  // rows of a CTA (1 where a row has parts)
+};
+inline Kv4Grid kv4_grid(unsigned per_row)
+{
+    return Kv4Grid{per_row, per_row < KV4_THREADS ? KV4_THREADS / per_row : 1, (per_row + KV4_THREADS - 1) / KV4_THREADS};
+}
+// Thread's row and word of it; false for a thread that has none.
+FYB_DEV bool kv4_place(const Kv4Grid &g, unsigned cta, size_t rows, size_t &row, unsigned &j)
+{
+    if (g.rows == 1) {
+        row = cta / g.parts;
+        j = cta % g.parts * KV4_THREADS + threadIdx.x;
+        return j < g.per_row;
+    }
+    const unsigned r = threadIdx.x / g.per_row;
+    row = (size_t)cta * g.rows + r;
+    j = threadIdx.x % g.per_row;
+    return r < g.rows && row < rows;
+}
+
 struct Kv4Append {
     fyb_kv4_cache c;
     const int *slots, *positions;
@@ -23,59 +45,69 @@ struct Kv4Append {
     RopeRows q;       // rotated in the same launch where rows are few (heads 0: none)
     RopeWork work;
     unsigned shift, ctas, q_rows;  // ctas: of K and V; q_rows: CTAs of a row of q
+    Kv4Grid grid;
     bool vec, many;
     unsigned *error;
 };
 
-// Eight values from e of a row's head in F32, rotated when `turn`; row: the head's first value.
-template <typename T> FYB_DEV void kv4_load(const Kv4Append &A, const T *row, unsigned e, bool turn, size_t tab, float (&x)[8])
+// Eight values of a row's head as they lie there, and of the other half where half pairs are turned.
+template <typename T> struct Kv4Raw {
+    static constexpr int V = 16 / sizeof(T);
+    RopePack<T, V> own[8 / V], other[8 / V];
+};
+// The eight from e (aligned accesses): asked for before slot and position have come.
+template <typename T> FYB_DEV void kv4_ask(const Kv4Append &A, const T *row, unsigned e, bool turn, Kv4Raw<T> &r)
+{
+    constexpr int V = Kv4Raw<T>::V;
+    const unsigned pairs = A.rope.dims / 2;
+#pragma unroll
+    for (int i = 0; i < 8 / V; ++i) r.own[i] = rope_get<T, V, true>(row + e + i * V);
+    if (turn && A.rope.layout != 0 && e < A.rope.dims) {
+        const unsigned o = e < pairs ? e + pairs : e - pairs;
+#pragma unroll
+        for (int i = 0; i < 8 / V; ++i) r.other[i] = rope_get<T, V, true>(row + o + i * V);
+    }
+}
+// The same in F32, rotated when `turn`; tab: the position's place in the tables.
+template <typename T> FYB_DEV void kv4_turn(const Kv4Append &A, const Kv4Raw<T> &r, unsigned e, bool turn, size_t tab, float (&x)[8])
+{
+    constexpr int V = Kv4Raw<T>::V;
+    const unsigned dims = A.rope.dims, pairs = dims / 2;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = row_value(r.own[i / V].t[i % V]);
+    if (!turn || e >= dims) return;
+    if (A.rope.layout == 0) {
+        float cv[4], sv[4];
+        rope_row<4, true>(A.rope.cos + tab + e / 2, cv);
+        rope_row<4, true>(A.rope.sin + tab + e / 2, sv);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) rope_turn(x[2 * i], x[2 * i + 1], cv[i], sv[i]);
+    } else {
+        const bool low = e < pairs;  // pairs is a multiple of 8: the eight lie in one half
+        const unsigned p = low ? e : e - pairs;
+        float cv[8], sv[8];
+        rope_row<8, true>(A.rope.cos + tab + p, cv);
+        rope_row<8, true>(A.rope.sin + tab + p, sv);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            float o = row_value(r.other[i / V].t[i % V]);
+            if (low) rope_turn(x[i], o, cv[i], sv[i]); else rope_turn(o, x[i], cv[i], sv[i]);
+        }
+    }
+}
+// Both, one value at a time, for rows and tables that begin anywhere.
+template <typename T> __device__ __noinline__ void kv4_load(const Kv4Append &A, const T *row, unsigned e, bool turn, size_t tab, float *x)
 {
     const float *c = A.rope.cos + tab, *s = A.rope.sin + tab;
     const unsigned dims = A.rope.dims, pairs = dims / 2;
-    if (A.vec) {
-        constexpr int V = 16 / sizeof(T);
-        auto eight = [](const T *p, float (&y)[8]) {
-#pragma unroll
-            for (int i = 0; i < 8; i += V) {
-                const RopePack<T, V> u = rope_get<T, V, true>(p + i);
-#pragma unroll
-                for (int j = 0; j < V; ++j) y[i + j] = row_value(u.t[j]);
-            }
-        };
-        eight(row + e, x);
-        if (!turn || e >= dims) return;
+    for (int i = 0; i < 8; ++i) {
+        const unsigned d = e + i;
+        x[i] = row_value(row[d]);
+        if (!turn || d >= dims) continue;
         if (A.rope.layout == 0) {
-            float cv[4], sv[4];
-            rope_row<4, true>(c + e / 2, cv);
-            rope_row<4, true>(s + e / 2, sv);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) rope_turn(x[2 * i], x[2 * i + 1], cv[i], sv[i]);
+            float o = row_value(row[d ^ 1]);
+            if (d & 1) rope_turn(o, x[i], c[d / 2], s[d / 2]); else rope_turn(x[i], o, c[d / 2], s[d / 2]);
         } else {
-            const bool low = e < pairs;  // pairs is a multiple of 8: the eight lie in one half
-            const unsigned p = low ? e : e - pairs;
-            float o[8], cv[8], sv[8];
-            eight(row + (low ? e + pairs : p), o);
-            rope_row<8, true>(c + p, cv);
-            rope_row<8, true>(s + p, sv);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                if (low) rope_turn(x[i], o[i], cv[i], sv[i]); else rope_turn(o[i], x[i], cv[i], sv[i]);
-            }
-        }
-        return;
-    }
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = row_value(row[e + i]);
-    if (!turn) return;
-    if (A.rope.layout == 0) {
-#pragma unroll
-        for (int i = 0; i < 8; i += 2)
-            if (e + i < dims) rope_turn(x[i], x[i + 1], c[(e + i) / 2], s[(e + i) / 2]);
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const unsigned d = e + i;
-            if (d >= dims) continue;
             const bool low = d < pairs;
             const unsigned p = low ? d : d - pairs;
             float o = row_value(row[low ? d + pairs : p]);
@@ -84,38 +116,53 @@ template <typename T> FYB_DEV void kv4_load(const Kv4Append &A, const T *row, un
     }
 }
 
-// The number nearest to (x - low) / scale, 0..15, ties to even. `inv` is the F32 reciprocal of scale: the F32 quotient
-// y is within 4e-6 of the real one where it matters (0 <= y <= 15.1), so only next to a border between two numbers is
-// more needed: there x and the border, exact in 64 bits, are compared.
-FYB_DEV unsigned kv4_number(float x, float low, float scale, float inv)
+FYB_DEV float max_nan(float a, float b)  // NaN where one is
 {
-    const float y = fminf(fmaxf(__fmul_rn(__fsub_rn(x, low), inv), 0.f), 15.f);  // NaN to 0
-    const float n = rintf(y);
-    if (fabsf(fabsf(y - n) - 0.5f) > 1e-5f) return (unsigned)n;
-    const unsigned k = (unsigned)y;
-    const double border = (double)low + ((double)k + 0.5) * (double)scale;
-    return x > border || (x == border && (k & 1)) ? k + 1 : k;
+    float y;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+    return y;
+}
+// Eight numbers one by one: nearest to (x - low) / scale, 0..15, ties to even. `inv` is the F32 reciprocal of scale: the
+// F32 quotient y is within 4e-6 of the real one where it matters (0 <= y <= 15.1), so only next to a border between two
+// numbers is more needed: there x and the border, exact in 64 bits, are compared. NaN is held as 0 would be.
+static __device__ __noinline__ unsigned kv4_numbers(const float *x, float low, float scale, float inv)
+{
+    unsigned bits = 0;
+    if (!(scale > 0.f)) return 0;
+#pragma unroll 1
+    for (int t = 0; t < 8; ++t) {
+        const float v = isnan(x[t]) ? 0.f : x[t], y = fminf(fmaxf(__fmul_rn(__fsub_rn(v, low), inv), 0.f), 15.f), n = rintf(y);
+        unsigned k = (unsigned)n;
+        if (fabsf(fabsf(y - n) - 0.5f) <= 1e-5f) {
+            k = (unsigned)y;
+            const double border = (double)low + ((double)k + 0.5) * (double)scale;
+            if (v > border || (v == border && (k & 1))) ++k;
+        }
+        bits |= k << (4 * t);
+    }
+    return bits;
 }
 
-// CTAs of K and V: thread = word w of one head of one row of K or V; then those of q.
-template <typename T, int HD> __global__ void __launch_bounds__(KV4_THREADS) kv4_append_kernel(Kv4Append A)
+// CTAs of K and V: thread = word w of one head of one row of K or V; with Q then those of q.
+template <typename T, int HD, bool Q> __global__ void __launch_bounds__(KV4_THREADS) kv4_append_kernel(const __grid_constant__ Kv4Append A)
 {
     constexpr unsigned WORDS = HD / 8, GROUPS = HD / KV4_GROUP;
-    if (blockIdx.x >= A.ctas) {
+    if (Q && blockIdx.x >= A.ctas) {
         rope_row_of_q<T, HD, KV4_THREADS>(A, blockIdx.x - A.ctas);
         return;
     }
-    const unsigned per_row = 2 * A.c.kv_heads * WORDS;
-    const size_t i = (size_t)blockIdx.x * KV4_THREADS + threadIdx.x;
-    const size_t row = i / per_row;
-    const unsigned j = (unsigned)(i % per_row);
-    const bool is_k = j < per_row / 2;
-    const unsigned head = (is_k ? j : j - per_row / 2) / WORDS, lane = j % WORDS;
+    size_t row;
+    unsigned j;
+    const bool real = kv4_place(A.grid, blockIdx.x, A.rows, row, j);
+    const bool is_k = j < A.grid.per_row / 2;
+    const unsigned head = (is_k ? j : j - A.grid.per_row / 2) / WORDS, lane = j % WORDS;
     const unsigned group = lane / 8, word = (lane % 8) * GROUPS + group, e = kv4_first<HD>(word);
     const bool turn = is_k && A.rope.cos;
-    // the eight lanes of a group take the same way
-    int slot = -1, pos = 0;
-    if (row < A.rows) {
+    const T *src = static_cast<const T *>(is_k ? A.k : A.v) + row * (is_k ? A.k_stride : A.v_stride) + (size_t)head * HD;
+    int slot = -1, pos = 0;  // the eight lanes of a group take the same way
+    Kv4Raw<T> raw;
+    if (real) {
+        if (A.vec) kv4_ask<T>(A, src, e, turn, raw);
         slot = A.slots[row];
         if (turn) pos = A.positions[row];
         if (slot >= (int)(A.c.blocks << A.shift) || (slot >= 0 && turn && (unsigned)pos >= A.rope.rows)) {
@@ -127,14 +174,32 @@ template <typename T, int HD> __global__ void __launch_bounds__(KV4_THREADS) kv4
     float low = INFINITY, high = -INFINITY;
     bool bad = false;
     if (slot >= 0) {
-        const T *src = static_cast<const T *>(is_k ? A.k : A.v) + row * (is_k ? A.k_stride : A.v_stride) + (size_t)head * HD;
-        kv4_load<T>(A, src, e, turn, turn ? (size_t)pos * (A.rope.dims / 2) : 0, x);
+        const size_t tab = turn ? (size_t)pos * (A.rope.dims / 2) : 0;
+        if (A.vec) {
+            kv4_turn<T>(A, raw, e, turn, tab, x);
+        } else {
+            float y[8];
+            kv4_load<T>(A, src, e, turn, tab, y);
+#pragma unroll
+            for (int t = 0; t < 8; ++t) x[t] = y[t];
+        }
+        float peak = 0.f;
 #pragma unroll
         for (int t = 0; t < 8; ++t) {
-            const bool finite = fabsf(x[t]) <= 3.4028235e38f;
-            bad = bad || !finite;
-            low = fminf(low, finite ? x[t] : INFINITY);
-            high = fmaxf(high, finite ? x[t] : -INFINITY);
+            low = fminf(low, x[t]);
+            high = fmaxf(high, x[t]);
+            peak = max_nan(peak, fabsf(x[t]));
+        }
+        bad = !(peak <= 3.4028235e38f);
+        if (__builtin_expect(bad, 0)) {  // infinities and NaN do not count
+            low = INFINITY;
+            high = -INFINITY;
+#pragma unroll
+            for (int t = 0; t < 8; ++t)
+                if (fabsf(x[t]) <= 3.4028235e38f) {
+                    low = fminf(low, x[t]);
+                    high = fmaxf(high, x[t]);
+                }
         }
     }
 #pragma unroll
@@ -145,62 +210,92 @@ template <typename T, int HD> __global__ void __launch_bounds__(KV4_THREADS) kv4
     if (slot < 0) return;
     if (bad) raise_error(A.error, ERR_NONFINITE);
     if (low > high) low = high = 0.f;  // nothing finite
+    const bool wide = bad || low < -KV4_MOST || high > KV4_MOST;
     const __half lo = __float2half_rn(fminf(fmaxf(low, -KV4_MOST), KV4_MOST));
     const __half hi = __float2half_rn(fminf(fmaxf(high, -KV4_MOST), KV4_MOST));
     const float lf = __half2float(lo);
     const __half sc = __float2half_rn(__fdiv_rn(__fsub_rn(__half2float(hi), lf), 15.f));
     const float sf = __half2float(sc), inv = sf > 0.f ? __frcp_rn(sf) : 0.f;
+    // Four numbers at a time as one of 16 bits. A quotient that is no nearer than 1e-5 to a border is certain; the others
+    // are few, and eight values with one go one by one.
     unsigned bits = 0;
+    float off = 0.f;
+    constexpr float WHOLE = 12582912.f;  // 1.5 x 2^23: added, a number's fraction is rounded away, ties to even
 #pragma unroll
-    for (int t = 0; t < 8; ++t) {
-        float y = x[t];
-        if (bad && isnan(y)) y = 0.f;   // held as near to 0 as the group's values are
-        if (sf > 0.f) bits |= kv4_number(y, lf, sf, inv) << (4 * t);
+    for (int t = 0; t < 8; t += 4) {
+        float n[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float y = __fmul_rn(__fsub_rn(x[t + i], lf), inv);
+            n[i] = __fsub_rn(__fadd_rn(y, WHOLE), WHOLE);
+            off = fmaxf(off, fabsf(__fsub_rn(y, n[i])));
+        }
+        const float four = fmaf(fmaf(n[3], 16.f, n[2]), 256.f, fmaf(n[1], 16.f, n[0]));
+        bits |= (__float_as_uint(__fadd_rn(four, WHOLE)) & 0xffffu) << (4 * t);
+    }
+    if (__builtin_expect(wide || !(off < 0.49999f), 0)) {
+        float y[8];
+#pragma unroll
+        for (int t = 0; t < 8; ++t) y[t] = x[t];
+        bits = kv4_numbers(y, lf, sf, inv);
     }
     const size_t at = (((size_t)(slot >> A.shift) * A.c.kv_heads + head) << A.shift) + ((unsigned)slot & ((1u << A.shift) - 1));
     static_cast<unsigned *>(is_k ? A.c.k : A.c.v)[at * WORDS + word] = bits;
     if (lane % 8 == 0) static_cast<__half2 *>(is_k ? A.c.k_scale : A.c.v_scale)[at * GROUPS + group] = __halves2half2(sc, lo);
 }
 
-// Values at slots: thread = word w of K and of V of one head of a row.
+// Values at slots: thread = half a word (four values) of K and of V of READ4_ROWS rows, all loads out before the first is
+// used; a warp's stores lie together. Grid (rows / READ4_ROWS, half words of a row / 256).
+constexpr int READ4_ROWS = 4;
 template <int HD>
-__global__ void __launch_bounds__(256) kv4_read_kernel(fyb_kv4_cache c, const int *slots, size_t rows, float *k, float *v,
+__global__ void __launch_bounds__(KV4_THREADS) kv4_read_kernel(fyb_kv4_cache c, const int *slots, size_t rows, float *k, float *v,
     unsigned shift, unsigned *error)
 {
-    constexpr unsigned WORDS = HD / 8, GROUPS = HD / KV4_GROUP;
-    const unsigned per_row = c.kv_heads * WORDS;
-    const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x, row = i / per_row;
-    const unsigned j = (unsigned)(i % per_row), head = j / WORDS, lane = j % WORDS;
-    if (row >= rows) return;
-    const unsigned group = lane / 8, word = (lane % 8) * GROUPS + group;
-    int slot = slots[row];
-    if (slot >= (int)(c.blocks << shift)) {
-        if (lane == 0) raise_error(error, ERR_BOUNDS);
-        slot = -1;
+    constexpr unsigned PER = HD / 4, GROUPS = HD / KV4_GROUP;
+    const unsigned per_row = c.kv_heads * PER, j = blockIdx.y * KV4_THREADS + threadIdx.x;
+    if (j >= per_row) return;
+    const unsigned head = j / PER, e = j % PER * 4, group = e / KV4_GROUP, word = e % KV4_GROUP / 8 * GROUPS + group;
+    const size_t r0 = (size_t)blockIdx.x * READ4_ROWS;
+    int slot[READ4_ROWS];
+    unsigned kw[READ4_ROWS], vw[READ4_ROWS];
+    __half2 ks[READ4_ROWS], vs[READ4_ROWS];
+#pragma unroll
+    for (int u = 0; u < READ4_ROWS; ++u) slot[u] = r0 + u < rows ? slots[r0 + u] : -1;
+#pragma unroll
+    for (int u = 0; u < READ4_ROWS; ++u) {
+        kw[u] = vw[u] = 0;
+        ks[u] = vs[u] = __half2half2(__ushort_as_half(0));
+        if (slot[u] < 0) continue;
+        if (slot[u] >= (int)(c.blocks << shift)) { raise_error(error, ERR_BOUNDS); continue; }
+        const size_t at = (((size_t)(slot[u] >> shift) * c.kv_heads + head) << shift) + ((unsigned)slot[u] & ((1u << shift) - 1));
+        kw[u] = static_cast<const unsigned *>(c.k)[at * (HD / 8) + word];
+        vw[u] = static_cast<const unsigned *>(c.v)[at * (HD / 8) + word];
+        ks[u] = static_cast<const __half2 *>(c.k_scale)[at * GROUPS + group];
+        vs[u] = static_cast<const __half2 *>(c.v_scale)[at * GROUPS + group];
     }
-    unsigned kw = 0, vw = 0;
-    float2 ks = make_float2(0.f, 0.f), vs = ks;
-    if (slot >= 0) {
-        const size_t at = (((size_t)(slot >> shift) * c.kv_heads + head) << shift) + ((unsigned)slot & ((1u << shift) - 1));
-        kw = static_cast<const unsigned *>(c.k)[at * WORDS + word];
-        vw = static_cast<const unsigned *>(c.v)[at * WORDS + word];
-        ks = __half22float2(static_cast<const __half2 *>(c.k_scale)[at * GROUPS + group]);
-        vs = __half22float2(static_cast<const __half2 *>(c.v_scale)[at * GROUPS + group]);
-    }
-    const size_t out = (row * c.kv_heads + head) * HD + kv4_first<HD>(word);
-    auto eight = [&](float *p, unsigned w, float2 s) {
-        float4 *o = reinterpret_cast<float4 *>(p + out);
-        o[0] = make_float4(kv4_value(w, 0, s), kv4_value(w, 1, s), kv4_value(w, 2, s), kv4_value(w, 3, s));
-        o[1] = make_float4(kv4_value(w, 4, s), kv4_value(w, 5, s), kv4_value(w, 6, s), kv4_value(w, 7, s));
+    auto four = [&](unsigned w, __half2 scale_low) {
+        const float2 s = __half22float2(scale_low);
+        w >>= e & 4 ? 16 : 0;
+        return make_float4(kv4_value(w, 0, s), kv4_value(w, 1, s), kv4_value(w, 2, s), kv4_value(w, 3, s));
     };
-    eight(k, kw, ks);
-    eight(v, vw, vs);
+#pragma unroll
+    for (int u = 0; u < READ4_ROWS; ++u) {
+        if (r0 + u >= rows) break;
+        reinterpret_cast<float4 *>(k)[(r0 + u) * per_row + j] = four(kw[u], ks[u]);
+        reinterpret_cast<float4 *>(v)[(r0 + u) * per_row + j] = four(vw[u], vs[u]);
+    }
 }
 
 template <typename T> static void append_launch(const Kv4Append &A, unsigned grid, cudaStream_t s)
 {
-    if (A.c.head_dim == 128) kv4_append_kernel<T, 128><<<grid, KV4_THREADS, 0, s>>>(A);
-    else kv4_append_kernel<T, 64><<<grid, KV4_THREADS, 0, s>>>(A);
+    const bool q = A.q_rows > 0;
+    if (A.c.head_dim == 128) {
+        if (q) kv4_append_kernel<T, 128, true><<<grid, KV4_THREADS, 0, s>>>(A);
+        else kv4_append_kernel<T, 128, false><<<grid, KV4_THREADS, 0, s>>>(A);
+    } else {
+        if (q) kv4_append_kernel<T, 64, true><<<grid, KV4_THREADS, 0, s>>>(A);
+        else kv4_append_kernel<T, 64, false><<<grid, KV4_THREADS, 0, s>>>(A);
+    }
 }
 
 }  // namespace fyb
@@ -234,7 +329,8 @@ extern "C" int fyb_kv4_append(const fyb_kv4_cache *cache, const int32_t *slots, 
     if (rope) A.vec = A.vec && rope_vectors(A.rope, hd, width, A.q) && A.rope.dims % (A.rope.layout == 0 ? 8 : 16) == 0 &&
                     ((uintptr_t)A.rope.cos | (uintptr_t)A.rope.sin) % 16 == 0;
     cudaStream_t s = (cudaStream_t)stream;
-    const size_t ctas = (rows * 2 * kv * (hd / 8) + KV4_THREADS - 1) / KV4_THREADS;
+    A.grid = kv4_grid(2 * kv * (hd / 8));
+    const size_t ctas = (rows + A.grid.rows - 1) / A.grid.rows * A.grid.parts;
     if (heads && rows > 148) {  // a launch more is little beside a prompt
         const int r = rope_run(type, A.rope, positions, rows, hd, A.q, RopeRows{}, error, s);
         if (r) return r;
@@ -259,10 +355,10 @@ extern "C" int fyb_kv4_read(const fyb_kv4_cache *cache, const int32_t *slots, si
     if (kv4_check(cache) || (rows && (!k || !v)) || ((uintptr_t)k | (uintptr_t)v) % 16 || rows > 0x7fffffffu) return -1;
     if (!rows) return 0;
     if (!slots) return -1;
-    const size_t ctas = (rows * cache->kv_heads * (cache->head_dim / 8) + 255) / 256;
-    if (ctas > 0x7fffffffu) return -1;
+    const dim3 grid((unsigned)((rows + READ4_ROWS - 1) / READ4_ROWS), (cache->kv_heads * (cache->head_dim / 4) + KV4_THREADS - 1) / KV4_THREADS);
+    if (grid.y > 65535) return -1;
     cudaStream_t s = (cudaStream_t)stream;
-    if (cache->head_dim == 128) kv4_read_kernel<128><<<(unsigned)ctas, 256, 0, s>>>(*cache, slots, rows, k, v, kv4_shift(cache), error);
-    else kv4_read_kernel<64><<<(unsigned)ctas, 256, 0, s>>>(*cache, slots, rows, k, v, kv4_shift(cache), error);
+    if (cache->head_dim == 128) kv4_read_kernel<128><<<grid, KV4_THREADS, 0, s>>>(*cache, slots, rows, k, v, kv4_shift(cache), error);
+    else kv4_read_kernel<64><<<grid, KV4_THREADS, 0, s>>>(*cache, slots, rows, k, v, kv4_shift(cache), error);
     return cudaGetLastError() == cudaSuccess ? 0 : -2;
 }
