@@ -26,8 +26,12 @@ inline Kv4Grid kv4_grid(unsigned per_row)
 FYB_DEV bool kv4_place(const Kv4Grid &g, unsigned cta, size_t rows, size_t &row, unsigned &j)
 {
     if (g.rows == 1) {
-        row = cta / g.parts;
-        j = cta % g.parts * KV4_THREADS + threadIdx.x;
+        row = cta;
+        j = threadIdx.x;
+        if (g.parts > 1) {
+            row = cta / g.parts;
+            j += cta % g.parts * KV4_THREADS;
+        }
         return j < g.per_row;
     }
     const unsigned r = threadIdx.x / g.per_row;
@@ -122,8 +126,21 @@ FYB_DEV float max_nan(float a, float b)  // NaN where one is
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
     return y;
 }
-// Eight numbers one by one: nearest to (x - low) / scale, 0..15, ties to even. `inv` is the F32 reciprocal of scale: the
-// F32 quotient y is within 4e-6 of the real one where it matters (0 <= y <= 15.1), so only next to a border between two
+// x / 15, correctly rounded: a quotient from the rounded reciprocal, and its remainder's (Markstein 1990).
+FYB_DEV float fifteenth(float x)
+{
+    constexpr float r = 1.f / 15.f;
+    const float q = x * r;
+    return fmaf(fmaf(-15.f, q, x), r, q);
+}
+FYB_DEV float rcp_approx(float x)  // within 2^-23 of it
+{
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+// Eight numbers one by one: nearest to (x - low) / scale, 0..15, ties to even. `inv` is the reciprocal of scale within 2^-23:
+// the F32 quotient y is within 4e-6 of the real one where it matters (0 <= y <= 15.1), so only next to a border between two
 // numbers is more needed: there x and the border, exact in 64 bits, are compared. NaN is held as 0 would be.
 static __device__ __noinline__ unsigned kv4_numbers(const float *x, float low, float scale, float inv)
 {
@@ -183,14 +200,15 @@ template <typename T, int HD, bool Q> __global__ void __launch_bounds__(KV4_THRE
 #pragma unroll
             for (int t = 0; t < 8; ++t) x[t] = y[t];
         }
-        float peak = 0.f;
+        F2 nothing = f2(0.f, 0.f);  // NaN where a value is none or infinite
 #pragma unroll
-        for (int t = 0; t < 8; ++t) {
-            low = fminf(low, x[t]);
-            high = fmaxf(high, x[t]);
-            peak = max_nan(peak, fabsf(x[t]));
+        for (int t = 0; t < 8; t += 2) {
+            low = fminf(fminf(low, x[t]), x[t + 1]);
+            high = fmaxf(fmaxf(high, x[t]), x[t + 1]);
+            nothing = f2_fma(f2(x[t], x[t + 1]), f2(0.f, 0.f), nothing);
         }
-        bad = !(peak <= 3.4028235e38f);
+        const float2 zero = f2_get(nothing);
+        bad = isnan(zero.x + zero.y);
         if (__builtin_expect(bad, 0)) {  // infinities and NaN do not count
             low = INFINITY;
             high = -INFINITY;
@@ -214,8 +232,8 @@ template <typename T, int HD, bool Q> __global__ void __launch_bounds__(KV4_THRE
     const __half lo = __float2half_rn(fminf(fmaxf(low, -KV4_MOST), KV4_MOST));
     const __half hi = __float2half_rn(fminf(fmaxf(high, -KV4_MOST), KV4_MOST));
     const float lf = __half2float(lo);
-    const __half sc = __float2half_rn(__fdiv_rn(__fsub_rn(__half2float(hi), lf), 15.f));
-    const float sf = __half2float(sc), inv = sf > 0.f ? __frcp_rn(sf) : 0.f;
+    const __half sc = __float2half_rn(fifteenth(__fsub_rn(__half2float(hi), lf)));
+    const float sf = __half2float(sc), inv = rcp_approx(sf);  // scale 0: no number is certain
     // Four numbers at a time as one of 16 bits. A quotient that is no nearer than 1e-5 to a border is certain; the others
     // are few, and eight values with one go one by one.
     unsigned bits = 0;
@@ -223,14 +241,16 @@ template <typename T, int HD, bool Q> __global__ void __launch_bounds__(KV4_THRE
     constexpr float WHOLE = 12582912.f;  // 1.5 x 2^23: added, a number's fraction is rounded away, ties to even
 #pragma unroll
     for (int t = 0; t < 8; t += 4) {
-        float n[4];
+        F2 n[2];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const float y = __fmul_rn(__fsub_rn(x[t + i], lf), inv);
-            n[i] = __fsub_rn(__fadd_rn(y, WHOLE), WHOLE);
-            off = fmaxf(off, fabsf(__fsub_rn(y, n[i])));
+        for (int i = 0; i < 2; ++i) {
+            const F2 y = f2_mul(f2_add(f2(x[t + 2 * i], x[t + 2 * i + 1]), f2(-lf, -lf)), f2(inv, inv));
+            n[i] = f2_add(f2_add(y, f2(WHOLE, WHOLE)), f2(-WHOLE, -WHOLE));
+            const float2 d = f2_get(f2_fma(n[i], f2(-1.f, -1.f), y));
+            off = max_nan(off, max_nan(fabsf(d.x), fabsf(d.y)));
         }
-        const float four = fmaf(fmaf(n[3], 16.f, n[2]), 256.f, fmaf(n[1], 16.f, n[0]));
+        const float2 a = f2_get(n[0]), b = f2_get(n[1]);
+        const float four = fmaf(fmaf(b.y, 16.f, b.x), 256.f, fmaf(a.y, 16.f, a.x));
         bits |= (__float_as_uint(__fadd_rn(four, WHOLE)) & 0xffffu) << (4 * t);
     }
     if (__builtin_expect(wide || !(off < 0.49999f), 0)) {
