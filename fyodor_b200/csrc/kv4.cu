@@ -5,7 +5,7 @@
 // value is held as the whole number nearest to (x - low) / scale, ties to even,
 // in 0..15. Every rounding is defined (quotients and borders as real numbers),
 // so the stored bits are. A token's groups need nothing of its neighbours: a
-// thread takes eight values (one word), eight lanes a group, whose bounds they
+// thread takes 16 values (two words), four lanes a group, whose bounds they
 // find by shuffles.
 #include "rope.cuh"
 #include "kv4.cuh"
@@ -13,8 +13,9 @@
 namespace fyb {
 
 constexpr unsigned KV4_THREADS = 256;
+constexpr int KV4_EACH = 16;  // values of a thread: with 8 an append of 6093 rows of 8 heads took 307 instructions a warp, 17.9 us
 
-// Where a CTA's threads stand among rows of `per_row` words: rows of a CTA, or CTAs of a row.
+// Where a CTA's threads stand among rows of `per_row` items: rows of a CTA, or CTAs of a row.
 struct Kv4Grid {
     unsigned per_row, rows, parts;  // rows of a CTA (1 where a row has parts)
 };
@@ -22,7 +23,7 @@ inline Kv4Grid kv4_grid(unsigned per_row)
 {
     return Kv4Grid{per_row, per_row < KV4_THREADS ? KV4_THREADS / per_row : 1, (per_row + KV4_THREADS - 1) / KV4_THREADS};
 }
-// Thread's row and word of it; false for a thread that has none.
+// Thread's row and item of it; false for a thread that has none.
 FYB_DEV bool kv4_place(const Kv4Grid &g, unsigned cta, size_t rows, size_t &row, unsigned &j)
 {
     if (g.rows == 1) {
@@ -54,48 +55,51 @@ struct Kv4Append {
     unsigned *error;
 };
 
-// Eight values of a row's head as they lie there, and of the other half where half pairs are turned.
+// A thread's values of a row's head as they lie there, and of the other half where half pairs are turned.
 template <typename T> struct Kv4Raw {
     static constexpr int V = 16 / sizeof(T);
-    RopePack<T, V> own[8 / V], other[8 / V];
+    RopePack<T, V> own[KV4_EACH / V], other[KV4_EACH / V];
 };
-// The eight from e (aligned accesses): asked for before slot and position have come.
+// Those from e (aligned accesses): asked for before slot and position have come.
 template <typename T> FYB_DEV void kv4_ask(const Kv4Append &A, const T *row, unsigned e, bool turn, Kv4Raw<T> &r)
 {
     constexpr int V = Kv4Raw<T>::V;
     const unsigned pairs = A.rope.dims / 2;
 #pragma unroll
-    for (int i = 0; i < 8 / V; ++i) r.own[i] = rope_get<T, V, true>(row + e + i * V);
+    for (int i = 0; i < KV4_EACH / V; ++i) r.own[i] = rope_get<T, V, true>(row + e + i * V);
     if (turn && A.rope.layout != 0 && e < A.rope.dims) {
         const unsigned o = e < pairs ? e + pairs : e - pairs;
 #pragma unroll
-        for (int i = 0; i < 8 / V; ++i) r.other[i] = rope_get<T, V, true>(row + o + i * V);
+        for (int i = 0; i < KV4_EACH / V; ++i) r.other[i] = rope_get<T, V, true>(row + o + i * V);
     }
 }
 // The same in F32, rotated when `turn`; tab: the position's place in the tables.
-template <typename T> FYB_DEV void kv4_turn(const Kv4Append &A, const Kv4Raw<T> &r, unsigned e, bool turn, size_t tab, float (&x)[8])
+template <typename T> FYB_DEV void kv4_turn(const Kv4Append &A, const Kv4Raw<T> &r, unsigned e, bool turn, size_t tab, float (&x)[KV4_EACH])
 {
     constexpr int V = Kv4Raw<T>::V;
     const unsigned dims = A.rope.dims, pairs = dims / 2;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = row_value(r.own[i / V].t[i % V]);
+    for (int i = 0; i < KV4_EACH; ++i) x[i] = row_value(r.own[i / V].t[i % V]);
     if (!turn || e >= dims) return;
     if (A.rope.layout == 0) {
-        float cv[4], sv[4];
-        rope_row<4, true>(A.rope.cos + tab + e / 2, cv);
-        rope_row<4, true>(A.rope.sin + tab + e / 2, sv);
+        float cv[KV4_EACH / 2], sv[KV4_EACH / 2];
+        rope_row<KV4_EACH / 2, true>(A.rope.cos + tab + e / 2, cv);
+        rope_row<KV4_EACH / 2, true>(A.rope.sin + tab + e / 2, sv);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) rope_turn(x[2 * i], x[2 * i + 1], cv[i], sv[i]);
+        for (int i = 0; i < KV4_EACH / 2; ++i) rope_turn(x[2 * i], x[2 * i + 1], cv[i], sv[i]);
     } else {
-        const bool low = e < pairs;  // pairs is a multiple of 8: the eight lie in one half
+        const bool low = e < pairs;  // pairs is a multiple of KV4_EACH: the values lie in one half
         const unsigned p = low ? e : e - pairs;
-        float cv[8], sv[8];
-        rope_row<8, true>(A.rope.cos + tab + p, cv);
-        rope_row<8, true>(A.rope.sin + tab + p, sv);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            float o = row_value(r.other[i / V].t[i % V]);
-            if (low) rope_turn(x[i], o, cv[i], sv[i]); else rope_turn(o, x[i], cv[i], sv[i]);
+        for (int i = 0; i < KV4_EACH; i += 4) {
+            float cv[4], sv[4];
+            rope_row<4, true>(A.rope.cos + tab + p + i, cv);
+            rope_row<4, true>(A.rope.sin + tab + p + i, sv);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                float o = row_value(r.other[(i + j) / V].t[(i + j) % V]);
+                if (low) rope_turn(x[i + j], o, cv[j], sv[j]); else rope_turn(o, x[i + j], cv[j], sv[j]);
+            }
         }
     }
 }
@@ -104,7 +108,7 @@ template <typename T> __device__ __noinline__ void kv4_load(const Kv4Append &A, 
 {
     const float *c = A.rope.cos + tab, *s = A.rope.sin + tab;
     const unsigned dims = A.rope.dims, pairs = dims / 2;
-    for (int i = 0; i < 8; ++i) {
+    for (int i = 0; i < KV4_EACH; ++i) {
         const unsigned d = e + i;
         x[i] = row_value(row[d]);
         if (!turn || d >= dims) continue;
@@ -160,10 +164,11 @@ static __device__ __noinline__ unsigned kv4_numbers(const float *x, float low, f
     return bits;
 }
 
-// CTAs of K and V: thread = word w of one head of one row of K or V; with Q then those of q.
+// CTAs of K and V: thread = KV4_EACH values of one head of one row of K or V; with Q then those of q.
 template <typename T, int HD, bool Q> __global__ void __launch_bounds__(KV4_THREADS) kv4_append_kernel(const __grid_constant__ Kv4Append A)
 {
-    constexpr unsigned WORDS = HD / 8, GROUPS = HD / KV4_GROUP;
+    constexpr unsigned LANES = HD / KV4_EACH, GROUPS = HD / KV4_GROUP, PART = KV4_GROUP / KV4_EACH;  // threads of a head, of a group
+    constexpr unsigned WORDS = HD / 8;
     if (Q && blockIdx.x >= A.ctas) {
         rope_row_of_q<T, HD, KV4_THREADS>(A, blockIdx.x - A.ctas);
         return;
@@ -172,11 +177,10 @@ template <typename T, int HD, bool Q> __global__ void __launch_bounds__(KV4_THRE
     unsigned j;
     const bool real = kv4_place(A.grid, blockIdx.x, A.rows, row, j);
     const bool is_k = j < A.grid.per_row / 2;
-    const unsigned head = (is_k ? j : j - A.grid.per_row / 2) / WORDS, lane = j % WORDS;
-    const unsigned group = lane / 8, word = (lane % 8) * GROUPS + group, e = kv4_first<HD>(word);
+    const unsigned head = (is_k ? j : j - A.grid.per_row / 2) / LANES, lane = j % LANES, group = lane / PART, e = lane * KV4_EACH;
     const bool turn = is_k && A.rope.cos;
     const T *src = static_cast<const T *>(is_k ? A.k : A.v) + row * (is_k ? A.k_stride : A.v_stride) + (size_t)head * HD;
-    int slot = -1, pos = 0;  // the eight lanes of a group take the same way
+    int slot = -1, pos = 0;  // the lanes of a group take the same way
     Kv4Raw<T> raw;
     if (real) {
         if (A.vec) kv4_ask<T>(A, src, e, turn, raw);
@@ -187,7 +191,7 @@ template <typename T, int HD, bool Q> __global__ void __launch_bounds__(KV4_THRE
             slot = -1;
         }
     }
-    float x[8];
+    float x[KV4_EACH];
     float low = INFINITY, high = -INFINITY;
     bool bad = false;
     if (slot >= 0) {
@@ -195,14 +199,14 @@ template <typename T, int HD, bool Q> __global__ void __launch_bounds__(KV4_THRE
         if (A.vec) {
             kv4_turn<T>(A, raw, e, turn, tab, x);
         } else {
-            float y[8];
+            float y[KV4_EACH];
             kv4_load<T>(A, src, e, turn, tab, y);
 #pragma unroll
-            for (int t = 0; t < 8; ++t) x[t] = y[t];
+            for (int t = 0; t < KV4_EACH; ++t) x[t] = y[t];
         }
         F2 nothing = f2(0.f, 0.f);  // NaN where a value is none or infinite
 #pragma unroll
-        for (int t = 0; t < 8; t += 2) {
+        for (int t = 0; t < KV4_EACH; t += 2) {
             low = fminf(fminf(low, x[t]), x[t + 1]);
             high = fmaxf(fmaxf(high, x[t]), x[t + 1]);
             nothing = f2_fma(f2(x[t], x[t + 1]), f2(0.f, 0.f), nothing);
@@ -213,7 +217,7 @@ template <typename T, int HD, bool Q> __global__ void __launch_bounds__(KV4_THRE
             low = INFINITY;
             high = -INFINITY;
 #pragma unroll
-            for (int t = 0; t < 8; ++t)
+            for (int t = 0; t < KV4_EACH; ++t)
                 if (fabsf(x[t]) <= 3.4028235e38f) {
                     low = fminf(low, x[t]);
                     high = fmaxf(high, x[t]);
@@ -221,7 +225,7 @@ template <typename T, int HD, bool Q> __global__ void __launch_bounds__(KV4_THRE
         }
     }
 #pragma unroll
-    for (int o = 1; o < 8; o <<= 1) {
+    for (unsigned o = 1; o < PART; o <<= 1) {
         low = fminf(low, __shfl_xor_sync(0xffffffffu, low, o));
         high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, o));
     }
@@ -234,34 +238,38 @@ template <typename T, int HD, bool Q> __global__ void __launch_bounds__(KV4_THRE
     const float lf = __half2float(lo);
     const __half sc = __float2half_rn(fifteenth(__fsub_rn(__half2float(hi), lf)));
     const float sf = __half2float(sc), inv = rcp_approx(sf);  // scale 0: no number is certain
+    const size_t at = (((size_t)(slot >> A.shift) * A.c.kv_heads + head) << A.shift) + ((unsigned)slot & ((1u << A.shift) - 1));
+    unsigned *words = static_cast<unsigned *>(is_k ? A.c.k : A.c.v) + at * WORDS + lane % PART * (KV4_EACH / 8) * GROUPS + group;
     // Four numbers at a time as one of 16 bits. A quotient that is no nearer than 1e-5 to a border is certain; the others
     // are few, and eight values with one go one by one.
-    unsigned bits = 0;
-    float off = 0.f;
     constexpr float WHOLE = 12582912.f;  // 1.5 x 2^23: added, a number's fraction is rounded away, ties to even
 #pragma unroll
-    for (int t = 0; t < 8; t += 4) {
-        F2 n[2];
+    for (int w = 0; w < KV4_EACH / 8; ++w) {
+        unsigned bits = 0;
+        float off = 0.f;
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const F2 y = f2_mul(f2_add(f2(x[t + 2 * i], x[t + 2 * i + 1]), f2(-lf, -lf)), f2(inv, inv));
-            n[i] = f2_add(f2_add(y, f2(WHOLE, WHOLE)), f2(-WHOLE, -WHOLE));
-            const float2 d = f2_get(f2_fma(n[i], f2(-1.f, -1.f), y));
-            off = max_nan(off, max_nan(fabsf(d.x), fabsf(d.y)));
+        for (int t = 0; t < 8; t += 4) {
+            F2 n[2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const F2 y = f2_mul(f2_add(f2(x[8 * w + t + 2 * i], x[8 * w + t + 2 * i + 1]), f2(-lf, -lf)), f2(inv, inv));
+                n[i] = f2_add(f2_add(y, f2(WHOLE, WHOLE)), f2(-WHOLE, -WHOLE));
+                const float2 d = f2_get(f2_fma(n[i], f2(-1.f, -1.f), y));
+                off = max_nan(off, max_nan(fabsf(d.x), fabsf(d.y)));
+            }
+            const float2 a = f2_get(n[0]), b = f2_get(n[1]);
+            const float four = fmaf(fmaf(b.y, 16.f, b.x), 256.f, fmaf(a.y, 16.f, a.x));
+            bits |= (__float_as_uint(__fadd_rn(four, WHOLE)) & 0xffffu) << (4 * t);
         }
-        const float2 a = f2_get(n[0]), b = f2_get(n[1]);
-        const float four = fmaf(fmaf(b.y, 16.f, b.x), 256.f, fmaf(a.y, 16.f, a.x));
-        bits |= (__float_as_uint(__fadd_rn(four, WHOLE)) & 0xffffu) << (4 * t);
-    }
-    if (__builtin_expect(wide || !(off < 0.49999f), 0)) {
-        float y[8];
+        if (__builtin_expect(wide || !(off < 0.49999f), 0)) {
+            float y[8];
 #pragma unroll
-        for (int t = 0; t < 8; ++t) y[t] = x[t];
-        bits = kv4_numbers(y, lf, sf, inv);
+            for (int t = 0; t < 8; ++t) y[t] = x[8 * w + t];
+            bits = kv4_numbers(y, lf, sf, inv);
+        }
+        words[w * GROUPS] = bits;
     }
-    const size_t at = (((size_t)(slot >> A.shift) * A.c.kv_heads + head) << A.shift) + ((unsigned)slot & ((1u << A.shift) - 1));
-    static_cast<unsigned *>(is_k ? A.c.k : A.c.v)[at * WORDS + word] = bits;
-    if (lane % 8 == 0) static_cast<__half2 *>(is_k ? A.c.k_scale : A.c.v_scale)[at * GROUPS + group] = __halves2half2(sc, lo);
+    if (lane % PART == 0) static_cast<__half2 *>(is_k ? A.c.k_scale : A.c.v_scale)[at * GROUPS + group] = __halves2half2(sc, lo);
 }
 
 // Values at slots: thread = half a word (four values) of K and of V of READ4_ROWS rows, all loads out before the first is
@@ -344,12 +352,12 @@ extern "C" int fyb_kv4_append(const fyb_kv4_cache *cache, const int32_t *slots, 
     A.q = RopeRows{q, q_out, q_stride, q_out_stride, heads};
     A.shift = kv4_shift(cache);
     A.error = error;
-    // 16-byte accesses to rows and tables: eight values of a thread rotate alike, their tables' rows are aligned
+    // 16-byte accesses to rows and tables: the values of a thread rotate alike, their tables' rows are aligned
     A.vec = ((uintptr_t)k | (uintptr_t)v) % 16 == 0 && k_stride % el == 0 && v_stride % el == 0;
-    if (rope) A.vec = A.vec && rope_vectors(A.rope, hd, width, A.q) && A.rope.dims % (A.rope.layout == 0 ? 8 : 16) == 0 &&
+    if (rope) A.vec = A.vec && rope_vectors(A.rope, hd, width, A.q) && A.rope.dims % (A.rope.layout == 0 ? KV4_EACH : 2 * KV4_EACH) == 0 &&
                     ((uintptr_t)A.rope.cos | (uintptr_t)A.rope.sin) % 16 == 0;
     cudaStream_t s = (cudaStream_t)stream;
-    A.grid = kv4_grid(2 * kv * (hd / 8));
+    A.grid = kv4_grid(2 * kv * (hd / KV4_EACH));
     const size_t ctas = (rows + A.grid.rows - 1) / A.grid.rows * A.grid.parts;
     if (heads && rows > 148) {  // a launch more is little beside a prompt
         const int r = rope_run(type, A.rope, positions, rows, hd, A.q, RopeRows{}, error, s);
