@@ -24,7 +24,7 @@
 
 namespace fyb {
 
-constexpr int LP_THREADS = 256, LP_WARPS = LP_THREADS / 32, LP_LOADS = 4, LP_GRID = 4 * 148;
+constexpr int LP_THREADS = 256, LP_WARPS = LP_THREADS / 32, LP_LOADS = 4, LP_CTAS = 3, LP_GRID = LP_CTAS * 148;
 constexpr float LP_LOWEST = -3.402823466e38f, LP_FAR = -1e4f;  // e^LP_FAR is 0
 
 struct LpSums {
@@ -118,42 +118,107 @@ FYB_DEV float lp_kth(float v, unsigned k, unsigned lane)
     return __shfl_sync(0xffffffffu, v, (int)k);
 }
 
-template <typename T> struct LpVec;  // the values of a 16-byte access
+// The values of a 16-byte access, -inf taken as the type's lowest number (its exponential is 0 all the same, and the
+// product with it too, where -inf would leave NaN): `far` says whether that holds against a reference m. Largest and
+// count of those above (or at) a value, NaN being neither.
+template <typename T> struct LpVec;
 template <> struct LpVec<float> {
     static constexpr int V = 4;
+    static FYB_DEV uint4 none() { const unsigned x = 0xff800000u; return make_uint4(x, x, x, x); }
     static FYB_DEV void get(const uint4 &u, float *x)
     {
         x[0] = __uint_as_float(u.x); x[1] = __uint_as_float(u.y); x[2] = __uint_as_float(u.z); x[3] = __uint_as_float(u.w);
     }
+    static FYB_DEV void finite(const uint4 &u, float *x)
+    {
+        get(u, x);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) asm("max.NaN.f32 %0, %1, %2;" : "=f"(x[i]) : "f"(x[i]), "f"(LP_LOWEST));
+    }
+    static FYB_DEV bool far(float m) { return m > -1e30f && m < 1e30f; }
+    template <int N> static FYB_DEV float largest(const uint4 (&u)[N])
+    {
+        float h = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            float x[4];
+            get(u[i], x);
+            h = fmaxf(fmaxf(h, fmaxf(x[0], x[1])), fmaxf(x[2], x[3]));
+        }
+        return h;
+    }
+    template <bool EQUAL, int N> static FYB_DEV unsigned above(const uint4 (&u)[N], float than)
+    {
+        unsigned c = 0;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            float x[4];
+            get(u[i], x);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) c += EQUAL ? x[j] >= than : x[j] > than;
+        }
+        return c;
+    }
 };
-template <> struct LpVec<__half> {
+template <typename H2> struct LpPairs {  // two values a word
     static constexpr int V = 8;
+    static FYB_DEV H2 pair(unsigned w) { return *reinterpret_cast<const H2 *>(&w); }
+    static FYB_DEV unsigned word(H2 p) { return *reinterpret_cast<const unsigned *>(&p); }
+};
+template <> struct LpVec<__half> : LpPairs<__half2> {
+    static FYB_DEV uint4 none() { const unsigned x = 0xfc00fc00u; return make_uint4(x, x, x, x); }
+    static FYB_DEV float2 two(unsigned w) { return __half22float2(pair(w)); }
+    static FYB_DEV unsigned finite(unsigned w) { return word(__hmax2_nan(pair(w), pair(0xfbfffbffu))); }
+    static FYB_DEV bool far(float m) { return m > -65000.f; }
+    static FYB_DEV __half2 one(float x) { return __float2half2_rn(x); }
+};
+template <> struct LpVec<__nv_bfloat16> : LpPairs<__nv_bfloat162> {
+    static FYB_DEV uint4 none() { const unsigned x = 0xff80ff80u; return make_uint4(x, x, x, x); }
+    static FYB_DEV float2 two(unsigned w) { return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)); }
+    static FYB_DEV unsigned finite(unsigned w) { return word(__hmax2_nan(pair(w), pair(0xff7fff7fu))); }
+    static FYB_DEV bool far(float m) { return m > -1e30f && m < 1e30f; }
+    static FYB_DEV __nv_bfloat162 one(float x) { return __float2bfloat162_rn(x); }
+};
+template <typename T> struct LpRow : LpVec<T> {  // what both 16-bit types do alike
+    using B = LpVec<T>;
     static FYB_DEV void get(const uint4 &u, float *x)
     {
         const unsigned w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w[i]));
-            x[2 * i] = f.x;
-            x[2 * i + 1] = f.y;
-        }
+        for (int i = 0; i < 4; ++i) { const float2 f = B::two(w[i]); x[2 * i] = f.x; x[2 * i + 1] = f.y; }
     }
-};
-template <> struct LpVec<__nv_bfloat16> {
-    static constexpr int V = 8;
-    static FYB_DEV void get(const uint4 &u, float *x)
+    static FYB_DEV void finite(const uint4 &u, float *x)
     {
-        const unsigned w[4] = {u.x, u.y, u.z, u.w};
+        get(make_uint4(B::finite(u.x), B::finite(u.y), B::finite(u.z), B::finite(u.w)), x);
+    }
+    template <int N> static FYB_DEV float largest(const uint4 (&u)[N])
+    {
+        auto h = B::pair(B::none().x);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            x[2 * i] = __uint_as_float(w[i] << 16);
-            x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+        for (int i = 0; i < N; ++i)
+            h = __hmax2(h, __hmax2(__hmax2(B::pair(u[i].x), B::pair(u[i].y)), __hmax2(B::pair(u[i].z), B::pair(u[i].w))));
+        const float2 f = B::two(B::word(h));
+        return fmaxf(f.x, f.y);
+    }
+    template <bool EQUAL, int N> static FYB_DEV unsigned above(const uint4 (&u)[N], float than)
+    {
+        const auto t = B::one(than);  // of this type, so exactly itself
+        auto c = B::one(0.f);
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const unsigned w[4] = {u[i].x, u[i].y, u[i].z, u[i].w};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) c = __hadd2(c, EQUAL ? __hge2(B::pair(w[j]), t) : __hgt2(B::pair(w[j]), t));  // 1 or 0 each
         }
+        const float2 f = B::two(B::word(c));
+        return (unsigned)(f.x + f.y);
     }
 };
+template <> struct LpRow<float> : LpVec<float> {};
 
 // What a thread (and its warp) carries along a row.
-template <bool TOP> struct LpState {
+template <typename T, bool TOP> struct LpState {
+    using Row = LpRow<T>;
     float top, m;
     F2 s, t;
     unsigned before;
@@ -170,13 +235,8 @@ template <bool TOP> struct LpState {
         last = -INFINITY;
         first = true;
     }
-    // N logits, the j-th of index(j); all lanes of the warp call it, with -inf of index INT_MAX for what they do not have
-    template <int N, typename Index>
-    FYB_DEV void take(const float (&x)[N], float given, int token, int lo, int hi, unsigned k, volatile unsigned *bound, unsigned lane, Index index)
+    FYB_DEV void reach(float high)
     {
-        float high = x[0];
-#pragma unroll
-        for (int j = 1; j < N; ++j) high = fmaxf(high, x[j]);
         top = fmaxf(top, high);
         if (high - m > 8.f) {
             float2 a = f2_get(s), b = f2_get(t);
@@ -185,52 +245,103 @@ template <bool TOP> struct LpState {
             s = f2(sum, 0.f);
             t = f2(weighted, 0.f);
         }
-        const F2 minus = f2(-m, -m), unit = f2(LP_LOG2E, LP_LOG2E);
-        static_assert(N == 1 || N % 2 == 0, "");
-#pragma unroll
-        for (int j = 0; j < N; j += 2) {
-            const F2 d = f2_add(f2(x[j], N > 1 ? x[j + 1 < N ? j + 1 : j] : -INFINITY), minus);
-            const float2 q = f2_get(f2_mul(d, unit)), dd = f2_get(d);
-            const F2 e = f2(lp_exp2(q.x), lp_exp2(q.y));
-            s = f2_add(s, e);  // NaN stays here
-            t = f2_fma(e, f2(fmaxf(dd.x, LP_FAR), fmaxf(dd.y, LP_FAR)), t);
+    }
+    template <bool FAR> FYB_DEV void add(float x, float y)
+    {
+        const F2 d = f2_add(f2(x, y), f2(-m, -m));
+        const float2 q = f2_get(f2_mul(d, f2(LP_LOG2E, LP_LOG2E))), dd = f2_get(d);
+        const F2 e = f2(lp_exp2(q.x), lp_exp2(q.y));
+        s = f2_add(s, e);  // NaN stays here
+        t = f2_fma(e, FAR ? d : f2(fmaxf(dd.x, LP_FAR), fmaxf(dd.y, LP_FAR)), t);
+    }
+    // Candidates for the list: N logits of which high is the largest, the j-th of index(j). A warp's batches ascend: of
+    // equal logits those in the list come first, so the next has to be above its last. Another warp's last is a bound too;
+    // logits that equal it may come first.
+    template <int N, typename Get, typename Index>
+    FYB_DEV void choose(float high, unsigned k, volatile unsigned *bound, unsigned lane, Get get, Index index)
+    {
+        const float other = float_from_order_key(*bound);
+        if (!__any_sync(0xffffffffu, high > last && high >= other)) return;
+        float least = other;
+        if (N > 1 && first) {
+            least = fmaxf(least, k == 1 ? float_from_order_key(__reduce_max_sync(0xffffffffu, isnan(high) ? 0u : float_order_key(high)))
+                                        : lp_kth(high, k - 1, lane));
+            first = false;
         }
-        // logits from index lo to hi: before the token equal ones count too
-        if (hi < token && given > -INFINITY) {
+        const float was = last;
+        float x[N];
+        get(x);
 #pragma unroll
-            for (int j = 0; j < N; ++j) before += x[j] >= given;
-        } else if (lo > token) {
-#pragma unroll
-            for (int j = 0; j < N; ++j) before += x[j] > given;
-        } else {
-#pragma unroll
-            for (int j = 0; j < N; ++j) before += x[j] > given || (x[j] == given && index(j) < token);
-        }
-        if constexpr (TOP) {
-            // A warp's batches ascend: of equal logits those in the list come first, so the next has to be above its last.
-            // Another warp's last is a bound too; logits that equal it may come first.
-            const float other = float_from_order_key(*bound);
-            if (!__any_sync(0xffffffffu, high > last && high >= other)) return;
-            float least = other;
-            if (N > 1 && first) {
-                least = fmaxf(least, lp_kth(high, k - 1, lane));
-                first = false;
+        for (int j = 0; j < N; ++j) {
+            unsigned left = __ballot_sync(0xffffffffu, x[j] > was && x[j] >= least);
+            while (left) {
+                const int from = __ffs((int)left) - 1;
+                left &= left - 1;
+                lp_insert(best, LpBest{__shfl_sync(0xffffffffu, x[j], from), __shfl_sync(0xffffffffu, index(j), from)}, lane);
+                least = fmaxf(least, __shfl_sync(0xffffffffu, best.v, (int)k - 1));
+                left &= __ballot_sync(0xffffffffu, x[j] >= least);
             }
-            const float was = last;
+        }
+        last = __shfl_sync(0xffffffffu, best.v, (int)k - 1);
+        if (lane == 0 && last > other) atomicMax(const_cast<unsigned *>(bound), float_order_key(last));
+    }
+    // PER accesses, the j-th logit of index(j) (INT_MAX for what is not the row's, which is -inf), from lo to hi; all
+    // lanes of the warp call it
+    template <int PER, typename Index>
+    FYB_DEV void take(const uint4 (&u)[PER], float given, int token, int lo, int hi, unsigned k, volatile unsigned *bound, unsigned lane, Index index)
+    {
+        constexpr int N = PER * Row::V;
+        const float high = Row::largest(u);
+        reach(high);
+        if (__builtin_expect(Row::far(m), 1)) {
 #pragma unroll
-            for (int j = 0; j < N; ++j) {
-                unsigned left = __ballot_sync(0xffffffffu, x[j] > was && x[j] >= least);
-                while (left) {
-                    const int from = __ffs((int)left) - 1;
-                    left &= left - 1;
-                    lp_insert(best, LpBest{__shfl_sync(0xffffffffu, x[j], from), __shfl_sync(0xffffffffu, index(j), from)}, lane);
-                    least = fmaxf(least, __shfl_sync(0xffffffffu, best.v, (int)k - 1));
-                    left &= __ballot_sync(0xffffffffu, x[j] >= least);
+            for (int i = 0; i < PER; ++i) {
+                float x[Row::V];
+                Row::finite(u[i], x);
+#pragma unroll
+                for (int j = 0; j < Row::V; j += 2) add<true>(x[j], x[j + 1]);
+            }
+        } else {
+#pragma unroll 1
+            for (int i = 0; i < PER; ++i) {
+                uint4 w = u[0];
+#pragma unroll
+                for (int j = 1; j < PER; ++j) if (i == j) w = u[j];
+                float x[Row::V];
+                Row::get(w, x);
+#pragma unroll
+                for (int j = 0; j < Row::V; j += 2) add<false>(x[j], x[j + 1]);
+            }
+        }
+        // rank: before the token equal ones count too
+        if (__any_sync(0xffffffffu, high >= given)) {
+            if (lo > token) {
+                before += Row::template above<false>(u, given);
+            } else if (hi < token && given > -INFINITY) {
+                before += Row::template above<true>(u, given);
+            } else {
+#pragma unroll
+                for (int i = 0; i < PER; ++i) {
+                    float x[Row::V];
+                    Row::get(u[i], x);
+#pragma unroll
+                    for (int j = 0; j < Row::V; ++j) before += x[j] > given || (x[j] == given && index(i * Row::V + j) < token);
                 }
             }
-            last = __shfl_sync(0xffffffffu, best.v, (int)k - 1);
-            if (lane == 0 && last > other) atomicMax(const_cast<unsigned *>(bound), float_order_key(last));
         }
+        if constexpr (TOP)
+            choose<N>(high, k, bound, lane, [&](float (&x)[N]) {
+#pragma unroll
+                for (int i = 0; i < PER; ++i) Row::get(u[i], x + i * Row::V);
+            }, index);
+    }
+    // One logit a lane, -inf of index INT_MAX for none.
+    FYB_DEV void take(float x, int i, float given, int token, unsigned k, volatile unsigned *bound, unsigned lane)
+    {
+        reach(x);
+        add<false>(x, -INFINITY);
+        before += x > given || (x == given && i < token);
+        if constexpr (TOP) choose<1>(x, k, bound, lane, [&](float (&y)[1]) { y[0] = x; }, [&](int) { return i; });
     }
 };
 
@@ -247,67 +358,72 @@ FYB_DEV void lp_merge_warps(LpBest (&best)[LP_WARPS][32])
     }
 }
 
-template <typename T, bool TOP> __global__ void __launch_bounds__(LP_THREADS, 4) logprobs_kernel(const __grid_constant__ Logprobs A)
+template <typename T, bool TOP> __global__ void __launch_bounds__(LP_THREADS, LP_CTAS) logprobs_kernel(const __grid_constant__ Logprobs A)
 {
-    constexpr int V = LpVec<T>::V, CHUNK = LP_LOADS * LP_THREADS;  // 16-byte accesses of a chunk
-    constexpr int N = 16, PER = N / V;                              // logits that are taken at once, accesses of them
-    __shared__ LpSums sums_s[LP_WARPS];
-    __shared__ unsigned rank_s[LP_WARPS], bound_s, flag_s;
-    __shared__ LpBest best_s[LP_WARPS][32];
+    using Row = LpRow<T>;
+    constexpr int V = Row::V, CHUNK = LP_LOADS * LP_THREADS;  // 16-byte accesses of a chunk
+    constexpr int PER = 16 / V;                                // accesses that are taken at once
+    // what the warps hold of a row, of two rows in turn: one warp joins them while the others go on
+    __shared__ LpSums sums_s[2][LP_WARPS];
+    __shared__ unsigned rank_s[2][LP_WARPS], bound_s[2], flag_s;
+    __shared__ LpBest best_s[2][LP_WARPS][32];
     const unsigned tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, C = gridDim.x;
     const unsigned long long U = (unsigned long long)A.rows * A.chunks;
     unsigned at = lp_begin(U, C, blockIdx.x);
     const unsigned end = lp_begin(U, C, blockIdx.x + 1);
-    LpState<TOP> st;
-    while (at < end) {
+    LpState<T, TOP> st;
+    unsigned turn = 0;
+    if (tid == 0) bound_s[0] = float_order_key(-INFINITY);
+    __syncthreads();
+    for (; at < end; ++turn) {
+        const unsigned use = turn & 1;
         const unsigned row = at / A.chunks, c0 = at % A.chunks, c1 = min(A.chunks, c0 + (end - at));
         const T *x = static_cast<const T *>(A.x) + row * A.stride;
         // elements before the first 16-byte boundary, whole accesses, elements behind them
         const unsigned head = min(A.n, (unsigned)((16 - ((uintptr_t)x & 15)) & 15) / (unsigned)sizeof(T));
         const unsigned vectors = (A.n - head) / V, tail = head + vectors * V;
         const uint4 *body = reinterpret_cast<const uint4 *>(x + head);
+        // a chunk is asked for while the one before is taken, the first before all else
+        uint4 raw[LP_LOADS];
+        unsigned v0 = c0 * CHUNK + warp * LP_LOADS * 32 + lane;
+        auto ask = [&] {
+#pragma unroll
+            for (int u = 0; u < LP_LOADS; ++u) {
+                raw[u] = Row::none();
+                if (v0 + u * 32 < vectors) raw[u] = ldg_stream_u4(body + v0 + u * 32);
+            }
+        };
+        ask();
+        const bool begins = c0 == 0 && warp == 0 && head, ends = c1 == A.chunks && warp == 0 && tail < A.n;
+        const float early = begins && lane < head ? row_value(x[lane]) : -INFINITY;
+        const float late = ends && tail + lane < A.n ? row_value(x[tail + lane]) : -INFINITY;
         int token = A.tokens ? A.tokens[row] : -1;
         if (token >= (int)A.n) {
             if (tid == 0 && c0 == 0) raise_error(A.error, ERR_BOUNDS);
             token = -1;
         }
         const float given = token >= 0 ? row_value(x[token]) : INFINITY;
-        if (TOP) {
-            __syncthreads();
-            if (tid == 0) bound_s = float_order_key(-INFINITY);
-            __syncthreads();
-        }
         st.begin();
-        auto edge = [&](unsigned from, unsigned to) {  // fewer than V elements, warp 0
-            const unsigned i = from + lane;
-            const float y[1] = {i < to ? row_value(x[i]) : -INFINITY};
-            st.take(y, given, token, 0, (int)A.n, A.top, &bound_s, lane, [&](int) { return i < to ? (int)i : INT_MAX; });
-        };
-        if (c0 == 0 && warp == 0 && head) edge(0, head);
-        for (unsigned c = c0; c < c1; ++c) {
-            const unsigned v0 = c * CHUNK + warp * LP_LOADS * 32 + lane;
-            uint4 raw[LP_LOADS];
+        if (begins) st.take(early, lane < head ? (int)lane : INT_MAX, given, token, A.top, &bound_s[use], lane);
+#pragma unroll 1
+        for (unsigned c = c0; c < c1 && v0 - lane < vectors; ++c) {
+            uint4 now[LP_LOADS];
 #pragma unroll
-            for (int u = 0; u < LP_LOADS; ++u)
-                if (v0 + u * 32 < vectors) raw[u] = ldg_stream_u4(body + v0 + u * 32);
-            if (v0 - lane >= vectors) break;  // the warp has none
+            for (int u = 0; u < LP_LOADS; ++u) now[u] = raw[u];
+            const unsigned v = v0;
+            v0 += CHUNK;
+            if (c + 1 < c1) ask();
 #pragma unroll
             for (int u = 0; u < LP_LOADS; u += PER) {
-                float y[N];
+                uint4 part[PER];
 #pragma unroll
-                for (int w = 0; w < PER; ++w) {
-                    LpVec<T>::get(raw[u + w], y + w * V);
-                    if (v0 + (u + w) * 32 >= vectors) {
-#pragma unroll
-                        for (int j = 0; j < V; ++j) y[w * V + j] = -INFINITY;
-                    }
-                }
-                const unsigned first = head + (v0 + u * 32) * V;
-                st.take(y, given, token, (int)first, (int)(first + ((PER - 1) * 32 + 1) * V - 1), A.top, &bound_s, lane,
-                        [&](int j) { return v0 + (u + j / V) * 32 < vectors ? (int)(first + (j / V) * 32 * V + j % V) : INT_MAX; });
+                for (int w = 0; w < PER; ++w) part[w] = now[u + w];
+                const unsigned first = head + (v + u * 32) * V;
+                st.take(part, given, token, (int)first, (int)(first + ((PER - 1) * 32 + 1) * V - 1), A.top, &bound_s[use], lane,
+                        [&](int j) { return v + (u + j / V) * 32 < vectors ? (int)(first + (j / V) * 32 * V + j % V) : INT_MAX; });
             }
         }
-        if (c1 == A.chunks && warp == 0 && tail < A.n) edge(tail, A.n);
+        if (ends) st.take(late, tail + lane < A.n ? (int)(tail + lane) : INT_MAX, given, token, A.top, &bound_s[use], lane);
 
         // ---- the CTA's part of the row
         const float2 s2 = f2_get(st.s), t2 = f2_get(st.t);
@@ -317,66 +433,89 @@ template <typename T, bool TOP> __global__ void __launch_bounds__(LP_THREADS, 4)
             sums = lp_join(sums, lp_shuffle(sums, o));
             st.before += __shfl_xor_sync(0xffffffffu, st.before, o);
         }
-        if (lane == 0) { sums_s[warp] = sums; rank_s[warp] = st.before; }
-        if (TOP) best_s[warp][lane] = st.best;
+        if (lane == 0) { sums_s[use][warp] = sums; rank_s[use][warp] = st.before; }
+        if (TOP) best_s[use][warp][lane] = st.best;
+        if (tid == 0) bound_s[use ^ 1] = float_order_key(-INFINITY);
         __syncthreads();
-        if (TOP) lp_merge_warps(best_s);
+        at += c1 - c0;
+        const bool last = at >= end;  // nothing to go on with: all warps help
+        if (!last && warp != turn % LP_WARPS) continue;
+        const bool lead = !last || warp == 0;
         unsigned before = 0;
-        if (warp == 0) {
-            sums = lane < LP_WARPS ? sums_s[lane] : LpSums{-INFINITY, LP_LOWEST, 0.f, 0.f};
-            before = lane < LP_WARPS ? rank_s[lane] : 0;
+        LpBest best = lp_none();
+        auto whole = [&] {  // sums over the lanes: every lane writes an alternative and needs them
 #pragma unroll
-            for (int o = 16; o; o >>= 1) {  // every lane writes an alternative: all need them
+            for (int o = 16; o; o >>= 1) {
                 sums = lp_join(sums, lp_shuffle(sums, o));
                 before += __shfl_xor_sync(0xffffffffu, before, o);
             }
+        };
+        auto merge = [&] {  // the warps' lists
+            if constexpr (TOP) {
+                if (last) {
+                    lp_merge_warps(best_s[use]);
+                    best = best_s[use][0][lane];
+                } else {
+                    best = best_s[use][0][lane];
+#pragma unroll 1
+                    for (int w = 1; w < LP_WARPS; ++w) best = lp_merge(best, best_s[use][w][lane], lane);
+                }
+            }
+        };
+        if (lead) {
+            sums = lane < LP_WARPS ? sums_s[use][lane] : LpSums{-INFINITY, LP_LOWEST, 0.f, 0.f};
+            before = lane < LP_WARPS ? rank_s[use][lane] : 0;
+            whole();
         }
-        bool write = true;
+        merge();
         if (c0 || c1 < A.chunks) {
             // ---- a part: the last CTA of the row joins them all in order
             const unsigned first = row * A.chunks, f = lp_cta_of(U, C, first), l = lp_cta_of(U, C, first + A.chunks - 1);
             const unsigned slot = 2 * blockIdx.x + (blockIdx.x == f ? 1 : 0);
-            if (warp == 0) {
+            unsigned all = 0;
+            if (lead) {
                 if (lane == 0) { A.part[slot] = sums; A.part_rank[slot] = before; }
-                if (TOP) A.part_best[slot * 32 + lane] = best_s[0][lane];
+                if (TOP) A.part_best[slot * 32 + lane] = best;
                 __threadfence();
                 __syncwarp();
-                if (lane == 0) flag_s = atomicAdd(&A.counters[f], 1u) == l - f;
+                if (lane == 0) all = atomicAdd(&A.counters[f], 1u) == l - f;
+                all = __shfl_sync(0xffffffffu, all, 0);
             }
-            __syncthreads();
-            write = flag_s;
-            if (write) {
-                __threadfence();
-                if (tid == 0) A.counters[f] = 0;
-                auto slot_of = [&](unsigned p) { return 2 * (f + p) + (p == 0 ? 1 : 0); };
-                const unsigned parts = l - f + 1;
-                if (warp == 0) {
-                    sums = LpSums{-INFINITY, LP_LOWEST, 0.f, 0.f};
-                    before = 0;
-                    for (unsigned p = lane; p < parts; p += 32) {
-                        const float4 y = __ldcg(reinterpret_cast<const float4 *>(A.part) + slot_of(p));
-                        sums = lp_join(sums, LpSums{y.x, y.y, y.z, y.w});
-                        before += __ldcg(A.part_rank + slot_of(p));
-                    }
-#pragma unroll
-                    for (int o = 16; o; o >>= 1) {
-                        sums = lp_join(sums, lp_shuffle(sums, o));
-                        before += __shfl_xor_sync(0xffffffffu, before, o);
-                    }
+            if (last) {
+                if (tid == 0) flag_s = all;
+                __syncthreads();
+                all = flag_s;
+            }
+            if (!all) continue;
+            __threadfence();
+            if (lead && lane == 0) A.counters[f] = 0;
+            auto slot_of = [&](unsigned p) { return 2 * (f + p) + (p == 0 ? 1 : 0); };
+            const unsigned parts = l - f + 1, step = last ? LP_WARPS : 1;
+            if (lead) {
+                sums = LpSums{-INFINITY, LP_LOWEST, 0.f, 0.f};
+                before = 0;
+                for (unsigned p = lane; p < parts; p += 32) {
+                    const float4 y = __ldcg(reinterpret_cast<const float4 *>(A.part) + slot_of(p));
+                    sums = lp_join(sums, LpSums{y.x, y.y, y.z, y.w});
+                    before += __ldcg(A.part_rank + slot_of(p));
                 }
-                if (TOP) {
-                    LpBest mine = lp_none();
-                    for (unsigned p = warp; p < parts; p += LP_WARPS) {
-                        const float2 y = __ldcg(reinterpret_cast<const float2 *>(A.part_best) + slot_of(p) * 32 + lane);
-                        mine = lp_merge(mine, LpBest{y.x, __float_as_int(y.y)}, lane);
-                    }
-                    best_s[warp][lane] = mine;
+                whole();
+            }
+            if constexpr (TOP) {
+                best = lp_none();
+#pragma unroll 1
+                for (unsigned p = last ? warp : 0; p < parts; p += step) {
+                    const float2 y = __ldcg(reinterpret_cast<const float2 *>(A.part_best) + slot_of(p) * 32 + lane);
+                    best = lp_merge(best, LpBest{y.x, __float_as_int(y.y)}, lane);
+                }
+                if (last) {
+                    best_s[use][warp][lane] = best;
                     __syncthreads();
-                    lp_merge_warps(best_s);
+                    merge();
                 }
             }
         }
-        if (write && warp == 0) {
+        if (lead) {
             const bool bad = isnan(sums.s), none = sums.top == -INFINITY && !bad;
             const float log_sum = logf(sums.s);
             if (lane == 0) {
@@ -386,13 +525,10 @@ template <typename T, bool TOP> __global__ void __launch_bounds__(LP_THREADS, 4)
                 if (A.entropy) A.entropy[row] = bad ? NAN : none ? 0.f : log_sum - sums.t / sums.s;
             }
             if (TOP && lane < A.top) {
-                const LpBest b = best_s[0][lane];
-                A.top_tokens[(size_t)row * A.top + lane] = b.i;
-                A.top_logprobs[(size_t)row * A.top + lane] = bad ? NAN : b.i < 0 ? -INFINITY : b.v - sums.m - log_sum;
+                A.top_tokens[(size_t)row * A.top + lane] = best.i;
+                A.top_logprobs[(size_t)row * A.top + lane] = bad ? NAN : best.i < 0 ? -INFINITY : best.v - sums.m - log_sum;
             }
         }
-        __syncthreads();
-        at += c1 - c0;
     }
 }
 
