@@ -12,11 +12,16 @@
 //
 // A thread sums against a reference of its own that moves only when a logit is more
 // than 8 above it, so sums are not rescaled at every new maximum (their terms are
-// at most e^8); pairs of terms go through the packed F32 instructions. A warp
-// keeps the best 32 logits sorted over its lanes; a logit is looked at only if it
-// is above the last of them that counts, so alternatives cost a comparison for
-// 16 logits but for some K ln(n) insertions. The first batch of a row bounds the
-// list from below by the K-th largest of the lanes' maxima.
+// at most e^8); pairs of terms go through the packed F32 instructions.
+//
+// Alternatives: a warp keeps the best 32 logits sorted over its lanes, and looks at
+// one only if it is above the last of them that counts and not below a bound that
+// the CTA's warps share. The bound: of the largest logits that the 256 threads have
+// seen, taken together by lane, the K-th of 32 largest has K logits at or above it.
+// It is found before the first chunk is looked at and again as chunks pass, so some
+// 30 logits of a chunk, then of each doubling of them, are looked at by all warps
+// together (with the lists' own last ones alone each warp looked at K ln(n) of its
+// own: a prompt of 400 rows with 20 alternatives 83 us, so 67).
 #include "common.cuh"
 #include "kernels.h"
 #include "fyodor_b200.h"
@@ -224,7 +229,6 @@ template <typename T, bool TOP> struct LpState {
     unsigned before;
     LpBest best;  // lane's place of the warp's list
     float last;   // the top-th of it
-    bool first;
     FYB_DEV void begin()
     {
         top = -INFINITY;
@@ -233,7 +237,6 @@ template <typename T, bool TOP> struct LpState {
         before = 0;
         best = lp_none();
         last = -INFINITY;
-        first = true;
     }
     FYB_DEV void reach(float high)
     {
@@ -254,41 +257,42 @@ template <typename T, bool TOP> struct LpState {
         s = f2_add(s, e);  // NaN stays here
         t = f2_fma(e, FAR ? d : f2(fmaxf(dd.x, LP_FAR), fmaxf(dd.y, LP_FAR)), t);
     }
-    // Candidates for the list: N logits of which high is the largest, the j-th of index(j). A warp's batches ascend: of
-    // equal logits those in the list come first, so the next has to be above its last. Another warp's last is a bound too;
-    // logits that equal it may come first.
+    // Candidates for the list: N logits of a lane, of which high is the largest; index(l, j) is that of lane l's j-th. A
+    // warp's batches ascend: of equal logits those in the list come first, so the next has to be above its last; logits
+    // that equal the bound may come first. stage: [32][20] of the warp.
     template <int N, typename Get, typename Index>
-    FYB_DEV void choose(float high, unsigned k, volatile unsigned *bound, unsigned lane, Get get, Index index)
+    FYB_DEV void choose(float high, unsigned k, volatile unsigned *bound, float *stage, unsigned lane, Get get, Index index)
     {
-        const float other = float_from_order_key(*bound);
-        if (!__any_sync(0xffffffffu, high > last && high >= other)) return;
-        float least = other;
-        if (N > 1 && first) {
-            least = fmaxf(least, k == 1 ? float_from_order_key(__reduce_max_sync(0xffffffffu, isnan(high) ? 0u : float_order_key(high)))
-                                        : lp_kth(high, k - 1, lane));
-            first = false;
-        }
-        const float was = last;
+        float least = float_from_order_key(*bound);
+        if (!__any_sync(0xffffffffu, high > last && high >= least)) return;
         float x[N];
         get(x);
+        unsigned mask = 0;
 #pragma unroll
-        for (int j = 0; j < N; ++j) {
-            unsigned left = __ballot_sync(0xffffffffu, x[j] > was && x[j] >= least);
-            while (left) {
-                const int from = __ffs((int)left) - 1;
-                left &= left - 1;
-                lp_insert(best, LpBest{__shfl_sync(0xffffffffu, x[j], from), __shfl_sync(0xffffffffu, index(j), from)}, lane);
-                least = fmaxf(least, __shfl_sync(0xffffffffu, best.v, (int)k - 1));
-                left &= __ballot_sync(0xffffffffu, x[j] >= least);
-            }
+        for (int j = 0; j < N; ++j) mask |= (x[j] > last && x[j] >= least ? 1u : 0u) << j;
+        __syncwarp();
+        if constexpr (N == 1) {
+            stage[lane * 20] = x[0];
+        } else {
+#pragma unroll
+            for (int j = 0; j < N; j += 4) *reinterpret_cast<float4 *>(stage + lane * 20 + j) = make_float4(x[j], x[j + 1], x[j + 2], x[j + 3]);
+        }
+        __syncwarp();
+#pragma unroll 1
+        for (unsigned left; (left = __ballot_sync(0xffffffffu, mask != 0)) != 0;) {
+            const int from = __ffs((int)left) - 1, j = __ffs((int)__shfl_sync(0xffffffffu, mask, from)) - 1;
+            if ((int)lane == from) mask &= mask - 1;
+            const float v = stage[from * 20 + j];
+            if (v < least) continue;
+            lp_insert(best, LpBest{v, index(from, j)}, lane);
+            least = fmaxf(least, __shfl_sync(0xffffffffu, best.v, (int)k - 1));
         }
         last = __shfl_sync(0xffffffffu, best.v, (int)k - 1);
-        if (lane == 0 && last > other) atomicMax(const_cast<unsigned *>(bound), float_order_key(last));
     }
-    // PER accesses, the j-th logit of index(j) (INT_MAX for what is not the row's, which is -inf), from lo to hi; all
+    // PER accesses, index(l, j) that of lane l's j-th logit (INT_MAX for what is not the row's, which is -inf), from lo to hi; all
     // lanes of the warp call it
     template <int PER, typename Index>
-    FYB_DEV void take(const uint4 (&u)[PER], float given, int token, int lo, int hi, unsigned k, volatile unsigned *bound, unsigned lane, Index index)
+    FYB_DEV void take(const uint4 (&u)[PER], float given, int token, int lo, int hi, unsigned k, volatile unsigned *bound, float *stage, unsigned lane, Index index)
     {
         constexpr int N = PER * Row::V;
         const float high = Row::largest(u);
@@ -325,23 +329,23 @@ template <typename T, bool TOP> struct LpState {
                     float x[Row::V];
                     Row::get(u[i], x);
 #pragma unroll
-                    for (int j = 0; j < Row::V; ++j) before += x[j] > given || (x[j] == given && index(i * Row::V + j) < token);
+                    for (int j = 0; j < Row::V; ++j) before += x[j] > given || (x[j] == given && index((int)lane, i * Row::V + j) < token);
                 }
             }
         }
         if constexpr (TOP)
-            choose<N>(high, k, bound, lane, [&](float (&x)[N]) {
+            choose<N>(high, k, bound, stage, lane, [&](float (&x)[N]) {
 #pragma unroll
                 for (int i = 0; i < PER; ++i) Row::get(u[i], x + i * Row::V);
             }, index);
     }
-    // One logit a lane, -inf of index INT_MAX for none.
-    FYB_DEV void take(float x, int i, float given, int token, unsigned k, volatile unsigned *bound, unsigned lane)
+    // One logit a lane, the l-th of index i0 + l; -inf of index INT_MAX for none.
+    FYB_DEV void take(float x, int i, float given, int token, unsigned k, volatile unsigned *bound, float *stage, unsigned lane, int i0)
     {
         reach(x);
         add<false>(x, -INFINITY);
         before += x > given || (x == given && i < token);
-        if constexpr (TOP) choose<1>(x, k, bound, lane, [&](float (&y)[1]) { y[0] = x; }, [&](int) { return i; });
+        if constexpr (TOP) choose<1>(x, k, bound, stage, lane, [&](float (&y)[1]) { y[0] = x; }, [&](int l, int) { return i0 + l; });
     }
 };
 
@@ -367,6 +371,8 @@ template <typename T, bool TOP> __global__ void __launch_bounds__(LP_THREADS, LP
     __shared__ LpSums sums_s[2][LP_WARPS];
     __shared__ unsigned rank_s[2][LP_WARPS], bound_s[2], flag_s;
     __shared__ LpBest best_s[2][LP_WARPS][32];
+    __shared__ float seen_s[TOP ? LP_WARPS : 1][32];                 // largest logit that each thread has seen of the row
+    __shared__ __align__(16) float stage_s[TOP ? LP_WARPS : 1][32 * 20];
     const unsigned tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, C = gridDim.x;
     const unsigned long long U = (unsigned long long)A.rows * A.chunks;
     unsigned at = lp_begin(U, C, blockIdx.x);
@@ -404,7 +410,22 @@ template <typename T, bool TOP> __global__ void __launch_bounds__(LP_THREADS, LP
         }
         const float given = token >= 0 ? row_value(x[token]) : INFINITY;
         st.begin();
-        if (begins) st.take(early, lane < head ? (int)lane : INT_MAX, given, token, A.top, &bound_s[use], lane);
+        float *stage = stage_s[TOP ? warp : 0];
+        // the K-th largest of the lanes' largest logits, all warps': K logits of the row are at or above it
+        auto bound = [&] {
+            float h = seen_s[0][lane];
+#pragma unroll
+            for (int w = 1; w < (TOP ? LP_WARPS : 1); ++w) h = fmaxf(h, *(volatile float *)&seen_s[w][lane]);
+            h = lp_kth(h, A.top - 1, lane);
+            if (lane == 0) atomicMax(&bound_s[use], float_order_key(h));
+        };
+        if constexpr (TOP) {
+            seen_s[warp][lane] = Row::largest(raw);
+            __syncthreads();
+            if (warp == 0) bound();
+            __syncthreads();
+        }
+        if (begins) st.take(early, lane < head ? (int)lane : INT_MAX, given, token, A.top, &bound_s[use], stage, lane, 0);
 #pragma unroll 1
         for (unsigned c = c0; c < c1 && v0 - lane < vectors; ++c) {
             uint4 now[LP_LOADS];
@@ -419,11 +440,22 @@ template <typename T, bool TOP> __global__ void __launch_bounds__(LP_THREADS, LP
 #pragma unroll
                 for (int w = 0; w < PER; ++w) part[w] = now[u + w];
                 const unsigned first = head + (v + u * 32) * V;
-                st.take(part, given, token, (int)first, (int)(first + ((PER - 1) * 32 + 1) * V - 1), A.top, &bound_s[use], lane,
-                        [&](int j) { return v + (u + j / V) * 32 < vectors ? (int)(first + (j / V) * 32 * V + j % V) : INT_MAX; });
+                st.take(part, given, token, (int)first, (int)(first + ((PER - 1) * 32 + 1) * V - 1), A.top, &bound_s[use], stage, lane,
+                        [&](int l, int j) {
+                            const unsigned at = v - lane + (unsigned)l + (u + j / V) * 32;
+                            return at < vectors ? (int)(head + at * V + j % V) : INT_MAX;
+                        });
+            }
+            if constexpr (TOP) {
+                const unsigned i = c - c0;
+                if (i) {
+                    seen_s[warp][lane] = st.top;
+                    __syncwarp();
+                    if (((i & (i - 1)) == 0 || i % 4 == 0) && warp == i % LP_WARPS) bound();
+                }
             }
         }
-        if (ends) st.take(late, tail + lane < A.n ? (int)(tail + lane) : INT_MAX, given, token, A.top, &bound_s[use], lane);
+        if (ends) st.take(late, tail + lane < A.n ? (int)(tail + lane) : INT_MAX, given, token, A.top, &bound_s[use], stage, lane, (int)tail);
 
         // ---- the CTA's part of the row
         const float2 s2 = f2_get(st.s), t2 = f2_get(st.t);
@@ -504,9 +536,14 @@ template <typename T, bool TOP> __global__ void __launch_bounds__(LP_THREADS, LP
             if constexpr (TOP) {
                 best = lp_none();
 #pragma unroll 1
-                for (unsigned p = last ? warp : 0; p < parts; p += step) {
-                    const float2 y = __ldcg(reinterpret_cast<const float2 *>(A.part_best) + slot_of(p) * 32 + lane);
-                    best = lp_merge(best, LpBest{y.x, __float_as_int(y.y)}, lane);
+                for (unsigned p = last ? warp : 0; p < parts; p += 4 * step) {
+                    float2 y[4];
+#pragma unroll
+                    for (unsigned u = 0; u < 4; ++u)
+                        if (p + u * step < parts) y[u] = __ldcg(reinterpret_cast<const float2 *>(A.part_best) + slot_of(p + u * step) * 32 + lane);
+#pragma unroll
+                    for (unsigned u = 0; u < 4; ++u)
+                        if (p + u * step < parts) best = lp_merge(best, LpBest{y[u].x, __float_as_int(y[u].y)}, lane);
                 }
                 if (last) {
                     best_s[use][warp][lane] = best;
