@@ -23,11 +23,11 @@ static int kv4_tensor_map(CUtensorMap *map, const fyb_kv4_cache &c, const void *
 
 // Row tile of the many-row kernel.
 static unsigned tile_rows(unsigned long long group_rows) { return group_rows <= 32 ? 32 : group_rows <= 64 ? 64 : 256; }
-// Query rows of a call's partials, two for each CTA of its kernel (F32 rows need 2 KA_GRID of eight: fewer than tiles do).
+// Query rows of a call's partials, two for each CTA of its kernel (F32 rows need 2 K4_GRID of eight: fewer than tiles do).
 static size_t part_rows(unsigned long long group_rows)
 {
-    static_assert(2 * KA_GRID * KV8_DECODE_ROWS <= 2 * K4T_GRID * 32, "");
-    return group_rows <= KV8_DECODE_ROWS ? 2 * KA_GRID * KV8_DECODE_ROWS : 2 * K4T_GRID * tile_rows(group_rows);
+    static_assert(2 * K4_GRID * KV8_DECODE_ROWS <= 2 * K4T_GRID * 32, "");
+    return group_rows <= KV8_DECODE_ROWS ? 2 * K4_GRID * KV8_DECODE_ROWS : 2 * K4T_GRID * tile_rows(group_rows);
 }
 
 }  // namespace fyb
@@ -40,7 +40,7 @@ extern "C" size_t fyb_kv4_attention_workspace(uint32_t requests, uint32_t max_ro
     if (!requests || !max_rows || !kv_heads || heads < kv_heads || heads % kv_heads || heads / kv_heads > 64 ||
         (head_dim != 64 && head_dim != 128))
         return 0;
-    return KA_COUNTER_BYTES + part_rows((unsigned long long)max_rows * (heads / kv_heads)) * (head_dim + 2) * sizeof(float);
+    return K4_COUNTER_BYTES + part_rows((unsigned long long)max_rows * (heads / kv_heads)) * (head_dim + 2) * sizeof(float);
 }
 
 extern "C" int fyb_kv4_attention(const fyb_kv4_cache *cache, const int32_t *lengths, const int32_t *row_start,
@@ -68,7 +68,7 @@ extern "C" int fyb_kv4_attention(const fyb_kv4_cache *cache, const int32_t *leng
     const unsigned long long group_rows = (unsigned long long)max_rows * A.group;
     unsigned char *ws = static_cast<unsigned char *>(workspace);
     A.counters = reinterpret_cast<unsigned *>(ws);
-    A.part_ml = reinterpret_cast<float2 *>(ws + KA_COUNTER_BYTES);
+    A.part_ml = reinterpret_cast<float2 *>(ws + K4_COUNTER_BYTES);
     A.part_o = reinterpret_cast<float *>(A.part_ml + part_rows(group_rows));
     CUtensorMap k, v;
     if (kv4_tensor_map(&k, *cache, cache->k) || kv4_tensor_map(&v, *cache, cache->v)) return -2;
@@ -85,7 +85,7 @@ extern "C" int fyb_kv4_attention(const fyb_kv4_cache *cache, const int32_t *leng
         A.c.kv_heads = cache->kv_heads * A.split;
         A.row_tile = std::min(max_rows, KV8_DECODE_ROWS / A.group);
         const unsigned long long units = tiles * A.c.kv_heads * std::min<unsigned long long>((max_rows + A.row_tile - 1) / A.row_tile, 1u << 20);
-        return launch_kv4_decode(A, k, v, (unsigned)std::min<unsigned long long>(KA_GRID, units), s);
+        return launch_kv4_decode(A, k, v, (unsigned)std::min<unsigned long long>(K4_GRID, units), s);
     }
     const unsigned n = tile_rows(group_rows);
     A.vec = (uintptr_t)q % 16 == 0 && q_stride % 8 == 0;

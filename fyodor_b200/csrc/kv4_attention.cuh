@@ -15,5 +15,7 @@ struct Kv4Attention : Kv8Attention {
 
 int launch_kv4_decode(const Kv4Attention &A, const CUtensorMap &k, const CUtensorMap &v, unsigned grid, cudaStream_t s);
 constexpr int K4_TILE = 128;  // positions of a unit
+constexpr unsigned K4_CTAS = 3, K4_GRID = K4_CTAS * 148;  // of the few-row kernel: CTAs per SM, largest grid
+constexpr size_t K4_COUNTER_BYTES = (K4_GRID * 4 + 255) / 256 * 256;
 
 }  // namespace fyb

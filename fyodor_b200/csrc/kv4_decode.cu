@@ -21,7 +21,19 @@
 
 namespace fyb {
 
-constexpr int K4_WARPS = 4, K4_THREADS = 32 * (K4_WARPS + 1);
+// SHARE: groups of 16 positions of a tile that a warp takes
+constexpr int K4_WARPS = 4, K4_SHARE = K4_TILE / 16 / K4_WARPS, K4_THREADS = 32 * (K4_WARPS + 1);
+
+// Words of shared memory: the address of a lane, and what is the same for all of them as the offset.
+FYB_DEV void lds(unsigned (&x)[4], unsigned at, unsigned off) { asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3]) : "r"(at + off)); }
+FYB_DEV void lds(unsigned (&x)[2], unsigned at, unsigned off) { asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(x[0]), "=r"(x[1]) : "r"(at + off)); }
+FYB_DEV void lds(unsigned (&x)[1], unsigned at, unsigned off) { asm volatile("ld.shared.u32 %0, [%1];" : "=r"(x[0]) : "r"(at + off)); }
+FYB_DEV unsigned pack2(float lo, float hi)  // fp16 pair
+{
+    const __half2 p = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const unsigned *>(&p);
+}
+FYB_DEV float2 unpack2(unsigned p) { return __half22float2(*reinterpret_cast<const __half2 *>(&p)); }
 
 template <int HD> struct K4Shape {
     static constexpr int ROW = HD / 2, SCALES = HD / 64 * 4;               // bytes of a token's row, of its scales
@@ -32,7 +44,7 @@ template <int HD> struct K4Shape {
 // W: rows a thread holds scores of (1: up to four query rows, 2: up to eight). LO: whether q and the weights have low
 // halves at W = 2 (at W = 1 they are columns that cost nothing).
 template <int HD, int W, bool LO>
-__global__ void __launch_bounds__(K4_THREADS, 3) kv4_decode_kernel(const __grid_constant__ Kv4Attention A, const __grid_constant__ CUtensorMap kmap,
+__global__ void __launch_bounds__(K4_THREADS, K4_CTAS) kv4_decode_kernel(const __grid_constant__ Kv4Attention A, const __grid_constant__ CUtensorMap kmap,
     const __grid_constant__ CUtensorMap vmap)
 {
     using S = K4Shape<HD>;
@@ -119,7 +131,11 @@ __global__ void __launch_bounds__(K4_THREADS, 3) kv4_decode_kernel(const __grid_
     constexpr unsigned X = HD == 128 ? 3 : 7;
     auto order = [](unsigned t) { return HD == 128 ? (t & 1) + 4 * (t >> 1) : t; };
     const unsigned ta = order(t4), tau = order(g >> 1) ^ (g & 1 ? X : 0u);
+    // this lane's place in a tile: of K, of V (two rows), of scales; 8 rows, 16 and tiles further on all of them grow alike
     auto swizzled = [](unsigned pos, unsigned byte) { return pos * S::ROW + (HD == 128 ? byte ^ ((pos >> 1 & 3) << 4) : byte); };
+    const unsigned mine = smem_u32(ring) + warp * K4_SHARE * 16 * S::ROW;
+    const unsigned k_at = mine + swizzled(tau, 4 * NW * t4), v_at0 = mine + S::OFF_V + swizzled(ta, 4 * G * g), v_at1 = mine + S::OFF_V + swizzled(ta ^ X, 4 * G * g);
+    const unsigned s_at = smem_u32(ring) + S::OFF_KS + (warp * K4_SHARE * 16 + tau) * S::SCALES;
     constexpr float P_SCALE = 32.f;  // keeps small weights clear of fp16's smallest numbers; the largest is 2^14
     auto bar = [] { asm volatile("bar.sync 1, %0;" :: "n"(32 * K4_WARPS) : "memory"); };
 
@@ -212,12 +228,12 @@ __global__ void __launch_bounds__(K4_THREADS, 3) kv4_decode_kernel(const __grid_
 
         for (int t = s.t0; t < s.t1; ++t) {
             wait(full + stage, phase);
-            const unsigned char *tile = ring + stage * S::STAGE;
+            const unsigned tile = stage * S::STAGE;
             const unsigned loaded = here[stage];
 #pragma unroll 1
-            for (int u0 = 0; u0 < 2; u0 += J) {
+            for (int u0 = 0; u0 < K4_SHARE; u0 += J) {
                 // J groups of 16 positions at a time, from position `first`
-                const unsigned in_tile = (warp * 2 + (unsigned)u0) * 16, use = loaded >> (in_tile / 16) & ((1u << J) - 1);
+                const unsigned in_tile = (warp * K4_SHARE + (unsigned)u0) * 16, use = loaded >> (in_tile / 16) & ((1u << J) - 1);
                 const int first = t * K4_TILE + (int)in_tile;
                 if (first >= any || !use) continue;
                 // ---- scores
@@ -227,18 +243,8 @@ __global__ void __launch_bounds__(K4_THREADS, 3) kv4_decode_kernel(const __grid_
 #pragma unroll
                     for (int h = 0; h < G; ++h) c[u][h][0] = c[u][h][1] = c[u][h][2] = c[u][h][3] = 0.f;
                     unsigned ka[NW], kb[NW];
-                    const unsigned pa = in_tile + 16 * u + tau;
-                    if constexpr (HD == 128) {
-                        const uint4 a = *reinterpret_cast<const uint4 *>(tile + swizzled(pa, 16 * t4));
-                        const uint4 b = *reinterpret_cast<const uint4 *>(tile + swizzled(pa + 8, 16 * t4));
-                        ka[0] = a.x; ka[1] = a.y; ka[2] = a.z; ka[3] = a.w;
-                        kb[0] = b.x; kb[1] = b.y; kb[2] = b.z; kb[3] = b.w;
-                    } else {
-                        const uint2 a = *reinterpret_cast<const uint2 *>(tile + swizzled(pa, 8 * t4));
-                        const uint2 b = *reinterpret_cast<const uint2 *>(tile + swizzled(pa + 8, 8 * t4));
-                        ka[0] = a.x; ka[1] = a.y;
-                        kb[0] = b.x; kb[1] = b.y;
-                    }
+                    lds(ka, k_at + tile, (u0 + u) * 16 * S::ROW);
+                    lds(kb, k_at + tile, (u0 + u) * 16 * S::ROW + 8 * S::ROW);
 #pragma unroll
                     for (int i = 0; i < NW; ++i) {
 #pragma unroll
@@ -256,17 +262,9 @@ __global__ void __launch_bounds__(K4_THREADS, 3) kv4_decode_kernel(const __grid_
                 for (int u = 0; u < J; ++u)
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
-                        const unsigned pos = in_tile + 16 * u + tau + 8 * h;
                         unsigned kw[G], vw[G];
-                        if constexpr (G == 2) {
-                            const uint2 a = *reinterpret_cast<const uint2 *>(tile + S::OFF_KS + pos * 8);
-                            const uint2 b = *reinterpret_cast<const uint2 *>(tile + S::OFF_VS + pos * 8);
-                            kw[0] = a.x; kw[1] = a.y;
-                            vw[0] = b.x; vw[1] = b.y;
-                        } else {
-                            kw[0] = *reinterpret_cast<const unsigned *>(tile + S::OFF_KS + pos * 4);
-                            vw[0] = *reinterpret_cast<const unsigned *>(tile + S::OFF_VS + pos * 4);
-                        }
+                        lds(kw, s_at + tile, ((u0 + u) * 16 + 8 * h) * S::SCALES);
+                        lds(vw, s_at + tile, ((u0 + u) * 16 + 8 * h) * S::SCALES + S::OFF_VS - S::OFF_KS);
 #pragma unroll
                         for (int i = 0; i < G; ++i) {
                             ks[u][h][i] = __half22float2(*reinterpret_cast<const __half2 *>(&kw[i]));
@@ -359,42 +357,48 @@ __global__ void __launch_bounds__(K4_THREADS, 3) kv4_decode_kernel(const __grid_
 #pragma unroll
                 for (int u = 0; u < J; ++u) {
                     unsigned b[G][2], bl[G][2];
+                    float p[2][W];
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        float p[W];
+                    for (int h = 0; h < 2; ++h)
 #pragma unroll
                         for (int w = 0; w < W; ++w) {
-                            p[w] = ex2(x[u][h][w] - m[w]);
-                            l[w] += p[w];
+                            p[h][w] = ex2(x[u][h][w] - m[w]);
+                            l[w] += p[h][w];
                         }
 #pragma unroll
-                        for (int i = 0; i < G; ++i) {
-                            __half ph[W], pl[W];
+                    for (int i = 0; i < G; ++i) {
+                        float wt[2][W];
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
                             const float unit = vs[u][h][i].x * vref;
 #pragma unroll
                             for (int w = 0; w < W; ++w) {
-                                zero[w][i] = fmaf(p[w], vs[u][h][i].y, zero[w][i]);
-                                split_half(p[w] * unit, ph[w], pl[w]);
+                                zero[w][i] = fmaf(p[h][w], vs[u][h][i].y, zero[w][i]);
+                                wt[h][w] = p[h][w] * unit;
                             }
-                            if constexpr (W == 1) b[i][h] = movmatrix(pack(ph[0], pl[0]));
-                            else {
-                                b[i][h] = movmatrix(pack(ph[0], ph[1]));
-                                if constexpr (LO) bl[i][h] = movmatrix(pack(pl[0], pl[1]));
+                        }
+                        if constexpr (W == 1) {  // columns: high and low half of a row
+                            const unsigned hi = pack2(wt[0][0], wt[1][0]);
+                            const float2 back = unpack2(hi);
+                            const unsigned lo = pack2(wt[0][0] - back.x, wt[1][0] - back.y);
+                            b[i][0] = movmatrix(__byte_perm(hi, lo, 0x5410));
+                            b[i][1] = movmatrix(__byte_perm(hi, lo, 0x7632));
+                        } else {
+#pragma unroll
+                            for (int h = 0; h < 2; ++h) {
+                                const unsigned hi = pack2(wt[h][0], wt[h][W - 1]);
+                                b[i][h] = movmatrix(hi);
+                                if constexpr (LO) {
+                                    const float2 back = unpack2(hi);
+                                    bl[i][h] = movmatrix(pack2(wt[h][0] - back.x, wt[h][W - 1] - back.y));
+                                }
                             }
                         }
                     }
                     unsigned v[4][G];  // eight numbers of each group of positions ta, ta ^ X, and both + 8
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const unsigned pos = in_tile + 16 * u + ((i & 1 ? ta ^ X : ta) + (i & 2 ? 8 : 0));
-                        if constexpr (G == 2) {
-                            const uint2 y = *reinterpret_cast<const uint2 *>(tile + S::OFF_V + swizzled(pos, 8 * g));
-                            v[i][0] = y.x;
-                            v[i][1] = y.y;
-                        } else {
-                            v[i][0] = *reinterpret_cast<const unsigned *>(tile + S::OFF_V + swizzled(pos, 4 * g));
-                        }
-                    }
+                    for (int i = 0; i < 4; ++i)
+                        lds(v[i], (i & 1 ? v_at1 : v_at0) + tile, ((u0 + u) * 16 + (i & 2 ? 8 : 0)) * S::ROW);
 #pragma unroll
                     for (int i = 0; i < G; ++i)
 #pragma unroll
@@ -415,7 +419,7 @@ __global__ void __launch_bounds__(K4_THREADS, 3) kv4_decode_kernel(const __grid_
             if (lane == 0) mbar_arrive(empty + stage);
             advance();
         }
-        // ---- the four warps' parts: sums over the lanes of a row, then over the warps
+        // ---- the warps' parts: sums over the lanes of a row, then over the warps
         const float back = vexp < -126 ? 0.f : power_of_two(vexp) * (16777216.f / P_SCALE);
 #pragma unroll
         for (int w = 0; w < W; ++w) {
@@ -457,7 +461,7 @@ template <int HD, int W, bool LO> static int decode_launch(const Kv4Attention &A
     using S = K4Shape<HD>;
     constexpr int R = 4 * W;
     constexpr size_t smem = 1024 + (size_t)S::STAGES * S::STAGE + K4_WARPS * R * HD * 4 + K4_WARPS * R * 8 + S::STAGES * 20 + 16;
-    static_assert(smem <= 75 * 1024, "three CTAs per SM");
+    static_assert(smem <= 227 * 1024 / K4_CTAS - 1024, "CTAs of an SM");
     static std::atomic<unsigned> allowed{0};
     if (allow_shared((const void *)kv4_decode_kernel<HD, W, LO>, smem, allowed)) return -2;
     kv4_decode_kernel<HD, W, LO><<<grid, K4_THREADS, smem, s>>>(A, k, v);
