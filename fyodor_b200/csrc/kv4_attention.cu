@@ -13,12 +13,13 @@ TilesLaunch kv4_tiles_128_32, kv4_tiles_128_64, kv4_tiles_128_256, kv4_tiles_64_
 
 constexpr unsigned K4T_GRID = 148;  // one CTA per SM
 
-// K or V as token rows of head_dim / 2 bytes, boxes of one block (128 rows at most), rows of 64 bytes in the swizzle of
-// 64 bytes: 16-byte chunk c of token row t lies at chunk c ^ (t >> 1 & 3).
+// K or V as rows of 128 bytes (two tokens of 64, or four of 32 bytes), boxes of one block (128 tokens at most), in the
+// swizzle of 128 bytes (kv4_at). Rows of one token each kept the copies from more than 0.68 of HBM's rate.
 static int kv4_tensor_map(CUtensorMap *map, const fyb_kv4_cache &c, const void *pool)
 {
-    return kv8_tensor_map(map, pool, c.head_dim / 2, (size_t)c.blocks * c.kv_heads * c.block_size,
-                          std::min(c.block_size, (unsigned)K4_TILE), c.head_dim == 128 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_NONE);
+    const unsigned tokens = 256 / c.head_dim;
+    return kv8_tensor_map(map, pool, 128, (size_t)c.blocks * c.kv_heads * c.block_size / tokens,
+                          std::min(c.block_size, (unsigned)K4_TILE) / tokens, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
 // Row tile of the many-row kernel.

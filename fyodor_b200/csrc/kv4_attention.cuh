@@ -13,6 +13,24 @@ struct Kv4Attention : Kv8Attention {
     bool vec, vec_out;       // rows of 16 bits of q, of out begin on 16 bytes
 };
 
+// Byte `byte` of token `pos` of a tile of K or V in shared memory: rows of 128 bytes, 16-byte chunk c of row r at c ^ (r & 7).
+template <int HD> FYB_HOST_DEV unsigned kv4_at(unsigned pos, unsigned byte)
+{
+    constexpr unsigned ROW = HD / 2, TOKENS = 128 / ROW;
+    const unsigned row = pos / TOKENS;
+    return row * 128 + ((pos % TOKENS * ROW + byte) ^ ((row & 7) << 4));
+}
+FYB_DEV void k4_copy(unsigned dst, const void *src, unsigned bytes, unsigned bar)
+{
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                 :: "r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
+}
+FYB_DEV void k4_load_rows(unsigned dst, const CUtensorMap *map, int row, unsigned bar)
+{
+    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
+                 :: "r"(dst), "l"(map), "r"(0), "r"(row), "r"(bar) : "memory");
+}
+
 int launch_kv4_decode(const Kv4Attention &A, const CUtensorMap &k, const CUtensorMap &v, unsigned grid, cudaStream_t s);
 constexpr int K4_TILE = 128;  // positions of a unit
 constexpr unsigned K4_CTAS = 3, K4_GRID = K4_CTAS * 148;  // of the few-row kernel: CTAs per SM, largest grid

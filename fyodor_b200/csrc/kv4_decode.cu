@@ -94,8 +94,8 @@ __global__ void __launch_bounds__(K4_THREADS, K4_CTAS) kv4_decode_kernel(const _
                     }
                 }
                 wait(empty + stage, phase ^ 1);
-                const int mine = __shfl_sync(0xffffffffu, id, (b0 & 31) + (int)(lane % per));
-                const bool load = lane < per && mine >= 0;
+                const int block = __shfl_sync(0xffffffffu, id, (b0 & 31) + (int)(lane % per));
+                const bool load = lane < per && block >= 0;
                 const unsigned boxes = __ballot_sync(0xffffffffu, load);
                 // groups of 16 positions whose block is among the loaded ones
                 const unsigned groups = __ballot_sync(0xffffffffu, lane < K4_TILE / 16 && (boxes >> (lane * 16 / box) & 1));
@@ -105,12 +105,12 @@ __global__ void __launch_bounds__(K4_THREADS, K4_CTAS) kv4_decode_kernel(const _
                 }
                 __syncwarp();
                 if (load && !*dead) {
-                    const unsigned row = (((unsigned)mine * kv + s.head / A.split) << A.shift) + ((unsigned)(t * K4_TILE) & (size - 1));
-                    unsigned char *dst = ring + stage * S::STAGE;
-                    tma_load_rows(dst + lane * box * S::ROW, &kmap, (int)row, full + stage);
-                    tma_load_rows(dst + S::OFF_V + lane * box * S::ROW, &vmap, (int)row, full + stage);
-                    bulk_copy_g2s(dst + S::OFF_KS + lane * box * S::SCALES, A.ks + (size_t)row * G, box * S::SCALES, full + stage);
-                    bulk_copy_g2s(dst + S::OFF_VS + lane * box * S::SCALES, A.vs + (size_t)row * G, box * S::SCALES, full + stage);
+                    const unsigned row = (((unsigned)block * kv + s.head / A.split) << A.shift) + ((unsigned)(t * K4_TILE) & (size - 1));  // a token
+                    const unsigned dst = smem_u32(ring + stage * S::STAGE), at = lane * box, bar = smem_u32(full + stage);
+                    k4_load_rows(dst + at * S::ROW, &kmap, (int)(row / (128 / S::ROW)), bar);
+                    k4_load_rows(dst + S::OFF_V + at * S::ROW, &vmap, (int)(row / (128 / S::ROW)), bar);
+                    k4_copy(dst + S::OFF_KS + at * S::SCALES, A.ks + (size_t)row * G, box * S::SCALES, bar);
+                    k4_copy(dst + S::OFF_VS + at * S::SCALES, A.vs + (size_t)row * G, box * S::SCALES, bar);
                 }
                 __syncwarp();
                 ++issued;
@@ -126,15 +126,17 @@ __global__ void __launch_bounds__(K4_THREADS, K4_CTAS) kv4_decode_kernel(const _
     // ---- consumers
     const unsigned g = lane >> 2, t4 = lane & 3;
     // Positions of a tile's 16 in the order of the MMAs: a thread has, of K, rows tau and tau + 8, of V rows ta, ta ^ X
-    // and both + 8 (the same as k indexes 2 t4, 2 t4 + 1 and both + 8). Chosen so that the rows that one phase of a
-    // load reads lie in different banks (rows of 64 bytes in the swizzle of 64, of 32 bytes in none).
+    // and both + 8 (the same as k indexes 2 t4, 2 t4 + 1 and both + 8). Chosen so that what one phase of a load reads lies
+    // in different banks.
     constexpr unsigned X = HD == 128 ? 3 : 7;
     auto order = [](unsigned t) { return HD == 128 ? (t & 1) + 4 * (t >> 1) : t; };
     const unsigned ta = order(t4), tau = order(g >> 1) ^ (g & 1 ? X : 0u);
-    // this lane's place in a tile: of K, of V (two rows), of scales; 8 rows, 16 and tiles further on all of them grow alike
-    auto swizzled = [](unsigned pos, unsigned byte) { return pos * S::ROW + (HD == 128 ? byte ^ ((pos >> 1 & 3) << 4) : byte); };
+    // this lane's place in a tile: of K, of V (two rows), of scales; eight rows further on it is `ahead` away
     const unsigned mine = smem_u32(ring) + warp * K4_SHARE * 16 * S::ROW;
-    const unsigned k_at = mine + swizzled(tau, 4 * NW * t4), v_at0 = mine + S::OFF_V + swizzled(ta, 4 * G * g), v_at1 = mine + S::OFF_V + swizzled(ta ^ X, 4 * G * g);
+    const unsigned k_at = mine + kv4_at<HD>(tau, 4 * NW * t4), v_at0 = mine + S::OFF_V + kv4_at<HD>(ta, 4 * G * g), v_at1 = mine + S::OFF_V + kv4_at<HD>(ta ^ X, 4 * G * g);
+    auto ahead = [](unsigned at, unsigned tile, unsigned eights) {  // rows of 128 bytes move by 8 ROW / 128 each, and the swizzle with them
+        return (at ^ (eights * (8 * S::ROW / 128) % 8 << 4)) + eights * 8 * S::ROW + tile;
+    };
     const unsigned s_at = smem_u32(ring) + S::OFF_KS + (warp * K4_SHARE * 16 + tau) * S::SCALES;
     constexpr float P_SCALE = 32.f;  // keeps small weights clear of fp16's smallest numbers; the largest is 2^14
     auto bar = [] { asm volatile("bar.sync 1, %0;" :: "n"(32 * K4_WARPS) : "memory"); };
@@ -243,8 +245,8 @@ __global__ void __launch_bounds__(K4_THREADS, K4_CTAS) kv4_decode_kernel(const _
 #pragma unroll
                     for (int h = 0; h < G; ++h) c[u][h][0] = c[u][h][1] = c[u][h][2] = c[u][h][3] = 0.f;
                     unsigned ka[NW], kb[NW];
-                    lds(ka, k_at + tile, (u0 + u) * 16 * S::ROW);
-                    lds(kb, k_at + tile, (u0 + u) * 16 * S::ROW + 8 * S::ROW);
+                    lds(ka, ahead(k_at, tile, (u0 + u) * 2), 0);
+                    lds(kb, ahead(k_at, tile, (u0 + u) * 2 + 1), 0);
 #pragma unroll
                     for (int i = 0; i < NW; ++i) {
 #pragma unroll
@@ -398,7 +400,7 @@ __global__ void __launch_bounds__(K4_THREADS, K4_CTAS) kv4_decode_kernel(const _
                     unsigned v[4][G];  // eight numbers of each group of positions ta, ta ^ X, and both + 8
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
-                        lds(v[i], (i & 1 ? v_at1 : v_at0) + tile, ((u0 + u) * 16 + (i & 2 ? 8 : 0)) * S::ROW);
+                        lds(v[i], ahead(i & 1 ? v_at1 : v_at0, tile, (u0 + u) * 2 + (i >> 1)), 0);
 #pragma unroll
                     for (int i = 0; i < G; ++i)
 #pragma unroll

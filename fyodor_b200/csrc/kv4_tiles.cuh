@@ -32,11 +32,11 @@ namespace fyb {
 constexpr int K4T_CONV = 4, K4T_META = 8;
 FYB_HOST_DEV constexpr unsigned k4t_segs(int NR) { return NR == 256 ? 2 : 4; }   // segments handed on at a time (room for no more)
 FYB_HOST_DEV constexpr int k4t_groups(int NR) { return NR == 256 ? 2 : 1; }      // groups of four softmax warps
-FYB_HOST_DEV constexpr int k4t_threads(int NR) { return 32 * (4 * k4t_groups(NR) + 2 * K4T_CONV + 2); }
+FYB_HOST_DEV constexpr int k4t_threads(int NR) { return 32 * (4 * k4t_groups(NR) + 2 * K4T_CONV + 3); }
 
 template <int HD, int NR> struct K4tShape {
     static constexpr int ROW = HD / 2, SCALES = HD / 64 * 4;                 // bytes of a token's row, of its scales
-    static constexpr int RAW = K4_TILE * (ROW + SCALES), RAW_S = K4_TILE * ROW;  // a tile of K or V as it lies in the cache
+    static constexpr int RAW_S = K4_TILE * ROW, RAW = RAW_S + 1024;           // a tile of K or V as it lies in the cache, and its scales
     static constexpr bool Q_TM = NR < 256;                                   // q in tensor memory
     // raw tiles on their way: as many as there is room for
     static constexpr int KS = HD == 64 || Q_TM ? 4 : 2, VS = HD == 64 || Q_TM ? 4 : 1;
@@ -106,7 +106,7 @@ __global__ void __launch_bounds__(k4t_threads(NR), 1) kv4_tiles_kernel(const __g
     const __grid_constant__ CUtensorMap vmap)
 {
     using S = K4tShape<HD, NR>;
-    constexpr unsigned GROUPS = k4t_groups(NR), SOFT = 4 * GROUPS, W_CONV = SOFT, W_TMA = SOFT + 2 * K4T_CONV, W_MMA = W_TMA + 1;
+    constexpr unsigned GROUPS = k4t_groups(NR), SOFT = 4 * GROUPS, W_CONV = SOFT, W_TMA = SOFT + 2 * K4T_CONV, W_MMA = W_TMA + 2;
     constexpr unsigned CP = GROUPS == 2 ? 1 : 128 / NR, CW = 128 / CP, CHUNKS = CW / 32;   // copies, and the positions and blocks of 32 of a copy
     constexpr unsigned SEGS = k4t_segs(NR);
     constexpr int G64 = HD / 64;
@@ -130,7 +130,7 @@ __global__ void __launch_bounds__(k4t_threads(NR), 1) kv4_tiles_kernel(const __g
         for (unsigned i = 0; i < SEGS; ++i) {
             mbar_init(sh.q_full + i, GROUPS * K4T_CONV);
             mbar_init(sh.seg_full + i, 1);
-            mbar_init(sh.seg_empty + i, SOFT + 2 * K4T_CONV + 1);
+            mbar_init(sh.seg_empty + i, SOFT + 2 * K4T_CONV + 2);
         }
         sh.dead = 0;
         fence_barrier_init();
@@ -475,6 +475,7 @@ __global__ void __launch_bounds__(k4t_threads(NR), 1) kv4_tiles_kernel(const __g
                 const unsigned char *raw = ring + (is_v ? S::OFF_RV : S::OFF_RK) + st * S::RAW, *scales = raw + S::RAW_S;
                 unsigned char *dst = ring + (is_v ? S::OFF_V : S::OFF_K) + b * S::TILE;
                 // V of positions that no row attends, or never loaded, is 0 and not what lies there (a NaN stays one times 0)
+                wait(sh.meta_full + n % K4T_META, n / K4T_META);
                 const unsigned here = sh.here[n % K4T_META];
                 const bool patchy = is_v && (here != 0xffu || any < (t + 1) * K4_TILE);
                 // four tokens' words and scales at a time, before the first of their stores (which they might overlap, as
@@ -486,12 +487,12 @@ __global__ void __launch_bounds__(k4t_threads(NR), 1) kv4_tiles_kernel(const __g
                     for (unsigned i = 0; i < 4; ++i) {
                         const unsigned tok = tok0 + 4 * (i0 + i);
                         if constexpr (G64 == 2) {
-                            const uint2 x = *reinterpret_cast<const uint2 *>(raw + tok * 64 + ((8 * j) ^ ((tok >> 1 & 3) << 4)));
+                            const uint2 x = *reinterpret_cast<const uint2 *>(raw + kv4_at<HD>(tok, 8 * j));
                             const uint2 y = *reinterpret_cast<const uint2 *>(scales + tok * 8);
                             w[i][0] = x.x; w[i][1] = x.y;
                             sc[i][0] = y.x; sc[i][1] = y.y;
                         } else {
-                            w[i][0] = *reinterpret_cast<const unsigned *>(raw + tok * 32 + 4 * j);
+                            w[i][0] = *reinterpret_cast<const unsigned *>(raw + kv4_at<HD>(tok, 4 * j));
                             sc[i][0] = *reinterpret_cast<const unsigned *>(scales + tok * 4);
                         }
                     }
@@ -520,25 +521,38 @@ __global__ void __launch_bounds__(k4t_threads(NR), 1) kv4_tiles_kernel(const __g
             }
             done();
         }
-    } else if (warp == W_TMA) {
-        // ================================================== TMA
-        const unsigned size = 1u << A.shift, box = min(size, (unsigned)K4_TILE), per = K4_TILE / box;
+    } else if (warp < W_MMA) {
+        // ================================================== TMA: a warp for K, which walks the line, and one for V (one for
+        // both took 1850 cycles a tile, as long as the tile)
+        const bool is_v = warp > W_TMA;
+        const unsigned size = 1u << A.shift, box = min(size, (unsigned)K4_TILE), per = K4_TILE / box, stages = is_v ? S::VS : S::KS;
+        const CUtensorMap *map = is_v ? &vmap : &kmap;
+        const __half2 *scale = is_v ? A.vs : A.ks;
+        uint64_t *full = is_v ? sh.rv_full : sh.rk_full, *empty = is_v ? sh.rv_empty : sh.rk_empty;
+        const unsigned raw = smem_u32(ring + (is_v ? S::OFF_RV : S::OFF_RK)), lane_at = lane % per * box;
         __syncwarp();
         Kv8Walk<K4_TILE> walk(A, sh.place);
-        Kv8Segment s;
-        for (;; ++seg) {
-            const bool more = walk.next(s);
-            if (seg >= SEGS) wait(sh.seg_empty + seg % SEGS, seg / SEGS - 1);
-            if (lane == 0 && !*dead) {
-                if (more) sh.seg[seg % SEGS] = s; else sh.seg[seg % SEGS].t1 = 0;
-                mbar_arrive(sh.seg_full + seg % SEGS);
+        Kv8Segment own;
+        for (;;) {
+            const Kv8Segment *s = &own;
+            if (is_v) {
+                s = next();
+                if (!s) break;
+            } else {
+                const bool more = walk.next(own);
+                if (seg >= SEGS) wait(sh.seg_empty + seg % SEGS, seg / SEGS - 1);
+                if (lane == 0 && !*dead) {
+                    if (more) sh.seg[seg % SEGS] = own; else sh.seg[seg % SEGS].t1 = 0;
+                    mbar_arrive(sh.seg_full + seg % SEGS);
+                }
+                __syncwarp();
+                if (!more) break;
             }
-            __syncwarp();
-            if (!more) break;
-            const int blocks = (kv8_attended(A, s.q, s.row_tile) + (int)size - 1) >> A.shift;
-            const int *ids = A.table + (size_t)s.request * A.table_stride;
+            const int blocks = (kv8_attended(A, s->q, s->row_tile) + (int)size - 1) >> A.shift, t1 = s->t1;
+            const int *ids = A.table + (size_t)s->request * A.table_stride;
+            const unsigned head = s->head;
             int have = -1, id = 0;  // lane holds block 32 * have + lane
-            for (int t = s.t0; t < s.t1; ++t, ++n) {
+            for (int t = s->t0; t < t1; ++t, ++n) {
                 const int b0 = t * K4_TILE >> A.shift;
                 if (b0 / 32 != have) {
                     have = b0 / 32;
@@ -549,39 +563,36 @@ __global__ void __launch_bounds__(k4t_threads(NR), 1) kv4_tiles_kernel(const __g
                         id = -1;
                     }
                 }
-                const int own = __shfl_sync(0xffffffffu, id, (b0 & 31) + (int)(lane % per));
-                const bool load = lane < per && own >= 0;
+                const unsigned st = n % stages;
+                const int block = __shfl_sync(0xffffffffu, id, (b0 & 31) + (int)(lane % per));
+                const bool load = lane < per && block >= 0;
                 const unsigned boxes = __ballot_sync(0xffffffffu, load);
-                // groups of 16 positions whose block is among the loaded ones
-                const unsigned groups = __ballot_sync(0xffffffffu, lane < K4_TILE / 16 && (boxes >> (lane * 16 / box) & 1));
-                const unsigned row = (((unsigned)own * kv + s.head) << A.shift) + ((unsigned)(t * K4_TILE) & (size - 1));
-                auto bring = [&](const CUtensorMap &map, const __half2 *scale, unsigned off, unsigned stages, uint64_t *full, uint64_t *empty, bool first) {
-                    const unsigned st = n % stages;
-                    if (n >= stages) wait(empty + st, n / stages - 1);
+                if (n >= stages) wait(empty + st, n / stages - 1);
+                if (!is_v) {  // groups of 16 positions whose block is among the loaded ones
+                    const unsigned groups = __ballot_sync(0xffffffffu, lane < K4_TILE / 16 && (boxes >> (lane * 16 / box) & 1));
                     if (lane == 0) {
-                        if (first) {
-                            sh.here[n % K4T_META] = groups;
-                            mbar_arrive(sh.meta_full + n % K4T_META);
-                        }
-                        if (boxes) mbar_expect_tx(full + st, __popc(boxes) * box * (S::ROW + S::SCALES)); else mbar_arrive(full + st);
+                        sh.here[n % K4T_META] = groups;
+                        mbar_arrive(sh.meta_full + n % K4T_META);
                     }
-                    __syncwarp();
-                    if (load && !*dead) {
-                        unsigned char *dst = ring + off + st * S::RAW;
-                        tma_load_rows(dst + lane * box * S::ROW, &map, (int)row, full + st);
-                        bulk_copy_g2s(dst + S::RAW_S + lane * box * S::SCALES, scale + (size_t)row * G64, box * S::SCALES, full + st);
-                    }
-                    __syncwarp();
-                };
-                bring(kmap, A.ks, S::OFF_RK, S::KS, sh.rk_full, sh.rk_empty, true);
-                bring(vmap, A.vs, S::OFF_RV, S::VS, sh.rv_full, sh.rv_empty, false);
+                }
+                if (lane == 0) {
+                    if (boxes) mbar_expect_tx(full + st, __popc(boxes) * box * (S::ROW + S::SCALES)); else mbar_arrive(full + st);
+                }
+                __syncwarp();
+                if (load && !*dead) {
+                    const unsigned row = (((unsigned)block * kv + head) << A.shift) + ((unsigned)(t * K4_TILE) & (size - 1));
+                    const unsigned dst = raw + st * S::RAW, bar = smem_u32(full + st);
+                    k4_load_rows(dst + lane_at * S::ROW, map, (int)(row / (128 / S::ROW)), bar);
+                    k4_copy(dst + S::RAW_S + lane_at * S::SCALES, scale + (size_t)row * G64, box * S::SCALES, bar);
+                }
+                __syncwarp();
             }
+            if (is_v) done(); else ++seg;
         }
         if (*dead) {  // copies in flight land before the CTA leaves its shared memory
-            for (unsigned i = 0; i < min(n, 4u); ++i) {
+            for (unsigned i = 0; i < min(n, stages); ++i) {
                 const unsigned k = n - 1 - i;
-                if (i < S::KS) mbar_wait_bounded(sh.rk_full + k % S::KS, k / S::KS & 1);
-                if (i < S::VS) mbar_wait_bounded(sh.rv_full + k % S::VS, k / S::VS & 1);
+                mbar_wait_bounded(full + k % stages, k / stages & 1);
             }
         }
     } else {
