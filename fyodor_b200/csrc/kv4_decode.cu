@@ -22,6 +22,7 @@
 namespace fyb {
 
 // SHARE: groups of 16 positions of a tile that a warp takes
+constexpr int K4_COST = 3;  // a segment's beginning and end, in tiles
 constexpr int K4_WARPS = 4, K4_SHARE = K4_TILE / 16 / K4_WARPS, K4_THREADS = 32 * (K4_WARPS + 1);
 
 // Words of shared memory: the address of a lane, and what is the same for all of them as the offset.
@@ -63,8 +64,8 @@ __global__ void __launch_bounds__(K4_THREADS, K4_CTAS) kv4_decode_kernel(const _
         *dead = 0;
         fence_barrier_init();
     }
-    const Kv8Place place = kv8_place<K4_TILE, K4_THREADS, 5>(A);  // a CTA barrier inside
-    Kv8Walk<K4_TILE> walk(A, place);
+    const Kv8Place place = kv8_place<K4_TILE, K4_THREADS, 5, K4_COST>(A);  // a CTA barrier inside
+    Kv8Walk<K4_TILE, K4_COST> walk(A, place);
     Kv8Segment s;
     unsigned stage = 0, phase = 0;
     auto advance = [&] { if (++stage == S::STAGES) { stage = 0; phase ^= 1; } };

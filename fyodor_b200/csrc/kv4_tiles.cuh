@@ -34,6 +34,8 @@ FYB_HOST_DEV constexpr unsigned k4t_segs(int NR) { return NR == 256 ? 2 : 4; }  
 FYB_HOST_DEV constexpr int k4t_groups(int NR) { return NR == 256 ? 2 : 1; }      // groups of four softmax warps
 FYB_HOST_DEV constexpr int k4t_threads(int NR) { return 32 * (4 * k4t_groups(NR) + 2 * K4T_CONV + 3); }
 
+FYB_HOST_DEV constexpr int k4t_cost(int NR) { return NR == 256 ? 9 : 6; }        // a segment's beginning and end, in tiles
+
 template <int HD, int NR> struct K4tShape {
     static constexpr int ROW = HD / 2, SCALES = HD / 64 * 4;                 // bytes of a token's row, of its scales
     static constexpr int RAW_S = K4_TILE * ROW, RAW = RAW_S + 1024;           // a tile of K or V as it lies in the cache, and its scales
@@ -60,9 +62,9 @@ template <int NR> struct K4tShared {
     unsigned flag, dead;
 };
 
-static __device__ __noinline__ void k4t_segment(const Kv4Attention &A, const Kv8Place &place, unsigned k, Kv8Segment *s)
+template <int COST> static __device__ __noinline__ void k4t_segment(const Kv4Attention &A, const Kv8Place &place, unsigned k, Kv8Segment *s)
 {
-    Kv8Walk<K4_TILE> walk(A, place);
+    Kv8Walk<K4_TILE, COST> walk(A, place);
     for (unsigned i = 0; i <= k; ++i)
         if (!walk.next(*s)) { s->t1 = 0; break; }
 }
@@ -141,7 +143,7 @@ __global__ void __launch_bounds__(k4t_threads(NR), 1) kv4_tiles_kernel(const __g
     }
     kt_fence_before();
     {
-        const Kv8Place place = kv8_place<K4_TILE, k4t_threads(NR), 2>(A);  // CTA barriers inside
+        const Kv8Place place = kv8_place<K4_TILE, k4t_threads(NR), 2, k4t_cost(NR)>(A);  // CTA barriers inside
         if (tid == 0) sh.place = place;
     }
     __syncthreads();
@@ -158,7 +160,7 @@ __global__ void __launch_bounds__(k4t_threads(NR), 1) kv4_tiles_kernel(const __g
         const Kv8Segment *s = sh.seg + seg % SEGS;
         if (__builtin_expect(*dead, 0)) {
             s = sh.walked + warp;
-            if (lane == 0) k4t_segment(A, sh.place, seg, sh.walked + warp);
+            if (lane == 0) k4t_segment<k4t_cost(NR)>(A, sh.place, seg, sh.walked + warp);
             __syncwarp();
         }
         return s->t1 ? s : nullptr;
@@ -531,7 +533,7 @@ __global__ void __launch_bounds__(k4t_threads(NR), 1) kv4_tiles_kernel(const __g
         uint64_t *full = is_v ? sh.rv_full : sh.rk_full, *empty = is_v ? sh.rv_empty : sh.rk_empty;
         const unsigned raw = smem_u32(ring + (is_v ? S::OFF_RV : S::OFF_RK)), lane_at = lane % per * box;
         __syncwarp();
-        Kv8Walk<K4_TILE> walk(A, sh.place);
+        Kv8Walk<K4_TILE, k4t_cost(NR)> walk(A, sh.place);
         Kv8Segment own;
         for (;;) {
             const Kv8Segment *s = &own;

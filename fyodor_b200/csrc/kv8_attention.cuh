@@ -65,10 +65,12 @@ FYB_DEV int kv8_row_tiles(const Kv8Attention &A, const Kv8Request &q)
 {
     return (q.rows + (int)A.row_tile - 1) / (int)A.row_tile;
 }
-template <int TILE> FYB_DEV unsigned kv8_units(const Kv8Attention &A, const Kv8Request &q)
+// COST: units without work before the tiles of each segment, as many as beginning and ending it takes the time of: a CTA
+// with several short segments gets fewer tiles.
+template <int TILE, int COST = 0> FYB_DEV unsigned kv8_units(const Kv8Attention &A, const Kv8Request &q)
 {
     unsigned u = 0;
-    for (int i = 0; i < kv8_row_tiles(A, q); ++i) u += (unsigned)kv8_tiles<TILE>(A, q, i);
+    for (int i = 0; i < kv8_row_tiles(A, q); ++i) u += (unsigned)kv8_tiles<TILE>(A, q, i) + COST;
     return u * A.c.kv_heads;
 }
 // CTAs that take part, and where their ranges begin. Few units go to fewer
@@ -100,7 +102,7 @@ struct Kv8Place {
 // parts to join, and a request's result does not depend on the others (16
 // requests of 20 to 60 tokens: 17.6 us on the line's ranges, 6.2 so; one of 300
 // with eight rows of four heads: 28.8 and 17.3).
-template <int TILE, int THREADS, int LEAST> FYB_DEV Kv8Place kv8_place(const Kv8Attention &A)
+template <int TILE, int THREADS, int LEAST, int COST = 0> FYB_DEV Kv8Place kv8_place(const Kv8Attention &A)
 {
     __shared__ uint2 warp_sum[THREADS / 32];
     __shared__ unsigned found[4], longest;
@@ -111,7 +113,7 @@ template <int TILE, int THREADS, int LEAST> FYB_DEV Kv8Place kv8_place(const Kv8
     for (unsigned r = r0; r < r1; ++r) {
         const Kv8Request q = kv8_request(A, r, blockIdx.x == 0);
         const int tiles = kv8_row_tiles(A, q);
-        units += kv8_units<TILE>(A, q);
+        units += kv8_units<TILE, COST>(A, q);
         segments += (unsigned)tiles * kv;
         if (tiles) most = max(most, (unsigned)kv8_tiles<TILE>(A, q, tiles - 1));  // the last row tile attends most
     }
@@ -145,7 +147,7 @@ template <int TILE, int THREADS, int LEAST> FYB_DEV Kv8Place kv8_place(const Kv8
         unsigned r = r0, at = before, seg = segments_before;
         for (;; ++r) {
             const Kv8Request q = kv8_request(A, r, false);
-            const unsigned u = kv8_units<TILE>(A, q), n = (unsigned)kv8_row_tiles(A, q) * kv;
+            const unsigned u = kv8_units<TILE, COST>(A, q), n = (unsigned)kv8_row_tiles(A, q) * kv;
             if (whole ? blockIdx.x < seg + n : p.begin < at + u) break;
             at += u;
             seg += n;
@@ -157,8 +159,8 @@ template <int TILE, int THREADS, int LEAST> FYB_DEV Kv8Place kv8_place(const Kv8
             const Kv8Request q = kv8_request(A, r, false);
             unsigned left = blockIdx.x - seg, u = at;
             int i = 0;
-            for (; left >= kv; ++i, left -= kv) u += (unsigned)kv8_tiles<TILE>(A, q, i) * kv;
-            const unsigned tiles = (unsigned)kv8_tiles<TILE>(A, q, i);
+            for (; left >= kv; ++i, left -= kv) u += ((unsigned)kv8_tiles<TILE>(A, q, i) + COST) * kv;
+            const unsigned tiles = (unsigned)kv8_tiles<TILE>(A, q, i) + COST;
             found[2] = u + left * tiles;
             found[3] = u + (left + 1) * tiles;
         }
@@ -181,7 +183,7 @@ struct Kv8Segment {
     unsigned first_unit;   // line unit of tile 0
 };
 // Walks a CTA's segments in order.
-template <int TILE> struct Kv8Walk {
+template <int TILE, int COST = 0> struct Kv8Walk {
     const Kv8Attention &A;
     unsigned at, end, r, before;
     int i, tiles_i;
@@ -196,34 +198,40 @@ template <int TILE> struct Kv8Walk {
         q = kv8_request(A, r, false);
         i = 0;
         i_before = 0;
-        tiles_i = kv8_row_tiles(A, q) ? kv8_tiles<TILE>(A, q, 0) : 0;
+        tiles_i = kv8_row_tiles(A, q) ? kv8_tiles<TILE>(A, q, 0) + COST : 0;
     }
     FYB_DEV bool next(Kv8Segment &s)
     {
-        if (at >= end) return false;
         for (;;) {
+            if (at >= end) return false;
             const unsigned size = (unsigned)tiles_i * A.c.kv_heads;
-            if (at < before + i_before + size) break;
-            i_before += size;
-            if (i + 1 < kv8_row_tiles(A, q)) {
-                tiles_i = kv8_tiles<TILE>(A, q, ++i);
-            } else {
-                before += i_before;
-                if (++r >= A.requests) { at = end; return false; }
-                open();
+            if (at >= before + i_before + size) {
+                i_before += size;
+                if (i + 1 < kv8_row_tiles(A, q)) {
+                    tiles_i = kv8_tiles<TILE>(A, q, ++i) + COST;
+                } else {
+                    before += i_before;
+                    if (++r >= A.requests) { at = end; return false; }
+                    open();
+                }
+                continue;
             }
+            const unsigned x = at - before - i_before, in = x % (unsigned)tiles_i;
+            if (COST && in < COST) {  // up to the first tile
+                at += COST - in;
+                continue;
+            }
+            s.q = q;
+            s.request = r;
+            s.row_tile = i;
+            s.tiles = tiles_i - COST;
+            s.head = x / (unsigned)tiles_i;
+            s.t0 = (int)in - COST;
+            s.t1 = min(s.tiles, s.t0 + (int)(end - at));
+            s.first_unit = at - (unsigned)s.t0;
+            at += (unsigned)(s.t1 - s.t0);
+            return true;
         }
-        const unsigned x = at - before - i_before;
-        s.q = q;
-        s.request = r;
-        s.row_tile = i;
-        s.tiles = tiles_i;
-        s.head = x / (unsigned)tiles_i;
-        s.t0 = (int)(x % (unsigned)tiles_i);
-        s.t1 = min(tiles_i, s.t0 + (int)(end - at));
-        s.first_unit = at - (unsigned)s.t0;
-        at += (unsigned)(s.t1 - s.t0);
-        return true;
     }
 };
 
