@@ -186,6 +186,9 @@ def _load():
     lib.fyb_batch_create.argtypes = [_P, C.c_uint]
     lib.fyb_batch_create_kv8.restype = _P
     lib.fyb_batch_create_kv8.argtypes = [_P, C.c_uint, C.c_uint32, C.c_uint32, C.c_uint32]
+    lib.fyb_batch_create_kv4.restype = _P
+    lib.fyb_batch_create_kv4.argtypes = [_P, C.c_uint, C.c_uint32, C.c_uint32]
+    lib.fyb_batch_score.argtypes = [_P, _P, _P, _P, _P, _P, _P, C.c_uint32, _P, _P]
     lib.fyb_batch_free_blocks.restype = C.c_long
     lib.fyb_batch_free_blocks.argtypes = [_P]
     lib.fyb_batch_free.argtypes = [_P]
@@ -216,7 +219,7 @@ EXPORTS = ["nya_cuda_backend", "fyb_version", "fyb_device_count", "fyb_dequantiz
            "fyb_plan_time_greedy", "fyb_plan_launches_per_token", "fyb_plan_decode_form", "fyb_plan_profile", "fyb_plan_trace",
            "fyb_plan_tp_info", "fyb_plan_tp_handle", "fyb_plan_tp_connect", "fyb_plan_tp_disconnect",
            "fyb_plan_tp_connect_local", "fyb_plan_error", "fyb_plan_time_projection",
-           "fyb_batch_create", "fyb_batch_create_kv8", "fyb_batch_free_blocks", "fyb_batch_free", "fyb_batch_step", "fyb_batch_decode_greedy", "fyb_batch_time_greedy",
+           "fyb_batch_create", "fyb_batch_create_kv8", "fyb_batch_create_kv4", "fyb_batch_score", "fyb_batch_free_blocks", "fyb_batch_free", "fyb_batch_step", "fyb_batch_decode_greedy", "fyb_batch_time_greedy",
            "fyb_batch_launches_per_step",
            "fyb_synth_create",
            "fyb_synth_free", "fyb_synth_fill"]
@@ -599,7 +602,8 @@ class Batch:
 
     kv "int8" or "e4m3": a paged 8-bit cache of `blocks` blocks of block_size
     tokens that the sequences share, instead of an fp16 cache of the plan's
-    capacity each (fyb_batch_create_kv8)."""
+    capacity each (fyb_batch_create_kv8); "uint4": one in 4 bits
+    (fyb_batch_create_kv4)."""
 
     _ptr = None  # until it is made, and where it is declined
 
@@ -608,6 +612,8 @@ class Batch:
         self.V = plan.model.vocabulary
         if kv is None:
             ptr = lib.fyb_batch_create(C.c_void_p(plan.ptr), batch)
+        elif kv == "uint4":
+            ptr = lib.fyb_batch_create_kv4(C.c_void_p(plan.ptr), batch, blocks, block_size)
         else:
             ptr = lib.fyb_batch_create_kv8(C.c_void_p(plan.ptr), batch, blocks, block_size, _format(kv))
         if not ptr:
@@ -635,6 +641,27 @@ class Batch:
         if r:
             raise RuntimeError("fyb_batch_step failed (%d)" % r)
         return lg, am
+
+    def score(self, tokens, positions, targets=None, top=0):
+        """One step whose logits stay on the device (fyb_batch_score): dict of
+        logprob, rank (with targets, the tokens that follow; negative: none),
+        entropy [B], top_tokens and top_logprobs [B][top]."""
+        t, p = self._req(tokens, positions)
+        if not 0 <= top <= 32:
+            raise ValueError("top is 0 to 32")
+        out = dict(entropy=np.empty(self.B, np.float32), top_tokens=np.empty((self.B, top), np.int32),
+                   top_logprobs=np.empty((self.B, top), np.float32))
+        if targets is not None:
+            targets = np.ascontiguousarray(targets, np.int32)
+            if targets.shape != (self.B,):
+                raise ValueError("targets has to have one token for each sequence")
+            out |= dict(logprob=np.empty(self.B, np.float32), rank=np.empty(self.B, np.int32))
+        r = lib.fyb_batch_score(C.c_void_p(self.ptr), _ptr(t), _ptr(p), _ptr(targets), _ptr(out.get("logprob")),
+                                _ptr(out.get("rank")), _ptr(out["entropy"]), top, _ptr(out["top_tokens"]),
+                                _ptr(out["top_logprobs"]))
+        if r:
+            raise RuntimeError("fyb_batch_score failed (%d)" % r)
+        return out
 
     def decode_greedy(self, tokens, positions, steps):
         """Greedy tokens [steps][B] decoded on the device."""

@@ -32,7 +32,7 @@
 namespace fyb { struct Plan; }
 struct Batch;
 static void batch_free(Batch *bt);
-static Batch *batch_create(fyb::Plan *p, unsigned batch, bool chunk, const fyb_kv8_cache *paged = nullptr);
+static Batch *batch_create(fyb::Plan *p, unsigned batch, bool chunk, const fyb_kv8_cache *paged = nullptr, bool four = false);
 static int prefill_chunks(fyb::Plan *p, Batch *bt, const uint32_t *tokens, size_t count, size_t position, float *out);
 
 namespace fyb {
@@ -1239,9 +1239,9 @@ struct Batch {
     cudaGraphExec_t graphs[2] = {nullptr, nullptr};  // logits step, greedy step
     bool sized[2] = {false, false};
     unsigned long long launches = 0;
-    // a paged 8-bit cache in place of kc / vc (fyb_batch_create_kv8)
-    bool paged = false;
-    fyb_kv8_cache cache = {};            // layer 0; layer l's tensors follow
+    // a paged 8-bit or 4-bit cache in place of kc / vc (fyb_batch_create_kv8, _kv4)
+    bool paged = false, four = false;
+    fyb_kv8_cache cache = {};            // layer 0; layer l's tensors follow (4-bit: its scales are pairs of F16)
     unsigned table_stride = 0;
     int32_t *kv_len = nullptr;           // [B] lengths | free count
     int32_t *kv_next = nullptr;          // the same after the step
@@ -1249,6 +1249,11 @@ struct Batch {
     int32_t *kv_step = nullptr;          // [B + 1] row starts | [B] slots | [B] positions | [B] requests | [B] status
     float *qkv = nullptr;                // [B][QKV rows] in natural order
     std::vector<uint32_t> held;          // tokens of each sequence
+    // what fyb_batch_score takes and gives, by sequence
+    int32_t *targets = nullptr, *rank = nullptr, *top_tokens = nullptr;
+    float *logprob = nullptr, *entropy = nullptr, *top_logprobs = nullptr;
+    void *score_ws = nullptr;
+    size_t score_ws_bytes = 0;
 };
 
 static void batch_free(Batch *bt)
@@ -1303,15 +1308,28 @@ static int batch_blocks(const Batch *bt, cudaStream_t s)
     return cudaMemcpyAsync(bt->kv_len, bt->kv_next, (B + 1) * 4, cudaMemcpyDeviceToDevice, s) == cudaSuccess ? 0 : -2;
 }
 
+// 32-bit scales (4-bit: scale and low) and bytes of K or of V of a layer.
+static size_t batch_layer_scales(const fyb_kv8_cache &c, bool four)
+{
+    return (size_t)c.blocks * c.kv_heads * (four ? (size_t)c.block_size * (c.head_dim / 64) : 1);
+}
+static size_t batch_layer_bytes(const fyb_kv8_cache &c, bool four)
+{
+    return (size_t)c.blocks * c.kv_heads * c.block_size * c.head_dim / (four ? 2 : 1);
+}
 static fyb_kv8_cache batch_layer_cache(const Batch *bt, unsigned l)
 {
     fyb_kv8_cache c = bt->cache;
-    const size_t scales = (size_t)c.blocks * c.kv_heads, bytes = scales * c.block_size * c.head_dim;
+    const size_t scales = batch_layer_scales(c, bt->four), bytes = batch_layer_bytes(c, bt->four);
     c.k = (unsigned char *)c.k + l * bytes;
     c.v = (unsigned char *)c.v + l * bytes;
     c.k_scale += l * scales;
     c.v_scale += l * scales;
     return c;
+}
+static fyb_kv4_cache batch_four(const fyb_kv8_cache &c)
+{
+    return fyb_kv4_cache{c.k, c.v, c.k_scale, c.v_scale, c.blocks, c.kv_heads, c.block_size, c.head_dim};
 }
 
 // Layer l's append (q and K rotated on the way) and attention over it.
@@ -1323,13 +1341,19 @@ static int batch_paged_attention(Batch *bt, unsigned l, unsigned qkv_rows, cudaS
     const fyb_rope_desc rope = {p->rope_cos, p->rope_sin, (uint32_t)bt->capacity, p->hd, FYB_ROPE_INTERLEAVED};
     int r = launch_bt_qkv_rows(bt->y, qkv_rows, bt->qkv, B, s);
     if (r) return r;
+    const fyb_kv4_cache c4 = batch_four(c);
+    const float scale = 1.0f / std::sqrt((float)p->hd);
+    bt->launches += 2;  // the caller counts one
+    if (bt->four) {
+        r = fyb_kv4_append(&c4, bt->kv_step + B + 1, B, T_F32, bt->qkv + nq, qkv_rows, bt->qkv + nq + nk, qkv_rows, &rope,
+                           bt->kv_step + 2 * B + 1, bt->qkv, qkv_rows, bt->q, nq, p->H, p->err_dev, s);
+        return r ? r : fyb_kv4_attention(&c4, bt->kv_next, nullptr, B, 1, B, bt->kv_table, bt->table_stride, T_F32, bt->q, nq,
+                                         bt->attn, nq, p->H, scale, bt->attn_ws, bt->attn_ws_bytes, p->err_dev, s);
+    }
     r = fyb_kv8_append(&c, bt->kv_step + B + 1, B, T_F32, bt->qkv + nq, qkv_rows, bt->qkv + nq + nk, qkv_rows, &rope,
                        bt->kv_step + 2 * B + 1, bt->qkv, qkv_rows, bt->q, nq, p->H, p->err_dev, s);
-    if (r) return r;
-    bt->launches += 2;  // the caller counts one
-    return fyb_kv8_attention(&c, bt->kv_next, nullptr, B, 1, B, bt->kv_table, bt->table_stride, T_F32, bt->q, nq,
-                             bt->attn, nq, p->H, 1.0f / std::sqrt((float)p->hd), bt->attn_ws, bt->attn_ws_bytes,
-                             p->err_dev, s);
+    return r ? r : fyb_kv8_attention(&c, bt->kv_next, nullptr, B, 1, B, bt->kv_table, bt->table_stride, T_F32, bt->q, nq,
+                                     bt->attn, nq, p->H, scale, bt->attn_ws, bt->attn_ws_bytes, p->err_dev, s);
 }
 
 // One batched step reading tokens and positions from bt->req; greedy steps
@@ -1439,7 +1463,7 @@ static int batch_set(Batch *bt, const uint32_t *tokens, const uint32_t *position
 
 // A batch of `batch` sequences with their own caches, or (chunk) a prompt
 // chunker of up to `batch` consecutive positions of the plan's own sequence.
-static Batch *batch_create(Plan *p, unsigned batch, bool chunk, const fyb_kv8_cache *paged)
+static Batch *batch_create(Plan *p, unsigned batch, bool chunk, const fyb_kv8_cache *paged, bool four)
 {
     if (!p || p->failed || batch < 1 || batch > BATCH_MAX || p->tp_size != 1 || p->hd % 16 || p->ffn % 8 ||
         p->d % 4)
@@ -1466,8 +1490,9 @@ static Batch *batch_create(Plan *p, unsigned batch, bool chunk, const fyb_kv8_ca
         bt->kc = p->kcache; bt->vc = p->vcache;
     } else if (paged) {
         bt->paged = true;
+        bt->four = four;
         bt->cache = *paged;
-        const size_t scales = (size_t)p->nl * paged->blocks * p->Hkv, bytes = scales * paged->block_size * p->hd;
+        const size_t scales = p->nl * batch_layer_scales(*paged, four), bytes = p->nl * batch_layer_bytes(*paged, four);
         bt->cache.k = A(bytes); bt->cache.v = A(bytes);
         bt->cache.k_scale = (float *)A(scales * 4); bt->cache.v_scale = (float *)A(scales * 4);
         bt->table_stride = (unsigned)((bt->capacity + paged->block_size - 1) / paged->block_size);
@@ -1505,9 +1530,18 @@ static Batch *batch_create(Plan *p, unsigned batch, bool chunk, const fyb_kv8_ca
     bt->splits = (unsigned)std::max<size_t>(4, std::min<size_t>(16, ((size_t)4 * p->ctx->sms + seqs * p->Hkv - 1) /
                                                                         (seqs * p->Hkv)));
     if (ok) {
-        bt->attn_ws_bytes = paged ? fyb_kv8_attention_workspace(batch, 1, p->H, p->Hkv, p->hd)
+        bt->attn_ws_bytes = four ? fyb_kv4_attention_workspace(batch, 1, p->H, p->Hkv, p->hd)
+                            : paged ? fyb_kv8_attention_workspace(batch, 1, p->H, p->Hkv, p->hd)
                                   : attention_workspace_bytes(batch_attention(bt, 0));
         bt->attn_ws = A(bt->attn_ws_bytes);
+    }
+    if (ok && !chunk) {
+        bt->score_ws_bytes = fyb_logprobs_workspace(batch, p->V, FYB_LOGPROBS_TOP);
+        bt->targets = (int32_t *)A(batch * 4); bt->rank = (int32_t *)A(batch * 4);
+        bt->logprob = (float *)A(batch * 4); bt->entropy = (float *)A(batch * 4);
+        bt->top_tokens = (int32_t *)A(batch * FYB_LOGPROBS_TOP * 4); bt->top_logprobs = (float *)A(batch * FYB_LOGPROBS_TOP * 4);
+        bt->score_ws = A(bt->score_ws_bytes);
+        if (ok) ok = cudaMemset(bt->score_ws, 0, bt->score_ws_bytes) == cudaSuccess;
     }
     if (ok) ok = (chunk || paged || (cudaMemset(bt->kc, 0, kv * 2) == cudaSuccess && cudaMemset(bt->vc, 0, kv * 2) == cudaSuccess)) &&
                  cudaMemset(bt->attn_ws, 0, bt->attn_ws_bytes) == cudaSuccess &&
@@ -1531,6 +1565,17 @@ extern "C" void *fyb_batch_create_kv8(void *plan, unsigned batch, uint32_t block
     fyb_kv8_cache c = {};
     c.blocks = blocks; c.kv_heads = p->Hkv; c.block_size = block_size; c.head_dim = p->hd; c.format = format;
     return batch_create((Plan *)plan, batch, false, &c);
+}
+
+extern "C" void *fyb_batch_create_kv4(void *plan, unsigned batch, uint32_t blocks, uint32_t block_size)
+{
+    const Plan *p = (const Plan *)plan;
+    if (!p || blocks == 0 || block_size < 16 || block_size > 256 || (block_size & (block_size - 1)) ||
+        (p->hd != 64 && p->hd != 128) || (unsigned long long)blocks * p->Hkv * block_size > 0x7fffffffull)
+        return nullptr;
+    fyb_kv8_cache c = {};
+    c.blocks = blocks; c.kv_heads = p->Hkv; c.block_size = block_size; c.head_dim = p->hd;
+    return batch_create((Plan *)plan, batch, false, &c, true);
 }
 
 extern "C" long fyb_batch_free_blocks(const void *batch)
@@ -1630,6 +1675,38 @@ extern "C" int fyb_batch_step(void *batch, const uint32_t *tokens, const uint32_
     if (argmax && cudaMemcpyAsync(argmax, bt->tokens, (size_t)bt->B * 4, cudaMemcpyDeviceToHost, s) != cudaSuccess)
         return -2;
     if (cudaStreamSynchronize(s) != cudaSuccess || *(volatile unsigned *)bt->p->err_host) return -2;
+    return 0;
+}
+
+// One step whose logits stay on the device: of each sequence the log probability and rank of targets[b], the entropy and
+// the `top` most probable tokens.
+extern "C" int fyb_batch_score(void *batch, const uint32_t *tokens, const uint32_t *positions, const int32_t *targets,
+    float *logprob, int32_t *rank, float *entropy, uint32_t top, int32_t *top_tokens, float *top_logprobs)
+{
+    Batch *bt = (Batch *)batch;
+    if (!bt || !tokens || !positions || bt->p->failed || top > FYB_LOGPROBS_TOP || ((logprob || rank) && !targets) ||
+        (top && (!top_tokens || !top_logprobs)))
+        return -1;
+    const unsigned B = bt->B, V = bt->p->V;
+    for (unsigned b = 0; targets && b < B; ++b) if (targets[b] >= (int64_t)V) return -1;
+    DeviceScope scope(bt->p->ctx->device);
+    if (!scope.ok) return -1;
+    cudaStream_t s = bt->p->ctx->stream;
+    int r = batch_set(bt, tokens, positions, 1);
+    if (r) return r;
+    if ((r = batch_run(bt, false)) != 0) return r;
+    if (targets && cudaMemcpyAsync(bt->targets, targets, B * 4, cudaMemcpyHostToDevice, s) != cudaSuccess) return -2;
+    r = fyb_logprobs(T_F32, bt->logits, V, B, V, targets ? bt->targets : nullptr, targets ? bt->logprob : nullptr,
+                     rank ? bt->rank : nullptr, bt->entropy, top, bt->top_tokens, bt->top_logprobs, bt->score_ws,
+                     bt->score_ws_bytes, bt->p->err_dev, s);
+    if (r) return r;
+    auto give = [&](void *to, const void *from, size_t words) {
+        return !to || !words || cudaMemcpyAsync(to, from, words * 4, cudaMemcpyDeviceToHost, s) == cudaSuccess;
+    };
+    if (!give(logprob, bt->logprob, B) || !give(rank, bt->rank, B) || !give(entropy, bt->entropy, B) ||
+        !give(top_tokens, bt->top_tokens, (size_t)B * top) || !give(top_logprobs, bt->top_logprobs, (size_t)B * top) ||
+        cudaStreamSynchronize(s) != cudaSuccess || *(volatile unsigned *)bt->p->err_host)
+        return -2;
     return 0;
 }
 

@@ -227,10 +227,21 @@ void *fyb_batch_create(void *plan, unsigned batch);
    blocks past it back first. A step, or a run of greedy steps, that needs more
    blocks than there are is refused (-1) before anything is launched. */
 void *fyb_batch_create_kv8(void *plan, unsigned batch, uint32_t blocks, uint32_t block_size, uint32_t format);
+/* The same over a paged 4-bit cache (fyb_kv4_append, fyb_kv4_attention; head
+   dimension 64 or 128): 0.56 of its bytes. */
+void *fyb_batch_create_kv4(void *plan, unsigned batch, uint32_t blocks, uint32_t block_size);
 /* Blocks of a paged batch that no sequence holds (-1 for other batches). */
 long fyb_batch_free_blocks(const void *batch);
 void fyb_batch_free(void *batch);
 int fyb_batch_step(void *batch, const uint32_t *tokens, const uint32_t *positions, float *logits, uint32_t *argmax);
+/* fyb_batch_step whose logits stay on the device (raw, no suppressed ids): of
+   each sequence b the log probability and rank of targets[b] (the token that
+   follows tokens[b] in a text; negative: none), the entropy, and the top (0..32)
+   most probable tokens, as fyb_logprobs gives them (host arrays [B], [B][top]).
+   targets, logprob, rank and entropy may be NULL, logprob and rank need targets.
+   What scores a text, or a cache of fewer bits by what it costs. */
+int fyb_batch_score(void *batch, const uint32_t *tokens, const uint32_t *positions, const int32_t *targets,
+    float *logprob, int32_t *rank, float *entropy, uint32_t top, int32_t *top_tokens, float *top_logprobs);
 int fyb_batch_decode_greedy(void *batch, const uint32_t *tokens, const uint32_t *positions, size_t steps,
     uint32_t *out);
 double fyb_batch_time_greedy(void *batch, const uint32_t *tokens, const uint32_t *positions, size_t steps);

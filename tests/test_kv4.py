@@ -112,3 +112,8 @@ def test_wrappers_refuse_host_tensors():
     x = torch.zeros((2, 7))
     with pytest.raises(ValueError):
         F.logprobs(x, None, None, None, None, None, None, torch.zeros(256, dtype=torch.uint8))
+
+
+def test_batch_refuses():
+    assert not F.lib.fyb_batch_create_kv4(None, 4, 16, 32)
+    assert F.lib.fyb_batch_score(None, P, P, P, P, P, P, 0, None, None) == -1
