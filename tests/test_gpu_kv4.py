@@ -296,7 +296,7 @@ def reference(cache, table, lengths, starts, q, scale, kind):
     q = q.cpu().double()
     rows, heads, _ = q.shape
     out, tol = torch.zeros(rows, heads, hd, dtype=torch.float64), torch.zeros(rows, heads, 1, dtype=torch.float64)
-    wide = kind == "f32"
+    wide, peak = kind == "f32", 0.0
     for r, n in enumerate(lengths):
         use = table[r, :-(-n // size)].tolist()
         if not use:
@@ -309,6 +309,7 @@ def reference(cache, table, lengths, starts, q, scale, kind):
                 continue
             row = q[starts[r] + j].reshape(kv, heads // kv, hd)
             sc = torch.einsum("ghd,gtd->ght", row, kk[:, :end]) * scale
+            peak = max(peak, float(sc.abs().amax()))
             mag = torch.einsum("ghd,gtd->ght", row.abs(), km[:, :end]).amax(2) * abs(scale)
             p = torch.softmax(sc, 2)
             out[starts[r] + j] = torch.einsum("ght,gtd->ghd", p, vv[:, :end]).reshape(heads, hd)
@@ -318,7 +319,7 @@ def reference(cache, table, lengths, starts, q, scale, kind):
                 e = e + row.abs().sum(2) * abs(scale) * 2.0 ** -25
             bound = top * (2 * e + (end + 16) * 2.0 ** -23 + (0 if wide else 3 * 2.0 ** -11)) + (0 if wide else 2.0 ** -25)
             tol[starts[r] + j] = bound.reshape(heads, 1)
-    return out, tol
+    return out, tol, peak
 
 
 def run_attention(lengths, new, heads, kv, hd, size, kind, seed=0, scale=None, q=None, change=None, stride=0):
@@ -341,13 +342,15 @@ def run_attention(lengths, new, heads, kv, hd, size, kind, seed=0, scale=None, q
     cache.attention(q, i32(lengths), i32(table), again, ws, **args)  # the workspace is left as it has to be
     assert err.item() == 0
     assert torch.equal(out.view(torch.uint8), again.view(torch.uint8))
-    want, tol = reference(cache, table, lengths, starts, q, scale, kind)
+    want, tol, peak = reference(cache, table, lengths, starts, q, scale, kind)
     got = out.cpu().double()
     assert got.isfinite().all()
     far = (got - want).abs() - tol - want.abs() * HALF_UNIT[kind] - 2.0 ** -25
     assert (far <= 0).all(), float(far.max())
-    if want.norm() > 0:  # and in the mean far nearer than the worst case
-        assert (got - want).norm() <= (2e-5 if kind == "f32" else 1e-2) * want.norm()
+    # and in the mean far nearer than the worst case. A score s in 32 bits is off by up to 2^-24 |s|, its weight by as much
+    # of itself; weights and their sum together move an output by up to twice that of the values' size: 2^-23 |s|
+    if want.norm() > 0:
+        assert (got - want).norm() <= ((2e-5 if kind == "f32" else 1e-2) + 2.0 ** -23 * peak) * want.norm()
     return out
 
 
@@ -624,7 +627,7 @@ def test_steps_together():
         q, out = torch.empty(rows, heads, hd, device="cuda"), torch.empty(rows, heads, hd, device="cuda")
         cache.append(y[:, heads:heads + kv], y[:, heads + kv:], slots, pos, cos, sin, "interleaved", y[:, :heads], q)
         cache.attention(q, lengths, table, out, ws[max(new)], row_start=start, most_rows=max(new))
-        want, tol = reference(cache, table.cpu().numpy(), lengths.tolist(), start.tolist(), q, hd ** -0.5, "f32")
+        want, tol, _ = reference(cache, table.cpu().numpy(), lengths.tolist(), start.tolist(), q, hd ** -0.5, "f32")
         assert ((out.cpu().double() - want).abs() <= tol + want.abs() * 2.0 ** -24 + 2.0 ** -25).all(), step
     F.kv_release(lengths, i32([0, 999, -1]), table, free, count, size)
     assert lengths.tolist()[0] == 0 and count.item() == 40 - -(-lengths.tolist()[1] // size)
