@@ -54,7 +54,7 @@ template <int NR> struct K4tShared {
     Kv8Segment seg[SEGS], walked[k4t_threads(NR) / 32];
     Kv8Place place;
     uint64_t seg_full[SEGS], seg_empty[SEGS], rk_full[4], rk_empty[4], rv_full[4], rv_empty[4], k_full[2], k_empty[2],
-        v_full[2], v_empty[2], s_full[2], p_full[2], o_done[2], o_free[2], q_full[SEGS], q_empty, meta_full[K4T_META], drained;
+        v_full[2], v_empty[2], s_full[2], p_full[4], o_done[4], o_free[2], q_full[SEGS], q_empty, meta_full[K4T_META], drained;
     float factor[SEGS][k4t_groups(NR) * 128];  // score factor of each lane's row
     float2 ml[NR < 256 ? 128 : 1];
     unsigned here[K4T_META];                       // which groups of 16 positions of a tile are loaded
@@ -103,13 +103,75 @@ FYB_DEV void k4t_load8(const Kv4Attention &A, size_t at, float4 &a, float4 &b)
     }
 }
 
+// The CTA's partial (of `rows` rows) is written: the last CTA of the segment joins them all in order, head_dim / 4 lanes
+// a row. L2's latency is what takes time: four parts of two rows are on their way at once, their weights too.
+template <int NR, int HD, int THREADS, typename Bar, typename Put>
+FYB_DEV void k4t_join(const Kv4Attention &A, const Kv8Parts &of, unsigned tid, unsigned rows, unsigned *flag, Bar bar, Put put)
+{
+    constexpr unsigned LANES = HD / 4, STEP = THREADS / LANES, ROWS = 2, PARTS = 4;
+    __threadfence();
+    bar();
+    if (tid == 0) *flag = atomicAdd(&A.counters[of.first], 1u) == of.last - of.first;
+    bar();
+    if (!*flag) return;
+    __threadfence();
+    if (tid == 0) A.counters[of.first] = 0;
+    const unsigned parts = of.last - of.first + 1, piece = tid % LANES;
+#pragma unroll 1
+    for (unsigned row = tid / LANES; row < rows; row += ROWS * STEP) {
+        float4 v[ROWS];
+        float m[ROWS], l[ROWS];
+#pragma unroll
+        for (unsigned u = 0; u < ROWS; ++u) { v[u] = make_float4(0.f, 0.f, 0.f, 0.f); m[u] = -3.4e38f; l[u] = 0.f; }
+#pragma unroll 1
+        for (unsigned p = 0; p < parts; p += PARTS) {
+            float4 x[ROWS][PARTS];
+            float2 ml[ROWS][PARTS];
+#pragma unroll
+            for (unsigned u = 0; u < ROWS; ++u)
+#pragma unroll
+                for (unsigned i = 0; i < PARTS; ++i) {
+                    x[u][i] = make_float4(0.f, 0.f, 0.f, 0.f);
+                    ml[u][i] = make_float2(-3.4e38f, 0.f);
+                    if (p + i < parts && row + u * STEP < rows) {
+                        const size_t at = (size_t)(2 * (of.first + p + i) + (p + i == 0 ? 1 : 0)) * NR + row + u * STEP;
+                        x[u][i] = __ldcg(reinterpret_cast<const float4 *>(A.part_o + at * HD) + piece);
+                        ml[u][i] = __ldcg(A.part_ml + at);
+                    }
+                }
+#pragma unroll
+            for (unsigned u = 0; u < ROWS; ++u) {
+                float top = m[u];
+#pragma unroll
+                for (unsigned i = 0; i < PARTS; ++i) top = fmaxf(top, ml[u][i].x);
+                const float old = ex2(m[u] - top);
+                m[u] = top;
+                l[u] *= old;
+                v[u].x *= old; v[u].y *= old; v[u].z *= old; v[u].w *= old;
+#pragma unroll
+                for (unsigned i = 0; i < PARTS; ++i) {
+                    const float w = ex2(ml[u][i].x - top);
+                    l[u] = fmaf(w, ml[u][i].y, l[u]);
+                    v[u].x = fmaf(w, x[u][i].x, v[u].x); v[u].y = fmaf(w, x[u][i].y, v[u].y);
+                    v[u].z = fmaf(w, x[u][i].z, v[u].z); v[u].w = fmaf(w, x[u][i].w, v[u].w);
+                }
+            }
+        }
+#pragma unroll
+        for (unsigned u = 0; u < ROWS; ++u) {
+            const float n = l[u] > 0.f || isnan(l[u]) ? 1.f / l[u] : 0.f;
+            if (row + u * STEP < rows) put(row + u * STEP, piece, make_float4(v[u].x * n, v[u].y * n, v[u].z * n, v[u].w * n));
+        }
+    }
+}
+
 template <int HD, int NR>
 __global__ void __launch_bounds__(k4t_threads(NR), 1) kv4_tiles_kernel(const __grid_constant__ Kv4Attention A, const __grid_constant__ CUtensorMap kmap,
     const __grid_constant__ CUtensorMap vmap)
 {
     using S = K4tShape<HD, NR>;
     constexpr unsigned GROUPS = k4t_groups(NR), SOFT = 4 * GROUPS, W_CONV = SOFT, W_TMA = SOFT + 2 * K4T_CONV, W_MMA = W_TMA + 2;
-    constexpr unsigned CP = GROUPS == 2 ? 1 : 128 / NR, CW = 128 / CP, CHUNKS = CW / 32;   // copies, and the positions and blocks of 32 of a copy
+    constexpr unsigned CP = GROUPS == 2 ? 1 : 128 / NR, HALVES = GROUPS, CW = 128 / CP / HALVES, CHUNKS = CW / 32;   // copies, and the positions and blocks of 32 taken at a time
     constexpr unsigned SEGS = k4t_segs(NR);
     constexpr int G64 = HD / 64;
     extern __shared__ unsigned char k4t_smem[];
@@ -124,9 +186,9 @@ __global__ void __launch_bounds__(k4t_threads(NR), 1) kv4_tiles_kernel(const __g
         for (int i = 0; i < 2; ++i) {
             mbar_init(sh.k_full + i, K4T_CONV); mbar_init(sh.k_empty + i, 1);
             mbar_init(sh.v_full + i, K4T_CONV); mbar_init(sh.v_empty + i, 1);
-            mbar_init(sh.s_full + i, 1); mbar_init(sh.p_full + i, 4);
-            mbar_init(sh.o_done + i, 1); mbar_init(sh.o_free + i, 4);
+            mbar_init(sh.s_full + i, 1); mbar_init(sh.o_free + i, 4);
         }
+        for (int i = 0; i < 4; ++i) { mbar_init(sh.p_full + i, 4); mbar_init(sh.o_done + i, 1); }
         mbar_init(&sh.q_empty, 1); mbar_init(&sh.drained, 1);
         for (int i = 0; i < K4T_META; ++i) mbar_init(sh.meta_full + i, 1);
         for (unsigned i = 0; i < SEGS; ++i) {
@@ -190,99 +252,93 @@ __global__ void __launch_bounds__(k4t_threads(NR), 1) kv4_tiles_kernel(const __g
             const unsigned tiles = (unsigned)(t1 - t0);
             if (!mine) n += tiles;
             for (int t = t0; mine && t < t1; ++t, ++n, ++k) {
-                // S of a tile: the group's, or the tile's of two; what it waits for has come k, or k / 2, times before
-                const unsigned b = GROUPS == 2 ? wg : k & 1, turn = GROUPS == 2 ? k : k >> 1;
                 wait(sh.meta_full + n % K4T_META, n / K4T_META);
                 const unsigned here = sh.here[n % K4T_META];
-                wait(sh.s_full + b, turn);
-                kt_fence_after();
-                const uint32_t s_at = tmem + lanes + b * 128 + first, p_at = tmem + lanes + b * 128 + S::P;
-                if (__builtin_expect(here != 0xffu || (t + 1) * K4_TILE > all, 0)) {
-                    // what the row does not attend becomes -inf where it lies: the rest has one form, and fits the
-                    // instruction cache with the other roles
 #pragma unroll 1
-                    for (unsigned c = 0; c < CW; c += 16) {
-                        float y[16];
-                        kt_ld16(s_at + c, y);
-                        kt_wait_ld();
-                        const int left = here >> ((first + c) / 16) & 1 ? limit - (t * K4_TILE + (int)(first + c)) : 0;
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) y[i] = i < left ? y[i] : -INFINITY;
-                        kt_st16(s_at + c, y);
-                    }
-                    kt_wait_st();
-                }
-                constexpr unsigned KEEP = CHUNKS < 2 ? CHUNKS : 2;  // blocks that stay in registers between the two looks at them
-                float x[KEEP][32], tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-                for (unsigned c = 0; c < CHUNKS; c += KEEP) {
-#pragma unroll
-                    for (unsigned k = 0; k < KEEP; ++k) kt_ld32(s_at + 32 * (c + k), x[k]);
-                    kt_wait_ld();
-#pragma unroll
-                    for (unsigned k = 0; k < KEEP; ++k)
-#pragma unroll
-                        for (int i = 0; i < 32; i += 2) tops[i / 2 % 4] = fmaxf(tops[i / 2 % 4], fmaxf(x[k][i], x[k][i + 1]));
-                }
-                const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])) * f;
-                const bool up = top - m > 8.f + P_UP;
-                if (__any_sync(0xffffffffu, up)) {
-                    // ---- new maxima, and the sums so far in their units
-                    const float now = up ? top - P_UP : m, alpha = up ? ex2(m - now) : 1.f;
-                    m = now;
-                    l *= alpha;
-                    if (t > t0) {
-                        if (GROUPS == 2) wait(sh.o_done + b, k - 1); else wait(sh.o_done + (b ^ 1), (k - 1) >> 1);
+                for (unsigned h = 0; h < HALVES; ++h) {
+                    // S: the group's, or the tile's of two, its weights (P); what it waits for has come k, or k / 2, times before
+                    const unsigned b = GROUPS == 2 ? 2 * wg + h : k & 1, turn = GROUPS == 2 ? k : k >> 1;
+                    const unsigned from = GROUPS == 2 ? 64 * h : first;  // first position in the tile
+                    const unsigned of = GROUPS == 2 ? wg : b;
+                    if (h == 0) {
+                        wait(sh.s_full + of, turn);
                         kt_fence_after();
+                    }
+                    const uint32_t s_of = tmem + lanes + of * 128, s_at = s_of + from, p_at = s_of + (GROUPS == 2 ? from + 32 : S::P);
+                    if (__builtin_expect(here != 0xffu || (t + 1) * K4_TILE > all, 0)) {
+                        // what the row does not attend becomes -inf where it lies: the rest has one form, and fits the
+                        // instruction cache with the other roles
 #pragma unroll 1
-                        for (int c = 0; c < HD; c += 16) {
+                        for (unsigned c = 0; c < CW; c += 16) {
                             float y[16];
-                            kt_ld16(o_at + c, y);
+                            kt_ld16(s_at + c, y);
                             kt_wait_ld();
+                            const int left = here >> ((from + c) / 16) & 1 ? limit - (t * K4_TILE + (int)(from + c)) : 0;
 #pragma unroll
-                            for (int i = 0; i < 16; ++i) y[i] *= alpha;
-                            kt_st16(o_at + c, y);
+                            for (int i = 0; i < 16; ++i) y[i] = i < left ? y[i] : -INFINITY;
+                            kt_st16(s_at + c, y);
                         }
                         kt_wait_st();
                     }
-                }
-                // ---- weights, blocks from the last to the first: P takes the place of scores that have been read
-                const F2 f2x = f2(f, f), mx = f2(-m, -m);
-                F2 sums[2] = {f2(0.f, 0.f), f2(0.f, 0.f)};
-                auto weights = [&](float (&y)[32], unsigned c) {
-                    unsigned w[16];
+                    float x[CHUNKS][32], tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                    for (int i = 0; i < 32; i += 2) {
-                        const float2 e = f2_get(f2_fma(f2(y[i], y[i + 1]), f2x, mx));
-                        const float p0 = ex2(e.x), p1 = ex2(e.y);
-                        sums[i / 2 % 2] = f2_add(sums[i / 2 % 2], f2(p0, p1));
-                        w[i / 2] = kt_pack(p0, p1);
+                    for (unsigned c = 0; c < CHUNKS; ++c) kt_ld32(s_at + 32 * c, x[c]);
+                    kt_wait_ld();
+#pragma unroll
+                    for (unsigned c = 0; c < CHUNKS; ++c)
+#pragma unroll
+                        for (int i = 0; i < 32; i += 2) tops[i / 2 % 4] = fmaxf(tops[i / 2 % 4], fmaxf(x[c][i], x[c][i + 1]));
+                    const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])) * f;
+                    const bool up = top - m > 8.f + P_UP;
+                    if (__any_sync(0xffffffffu, up)) {
+                        // ---- new maxima, and the sums so far in their units
+                        const float now = up ? top - P_UP : m, alpha = up ? ex2(m - now) : 1.f;
+                        m = now;
+                        l *= alpha;
+                        if (t > t0 || h) {
+                            if (GROUPS == 2) wait(sh.o_done + (b ^ 1), h ? k : k - 1); else wait(sh.o_done + (b ^ 1), (k - 1) >> 1);
+                            kt_fence_after();
+#pragma unroll 1
+                            for (int c = 0; c < HD; c += 16) {
+                                float y[16];
+                                kt_ld16(o_at + c, y);
+                                kt_wait_ld();
+#pragma unroll
+                                for (int i = 0; i < 16; ++i) y[i] *= alpha;
+                                kt_st16(o_at + c, y);
+                            }
+                            kt_wait_st();
+                        }
                     }
-                    kt_st16(p_at + first / 2 + 16 * c, reinterpret_cast<const float *>(w));
-                };
-                if constexpr (CP > 1) {  // 0 for the positions of the other copies
-                    float z[16];
+                    // ---- weights: P takes the place of scores that have been read
+                    const F2 f2x = f2(f, f), mx = f2(-m, -m);
+                    F2 sums[2] = {f2(0.f, 0.f), f2(0.f, 0.f)};
+                    if constexpr (CP > 1) {  // 0 for the positions of the other copies
+                        float z[16];
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) z[i] = 0.f;
+                        for (int i = 0; i < 16; ++i) z[i] = 0.f;
 #pragma unroll
-                    for (unsigned c = 0; c < 64; c += 16)
-                        if (c < first / 2 || c >= (first + CW) / 2) kt_st16(p_at + c, z);
-                }
-#pragma unroll
-                for (unsigned c = CHUNKS; c; c -= KEEP) {
-                    if (c != CHUNKS) {
-#pragma unroll
-                        for (unsigned k = 0; k < KEEP; ++k) kt_ld32(s_at + 32 * (c - KEEP + k), x[k]);
-                        kt_wait_ld();
+                        for (unsigned c = 0; c < 64; c += 16)
+                            if (c < first / 2 || c >= (first + CW) / 2) kt_st16(p_at + c, z);
                     }
 #pragma unroll
-                    for (unsigned k = KEEP; k; --k) weights(x[k - 1], c - KEEP + k - 1);
+                    for (unsigned c = 0; c < CHUNKS; ++c) {
+                        unsigned w[16];
+#pragma unroll
+                        for (int i = 0; i < 32; i += 2) {
+                            const float2 e = f2_get(f2_fma(f2(x[c][i], x[c][i + 1]), f2x, mx));
+                            const float p0 = ex2(e.x), p1 = ex2(e.y);
+                            sums[i / 2 % 2] = f2_add(sums[i / 2 % 2], f2(p0, p1));
+                            w[i / 2] = kt_pack(p0, p1);
+                        }
+                        kt_st16(p_at + first / 2 + 16 * c, reinterpret_cast<const float *>(w));
+                    }
+                    const float2 l2 = f2_get(f2_add(sums[0], sums[1]));
+                    l += l2.x + l2.y;
+                    kt_wait_st();
+                    kt_fence_before();
+                    arrive(sh.p_full + b);
                 }
-                const float2 l2 = f2_get(f2_add(sums[0], sums[1]));
-                l += l2.x + l2.y;
-                kt_wait_st();
-                kt_fence_before();
-                arrive(sh.p_full + b);
             }
             // ---- the segment's part
             const bool whole = s.t0 == 0 && s.t1 == s.tiles;
@@ -314,7 +370,7 @@ __global__ void __launch_bounds__(k4t_threads(NR), 1) kv4_tiles_kernel(const __g
             };
             if constexpr (GROUPS == 2) {
                 if (mine) {
-                    wait(sh.o_done + wg, k - 1);
+                    wait(sh.o_done + 2 * wg + 1, k - 1);
                     kt_fence_after();
                     const float own = !whole ? 1.f : l > 0.f || isnan(l) ? 1.f / l : 0.f;
                     const bool real = (int)rho < nrows;
@@ -384,7 +440,7 @@ __global__ void __launch_bounds__(k4t_threads(NR), 1) kv4_tiles_kernel(const __g
                 arrive(sh.o_free);
             }
             if (!whole) {
-                kv8_arrive<NR, HD, 32 * SOFT, 4>(A, of, tid, (unsigned)nrows, stage, S::STAGED, &sh.flag, bar, put);
+                k4t_join<NR, HD, 32 * SOFT>(A, of, tid, (unsigned)nrows, &sh.flag, bar, put);
                 bar();
             }
             done();
@@ -603,42 +659,48 @@ __global__ void __launch_bounds__(k4t_threads(NR), 1) kv4_tiles_kernel(const __g
         const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
         const uint64_t qs = kt_desc(smem_u32(ring + S::OFF_Q), 16), ks = kt_desc(smem_u32(ring + S::OFF_K), 16),
                        vs = kt_desc(smem_u32(ring + S::OFF_V), S::HALF);
-        // what has been asked for so far: scores and values (tiles; each group's), segments of a group
-        unsigned ns = 0, scored[2] = {0, 0}, valued[2] = {0, 0}, segs[2] = {0, 0};
-        auto scores = [&](unsigned g, bool last_group, bool last) {
-            const unsigned b = GROUPS == 2 ? g : ns & 1, turn = GROUPS == 2 ? scored[g] : ns >> 1;
-            if (turn) wait(sh.o_done + b, turn - 1);  // P in this S has been read
+        // what has been asked for so far: scores and values of each group (tiles), segments of a group
+        unsigned scored[2] = {0, 0}, valued[2] = {0, 0}, segs[2] = {0, 0};
+        // scores of tile t of the segment
+        auto ask = [&](unsigned g, int t, bool last_group, bool last) {
+            const unsigned tile = n + (unsigned)t, b = GROUPS == 2 ? g : tile & 1, turn = GROUPS == 2 ? scored[g] : tile >> 1;
+            if (g == 0) wait(sh.k_full + (tile & 1), tile >> 1);
+            if (turn) wait(sh.o_done + (GROUPS == 2 ? 2 * g + 1 : b), turn - 1);  // P in this S has been read
             kt_fence_after();
             __syncwarp();
             if (kt_elect()) {
 #pragma unroll
                 for (int k = 0; k < HD / 16; ++k) {
-                    const uint64_t step = (uint64_t)((k / 4 * S::HALF + k % 4 * 32) >> 4), kt = ks + ((ns & 1) * S::TILE >> 4) + step;
+                    const uint64_t step = (uint64_t)((k / 4 * S::HALF + k % 4 * 32) >> 4), kt = ks + ((tile & 1) * S::TILE >> 4) + step;
                     if constexpr (S::Q_TM) kt_mma(tm + b * 128, tm + S::Q + 8 * k, kt, kt_idesc(128, false), k > 0);
                     else kt_mma_ss(tm + b * 128, qs + (g * S::TILE >> 4) + step, kt, kt_idesc(128, false), k > 0);
                 }
-                if (last_group) kt_commit(sh.k_empty + (ns & 1));
+                if (last_group) kt_commit(sh.k_empty + (tile & 1));
                 kt_commit(sh.s_full + b);
                 if (last_group && last) kt_commit(&sh.q_empty);
             }
             __syncwarp();
             ++scored[g];
         };
-        auto values = [&](unsigned g, bool last_group, bool first) {
-            const unsigned b = GROUPS == 2 ? g : n & 1, turn = GROUPS == 2 ? valued[g] : n >> 1;
+        // values of it, or of its half h for one of two groups
+        auto give = [&](unsigned g, unsigned h, int t, bool last_group) {
+            const unsigned tile = n + (unsigned)t, b = GROUPS == 2 ? 2 * g + h : tile & 1, turn = GROUPS == 2 ? valued[g] : tile >> 1;
+            const bool first = t == 0 && h == 0;
+            if (g == 0 && h == 0) wait(sh.v_full + (tile & 1), tile >> 1);
             wait(sh.p_full + b, turn);
             if (first && segs[g]) wait(sh.o_free + g, segs[g] - 1);
             kt_fence_after();
             __syncwarp();
             if (kt_elect()) {
+                const uint32_t from = tm + (GROUPS == 2 ? g * 128 + h * 64 + 32 : b * 128 + S::P);
 #pragma unroll
-                for (int k = 0; k < K4_TILE / 16; ++k)
-                    kt_mma(tm + S::O + g * HD, tm + b * 128 + S::P + 8 * k, vs + (((n & 1) * S::TILE + k * 2048) >> 4), kt_idesc(HD, true), !first || k);
-                if (last_group) kt_commit(sh.v_empty + (n & 1));
+                for (int k = 0; k < K4_TILE / 16 / (int)HALVES; ++k)
+                    kt_mma(tm + S::O + g * HD, from + 8 * k, vs + (((tile & 1) * S::TILE + h * 8192 + k * 2048) >> 4), kt_idesc(HD, true), !first || k);
+                if (last_group && h + 1 == HALVES) kt_commit(sh.v_empty + (tile & 1));
                 kt_commit(sh.o_done + b);
             }
             __syncwarp();
-            ++valued[g];
+            if (h + 1 == HALVES) ++valued[g];
             if (first) ++segs[g];
         };
         while (const Kv8Segment *s = next()) {
@@ -646,33 +708,33 @@ __global__ void __launch_bounds__(k4t_threads(NR), 1) kv4_tiles_kernel(const __g
             const int tiles = s->t1 - s->t0;
             const int nrows = min((int)A.row_tile, s->q.rows - s->row_tile * (int)A.row_tile) * (int)GR;
             const bool two = GROUPS == 2 && nrows > 128;
-            auto ask = [&](unsigned g, int t) {
-                if (g == 0) wait(sh.k_full + (ns & 1), ns >> 1);
-                const bool last_group = g || !two;
-                scores(g, last_group, t + 1 == tiles);
-                if (last_group) ++ns;
-            };
-            auto give = [&](unsigned g, int t) {
-                if (g == 0) wait(sh.v_full + (n & 1), n >> 1);
-                const bool last_group = g || !two;
-                values(g, last_group, t == 0);
-                if (last_group) ++n;
-            };
-            // one group: scores a tile ahead of values. Two: P takes the place of a group's scores, so its next come after,
-            // and the other group's weights are made meanwhile
-            ask(0, 0);
-            if (two) ask(1, 0);
+            if constexpr (GROUPS == 1) {
+                // scores a tile ahead of values
+                ask(0, 0, true, tiles == 1);
 #pragma unroll 1
-            for (int t = 0; t < tiles; ++t) {
-                const bool more = t + 1 < tiles;
-                if (GROUPS == 1 && more) ask(0, t + 1);
-                give(0, t);
-                if (GROUPS == 2 && more) ask(0, t + 1);
-                if (two) {
-                    give(1, t);
-                    if (more) ask(1, t + 1);
+                for (int t = 0; t < tiles; ++t) {
+                    if (t + 1 < tiles) ask(0, t + 1, true, t + 2 == tiles);
+                    give(0, 0, t, true);
                 }
+            } else {
+                // P takes the place of scores, so a group's next scores come after all its values; the other group is half a
+                // tile behind, so one's products run while the other's weights are made
+                ask(0, 0, !two, tiles == 1);
+                if (two) ask(1, 0, true, tiles == 1);
+#pragma unroll 1
+                for (int t = 0; t < tiles; ++t) {
+                    give(0, 0, t, !two);
+                    if (two && t) {
+                        give(1, 1, t - 1, true);
+                        ask(1, t, true, t + 1 == tiles);
+                    }
+                    give(0, 1, t, !two);
+                    if (t + 1 < tiles) ask(0, t + 1, !two, t + 2 == tiles);
+                    if (two) give(1, 0, t, true);
+                }
+                if (two) give(1, 1, tiles - 1, true);
             }
+            n += (unsigned)tiles;
             done();
         }
         if (kt_elect()) {
