@@ -103,12 +103,18 @@ FYB_DEV void k4t_load8(const Kv4Attention &A, size_t at, float4 &a, float4 &b)
     }
 }
 
-// The CTA's partial (of `rows` rows) is written: the last CTA of the segment joins them all in order, head_dim / 4 lanes
-// a row. L2's latency is what takes time: four parts of two rows are on their way at once, their weights too.
+// Partials lie as [4 columns][row]: a warp's rows, a lane each, are written and read side by side (as rows of head_dim
+// values each 16 bytes were a sector of their own: a prompt's partial took 12000 to 20000 cycles to be seen, its join 45000).
+template <int NR, int HD> FYB_DEV size_t k4t_part(unsigned slot, unsigned piece, unsigned row)
+{
+    return ((size_t)slot * (HD / 4) + piece) * NR + row;
+}
+// The CTA's partial (of `rows` rows) is written: the last CTA of the segment joins them all in order. L2's latency is what
+// takes time: four parts of four pieces are on their way at once.
 template <int NR, int HD, int THREADS, typename Bar, typename Put>
 FYB_DEV void k4t_join(const Kv4Attention &A, const Kv8Parts &of, unsigned tid, unsigned rows, unsigned *flag, Bar bar, Put put)
 {
-    constexpr unsigned LANES = HD / 4, STEP = THREADS / LANES, ROWS = 2, PARTS = 4;
+    constexpr unsigned LANES = THREADS / NR, PIECES = 4, PARTS = 4;
     __threadfence();
     bar();
     if (tid == 0) *flag = atomicAdd(&A.counters[of.first], 1u) == of.last - of.first;
@@ -116,52 +122,49 @@ FYB_DEV void k4t_join(const Kv4Attention &A, const Kv8Parts &of, unsigned tid, u
     if (!*flag) return;
     __threadfence();
     if (tid == 0) A.counters[of.first] = 0;
-    const unsigned parts = of.last - of.first + 1, piece = tid % LANES;
+    const unsigned parts = of.last - of.first + 1, row = tid % NR;
+    if (row >= rows) return;
+    auto slot_of = [&](unsigned p) { return 2 * (of.first + p) + (p == 0 ? 1 : 0); };
+    float m = -3.4e38f, l = 0.f;
+#pragma unroll 4
+    for (unsigned p = 0; p < parts; ++p) m = fmaxf(m, __ldcg(&A.part_ml[(size_t)slot_of(p) * NR + row].x));
+#pragma unroll 4
+    for (unsigned p = 0; p < parts; ++p) {
+        const float2 y = __ldcg(&A.part_ml[(size_t)slot_of(p) * NR + row]);
+        l = fmaf(ex2(y.x - m), y.y, l);
+    }
+    const float n = l > 0.f || isnan(l) ? 1.f / l : 0.f;
 #pragma unroll 1
-    for (unsigned row = tid / LANES; row < rows; row += ROWS * STEP) {
-        float4 v[ROWS];
-        float m[ROWS], l[ROWS];
+    for (unsigned c = tid / NR * PIECES; c < HD / 4; c += LANES * PIECES) {
+        float4 v[PIECES];
 #pragma unroll
-        for (unsigned u = 0; u < ROWS; ++u) { v[u] = make_float4(0.f, 0.f, 0.f, 0.f); m[u] = -3.4e38f; l[u] = 0.f; }
+        for (unsigned u = 0; u < PIECES; ++u) v[u] = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 1
         for (unsigned p = 0; p < parts; p += PARTS) {
-            float4 x[ROWS][PARTS];
-            float2 ml[ROWS][PARTS];
+            float4 x[PARTS][PIECES];
+            float w[PARTS];
 #pragma unroll
-            for (unsigned u = 0; u < ROWS; ++u)
+            for (unsigned i = 0; i < PARTS; ++i) {
+                w[i] = -INFINITY;
+                if (p + i < parts) w[i] = __ldcg(&A.part_ml[(size_t)slot_of(p + i) * NR + row].x);
 #pragma unroll
-                for (unsigned i = 0; i < PARTS; ++i) {
-                    x[u][i] = make_float4(0.f, 0.f, 0.f, 0.f);
-                    ml[u][i] = make_float2(-3.4e38f, 0.f);
-                    if (p + i < parts && row + u * STEP < rows) {
-                        const size_t at = (size_t)(2 * (of.first + p + i) + (p + i == 0 ? 1 : 0)) * NR + row + u * STEP;
-                        x[u][i] = __ldcg(reinterpret_cast<const float4 *>(A.part_o + at * HD) + piece);
-                        ml[u][i] = __ldcg(A.part_ml + at);
-                    }
+                for (unsigned u = 0; u < PIECES; ++u) {
+                    x[i][u] = make_float4(0.f, 0.f, 0.f, 0.f);
+                    if (p + i < parts) x[i][u] = __ldcg(reinterpret_cast<const float4 *>(A.part_o) + k4t_part<NR, HD>(slot_of(p + i), c + u, row));
                 }
+            }
 #pragma unroll
-            for (unsigned u = 0; u < ROWS; ++u) {
-                float top = m[u];
+            for (unsigned i = 0; i < PARTS; ++i) {
+                const float f = ex2(w[i] - m) * n;
 #pragma unroll
-                for (unsigned i = 0; i < PARTS; ++i) top = fmaxf(top, ml[u][i].x);
-                const float old = ex2(m[u] - top);
-                m[u] = top;
-                l[u] *= old;
-                v[u].x *= old; v[u].y *= old; v[u].z *= old; v[u].w *= old;
-#pragma unroll
-                for (unsigned i = 0; i < PARTS; ++i) {
-                    const float w = ex2(ml[u][i].x - top);
-                    l[u] = fmaf(w, ml[u][i].y, l[u]);
-                    v[u].x = fmaf(w, x[u][i].x, v[u].x); v[u].y = fmaf(w, x[u][i].y, v[u].y);
-                    v[u].z = fmaf(w, x[u][i].z, v[u].z); v[u].w = fmaf(w, x[u][i].w, v[u].w);
+                for (unsigned u = 0; u < PIECES; ++u) {
+                    v[u].x = fmaf(f, x[i][u].x, v[u].x); v[u].y = fmaf(f, x[i][u].y, v[u].y);
+                    v[u].z = fmaf(f, x[i][u].z, v[u].z); v[u].w = fmaf(f, x[i][u].w, v[u].w);
                 }
             }
         }
 #pragma unroll
-        for (unsigned u = 0; u < ROWS; ++u) {
-            const float n = l[u] > 0.f || isnan(l[u]) ? 1.f / l[u] : 0.f;
-            if (row + u * STEP < rows) put(row + u * STEP, piece, make_float4(v[u].x * n, v[u].y * n, v[u].z * n, v[u].w * n));
-        }
+        for (unsigned u = 0; u < PIECES; u += 2) put(row, c + u, v[u], v[u + 1]);
     }
 }
 
@@ -347,25 +350,29 @@ __global__ void __launch_bounds__(k4t_threads(NR), 1) kv4_tiles_kernel(const __g
                 const size_t r = (size_t)(s.q.first + j0 + (int)(row / GR));
                 return r * A.out_stride + (size_t)(s.head * GR + row % GR) * HD;
             };
-            auto put = [&](unsigned row, unsigned chunk, float4 v) { kv8_store4(A.out, A.type, place_of(row) + 4 * chunk, v); };
-            // columns 8 chunk.. of a row, in the order of a word's numbers
-            auto leave = [&](unsigned row, size_t out, unsigned chunk, const float *z) {
-                const float4 lo = make_float4(z[0], z[2], z[4], z[6]), hi = make_float4(z[1], z[3], z[5], z[7]);
-                if (!whole) {
-                    float4 *o = reinterpret_cast<float4 *>(A.part_o + ((size_t)of.slot * NR + row) * HD) + 2 * chunk;
-                    o[0] = lo;
-                    o[1] = hi;
-                } else if (A.vec_out) {
+            auto write = [&](size_t out, float4 lo, float4 hi) {
+                if (A.vec_out) {
                     auto two = [&](float x, float y) {
                         if (A.type == T_F16) return kt_pack(x, y);
                         const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
                         return *reinterpret_cast<const unsigned *>(&h);
                     };
-                    *reinterpret_cast<uint4 *>(static_cast<unsigned short *>(A.out) + out + 8 * chunk) =
+                    *reinterpret_cast<uint4 *>(static_cast<unsigned short *>(A.out) + out) =
                         make_uint4(two(lo.x, lo.y), two(lo.z, lo.w), two(hi.x, hi.y), two(hi.z, hi.w));
                 } else {
-                    kv8_store4(A.out, A.type, out + 8 * chunk, lo);
-                    kv8_store4(A.out, A.type, out + 8 * chunk + 4, hi);
+                    kv8_store4(A.out, A.type, out, lo);
+                    kv8_store4(A.out, A.type, out + 4, hi);
+                }
+            };
+            // columns 8 chunk.. of a row, in the order of a word's numbers
+            auto leave = [&](unsigned row, size_t out, unsigned chunk, const float *z) {
+                const float4 lo = make_float4(z[0], z[2], z[4], z[6]), hi = make_float4(z[1], z[3], z[5], z[7]);
+                if (!whole) {
+                    float4 *o = reinterpret_cast<float4 *>(A.part_o) + k4t_part<NR, HD>(of.slot, 2 * chunk, row);
+                    o[0] = lo;
+                    o[NR] = hi;
+                } else {
+                    write(out + 8 * chunk, lo, hi);
                 }
             };
             if constexpr (GROUPS == 2) {
@@ -440,7 +447,8 @@ __global__ void __launch_bounds__(k4t_threads(NR), 1) kv4_tiles_kernel(const __g
                 arrive(sh.o_free);
             }
             if (!whole) {
-                k4t_join<NR, HD, 32 * SOFT>(A, of, tid, (unsigned)nrows, &sh.flag, bar, put);
+                k4t_join<NR, HD, 32 * SOFT>(A, of, tid, (unsigned)nrows, &sh.flag, bar,
+                    [&](unsigned row, unsigned piece, float4 lo, float4 hi) { write(place_of(row) + 4 * piece, lo, hi); });
                 bar();
             }
             done();
