@@ -34,7 +34,7 @@ FYB_HOST_DEV constexpr unsigned k4t_segs(int NR) { return NR == 256 ? 2 : 4; }  
 FYB_HOST_DEV constexpr int k4t_groups(int NR) { return NR == 256 ? 2 : 1; }      // groups of four softmax warps
 FYB_HOST_DEV constexpr int k4t_threads(int NR) { return 32 * (4 * k4t_groups(NR) + 2 * K4T_CONV + 3); }
 
-FYB_HOST_DEV constexpr int k4t_cost(int NR) { return NR == 256 ? 9 : 6; }        // a segment's beginning and end, in tiles
+FYB_HOST_DEV constexpr int k4t_cost(int NR) { return NR == 256 ? 6 : 8; }        // a segment's beginning and end, in tiles
 
 template <int HD, int NR> struct K4tShape {
     static constexpr int ROW = HD / 2, SCALES = HD / 64 * 4;                 // bytes of a token's row, of its scales
@@ -173,7 +173,7 @@ __global__ void __launch_bounds__(k4t_threads(NR), 1) kv4_tiles_kernel(const __g
     const __grid_constant__ CUtensorMap vmap)
 {
     using S = K4tShape<HD, NR>;
-    constexpr unsigned GROUPS = k4t_groups(NR), SOFT = 4 * GROUPS, W_CONV = SOFT, W_TMA = SOFT + 2 * K4T_CONV, W_MMA = W_TMA + 2;
+    constexpr unsigned CONV = K4T_CONV, GROUPS = k4t_groups(NR), SOFT = 4 * GROUPS, W_CONV = SOFT, W_TMA = SOFT + 2 * CONV, W_MMA = W_TMA + 2;
     constexpr unsigned CP = GROUPS == 2 ? 1 : 128 / NR, HALVES = GROUPS, CW = 128 / CP / HALVES, CHUNKS = CW / 32;   // copies, and the positions and blocks of 32 taken at a time
     constexpr unsigned SEGS = k4t_segs(NR);
     constexpr int G64 = HD / 64;
@@ -183,21 +183,21 @@ __global__ void __launch_bounds__(k4t_threads(NR), 1) kv4_tiles_kernel(const __g
     const unsigned tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), kv = A.c.kv_heads, GR = A.group;
     if (tid == 0) {
         for (int i = 0; i < 4; ++i) {
-            mbar_init(sh.rk_full + i, 1); mbar_init(sh.rk_empty + i, K4T_CONV);
-            mbar_init(sh.rv_full + i, 1); mbar_init(sh.rv_empty + i, K4T_CONV);
+            mbar_init(sh.rk_full + i, 1); mbar_init(sh.rk_empty + i, CONV);
+            mbar_init(sh.rv_full + i, 1); mbar_init(sh.rv_empty + i, CONV);
         }
         for (int i = 0; i < 2; ++i) {
-            mbar_init(sh.k_full + i, K4T_CONV); mbar_init(sh.k_empty + i, 1);
-            mbar_init(sh.v_full + i, K4T_CONV); mbar_init(sh.v_empty + i, 1);
+            mbar_init(sh.k_full + i, CONV); mbar_init(sh.k_empty + i, 1);
+            mbar_init(sh.v_full + i, CONV); mbar_init(sh.v_empty + i, 1);
             mbar_init(sh.s_full + i, 1); mbar_init(sh.o_free + i, 4);
         }
         for (int i = 0; i < 4; ++i) { mbar_init(sh.p_full + i, 4); mbar_init(sh.o_done + i, 1); }
         mbar_init(&sh.q_empty, 1); mbar_init(&sh.drained, 1);
         for (int i = 0; i < K4T_META; ++i) mbar_init(sh.meta_full + i, 1);
         for (unsigned i = 0; i < SEGS; ++i) {
-            mbar_init(sh.q_full + i, GROUPS * K4T_CONV);
+            mbar_init(sh.q_full + i, S::Q_TM ? 4 : 2 * CONV);
             mbar_init(sh.seg_full + i, 1);
-            mbar_init(sh.seg_empty + i, SOFT + 2 * K4T_CONV + 2);
+            mbar_init(sh.seg_empty + i, SOFT + 2 * CONV + 2);
         }
         sh.dead = 0;
         fence_barrier_init();
@@ -455,13 +455,14 @@ __global__ void __launch_bounds__(k4t_threads(NR), 1) kv4_tiles_kernel(const __g
         }
     } else if (warp < W_TMA) {
         // ================================================== K or V, 4 bits to fp16 rows; q
-        const bool is_v = warp >= W_CONV + K4T_CONV;
-        const unsigned cw = (warp - W_CONV) % K4T_CONV, ct = cw * 32 + lane;
-        const unsigned j = lane & 7, tok0 = cw * 32 + (lane >> 3);  // eight lanes a token, a warp 32 tokens
+        const bool is_v = warp >= W_CONV + CONV;
+        const unsigned cw = (warp - W_CONV) % CONV, ct = cw * 32 + lane;
+        constexpr unsigned TOKENS = K4_TILE / CONV;  // of a warp, eight lanes a token
+        const unsigned j = lane & 7, tok0 = cw * TOKENS + (lane >> 3);
         while (const Kv8Segment *sp = next()) {
             const Kv8Segment &s = *sp;
             const int any = kv8_attended(A, s.q, s.row_tile), t0 = s.t0, t1 = s.t1;
-            if (GROUPS == 2 || !is_v) {
+            if (GROUPS == 2 || (!is_v && cw < 4)) {
                 // ---- q rows by a power of two each. The score factor's sign goes with q: a row's largest product is its
                 // largest score
                 const int j0 = s.row_tile * (int)A.row_tile, nrows = min((int)A.row_tile, s.q.rows - j0) * (int)GR;
@@ -509,7 +510,7 @@ __global__ void __launch_bounds__(k4t_threads(NR), 1) kv4_tiles_kernel(const __g
                     kt_fence_before();
                 } else {
                     // to shared memory, eight values a lane
-                    constexpr unsigned LANES = HD / 8, STEP = 32 / LANES, STEPS = NR / (2 * K4T_CONV) / STEP, AHEAD = 4;  // lanes of a row, rows of a load
+                    constexpr unsigned LANES = HD / 8, STEP = 32 / LANES, STEPS = NR / (2 * CONV) / STEP, AHEAD = 4;  // lanes of a row, rows of a load
                     const unsigned piece = lane % LANES, row0 = (warp - W_CONV) * STEPS * STEP + lane / LANES;
 #pragma unroll 1
                     for (unsigned i = 0; i < STEPS; i += AHEAD) {
@@ -547,7 +548,7 @@ __global__ void __launch_bounds__(k4t_threads(NR), 1) kv4_tiles_kernel(const __g
                 // four tokens' words and scales at a time, before the first of their stores (which they might overlap, as
                 // far as the compiler can tell: a token after the other took 1500 cycles a tile)
 #pragma unroll
-                for (unsigned i0 = 0; i0 < 8; i0 += 4) {
+                for (unsigned i0 = 0; i0 < TOKENS / 4; i0 += 4) {
                     unsigned w[4][G64], sc[4][G64];
 #pragma unroll
                     for (unsigned i = 0; i < 4; ++i) {
