@@ -11,8 +11,6 @@ namespace fyb {
 using TilesLaunch = int(const Kv4Attention &, const CUtensorMap &, const CUtensorMap &, unsigned, cudaStream_t);
 TilesLaunch kv4_tiles_128_32, kv4_tiles_128_64, kv4_tiles_128_256, kv4_tiles_64_32, kv4_tiles_64_64, kv4_tiles_64_256;
 
-constexpr unsigned K4T_GRID = 148;  // one CTA per SM
-
 // K or V as rows of 128 bytes (two tokens of 64, or four of 32 bytes), boxes of one block (128 tokens at most), in the
 // swizzle of 128 bytes (kv4_at). Rows of one token each kept the copies from more than 0.68 of HBM's rate.
 static int kv4_tensor_map(CUtensorMap *map, const fyb_kv4_cache &c, const void *pool)
@@ -41,7 +39,7 @@ extern "C" size_t fyb_kv4_attention_workspace(uint32_t requests, uint32_t max_ro
     if (!requests || !max_rows || !kv_heads || heads < kv_heads || heads % kv_heads || heads / kv_heads > 64 ||
         (head_dim != 64 && head_dim != 128))
         return 0;
-    return K4_COUNTER_BYTES + part_rows((unsigned long long)max_rows * (heads / kv_heads)) * (head_dim + 2) * sizeof(float);
+    return K4_COUNTER_BYTES + K4_JOIN_BYTES + part_rows((unsigned long long)max_rows * (heads / kv_heads)) * (head_dim + 2) * sizeof(float);
 }
 
 extern "C" int fyb_kv4_attention(const fyb_kv4_cache *cache, const int32_t *lengths, const int32_t *row_start,
@@ -69,7 +67,8 @@ extern "C" int fyb_kv4_attention(const fyb_kv4_cache *cache, const int32_t *leng
     const unsigned long long group_rows = (unsigned long long)max_rows * A.group;
     unsigned char *ws = static_cast<unsigned char *>(workspace);
     A.counters = reinterpret_cast<unsigned *>(ws);
-    A.part_ml = reinterpret_cast<float2 *>(ws + K4_COUNTER_BYTES);
+    A.join = reinterpret_cast<K4tJoin *>(ws + K4_COUNTER_BYTES);
+    A.part_ml = reinterpret_cast<float2 *>(ws + K4_COUNTER_BYTES + K4_JOIN_BYTES);
     A.part_o = reinterpret_cast<float *>(A.part_ml + part_rows(group_rows));
     CUtensorMap k, v;
     if (kv4_tensor_map(&k, *cache, cache->k) || kv4_tensor_map(&v, *cache, cache->v)) return -2;

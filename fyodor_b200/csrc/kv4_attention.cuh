@@ -7,7 +7,13 @@
 
 namespace fyb {
 
+// The segment that begins in a CTA of the many-row kernel and goes on in others: its last CTA, its query rows (0: there is
+// none), the first of its call's rows, its head.
+struct K4tJoin {
+    unsigned last, rows, first_row, head;
+};
 struct Kv4Attention : Kv8Attention {
+    K4tJoin *join;
     const __half2 *ks, *vs;  // scale and low of each group
     unsigned split;          // parts of a KV head's group of query heads, each counted as a head (c.kv_heads, group)
     bool vec, vec_out;       // rows of 16 bits of q, of out begin on 16 bytes
@@ -34,6 +40,7 @@ FYB_DEV void k4_load_rows(unsigned dst, const CUtensorMap *map, int row, unsigne
 int launch_kv4_decode(const Kv4Attention &A, const CUtensorMap &k, const CUtensorMap &v, unsigned grid, cudaStream_t s);
 constexpr int K4_TILE = 128;  // positions of a unit
 constexpr unsigned K4_CTAS = 3, K4_GRID = K4_CTAS * 148;  // of the few-row kernel: CTAs per SM, largest grid
-constexpr size_t K4_COUNTER_BYTES = (K4_GRID * 4 + 255) / 256 * 256;
+constexpr unsigned K4T_GRID = 148;                        // of the many-row kernel: one CTA per SM
+constexpr size_t K4_COUNTER_BYTES = (K4_GRID * 4 + 255) / 256 * 256, K4_JOIN_BYTES = (K4T_GRID * sizeof(K4tJoin) + 255) / 256 * 256;
 
 }  // namespace fyb

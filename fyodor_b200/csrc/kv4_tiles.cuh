@@ -45,7 +45,7 @@ template <int HD, int NR> struct K4tShape {
     static constexpr int HALF = 128 * 128, TILE = HD / 64 * HALF;            // fp16 rows of 64 values in 128 bytes
     static constexpr int O_STRIDE = 20;                                      // floats between lanes of 16 columns of O of copies
     static constexpr int OFF_K = 0, OFF_V = 2 * TILE, OFF_Q = 4 * TILE, OFF_RK = OFF_Q + (Q_TM ? 0 : 2 * TILE), OFF_RV = OFF_RK + KS * RAW,
-                         OFF_O = OFF_RV + VS * RAW, STAGED = Q_TM ? 128 * O_STRIDE : 256, OFF_END = OFF_O + STAGED * 4;
+                         OFF_O = OFF_RV + VS * RAW, STAGED = Q_TM ? 128 * O_STRIDE : 0, OFF_END = OFF_O + STAGED * 4;
     // tensor memory columns: two S with P in the upper half, O of each group, q
     static constexpr int P = 64, O = 256, Q = 256 + HD;
 };
@@ -59,7 +59,7 @@ template <int NR> struct K4tShared {
     float2 ml[NR < 256 ? 128 : 1];
     unsigned here[K4T_META];                       // which groups of 16 positions of a tile are loaded
     uint32_t tmem;
-    unsigned flag, dead;
+    unsigned dead;
 };
 
 template <int COST> static __device__ __noinline__ void k4t_segment(const Kv4Attention &A, const Kv8Place &place, unsigned k, Kv8Segment *s)
@@ -104,67 +104,87 @@ FYB_DEV void k4t_load8(const Kv4Attention &A, size_t at, float4 &a, float4 &b)
 }
 
 // Partials lie as [4 columns][row]: a warp's rows, a lane each, are written and read side by side (as rows of head_dim
-// values each 16 bytes were a sector of their own: a prompt's partial took 12000 to 20000 cycles to be seen, its join 45000).
+// values each 16 bytes were a sector of their own: a prompt's partial took 12000 to 20000 cycles to be seen).
 template <int NR, int HD> FYB_DEV size_t k4t_part(unsigned slot, unsigned piece, unsigned row)
 {
     return ((size_t)slot * (HD / 4) + piece) * NR + row;
 }
-// The CTA's partial (of `rows` rows) is written: the last CTA of the segment joins them all in order. L2's latency is what
-// takes time: four parts of four pieces are on their way at once.
-template <int NR, int HD, int THREADS, typename Bar, typename Put>
-FYB_DEV void k4t_join(const Kv4Attention &A, const Kv8Parts &of, unsigned tid, unsigned rows, unsigned *flag, Bar bar, Put put)
+// Where row `row` of a segment lies in the output, and eight of its values.
+FYB_DEV size_t k4t_out(const Kv4Attention &A, unsigned first_row, unsigned head, unsigned row, unsigned hd)
 {
-    constexpr unsigned LANES = THREADS / NR, PIECES = 4, PARTS = 4;
-    __threadfence();
-    bar();
-    if (tid == 0) *flag = atomicAdd(&A.counters[of.first], 1u) == of.last - of.first;
-    bar();
-    if (!*flag) return;
-    __threadfence();
-    if (tid == 0) A.counters[of.first] = 0;
-    const unsigned parts = of.last - of.first + 1, row = tid % NR;
-    if (row >= rows) return;
-    auto slot_of = [&](unsigned p) { return 2 * (of.first + p) + (p == 0 ? 1 : 0); };
-    float m = -3.4e38f, l = 0.f;
-#pragma unroll 4
-    for (unsigned p = 0; p < parts; ++p) m = fmaxf(m, __ldcg(&A.part_ml[(size_t)slot_of(p) * NR + row].x));
-#pragma unroll 4
-    for (unsigned p = 0; p < parts; ++p) {
-        const float2 y = __ldcg(&A.part_ml[(size_t)slot_of(p) * NR + row]);
-        l = fmaf(ex2(y.x - m), y.y, l);
+    return (size_t)(first_row + row / A.group) * A.out_stride + (size_t)(head * A.group + row % A.group) * hd;
+}
+FYB_DEV void k4t_write(const Kv4Attention &A, size_t out, float4 lo, float4 hi)
+{
+    if (A.vec_out) {
+        auto two = [&](float x, float y) {
+            if (A.type == T_F16) return kt_pack(x, y);
+            const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+            return *reinterpret_cast<const unsigned *>(&h);
+        };
+        *reinterpret_cast<uint4 *>(static_cast<unsigned short *>(A.out) + out) =
+            make_uint4(two(lo.x, lo.y), two(lo.z, lo.w), two(hi.x, hi.y), two(hi.z, hi.w));
+    } else {
+        kv8_store4(A.out, A.type, out, lo);
+        kv8_store4(A.out, A.type, out + 4, hi);
     }
-    const float n = l > 0.f || isnan(l) ? 1.f / l : 0.f;
+}
+
+// Joins the parts of the segment that begins in each CTA of the tiles kernel and goes on in others, in order: 32 rows a
+// CTA, a lane each, and the warps share the columns. L2's latency is what takes time: four parts of PIECES pieces are on
+// their way at once. A launch of its own, so that all SMs join: by the segment's last CTA a prompt of 64 rows at 16000
+// took 86 us instead of JJ.
+constexpr int K4T_JOIN = 256;
+template <int HD, int NR> __global__ void __launch_bounds__(K4T_JOIN) kv4_join_kernel(const __grid_constant__ Kv4Attention A)
+{
+    constexpr unsigned PIECES = HD / 4 / (K4T_JOIN / 32), PARTS = 4;
+    const K4tJoin j = A.join[blockIdx.x];
+    const unsigned row = blockIdx.y * 32 + (threadIdx.x & 31), c = threadIdx.x / 32 * PIECES, parts = j.last - blockIdx.x + 1;
+    if (row >= j.rows) return;
+    auto slot_of = [&](unsigned p) { return 2 * (blockIdx.x + p) + (p == 0 ? 1 : 0); };
+    float m = -3.4e38f, l = 0.f;
+    float4 v[PIECES];
+#pragma unroll
+    for (unsigned u = 0; u < PIECES; ++u) v[u] = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 1
-    for (unsigned c = tid / NR * PIECES; c < HD / 4; c += LANES * PIECES) {
-        float4 v[PIECES];
+    for (unsigned p = 0; p < parts; p += PARTS) {
+        float4 x[PARTS][PIECES];
+        float2 ml[PARTS];
 #pragma unroll
-        for (unsigned u = 0; u < PIECES; ++u) v[u] = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 1
-        for (unsigned p = 0; p < parts; p += PARTS) {
-            float4 x[PARTS][PIECES];
-            float w[PARTS];
+        for (unsigned i = 0; i < PARTS; ++i) {
+            ml[i] = make_float2(-3.4e38f, 0.f);
+            if (p + i < parts) ml[i] = __ldcg(&A.part_ml[(size_t)slot_of(p + i) * NR + row]);
 #pragma unroll
-            for (unsigned i = 0; i < PARTS; ++i) {
-                w[i] = -INFINITY;
-                if (p + i < parts) w[i] = __ldcg(&A.part_ml[(size_t)slot_of(p + i) * NR + row].x);
-#pragma unroll
-                for (unsigned u = 0; u < PIECES; ++u) {
-                    x[i][u] = make_float4(0.f, 0.f, 0.f, 0.f);
-                    if (p + i < parts) x[i][u] = __ldcg(reinterpret_cast<const float4 *>(A.part_o) + k4t_part<NR, HD>(slot_of(p + i), c + u, row));
-                }
-            }
-#pragma unroll
-            for (unsigned i = 0; i < PARTS; ++i) {
-                const float f = ex2(w[i] - m) * n;
-#pragma unroll
-                for (unsigned u = 0; u < PIECES; ++u) {
-                    v[u].x = fmaf(f, x[i][u].x, v[u].x); v[u].y = fmaf(f, x[i][u].y, v[u].y);
-                    v[u].z = fmaf(f, x[i][u].z, v[u].z); v[u].w = fmaf(f, x[i][u].w, v[u].w);
-                }
+            for (unsigned u = 0; u < PIECES; ++u) {
+                x[i][u] = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (p + i < parts) x[i][u] = __ldcg(reinterpret_cast<const float4 *>(A.part_o) + k4t_part<NR, HD>(slot_of(p + i), c + u, row));
             }
         }
+        float top = m;
 #pragma unroll
-        for (unsigned u = 0; u < PIECES; u += 2) put(row, c + u, v[u], v[u + 1]);
+        for (unsigned i = 0; i < PARTS; ++i) top = fmaxf(top, ml[i].x);
+        const float old = ex2(m - top);
+        m = top;
+        l *= old;
+#pragma unroll
+        for (unsigned u = 0; u < PIECES; ++u) { v[u].x *= old; v[u].y *= old; v[u].z *= old; v[u].w *= old; }
+#pragma unroll
+        for (unsigned i = 0; i < PARTS; ++i) {
+            const float w = ex2(ml[i].x - m);
+            l = fmaf(w, ml[i].y, l);
+#pragma unroll
+            for (unsigned u = 0; u < PIECES; ++u) {
+                v[u].x = fmaf(w, x[i][u].x, v[u].x); v[u].y = fmaf(w, x[i][u].y, v[u].y);
+                v[u].z = fmaf(w, x[i][u].z, v[u].z); v[u].w = fmaf(w, x[i][u].w, v[u].w);
+            }
+        }
+    }
+    const float n = l > 0.f || isnan(l) ? 1.f / l : 0.f;
+    const size_t out = k4t_out(A, j.first_row, j.head, row, HD);
+#pragma unroll
+    for (unsigned u = 0; u < PIECES; u += 2) {
+        auto times = [&](float4 y) { return make_float4(y.x * n, y.y * n, y.z * n, y.w * n); };
+        k4t_write(A, out + 4 * (c + u), times(v[u]), times(v[u + 1]));
     }
 }
 
@@ -240,6 +260,7 @@ __global__ void __launch_bounds__(k4t_threads(NR), 1) kv4_tiles_kernel(const __g
         const uint32_t o_at = tmem + lanes + S::O + wg * HD;
         float *stage = reinterpret_cast<float *>(ring + S::OFF_O);
         unsigned k = 0;  // tiles of this group so far
+        bool goes_on = false;  // the last segment, in the next CTA
         auto bar = [] { asm volatile("bar.sync 1, %0;" :: "n"(32 * SOFT) : "memory"); };
         constexpr float P_UP = 6.f;  // weights are 2^6 times themselves, clear of fp16's smallest numbers; the largest is 2^14
         while (const Kv8Segment *sp = next()) {
@@ -346,24 +367,7 @@ __global__ void __launch_bounds__(k4t_threads(NR), 1) kv4_tiles_kernel(const __g
             // ---- the segment's part
             const bool whole = s.t0 == 0 && s.t1 == s.tiles;
             const Kv8Parts of = kv8_parts(s, sh.place);
-            auto place_of = [&](unsigned row) {
-                const size_t r = (size_t)(s.q.first + j0 + (int)(row / GR));
-                return r * A.out_stride + (size_t)(s.head * GR + row % GR) * HD;
-            };
-            auto write = [&](size_t out, float4 lo, float4 hi) {
-                if (A.vec_out) {
-                    auto two = [&](float x, float y) {
-                        if (A.type == T_F16) return kt_pack(x, y);
-                        const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
-                        return *reinterpret_cast<const unsigned *>(&h);
-                    };
-                    *reinterpret_cast<uint4 *>(static_cast<unsigned short *>(A.out) + out) =
-                        make_uint4(two(lo.x, lo.y), two(lo.z, lo.w), two(hi.x, hi.y), two(hi.z, hi.w));
-                } else {
-                    kv8_store4(A.out, A.type, out, lo);
-                    kv8_store4(A.out, A.type, out + 4, hi);
-                }
-            };
+            auto place_of = [&](unsigned row) { return k4t_out(A, (unsigned)(s.q.first + j0), s.head, row, HD); };
             // columns 8 chunk.. of a row, in the order of a word's numbers
             auto leave = [&](unsigned row, size_t out, unsigned chunk, const float *z) {
                 const float4 lo = make_float4(z[0], z[2], z[4], z[6]), hi = make_float4(z[1], z[3], z[5], z[7]);
@@ -372,7 +376,7 @@ __global__ void __launch_bounds__(k4t_threads(NR), 1) kv4_tiles_kernel(const __g
                     o[0] = lo;
                     o[NR] = hi;
                 } else {
-                    write(out + 8 * chunk, lo, hi);
+                    k4t_write(A, out + 8 * chunk, lo, hi);
                 }
             };
             if constexpr (GROUPS == 2) {
@@ -446,13 +450,13 @@ __global__ void __launch_bounds__(k4t_threads(NR), 1) kv4_tiles_kernel(const __g
                 kt_fence_before();
                 arrive(sh.o_free);
             }
-            if (!whole) {
-                k4t_join<NR, HD, 32 * SOFT>(A, of, tid, (unsigned)nrows, &sh.flag, bar,
-                    [&](unsigned row, unsigned piece, float4 lo, float4 hi) { write(place_of(row) + 4 * piece, lo, hi); });
-                bar();
+            if (!whole && t0 == 0) {  // goes on in other CTAs
+                if (tid == 0) A.join[blockIdx.x] = K4tJoin{of.last, (unsigned)nrows, (unsigned)(s.q.first + j0), s.head};
+                goes_on = true;
             }
             done();
         }
+        if (!goes_on && tid == 0) A.join[blockIdx.x].rows = 0;
     } else if (warp < W_TMA) {
         // ================================================== K or V, 4 bits to fp16 rows; q
         const bool is_v = warp >= W_CONV + CONV;
@@ -769,6 +773,7 @@ int kv4_tiles_go(const Kv4Attention &A, const CUtensorMap &k, const CUtensorMap 
     static std::atomic<unsigned> allowed{0};
     if (allow_shared((const void *)kv4_tiles_kernel<HD, NR>, smem, allowed)) return -2;
     kv4_tiles_kernel<HD, NR><<<grid, k4t_threads(NR), smem, s>>>(A, k, v);
+    kv4_join_kernel<HD, NR><<<dim3(grid, NR / 32), K4T_JOIN, 0, s>>>(A);
     return cudaGetLastError() == cudaSuccess ? 0 : -2;
 }
 

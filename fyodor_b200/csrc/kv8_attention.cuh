@@ -264,8 +264,8 @@ FYB_DEV Kv8Parts kv8_parts(const Kv8Segment &s, const Kv8Place &place)
     return p;
 }
 // THREADS threads call it once the CTA's partial (of `rows` of R rows) is written: the last CTA of the segment puts the
-// joined rows out, a thread ITEMS of four values at a time. bar(): a barrier over them.
-template <int R, int HD, int THREADS, int ITEMS = 1, typename Bar, typename Put>
+// joined rows out. bar(): a barrier over them.
+template <int R, int HD, int THREADS, typename Bar, typename Put>
 FYB_DEV void kv8_arrive(const Kv8Attention &A, const Kv8Parts &of, unsigned tid, unsigned rows, float *weights,
     unsigned max_weights, unsigned *flag, Bar bar, Put put)
 {
@@ -304,35 +304,6 @@ FYB_DEV void kv8_arrive(const Kv8Attention &A, const Kv8Parts &of, unsigned tid,
         if (i < some)
             for (unsigned p = lane; p < parts; p += G) weights[p * some + i] *= n;
         bar();
-        if constexpr (ITEMS > 1) {  // L2's latency is what counts: several loads in flight, and few parts to add up
-#pragma unroll 1
-            for (unsigned i0 = tid; i0 < some * (HD / 4); i0 += ITEMS * THREADS) {
-                float4 v[ITEMS];
-#pragma unroll
-                for (int u = 0; u < ITEMS; ++u) v[u] = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 1
-                for (unsigned p = 0; p < parts; ++p) {
-                    const float4 *o = reinterpret_cast<const float4 *>(A.part_o + slot_of(p) * R * HD) + (size_t)row0 * (HD / 4);
-                    float4 x[ITEMS];
-#pragma unroll
-                    for (int u = 0; u < ITEMS; ++u)
-                        if (i0 + u * THREADS < some * (HD / 4)) x[u] = __ldcg(o + i0 + u * THREADS);
-#pragma unroll
-                    for (int u = 0; u < ITEMS; ++u) {
-                        const unsigned i = i0 + u * THREADS;
-                        if (i >= some * (HD / 4)) break;
-                        const float w = weights[p * some + i / (HD / 4)];
-                        v[u].x = fmaf(w, x[u].x, v[u].x); v[u].y = fmaf(w, x[u].y, v[u].y);
-                        v[u].z = fmaf(w, x[u].z, v[u].z); v[u].w = fmaf(w, x[u].w, v[u].w);
-                    }
-                }
-#pragma unroll
-                for (int u = 0; u < ITEMS; ++u) {
-                    const unsigned i = i0 + u * THREADS;
-                    if (i < some * (HD / 4)) put(row0 + i / (HD / 4), i % (HD / 4), v[u]);
-                }
-            }
-        } else
         for (unsigned i = tid; i < some * (HD / 4); i += THREADS) {
             const unsigned row = i / (HD / 4);
             float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
