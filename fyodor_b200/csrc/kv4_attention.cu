@@ -3,7 +3,10 @@
 //
 // Up to eight query rows per KV head (rows of a request x heads of a group), and
 // rows of F32 whatever their number, run on kv4_decode.cu, many rows in row tiles of
-// eight; many rows of 16 bits on kv4_tiles.cuh, in row tiles of 32, 64 or 256.
+// eight; many rows of 16 bits on kv4_tiles.cuh, in row tiles of 32, 64 or 256. With 8
+// rows 32 ragged requests take 64 us there and 99 in tiles; with 16 rows, two row
+// tiles, 112 and 100, 16 requests at 8100 82 and 75, with 32 rows 149 and 77 (what is
+// short is still quicker: four requests of 500 with 16 rows 12 us and 18).
 #include "kv4_attention.cuh"
 
 namespace fyb {
@@ -20,8 +23,10 @@ static int kv4_tensor_map(CUtensorMap *map, const fyb_kv4_cache &c, const void *
                           std::min(c.block_size, (unsigned)K4_TILE) / tokens, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
-// Row tile of the many-row kernel.
-static unsigned tile_rows(unsigned long long group_rows) { return group_rows <= 32 ? 32 : group_rows <= 64 ? 64 : 256; }
+// Row tile of the many-row kernel. 128 rows of a request are two tiles of 64 (one of 16000 tokens: 40 us, in tiles of 256
+// 52; four of them 77 and 90); 256 rows of one of 16000 would still be quicker so (51 and 59), of one of 64000 not (127
+// and 111), 500 rows at 16000 not either (76 and 70), 2000 rows far from it (234 and 165).
+static unsigned tile_rows(unsigned long long group_rows) { return group_rows <= 32 ? 32 : group_rows <= 128 ? 64 : 256; }
 // Query rows of a call's partials, two for each CTA of its kernel (F32 rows need 2 K4_GRID of eight: fewer than tiles do).
 static size_t part_rows(unsigned long long group_rows)
 {

@@ -59,7 +59,7 @@ template <int NR> struct K4tShared {
     float2 ml[NR < 256 ? 128 : 1];
     unsigned here[K4T_META];                       // which groups of 16 positions of a tile are loaded
     uint32_t tmem;
-    unsigned dead;
+    unsigned flag, dead;
 };
 
 template <int COST> static __device__ __noinline__ void k4t_segment(const Kv4Attention &A, const Kv8Place &place, unsigned k, Kv8Segment *s)
@@ -130,10 +130,10 @@ FYB_DEV void k4t_write(const Kv4Attention &A, size_t out, float4 lo, float4 hi)
     }
 }
 
-// Joins the parts of the segment that begins in each CTA of the tiles kernel and goes on in others, in order: 32 rows a
-// CTA, a lane each, and the warps share the columns. L2's latency is what takes time: four parts of PIECES pieces are on
-// their way at once. A launch of its own, so that all SMs join: by the segment's last CTA a prompt of 64 rows at 16000
-// took 86 us instead of JJ.
+// Row tiles of 256: the parts of the segment that begins in each CTA of the tiles kernel and goes on in others, joined in
+// order, 32 rows a CTA, a lane each, and the warps share the columns. L2's latency is what takes time: four parts of PIECES
+// pieces are on their way at once. A launch of its own, so that all SMs join: by the segment's last CTA, as below, a prompt
+// of 64 rows of four heads at 16000 took 86 us instead of 59, one of 500 rows 174 instead of 167.
 constexpr int K4T_JOIN = 256;
 template <int HD, int NR> __global__ void __launch_bounds__(K4T_JOIN) kv4_join_kernel(const __grid_constant__ Kv4Attention A)
 {
@@ -185,6 +185,65 @@ template <int HD, int NR> __global__ void __launch_bounds__(K4T_JOIN) kv4_join_k
     for (unsigned u = 0; u < PIECES; u += 2) {
         auto times = [&](float4 y) { return make_float4(y.x * n, y.y * n, y.z * n, y.w * n); };
         k4t_write(A, out + 4 * (c + u), times(v[u]), times(v[u + 1]));
+    }
+}
+
+// Row tiles of 64 or 32: the CTA's partial is written, and the last CTA of the segment joins them all (a launch more took
+// 32 ragged drafts of 32 rows from 242 to 250 us, 16 requests of 32 rows at 8100 from 77 to 81).
+template <int NR, int HD, int THREADS, typename Bar, typename Put>
+FYB_DEV void k4t_join(const Kv4Attention &A, const Kv8Parts &of, unsigned tid, unsigned rows, unsigned *flag, Bar bar, Put put)
+{
+    constexpr unsigned LANES = THREADS / NR, PIECES = 4, PARTS = 4;
+    __threadfence();
+    bar();
+    if (tid == 0) *flag = atomicAdd(&A.counters[of.first], 1u) == of.last - of.first;
+    bar();
+    if (!*flag) return;
+    __threadfence();
+    if (tid == 0) A.counters[of.first] = 0;
+    const unsigned parts = of.last - of.first + 1, row = tid % NR;
+    if (row >= rows) return;
+    auto slot_of = [&](unsigned p) { return 2 * (of.first + p) + (p == 0 ? 1 : 0); };
+    float m = -3.4e38f, l = 0.f;
+#pragma unroll 4
+    for (unsigned p = 0; p < parts; ++p) m = fmaxf(m, __ldcg(&A.part_ml[(size_t)slot_of(p) * NR + row].x));
+#pragma unroll 4
+    for (unsigned p = 0; p < parts; ++p) {
+        const float2 y = __ldcg(&A.part_ml[(size_t)slot_of(p) * NR + row]);
+        l = fmaf(ex2(y.x - m), y.y, l);
+    }
+    const float n = l > 0.f || isnan(l) ? 1.f / l : 0.f;
+#pragma unroll 1
+    for (unsigned c = tid / NR * PIECES; c < HD / 4; c += LANES * PIECES) {
+        float4 v[PIECES];
+#pragma unroll
+        for (unsigned u = 0; u < PIECES; ++u) v[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 1
+        for (unsigned p = 0; p < parts; p += PARTS) {
+            float4 x[PARTS][PIECES];
+            float w[PARTS];
+#pragma unroll
+            for (unsigned i = 0; i < PARTS; ++i) {
+                w[i] = -INFINITY;
+                if (p + i < parts) w[i] = __ldcg(&A.part_ml[(size_t)slot_of(p + i) * NR + row].x);
+#pragma unroll
+                for (unsigned u = 0; u < PIECES; ++u) {
+                    x[i][u] = make_float4(0.f, 0.f, 0.f, 0.f);
+                    if (p + i < parts) x[i][u] = __ldcg(reinterpret_cast<const float4 *>(A.part_o) + k4t_part<NR, HD>(slot_of(p + i), c + u, row));
+                }
+            }
+#pragma unroll
+            for (unsigned i = 0; i < PARTS; ++i) {
+                const float f = ex2(w[i] - m) * n;
+#pragma unroll
+                for (unsigned u = 0; u < PIECES; ++u) {
+                    v[u].x = fmaf(f, x[i][u].x, v[u].x); v[u].y = fmaf(f, x[i][u].y, v[u].y);
+                    v[u].z = fmaf(f, x[i][u].z, v[u].z); v[u].w = fmaf(f, x[i][u].w, v[u].w);
+                }
+            }
+        }
+#pragma unroll
+        for (unsigned u = 0; u < PIECES; u += 2) put(row, c + u, v[u], v[u + 1]);
     }
 }
 
@@ -450,13 +509,20 @@ __global__ void __launch_bounds__(k4t_threads(NR), 1) kv4_tiles_kernel(const __g
                 kt_fence_before();
                 arrive(sh.o_free);
             }
-            if (!whole && t0 == 0) {  // goes on in other CTAs
+            if constexpr (GROUPS == 1) {
+                if (!whole) {
+                    k4t_join<NR, HD, 32 * SOFT>(A, of, tid, (unsigned)nrows, &sh.flag, bar, [&](unsigned row, unsigned piece, float4 lo, float4 hi) {
+                        k4t_write(A, place_of(row) + 4 * piece, lo, hi);
+                    });
+                    bar();
+                }
+            } else if (!whole && t0 == 0) {  // goes on in other CTAs
                 if (tid == 0) A.join[blockIdx.x] = K4tJoin{of.last, (unsigned)nrows, (unsigned)(s.q.first + j0), s.head};
                 goes_on = true;
             }
             done();
         }
-        if (!goes_on && tid == 0) A.join[blockIdx.x].rows = 0;
+        if (GROUPS == 2 && !goes_on && tid == 0) A.join[blockIdx.x].rows = 0;
     } else if (warp < W_TMA) {
         // ================================================== K or V, 4 bits to fp16 rows; q
         const bool is_v = warp >= W_CONV + CONV;
@@ -773,7 +839,7 @@ int kv4_tiles_go(const Kv4Attention &A, const CUtensorMap &k, const CUtensorMap 
     static std::atomic<unsigned> allowed{0};
     if (allow_shared((const void *)kv4_tiles_kernel<HD, NR>, smem, allowed)) return -2;
     kv4_tiles_kernel<HD, NR><<<grid, k4t_threads(NR), smem, s>>>(A, k, v);
-    kv4_join_kernel<HD, NR><<<dim3(grid, NR / 32), K4T_JOIN, 0, s>>>(A);
+    if constexpr (NR == 256) kv4_join_kernel<HD, NR><<<dim3(grid, NR / 32), K4T_JOIN, 0, s>>>(A);
     return cudaGetLastError() == cudaSuccess ? 0 : -2;
 }
 
