@@ -86,21 +86,42 @@ FYB_DEV uint4 k4t_values(unsigned x, __half2 scale, __half2 low)
     return make_uint4(out[0], out[1], out[2], out[3]);
 }
 
-// Eight values of a query row of 16 bits; vec: in one access.
-FYB_DEV void k4t_load8(const Kv4Attention &A, size_t at, float4 &a, float4 &b)
+// Eight values of a query row of 16 bits as they lie; vec: in one access. (What runs once a segment is kept small: its
+// instructions come from L2, 128 bytes in some 600 cycles.)
+static __device__ __noinline__ uint4 k4t_gather8(const unsigned short *q)
 {
-    if (A.vec) {
-        const uint4 u = __ldg(reinterpret_cast<const uint4 *>(static_cast<const unsigned short *>(A.q) + at));
-        auto two = [&](unsigned w) {
-            return A.type == T_F16 ? kt_unpack(w) : make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
-        };
-        const float2 p = two(u.x), q = two(u.y), r = two(u.z), s = two(u.w);
-        a = make_float4(p.x, p.y, q.x, q.y);
-        b = make_float4(r.x, r.y, s.x, s.y);
-    } else {
-        a = kv8_load4(A.q, A.type, at);
-        b = kv8_load4(A.q, A.type, at + 4);
-    }
+    unsigned w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = __ldg(q + 2 * i) | (unsigned)__ldg(q + 2 * i + 1) << 16;
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+FYB_DEV uint4 k4t_load8(const Kv4Attention &A, size_t at)
+{
+    const unsigned short *q = static_cast<const unsigned short *>(A.q) + at;
+    return A.vec ? __ldg(reinterpret_cast<const uint4 *>(q)) : k4t_gather8(q);
+}
+// 16 bytes global -> shared by this thread, and until all that it asked for have come.
+FYB_DEV void k4t_async16(void *dst, const void *src)
+{
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" :: "r"(smem_u32(dst)), "l"(src) : "memory");
+}
+FYB_DEV void k4t_async_wait() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+// Sizes of the two values of a word, the larger of each of two words: bits without a sign are in order, NaN last.
+FYB_DEV unsigned k4t_larger(unsigned x, unsigned y) { return __vmaxu2(x & 0x7fff7fffu, y & 0x7fff7fffu); }
+FYB_DEV float2 k4t_two(bool f16, unsigned w) { return f16 ? kt_unpack(w) : make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)); }
+// Power of two that a row with this largest size is multiplied by, to lie below 2^13.
+FYB_DEV int k4t_up(bool f16, unsigned sizes)
+{
+    const float2 y = k4t_two(f16, sizes);
+    return 12 - kt_exponent(fmaxf(y.x, y.y));
+}
+// Eight values times 2^e (and the sign of scale) as fp16, in the order of a word's numbers.
+FYB_DEV uint4 k4t_halves(bool f16, uint4 q, int e, float scale)
+{
+    const float up = copysignf(kt_power(min(e, 127)), scale), up2 = kt_power(e - min(e, 127));
+    const float2 a = k4t_two(f16, q.x), b = k4t_two(f16, q.y), c = k4t_two(f16, q.z), d = k4t_two(f16, q.w);
+    auto pair = [&](float y, float z) { return kt_pack(y * up * up2, z * up * up2); };
+    return make_uint4(pair(a.x, c.x), pair(a.y, c.y), pair(b.x, d.x), pair(b.y, d.y));
 }
 
 // Partials lie as [4 columns][row]: a warp's rows, a lane each, are written and read side by side (as rows of head_dim
@@ -525,7 +546,7 @@ __global__ void __launch_bounds__(k4t_threads(NR), 1) kv4_tiles_kernel(const __g
         if (GROUPS == 2 && !goes_on && tid == 0) A.join[blockIdx.x].rows = 0;
     } else if (warp < W_TMA) {
         // ================================================== K or V, 4 bits to fp16 rows; q
-        const bool is_v = warp >= W_CONV + CONV;
+        const bool f16 = A.type == T_F16, is_v = warp >= W_CONV + CONV;
         const unsigned cw = (warp - W_CONV) % CONV, ct = cw * 32 + lane;
         constexpr unsigned TOKENS = K4_TILE / CONV;  // of a warp, eight lanes a token
         const unsigned j = lane & 7, tok0 = cw * TOKENS + (lane >> 3);
@@ -539,67 +560,61 @@ __global__ void __launch_bounds__(k4t_threads(NR), 1) kv4_tiles_kernel(const __g
                 auto at_of = [&](unsigned rho) {
                     return (size_t)(s.q.first + j0 + (int)(rho / GR)) * A.q_stride + (size_t)(s.head * GR + rho % GR) * HD;
                 };
-                auto size_of = [](float4 a) { return fmaxf(fmaxf(fabsf(a.x), fabsf(a.y)), fmaxf(fabsf(a.z), fabsf(a.w))); };
-                auto halves = [&](float4 a, float4 b, int e) {
-                    const float up = copysignf(kt_power(min(e, 127)), A.scale), up2 = kt_power(e - min(e, 127));
-                    auto pair = [&](float y, float z) { return kt_pack(y * up * up2, z * up * up2); };
-                    return make_uint4(pair(a.x, b.x), pair(a.y, b.y), pair(a.z, b.z), pair(a.w, b.w));
-                };
                 // at least the smallest normal number: -inf times it stays -inf
-                auto factor_of = [&](int e) { return fmaxf(ldexpf(fabsf(A.scale), -e), 1.17549435e-38f); };
+                auto factor_of = [&](int e) { return fmaxf(fabsf(A.scale) * kt_power(-e), 1.17549435e-38f); };
                 if constexpr (S::Q_TM) {
                     // to tensor memory, a thread a lane's row
                     const unsigned rho = ct % NR;
                     const bool real = (int)rho < nrows;
                     const size_t at = at_of(real ? rho : 0);
-                    float top = 0.f;
-                    if (real) {
-#pragma unroll 8
-                        for (int i = 0; i < HD; i += 8) {
-                            float4 a, b;
-                            k4t_load8(A, at + i, a, b);
-                            top = fmaxf(top, fmaxf(size_of(a), size_of(b)));
-                        }
+                    unsigned top = 0;
+#pragma unroll 1
+                    for (int i = 0; real && i < HD; i += 64) {
+                        uint4 x[8];
+#pragma unroll
+                        for (int u = 0; u < 8; ++u) x[u] = k4t_load8(A, at + i + 8 * u);
+#pragma unroll
+                        for (int u = 0; u < 8; ++u) top = k4t_larger(top, k4t_larger(k4t_larger(x[u].x, x[u].y), k4t_larger(x[u].z, x[u].w)));
                     }
-                    const int e = 12 - kt_exponent(top);
+                    const int e = k4t_up(f16, top);
                     if (seg) wait(&sh.q_empty, seg - 1);  // the last segment's products have read their q
                     kt_fence_after();
-#pragma unroll 2
+#pragma unroll 1
                     for (int i = 0; i < HD; i += 32) {
                         uint4 h[4];
 #pragma unroll
-                        for (int u = 0; u < 4; ++u) {
-                            float4 a = make_float4(0.f, 0.f, 0.f, 0.f), b = a;
-                            if (real) k4t_load8(A, at + i + 8 * u, a, b);
-                            h[u] = halves(a, b, e);
-                        }
+                        for (int u = 0; u < 4; ++u) h[u] = real ? k4t_halves(f16, k4t_load8(A, at + i + 8 * u), e, A.scale) : make_uint4(0, 0, 0, 0);
                         kt_st16(tmem + (cw << 21) + S::Q + i / 2, reinterpret_cast<const float *>(h));
                     }
                     kt_wait_st();
                     sh.factor[seg % SEGS][ct] = factor_of(e);
                     kt_fence_before();
                 } else {
-                    // to shared memory, eight values a lane
-                    constexpr unsigned LANES = HD / 8, STEP = 32 / LANES, STEPS = NR / (2 * CONV) / STEP, AHEAD = 4;  // lanes of a row, rows of a load
+                    // to shared memory, eight values a lane: all rows as they lie first, and then each in its place
+                    constexpr unsigned LANES = HD / 8, STEP = 32 / LANES, STEPS = NR / (2 * CONV) / STEP;  // lanes of a row, rows of a load
                     const unsigned piece = lane % LANES, row0 = (warp - W_CONV) * STEPS * STEP + lane / LANES;
+                    auto place = [&](unsigned rho) {
+                        return ring + S::OFF_Q + rho / 128 * S::TILE + piece / 8 * S::HALF + rho % 128 * 128 + ((piece % 8 ^ (rho & 7u)) << 4);
+                    };
+                    if (seg) wait(&sh.q_empty, seg - 1);  // the last segment's products have read their q
 #pragma unroll 1
-                    for (unsigned i = 0; i < STEPS; i += AHEAD) {
-                        float4 x[AHEAD][2];
-#pragma unroll
-                        for (unsigned u = 0; u < AHEAD; ++u) {
-                            const unsigned rho = row0 + (i + u) * STEP;
-                            x[u][0] = x[u][1] = make_float4(0.f, 0.f, 0.f, 0.f);
-                            if ((int)rho < nrows) k4t_load8(A, at_of(rho) + 8 * piece, x[u][0], x[u][1]);
-                        }
-                        if (seg && i == 0) wait(&sh.q_empty, seg - 1);  // the last segment's products have read their q
-#pragma unroll
-                        for (unsigned u = 0; u < AHEAD; ++u) {
-                            const unsigned rho = row0 + (i + u) * STEP;
-                            const int e = 12 - kt_exponent(group_max<LANES>(fmaxf(size_of(x[u][0]), size_of(x[u][1]))));
-                            *reinterpret_cast<uint4 *>(ring + S::OFF_Q + rho / 128 * S::TILE + piece / 8 * S::HALF + rho % 128 * 128 + ((piece % 8 ^ (rho & 7u)) << 4)) =
-                                halves(x[u][0], x[u][1], e);
-                            if (piece == 0) sh.factor[seg % SEGS][rho] = factor_of(e);
-                        }
+                    for (unsigned i = 0; i < STEPS; ++i) {
+                        const unsigned rho = row0 + i * STEP;
+                        uint4 *to = reinterpret_cast<uint4 *>(place(rho));
+                        if ((int)rho >= nrows) *to = make_uint4(0, 0, 0, 0);
+                        else if (A.vec) k4t_async16(to, static_cast<const unsigned short *>(A.q) + at_of(rho) + 8 * piece);
+                        else *to = k4t_load8(A, at_of(rho) + 8 * piece);
+                    }
+                    k4t_async_wait();
+#pragma unroll 2
+                    for (unsigned i = 0; i < STEPS; ++i) {
+                        const unsigned rho = row0 + i * STEP;
+                        uint4 *at = reinterpret_cast<uint4 *>(place(rho));
+                        const uint4 x = *at;
+                        const unsigned top = k4t_larger(k4t_larger(x.x, x.y), k4t_larger(x.z, x.w));
+                        const int e = k4t_up(f16, __reduce_max_sync(((1u << LANES) - 1) << (lane / LANES * LANES), max(top >> 16, top & 0xffffu)));
+                        *at = k4t_halves(f16, x, e, A.scale);
+                        if (piece == 0) sh.factor[seg % SEGS][rho] = factor_of(e);
                     }
                 }
                 fence_proxy_async();
