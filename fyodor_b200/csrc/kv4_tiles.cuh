@@ -43,7 +43,7 @@ template <int HD, int NR> struct K4tShape {
     // raw tiles on their way: as many as there is room for
     static constexpr int KS = HD == 64 || Q_TM ? 4 : 2, VS = HD == 64 || Q_TM ? 4 : 1;
     static constexpr int HALF = 128 * 128, TILE = HD / 64 * HALF;            // fp16 rows of 64 values in 128 bytes
-    static constexpr int O_STRIDE = 20;                                      // floats between lanes of 16 columns of O of copies
+    static constexpr int O_COLS = 32, O_STRIDE = O_COLS + 4;                  // columns of O of copies at a time, floats between lanes of them
     static constexpr int OFF_K = 0, OFF_V = 2 * TILE, OFF_Q = 4 * TILE, OFF_RK = OFF_Q + (Q_TM ? 0 : 2 * TILE), OFF_RV = OFF_RK + KS * RAW,
                          OFF_O = OFF_RV + VS * RAW, STAGED = Q_TM ? 128 * O_STRIDE : 0, OFF_END = OFF_O + STAGED * 4;
     // tensor memory columns: two S with P in the upper half, O of each group, q
@@ -503,16 +503,17 @@ __global__ void __launch_bounds__(k4t_threads(NR), 1) kv4_tiles_kernel(const __g
                     if (!whole && (int)tid < nrows) A.part_ml[(size_t)of.slot * NR + tid] = make_float2(top, sum);
                 }
 #pragma unroll 1
-                for (unsigned c = 0; c < HD; c += 16) {
-                    float y[16];
-                    kt_ld16(o_at + c, y);
+                for (unsigned c = 0; c < HD; c += S::O_COLS) {
+                    float y[S::O_COLS];
+                    kt_ld32(o_at + c, y);
                     kt_wait_ld();
 #pragma unroll
-                    for (int i = 0; i < 16; i += 4)
+                    for (int i = 0; i < S::O_COLS; i += 4)
                         *reinterpret_cast<float4 *>(stage + tid * S::O_STRIDE + i) = make_float4(y[i] * own, y[i + 1] * own, y[i + 2] * own, y[i + 3] * own);
                     bar();
-                    for (unsigned i = tid; i < (unsigned)nrows * 2; i += 32 * SOFT) {
-                        const unsigned row = i >> 1, half = i & 1;
+#pragma unroll 1
+                    for (unsigned i = tid; i < (unsigned)nrows * (S::O_COLS / 8); i += 32 * SOFT) {
+                        const unsigned row = i / (S::O_COLS / 8), part = i % (S::O_COLS / 8);
                         float z[8];
 #pragma unroll
                         for (int j = 0; j < 8; ++j) z[j] = 0.f;
@@ -520,10 +521,10 @@ __global__ void __launch_bounds__(k4t_threads(NR), 1) kv4_tiles_kernel(const __g
                         for (unsigned p = 0; p < CP; ++p)
 #pragma unroll
                             for (int j = 0; j < 8; j += 4) {
-                                const float4 u = *reinterpret_cast<const float4 *>(stage + (p * NR + row) * S::O_STRIDE + 8 * half + j);
+                                const float4 u = *reinterpret_cast<const float4 *>(stage + (p * NR + row) * S::O_STRIDE + 8 * part + j);
                                 z[j] += u.x; z[j + 1] += u.y; z[j + 2] += u.z; z[j + 3] += u.w;
                             }
-                        leave(row, place_of(row), c / 8 + half, z);
+                        leave(row, place_of(row), c / 8 + part, z);
                     }
                     bar();
                 }
@@ -547,6 +548,7 @@ __global__ void __launch_bounds__(k4t_threads(NR), 1) kv4_tiles_kernel(const __g
     } else if (warp < W_TMA) {
         // ================================================== K or V, 4 bits to fp16 rows; q
         const bool f16 = A.type == T_F16, is_v = warp >= W_CONV + CONV;
+        const unsigned by_group = 65536 / GR + 1;  // rho times it: off by less than rho / 65536, so by less than 1 / GR
         const unsigned cw = (warp - W_CONV) % CONV, ct = cw * 32 + lane;
         constexpr unsigned TOKENS = K4_TILE / CONV;  // of a warp, eight lanes a token
         const unsigned j = lane & 7, tok0 = cw * TOKENS + (lane >> 3);
@@ -557,8 +559,10 @@ __global__ void __launch_bounds__(k4t_threads(NR), 1) kv4_tiles_kernel(const __g
                 // ---- q rows by a power of two each. The score factor's sign goes with q: a row's largest product is its
                 // largest score
                 const int j0 = s.row_tile * (int)A.row_tile, nrows = min((int)A.row_tile, s.q.rows - j0) * (int)GR;
+                const size_t q0 = (size_t)(s.q.first + j0) * A.q_stride + (size_t)s.head * GR * HD;
                 auto at_of = [&](unsigned rho) {
-                    return (size_t)(s.q.first + j0 + (int)(rho / GR)) * A.q_stride + (size_t)(s.head * GR + rho % GR) * HD;
+                    const unsigned j = rho * by_group >> 16;  // rho / GR
+                    return q0 + j * A.q_stride + (rho - j * GR) * HD;
                 };
                 // at least the smallest normal number: -inf times it stays -inf
                 auto factor_of = [&](int e) { return fmaxf(fabsf(A.scale) * kt_power(-e), 1.17549435e-38f); };
@@ -597,7 +601,7 @@ __global__ void __launch_bounds__(k4t_threads(NR), 1) kv4_tiles_kernel(const __g
                         return ring + S::OFF_Q + rho / 128 * S::TILE + piece / 8 * S::HALF + rho % 128 * 128 + ((piece % 8 ^ (rho & 7u)) << 4);
                     };
                     if (seg) wait(&sh.q_empty, seg - 1);  // the last segment's products have read their q
-#pragma unroll 1
+#pragma unroll 4
                     for (unsigned i = 0; i < STEPS; ++i) {
                         const unsigned rho = row0 + i * STEP;
                         uint4 *to = reinterpret_cast<uint4 *>(place(rho));
