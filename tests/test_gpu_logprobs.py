@@ -199,6 +199,15 @@ def test_outputs_left_out_and_refusals():
     F.logprobs(x[:0], i32([]), workspace=ws, **none)
 
 
+@pytest.mark.parametrize("rows,n,top", [(1, 140000, 3), (1, 300001, 8), (1, 300001, 9), (2, 200001, 32), (1, 2000000, 5)])
+def test_rows_of_many_ctas(rows, n, top):
+    """More than 32 CTAs hold a part of a row, with alternatives of both forms of the join; then a row whose largest
+    logits ascend to its end, so every batch holds new ones."""
+    x, t = some(rows, n, rows + n)
+    check(x, t, top)
+    check(x.sort(1).values, t, top)
+
+
 def test_streams_and_graph():
     """On another stream behind work of its own, twice at once with a workspace each, and captured."""
     x, t = some(16, 50000, 7)
