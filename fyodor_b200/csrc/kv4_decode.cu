@@ -7,22 +7,37 @@
 //   o_g   = sum_t (p_t scale_tg) n_tg + sum_t p_t low_tg
 //
 // so the tensor cores multiply the whole numbers n themselves, S^T = N Q^T and
-// O_g^T = N_g^T W_g^T with mma.sync m16n8k16: a masked word of the cache is already
-// a pair of fp16 operands, the subnormal n 2^-24 (or 16 n 2^-24 for the upper
+// O_g^T = (N_g - 8)^T W_g^T with mma.sync m16n8k16: a masked word of the cache is
+// already a pair of fp16 operands, the subnormal n 2^-22 (or 16 n 2^-22 for the upper
 // number of a byte, which q and the output take back), with nothing to convert.
 // Scales and lows meet the scores and the weights in F32.
+//
+// The tensor cores line products up by the operands' exponents, and a subnormal's
+// is 2^-14 whatever its size: the higher a number's bits lie, the fewer are lost.
+// Two bits further down (n 2^-24) a row of F32 of 257 tokens was 1.1e-5 off and not
+// 1.6e-6, for 3 us of 158 of a ragged batch; numbers made normal, by an addition each,
+// left 2.4e-7 and took 186. Values are taken as low + 8 scale + (n - 8) scale, the sums of
+// which stay as small as an output: sums of n and of low cancel, and the accumulators
+// round towards zero (ragged rows of up to 32768 3.5e-4 off, for 15 us). -8 is an MMA more
+// with the same weights; F32 rows of five and more, whose low halves share the
+// accumulators of the high ones, have V's numbers made normal, and 8 taken off with that.
 //
 // q and the weights are two fp16 halves, hi + lo, 22 bits: with up to four rows
 // the eight columns are the hi and lo halves of the rows, one MMA for both; with up
 // to eight they are the rows, with low halves in an MMA of their own for F32 rows.
-// Rows of 16 bits fit the high half, and their weights are rounded to it (2^-11,
-// below the output's own rounding).
+// Rows of 16 bits fit the high half, and at five rows and more their weights are
+// rounded to it (2^-12 each at the most, of no common sign).
+//
+// Bound by instructions: 16 at 8100 with eight rows takes 56 us for 22 of bytes (0.40
+// of the measured copy), 32 ragged requests of 128 to 32768 162 us for 99 (0.61). Three CTAs of four consumer warps and one for the copies
+// fit an SM at 128 registers (when they took 147 us two CTAs of eight took 175, four
+// of four, with fewer registers, 162).
 #include "kv4_attention.cuh"
 
 namespace fyb {
 
 // SHARE: groups of 16 positions of a tile that a warp takes
-constexpr int K4_COST = 3;  // a segment's beginning and end, in tiles
+constexpr int K4_COST = 3;  // a segment's beginning and end, in tiles (ragged 32 without them 147 us, with them 140, when it was measured)
 constexpr int K4_WARPS = 4, K4_SHARE = K4_TILE / 16 / K4_WARPS, K4_THREADS = 32 * (K4_WARPS + 1);
 
 // Words of shared memory: the address of a lane, and what is the same for all of them as the offset.
@@ -35,6 +50,21 @@ FYB_DEV unsigned pack2(float lo, float hi)  // fp16 pair
     return *reinterpret_cast<const unsigned *>(&p);
 }
 FYB_DEV float2 unpack2(unsigned p) { return __half22float2(*reinterpret_cast<const __half2 *>(&p)); }
+
+// The lower (upper) numbers of two bytes of a word, 16 bits apart, less 8: a number under the bits of 1024 (of 64) is that
+// much more, taken off exactly.
+FYB_DEV unsigned lower8(unsigned x)
+{
+    const unsigned y = (x & 0x000f000fu) | 0x64006400u;
+    const __half2 n = __hadd2(*reinterpret_cast<const __half2 *>(&y), __float2half2_rn(-1032.f));
+    return *reinterpret_cast<const unsigned *>(&n);
+}
+FYB_DEV unsigned upper8(unsigned x)
+{
+    const unsigned y = (x & 0x00f000f0u) | 0x54005400u;
+    const __half2 n = __hadd2(*reinterpret_cast<const __half2 *>(&y), __float2half2_rn(-72.f));
+    return *reinterpret_cast<const unsigned *>(&n);
+}
 
 template <int HD> struct K4Shape {
     static constexpr int ROW = HD / 2, SCALES = HD / 64 * 4;               // bytes of a token's row, of its scales
@@ -139,7 +169,13 @@ __global__ void __launch_bounds__(K4_THREADS, K4_CTAS) kv4_decode_kernel(const _
         return (at ^ (eights * (8 * S::ROW / 128) % 8 << 4)) + eights * 8 * S::ROW + tile;
     };
     const unsigned s_at = smem_u32(ring) + S::OFF_KS + (warp * K4_SHARE * 16 + tau) * S::SCALES;
-    constexpr float P_SCALE = 32.f;  // keeps small weights clear of fp16's smallest numbers; the largest is 2^14
+    // Weights are up to 2^LAG, and P_SCALE times themselves in fp16, so below 2^15. What both halves lose is 2^-25 of that at
+    // the most, 2^-38 of the largest weight: there are many of the smallest in a long row.
+    constexpr float LAG = 2.f, P_SCALE = 8192.f;
+    constexpr int FLUSH = 8;
+    constexpr bool SUMS = W == 1 || LO;
+    // -8 for each number, as they lie in the operands
+    const unsigned minus8[4] = {0x80208020u, 0x82008200u, 0x80208020u, 0x82008200u};
     auto bar = [] { asm volatile("bar.sync 1, %0;" :: "n"(32 * K4_WARPS) : "memory"); };
 
     while (walk.next(s)) {
@@ -229,7 +265,34 @@ __global__ void __launch_bounds__(K4_THREADS, K4_CTAS) kv4_decode_kernel(const _
             for (int h = 0; h < G; ++h) zero[w][h] = 0.f;
         }
 
-        for (int t = s.t0; t < s.t1; ++t) {
+        // The accumulators go to this thread's sums in shared memory: every FLUSH tiles, as they round towards zero (once a
+        // segment ragged 32 was 6.2e-6 off and not 3.7e-6, for 4 us of 162), at the end where rows are of 16 bits.
+        auto sum_of = [&](int h, int k, int w) {
+            return reinterpret_cast<float2 *>(o_s + (warp * R + W * t4 + w) * HD + 64 * h + 8 * g + 2 * k);
+        };
+        auto flush = [&](bool first) {
+            const float back = vexp < -126 ? 0.f : power_of_two(vexp) * ((LO ? 1.f : 4194304.f) / P_SCALE), back16 = LO ? back : back * 0.0625f;
+#pragma unroll
+            for (int h = 0; h < G; ++h)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    float (&a)[4] = acc[h][k];
+#pragma unroll
+                    for (int w = 0; w < W; ++w) {
+                        const float even = W == 1 ? a[0] + a[1] : a[w], odd = W == 1 ? a[2] + a[3] : a[2 + w];
+                        float2 *o = sum_of(h, k, w);
+                        const float2 y = first ? make_float2(0.f, 0.f) : *o;
+                        *o = make_float2(fmaf(even, back, y.x), fmaf(odd, back16, y.y));
+                    }
+                    a[0] = a[1] = a[2] = a[3] = 0.f;
+                }
+        };
+        if (SUMS) flush(true);
+        for (int t = s.t0, left = FLUSH; t < s.t1; ++t, --left) {
+            if (SUMS && left == 0) {
+                flush(false);
+                left = FLUSH;
+            }
             wait(full + stage, phase);
             const unsigned tile = stage * S::STAGE;
             const unsigned loaded = here[stage];
@@ -252,8 +315,8 @@ __global__ void __launch_bounds__(K4_THREADS, K4_CTAS) kv4_decode_kernel(const _
                     for (int i = 0; i < NW; ++i) {
 #pragma unroll
                         for (int j = 0; j < 2; ++j) {
-                            const unsigned x = ka[i] >> (8 * j), y = kb[i] >> (8 * j);
-                            const unsigned a[4] = {x & 0x000f000fu, y & 0x000f000fu, x & 0x00f000f0u, y & 0x00f000f0u};
+                            const unsigned x = j ? ka[i] >> 6 : ka[i] * 4, y = j ? kb[i] >> 6 : kb[i] * 4;
+                            const unsigned a[4] = {x & 0x003c003cu, y & 0x003c003cu, x & 0x03c003c0u, y & 0x03c003c0u};
                             mma_f16(c[u][i % G], a, qh[2 * i + j][0], qh[2 * i + j][1]);
                             if constexpr (LO) mma_f16(c[u][i % G], a, ql[2 * i + j][0], ql[2 * i + j][1]);
                         }
@@ -272,6 +335,7 @@ __global__ void __launch_bounds__(K4_THREADS, K4_CTAS) kv4_decode_kernel(const _
                         for (int i = 0; i < G; ++i) {
                             ks[u][h][i] = __half22float2(*reinterpret_cast<const __half2 *>(&kw[i]));
                             vs[u][h][i] = __half22float2(*reinterpret_cast<const __half2 *>(&vw[i]));
+                            vs[u][h][i].y = fmaf(8.f, vs[u][h][i].x, vs[u][h][i].y);  // the value of n = 8
                         }
                     }
                 float x[J][2][W];  // [group of 16][position tau, tau + 8][row], in units of log2
@@ -288,7 +352,7 @@ __global__ void __launch_bounds__(K4_THREADS, K4_CTAS) kv4_decode_kernel(const _
                                 dot = fmaf(n, ks[u][h][i].x, dot);
                                 low = fmaf(ks[u][h][i].y, fq[w][i], low);
                             }
-                            x[u][h][w] = fmaf(dot * 16777216.f, fn[w], low);  // n was 2^24 too small
+                            x[u][h][w] = fmaf(dot * 4194304.f, fn[w], low);  // n was 2^22 too small
                         }
                 if (first + 16 * J > all || use != (1u << J) - 1) {
 #pragma unroll
@@ -306,22 +370,22 @@ __global__ void __launch_bounds__(K4_THREADS, K4_CTAS) kv4_decode_kernel(const _
                             }
                         }
                 }
-                // ---- running maximum: moved only when a score is 2^8 above it. Their difference says so: it is exact
-                // where they are near, and m + 8 is not (from 2^27 on it can round to m + 16, a weight of 2^16)
+                // ---- running maximum: moved only when a weight is 2^LAG. The scores' difference says so: it is exact where
+                // they are near, and m + LAG is not (from 2^25 on it can round to m + 4, a weight of 2^4)
                 bool over = false;
                 float top[W];
 #pragma unroll
                 for (int w = 0; w < W; ++w) {
                     top[w] = fmaxf(x[0][0][w], x[0][1][w]);
                     if constexpr (J == 2) top[w] = fmaxf(top[w], fmaxf(x[J - 1][0][w], x[J - 1][1][w]));
-                    over = over || top[w] - m[w] > 8.f;
+                    over = over || top[w] - m[w] > LAG;
                 }
                 if (__any_sync(0xffffffffu, over)) {
 #pragma unroll
                     for (int w = 0; w < W; ++w) {
 #pragma unroll
                         for (int o = 4; o < 32; o <<= 1) top[w] = fmaxf(top[w], __shfl_xor_sync(0xffffffffu, top[w], o));
-                        if (top[w] - m[w] > 8.f) {  // each row by its own scores: the same on all lanes that hold it
+                        if (top[w] - m[w] > LAG) {  // each row by its own scores: the same on all lanes that hold it
                             const float alpha = ex2(m[w] - top[w]);
                             m[w] = top[w];
                             l[w] *= alpha;
@@ -330,6 +394,10 @@ __global__ void __launch_bounds__(K4_THREADS, K4_CTAS) kv4_decode_kernel(const _
                                 zero[w][h] *= alpha;
 #pragma unroll
                                 for (int k = 0; k < 4; ++k) {
+                                    if (SUMS) {
+                                        float2 *o = sum_of(h, k, w);
+                                        *o = make_float2(o->x * alpha, o->y * alpha);
+                                    }
                                     if constexpr (W == 1) { acc[h][k][0] *= alpha; acc[h][k][1] *= alpha; acc[h][k][2] *= alpha; acc[h][k][3] *= alpha; }
                                     else { acc[h][k][w] *= alpha; acc[h][k][2 + w] *= alpha; }
                                 }
@@ -410,10 +478,18 @@ __global__ void __launch_bounds__(K4_THREADS, K4_CTAS) kv4_decode_kernel(const _
                             const unsigned cd = __byte_perm(v[2][i], v[3][i], half ? 0x7632 : 0x5410);
 #pragma unroll
                             for (int j = 0; j < 2; ++j) {
-                                const unsigned y = ab >> (8 * j), z = cd >> (8 * j);
-                                const unsigned a[4] = {y & 0x000f000fu, y & 0x00f000f0u, z & 0x000f000fu, z & 0x00f000f0u};
-                                mma_f16(acc[i][2 * half + j], a, b[i][0], b[i][1]);
-                                if constexpr (LO) mma_f16(acc[i][2 * half + j], a, bl[i][0], bl[i][1]);
+                                float (&o)[4] = acc[i][2 * half + j];
+                                if constexpr (LO) {
+                                    const unsigned y = ab >> (8 * j), z = cd >> (8 * j);
+                                    const unsigned a[4] = {lower8(y), upper8(y), lower8(z), upper8(z)};
+                                    mma_f16(o, a, b[i][0], b[i][1]);
+                                    mma_f16(o, a, bl[i][0], bl[i][1]);
+                                } else {
+                                    const unsigned y = j ? ab >> 6 : ab * 4, z = j ? cd >> 6 : cd * 4;
+                                    const unsigned a[4] = {y & 0x003c003cu, y & 0x03c003c0u, z & 0x003c003cu, z & 0x03c003c0u};
+                                    mma_f16(o, minus8, b[i][0], b[i][1]);
+                                    mma_f16(o, a, b[i][0], b[i][1]);
+                                }
                             }
                         }
                 }
@@ -423,7 +499,7 @@ __global__ void __launch_bounds__(K4_THREADS, K4_CTAS) kv4_decode_kernel(const _
             advance();
         }
         // ---- the warps' parts: sums over the lanes of a row, then over the warps
-        const float back = vexp < -126 ? 0.f : power_of_two(vexp) * (16777216.f / P_SCALE);
+        flush(!SUMS);
 #pragma unroll
         for (int w = 0; w < W; ++w) {
 #pragma unroll
@@ -440,10 +516,8 @@ __global__ void __launch_bounds__(K4_THREADS, K4_CTAS) kv4_decode_kernel(const _
             for (int k = 0; k < 4; ++k)
 #pragma unroll
                 for (int w = 0; w < W; ++w) {
-                    const float even = W == 1 ? acc[h][k][0] + acc[h][k][1] : acc[h][k][w];
-                    const float odd = W == 1 ? acc[h][k][2] + acc[h][k][3] : acc[h][k][2 + w];
-                    *reinterpret_cast<float2 *>(o_s + (warp * R + W * t4 + w) * HD + 64 * h + 8 * g + 2 * k) =
-                        make_float2(fmaf(even, back, zero[w][h]), fmaf(odd, back * 0.0625f, zero[w][h]));
+                    float2 *o = sum_of(h, k, w);
+                    *o = make_float2(o->x + zero[w][h], o->y + zero[w][h]);
                 }
         bar();
         kv8_join_warps<R, HD, K4_WARPS>(tid, ml_s, o_s, bar);

@@ -13,16 +13,29 @@
 // is a fifteenth of its group's range), in the order of a word's numbers: 0 4 1 5
 // 2 6 3 7. q lies in the same order, the output is put back.
 //
-// P lies in the upper half of its S. Row tiles of 256 rows (prompt chunks) are two
-// groups of 128 lanes, each with four softmax warps, S and O of its own, over the
-// same K and V: a tile is converted once for both, and one group's products run while
-// the other's weights are made. Row tiles of 64 or 32 rows (drafts): one group, whose
-// lanes hold two or four copies of the rows; copy c takes the positions of its part of
-// a tile, its P being 0 elsewhere: every thread has positions to do, and what the
-// copies hold is joined like any parts. One O leaves room for S of two tiles and for q
-// in tensor memory, which saves its reads and its place in shared memory.
+// Row tiles of 256 rows (prompt chunks) are two groups of 128 lanes, each with four
+// softmax warps, S and O of its own, over the same K and V: a tile is converted once for
+// both. A group makes and hands on the weights of half a tile at a time, P in the place
+// of scores that have been read, and the groups are half a tile apart, so one group's
+// products run while the other's weights are made. Row tiles of 64 or 32 rows (drafts):
+// one group, whose lanes hold two or four copies of the rows; copy c takes the positions
+// of its part of a tile, its P (in the upper half of S) being 0 elsewhere: every thread
+// has positions to do, and what the copies hold is joined like any parts. One O leaves
+// room for S of two tiles and for q in tensor memory, which saves its reads and its
+// place in shared memory.
 //
-// The maximum m of a row moves only when a score is more than 2^8 above it.
+// Bound, at 256 rows, by the chain of a half tile's products and weights: a tile of 128
+// positions takes 4200 cycles, of which its products alone would take 2050 and its
+// exponentials 2050; a chunk of 500 rows of four heads at 16000 160 us (805 TFLOP/s,
+// 0.49 of the measured rate; weights of a whole tile at a time 205, products of 64 columns for
+// the half tiles 259, since K is then read twice as often). At 32 rows by the products of
+// full 128-lane tiles, 1250 of a tile's 1820 cycles, and the MMA warp's waits: 32 ragged
+// drafts of eight rows of four heads 245 us, 0.38 of the measured copy. What runs once a
+// segment costs as much as 8 tiles (6 of 256 rows), and its instructions more than its
+// data.
+//
+// The maximum m of a row moves only when a weight is above 2^8 (with 2^4 a chunk of 500
+// at 16000 took 170 us, with 2^8 160).
 #pragma once
 #include "kv4_attention.cuh"
 #include "kt_mma.cuh"
@@ -34,7 +47,8 @@ FYB_HOST_DEV constexpr unsigned k4t_segs(int NR) { return NR == 256 ? 2 : 4; }  
 FYB_HOST_DEV constexpr int k4t_groups(int NR) { return NR == 256 ? 2 : 1; }      // groups of four softmax warps
 FYB_HOST_DEV constexpr int k4t_threads(int NR) { return 32 * (4 * k4t_groups(NR) + 2 * K4T_CONV + 3); }
 
-FYB_HOST_DEV constexpr int k4t_cost(int NR) { return NR == 256 ? 6 : 8; }        // a segment's beginning and end, in tiles
+// A segment's beginning and end, in tiles (drafts as above: with 4 tiles 266 us, 6 259, 8 242, 10 243; the chunk with 9 181, 6 174, 3 176)
+FYB_HOST_DEV constexpr int k4t_cost(int NR) { return NR == 256 ? 6 : 8; }
 
 template <int HD, int NR> struct K4tShape {
     static constexpr int ROW = HD / 2, SCALES = HD / 64 * 4;                 // bytes of a token's row, of its scales
@@ -342,7 +356,7 @@ __global__ void __launch_bounds__(k4t_threads(NR), 1) kv4_tiles_kernel(const __g
         unsigned k = 0;  // tiles of this group so far
         bool goes_on = false;  // the last segment, in the next CTA
         auto bar = [] { asm volatile("bar.sync 1, %0;" :: "n"(32 * SOFT) : "memory"); };
-        constexpr float P_UP = 6.f;  // weights are 2^6 times themselves, clear of fp16's smallest numbers; the largest is 2^14
+        constexpr float LAG = 8.f, P_UP = 6.f;  // weights are 2^P_UP times themselves, clear of fp16's smallest numbers, and up to 2^14
         while (const Kv8Segment *sp = next()) {
             const Kv8Segment &s = *sp;
             const int t0 = s.t0, t1 = s.t1, j0 = s.row_tile * (int)A.row_tile;
@@ -393,7 +407,7 @@ __global__ void __launch_bounds__(k4t_threads(NR), 1) kv4_tiles_kernel(const __g
 #pragma unroll
                         for (int i = 0; i < 32; i += 2) tops[i / 2 % 4] = fmaxf(tops[i / 2 % 4], fmaxf(x[c][i], x[c][i + 1]));
                     const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])) * f;
-                    const bool up = top - m > 8.f + P_UP;
+                    const bool up = top - m > LAG + P_UP;
                     if (__any_sync(0xffffffffu, up)) {
                         // ---- new maxima, and the sums so far in their units
                         const float now = up ? top - P_UP : m, alpha = up ? ex2(m - now) : 1.f;

@@ -466,6 +466,28 @@ def test_long_tail_of_small_weights():
         assert np.abs(out.cpu().numpy()[:, 0] / want[:, None] - 1).max() <= n * 2.0 ** -23 + 2 * 16 * (hd + 16) * 2.0 ** -24
 
 
+@pytest.mark.parametrize("n", [257, 4000, 30000])
+@pytest.mark.parametrize("heads", [2, 8, 16, 40])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_outputs_far_smaller_than_the_values(n, heads, hd):
+    """Values of either sign and nearly equal weights: an output is some 1 / sqrt(n) of a value.
+
+    Tolerance: the tensor cores line 16 products w (m 2^-22), m < 16 or 16 m, up at the exponent 2^-14 of a subnormal
+    operand and round 24 bits below it towards zero: by up to 2^-38 w, 2^-16 w of a step of the cache, half of that in the
+    mean, once for 16 positions, so 2^-21 of the sum of w. An output has the norm of sqrt(n) w values of 15 / sqrt(12)
+    steps, n w of the sum of w: 2^-21 sqrt(n) / 4.3 of it. Weights, scores and the rest: 2^-20."""
+    g = torch.Generator(device="cuda").manual_seed(n + heads)
+    blocks = -(-n // 64)
+    cache = F.KV4Cache.empty(blocks, 2, 64, hd)
+    k, v = (torch.randn((n, 2, hd), generator=g, device="cuda") for _ in "kv")
+    cache.append(k, v, i32(range(n)))
+    q = torch.randn((1, heads, hd), generator=g, device="cuda")
+    out, table = torch.empty_like(q), np.arange(blocks, dtype=np.int32)[None]
+    cache.attention(q, i32([n]), i32(table), out, cache.attention_workspace(1, 1, heads), scale=0.02)
+    want, _, _ = reference(cache, table, [n], [0, 1], q, 0.02, "f32")
+    assert (out.cpu().double() - want).norm() <= (2.0 ** -21 * n ** 0.5 / 4.3 + 2.0 ** -20) * want.norm()
+
+
 @pytest.mark.parametrize("most", [1, 20])
 def test_bad_tables_and_lengths(most):
     """Blocks outside the pool and lengths beyond the table are left out and raise the error word; other requests
