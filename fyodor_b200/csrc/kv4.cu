@@ -9,7 +9,7 @@
 // find by shuffles.
 //
 // A step's append is one launch, 4 us. Prompts: 6093 rows of 32 / 8 heads of 128, bf16,
-// take 16 us for K and V (31 MB: instructions, some 200 a warp for 512 values), 23 for
+// take 16 us for K and V (31 MB: instructions, some 430 a warp for 512 values), 23 for
 // q's rotation (0.67 of the measured copy; in one launch with K and V 55 us together
 // instead of 39, so q goes along only with few rows, where a launch more would count)
 // and 12 to be read back in F32 (0.79).
