@@ -4,9 +4,9 @@
 // Up to eight query rows per KV head (rows of a request x heads of a group), and
 // rows of F32 whatever their number, run on kv4_decode.cu, many rows in row tiles of
 // eight; many rows of 16 bits on kv4_tiles.cuh, in row tiles of 32, 64 or 256. With 8
-// rows 32 ragged requests take 64 us there and 99 in tiles; with 16 rows, two row
-// tiles, 112 and 100, 16 requests at 8100 82 and 75, with 32 rows 149 and 77 (what is
-// short is still quicker: four requests of 500 with 16 rows 12 us and 18).
+// rows 32 ragged requests take 71 us there and 97 in tiles; with 16 rows, two row
+// tiles, 126 and 97, 16 requests at 8100 92 and 72, with 32 rows 167 and 74 (what is
+// short is still as quick: four requests of 500 with 16 rows 13 us and 15).
 #include "kv4_attention.cuh"
 
 namespace fyb {

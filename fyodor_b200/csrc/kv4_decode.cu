@@ -7,7 +7,7 @@
 //   o_g   = sum_t (p_t scale_tg) n_tg + sum_t p_t low_tg
 //
 // so the tensor cores multiply the whole numbers n themselves, S^T = N Q^T and
-// O_g^T = (N_g - 8)^T W_g^T with mma.sync m16n8k16: a masked word of the cache is
+// O_g^T = N_g^T W_g^T with mma.sync m16n8k16: a masked word of the cache is
 // already a pair of fp16 operands, the subnormal n 2^-22 (or 16 n 2^-22 for the upper
 // number of a byte, which q and the output take back), with nothing to convert.
 // Scales and lows meet the scores and the weights in F32.
@@ -15,12 +15,15 @@
 // The tensor cores line products up by the operands' exponents, and a subnormal's
 // is 2^-14 whatever its size: the higher a number's bits lie, the fewer are lost.
 // Two bits further down (n 2^-24) a row of F32 of 257 tokens was 1.1e-5 off and not
-// 1.6e-6, for 3 us of 158 of a ragged batch; numbers made normal, by an addition each,
-// left 2.4e-7 and took 186. Values are taken as low + 8 scale + (n - 8) scale, the sums of
-// which stay as small as an output: sums of n and of low cancel, and the accumulators
-// round towards zero (ragged rows of up to 32768 3.5e-4 off, for 15 us). -8 is an MMA more
-// with the same weights; F32 rows of five and more, whose low halves share the
-// accumulators of the high ones, have V's numbers made normal, and 8 taken off with that.
+// 1.6e-6, for 3 us of a ragged batch; numbers made normal, by an addition each, left
+// 2.4e-7 and took 28. Sums of n are far larger than an output, and the accumulators round
+// towards zero (a row of 30000 is 3.5e-4 off). So V's numbers count up from low in one
+// group of 16 positions and down from the highest, with negative weights, in the next (the
+// complement is part of the mask); -8 times the weights, by an MMA more each, took 15 us of
+// a ragged batch. Five rows and more take that one nevertheless: their weights are
+// rounded to one half, an error that goes with the numbers' size (fp16 rows at 8100:
+// 2.8e-4 off and not 5.1e-4, for 4 us of 59). F32 rows of five and more, whose low halves
+// share the accumulators of the high ones, have V's numbers made normal, less 8.
 //
 // q and the weights are two fp16 halves, hi + lo, 22 bits: with up to four rows
 // the eight columns are the hi and lo halves of the rows, one MMA for both; with up
@@ -28,8 +31,8 @@
 // Rows of 16 bits fit the high half, and at five rows and more their weights are
 // rounded to it (2^-12 each at the most, of no common sign).
 //
-// Bound by instructions: 16 at 8100 with eight rows takes 56 us for 22 of bytes (0.40
-// of the measured copy), 32 ragged requests of 128 to 32768 162 us for 99 (0.61). Three CTAs of four consumer warps and one for the copies
+// Bound by instructions: 16 at 8100 with eight rows takes 59 us for 22 of bytes (0.38
+// of the measured copy), 32 ragged requests of 128 to 32768 150 us for 99 (0.66). Three CTAs of four consumer warps and one for the copies
 // fit an SM at 128 registers (when they took 147 us two CTAs of eight took 175, four
 // of four, with fewer registers, 162).
 #include "kv4_attention.cuh"
@@ -173,9 +176,8 @@ __global__ void __launch_bounds__(K4_THREADS, K4_CTAS) kv4_decode_kernel(const _
     // the most, 2^-38 of the largest weight: there are many of the smallest in a long row.
     constexpr float LAG = 2.f, P_SCALE = 8192.f;
     constexpr int FLUSH = 8;
+    const unsigned minus8[4] = {0x80208020u, 0x82008200u, 0x80208020u, 0x82008200u};  // as numbers lie in the operands
     constexpr bool SUMS = W == 1 || LO;
-    // -8 for each number, as they lie in the operands
-    const unsigned minus8[4] = {0x80208020u, 0x82008200u, 0x80208020u, 0x82008200u};
     auto bar = [] { asm volatile("bar.sync 1, %0;" :: "n"(32 * K4_WARPS) : "memory"); };
 
     while (walk.next(s)) {
@@ -266,7 +268,7 @@ __global__ void __launch_bounds__(K4_THREADS, K4_CTAS) kv4_decode_kernel(const _
         }
 
         // The accumulators go to this thread's sums in shared memory: every FLUSH tiles, as they round towards zero (once a
-        // segment ragged 32 was 6.2e-6 off and not 3.7e-6, for 4 us of 162), at the end where rows are of 16 bits.
+        // segment ragged 32 was 6.2e-6 off when it was 3.7e-6 so, for 4 us of 162), at the end where rows are of 16 bits.
         auto sum_of = [&](int h, int k, int w) {
             return reinterpret_cast<float2 *>(o_s + (warp * R + W * t4 + w) * HD + 64 * h + 8 * g + 2 * k);
         };
@@ -302,6 +304,9 @@ __global__ void __launch_bounds__(K4_THREADS, K4_CTAS) kv4_decode_kernel(const _
                 const unsigned in_tile = (warp * K4_SHARE + (unsigned)u0) * 16, use = loaded >> (in_tile / 16) & ((1u << J) - 1);
                 const int first = t * K4_TILE + (int)in_tile;
                 if (first >= any || !use) continue;
+                // up to four rows: every other 16 positions count down from 15, with negative weights; else from 8
+                auto down = [](int u) { return W == 1 && u == 1; };
+                auto base = [&](int u) { return W == 2 ? 8.f : down(u) ? 15.f : 0.f; };
                 // ---- scores
                 float c[J][G][4];
 #pragma unroll
@@ -335,7 +340,7 @@ __global__ void __launch_bounds__(K4_THREADS, K4_CTAS) kv4_decode_kernel(const _
                         for (int i = 0; i < G; ++i) {
                             ks[u][h][i] = __half22float2(*reinterpret_cast<const __half2 *>(&kw[i]));
                             vs[u][h][i] = __half22float2(*reinterpret_cast<const __half2 *>(&vw[i]));
-                            vs[u][h][i].y = fmaf(8.f, vs[u][h][i].x, vs[u][h][i].y);  // the value of n = 8
+                            vs[u][h][i].y = fmaf(base(u), vs[u][h][i].x, vs[u][h][i].y);  // the value of that number
                         }
                     }
                 float x[J][2][W];  // [group of 16][position tau, tau + 8][row], in units of log2
@@ -441,7 +446,7 @@ __global__ void __launch_bounds__(K4_THREADS, K4_CTAS) kv4_decode_kernel(const _
                         float wt[2][W];
 #pragma unroll
                         for (int h = 0; h < 2; ++h) {
-                            const float unit = vs[u][h][i].x * vref;
+                            const float unit = vs[u][h][i].x * (down(u) ? -vref : vref);
 #pragma unroll
                             for (int w = 0; w < W; ++w) {
                                 zero[w][i] = fmaf(p[h][w], vs[u][h][i].y, zero[w][i]);
@@ -485,9 +490,9 @@ __global__ void __launch_bounds__(K4_THREADS, K4_CTAS) kv4_decode_kernel(const _
                                     mma_f16(o, a, b[i][0], b[i][1]);
                                     mma_f16(o, a, bl[i][0], bl[i][1]);
                                 } else {
-                                    const unsigned y = j ? ab >> 6 : ab * 4, z = j ? cd >> 6 : cd * 4;
-                                    const unsigned a[4] = {y & 0x003c003cu, y & 0x03c003c0u, z & 0x003c003cu, z & 0x03c003c0u};
-                                    mma_f16(o, minus8, b[i][0], b[i][1]);
+                                    const unsigned y = j ? ab >> 6 : ab * 4, z = j ? cd >> 6 : cd * 4, turn = down(u) ? ~0u : 0u;
+                                    const unsigned a[4] = {(y ^ turn) & 0x003c003cu, (y ^ turn) & 0x03c003c0u, (z ^ turn) & 0x003c003cu, (z ^ turn) & 0x03c003c0u};
+                                    if constexpr (W == 2) mma_f16(o, minus8, b[i][0], b[i][1]);
                                     mma_f16(o, a, b[i][0], b[i][1]);
                                 }
                             }
