@@ -28,7 +28,7 @@
 // positions takes 4200 cycles, of which its products alone would take 2050 and its
 // exponentials 2050; a chunk of 500 rows of four heads at 16000 160 us (805 TFLOP/s,
 // 0.49 of the measured rate; weights of a whole tile at a time 205, products of 64 columns for
-// the half tiles 259, since K is then read twice as often). At 32 rows by the products of
+// the half tiles 259, since q is then read twice as often). At 32 rows by the products of
 // full 128-lane tiles, 1250 of a tile's 1820 cycles, and the MMA warp's waits: 32 ragged
 // drafts of eight rows of four heads 245 us, 0.38 of the measured copy. What runs once a
 // segment costs as much as 8 tiles (6 of 256 rows), and its instructions more than its
