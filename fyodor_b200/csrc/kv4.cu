@@ -238,12 +238,14 @@ template <typename T, int HD, bool Q> __global__ void __launch_bounds__(KV4_THRE
     if (slot < 0) return;
     if (bad) raise_error(A.error, ERR_NONFINITE);
     if (low > high) low = high = 0.f;  // nothing finite
-    const bool wide = bad || low < -KV4_MOST || high > KV4_MOST;
     const __half lo = __float2half_rn(fminf(fmaxf(low, -KV4_MOST), KV4_MOST));
     const __half hi = __float2half_rn(fminf(fmaxf(high, -KV4_MOST), KV4_MOST));
     const float lf = __half2float(lo);
     const __half sc = __float2half_rn(fifteenth(__fsub_rn(__half2float(hi), lf)));
     const float sf = __half2float(sc), inv = rcp_approx(sf);  // scale 0: no number is certain
+    // Low and high as F16, and scale, need not enclose the group (a range of a few steps of F16, a scale below its normal
+    // numbers, values beyond KV4_MOST): where a quotient can leave 0..15 the values go one by one, which clamps.
+    const bool wide = bad || !(__fmul_rn(__fsub_rn(low, lf), inv) >= -0.49f && __fmul_rn(__fsub_rn(high, lf), inv) <= 15.49f);
     const size_t at = (((size_t)(slot >> A.shift) * A.c.kv_heads + head) << A.shift) + ((unsigned)slot & ((1u << A.shift) - 1));
     unsigned *words = static_cast<unsigned *>(is_k ? A.c.k : A.c.v) + at * WORDS + lane % PART * (KV4_EACH / 8) * GROUPS + group;
     // Four numbers at a time as one of 16 bits. A quotient that is no nearer than 1e-5 to a border is certain; the others
