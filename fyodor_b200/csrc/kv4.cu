@@ -143,6 +143,22 @@ FYB_DEV float fifteenth(float x)
     const float q = x * r;
     return fmaf(fmaf(-15.f, q, x), r, q);
 }
+// (high - low) / 15 of two halves as a real number, rounded to F16 once. In F32 the difference and the quotient are off by
+// 2^-23 of it together, which matters only next to a border between two normal halves (of subnormal ones differences are
+// exact, and quotients no nearer to a border than a thirtieth of a step): there 15 borders and the difference, exact in 64
+// bits, are compared.
+static __device__ __noinline__ __half kv4_scale_at(float q, float low, float high)
+{
+    const __half a = __float2half_rd(q), b = __float2half_ru(q);
+    const double border = 7.5 * ((double)__half2float(a) + (double)__half2float(b)), d = (double)high - (double)low;
+    return d > border || (d == border && (__half_as_ushort(a) & 1)) ? b : a;
+}
+FYB_DEV __half kv4_scale(float low, float high)
+{
+    const float q = fifteenth(__fsub_rn(high, low));
+    if (__builtin_expect((__float_as_uint(q) & 0x1fffu) - 0xffeu <= 4u, 0)) return kv4_scale_at(q, low, high);
+    return __float2half_rn(q);
+}
 FYB_DEV float rcp_approx(float x)  // within 2^-23 of it
 {
     float y;
@@ -241,7 +257,7 @@ template <typename T, int HD, bool Q> __global__ void __launch_bounds__(KV4_THRE
     const __half lo = __float2half_rn(fminf(fmaxf(low, -KV4_MOST), KV4_MOST));
     const __half hi = __float2half_rn(fminf(fmaxf(high, -KV4_MOST), KV4_MOST));
     const float lf = __half2float(lo);
-    const __half sc = __float2half_rn(fifteenth(__fsub_rn(__half2float(hi), lf)));
+    const __half sc = kv4_scale(lf, __half2float(hi));
     const float sf = __half2float(sc), inv = rcp_approx(sf);  // scale 0: no number is certain
     // Low and high as F16, and scale, need not enclose the group (a range of a few steps of F16, a scale below its normal
     // numbers, values beyond KV4_MOST): where a quotient can leave 0..15 the values go one by one, which clamps.
