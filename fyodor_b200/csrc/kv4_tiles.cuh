@@ -357,6 +357,7 @@ __global__ void __launch_bounds__(k4t_threads(NR), 1) kv4_tiles_kernel(const __g
         bool goes_on = false;  // the last segment, in the next CTA
         auto bar = [] { asm volatile("bar.sync 1, %0;" :: "n"(32 * SOFT) : "memory"); };
         constexpr float LAG = 8.f, P_UP = 6.f;  // weights are 2^P_UP times themselves, clear of fp16's smallest numbers, and up to 2^14
+        constexpr unsigned FAR = 0x4b800000u;  // bits of 2^24
         while (const Kv8Segment *sp = next()) {
             const Kv8Segment &s = *sp;
             const int t0 = s.t0, t1 = s.t1, j0 = s.row_tile * (int)A.row_tile;
@@ -407,8 +408,28 @@ __global__ void __launch_bounds__(k4t_threads(NR), 1) kv4_tiles_kernel(const __g
 #pragma unroll
                         for (int i = 0; i < 32; i += 2) tops[i / 2 % 4] = fmaxf(tops[i / 2 % 4], fmaxf(x[c][i], x[c][i + 1]));
                     const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])) * f;
-                    const bool up = top - m > LAG + P_UP;
-                    if (__any_sync(0xffffffffu, up)) {
+                    float fx = f;
+                    const bool up = top - m > LAG + P_UP, far = (__float_as_uint(top) & 0x7fffffffu) - FAR < 0x7f800000u - FAR;
+                    if (__any_sync(0xffffffffu, up || far)) {
+                        if (__any_sync(0xffffffffu, far)) {
+                            // rows of scores so large that m is off by a half and more of a unit: their products are rounded as
+                            // m is, or a weight's exponent could be beyond fp16's (at 2^28 by half of 32)
+                            const float times = far ? f : 1.f;
+#pragma unroll 1
+                            for (unsigned c = 0; c < CW; c += 16) {
+                                float y[16];
+                                kt_ld16(s_at + c, y);
+                                kt_wait_ld();
+#pragma unroll
+                                for (int i = 0; i < 16; ++i) y[i] *= times;
+                                kt_st16(s_at + c, y);
+                            }
+                            kt_wait_st();
+#pragma unroll
+                            for (unsigned c = 0; c < CHUNKS; ++c) kt_ld32(s_at + 32 * c, x[c]);
+                            kt_wait_ld();
+                            if (far) fx = 1.f;
+                        }
                         // ---- new maxima, and the sums so far in their units
                         const float now = up ? top - P_UP : m, alpha = up ? ex2(m - now) : 1.f;
                         m = now;
@@ -429,7 +450,7 @@ __global__ void __launch_bounds__(k4t_threads(NR), 1) kv4_tiles_kernel(const __g
                         }
                     }
                     // ---- weights: P takes the place of scores that have been read
-                    const F2 f2x = f2(f, f), mx = f2(-m, -m);
+                    const F2 f2x = f2(fx, fx), mx = f2(-m, -m);
                     F2 sums[2] = {f2(0.f, 0.f), f2(0.f, 0.f)};
                     if constexpr (CP > 1) {  // 0 for the positions of the other copies
                         float z[16];
