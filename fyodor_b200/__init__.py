@@ -501,7 +501,8 @@ def logprobs(logits, tokens, logprob, entropy, rank, top_tokens, top_logprobs, w
     tokens[row], entropy, and the most probable tokens with their log
     probabilities (fyb_logprobs). tokens and rank int32, logprob and entropy
     float32 [rows]; top_tokens int32 and top_logprobs float32 [rows][top]; any
-    output may be None (tokens with logprob and rank)."""
+    output may be None (tokens with logprob and rank, top_tokens with
+    top_logprobs)."""
     (_native or _bind_tensors()).logprobs(logits, tokens, logprob, entropy, rank, top_tokens, top_logprobs, workspace, error,
                                      stream)
 

@@ -342,6 +342,10 @@ PyObject *logprobs(PyObject *, PyObject *const *a, Py_ssize_t n)
             if (t.dim() != 2 || t.size(0) != rows || t.size(1) > 0x7fffffff) refuse("top_tokens", "has to be [rows][top]");
             top = t.size(1);
         }
+        if (a[6] != Py_None) {  // not without tokens, nor of another width: it would be left, or filled in other places
+            const at::Tensor &t = c.tensor(a[6], "top_logprobs");
+            if ((t.dim() == 2 && t.size(1) != top) || (!top && t.numel())) refuse("top_logprobs", "has to be [rows][top], with top_tokens");
+        }
         const at::Tensor &ws = c.tensor(a[7], "workspace");
         if (!ws.is_contiguous()) refuse("workspace", "has to be contiguous");
         return answer(entry.logprobs(type_of(x.scalar_type(), "logits"), x.data_ptr(), (size_t)stride, (size_t)rows,
