@@ -10,6 +10,9 @@
 
 namespace fyb {
 
+// Whether some of these addresses (NULL ones aside) lie off a whole element of `width` bytes.
+template <typename... P> bool off_element(size_t width, const P *...p) { return ((uintptr_t(p) | ... | 0) & (width - 1)) != 0; }
+
 // ---------------------------------------------------------------- generic.cu
 int launch_dequant(const void *w, unsigned type, size_t count, float *out, cudaStream_t s);
 int launch_generic_matmul(const void *w, size_t row_bytes, size_t rows, size_t cols, unsigned type,

@@ -369,7 +369,7 @@ extern "C" int fyb_kv4_append(const fyb_kv4_cache *cache, const int32_t *slots, 
                   (q == q_out && q_stride != q_out_stride)))
         return -1;
     if (!rows) return 0;
-    if (!slots || (rope && !positions)) return -1;
+    if (!slots || (rope && !positions) || off_element(width, k, v) || (heads && off_element(width, q, q_out))) return -1;
     A.c = *cache;
     A.slots = slots; A.positions = positions;
     A.k = k; A.v = v; A.k_stride = k_stride; A.v_stride = v_stride; A.rows = rows;

@@ -61,6 +61,7 @@ extern "C" int fyb_kv4_attention(const fyb_kv4_cache *cache, const int32_t *leng
         (uintptr_t)workspace % 16 || workspace_bytes < need || (!row_start && rows != requests))
         return -1;
     if (!rows) return 0;
+    if (off_element(type == T_F32 ? 4 : 2, q, out)) return -1;
     Kv4Attention A{};
     A.c.blocks = cache->blocks; A.c.kv_heads = cache->kv_heads; A.c.block_size = cache->block_size;
     A.c.head_dim = cache->head_dim;

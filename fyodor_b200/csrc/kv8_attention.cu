@@ -79,6 +79,7 @@ extern "C" int fyb_kv8_attention(const fyb_kv8_cache *cache, const int32_t *leng
         (uintptr_t)workspace % 16 || workspace_bytes < need || (!row_start && rows != requests))
         return -1;
     if (!rows) return 0;
+    if (off_element(type == T_F32 ? 4 : 2, q, out)) return -1;
     Kv8Attention A{};
     A.c = *cache;
     A.lengths = lengths; A.row_start = row_start; A.table = table; A.table_stride = table_stride;

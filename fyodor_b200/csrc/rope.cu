@@ -290,7 +290,8 @@ extern "C" int fyb_rope(const fyb_rope_desc *rope, const int32_t *positions, siz
         return -1;
     if (type != T_F32 && type != T_F16 && type != T_BF16) return -1;
     if (!rows) return 0;
-    if (!positions) return -1;
+    const size_t width = type == T_F32 ? 4 : 2;
+    if (!positions || (heads && off_element(width, q, q_out)) || (kv_heads && off_element(width, k, k_out))) return -1;
     const RopeRows rq{q, q_out, q_stride, q_out_stride, heads}, rk{k, k_out, k_stride, k_out_stride, kv_heads};
     return rope_run(type, t, positions, rows, hd, rq, rk, error, (cudaStream_t)stream);
 }
