@@ -599,8 +599,11 @@ __global__ void __launch_bounds__(k4t_threads(NR), 1) kv4_tiles_kernel(const __g
                     const unsigned j = rho * by_group >> 16;  // rho / GR
                     return q0 + j * A.q_stride + (rho - j * GR) * HD;
                 };
-                // at least the smallest normal number: -inf times it stays -inf
-                auto factor_of = [&](int e) { return fmaxf(fabsf(A.scale) * kt_power(-e), 1.17549435e-38f); };
+                // at least the smallest normal number: -inf times it stays -inf; NaN stays
+                auto factor_of = [&](int e) {
+                    const float y = fabsf(A.scale) * kt_power(-e);
+                    return y < 1.17549435e-38f ? 1.17549435e-38f : y;
+                };
                 if constexpr (S::Q_TM) {
                     // to tensor memory, a thread a lane's row
                     const unsigned rho = ct % NR;
