@@ -9,10 +9,11 @@
 // find by shuffles.
 //
 // A step's append is one launch, 4 us. Prompts: 6093 rows of 32 / 8 heads of 128, bf16,
-// take 16 us for K and V (31 MB: instructions, some 430 a warp for 512 values), 23 for
+// take 17 us for K and V (31 MB: instructions, some 440 a warp for 512 values), 23 for
 // q's rotation (0.67 of the measured copy; in one launch with K and V 55 us together
-// instead of 39, so q goes along only with few rows, where a launch more would count)
-// and 12 to be read back in F32 (0.79).
+// when one after the other took 39, so q goes along only with few rows, where a launch
+// more would count) and 12 to be read back in F32 (0.79). Of the 17, 0.6 are the tests
+// whether a group's numbers can leave 0..15 and its scale lies next to a border.
 #include "rope.cuh"
 #include "kv4.cuh"
 

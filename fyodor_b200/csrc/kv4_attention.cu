@@ -3,10 +3,18 @@
 //
 // Up to eight query rows per KV head (rows of a request x heads of a group), and
 // rows of F32 whatever their number, run on kv4_decode.cu, many rows in row tiles of
-// eight; many rows of 16 bits on kv4_tiles.cuh, in row tiles of 32, 64 or 256. With 8
-// rows 32 ragged requests take 71 us there and 97 in tiles; with 16 rows, two row
-// tiles, 126 and 97, 16 requests at 8100 92 and 72, with 32 rows 167 and 74 (what is
-// short is still as quick: four requests of 500 with 16 rows 13 us and 15).
+// eight; many rows of 16 bits on kv4_tiles.cuh, in row tiles of 32, 64 or 256. Both
+// kernels, us, with that many bf16 rows per KV head (four heads a group, 8 KV heads):
+//
+//                                    8 rows     16 rows    32 rows
+//   16 requests at 8100              57 /  73   97 /  73   175 /  74
+//   32 of 128 to 8192 (145 MB)       57 /  75   99 /  77   179 /  78
+//   32 of 128 to 32768 (649 MB)     185 / 248  353 / 255
+//   4 of 500                                  13.7 / 15.4  15.6 / 16.3
+//
+// F32 rows pay for each eight of them (16 requests at 8100: 8 rows 76 us, 16 131, 32
+// 241; a chunk of 2000 rows of one of 16000 1703, in bf16 161): the tiles round K, V and
+// the weights to 16 bits, which is not enough for them.
 #include "kv4_attention.cuh"
 
 namespace fyb {

@@ -31,10 +31,12 @@
 // Rows of 16 bits fit the high half, and at five rows and more their weights are
 // rounded to it (2^-12 each at the most, of no common sign).
 //
-// Bound by instructions: 16 at 8100 with eight rows takes 59 us for 22 of bytes (0.38
-// of the measured copy), 32 ragged requests of 128 to 32768 150 us for 99 (0.66). Three CTAs of four consumer warps and one for the copies
-// fit an SM at 128 registers (when they took 147 us two CTAs of eight took 175, four
-// of four, with fewer registers, 162).
+// Bound by the latency between dependent instructions of 12 consumer warps an SM: issue
+// 0.57, the ALU pipe 54 %, no other pipe above that, fixed latencies the largest stall.
+// 16 at 8100 with eight rows takes 59 us for 22 of bytes (0.38 of the measured copy), 32
+// ragged requests of 128 to 32768 150 us for 99 (0.66). Three CTAs of four consumer warps
+// and one for the copies fit an SM at 128 registers (when they took 147 us two CTAs of
+// eight took 175, four of four, with fewer registers, 162).
 #include "kv4_attention.cuh"
 
 namespace fyb {
@@ -268,7 +270,8 @@ __global__ void __launch_bounds__(K4_THREADS, K4_CTAS) kv4_decode_kernel(const _
         }
 
         // The accumulators go to this thread's sums in shared memory: every FLUSH tiles, as they round towards zero (once a
-        // segment ragged 32 was 6.2e-6 off when it was 3.7e-6 so, for 4 us of 162), at the end where rows are of 16 bits.
+        // segment ragged 32 was 6.2e-6 off when it was 3.7e-6 so, for 4 us of 162); with five to eight rows of 16 bits once, at
+        // the segment's end.
         auto sum_of = [&](int h, int k, int w) {
             return reinterpret_cast<float2 *>(o_s + (warp * R + W * t4 + w) * HD + 64 * h + 8 * g + 2 * k);
         };

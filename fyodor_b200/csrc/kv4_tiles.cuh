@@ -26,16 +26,21 @@
 //
 // Bound, at 256 rows, by the chain of a half tile's products and weights: a tile of 128
 // positions takes 4200 cycles, of which its products alone would take 2050 and its
-// exponentials 2050; a chunk of 500 rows of four heads at 16000 160 us (805 TFLOP/s,
+// exponentials 2050; a chunk of 500 rows of four heads at 16000 161 us (800 TFLOP/s,
 // 0.49 of the measured rate; weights of a whole tile at a time 205, products of 64 columns for
 // the half tiles 259, since q is then read twice as often). At 32 rows by the products of
 // full 128-lane tiles, 1250 of a tile's 1820 cycles, and the MMA warp's waits: 32 ragged
-// drafts of eight rows of four heads 245 us, 0.38 of the measured copy. What runs once a
+// drafts of eight rows of four heads 249 us, 0.38 of the measured copy. What runs once a
 // segment costs as much as 8 tiles (6 of 256 rows), and its instructions more than its
 // data.
 //
 // The maximum m of a row moves only when a weight is above 2^8 (with 2^4 a chunk of 500
 // at 16000 took 170 us, with 2^8 160).
+//
+// K, V and the weights are rounded to fp16 once each (the sum of the weights is not):
+// fp16 rows are 3.0e-4 to 4.1e-4 of the norm off at 20 to 9000 tokens (5.0e-4 where K
+// has strong channels), their rounded output alone 2.1e-4; bf16 rows are at their
+// output's rounding.
 #pragma once
 #include "kv4_attention.cuh"
 #include "kt_mma.cuh"
@@ -413,7 +418,8 @@ __global__ void __launch_bounds__(k4t_threads(NR), 1) kv4_tiles_kernel(const __g
                     if (__any_sync(0xffffffffu, up || far)) {
                         if (__any_sync(0xffffffffu, far)) {
                             // rows of scores so large that m is off by a half and more of a unit: their products are rounded as
-                            // m is, or a weight's exponent could be beyond fp16's (at 2^28 by half of 32)
+                            // m is, or a weight's exponent could be beyond fp16's (at 2^28 by half of 32). Asked with `up`, in
+                            // one vote: ragged drafts 246 us without it, 249 so, 251 in a vote of its own
                             const float times = far ? f : 1.f;
 #pragma unroll 1
                             for (unsigned c = 0; c < CW; c += 16) {

@@ -418,7 +418,12 @@ int fyb_kv4_append(const fyb_kv4_cache *cache, const int32_t *slots, size_t rows
 int fyb_kv4_read(const fyb_kv4_cache *cache, const int32_t *slots, size_t rows, float *k_out, float *v_out,
     uint32_t *error, void *stream);
 /* Causal attention of the newest rows of each request over its blocks:
-   fyb_kv8_attention's arguments, workspace rules and results over this cache. */
+   fyb_kv8_attention's arguments, workspace rules and results over this cache.
+   Rows of 16 bits are computed with weights of one fp16 half from five rows per
+   KV head on (max_rows x heads of a group), from nine on with K and V rounded to
+   fp16 too: fp16 rows are then some 3e-4 and 4e-4 of the norm off, where rounding
+   the output alone is 2e-4. F32 rows are not (3e-6), whatever their number, but
+   each eight of them read the cache once. */
 size_t fyb_kv4_attention_workspace(uint32_t requests, uint32_t max_rows, uint32_t heads, uint32_t kv_heads,
     uint32_t head_dim);
 int fyb_kv4_attention(const fyb_kv4_cache *cache, const int32_t *lengths, const int32_t *row_start, uint32_t requests,
