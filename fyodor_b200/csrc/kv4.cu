@@ -261,7 +261,8 @@ template <typename T, int HD, bool Q> __global__ void __launch_bounds__(KV4_THRE
     const __half sc = kv4_scale(lf, __half2float(hi));
     const float sf = __half2float(sc), inv = rcp_approx(sf);  // scale 0: no number is certain
     // Low and high as F16, and scale, need not enclose the group (a range of a few steps of F16, a scale below its normal
-    // numbers, values beyond KV4_MOST): where a quotient can leave 0..15 the values go one by one, which clamps.
+    // numbers, values beyond KV4_MOST): where a quotient can leave 0..15 the values go one by one, which clamps (6093 F32 rows of
+    // nothing else 23 us instead of 13).
     const bool wide = bad || !(__fmul_rn(__fsub_rn(low, lf), inv) >= -0.49f && __fmul_rn(__fsub_rn(high, lf), inv) <= 15.49f);
     const size_t at = (((size_t)(slot >> A.shift) * A.c.kv_heads + head) << A.shift) + ((unsigned)slot & ((1u << A.shift) - 1));
     unsigned *words = static_cast<unsigned *>(is_k ? A.c.k : A.c.v) + at * WORDS + lane % PART * (KV4_EACH / 8) * GROUPS + group;
