@@ -393,9 +393,10 @@ int fyb_kv8_attention(const fyb_kv8_cache *cache, const int32_t *lengths, const 
    values, those beyond +-61440 taken as +-61440, low and high are the least (-0
    less than 0) and the greatest rounded to F16, scale is (high - low) / 15
    rounded to F16, and n is the whole number nearest to (x - low) / scale, ties
-   to even, in 0..15 (0 where scale is 0). Infinities are held as 0 or 15, NaN as 0 would be; both
-   raise 2 in `error`. A group without a finite value has low and scale 0. A row
-   depends on no other: tokens may be written in any order, and again.
+   to even, in 0..15 (0 where scale is 0). Infinities are held as 0 or 15, NaN as
+   0 would be; both raise 2 in `error`. A group without a finite value has low
+   and scale 0. A row depends on no other: tokens may be written in any order,
+   and again.
    A token's row of a head is head_dim / 8 words of 32 bits, each eight values,
    the first in the lowest bits: word w holds dimensions 8w.. of a head of 64;
    of a head of 128 word 2j holds dimensions 8j.., word 2j + 1 64 + 8j... */
